@@ -10,12 +10,20 @@ instantiates it.  After that, the reference's graphs select it by name::
     program = chomikgrad.compile_graph(*outputs, compiler="cuda-b200",
                                        dynamic_inputs=...)
 
-``chomikgrad`` must be importable; the plugin has no front-end of its own.
+The plugin has no front-end of its own: its graphs need an importable
+``chomikgrad``.  The serving operators (``paged``, ``speculative``) and the C
+binding (``_lib``) take tensors, so without it the package still imports, with
+nothing registered, and ``install`` raises.
 """
 
 from __future__ import annotations
 
-import chomikgrad
+try:
+    import chomikgrad
+except ModuleNotFoundError as error:
+    if error.name != "chomikgrad":
+        raise
+    chomikgrad = None
 
 BACKEND = "cuda-b200"
 
@@ -29,9 +37,12 @@ def _factory():
 def install(chomikgrad_module=None, *, replace: bool = True) -> None:
     """(Re-)register ``cuda-b200`` in a chomikgrad module's registry (the imported one by default)."""
     module = chomikgrad if chomikgrad_module is None else chomikgrad_module
+    if module is None:
+        raise ImportError("chomikgrad is not importable: there is no registry for the cuda-b200 compiler")
     module.register_compiler(BACKEND, _factory, replace=replace)
 
 
-install()
+if chomikgrad is not None:
+    install()
 
 __all__ = ["BACKEND", "install"]

