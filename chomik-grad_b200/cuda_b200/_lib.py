@@ -15,7 +15,7 @@ import numpy as np
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "libchomik_b200.so"
 
-F32, BF16, F16, I32, I64 = 0, 1, 2, 3, 4
+F32, BF16, F16, I32, I64, I8, E4M3 = 0, 1, 2, 3, 4, 5, 6
 CAUSAL_SKIP, CAUSAL_ZERO_BELOW = 1, 2  # cb_sdpa_tc causal flags
 MAX_DIMS = 8
 EW_MAX_INPUTS = 8
@@ -231,6 +231,58 @@ class DecodeStepConfig(ctypes.Structure):
                 ("timeline", c_void_p)]
 
 
+class PagedCacheArgs(ctypes.Structure):
+    _fields_ = [
+        ("k_pages", c_void_p), ("v_pages", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("storage", c_int), ("kv_heads", c_int), ("page", c_int), ("head_size", c_int),
+        ("pages", c_longlong), ("table", c_void_p), ("lengths", c_void_p),
+        ("slots", c_longlong), ("columns", c_longlong),
+    ]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", PagedCacheArgs), ("k", c_void_p), ("v", c_void_p), ("dtype", c_int),
+        ("batch", c_longlong), ("tokens", c_longlong),
+        ("k_strides", c_longlong * 3), ("v_strides", c_longlong * 3),
+        ("counts", c_void_p), ("sequences", c_void_p), ("error_flag", c_void_p),
+    ]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", PagedCacheArgs), ("q", c_void_p), ("dtype", c_int),
+        ("batch", c_longlong), ("tokens", c_longlong), ("heads", c_longlong),
+        ("q_strides", c_longlong * 3), ("out", c_void_p),
+        ("counts", c_void_p), ("sequences", c_void_p), ("scale", c_float), ("error_flag", c_void_p),
+    ]
+
+
+class PageBook(ctypes.Structure):
+    _fields_ = [
+        ("table", c_void_p), ("lengths", c_void_p), ("refs", c_void_p), ("free_pages", c_void_p),
+        ("height", c_void_p), ("slots", c_longlong), ("columns", c_longlong), ("pages", c_longlong),
+        ("page", c_int),
+    ]
+
+
+class PagePools(ctypes.Structure):
+    _fields_ = [
+        ("k_pages", c_void_p), ("v_pages", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("layers", c_longlong), ("pages", c_longlong), ("page_bytes", c_longlong), ("kv_heads", c_int),
+    ]
+
+
+class VerifyArgs(ctypes.Structure):
+    _fields_ = [
+        ("target", c_void_p), ("draft", c_void_p), ("dtype", c_int),
+        ("batch", c_longlong), ("tokens", c_longlong), ("vocab", c_longlong),
+        ("target_strides", c_longlong * 2), ("draft_strides", c_longlong * 2),
+        ("drafted", c_void_p), ("uniforms", c_void_p), ("counts", c_void_p),
+        ("accepted", c_void_p), ("out", c_void_p), ("error_flag", c_void_p),
+    ]
+
+
 class KernelError(RuntimeError):
     """A libchomik_b200 entry point returned a non-zero status."""
 
@@ -310,6 +362,17 @@ _SIGNATURES = {
                                      c_void_p, c_void_p, c_void_p, c_void_p], c_int),
     "cb_sgd_update": ([c_void_p, c_void_p], c_int),
     "cb_sample_rows": ([c_void_p, c_void_p], c_int),
+    "cb_paged_append": ([POINTER(PagedAppendArgs), c_void_p], c_int),
+    "cb_paged_attention_scratch": ([POINTER(PagedAttentionArgs)], c_longlong),
+    "cb_paged_attention": ([POINTER(PagedAttentionArgs), c_void_p, c_void_p], c_int),
+    "cb_pages_scratch": ([POINTER(PageBook), c_longlong], c_longlong),
+    "cb_pages_extend": ([POINTER(PageBook), POINTER(PagePools), c_void_p, c_void_p, c_longlong, c_void_p, c_void_p,
+                         c_void_p], c_int),
+    "cb_pages_fork": ([POINTER(PageBook), c_void_p, c_void_p, c_longlong, c_void_p, c_void_p], c_int),
+    "cb_pages_truncate": ([POINTER(PageBook), c_void_p, c_void_p, c_longlong, c_void_p, c_void_p], c_int),
+    "cb_pages_compact": ([POINTER(PageBook), POINTER(PagePools), c_void_p, c_void_p, c_void_p], c_int),
+    "cb_pages_copy": ([POINTER(PagePools), c_void_p, c_void_p, c_longlong, c_void_p, c_void_p], c_int),
+    "cb_verify_draft": ([POINTER(VerifyArgs), c_void_p], c_int),
     "cb_decode_advance": ([c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
                            c_int, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p], c_int),
     "cb_decode_advance_rows": ([c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int,
@@ -341,6 +404,7 @@ FLAG_INDEX, FLAG_POSITION, FLAG_CONTEXT = 1, 2, 3
 FLAG_WAIT_DATA, FLAG_WAIT_SLOT, FLAG_WAIT_DRAIN, FLAG_WAIT_PHASE = 4, 5, 6, 7
 FLAG_NAN = 8
 FLAG_WAIT_PEER = 9
+FLAG_PAGES, FLAG_BOOK = 10, 11
 
 
 def flag_error(value: int) -> Exception:
@@ -353,6 +417,10 @@ def flag_error(value: int) -> Exception:
         return IndexError("decode step would write past the KV-cache context")
     if value == FLAG_NAN:  # what NumPy's Generator.choice raises for the reference's sampler
         return ValueError("probabilities contain NaN")
+    if value == FLAG_PAGES:
+        return MemoryError("the cache has too few free pages, or a sequence would outgrow its table row")
+    if value == FLAG_BOOK:
+        return IndexError("a sequence, page, length or count of the paged cache is outside its range")
     waits = {FLAG_WAIT_DATA: "a consumer waiting for weight data",
              FLAG_WAIT_SLOT: "a producer waiting for a free ring slot",
              FLAG_WAIT_DRAIN: "the end-of-kernel drain of bulk copies",

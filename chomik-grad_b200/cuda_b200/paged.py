@@ -1,0 +1,304 @@
+"""A paged 8-bit KV cache and the operators that serve from it.
+
+The reference keeps one dense float32 cache per program, for one sequence of a
+fixed context (chomikgrad/llama.py:436-543).  ``PagedCache`` holds many
+sequences of unlike lengths in pages of 16 to 256 tokens, int8 or e4m3 with
+one float32 scale for each page and kv head, and pages can be shared:
+
+    cache = PagedCache.allocate(layers=22, pages=4096, kv_heads=4, page_size=64,
+                                head_size=64, sequences=32, pages_per_sequence=32)
+    cache.extend(counts)                      # room for counts[b] more tokens of slot b
+    for layer in range(22):
+        cache.append(layer, k, v, counts=counts)        # quantise them into their pages
+        out = cache.attend(layer, q, counts=counts)     # attention of the same tokens
+    cache.fork([0, 0], [5, 6])                # slots 5 and 6 continue slot 0, sharing its pages
+    cache.truncate(refused)                   # drop the last refused[b] tokens
+    cache.release([6])                        # all of slot 6
+    cache.compact()                           # move the held pages to the front of the pools
+
+Values are CUDA ``torch.Tensor`` or the device's ``DeviceArray``.  Every call
+runs on the current stream and reads lengths and tables on the device, with no
+host synchronisation, so a step can be captured in a CUDA graph.  Arguments
+that the host can see are checked at the call (``TypeError``, ``ValueError``);
+what only the device sees (a slot, page, length or count outside its range,
+too few free pages) sets the cache's error flag, which ``check_errors`` reads
+and raises.  There is no backward pass.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Any, Optional, Tuple
+
+import torch
+
+from . import _lib
+
+PAGE_SIZES = (16, 32, 64, 128, 256)
+HEAD_SIZES = (32, 64, 128)
+_VALUES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_STORAGE = {torch.int8: _lib.I8, torch.float8_e4m3fn: _lib.E4M3}
+
+
+def tensor_of(value: Any) -> torch.Tensor:
+    """The torch view of a tensor or a ``DeviceArray``."""
+    if isinstance(value, torch.Tensor):
+        return value
+    tensor = getattr(value, "tensor", None)
+    if not isinstance(tensor, torch.Tensor):
+        raise TypeError(f"a CUDA tensor or DeviceArray is required, got {type(value).__name__}")
+    return tensor[:value.size].view(value.shape)
+
+
+def require(value: torch.Tensor, name: str, device: torch.device, dtypes, shape: Tuple[Optional[int], ...],
+            dense: int) -> None:
+    """Checks of one argument: its device, dtype, shape (None: any) and that its last ``dense`` dims are contiguous."""
+    if value.device != device:
+        raise ValueError(f"{name} is on {value.device}, expected {device}")
+    if value.dtype not in dtypes:
+        raise TypeError(f"{name} has dtype {value.dtype}, expected one of {', '.join(map(str, dtypes))}")
+    if len(value.shape) != len(shape) or any(want is not None and got != want
+                                             for got, want in zip(value.shape, shape)):
+        raise ValueError(f"{name} has shape {tuple(value.shape)}, expected "
+                         f"{tuple('any' if n is None else n for n in shape)}")
+    step = 1 if value.numel() else None  # strides of an empty tensor say nothing
+    for at in range(len(shape) - 1, len(shape) - 1 - dense, -1):
+        if step is None:
+            break
+        if value.shape[at] != 1 and value.stride(at) != step:
+            raise ValueError(f"{name} has to be contiguous in its last {dense} dimension(s)")
+        step *= value.shape[at]
+    if value.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires grad: this operator has no backward pass")
+
+
+class PagedCache:
+    """Pools, book and the operators on them (see the module's text).
+
+    ``k_pages`` and ``v_pages`` (layers, pages, kv_heads, page_size, head_size),
+    ``k_scale`` and ``v_scale`` (layers, pages, kv_heads) and ``book``, one int32
+    tensor of the table (sequences, pages_per_sequence), the lengths
+    (sequences), the reference counts (pages), the stack of free pages (pages)
+    and its height, are used as they are.  ``allocate`` makes an empty cache.
+    """
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                 book: torch.Tensor, *, sequences: int, pages_per_sequence: int) -> None:
+        if k_pages.device.type != "cuda":
+            raise ValueError(f"the cache has to be on a CUDA device, got {k_pages.device}")
+        if k_pages.ndim != 5:
+            raise ValueError("k_pages has to be (layers, pages, kv_heads, page_size, head_size)")
+        self.device = k_pages.device
+        self.layers, self.pages, self.kv_heads, self.page_size, self.head_size = map(int, k_pages.shape)
+        self.sequences, self.pages_per_sequence = int(sequences), int(pages_per_sequence)
+        if self.page_size not in PAGE_SIZES:
+            raise ValueError(f"page_size has to be one of {PAGE_SIZES}, got {self.page_size}")
+        if self.head_size not in HEAD_SIZES:
+            raise ValueError(f"head_size has to be one of {HEAD_SIZES}, got {self.head_size}")
+        if min(self.layers, self.pages, self.kv_heads, self.sequences, self.pages_per_sequence) < 1:
+            raise ValueError("layers, pages, kv_heads, sequences and pages_per_sequence have to be positive")
+        if self.pages_per_sequence * self.page_size >= 2 ** 31:
+            raise ValueError("a sequence holds fewer than 2**31 tokens")
+        require(k_pages, "k_pages", self.device, tuple(_STORAGE), tuple(k_pages.shape), 5)
+        require(v_pages, "v_pages", self.device, (k_pages.dtype,), tuple(k_pages.shape), 5)
+        for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
+            require(scale, name, self.device, (torch.float32,), tuple(k_pages.shape[:3]), 3)
+        rows = self.sequences * self.pages_per_sequence
+        require(book, "book", self.device, (torch.int32,), (rows + self.sequences + 2 * self.pages + 1,), 1)
+        self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.book = k_pages, v_pages, k_scale, v_scale, book
+        self.table, self.lengths, self.refs, self.free, self.height = self.split(book)
+        self._flag = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._layer_args = [self._args_of(layer) for layer in range(self.layers)]
+        self._book_args, self._pool_args = _lib.PageBook(), _lib.PagePools()
+        b, p = self._book_args, self._pool_args
+        b.table, b.lengths, b.refs = (t.data_ptr() for t in (self.table, self.lengths, self.refs))
+        b.free_pages, b.height = self.free.data_ptr(), self.height.data_ptr()
+        b.slots, b.columns, b.pages, b.page = self.sequences, self.pages_per_sequence, self.pages, self.page_size
+        p.k_pages, p.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
+        p.k_scale, p.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+        p.layers, p.pages, p.kv_heads = self.layers, self.pages, self.kv_heads
+        p.page_bytes = self.kv_heads * self.page_size * self.head_size
+        _lib.load()
+
+    @classmethod
+    def allocate(cls, *, layers: int, pages: int, kv_heads: int, page_size: int, head_size: int, sequences: int,
+                 pages_per_sequence: int, storage: torch.dtype = torch.int8, device: Any = None) -> "PagedCache":
+        """An empty cache of ``sequences`` slots on ``device`` (the current CUDA device)."""
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        shape = (layers, pages, kv_heads, page_size, head_size)
+        pools = [torch.zeros(shape, dtype=torch.int8, device=device).view(storage) for _ in range(2)]
+        scale = [torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)]
+        book = torch.zeros(sequences * pages_per_sequence + sequences + 2 * pages + 1, dtype=torch.int32,
+                           device=device)
+        cache = cls(*pools, *scale, book, sequences=sequences, pages_per_sequence=pages_per_sequence)
+        cache.table.fill_(-1)
+        cache.free.copy_(torch.arange(pages - 1, -1, -1, dtype=torch.int32))
+        cache.height.fill_(pages)
+        return cache
+
+    def split(self, book: torch.Tensor) -> Tuple[torch.Tensor, ...]:
+        """Views of a book: table, lengths, reference counts, free pages, height of the free stack."""
+        rows = self.sequences * self.pages_per_sequence
+        table, lengths, refs, free, height = book.split([rows, self.sequences, self.pages, self.pages, 1])
+        return table.view(self.sequences, self.pages_per_sequence), lengths, refs, free, height
+
+    def _args_of(self, layer: int) -> _lib.PagedCacheArgs:
+        c = _lib.PagedCacheArgs()
+        c.k_pages, c.v_pages = self.k_pages[layer].data_ptr(), self.v_pages[layer].data_ptr()
+        c.k_scale, c.v_scale = self.k_scale[layer].data_ptr(), self.v_scale[layer].data_ptr()
+        c.storage, c.kv_heads = _STORAGE[self.k_pages.dtype], self.kv_heads
+        c.page, c.head_size, c.pages = self.page_size, self.head_size, self.pages
+        c.table, c.lengths = self.table.data_ptr(), self.lengths.data_ptr()
+        c.slots, c.columns = self.sequences, self.pages_per_sequence
+        return c
+
+    def _stream(self) -> int:
+        if torch.cuda.current_device() != self.device.index:
+            raise ValueError(f"the cache is on {self.device}, the current device is cuda:{torch.cuda.current_device()}")
+        return torch.cuda.current_stream().cuda_stream
+
+    def _list(self, value: Any, name: str, count: Optional[int]) -> torch.Tensor:
+        """An int32 list on the device (host lists are copied there)."""
+        if isinstance(value, (list, tuple)):
+            value = torch.tensor(value, dtype=torch.int32, device=self.device)
+        value = tensor_of(value)
+        require(value, name, self.device, (torch.int32,), (count,), 1)
+        return value
+
+    def _lists(self, counts: Any, sequences: Any, batch: int) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+        counts = None if counts is None else self._list(counts, "counts", batch)
+        if sequences is None:
+            if batch > self.sequences:
+                raise ValueError(f"{batch} rows, and the cache has {self.sequences} sequences")
+            return counts, None
+        return counts, self._list(sequences, "sequences", batch)
+
+    def _layer(self, layer: int) -> _lib.PagedCacheArgs:
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer {layer} of {self.layers}")
+        return self._layer_args[layer]
+
+    # -- values ------------------------------------------------------------
+    def append(self, layer: int, k: Any, v: Any, *, counts: Any = None, sequences: Any = None) -> None:
+        """Quantise new keys and values (batch, tokens, kv_heads, head_size) into ``layer``'s pages.
+
+        Row b's first ``counts[b]`` tokens (all without counts) are the last
+        ones of slot ``sequences[b]`` (slot b without), for which ``extend``
+        has made room.  float32, bfloat16 or float16, any strides with a
+        contiguous head.  See ``cb_paged_append`` for the scales.
+        """
+        k, v = tensor_of(k), tensor_of(v)
+        require(k, "k", self.device, tuple(_VALUES), (None, None, self.kv_heads, self.head_size), 1)
+        batch, tokens = k.shape[:2]
+        require(v, "v", self.device, (k.dtype,), (batch, tokens, self.kv_heads, self.head_size), 1)
+        counts, sequences = self._lists(counts, sequences, batch)
+        a = _lib.PagedAppendArgs()
+        a.cache = self._layer(layer)
+        a.k, a.v, a.dtype, a.batch, a.tokens = k.data_ptr(), v.data_ptr(), _VALUES[k.dtype], batch, tokens
+        a.k_strides[:], a.v_strides[:] = k.stride()[:3], v.stride()[:3]
+        a.counts = None if counts is None else counts.data_ptr()
+        a.sequences = None if sequences is None else sequences.data_ptr()
+        a.error_flag = self._flag.data_ptr()
+        _lib.call("cb_paged_append", ctypes.byref(a), self._stream())
+
+    def attend(self, layer: int, q: Any, *, counts: Any = None, sequences: Any = None, scale: Optional[float] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of q (batch, tokens, heads, head_size), the last tokens of their slots, over ``layer``.
+
+        Each token sees its slot's keys up to its own (``counts`` and
+        ``sequences`` as in ``append``; rows past ``counts[b]`` and rows that
+        see nothing give zeros).  ``scale`` is 1/sqrt(head_size) without one.
+        Returns (batch, tokens, heads, head_size) of q's dtype.
+        """
+        q = tensor_of(q)
+        require(q, "q", self.device, tuple(_VALUES), (None, None, None, self.head_size), 1)
+        batch, tokens, heads = q.shape[:3]
+        if heads == 0 or heads % self.kv_heads:
+            raise ValueError(f"{heads} query heads cannot share {self.kv_heads} kv heads")
+        counts, sequences = self._lists(counts, sequences, batch)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+        else:
+            require(out, "out", self.device, (q.dtype,), tuple(q.shape), 4)
+        a = _lib.PagedAttentionArgs()
+        a.cache = self._layer(layer)
+        a.q, a.out, a.dtype = q.data_ptr(), out.data_ptr(), _VALUES[q.dtype]
+        a.batch, a.tokens, a.heads = batch, tokens, heads
+        a.q_strides[:] = q.stride()[:3]
+        a.counts = None if counts is None else counts.data_ptr()
+        a.sequences = None if sequences is None else sequences.data_ptr()
+        a.scale = 1.0 / math.sqrt(self.head_size) if scale is None else scale
+        a.error_flag = self._flag.data_ptr()
+        lib = _lib.load()
+        scratch = torch.empty(lib.cb_paged_attention_scratch(ctypes.byref(a)), dtype=torch.uint8, device=self.device)
+        _lib.call("cb_paged_attention", ctypes.byref(a), scratch.data_ptr(), self._stream())
+        return out
+
+    # -- pages -------------------------------------------------------------
+    def extend(self, counts: Any, *, sequences: Any = None) -> None:
+        """Make room for ``counts[i]`` more tokens of slot ``sequences[i]`` (slot i without).
+
+        Lengths grow, missing pages are taken, and an open last page that
+        other slots hold too is copied first.  All or nothing: with too few
+        free pages nothing changes and ``check_errors`` raises MemoryError.
+        """
+        counts = self._list(counts, "counts", None)
+        n = counts.shape[0]
+        _, sequences = self._lists(None, sequences, n)
+        scratch = self._scratch(n)
+        _lib.call("cb_pages_extend", ctypes.byref(self._book_args), ctypes.byref(self._pool_args), counts.data_ptr(),
+                  None if sequences is None else sequences.data_ptr(), n, scratch.data_ptr(), self._flag.data_ptr(),
+                  self._stream())
+
+    def fork(self, parents: Any, children: Any) -> None:
+        """Slot ``children[i]``, which has to be empty, continues slot ``parents[i]`` and shares its pages."""
+        parents = self._list(parents, "parents", None)
+        n = parents.shape[0]
+        children = self._list(children, "children", n)
+        if n > self.sequences:
+            raise ValueError(f"{n} forks, and the cache has {self.sequences} sequences")
+        _lib.call("cb_pages_fork", ctypes.byref(self._book_args), parents.data_ptr(), children.data_ptr(), n,
+                  self._flag.data_ptr(), self._stream())
+
+    def truncate(self, counts: Any, *, sequences: Any = None) -> None:
+        """Drop the last ``counts[i]`` tokens of slot ``sequences[i]`` and let go of the pages that held only those."""
+        counts = self._list(counts, "counts", None)
+        self._truncate(counts, sequences, counts.shape[0])
+
+    def release(self, sequences: Any) -> None:
+        """Empty the slots ``sequences``."""
+        sequences = self._list(sequences, "sequences", None)
+        self._truncate(None, sequences, sequences.shape[0])
+
+    def _truncate(self, counts: Optional[torch.Tensor], sequences: Any, n: int) -> None:
+        _, sequences = self._lists(None, sequences, n)
+        if n > self.sequences:
+            raise ValueError(f"{n} slots, and the cache has {self.sequences} sequences")
+        _lib.call("cb_pages_truncate", ctypes.byref(self._book_args), None if counts is None else counts.data_ptr(),
+                  None if sequences is None else sequences.data_ptr(), n, self._flag.data_ptr(), self._stream())
+
+    def compact(self) -> None:
+        """Move the held pages to the front of the pools (page ids change; the table follows)."""
+        scratch = self._scratch(0)
+        _lib.call("cb_pages_compact", ctypes.byref(self._book_args), ctypes.byref(self._pool_args),
+                  scratch.data_ptr(), self._flag.data_ptr(), self._stream())
+
+    def copy_pages(self, source: Any, target: Any) -> None:
+        """Copy page ``source[i]`` to page ``target[i]`` in every layer (no page is both)."""
+        source = self._list(source, "source", None)
+        target = self._list(target, "target", source.shape[0])
+        _lib.call("cb_pages_copy", ctypes.byref(self._pool_args), source.data_ptr(), target.data_ptr(),
+                  source.shape[0], self._flag.data_ptr(), self._stream())
+
+    def _scratch(self, n: int) -> torch.Tensor:
+        size = _lib.load().cb_pages_scratch(ctypes.byref(self._book_args), n)
+        return torch.empty(size, dtype=torch.uint8, device=self.device)
+
+    # -- errors ------------------------------------------------------------
+    def check_errors(self) -> None:
+        """Raise what a call since the last check found on the device (reads one number back)."""
+        value = int(self._flag.item())
+        if value:
+            self._flag.zero_()
+            raise _lib.flag_error(value)

@@ -22,8 +22,9 @@
 extern "C" {
 #endif
 
-/* dtype codes: float32, bfloat16, float16, int32, int64 */
-enum { CB_F32 = 0, CB_BF16 = 1, CB_F16 = 2, CB_I32 = 3, CB_I64 = 4 };
+/* dtype codes: float32, bfloat16, float16, int32, int64; the paged cache's
+ * int8 and float8 (e4m3, finite) */
+enum { CB_F32 = 0, CB_BF16 = 1, CB_F16 = 2, CB_I32 = 3, CB_I64 = 4, CB_I8 = 5, CB_E4M3 = 6 };
 
 /* status codes */
 enum { CB_OK = 0, CB_ERR_INVALID = 1, CB_ERR_CUDA = 2 };
@@ -42,7 +43,9 @@ enum {
   CB_FLAG_WAIT_DRAIN = 6,
   CB_FLAG_WAIT_PHASE = 7, /* cb_decode_step: a block waiting for the previous phase */
   CB_FLAG_NAN = 8,        /* cb_sample_rows: NaN probabilities */
-  CB_FLAG_WAIT_PEER = 9   /* cb_peer_all_reduce: a rank of the group did not arrive in time */
+  CB_FLAG_WAIT_PEER = 9,  /* cb_peer_all_reduce: a rank of the group did not arrive in time */
+  CB_FLAG_PAGES = 10,     /* cb_pages_extend: the free pages or a table row's columns do not suffice */
+  CB_FLAG_BOOK = 11       /* cb_paged_*, cb_pages_*: a slot, page, length or count outside its range */
 };
 
 #define CB_MAX_DIMS 8
@@ -759,6 +762,159 @@ typedef struct {
   int* error_flag;             /* optional: CB_FLAG_NAN */
 } cb_sample_args;
 CB_API int cb_sample_rows(const cb_sample_args* a, cb_stream_t stream);
+
+/* ---- paged 8-bit KV cache --------------------------------------------------
+ * The cache of a serving program: sequences of unlike lengths, each a row of
+ * page ids (a "slot" of the table), whose pages can be shared.  The reference
+ * keeps one dense float32 cache per program and layer and rewrites it each
+ * step (chomikgrad/llama.py:511-512); these entry points have no counterpart
+ * there.
+ *
+ * Storage: k_pages and v_pages (pages, kv_heads, page, head_size) of one
+ * layer, CB_I8 or CB_E4M3, and one float32 scale for each page and kv head;
+ * an element stands for q * scale.  page is 16, 32, 64, 128 or 256 tokens,
+ * head_size 32, 64 or 128; pools are 16-byte aligned.  Token j of slot s lies
+ * in row j % page of page table[s * columns + j / page].
+ *
+ * A page id, slot, count or length outside its range sets *error_flag
+ * (CB_FLAG_BOOK); nothing is read or written through it. */
+typedef struct {
+  void* k_pages;
+  void* v_pages;
+  float* k_scale; /* (pages, kv_heads) */
+  float* v_scale;
+  int storage; /* CB_I8 or CB_E4M3 */
+  int kv_heads, page, head_size;
+  long long pages;
+  const int* table;   /* (slots, columns) */
+  const int* lengths; /* tokens of each slot, the new ones among them */
+  long long slots, columns;
+} cb_paged_cache;
+
+/* Quantise the last counts[b] tokens of slot sequences[b] into its pages (they
+ * are rows 0 .. counts[b]-1 of k[b], v[b]).  For each page and head, with a =
+ * the largest finite |x| of its new rows, top = 127 (int8) or 448 (e4m3):
+ *   scale' = max(older rows in the page ? scale : 0, a * (1 / top))
+ *   q      = round(x * (1 / scale')) to nearest even, saturated
+ * and where the scale grew, the page's older rows are requantised,
+ * q' = round(q * (scale * (1 / scale'))).  A NaN is stored as 0, an infinity
+ * as +-top; a scale below 2^-110 becomes 0 and its rows zeros.  All arithmetic
+ * float32, every operation rounded once.  Pages that other slots hold must
+ * have been made this slot's own (cb_pages_extend). */
+typedef struct {
+  cb_paged_cache cache;
+  const void* k; /* (batch, tokens, kv_heads, head_size), head_size contiguous */
+  const void* v;
+  int dtype; /* CB_F32, CB_BF16 or CB_F16, both */
+  long long batch, tokens;
+  long long k_strides[3], v_strides[3]; /* elements, over batch, tokens, kv_heads */
+  const int* counts;    /* NULL: tokens each */
+  const int* sequences; /* NULL: slot b */
+  int* error_flag;
+} cb_paged_append_args;
+CB_API int cb_paged_append(const cb_paged_append_args* args, cb_stream_t stream);
+
+/* softmax(scale * q k^T) v of the last counts[b] tokens of slot sequences[b]
+ * (rows 0 .. counts[b]-1 of q[b]; rows beyond them give zeros) over the slot's
+ * keys up to and including each token's own (token t of n sees keys 0 ..
+ * length - n + t), grouped kv heads, float32 softmax and sums.  A row that
+ * sees no key gives zeros.  out: as q, contiguous, q's dtype.  Serves single
+ * tokens, blocks of drafted tokens and short prompt chunks.  `scratch`:
+ * cb_paged_attention_scratch bytes, 16-byte aligned. */
+typedef struct {
+  cb_paged_cache cache;
+  const void* q; /* (batch, tokens, heads, head_size), head_size contiguous */
+  int dtype;     /* of q and out: CB_F32, CB_BF16 or CB_F16 */
+  long long batch, tokens, heads;
+  long long q_strides[3]; /* elements, over batch, tokens, heads */
+  void* out;
+  const int* counts;
+  const int* sequences;
+  float scale;
+  int* error_flag;
+} cb_paged_attention_args;
+CB_API long long cb_paged_attention_scratch(const cb_paged_attention_args* args);
+CB_API int cb_paged_attention(const cb_paged_attention_args* args, void* scratch, cb_stream_t stream);
+
+/* The book of a cache: who holds which page.  refs[p] slots hold page p;
+ * free[0 .. *height) is a stack of the pages that none holds.  A slot of
+ * length n holds ceil(n / page) pages, its other columns are -1. */
+typedef struct {
+  int* table; /* (slots, columns) */
+  int* lengths;
+  int* refs;   /* pages */
+  int* free_pages; /* pages */
+  int* height;
+  long long slots, columns, pages;
+  int page;
+} cb_page_book;
+/* The pools of all layers, whose pages move together. */
+typedef struct {
+  void* k_pages; /* (layers, pages, page_bytes) */
+  void* v_pages;
+  float* k_scale; /* (layers, pages, kv_heads) */
+  float* v_scale;
+  long long layers, pages, page_bytes; /* page_bytes = kv_heads * page * head_size, % 16 == 0 */
+  int kv_heads;
+} cb_page_pools;
+/* Room for counts[i] more tokens of slot sequences[i] (NULL: slot i), i < n:
+ * lengths grow, missing pages are popped from the stack in the order of i.
+ * Where a slot's last page is open (partly filled) and held by others too, it
+ * is copied to a popped page first, in every layer (copy on write; the last of
+ * its holders in this call keeps the page itself).  All or nothing: where
+ * pages or columns do not suffice, *error_flag is CB_FLAG_PAGES and nothing
+ * changes.  scratch: cb_pages_scratch(book, n) bytes. */
+CB_API long long cb_pages_scratch(const cb_page_book* book, long long n);
+CB_API int cb_pages_extend(const cb_page_book* book, const cb_page_pools* pools, const int* counts,
+                           const int* sequences, long long n, void* scratch, int* error_flag, cb_stream_t stream);
+/* Slot children[i], which has to be empty, becomes a copy of slot parents[i]
+ * that shares its pages. */
+CB_API int cb_pages_fork(const cb_page_book* book, const int* parents, const int* children, long long n,
+                         int* error_flag, cb_stream_t stream);
+/* The last counts[i] tokens (NULL: all) of slot sequences[i] (NULL: slot i)
+ * are dropped, and the pages that hold none of the rest let go: a page that no
+ * slot holds any more is pushed, in the reverse order of the last of its
+ * dropped table entries.  (So a release undoes the pops of an extend.) */
+CB_API int cb_pages_truncate(const cb_page_book* book, const int* counts, const int* sequences, long long n,
+                             int* error_flag, cb_stream_t stream);
+/* The n held pages become pages 0 .. n-1: in ascending order, those beyond
+ * move to the holes below, in every layer; table, counts and stack follow
+ * (the stack then pops the lowest free page first). */
+CB_API int cb_pages_compact(const cb_page_book* book, const cb_page_pools* pools, void* scratch, int* error_flag,
+                            cb_stream_t stream);
+/* Page source[i] copied to page target[i] in every layer, i < n (no page is
+ * both). */
+CB_API int cb_pages_copy(const cb_page_pools* pools, const int* source, const int* target, long long n,
+                         int* error_flag, cb_stream_t stream);
+
+/* Verification of drafted tokens (speculative sampling).  Greedy counterpart
+ * in the reference: verify_greedy_candidates (chomikgrad/generation.py:15-28).
+ * Row b has n = counts[b] drafted tokens (NULL: tokens), drawn from the rows
+ * of draft[b]; target[b] has the target model's probabilities after each
+ * prefix, one row more.  Token t is accepted while u[b][t] * q_t(x_t) <
+ * p_t(x_t) (float64 products).  At the first refusal i the next token is
+ * drawn from max(p_i - q_i, 0) (from p_i where that is empty), after n
+ * accepted ones from p_n, with the uniform u[b][tokens]: the first index whose
+ * cumulative weight exceeds floor(u * total), the weights trunc(min(w, 1) *
+ * 2^40) summed as 64-bit integers, so that no order of summing shows.
+ * accepted[b] = i; out[b] = the accepted tokens, the drawn one, then -1.  A
+ * NaN in a row that is drawn from, or weights that are all zero, give token -1
+ * and CB_FLAG_NAN; a drafted token outside the vocabulary is refused
+ * (CB_FLAG_INDEX). */
+typedef struct {
+  const void* target; /* (batch, tokens + 1, vocab), vocab contiguous */
+  const void* draft;  /* (batch, tokens, vocab) */
+  int dtype;          /* CB_F32, CB_BF16 or CB_F16, both */
+  long long batch, tokens, vocab;
+  long long target_strides[2], draft_strides[2]; /* elements, over batch, tokens */
+  const long long* drafted; /* (batch, tokens) */
+  const double* uniforms;   /* (batch, tokens + 1), in [0, 1) */
+  const int* counts;
+  int* accepted;  /* batch */
+  long long* out; /* (batch, tokens + 1) */
+  int* error_flag;
+} cb_verify_args;
+CB_API int cb_verify_draft(const cb_verify_args* args, cb_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -50,8 +50,9 @@ def pytest_make_collect_report(collector):
 @pytest.hookimpl(hookwrapper=True)
 def pytest_runtest_makereport(item, call):
     report = (yield).get_result()
-    error = call.excinfo.value if call.excinfo is not None else None
-    if report.failed and isinstance(error, ModuleNotFoundError) and (error.name or "").split(".")[0] == "chomikgrad":
+    # (a child process's ModuleNotFoundError arrives as text)
+    error = str(call.excinfo.value) if call.excinfo is not None else ""
+    if report.failed and "No module named" in error and "chomikgrad" in error:
         report.outcome = "skipped"
         report.longrepr = (str(item.path), 0, NO_FRONT_END)
 
