@@ -4,87 +4,703 @@
 // head h of kv head g = h / (heads / kv_heads):
 //   s_j = scale * ks[page(j), g] * sum_d q_d kq[j, d],  j <= length - n + t
 //   out = sum_j exp(s_j - m) vs[page(j), g] vq[j, :] / sum_j exp(s_j - m)
-// in one pass over the keys, with the running maximum m and sum.
 //
-// One block per (sequence, token, head); each warp takes every fourth key, its
-// lanes hold head_size / 32 neighbouring elements each, and the warps' partial
-// results are joined in shared memory.
+// What bounds it: the cache is read once, 2 * head_size bytes a key and kv
+// head, for 4 flops a byte and query row.  The rows that share a kv head
+// (tokens * heads / kv_heads of them) are multiplied together, so that the
+// bytes stay the bound up to about 32 rows; with 8 rows the multiply-adds
+// alone (184 a clock and SM at the measured 6.47 TB/s) are beyond the FP32
+// units, so the products go to the tensor cores as fp16 m16n8k16 products
+// with float32 sums:
+//   - int8 and e4m3 codes are exact in fp16, and the scales stay outside the
+//     products: one factor for each 16 keys, since a page is 16 tokens or more;
+//   - a query row is scaled by a power of two to below 2 and split into
+//     hi + lo (22 bits); up to 8 rows, the hi parts are rows 0-7 of the tile
+//     and the lo parts rows 8-15, at no cost.  16-bit queries in more than 8
+//     rows are used as they are (exact but for elements 2^-14 below the row's
+//     largest, whose error is below 2^-25 of that);
+//   - the probabilities of a step are taken against the step's own maximum and
+//     split the same way (16-bit outputs of more than 8 rows: hi only, a
+//     relative error of 2^-12 a weight, below the output's own rounding);
+//   - the step's product is then added to the float32 sums with the factor
+//     exp(step maximum - running maximum) * value scale, whose exponents are
+//     added first, so that neither over- nor underflows before the whole does.
+//
+// How the work is laid out.  The keys of all (slot, kv head, block of rows)
+// are one sequence of tiles, cut into equal ranges for a grid that fills the
+// GPU once, whatever the lengths: each block finds its range from the lengths
+// on the device.  An item that a cut divides leaves partial results (maximum,
+// sum, weighted values), joined in a fixed order by a second kernel that is
+// launched along with the first (programmatic dependent launch).
+//
+// Within a tile each warp takes its own 16, 32 or 64 keys (4 KB for any head
+// size) with running maxima of its own, joined at the end of an item: no
+// block barrier inside the loop.  A warp copies its keys through shared memory
+// with 16-byte asynchronous copies, kStages - 1 steps ahead; keys beyond the
+// length are filled with zeros, whatever the page holds there.
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace cb {
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kWarps = kThreads / 32;
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kStages = 4;
+constexpr int kStepBytes = 4096;                 // K and V of one warp's step
+constexpr int kHeadBytes = 64;                   // its scales: 4 of K, 4 of V
+constexpr int kSlotBytes = kStepBytes + kHeadBytes;
+constexpr int kRing = kWarps * kStages * kSlotBytes;
 
-template <int STORAGE>
-__device__ __forceinline__ float decode(uint8_t byte) {
-  if (STORAGE == CB_I8) return static_cast<float>(static_cast<int8_t>(byte));
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(byte, __NV_E4M3)));
+// How the query rows fill the tensor core's 16-row tiles.
+enum { kPacked = 0, kOneTile = 1, kTwoTiles = 2 };
+__host__ __device__ constexpr int rows_of(int mode) { return mode == kPacked ? 8 : 16 * mode; }
+__host__ __device__ constexpr int step_keys(int head_size) { return 2048 / head_size; }
+__host__ __device__ constexpr int tile_keys(int head_size) { return kWarps * step_keys(head_size); }
+
+// ---- loads -------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t shared_of(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_groups() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// Byte offset of 16-byte piece `piece` of row `row` in a buffer of rows of
+// SIZE bytes.  The 16-byte places of a 128-byte line are exchanged by the
+// line's number so that the reads below touch every bank once.
+template <int SIZE>
+__device__ __forceinline__ int swizzled(int row, int piece) {
+  const int at = row * (SIZE / 16) + piece, line = at >> 3;
+  const int turn = SIZE == 128 ? line & 7 : SIZE == 64 ? (line & 1) | ((line & 2) << 1) : (line & 1) << 2;
+  return (line << 7) + (((at & 7) ^ turn) << 4);
+}
+// Key of column n of an 8-key tile, and the first of the SIZE / 8 elements of
+// column n of the value tiles: the orders are free, and these go with `swizzled`.
+__device__ __forceinline__ int key_of(int n) { return (n >> 1) + (n & 1) * 4; }
+template <int SIZE>
+__device__ __forceinline__ int element_of(int n) {
+  if (SIZE == 128) return (((n & 1) << 2) | (n >> 1)) * 16;
+  if (SIZE == 64) return ((n >> 2) + ((n >> 1) & 1) * 2) * 16 + (n & 1) * 8;
+  return n * 4;
+}
+
+template <int WORDS>
+__device__ __forceinline__ void read_words(const char* p, uint32_t* w) {
+  if (WORDS == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else if (WORDS == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+// ---- fp16 operands -------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+
+// Four codes -> two pairs of halves.  int8: the byte x + 128 under the exponent
+// of 1024 is the number 1152 + x.
 template <int STORAGE>
-__global__ void __launch_bounds__(kThreads) attention_kernel(cb_paged_attention_args a) {
-  const cb_paged_cache& c = a.cache;
-  const int h = static_cast<int>(blockIdx.x), t = static_cast<int>(blockIdx.y), b = static_cast<int>(blockIdx.z);
-  const int g = h / static_cast<int>(a.heads / c.kv_heads);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = c.head_size / 32;
+__device__ __forceinline__ void to_halves(uint32_t w, uint32_t& a, uint32_t& b) {
+  if (STORAGE == CB_I8) {
+    w ^= 0x80808080u;
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    const uint32_t lo = __byte_perm(w, 0x64646464u, 0x4140), hi = __byte_perm(w, 0x64646464u, 0x4342);
+    a = bits(__hsub2(*reinterpret_cast<const __half2*>(&lo), bias));
+    b = bits(__hsub2(*reinterpret_cast<const __half2*>(&hi), bias));
+  } else {
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+        : "=r"(a), "=r"(b)
+        : "r"(w));
+  }
+}
+
+__device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  hi = bits(h);
+  lo = bits(__floats2half2_rn(x - __low2float(h), y - __high2float(h)));
+}
+
+__device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// ---- division of the work ------------------------------------------------------
+
+struct Plan {  // of one launch
+  cb_paged_attention_args a;
+  int group, rows, blocks;  // query heads of a kv head, rows of a kv head, blocks of them
+  int4* cuts;               // scratch: for each block, the item that it begins and does not end
+  float* partial;           // scratch: two partial results of each block
+};
+
+struct Slot {
   PagedRow row;
-  const bool ok = paged_row(c, a.sequences, a.counts, a.tokens, b, a.error_flag, &row);
-  const int keys = ok && t < row.count ? row.length - row.count + t + 1 : 0;
-  float q[4], o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
-  for (int i = 0; i < per; ++i)
-    q[i] = load_as_f32(a.q, b * a.q_strides[0] + t * a.q_strides[1] + h * a.q_strides[2] + lane * per + i, a.dtype);
-  for (int j = warp; j < keys; j += kWarps) {
-    const int page = row.table[j / c.page];
-    if (page < 0 || page >= c.pages) {
-      raise_flag(a.error_flag, CB_FLAG_BOOK);
-      continue;
-    }
-    const long long block = static_cast<long long>(page) * c.kv_heads + g;
-    const long long at = (block * c.page + j % c.page) * c.head_size + lane * per;
-    float s = 0.0f;
-    for (int i = 0; i < per; ++i) s += q[i] * decode<STORAGE>(static_cast<const uint8_t*>(c.k_pages)[at + i]);
-    s = warp_sum(s) * (c.k_scale[block] * a.scale * 1.4426950408889634f);
-    const float top = fmaxf(m, s), keep = exp2f(m - top), p = exp2f(s - top);
-    int exponent;  // of the value scale, which may make up for a weight below float32's range
-    const float fraction = frexpf(c.v_scale[block], &exponent);
-    const float weight = exp2f(s - top + exponent) * fraction;
-    l = l * keep + p;
-    for (int i = 0; i < per; ++i)
-      o[i] = o[i] * keep + weight * decode<STORAGE>(static_cast<const uint8_t*>(c.v_pages)[at + i]);
-    m = top;
+  int tiles;
+};
+template <int SIZE>
+__device__ __forceinline__ Slot slot_of(const Plan& p, long long b) {
+  Slot s;
+  if (!paged_row(p.a.cache, p.a.sequences, p.a.counts, p.a.tokens, b, p.a.error_flag, &s.row)) {
+    s.row.length = s.row.count = 0;
+    s.row.table = p.a.cache.table;
   }
-  __shared__ float sm[kWarps], sl[kWarps], so[kWarps][128];
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
+  const int keys = s.row.count > 0 ? s.row.length : 0;  // (an item without keys writes zeros)
+  s.tiles = max(1, (keys + tile_keys(SIZE) - 1) / tile_keys(SIZE));
+  return s;
+}
+
+__device__ __forceinline__ long long block_scan(long long v, long long* shared, long long* total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  long long incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
   }
-  for (int i = 0; i < per; ++i) so[warp][lane * per + i] = o[i];
   __syncthreads();
-  if (static_cast<int>(threadIdx.x) < c.head_size) {
-    float top = -INFINITY, sum = 0.0f, v = 0.0f;
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w]);
-    for (int w = 0; w < kWarps && keys > 0; ++w) {
-      const float f = sm[w] == -INFINITY ? 0.0f : exp2f(sm[w] - top);
-      sum += f * sl[w];
-      v += f * so[w][threadIdx.x];
+  if (lane == 31) shared[warp] = incl;
+  __syncthreads();
+  long long before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) before = all;
+    all += shared[w];
+  }
+  *total = all;
+  return before + incl - v;
+}
+
+// ---- one item ------------------------------------------------------------------
+
+// The sums of one warp: its rows g (and g + 8 of each 16-row tile), columns
+// 2c and 2c + 1 of each value tile, g = lane / 4, c = lane % 4.
+template <int SIZE, int MODE>
+struct Sums {
+  static constexpr int kTiles = MODE == kTwoTiles ? 2 : 1;
+  static constexpr int kHalves = MODE == kPacked ? 1 : 2;
+  float o[kTiles][kHalves][SIZE / 8][2];
+  float m[kTiles][kHalves], l[kTiles][kHalves];
+};
+
+template <int SIZE, int STORAGE, int MODE, int LO>
+__device__ __forceinline__ void warp_item(const Plan& p, const void* query, const Slot& s, int head, int first_row, int tile, int tiles,
+                                          char* ring, Sums<SIZE, MODE>& sums) {
+  using S = Sums<SIZE, MODE>;
+  constexpr int kKeys = step_keys(SIZE), kSubs = kKeys / 16;
+  constexpr int kDots = SIZE / 16;                        // 16-element products of a score
+  constexpr int kKeyWords = SIZE / 16 < 4 ? SIZE / 16 : 4;  // words of one read of a key row
+  constexpr int kKeyReads = SIZE / 16 / kKeyWords;
+  constexpr int kValueWords = SIZE / 32;
+  constexpr int kParts = LO ? 2 : 1;
+  const cb_paged_cache& c = p.a.cache;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
+
+  // limits: row r sees keys below limit[r]; all rows of the block see those below `common`
+  int limit[S::kTiles][S::kHalves];
+  uint32_t q[S::kTiles][kParts][kDots][4];
+  float factor[S::kTiles][S::kHalves];
+#pragma unroll
+  for (int mt = 0; mt < S::kTiles; ++mt) {
+#pragma unroll
+    for (int half = 0; half < S::kHalves; ++half) {
+      const int r = first_row + mt * 16 + half * 8 + g, t = r / p.group;
+      const bool real = r < p.rows && t < s.row.count;
+      limit[mt][half] = real ? s.row.length - s.row.count + t + 1 : 0;
+      const long long at = real ? t * p.a.q_strides[1] + (head * p.group + r % p.group) * p.a.q_strides[2] : 0;
+      float x[kDots][4], largest = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kDots; ++k) {
+        // the elements of word k % kKeyWords of this lane's read k / kKeyWords of a key row
+        const int d = (k / kKeyWords) * 64 + quad * (4 * kKeyWords) + (k % kKeyWords) * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[k][i] = real ? load_as_f32(query, at + d + i, p.a.dtype) : 0.0f;
+          largest = fmaxf(largest, fabsf(x[k][i]));
+        }
+      }
+      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+      // 2^e <= largest < 2^(e + 1); e in [-126, 127], and 2^-e is exact
+      const int e = min(max(static_cast<int>(__float_as_uint(largest) >> 23) - 127, -126), 127);
+      const float down = e == 127 ? 5.877471754111438e-39f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      factor[mt][half] = p.a.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+      for (int k = 0; k < kDots; ++k) {
+#pragma unroll
+        for (int pair = 0; pair < 2; ++pair) {
+          uint32_t hi, lo;
+          split(x[k][2 * pair] * down, x[k][2 * pair + 1] * down, hi, lo);
+          if (MODE == kPacked) {
+            q[mt][0][k][2 * pair] = hi;
+            q[mt][0][k][2 * pair + 1] = lo;
+          } else {
+            q[mt][0][k][2 * pair + half] = hi;
+            if (LO) q[mt][kParts - 1][k][2 * pair + half] = lo;
+          }
+        }
+      }
+      sums.m[mt][half] = -INFINITY;
+      sums.l[mt][half] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < SIZE / 8; ++j) sums.o[mt][half][j][0] = sums.o[mt][half][j][1] = 0.0f;
     }
-    const long long at = ((b * a.tokens + t) * a.heads + h) * c.head_size + threadIdx.x;
-    store_from_f32(a.out, at, a.dtype, sum > 0.0f || sum != sum ? v / sum : 0.0f);
+  }
+  const int common = s.row.length - s.row.count + first_row / p.group + 1;
+  const int length = s.row.count > 0 ? s.row.length : 0;
+
+  // page ids: lane i of a batch holds that of the warp's 16-key piece 32 * batch + i
+  const int shift = 31 - __clz(c.page);
+  auto piece_key = [&](int piece) {
+    return (tile + piece / kSubs) * tile_keys(SIZE) + warp * kKeys + (piece % kSubs) * 16;
+  };
+  auto ids_of = [&](int batch) {
+    const int piece = batch * 32 + lane, key = piece_key(piece);
+    if (piece >= tiles * kSubs || key >= length) return -1;
+    const int page = s.row.table[key >> shift];
+    if (page < 0 || page >= c.pages) {
+      raise_flag(p.a.error_flag, CB_FLAG_BOOK);
+      return -1;
+    }
+    return page;
+  };
+  int ids = ids_of(0), ids_next = ids_of(1), batch = 0;
+
+  const uint32_t ring_at = shared_of(ring);
+  auto prefetch = [&](int step) {
+    if (step < tiles) {
+      const uint32_t slot = ring_at + (step % kStages) * kSlotBytes;
+      if (step * kSubs / 32 > batch) {
+        ids = ids_next;
+        ids_next = ids_of(++batch + 1);
+      }
+#pragma unroll
+      for (int sub = 0; sub < kSubs; ++sub) {
+        const int piece = step * kSubs + sub, key = piece_key(piece);
+        const int page = __shfl_sync(0xffffffffu, ids, piece & 31);
+        const bool held = page >= 0;
+        const long long block = static_cast<long long>(held ? page : 0) * c.kv_heads + head;
+        const long long base = (block * c.page + (key & (c.page - 1))) * SIZE;
+        constexpr int kCopies = SIZE / 32;  // 16 rows of SIZE bytes by 32 lanes
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+          const int at = i * 32 + lane, row = at / (SIZE / 16), part = at % (SIZE / 16);
+          const bool real = held && key + row < length;
+          const uint32_t dst = slot + swizzled<SIZE>(sub * 16 + row, part);
+          copy16(dst, static_cast<const char*>(c.k_pages) + base + at * 16, real);
+          copy16(dst + 2048, static_cast<const char*>(c.v_pages) + base + at * 16, real);
+        }
+        if (lane < 2) copy4(slot + kStepBytes + lane * 16 + sub * 4, (lane ? c.v_scale : c.k_scale) + block, held);
+      }
+    }
+    commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) prefetch(i);
+
+  for (int step = 0; step < tiles; ++step) {
+    wait_groups<kStages - 2>();
+    __syncwarp();  // every lane's copies of this step have landed; every lane has left the slot filled next
+    prefetch(step + kStages - 1);
+    const char* slot = ring + (step % kStages) * kSlotBytes;
+    const int key = (tile + step) * tile_keys(SIZE) + warp * kKeys;
+    const float* scales = reinterpret_cast<const float*>(slot + kStepBytes);
+
+    float score[S::kTiles][2 * kSubs][4];
+#pragma unroll
+    for (int n = 0; n < 2 * kSubs; ++n) {
+#pragma unroll
+      for (int mt = 0; mt < S::kTiles; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) score[mt][n][i] = 0.0f;
+      const int row = n * 8 + key_of(g);
+#pragma unroll
+      for (int r = 0; r < kKeyReads; ++r) {
+        uint32_t w[kKeyWords];
+        const int element = r * 64 + quad * (4 * kKeyWords);
+        read_words<kKeyWords>(slot + swizzled<SIZE>(row, element / 16) + element % 16, w);
+#pragma unroll
+        for (int k = 0; k < kKeyWords; ++k) {
+          uint32_t b0, b1;
+          to_halves<STORAGE>(w[k], b0, b1);
+#pragma unroll
+          for (int mt = 0; mt < S::kTiles; ++mt)
+#pragma unroll
+            for (int part = 0; part < kParts; ++part)
+              mma(score[mt][n], q[mt][part][r * kKeyWords + k], b0, b1);
+        }
+      }
+    }
+
+    uint32_t weight[S::kTiles][kParts][kSubs][4];
+    float fold[S::kTiles][S::kHalves][kSubs];
+    bool grows = false;
+    float top[S::kTiles][S::kHalves];
+#pragma unroll
+    for (int mt = 0; mt < S::kTiles; ++mt) {
+#pragma unroll
+      for (int half = 0; half < S::kHalves; ++half) {
+        float x[2 * kSubs][2], most = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < 2 * kSubs; ++n) {
+          const float f = factor[mt][half] * scales[n / 2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float v = MODE == kPacked ? score[mt][n][i] + score[mt][n][2 + i] : score[mt][n][2 * half + i];
+            v *= f;
+            // columns 2 quad and 2 quad + 1
+            if (key + kKeys > common && key + n * 8 + quad + 4 * i >= limit[mt][half]) v = -INFINITY;
+            x[n][i] = v;
+            most = fmaxf(most, v);
+          }
+        }
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const float base = most == -INFINITY ? 0.0f : most;
+        float sum = 0.0f;
+#pragma unroll
+        for (int n = 0; n < 2 * kSubs; ++n) {
+          const float e0 = exp2f(x[n][0] - base), e1 = exp2f(x[n][1] - base);
+          sum += e0 + e1;
+          uint32_t hi, lo;
+          split(e0, e1, hi, lo);
+          if (MODE == kPacked) {
+            weight[mt][0][n / 2][2 * (n & 1)] = hi;
+            weight[mt][0][n / 2][2 * (n & 1) + 1] = lo;
+          } else {
+            weight[mt][0][n / 2][2 * (n & 1) + half] = hi;
+            if (LO) weight[mt][kParts - 1][n / 2][2 * (n & 1) + half] = lo;
+          }
+        }
+        const float old = sums.m[mt][half], now = fmaxf(old, most);
+        const float against = now == -INFINITY ? 0.0f : now;
+        grows = grows || now > old;
+        top[mt][half] = exp2f(old - against);
+        sums.l[mt][half] = sums.l[mt][half] * top[mt][half] + sum * exp2f(most - against);
+        sums.m[mt][half] = now;
+#pragma unroll
+        for (int sub = 0; sub < kSubs; ++sub) {
+          // exp2(most - now) * value scale = exp2(most - now + its exponent) * its fraction
+          const float vs = scales[4 + sub];
+          const uint32_t word = __float_as_uint(vs);
+          const int e = static_cast<int>(word >> 23 & 0xffu) - 127;
+          const bool normal = e > -127 && e < 128;
+          const float fraction = normal ? __uint_as_float((word & 0x807fffffu) | 0x3f800000u) : vs;
+          fold[mt][half][sub] = exp2f(most - against + (normal ? static_cast<float>(e) : 0.0f)) * fraction;
+        }
+      }
+    }
+    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+      for (int mt = 0; mt < S::kTiles; ++mt)
+#pragma unroll
+        for (int half = 0; half < S::kHalves; ++half)
+#pragma unroll
+          for (int j = 0; j < SIZE / 8; ++j) {
+            sums.o[mt][half][j][0] *= top[mt][half];
+            sums.o[mt][half][j][1] *= top[mt][half];
+          }
+    }
+#pragma unroll
+    for (int sub = 0; sub < kSubs; ++sub) {
+      uint32_t v[4][kValueWords];
+      const int element = element_of<SIZE>(g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)  // keys of columns 2 quad, 2 quad + 1 of both 8-key tiles
+        read_words<kValueWords>(slot + 2048 + swizzled<SIZE>(sub * 16 + quad + 4 * i, element / 16) + element % 16,
+                                v[i]);
+#pragma unroll
+      for (int w = 0; w < kValueWords; ++w) {
+        uint32_t b[4][2];  // of the word's four elements: keys 0-7, keys 8-15
+#pragma unroll
+        for (int pair = 0; pair < 2; ++pair) {
+          to_halves<STORAGE>(__byte_perm(v[2 * pair][w], v[2 * pair + 1][w], 0x5140), b[0][pair], b[1][pair]);
+          to_halves<STORAGE>(__byte_perm(v[2 * pair][w], v[2 * pair + 1][w], 0x7362), b[2][pair], b[3][pair]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int mt = 0; mt < S::kTiles; ++mt) {
+            float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) mma(t, weight[mt][part][sub], b[i][0], b[i][1]);
+            float(*o)[SIZE / 8][2] = sums.o[mt];
+            if (MODE == kPacked) {
+              o[0][w * 4 + i][0] += fold[mt][0][sub] * (t[0] + t[2]);
+              o[0][w * 4 + i][1] += fold[mt][0][sub] * (t[1] + t[3]);
+            } else {
+              o[0][w * 4 + i][0] += fold[mt][0][sub] * t[0];
+              o[0][w * 4 + i][1] += fold[mt][0][sub] * t[1];
+              o[S::kHalves - 1][w * 4 + i][0] += fold[mt][S::kHalves - 1][sub] * t[2];
+              o[S::kHalves - 1][w * 4 + i][1] += fold[mt][S::kHalves - 1][sub] * t[3];
+            }
+          }
+        }
+      }
+    }
+  }
+  wait_groups<0>();
+#pragma unroll
+  for (int mt = 0; mt < S::kTiles; ++mt)
+#pragma unroll
+    for (int half = 0; half < S::kHalves; ++half) {
+      float& l = sums.l[mt][half];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+    }
+}
+
+// Where row r of an item goes; r past the item's rows: nowhere.
+template <int SIZE>
+__device__ __forceinline__ long long out_row(const Plan& p, long long b, int head, int r) {
+  return ((b * p.a.tokens + r / p.group) * p.a.heads + head * p.group + r % p.group) * SIZE;
+}
+__device__ __forceinline__ void store4(const Plan& p, long long at, const float* v) {
+  if (p.a.dtype == CB_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(p.a.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    uint2 w;
+    if (p.a.dtype == CB_BF16) {
+      __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+      w = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+    } else {
+      w = make_uint2(bits(__floats2half2_rn(v[0], v[1])), bits(__floats2half2_rn(v[2], v[3])));
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.a.out) + at) = w;
   }
 }
+
+// Partial results: maxima and sums of the rows, then the rows.
+template <int SIZE, int MODE>
+__host__ __device__ constexpr int partial_floats() { return rows_of(MODE) * (SIZE + 2); }
+
+template <int SIZE, int STORAGE, int MODE, int LO>
+__global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_constant__ Plan p) {
+  using S = Sums<SIZE, MODE>;
+  constexpr int kRows = rows_of(MODE);
+  extern __shared__ __align__(128) char shared[];
+  __shared__ long long scan[kWarps];
+  __shared__ float most[kWarps][kRows], total[kWarps][kRows];
+  __shared__ long long found[2];
+  const long long batch = p.a.batch;
+  const int items = p.a.cache.kv_heads * p.blocks;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  pdl_launch_dependents();
+  // the tiles of all slots, and this block's range of them
+  long long mine = 0, all;
+  for (long long b = threadIdx.x; b < batch; b += kThreads) mine += slot_of<SIZE>(p, b).tiles;
+  block_scan(mine, scan, &all);
+  all *= items;
+  const long long per = (all + gridDim.x - 1) / gridDim.x;
+  long long at = per * blockIdx.x;
+  const long long end = at + per < all ? at + per : all;
+  if (threadIdx.x == 0) p.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (at >= end) return;
+  long long before = 0;
+  for (long long first = 0; first < batch; first += kThreads) {
+    const long long b = first + threadIdx.x;
+    const long long tiles = b < batch ? static_cast<long long>(slot_of<SIZE>(p, b).tiles) * items : 0;
+    long long sum;
+    const long long lower = before + block_scan(tiles, scan, &sum);
+    if (lower <= at && at < lower + tiles) {
+      found[0] = b;
+      found[1] = lower;
+    }
+    before += sum;
+    if (before > at) break;
+  }
+  __syncthreads();
+  long long b = found[0], origin = found[1];
+  Slot s = slot_of<SIZE>(p, b);
+  const long long range = at;
+
+  while (at < end) {
+    if (at - origin >= static_cast<long long>(s.tiles) * items) {
+      origin += static_cast<long long>(s.tiles) * items;
+      s = slot_of<SIZE>(p, ++b);
+    }
+    const int item = static_cast<int>((at - origin) / s.tiles), tile = static_cast<int>((at - origin) % s.tiles);
+    const int head = item / p.blocks, first_row = item % p.blocks * kRows;
+    const int tiles = static_cast<int>(min(static_cast<long long>(s.tiles - tile), end - at));
+    Sums<SIZE, MODE> sums;
+    const void* query = static_cast<const char*>(p.a.q) + b * p.a.q_strides[0] * (p.a.dtype == CB_F32 ? 4 : 2);
+    warp_item<SIZE, STORAGE, MODE, LO>(p, query, s, head, first_row, tile, tiles,
+                                       shared + warp * kStages * kSlotBytes, sums);
+
+    // join the warps
+    __syncthreads();  // every warp is done with the ring
+    float* rows = reinterpret_cast<float*>(shared);  // (warps, kRows, SIZE)
+#pragma unroll
+    for (int mt = 0; mt < S::kTiles; ++mt)
+#pragma unroll
+      for (int half = 0; half < S::kHalves; ++half) {
+        const int r = mt * 16 + half * 8 + (lane >> 2);
+        if ((lane & 3) == 0) {
+          most[warp][r] = sums.m[mt][half];
+          total[warp][r] = sums.l[mt][half];
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          float* to = rows + (warp * kRows + r) * SIZE + element_of<SIZE>(2 * (lane & 3) + n);
+#pragma unroll
+          for (int j = 0; j < SIZE / 8; j += 4)
+            *reinterpret_cast<float4*>(to + j) =
+                make_float4(sums.o[mt][half][j][n], sums.o[mt][half][j + 1][n], sums.o[mt][half][j + 2][n],
+                            sums.o[mt][half][j + 3][n]);
+        }
+      }
+    __syncthreads();
+    const bool whole = tile == 0 && tiles == s.tiles;
+    const bool begins = at == range;  // the block's first item takes its first partial result
+    float* partial = p.partial + (2LL * blockIdx.x + (begins ? 0 : 1)) * partial_floats<SIZE, MODE>();
+    for (int i = threadIdx.x; i < kRows * SIZE / 4; i += kThreads) {
+      const int r = i / (SIZE / 4), d = i % (SIZE / 4) * 4;
+      float top = -INFINITY, sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, most[w][r]);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = most[w][r] == -INFINITY ? 0.0f : exp2f(most[w][r] - top);
+        const float4 x = *reinterpret_cast<const float4*>(rows + (w * kRows + r) * SIZE + d);
+        sum += f * total[w][r];
+        v[0] += f * x.x; v[1] += f * x.y; v[2] += f * x.z; v[3] += f * x.w;
+      }
+      const int row = first_row + r;
+      if (whole) {
+        if (row < p.rows) {
+          const bool real = row / p.group < s.row.count && sum != 0.0f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = real ? v[k] / sum : 0.0f;
+          store4(p, out_row<SIZE>(p, b, head, row) + d, v);
+        }
+      } else {
+        *reinterpret_cast<float4*>(partial + 2 * kRows + r * SIZE + d) = make_float4(v[0], v[1], v[2], v[3]);
+        if (d == 0) {
+          partial[r] = top;
+          partial[kRows + r] = sum;
+        }
+      }
+    }
+    if (!whole && tile == 0 && threadIdx.x == 0) {
+      const long long last = (at + s.tiles - 1) / per;  // block of the item's last tile
+      p.cuts[blockIdx.x] = make_int4(static_cast<int>(b), item, static_cast<int>(last), begins ? 0 : 1);
+    }
+    at += tiles;
+    __syncthreads();  // the joined rows are read; the ring is free again
+  }
+}
+
+// The items that were cut: one block for each block that began one.
+template <int SIZE, int MODE>
+__global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ Plan p) {
+  constexpr int kRows = rows_of(MODE), kFloats = partial_floats<SIZE, MODE>();
+  pdl_wait();
+  const int4 cut = p.cuts[blockIdx.x];
+  if (cut.x < 0) return;
+  const int head = cut.y / p.blocks, first_row = cut.y % p.blocks * kRows, parts = cut.z - static_cast<int>(blockIdx.x) + 1;
+  // its first part, then the first partial results of the following blocks
+  const float* first = p.partial + (2LL * blockIdx.x + cut.w) * kFloats;
+  const float* rest = p.partial + 2LL * blockIdx.x * kFloats;
+  const int count = p.a.counts != nullptr ? p.a.counts[cut.x] : static_cast<int>(p.a.tokens);
+  for (int i = threadIdx.x; i < kRows * SIZE / 4; i += kThreads) {
+    const int r = i / (SIZE / 4), d = i % (SIZE / 4) * 4, row = first_row + r;
+    if (row >= p.rows) continue;
+    float top = -INFINITY, sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = 0; k < parts; ++k) top = fmaxf(top, (k ? rest + 2LL * k * kFloats : first)[r]);
+    for (int k = 0; k < parts; ++k) {
+      const float* part = k ? rest + 2LL * k * kFloats : first;
+      const float f = part[r] == -INFINITY ? 0.0f : exp2f(part[r] - top);
+      const float4 x = *reinterpret_cast<const float4*>(part + 2 * kRows + r * SIZE + d);
+      sum += f * part[kRows + r];
+      v[0] += f * x.x; v[1] += f * x.y; v[2] += f * x.z; v[3] += f * x.w;
+    }
+    const bool real = row / p.group < count && sum != 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = real ? v[k] / sum : 0.0f;
+    store4(p, out_row<SIZE>(p, cut.x, head, row) + d, v);
+  }
+}
+
+// ---- launch --------------------------------------------------------------------
 
 int attention_check(const cb_paged_attention_args& a) {
   const int status = paged_cache_check(a.cache, "cb_paged_attention");
   if (status != CB_OK) return status;
   CB_REQUIRE(a.dtype == CB_F32 || a.dtype == CB_BF16 || a.dtype == CB_F16,
              "cb_paged_attention: q must be float32, bfloat16 or float16");
-  CB_REQUIRE(a.heads >= 1 && a.heads % a.cache.kv_heads == 0, "cb_paged_attention: %lld heads for %d kv heads",
-             a.heads, a.cache.kv_heads);
-  CB_REQUIRE(a.batch >= 0 && a.batch <= 65535 && a.tokens >= 0 && a.tokens <= 65535,
+  CB_REQUIRE(a.heads >= 1 && a.heads <= (1 << 20) && a.heads % a.cache.kv_heads == 0,
+             "cb_paged_attention: %lld heads for %d kv heads", a.heads, a.cache.kv_heads);
+  CB_REQUIRE(a.batch >= 0 && a.batch <= 65535 && a.tokens >= 0 && a.tokens <= 65535 &&
+                 a.tokens * (a.heads / a.cache.kv_heads) < (1LL << 30),
              "cb_paged_attention: %lld sequences of %lld tokens", a.batch, a.tokens);
   return CB_OK;
+}
+
+template <int SIZE, int STORAGE, int MODE, int LO>
+int resident_blocks() {
+  static thread_local int device = -1, per_sm = 0;
+  int now = 0;
+  cudaGetDevice(&now);
+  if (now != device) {
+    auto kernel = attention_kernel<SIZE, STORAGE, MODE, LO>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, kRing) != cudaSuccess)
+      per_sm = 0;
+    device = per_sm > 0 ? now : -1;
+  }
+  return per_sm;
+}
+
+// Calls f with the template arguments of a launch: more rows than a packed tile
+// holds take 16- or 32-row tiles, float32 ones with their low parts.
+template <typename F>
+long long with_variant(const cb_paged_attention_args& a, F f) {
+  const long long rows = a.tokens * (a.heads / a.cache.kv_heads);
+  auto by_rows = [&](auto size, auto storage) {
+    using Z = std::integral_constant<int, 0>;
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, kTwoTiles>;
+    if (rows <= 8) return f(size, storage, Z{}, Z{});
+    if (a.dtype == CB_F32) return f(size, storage, One{}, One{});
+    return rows <= 16 ? f(size, storage, One{}, Z{}) : f(size, storage, Two{}, Z{});
+  };
+  auto by_storage = [&](auto size) {
+    return a.cache.storage == CB_I8 ? by_rows(size, std::integral_constant<int, CB_I8>{})
+                                    : by_rows(size, std::integral_constant<int, CB_E4M3>{});
+  };
+  if (a.cache.head_size == 32) return by_storage(std::integral_constant<int, 32>{});
+  if (a.cache.head_size == 64) return by_storage(std::integral_constant<int, 64>{});
+  return by_storage(std::integral_constant<int, 128>{});
+}
+
+// Blocks that fill the GPU once, and no more than there can be tiles.
+template <int SIZE, int MODE>
+long long grid_of(const cb_paged_attention_args& a, int per_sm) {
+  const long long rows = a.tokens * (a.heads / a.cache.kv_heads);
+  const long long blocks = (rows + rows_of(MODE) - 1) / rows_of(MODE);
+  const long long tiles = (a.cache.columns * a.cache.page + tile_keys(SIZE) - 1) / tile_keys(SIZE);
+  const long long most = a.batch * a.cache.kv_heads * blocks * tiles, fill = 1LL * per_sm * sm_count();
+  return most < fill ? most : fill;
 }
 
 }  // namespace
@@ -95,23 +711,42 @@ using namespace cb;
 extern "C" {
 
 long long cb_paged_attention_scratch(const cb_paged_attention_args* args) {
-  (void)args;
-  return 0;
+  if (args == nullptr || attention_check(*args) != CB_OK || args->batch == 0 || args->tokens == 0) return 0;
+  return with_variant(*args, [&](auto size, auto storage, auto mode, auto lo) -> long long {
+    const int per_sm = resident_blocks<size.value, storage.value, mode.value, lo.value>();
+    return grid_of<size.value, mode.value>(*args, per_sm) * (16 + 8LL * partial_floats<size.value, mode.value>());
+  });
 }
 
 int cb_paged_attention(const cb_paged_attention_args* args, void* scratch, cb_stream_t stream) {
-  (void)scratch;
   CB_REQUIRE(args != nullptr, "cb_paged_attention: null arguments");
   const cb_paged_attention_args& a = *args;
   const int status = attention_check(a);
   if (status != CB_OK) return status;
   if (a.batch == 0 || a.tokens == 0) return CB_OK;
-  CB_REQUIRE(a.q != nullptr && a.out != nullptr, "cb_paged_attention: a null pointer");
-  const dim3 grid(static_cast<unsigned>(a.heads), static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.batch));
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a.cache.storage == CB_I8) attention_kernel<CB_I8><<<grid, kThreads, 0, s>>>(a);
-  else attention_kernel<CB_E4M3><<<grid, kThreads, 0, s>>>(a);
-  return check_launch("cb_paged_attention");
+  CB_REQUIRE(a.q != nullptr && a.out != nullptr && scratch != nullptr, "cb_paged_attention: a null pointer");
+  CB_REQUIRE(reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && reinterpret_cast<uintptr_t>(scratch) % 16 == 0,
+             "cb_paged_attention: out and scratch must be 16-byte aligned");
+  return static_cast<int>(with_variant(a, [&](auto size, auto storage, auto mode, auto lo) -> long long {
+    constexpr int SIZE = size.value, STORAGE = storage.value, MODE = mode.value, LO = lo.value;
+    const int per_sm = resident_blocks<SIZE, STORAGE, MODE, LO>();
+    CB_REQUIRE(per_sm >= 1, "cb_paged_attention: the kernel does not fit this device");
+    const long long grid = grid_of<SIZE, MODE>(a, per_sm);
+    Plan p;
+    p.a = a;
+    p.group = static_cast<int>(a.heads / a.cache.kv_heads);
+    p.rows = static_cast<int>(a.tokens * p.group);
+    p.blocks = (p.rows + rows_of(MODE) - 1) / rows_of(MODE);
+    p.cuts = static_cast<int4*>(scratch);
+    p.partial = reinterpret_cast<float*>(p.cuts + grid);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const dim3 blocks(static_cast<unsigned>(grid));
+    launch(attention_kernel<SIZE, STORAGE, MODE, LO>, blocks, dim3(kThreads), kRing, s, false, p);
+    const int status = check_launch("cb_paged_attention");
+    if (status != CB_OK) return status;
+    launch(join_kernel<SIZE, MODE>, blocks, dim3(kThreads), 0, s, true, p);
+    return check_launch("cb_paged_attention: join");
+  }));
 }
 
 }  // extern "C"
