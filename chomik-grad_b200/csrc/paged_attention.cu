@@ -59,6 +59,14 @@ __host__ __device__ constexpr int rows_of(int mode) { return mode == kPacked ? 8
 __host__ __device__ constexpr int step_keys(int head_size) { return 2048 / head_size; }
 __host__ __device__ constexpr int tile_keys(int head_size) { return kWarps * step_keys(head_size); }
 
+// Shared memory of a block: the ring, and the queries that are not in registers.
+__host__ __device__ constexpr int shared_bytes(int head_size, int mode, int lo) {
+  return kRing + (mode == kPacked ? 0 : mode * (lo ? 2 : 1) * (head_size / 16) * 512);
+}
+// Tiles' time that beginning an item costs (queries, first loads, joining the
+// warps): counted when the work is divided.
+constexpr int kItemCost = 2;
+
 // ---- loads -------------------------------------------------------------------
 
 __device__ __forceinline__ uint32_t shared_of(const void* p) {
@@ -136,12 +144,49 @@ __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& 
   lo = bits(__floats2half2_rn(x - __low2float(h), y - __high2float(h)));
 }
 
+// c (+)= a b; FIRST: from zero.
+template <bool FIRST>
 __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  if (FIRST) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+  } else {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+
+// 2^x by the hardware's instruction: its relative error is below 2^-22, and
+// results below 2^-126 are zero (weights are at most one).
+__device__ __forceinline__ float exp2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 2^x as the square of this: a sum may be large enough that its share is
+// kept where 2^x itself would be below float32's range.
+__device__ __forceinline__ float root2_of(float x) { return exp2_of(0.5f * x); }
+
+// Pairs of float32: two sums or products in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(r))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(r))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+        "l"(reinterpret_cast<unsigned long long&>(c)));
+  return r;
 }
 
 // ---- division of the work ------------------------------------------------------
@@ -198,13 +243,13 @@ template <int SIZE, int MODE>
 struct Sums {
   static constexpr int kTiles = MODE == kTwoTiles ? 2 : 1;
   static constexpr int kHalves = MODE == kPacked ? 1 : 2;
-  float o[kTiles][kHalves][SIZE / 8][2];
+  float2 o[kTiles][kHalves][SIZE / 8];
   float m[kTiles][kHalves], l[kTiles][kHalves];
 };
 
 template <int SIZE, int STORAGE, int MODE, int LO>
 __device__ __forceinline__ void warp_item(const Plan& p, const void* query, const Slot& s, int head, int first_row, int tile, int tiles,
-                                          char* ring, Sums<SIZE, MODE>& sums) {
+                                          char* ring, uint4* queries, Sums<SIZE, MODE>& sums) {
   using S = Sums<SIZE, MODE>;
   constexpr int kKeys = step_keys(SIZE), kSubs = kKeys / 16;
   constexpr int kDots = SIZE / 16;                        // 16-element products of a score
@@ -217,7 +262,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
 
   // limits: row r sees keys below limit[r]; all rows of the block see those below `common`
   int limit[S::kTiles][S::kHalves];
-  uint32_t q[S::kTiles][kParts][kDots][4];
+  uint32_t q[kDots][4];  // a packed tile's queries; others lie in `queries`
   float factor[S::kTiles][S::kHalves];
 #pragma unroll
   for (int mt = 0; mt < S::kTiles; ++mt) {
@@ -251,18 +296,19 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
           uint32_t hi, lo;
           split(x[k][2 * pair] * down, x[k][2 * pair + 1] * down, hi, lo);
           if (MODE == kPacked) {
-            q[mt][0][k][2 * pair] = hi;
-            q[mt][0][k][2 * pair + 1] = lo;
-          } else {
-            q[mt][0][k][2 * pair + half] = hi;
-            if (LO) q[mt][kParts - 1][k][2 * pair + half] = lo;
+            q[k][2 * pair] = hi;
+            q[k][2 * pair + 1] = lo;
+          } else if (k % kWarps == warp) {  // every warp has them all; each stores a part
+            uint32_t* to = reinterpret_cast<uint32_t*>(queries + (mt * kParts * kDots + k) * 32 + lane);
+            to[2 * pair + half] = hi;
+            if (LO) to[kDots * 128 + 2 * pair + half] = lo;
           }
         }
       }
       sums.m[mt][half] = -INFINITY;
       sums.l[mt][half] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < SIZE / 8; ++j) sums.o[mt][half][j][0] = sums.o[mt][half][j][1] = 0.0f;
+      for (int j = 0; j < SIZE / 8; ++j) sums.o[mt][half][j] = make_float2(0.0f, 0.0f);
     }
   }
   const int common = s.row.length - s.row.count + first_row / p.group + 1;
@@ -301,13 +347,15 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
         const long long block = static_cast<long long>(held ? page : 0) * c.kv_heads + head;
         const long long base = (block * c.page + (key & (c.page - 1))) * SIZE;
         constexpr int kCopies = SIZE / 32;  // 16 rows of SIZE bytes by 32 lanes
+        const char* k = static_cast<const char*>(c.k_pages) + base + lane * 16;
+        const char* v = static_cast<const char*>(c.v_pages) + base + lane * 16;
+        const int rows = held ? length - key : 0;  // that exist
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
-          const int at = i * 32 + lane, row = at / (SIZE / 16), part = at % (SIZE / 16);
-          const bool real = held && key + row < length;
+          const int row = (i * 32 + lane) / (SIZE / 16), part = lane % (SIZE / 16);
           const uint32_t dst = slot + swizzled<SIZE>(sub * 16 + row, part);
-          copy16(dst, static_cast<const char*>(c.k_pages) + base + at * 16, real);
-          copy16(dst + 2048, static_cast<const char*>(c.v_pages) + base + at * 16, real);
+          copy16(dst, k + i * 512, row < rows);
+          copy16(dst + 2048, v + i * 512, row < rows);
         }
         if (lane < 2) copy4(slot + kStepBytes + lane * 16 + sub * 4, (lane ? c.v_scale : c.k_scale) + block, held);
       }
@@ -317,6 +365,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) prefetch(i);
 
+  if (MODE != kPacked) __syncthreads();
   for (int step = 0; step < tiles; ++step) {
     wait_groups<kStages - 2>();
     __syncwarp();  // every lane's copies of this step have landed; every lane has left the slot filled next
@@ -328,10 +377,6 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
     float score[S::kTiles][2 * kSubs][4];
 #pragma unroll
     for (int n = 0; n < 2 * kSubs; ++n) {
-#pragma unroll
-      for (int mt = 0; mt < S::kTiles; ++mt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) score[mt][n][i] = 0.0f;
       const int row = n * 8 + key_of(g);
 #pragma unroll
       for (int r = 0; r < kKeyReads; ++r) {
@@ -343,10 +388,22 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
           uint32_t b0, b1;
           to_halves<STORAGE>(w[k], b0, b1);
 #pragma unroll
-          for (int mt = 0; mt < S::kTiles; ++mt)
+          for (int mt = 0; mt < S::kTiles; ++mt) {
 #pragma unroll
-            for (int part = 0; part < kParts; ++part)
-              mma(score[mt][n], q[mt][part][r * kKeyWords + k], b0, b1);
+            for (int part = 0; part < kParts; ++part) {
+              const int dot = r * kKeyWords + k;
+              uint32_t a[4];
+              if (MODE == kPacked) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a[i] = q[dot][i];
+              } else {
+                const uint4 v = queries[((mt * kParts + part) * kDots + dot) * 32 + lane];
+                a[0] = v.x; a[1] = v.y; a[2] = v.z; a[3] = v.w;
+              }
+              if (dot == 0 && part == 0) mma<true>(score[mt][n], a, b0, b1);
+              else mma<false>(score[mt][n], a, b0, b1);
+            }
+          }
         }
       }
     }
@@ -354,7 +411,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
     uint32_t weight[S::kTiles][kParts][kSubs][4];
     float fold[S::kTiles][S::kHalves][kSubs];
     bool grows = false;
-    float top[S::kTiles][S::kHalves];
+    float root[S::kTiles][S::kHalves];
 #pragma unroll
     for (int mt = 0; mt < S::kTiles; ++mt) {
 #pragma unroll
@@ -366,20 +423,25 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             float v = MODE == kPacked ? score[mt][n][i] + score[mt][n][2 + i] : score[mt][n][2 * half + i];
-            v *= f;
-            // columns 2 quad and 2 quad + 1
-            if (key + kKeys > common && key + n * 8 + quad + 4 * i >= limit[mt][half]) v = -INFINITY;
-            x[n][i] = v;
-            most = fmaxf(most, v);
+            x[n][i] = v * f;
           }
         }
+        if (key + kKeys > common) {  // (the same for the warp) columns 2 quad and 2 quad + 1
+#pragma unroll
+          for (int n = 0; n < 2 * kSubs; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (key + n * 8 + quad + 4 * i >= limit[mt][half]) x[n][i] = -INFINITY;
+        }
+#pragma unroll
+        for (int n = 0; n < 2 * kSubs; ++n) most = fmaxf(most, fmaxf(x[n][0], x[n][1]));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         const float base = most == -INFINITY ? 0.0f : most;
         float sum = 0.0f;
 #pragma unroll
         for (int n = 0; n < 2 * kSubs; ++n) {
-          const float e0 = exp2f(x[n][0] - base), e1 = exp2f(x[n][1] - base);
+          const float e0 = exp2_of(x[n][0] - base), e1 = exp2_of(x[n][1] - base);
           sum += e0 + e1;
           uint32_t hi, lo;
           split(e0, e1, hi, lo);
@@ -394,8 +456,9 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
         const float old = sums.m[mt][half], now = fmaxf(old, most);
         const float against = now == -INFINITY ? 0.0f : now;
         grows = grows || now > old;
-        top[mt][half] = exp2f(old - against);
-        sums.l[mt][half] = sums.l[mt][half] * top[mt][half] + sum * exp2f(most - against);
+        const float r = root2_of(old - against);
+        root[mt][half] = r;
+        sums.l[mt][half] = sums.l[mt][half] * r * r + sum * exp2_of(most - against);
         sums.m[mt][half] = now;
 #pragma unroll
         for (int sub = 0; sub < kSubs; ++sub) {
@@ -405,7 +468,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
           const int e = static_cast<int>(word >> 23 & 0xffu) - 127;
           const bool normal = e > -127 && e < 128;
           const float fraction = normal ? __uint_as_float((word & 0x807fffffu) | 0x3f800000u) : vs;
-          fold[mt][half][sub] = exp2f(most - against + (normal ? static_cast<float>(e) : 0.0f)) * fraction;
+          fold[mt][half][sub] = exp2_of(most - against + (normal ? static_cast<float>(e) : 0.0f)) * fraction;
         }
       }
     }
@@ -416,8 +479,9 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
         for (int half = 0; half < S::kHalves; ++half)
 #pragma unroll
           for (int j = 0; j < SIZE / 8; ++j) {
-            sums.o[mt][half][j][0] *= top[mt][half];
-            sums.o[mt][half][j][1] *= top[mt][half];
+            const float r = root[mt][half];
+            sums.o[mt][half][j].x = sums.o[mt][half][j].x * r * r;
+            sums.o[mt][half][j].y = sums.o[mt][half][j].y * r * r;
           }
     }
 #pragma unroll
@@ -440,18 +504,19 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
           for (int mt = 0; mt < S::kTiles; ++mt) {
-            float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int part = 0; part < kParts; ++part) mma(t, weight[mt][part][sub], b[i][0], b[i][1]);
-            float(*o)[SIZE / 8][2] = sums.o[mt];
+            float t[4];
+            mma<true>(t, weight[mt][0][sub], b[i][0], b[i][1]);
+            if (LO) mma<false>(t, weight[mt][kParts - 1][sub], b[i][0], b[i][1]);
+            float2(*o)[SIZE / 8] = sums.o[mt];
+            const float f = fold[mt][0][sub], f8 = fold[mt][S::kHalves - 1][sub];
+            const float2 first = make_float2(t[0], t[1]), second = make_float2(t[2], t[3]);
+            float2& mine = o[0][w * 4 + i];
             if (MODE == kPacked) {
-              o[0][w * 4 + i][0] += fold[mt][0][sub] * (t[0] + t[2]);
-              o[0][w * 4 + i][1] += fold[mt][0][sub] * (t[1] + t[3]);
+              mine = fma2(make_float2(f, f), add2(first, second), mine);
             } else {
-              o[0][w * 4 + i][0] += fold[mt][0][sub] * t[0];
-              o[0][w * 4 + i][1] += fold[mt][0][sub] * t[1];
-              o[S::kHalves - 1][w * 4 + i][0] += fold[mt][S::kHalves - 1][sub] * t[2];
-              o[S::kHalves - 1][w * 4 + i][1] += fold[mt][S::kHalves - 1][sub] * t[3];
+              float2& other = o[S::kHalves - 1][w * 4 + i];
+              mine = fma2(make_float2(f, f), first, mine);
+              other = fma2(make_float2(f8, f8), second, other);
             }
           }
         }
@@ -494,7 +559,7 @@ template <int SIZE, int MODE>
 __host__ __device__ constexpr int partial_floats() { return rows_of(MODE) * (SIZE + 2); }
 
 template <int SIZE, int STORAGE, int MODE, int LO>
-__global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_constant__ Plan p) {
+__global__ void __launch_bounds__(kThreads, MODE == kTwoTiles ? 2 : 3) attention_kernel(const __grid_constant__ Plan p) {
   using S = Sums<SIZE, MODE>;
   constexpr int kRows = rows_of(MODE);
   extern __shared__ __align__(128) char shared[];
@@ -508,7 +573,7 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
   pdl_launch_dependents();
   // the tiles of all slots, and this block's range of them
   long long mine = 0, all;
-  for (long long b = threadIdx.x; b < batch; b += kThreads) mine += slot_of<SIZE>(p, b).tiles;
+  for (long long b = threadIdx.x; b < batch; b += kThreads) mine += slot_of<SIZE>(p, b).tiles + kItemCost;
   block_scan(mine, scan, &all);
   all *= items;
   const long long per = (all + gridDim.x - 1) / gridDim.x;
@@ -519,7 +584,7 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
   long long before = 0;
   for (long long first = 0; first < batch; first += kThreads) {
     const long long b = first + threadIdx.x;
-    const long long tiles = b < batch ? static_cast<long long>(slot_of<SIZE>(p, b).tiles) * items : 0;
+    const long long tiles = b < batch ? (slot_of<SIZE>(p, b).tiles + kItemCost) * static_cast<long long>(items) : 0;
     long long sum;
     const long long lower = before + block_scan(tiles, scan, &sum);
     if (lower <= at && at < lower + tiles) {
@@ -535,17 +600,31 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
   const long long range = at;
 
   while (at < end) {
-    if (at - origin >= static_cast<long long>(s.tiles) * items) {
-      origin += static_cast<long long>(s.tiles) * items;
+    int span = s.tiles + kItemCost;
+    if (at - origin >= static_cast<long long>(span) * items) {
+      origin += static_cast<long long>(span) * items;
       s = slot_of<SIZE>(p, ++b);
+      span = s.tiles + kItemCost;
     }
-    const int item = static_cast<int>((at - origin) / s.tiles), tile = static_cast<int>((at - origin) % s.tiles);
+    const int item = static_cast<int>((at - origin) / span);
+    const long long item_at = origin + static_cast<long long>(item) * span;  // its cost, then its tiles
+    const int tile = max(0, static_cast<int>(at - item_at) - kItemCost);
+    const int tiles = max(0, static_cast<int>(min(end - item_at, static_cast<long long>(span))) - kItemCost) - tile;
+    at = item_at + span;
+    if (tiles <= 0) continue;
     const int head = item / p.blocks, first_row = item % p.blocks * kRows;
-    const int tiles = static_cast<int>(min(static_cast<long long>(s.tiles - tile), end - at));
+    if (s.row.count == 0) {  // no rows: zeros, and no keys to read
+      for (int i = threadIdx.x; i < kRows * SIZE / 4; i += kThreads) {
+        const int row = first_row + i / (SIZE / 4);
+        const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (row < p.rows) store4(p, out_row<SIZE>(p, b, head, row) + i % (SIZE / 4) * 4, zero);
+      }
+      continue;
+    }
     Sums<SIZE, MODE> sums;
     const void* query = static_cast<const char*>(p.a.q) + b * p.a.q_strides[0] * (p.a.dtype == CB_F32 ? 4 : 2);
     warp_item<SIZE, STORAGE, MODE, LO>(p, query, s, head, first_row, tile, tiles,
-                                       shared + warp * kStages * kSlotBytes, sums);
+                                       shared + warp * kStages * kSlotBytes, reinterpret_cast<uint4*>(shared + kRing), sums);
 
     // join the warps
     __syncthreads();  // every warp is done with the ring
@@ -562,16 +641,17 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           float* to = rows + (warp * kRows + r) * SIZE + element_of<SIZE>(2 * (lane & 3) + n);
+          const float2* o = sums.o[mt][half];
 #pragma unroll
           for (int j = 0; j < SIZE / 8; j += 4)
             *reinterpret_cast<float4*>(to + j) =
-                make_float4(sums.o[mt][half][j][n], sums.o[mt][half][j + 1][n], sums.o[mt][half][j + 2][n],
-                            sums.o[mt][half][j + 3][n]);
+                make_float4(n ? o[j].y : o[j].x, n ? o[j + 1].y : o[j + 1].x, n ? o[j + 2].y : o[j + 2].x,
+                            n ? o[j + 3].y : o[j + 3].x);
         }
       }
     __syncthreads();
     const bool whole = tile == 0 && tiles == s.tiles;
-    const bool begins = at == range;  // the block's first item takes its first partial result
+    const bool begins = item_at + kItemCost <= range;  // the item of the range's first tile: the first partial result
     float* partial = p.partial + (2LL * blockIdx.x + (begins ? 0 : 1)) * partial_floats<SIZE, MODE>();
     for (int i = threadIdx.x; i < kRows * SIZE / 4; i += kThreads) {
       const int r = i / (SIZE / 4), d = i % (SIZE / 4) * 4;
@@ -580,10 +660,10 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, most[w][r]);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = most[w][r] == -INFINITY ? 0.0f : exp2f(most[w][r] - top);
+        const float f = most[w][r] == -INFINITY ? 0.0f : root2_of(most[w][r] - top);
         const float4 x = *reinterpret_cast<const float4*>(rows + (w * kRows + r) * SIZE + d);
-        sum += f * total[w][r];
-        v[0] += f * x.x; v[1] += f * x.y; v[2] += f * x.z; v[3] += f * x.w;
+        sum += f * total[w][r] * f;
+        v[0] += f * x.x * f; v[1] += f * x.y * f; v[2] += f * x.z * f; v[3] += f * x.w * f;
       }
       const int row = first_row + r;
       if (whole) {
@@ -602,10 +682,9 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
       }
     }
     if (!whole && tile == 0 && threadIdx.x == 0) {
-      const long long last = (at + s.tiles - 1) / per;  // block of the item's last tile
+      const long long last = (item_at + span - 1) / per;  // block of the item's last tile
       p.cuts[blockIdx.x] = make_int4(static_cast<int>(b), item, static_cast<int>(last), begins ? 0 : 1);
     }
-    at += tiles;
     __syncthreads();  // the joined rows are read; the ring is free again
   }
 }
@@ -629,10 +708,10 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
     for (int k = 0; k < parts; ++k) top = fmaxf(top, (k ? rest + 2LL * k * kFloats : first)[r]);
     for (int k = 0; k < parts; ++k) {
       const float* part = k ? rest + 2LL * k * kFloats : first;
-      const float f = part[r] == -INFINITY ? 0.0f : exp2f(part[r] - top);
+      const float f = part[r] == -INFINITY ? 0.0f : root2_of(part[r] - top);
       const float4 x = *reinterpret_cast<const float4*>(part + 2 * kRows + r * SIZE + d);
-      sum += f * part[kRows + r];
-      v[0] += f * x.x; v[1] += f * x.y; v[2] += f * x.z; v[3] += f * x.w;
+      sum += f * part[kRows + r] * f;
+      v[0] += f * x.x * f; v[1] += f * x.y * f; v[2] += f * x.z * f; v[3] += f * x.w * f;
     }
     const bool real = row / p.group < count && sum != 0.0f;
 #pragma unroll
@@ -663,8 +742,9 @@ int resident_blocks() {
   cudaGetDevice(&now);
   if (now != device) {
     auto kernel = attention_kernel<SIZE, STORAGE, MODE, LO>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, kRing) != cudaSuccess)
+    constexpr int kShared = shared_bytes(SIZE, MODE, LO);
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, kShared) != cudaSuccess)
       per_sm = 0;
     device = per_sm > 0 ? now : -1;
   }
@@ -699,7 +779,7 @@ long long grid_of(const cb_paged_attention_args& a, int per_sm) {
   const long long rows = a.tokens * (a.heads / a.cache.kv_heads);
   const long long blocks = (rows + rows_of(MODE) - 1) / rows_of(MODE);
   const long long tiles = (a.cache.columns * a.cache.page + tile_keys(SIZE) - 1) / tile_keys(SIZE);
-  const long long most = a.batch * a.cache.kv_heads * blocks * tiles, fill = 1LL * per_sm * sm_count();
+  const long long most = a.batch * a.cache.kv_heads * blocks * (tiles + kItemCost), fill = 1LL * per_sm * sm_count();
   return most < fill ? most : fill;
 }
 
@@ -741,7 +821,7 @@ int cb_paged_attention(const cb_paged_attention_args* args, void* scratch, cb_st
     p.partial = reinterpret_cast<float*>(p.cuts + grid);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const dim3 blocks(static_cast<unsigned>(grid));
-    launch(attention_kernel<SIZE, STORAGE, MODE, LO>, blocks, dim3(kThreads), kRing, s, false, p);
+    launch(attention_kernel<SIZE, STORAGE, MODE, LO>, blocks, dim3(kThreads), shared_bytes(SIZE, MODE, LO), s, false, p);
     const int status = check_launch("cb_paged_attention");
     if (status != CB_OK) return status;
     launch(join_kernel<SIZE, MODE>, blocks, dim3(kThreads), 0, s, true, p);

@@ -69,8 +69,42 @@ def require(value: torch.Tensor, name: str, device: torch.device, dtypes, shape:
         if value.shape[at] != 1 and value.stride(at) != step:
             raise ValueError(f"{name} has to be contiguous in its last {dense} dimension(s)")
         step *= value.shape[at]
-    if value.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires grad: this operator has no backward pass")
+
+
+def no_grad_needed(*values: torch.Tensor) -> None:
+    """Refuse values that a gradient should flow through."""
+    if torch.is_grad_enabled() and any([v.requires_grad for v in values]):
+        raise ValueError("an argument requires grad: this operator has no backward pass")
+
+
+def current_stream(device: torch.device) -> int:
+    """Handle of the current stream of ``device``, which has to be the current device (launches go there).
+
+    (``torch.cuda.current_stream`` makes a stream object first, 3 us of a call that takes 8.)
+    """
+    if torch.cuda.current_device() != device.index:
+        raise ValueError(f"the tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def signature(value: Optional[torch.Tensor]):
+    """What the checks of an argument look at: equal signatures pass or fail alike."""
+    return None if value is None else (value.shape, value.stride(), value.dtype, value.device)
+
+
+class Prepared(dict):
+    """Checked argument structures by the signatures they were made for, without pointers.
+
+    A call with shapes, strides and types that were seen before skips the
+    checks and copies the structure; only the pointers are new.
+    """
+
+    LIMIT = 512
+
+    def __setitem__(self, key, value) -> None:
+        if len(self) >= self.LIMIT:
+            self.clear()
+        super().__setitem__(key, value)
 
 
 class PagedCache:
@@ -119,7 +153,8 @@ class PagedCache:
         p.k_scale, p.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
         p.layers, p.pages, p.kv_heads = self.layers, self.pages, self.kv_heads
         p.page_bytes = self.kv_heads * self.page_size * self.head_size
-        _lib.load()
+        self._lib = _lib.load()
+        self._attend_args, self._append_args = Prepared(), Prepared()
 
     @classmethod
     def allocate(cls, *, layers: int, pages: int, kv_heads: int, page_size: int, head_size: int, sequences: int,
@@ -154,25 +189,31 @@ class PagedCache:
         return c
 
     def _stream(self) -> int:
-        if torch.cuda.current_device() != self.device.index:
-            raise ValueError(f"the cache is on {self.device}, the current device is cuda:{torch.cuda.current_device()}")
-        return torch.cuda.current_stream().cuda_stream
+        return current_stream(self.device)
+
+    def _ints(self, value: Any) -> Optional[torch.Tensor]:
+        """A list of whole numbers as a tensor (host lists are copied to the device)."""
+        if value is None or isinstance(value, torch.Tensor):
+            return value
+        if isinstance(value, (list, tuple)):
+            return torch.tensor(value, dtype=torch.int32, device=self.device)
+        return tensor_of(value)
 
     def _list(self, value: Any, name: str, count: Optional[int]) -> torch.Tensor:
-        """An int32 list on the device (host lists are copied there)."""
-        if isinstance(value, (list, tuple)):
-            value = torch.tensor(value, dtype=torch.int32, device=self.device)
-        value = tensor_of(value)
+        """An int32 list on the device."""
+        value = self._ints(value)
+        if value is None:
+            raise TypeError(f"{name} are required")
         require(value, name, self.device, (torch.int32,), (count,), 1)
         return value
 
-    def _lists(self, counts: Any, sequences: Any, batch: int) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
-        counts = None if counts is None else self._list(counts, "counts", batch)
-        if sequences is None:
-            if batch > self.sequences:
-                raise ValueError(f"{batch} rows, and the cache has {self.sequences} sequences")
-            return counts, None
-        return counts, self._list(sequences, "sequences", batch)
+    def _check_lists(self, counts: Optional[torch.Tensor], sequences: Optional[torch.Tensor], batch: int) -> None:
+        if counts is not None:
+            require(counts, "counts", self.device, (torch.int32,), (batch,), 1)
+        if sequences is not None:
+            require(sequences, "sequences", self.device, (torch.int32,), (batch,), 1)
+        elif batch > self.sequences:
+            raise ValueError(f"{batch} rows, and the cache has {self.sequences} sequences")
 
     def _layer(self, layer: int) -> _lib.PagedCacheArgs:
         if not 0 <= layer < self.layers:
@@ -188,19 +229,32 @@ class PagedCache:
         has made room.  float32, bfloat16 or float16, any strides with a
         contiguous head.  See ``cb_paged_append`` for the scales.
         """
-        k, v = tensor_of(k), tensor_of(v)
+        k, v, counts, sequences = tensor_of(k), tensor_of(v), self._ints(counts), self._ints(sequences)
+        no_grad_needed(k, v)
+        key = (layer, signature(k), signature(v), signature(counts), signature(sequences))
+        known = self._append_args.get(key)
+        if known is None:
+            known = self._append_args[key] = self._prepare_append(layer, k, v, counts, sequences)
+        a = _lib.PagedAppendArgs.from_buffer_copy(known)
+        a.k, a.v = k.data_ptr(), v.data_ptr()
+        if counts is not None:
+            a.counts = counts.data_ptr()
+        if sequences is not None:
+            a.sequences = sequences.data_ptr()
+        _lib.check(self._lib.cb_paged_append(ctypes.byref(a), self._stream()), "cb_paged_append")
+
+    def _prepare_append(self, layer: int, k: torch.Tensor, v: torch.Tensor, counts: Optional[torch.Tensor],
+                        sequences: Optional[torch.Tensor]) -> _lib.PagedAppendArgs:
         require(k, "k", self.device, tuple(_VALUES), (None, None, self.kv_heads, self.head_size), 1)
         batch, tokens = k.shape[:2]
         require(v, "v", self.device, (k.dtype,), (batch, tokens, self.kv_heads, self.head_size), 1)
-        counts, sequences = self._lists(counts, sequences, batch)
+        self._check_lists(counts, sequences, batch)
         a = _lib.PagedAppendArgs()
         a.cache = self._layer(layer)
-        a.k, a.v, a.dtype, a.batch, a.tokens = k.data_ptr(), v.data_ptr(), _VALUES[k.dtype], batch, tokens
+        a.dtype, a.batch, a.tokens = _VALUES[k.dtype], batch, tokens
         a.k_strides[:], a.v_strides[:] = k.stride()[:3], v.stride()[:3]
-        a.counts = None if counts is None else counts.data_ptr()
-        a.sequences = None if sequences is None else sequences.data_ptr()
         a.error_flag = self._flag.data_ptr()
-        _lib.call("cb_paged_append", ctypes.byref(a), self._stream())
+        return a
 
     def attend(self, layer: int, q: Any, *, counts: Any = None, sequences: Any = None, scale: Optional[float] = None,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -211,29 +265,42 @@ class PagedCache:
         see nothing give zeros).  ``scale`` is 1/sqrt(head_size) without one.
         Returns (batch, tokens, heads, head_size) of q's dtype.
         """
-        q = tensor_of(q)
+        q, counts, sequences = tensor_of(q), self._ints(counts), self._ints(sequences)
+        no_grad_needed(q)
+        key = (layer, signature(q), signature(counts), signature(sequences), scale)
+        known = self._attend_args.get(key)
+        if known is None:
+            known = self._attend_args[key] = self._prepare_attend(layer, q, counts, sequences, scale)
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        else:
+            require(out, "out", self.device, (q.dtype,), tuple(q.shape), 4)
+        a = _lib.PagedAttentionArgs.from_buffer_copy(known[0])
+        a.q, a.out = q.data_ptr(), out.data_ptr()
+        if counts is not None:
+            a.counts = counts.data_ptr()
+        if sequences is not None:
+            a.sequences = sequences.data_ptr()
+        scratch = self._flag.new_empty(known[1])
+        _lib.check(self._lib.cb_paged_attention(ctypes.byref(a), scratch.data_ptr(), self._stream()),
+                   "cb_paged_attention")
+        return out
+
+    def _prepare_attend(self, layer: int, q: torch.Tensor, counts: Optional[torch.Tensor],
+                        sequences: Optional[torch.Tensor],
+                        scale: Optional[float]) -> Tuple[_lib.PagedAttentionArgs, int]:
         require(q, "q", self.device, tuple(_VALUES), (None, None, None, self.head_size), 1)
         batch, tokens, heads = q.shape[:3]
         if heads == 0 or heads % self.kv_heads:
             raise ValueError(f"{heads} query heads cannot share {self.kv_heads} kv heads")
-        counts, sequences = self._lists(counts, sequences, batch)
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        else:
-            require(out, "out", self.device, (q.dtype,), tuple(q.shape), 4)
+        self._check_lists(counts, sequences, batch)
         a = _lib.PagedAttentionArgs()
         a.cache = self._layer(layer)
-        a.q, a.out, a.dtype = q.data_ptr(), out.data_ptr(), _VALUES[q.dtype]
-        a.batch, a.tokens, a.heads = batch, tokens, heads
+        a.dtype, a.batch, a.tokens, a.heads = _VALUES[q.dtype], batch, tokens, heads
         a.q_strides[:] = q.stride()[:3]
-        a.counts = None if counts is None else counts.data_ptr()
-        a.sequences = None if sequences is None else sequences.data_ptr()
         a.scale = 1.0 / math.sqrt(self.head_size) if scale is None else scale
         a.error_flag = self._flag.data_ptr()
-        lib = _lib.load()
-        scratch = torch.empty(lib.cb_paged_attention_scratch(ctypes.byref(a)), dtype=torch.uint8, device=self.device)
-        _lib.call("cb_paged_attention", ctypes.byref(a), scratch.data_ptr(), self._stream())
-        return out
+        return a, (self._lib.cb_paged_attention_scratch(ctypes.byref(a)) + 3) // 4
 
     # -- pages -------------------------------------------------------------
     def extend(self, counts: Any, *, sequences: Any = None) -> None:
@@ -243,13 +310,14 @@ class PagedCache:
         other slots hold too is copied first.  All or nothing: with too few
         free pages nothing changes and ``check_errors`` raises MemoryError.
         """
-        counts = self._list(counts, "counts", None)
+        counts, sequences = self._list(counts, "counts", None), self._ints(sequences)
         n = counts.shape[0]
-        _, sequences = self._lists(None, sequences, n)
+        self._check_lists(None, sequences, n)
         scratch = self._scratch(n)
-        _lib.call("cb_pages_extend", ctypes.byref(self._book_args), ctypes.byref(self._pool_args), counts.data_ptr(),
-                  None if sequences is None else sequences.data_ptr(), n, scratch.data_ptr(), self._flag.data_ptr(),
-                  self._stream())
+        _lib.check(self._lib.cb_pages_extend(
+            ctypes.byref(self._book_args), ctypes.byref(self._pool_args), counts.data_ptr(),
+            None if sequences is None else sequences.data_ptr(), n, scratch.data_ptr(), self._flag.data_ptr(),
+            self._stream()), "cb_pages_extend")
 
     def fork(self, parents: Any, children: Any) -> None:
         """Slot ``children[i]``, which has to be empty, continues slot ``parents[i]`` and shares its pages."""
@@ -258,8 +326,8 @@ class PagedCache:
         children = self._list(children, "children", n)
         if n > self.sequences:
             raise ValueError(f"{n} forks, and the cache has {self.sequences} sequences")
-        _lib.call("cb_pages_fork", ctypes.byref(self._book_args), parents.data_ptr(), children.data_ptr(), n,
-                  self._flag.data_ptr(), self._stream())
+        _lib.check(self._lib.cb_pages_fork(ctypes.byref(self._book_args), parents.data_ptr(), children.data_ptr(), n,
+                                           self._flag.data_ptr(), self._stream()), "cb_pages_fork")
 
     def truncate(self, counts: Any, *, sequences: Any = None) -> None:
         """Drop the last ``counts[i]`` tokens of slot ``sequences[i]`` and let go of the pages that held only those."""
@@ -272,28 +340,32 @@ class PagedCache:
         self._truncate(None, sequences, sequences.shape[0])
 
     def _truncate(self, counts: Optional[torch.Tensor], sequences: Any, n: int) -> None:
-        _, sequences = self._lists(None, sequences, n)
+        sequences = self._ints(sequences)
+        self._check_lists(None, sequences, n)
         if n > self.sequences:
             raise ValueError(f"{n} slots, and the cache has {self.sequences} sequences")
-        _lib.call("cb_pages_truncate", ctypes.byref(self._book_args), None if counts is None else counts.data_ptr(),
-                  None if sequences is None else sequences.data_ptr(), n, self._flag.data_ptr(), self._stream())
+        _lib.check(self._lib.cb_pages_truncate(
+            ctypes.byref(self._book_args), None if counts is None else counts.data_ptr(),
+            None if sequences is None else sequences.data_ptr(), n, self._flag.data_ptr(), self._stream()),
+            "cb_pages_truncate")
 
     def compact(self) -> None:
         """Move the held pages to the front of the pools (page ids change; the table follows)."""
         scratch = self._scratch(0)
-        _lib.call("cb_pages_compact", ctypes.byref(self._book_args), ctypes.byref(self._pool_args),
-                  scratch.data_ptr(), self._flag.data_ptr(), self._stream())
+        _lib.check(self._lib.cb_pages_compact(ctypes.byref(self._book_args), ctypes.byref(self._pool_args),
+                                              scratch.data_ptr(), self._flag.data_ptr(), self._stream()),
+                   "cb_pages_compact")
 
     def copy_pages(self, source: Any, target: Any) -> None:
         """Copy page ``source[i]`` to page ``target[i]`` in every layer (no page is both)."""
         source = self._list(source, "source", None)
         target = self._list(target, "target", source.shape[0])
-        _lib.call("cb_pages_copy", ctypes.byref(self._pool_args), source.data_ptr(), target.data_ptr(),
-                  source.shape[0], self._flag.data_ptr(), self._stream())
+        _lib.check(self._lib.cb_pages_copy(ctypes.byref(self._pool_args), source.data_ptr(), target.data_ptr(),
+                                           source.shape[0], self._flag.data_ptr(), self._stream()), "cb_pages_copy")
 
     def _scratch(self, n: int) -> torch.Tensor:
-        size = _lib.load().cb_pages_scratch(ctypes.byref(self._book_args), n)
-        return torch.empty(size, dtype=torch.uint8, device=self.device)
+        size = self._lib.cb_pages_scratch(ctypes.byref(self._book_args), n)
+        return self._flag.new_empty((size + 3) // 4)
 
     # -- errors ------------------------------------------------------------
     def check_errors(self) -> None:

@@ -16,7 +16,9 @@ from typing import Any, Optional, Tuple
 import torch
 
 from . import _lib
-from .paged import _VALUES, require, tensor_of
+from .paged import _VALUES, Prepared, current_stream, no_grad_needed, require, signature, tensor_of
+
+_VERIFY_ARGS = Prepared()
 
 
 def verify(target: Any, draft: Any, tokens: Any, uniforms: Any, *, counts: Any = None,
@@ -37,7 +39,31 @@ def verify(target: Any, draft: Any, tokens: Any, uniforms: Any, *, counts: Any =
     ``error_flag`` (an int32 of the caller's, read with ``check``).  Sums are
     exact, so equal inputs give equal tokens on any launch.
     """
-    target, draft, tokens, uniforms = (tensor_of(v) for v in (target, draft, tokens, uniforms))
+    target, draft, tokens, uniforms = tensor_of(target), tensor_of(draft), tensor_of(tokens), tensor_of(uniforms)
+    counts = None if counts is None else tensor_of(counts)
+    no_grad_needed(target, draft)
+    key = (signature(target), signature(draft), signature(tokens), signature(uniforms), signature(counts),
+           signature(error_flag))
+    known = _VERIFY_ARGS.get(key)
+    if known is None:
+        known = _VERIFY_ARGS[key] = _prepare(target, draft, tokens, uniforms, counts, error_flag)
+    stream = current_stream(target.device)
+    emitted = uniforms.new_empty(uniforms.shape, dtype=torch.int64)
+    accepted = uniforms.new_empty(uniforms.shape[0], dtype=torch.int32)
+    a = _lib.VerifyArgs.from_buffer_copy(known)
+    a.target, a.draft, a.drafted, a.uniforms = (target.data_ptr(), draft.data_ptr(), tokens.data_ptr(),
+                                                uniforms.data_ptr())
+    a.accepted, a.out = accepted.data_ptr(), emitted.data_ptr()
+    if counts is not None:
+        a.counts = counts.data_ptr()
+    if error_flag is not None:
+        a.error_flag = error_flag.data_ptr()
+    _lib.check(_lib.load().cb_verify_draft(ctypes.byref(a), stream), "cb_verify_draft")
+    return accepted, emitted
+
+
+def _prepare(target: torch.Tensor, draft: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor,
+             counts: Optional[torch.Tensor], error_flag: Optional[torch.Tensor]) -> _lib.VerifyArgs:
     if target.device.type != "cuda":
         raise ValueError(f"target is on {target.device}, expected a CUDA device")
     if target.ndim != 3 or target.shape[1] < 1 or target.shape[2] < 1:
@@ -48,24 +74,13 @@ def verify(target: Any, draft: Any, tokens: Any, uniforms: Any, *, counts: Any =
     require(tokens, "tokens", target.device, (torch.int64,), (batch, n), 2)
     require(uniforms, "uniforms", target.device, (torch.float64,), (batch, n + 1), 2)
     if counts is not None:
-        counts = tensor_of(counts)
         require(counts, "counts", target.device, (torch.int32,), (batch,), 1)
     if error_flag is not None:
         require(error_flag, "error_flag", target.device, (torch.int32,), (1,), 1)
-    if torch.cuda.current_device() != target.device.index:
-        raise ValueError(f"target is on {target.device}, the current device is cuda:{torch.cuda.current_device()}")
-    accepted = torch.empty(batch, dtype=torch.int32, device=target.device)
-    emitted = torch.empty(batch, n + 1, dtype=torch.int64, device=target.device)
     a = _lib.VerifyArgs()
-    a.target, a.draft, a.dtype = target.data_ptr(), draft.data_ptr(), _VALUES[target.dtype]
-    a.batch, a.tokens, a.vocab = batch, n, vocab
+    a.dtype, a.batch, a.tokens, a.vocab = _VALUES[target.dtype], batch, n, vocab
     a.target_strides[:], a.draft_strides[:] = target.stride()[:2], draft.stride()[:2]
-    a.drafted, a.uniforms = tokens.data_ptr(), uniforms.data_ptr()
-    a.counts = None if counts is None else counts.data_ptr()
-    a.accepted, a.out = accepted.data_ptr(), emitted.data_ptr()
-    a.error_flag = None if error_flag is None else error_flag.data_ptr()
-    _lib.call("cb_verify_draft", ctypes.byref(a), torch.cuda.current_stream().cuda_stream)
-    return accepted, emitted
+    return a
 
 
 def check(error_flag: torch.Tensor) -> None:

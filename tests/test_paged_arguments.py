@@ -122,7 +122,9 @@ def test_python_checks():
     with pytest.raises(ValueError):
         paged.require(x.transpose(1, 2), "x", cpu, (torch.float32,), (2, 4, 3), 1)
     with pytest.raises(ValueError):
-        paged.require(x.clone().requires_grad_(), "x", cpu, (torch.float32,), (2, 3, 4), 1)
+        paged.no_grad_needed(x, x.clone().requires_grad_())
+    with torch.no_grad():
+        paged.no_grad_needed(x.clone().requires_grad_())
     with pytest.raises(TypeError):
         paged.tensor_of([1, 2])
     pools = [torch.zeros(1, 2, 1, 16, 32, dtype=torch.int8) for _ in range(2)]
