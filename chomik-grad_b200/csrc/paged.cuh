@@ -11,6 +11,11 @@ __device__ __forceinline__ void raise_flag(int* flag, int code) {
   if (flag != nullptr) atomicMax(flag, code);
 }
 
+// A cluster's blocks write to one another's shared memory only once all have
+// begun: each arrives first thing, and waits before its first such write.
+__device__ __forceinline__ void cluster_begun() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_all_begun() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
 inline int paged_cache_check(const cb_paged_cache& c, const char* who) {
   CB_REQUIRE(c.storage == CB_I8 || c.storage == CB_E4M3, "%s: storage must be int8 or e4m3 (got code %d)", who,
              c.storage);

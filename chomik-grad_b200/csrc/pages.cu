@@ -5,13 +5,27 @@
 // handled one after the other in the order of the call would give: ranks are
 // prefix sums over the block, and where several slots drop or copy the same
 // page the choice goes by position, never by which atomic came first.
+//
+// What bounds them: the book operations read and write some KB to MB in chains
+// of dependent steps, so their time is latency; truncate and compact, whose
+// lists grow with the table and the pool, run as one cluster of up to eight
+// blocks that exchange their counts through distributed shared memory (64
+// slots of 128 pages: half released in 7 us; by one block 18).  The copies are
+// bound by memory: 8 loads of 16 bytes in flight for each thread of a grid that
+// fills the GPU, launched along with the book's kernel (programmatic dependent
+// launch), which leaves it the list.
+#include <cooperative_groups.h>
+
 #include "paged.cuh"
 
 namespace cb {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
+constexpr int kMostBlocks = 8;  // of a cluster: the portable limit
 
 // Exclusive prefix sum of v in thread order; *total receives the sum.
 __device__ __forceinline__ long long block_scan(long long v, long long* shared, long long* total) {
@@ -39,6 +53,23 @@ __device__ __forceinline__ long long block_scan(long long v, long long* shared, 
   return incl - v + (warp > 0 ? shared[warp - 1] : 0);
 }
 
+// The sum of `v` (one value of each block) over the blocks before this one, and
+// over the cluster.  `slots` is a shared array that no earlier call of the
+// kernel used; every thread calls it, and it orders the cluster's memory.
+__device__ __forceinline__ long long cluster_scan(long long v, long long* slots, long long* total) {
+  cg::cluster_group group = cg::this_cluster();
+  const int blocks = static_cast<int>(group.num_blocks()), rank = static_cast<int>(group.block_rank());
+  if (static_cast<int>(threadIdx.x) < blocks) *group.map_shared_rank(slots + rank, threadIdx.x) = v;
+  group.sync();
+  long long before = 0, all = 0;
+  for (int r = 0; r < blocks; ++r) {
+    if (r == rank) before = all;
+    all += slots[r];
+  }
+  *total = all;
+  return before;
+}
+
 // Scratch of cb_pages_extend and cb_pages_compact: the pages to copy (their
 // number, sources and targets), then lists of the kernel.
 struct Copies {
@@ -55,6 +86,7 @@ __host__ __device__ __forceinline__ Copies copies_of(void* scratch, long long n)
 __global__ void __launch_bounds__(kThreads) extend_kernel(cb_page_book k, const int* counts, const int* sequences,
                                                           long long n, void* scratch, int* flag) {
   __shared__ long long shared[kWarps];
+  pdl_launch_dependents();
   const Copies copies = copies_of(scratch, n);
   int* tails = copies.more;      // open last page of each slot, or -1
   int* plan = copies.more + n;   // pages it takes, negative - 1 where the first of them is a copy
@@ -177,119 +209,176 @@ __global__ void __launch_bounds__(256) fork_kernel(cb_page_book k, const int* pa
 // Entry e = i * columns + m of the call is dropped where need <= m < have of
 // slot i.  A page that nobody holds any more is claimed by the last of its
 // dropped entries: refs[page] goes from 0 to -(e + 1), the least of them.
+// Each block of the cluster takes a contiguous range of the entries, in
+// descending order; a thread keeps the pages of its first kKept entries.
+constexpr int kKept = 4;
+
 __global__ void __launch_bounds__(kThreads) truncate_kernel(cb_page_book k, const int* counts, const int* sequences,
-                                                            long long n, int* flag) {
-  __shared__ long long shared[kWarps];
+                                                            int n, int* flag) {
+  __shared__ long long shared[kWarps], first[kMostBlocks], second[kMostBlocks], third[kMostBlocks];
+  cluster_begun();
+  cg::cluster_group group = cg::this_cluster();
+  const int blocks = static_cast<int>(group.num_blocks()), rank = static_cast<int>(group.block_rank());
+  const int columns = static_cast<int>(k.columns), entries = n * columns;
   bool bad = false;
-  for (long long i = threadIdx.x; i < n; i += kThreads) {
-    const long long slot = sequences != nullptr ? sequences[i] : i;
+  for (int i = threadIdx.x; i < n; i += kThreads) {  // every block for itself
+    const int slot = sequences != nullptr ? sequences[i] : i;
     if (slot < 0 || slot >= k.slots) {
       bad = true;
       continue;
     }
     const int length = k.lengths[slot];
-    bad = bad || length < 0 || length > k.columns * k.page || (counts != nullptr && (counts[i] < 0 || counts[i] > length));
-    for (long long j = 0; j < i && sequences != nullptr; ++j) bad = bad || sequences[j] == slot;
+    bad = bad || length < 0 || length > k.columns * k.page ||
+          (counts != nullptr && (counts[i] < 0 || counts[i] > length));
+    for (int j = 0; j < i && sequences != nullptr; ++j) bad = bad || sequences[j] == slot;
   }
-  if (__syncthreads_or(bad)) {
+  const int per = ((entries + blocks - 1) / blocks + kThreads - 1) / kThreads * kThreads;
+  const int begin = rank * per, end = min(begin + per, entries);
+  auto entry = [&](int f) { return entries - 1 - f; };
+  auto place = [&](int e) -> int* {  // of a dropped entry in the table
+    const int i = e / columns, m = e % columns;
+    const int slot = sequences != nullptr ? sequences[i] : i;
+    const int length = k.lengths[slot], rest = counts != nullptr ? length - counts[i] : 0;
+    const long long token = static_cast<long long>(m) * k.page;
+    return token < length && token >= rest ? k.table + slot * k.columns + m : nullptr;
+  };
+  auto page_of = [&](int f) {
+    const int* at = f < end ? place(entry(f)) : nullptr;
+    if (at == nullptr) return -1;
+    return *at < 0 || *at >= k.pages ? -2 : *at;
+  };
+  if (__syncthreads_or(bad)) {  // the same in every block
     if (threadIdx.x == 0) raise_flag(flag, CB_FLAG_BOOK);
     return;
   }
-  const long long entries = n * k.columns;
-  auto dropped = [&](long long e) -> int* {
-    const long long i = e / k.columns, m = e % k.columns;
-    const long long slot = sequences != nullptr ? sequences[i] : i;
-    const long long length = k.lengths[slot], rest = counts != nullptr ? length - counts[i] : 0;
-    const bool drop = m * k.page < length && m * k.page >= rest;
-    return drop ? k.table + slot * k.columns + m : nullptr;
+  const int height = *k.height;
+  int pages[kKept];
+  for (int it = 0, f = begin + threadIdx.x; f < end; ++it, f += kThreads) {
+    const int page = page_of(f);
+    if (it < kKept) {
+#pragma unroll
+      for (int n = 0; n < kKept; ++n) pages[n] = n == it ? page : pages[n];
+    }
+    if (page >= 0) atomicSub(&k.refs[page], 1);
+    if (page == -2) raise_flag(flag, CB_FLAG_BOOK);
+  }
+  auto known = [&](int it, int f) {
+    int page = -1;
+#pragma unroll
+    for (int n = 0; n < kKept; ++n) page = n == it ? pages[n] : page;
+    return it < kKept ? page : page_of(f);
   };
-  for (long long e = threadIdx.x; e < entries; e += kThreads) {
-    const int* at = dropped(e);
-    if (at == nullptr) continue;
-    if (*at >= 0 && *at < k.pages) atomicSub(&k.refs[*at], 1);
-    else raise_flag(flag, CB_FLAG_BOOK);
+  long long total;
+  cluster_all_begun();
+  cluster_scan(0, first, &total);  // all are counted down
+  for (int it = 0, f = begin + threadIdx.x; f < end; ++it, f += kThreads) {
+    const int page = known(it, f);
+    if (page >= 0 && __ldcg(&k.refs[page]) <= 0) atomicMin(&k.refs[page], -(entry(f) + 1));
   }
-  __syncthreads();
-  for (long long e = threadIdx.x; e < entries; e += kThreads) {
-    const int* at = dropped(e);
-    if (at == nullptr || *at < 0 || *at >= k.pages) continue;
-    if (__ldcg(&k.refs[*at]) <= 0) atomicMin(&k.refs[*at], static_cast<int>(-(e + 1)));
+  cluster_scan(0, second, &total);  // all claims are in
+  int mine = 0;
+  for (int it = 0, f = begin + threadIdx.x; f < end; ++it, f += kThreads) {
+    const int page = known(it, f);
+    mine += page >= 0 && __ldcg(&k.refs[page]) == -(entry(f) + 1);
   }
-  __syncthreads();
-  long long pushed = *k.height;
-  for (long long done = 0; done < entries; done += kThreads) {
-    const long long e = entries - 1 - done - threadIdx.x;
-    int* at = e >= 0 ? dropped(e) : nullptr;
-    const int page = at != nullptr ? *at : -1;
-    const bool mine = page >= 0 && page < k.pages && __ldcg(&k.refs[page]) == static_cast<int>(-(e + 1));
-    long long total;
-    const long long rank = block_scan(mine ? 1 : 0, shared, &total);
-    if (mine) {
-      if (pushed + rank < k.pages) k.free_pages[pushed + rank] = page;
+  long long count;
+  block_scan(mine, shared, &count);
+  long long pushed = height + cluster_scan(count, third, &total);
+  for (int at = begin; at < end; at += kThreads) {
+    const int f = at + threadIdx.x, page = f < end ? known((at - begin) / kThreads, f) : -1;
+    const bool claimed = page >= 0 && __ldcg(&k.refs[page]) == -(entry(f) + 1);
+    long long sum;
+    const long long to = pushed + block_scan(claimed, shared, &sum);
+    if (claimed) {
+      if (to < k.pages) k.free_pages[to] = page;
       else raise_flag(flag, CB_FLAG_BOOK);
       k.refs[page] = 0;
     }
-    if (at != nullptr) *at = -1;
-    pushed += total;
+    if (f < end) {
+      int* gone = place(entry(f));
+      if (gone != nullptr) *gone = -1;
+    }
+    pushed += sum;
   }
-  __syncthreads();
-  for (long long i = threadIdx.x; i < n; i += kThreads) {
-    const long long slot = sequences != nullptr ? sequences[i] : i;
-    k.lengths[slot] = counts != nullptr ? k.lengths[slot] - counts[i] : 0;
+  group.sync();  // every block has used the lengths
+  if (rank == 0) {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const int slot = sequences != nullptr ? sequences[i] : i;
+      k.lengths[slot] = counts != nullptr ? k.lengths[slot] - counts[i] : 0;
+    }
+    if (threadIdx.x == 0) *k.height = static_cast<int>(height + total < k.pages ? height + total : k.pages);
   }
-  if (threadIdx.x == 0) *k.height = static_cast<int>(pushed < k.pages ? pushed : k.pages);
 }
 
 __global__ void __launch_bounds__(kThreads) compact_kernel(cb_page_book k, void* scratch, int* flag) {
-  __shared__ long long shared[kWarps];
+  __shared__ long long shared[kWarps], first[kMostBlocks], second[kMostBlocks], third[kMostBlocks];
+  cluster_begun();
+  pdl_launch_dependents();
+  cg::cluster_group group = cg::this_cluster();
+  const int blocks = static_cast<int>(group.num_blocks()), rank = static_cast<int>(group.block_rank());
+  const int pages = static_cast<int>(k.pages), thread = rank * kThreads + threadIdx.x, threads = blocks * kThreads;
   const Copies copies = copies_of(scratch, k.pages);
   int* to = copies.more;
-  long long held = 0;
-  for (long long at = 0; at < k.pages; at += kThreads) {
-    const long long p = at + threadIdx.x;
-    if (p < k.pages) to[p] = static_cast<int>(p);
-    held += __syncthreads_count(p < k.pages && k.refs[p] > 0);
+  const int per = ((pages + blocks - 1) / blocks + kThreads - 1) / kThreads * kThreads;
+  const int begin = rank * per, end = min(begin + per, pages);
+  int live = 0;
+  for (int p = begin + threadIdx.x; p < end; p += kThreads) {
+    to[p] = p;
+    live += k.refs[p] > 0;
   }
-  long long holes = 0, moves = 0;
-  for (long long at = 0; at < k.pages; at += kThreads) {
-    const long long p = at + threadIdx.x;
-    const bool live = p < k.pages && k.refs[p] > 0;
-    const bool hole = p < held && !live, move = p >= held && live;
-    long long total;
-    const long long rank = block_scan((static_cast<long long>(move) << 32) + (hole ? 1 : 0), shared, &total);
-    if (hole) copies.target[holes + (rank & 0xffffffffll)] = static_cast<int>(p);
-    if (move) copies.source[moves + (rank >> 32)] = static_cast<int>(p);
-    holes += total & 0xffffffffll;
-    moves += total >> 32;
+  long long sum, held;
+  block_scan(live, shared, &sum);
+  cluster_all_begun();
+  cluster_scan(sum, first, &held);
+  long long pair = 0;  // pages that move, holes
+  for (int p = begin + threadIdx.x; p < end; p += kThreads) {
+    const bool used = k.refs[p] > 0;
+    pair += (static_cast<long long>(p >= held && used) << 32) + (p < held && !used);
   }
-  __syncthreads();
-  for (long long r = threadIdx.x; r < moves; r += kThreads) {
-    const int source = copies.source[r], target = copies.target[r];
+  block_scan(pair, shared, &sum);
+  long long all;
+  long long before = cluster_scan(sum, second, &all);
+  const int moves = static_cast<int>(all >> 32);
+  for (int at = begin; at < end; at += kThreads) {
+    const int p = at + threadIdx.x;
+    const bool used = p < end && k.refs[p] > 0, move = used && p >= held, hole = p < end && !used && p < held;
+    const long long rank_of = before + block_scan((static_cast<long long>(move) << 32) + hole, shared, &sum);
+    if (hole) copies.target[rank_of & 0xffffffffll] = p;
+    if (move) copies.source[rank_of >> 32] = p;
+    before += sum;
+  }
+  cluster_scan(0, third, &sum);  // the lists are written
+  for (int r = thread; r < moves; r += threads) {
+    const int source = __ldcg(copies.source + r), target = __ldcg(copies.target + r);
     to[source] = target;
     k.refs[target] = k.refs[source];
     k.refs[source] = 0;
   }
-  __syncthreads();
-  for (long long e = threadIdx.x; e < k.slots * k.columns; e += kThreads) {
+  group.sync();
+  for (long long e = thread; e < k.slots * k.columns; e += threads) {
     const int page = k.table[e];
-    if (page >= k.pages) raise_flag(flag, CB_FLAG_BOOK);
-    else if (page >= held) k.table[e] = to[page];
+    if (page >= pages) raise_flag(flag, CB_FLAG_BOOK);
+    else if (page >= held) k.table[e] = __ldcg(to + page);
   }
-  for (long long i = threadIdx.x; i < k.pages - held; i += kThreads)
-    k.free_pages[i] = static_cast<int>(k.pages - 1 - i);
-  if (threadIdx.x == 0) {
-    *k.height = static_cast<int>(k.pages - held);
-    *copies.count = static_cast<int>(moves);
+  for (int i = thread; i < pages - held; i += threads) k.free_pages[i] = pages - 1 - i;
+  if (thread == 0) {
+    *k.height = static_cast<int>(pages - held);
+    *copies.count = moves;
   }
 }
 
 // Copies of whole pages: unit u = (copy, layer, K or V).
-__global__ void __launch_bounds__(256) copy_kernel(cb_page_pools p, const int* source, const int* target,
-                                                   const int* count, long long n, int* flag) {
-  const long long copies = count != nullptr ? *count : n;
-  const long long units = copies * p.layers * 2;
+constexpr int kCopyThreads = 256;
+constexpr int kBatch = 8;  // 16-byte loads a thread has in flight
+
+__global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constant__ cb_page_pools p, const int* source,
+                                                            const int* target, const int* count, int n, int* flag) {
+  pdl_wait();
+  const int copies = count != nullptr ? *count : n, layers = static_cast<int>(p.layers);
+  const long long units = 2LL * copies * layers;
+  const int vectors = static_cast<int>(p.page_bytes / 16);
   for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-    const long long r = u / (p.layers * 2), layer = u / 2 % p.layers;
+    const int r = static_cast<int>(u / (2 * layers)), layer = static_cast<int>(u % (2 * layers)) >> 1;
     const int from = source[r], to = target[r];
     if (from < 0 || from >= p.pages || to < 0 || to >= p.pages) {
       if (threadIdx.x == 0) raise_flag(flag, CB_FLAG_BOOK);
@@ -299,8 +388,16 @@ __global__ void __launch_bounds__(256) copy_kernel(cb_page_pools p, const int* s
     float* scale = (u % 2 ? p.v_scale : p.k_scale) + layer * p.pages * p.kv_heads;
     const uint4* src = reinterpret_cast<const uint4*>(pool + from * p.page_bytes);
     uint4* dst = reinterpret_cast<uint4*>(pool + to * p.page_bytes);
-    for (long long i = threadIdx.x; i < p.page_bytes / 16; i += blockDim.x) dst[i] = src[i];
-    for (int i = threadIdx.x; i < p.kv_heads; i += blockDim.x)
+    for (int at = threadIdx.x; at < vectors; at += kBatch * kCopyThreads) {
+      uint4 v[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (at + i * kCopyThreads < vectors) v[i] = __ldcs(src + at + i * kCopyThreads);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (at + i * kCopyThreads < vectors) __stcs(dst + at + i * kCopyThreads, v[i]);
+    }
+    for (int i = threadIdx.x; i < p.kv_heads; i += kCopyThreads)
       scale[static_cast<long long>(to) * p.kv_heads + i] = scale[static_cast<long long>(from) * p.kv_heads + i];
   }
 }
@@ -316,7 +413,8 @@ int book_check(const cb_page_book* k, long long n, const char* who) {
 
 int pools_check(const cb_page_pools* p, const char* who) {
   CB_REQUIRE(p != nullptr && p->k_pages && p->v_pages && p->k_scale && p->v_scale, "%s: a null pointer", who);
-  CB_REQUIRE(p->layers >= 1 && p->pages >= 1 && p->kv_heads >= 1 && p->page_bytes > 0 && p->page_bytes % 16 == 0,
+  CB_REQUIRE(p->layers >= 1 && p->layers < (1 << 20) && p->pages >= 1 && p->pages < (1LL << 31) &&
+                 p->page_bytes < (1LL << 31) && p->kv_heads >= 1 && p->page_bytes > 0 && p->page_bytes % 16 == 0,
              "%s: %lld layers of %lld pages of %lld bytes", who, p->layers, p->pages, p->page_bytes);
   CB_REQUIRE(reinterpret_cast<uintptr_t>(p->k_pages) % 16 == 0 && reinterpret_cast<uintptr_t>(p->v_pages) % 16 == 0,
              "%s: the pools must be 16-byte aligned", who);
@@ -324,11 +422,31 @@ int pools_check(const cb_page_pools* p, const char* who) {
 }
 
 int launch_copies(const cb_page_pools& p, const int* source, const int* target, const int* count, long long most,
-                  int* flag, cudaStream_t stream) {
-  const long long units = most * p.layers * 2, cap = 8LL * sm_count();
-  copy_kernel<<<static_cast<unsigned>(units < cap ? units : cap), 256, 0, stream>>>(p, source, target, count, most,
-                                                                                  flag);
+                  bool behind, int* flag, cudaStream_t stream) {
+  const long long units = most * p.layers * 2, cap = 1LL * (2048 / kCopyThreads) * sm_count();
+  launch(copy_kernel, dim3(static_cast<unsigned>(units < cap ? units : cap)), dim3(kCopyThreads), 0, stream, behind, p,
+         source, target, count, static_cast<int>(most), flag);
   return check_launch("cb_pages: copies");
+}
+
+// One cluster for `work` list entries: a block for each kThreads of them, up
+// to eight.
+template <typename... Expected, typename... Args>
+int launch_cluster(void (*kernel)(Expected...), const char* what, long long work, cudaStream_t stream, Args... args) {
+  unsigned blocks = 1;
+  while (blocks < kMostBlocks && work > 1LL * kThreads * blocks) blocks *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<Expected>(args)...);
+  return check_launch(what);
 }
 
 }  // namespace
@@ -358,7 +476,7 @@ int cb_pages_extend(const cb_page_book* book, const cb_page_pools* pools, const 
   status = check_launch("cb_pages_extend");
   if (status != CB_OK) return status;
   const Copies c = copies_of(scratch, n);
-  return launch_copies(*pools, c.source, c.target, c.count, n, error_flag, s);
+  return launch_copies(*pools, c.source, c.target, c.count, n, true, error_flag, s);
 }
 
 int cb_pages_fork(const cb_page_book* book, const int* parents, const int* children, long long n, int* error_flag,
@@ -377,8 +495,8 @@ int cb_pages_truncate(const cb_page_book* book, const int* counts, const int* se
   const int status = book_check(book, n, "cb_pages_truncate");
   if (status != CB_OK) return status;
   if (n == 0) return CB_OK;
-  truncate_kernel<<<1, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(*book, counts, sequences, n, error_flag);
-  return check_launch("cb_pages_truncate");
+  return launch_cluster(truncate_kernel, "cb_pages_truncate", n * book->columns, static_cast<cudaStream_t>(stream),
+                        *book, counts, sequences, n, error_flag);
 }
 
 int cb_pages_compact(const cb_page_book* book, const cb_page_pools* pools, void* scratch, int* error_flag,
@@ -390,21 +508,22 @@ int cb_pages_compact(const cb_page_book* book, const cb_page_pools* pools, void*
   CB_REQUIRE(pools->pages == book->pages, "cb_pages_compact: %lld pages in the pools, %lld in the book", pools->pages,
              book->pages);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  compact_kernel<<<1, kThreads, 0, s>>>(*book, scratch, error_flag);
-  status = check_launch("cb_pages_compact");
+  const long long entries = book->slots * book->columns;
+  status = launch_cluster(compact_kernel, "cb_pages_compact", book->pages > entries ? book->pages : entries, s, *book,
+                          scratch, error_flag);
   if (status != CB_OK) return status;
   const Copies c = copies_of(scratch, book->pages);
-  return launch_copies(*pools, c.source, c.target, c.count, book->pages, error_flag, s);
+  return launch_copies(*pools, c.source, c.target, c.count, book->pages, true, error_flag, s);
 }
 
 int cb_pages_copy(const cb_page_pools* pools, const int* source, const int* target, long long n, int* error_flag,
                   cb_stream_t stream) {
   const int status = pools_check(pools, "cb_pages_copy");
   if (status != CB_OK) return status;
-  CB_REQUIRE(n >= 0, "cb_pages_copy: %lld pages", n);
+  CB_REQUIRE(n >= 0 && n < (1LL << 31), "cb_pages_copy: %lld pages", n);
   if (n == 0) return CB_OK;
   CB_REQUIRE(source != nullptr && target != nullptr, "cb_pages_copy: a null pointer");
-  return launch_copies(*pools, source, target, nullptr, n, error_flag, static_cast<cudaStream_t>(stream));
+  return launch_copies(*pools, source, target, nullptr, n, false, error_flag, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -154,7 +154,8 @@ class PagedCache:
         p.layers, p.pages, p.kv_heads = self.layers, self.pages, self.kv_heads
         p.page_bytes = self.kv_heads * self.page_size * self.head_size
         self._lib = _lib.load()
-        self._attend_args, self._append_args = Prepared(), Prepared()
+        self._attend_args, self._append_args, self._lists = Prepared(), Prepared(), Prepared()
+        self._scratch_words = Prepared()
 
     @classmethod
     def allocate(cls, *, layers: int, pages: int, kv_heads: int, page_size: int, head_size: int, sequences: int,
@@ -204,14 +205,17 @@ class PagedCache:
         value = self._ints(value)
         if value is None:
             raise TypeError(f"{name} are required")
-        require(value, name, self.device, (torch.int32,), (count,), 1)
+        key = (name, count, signature(value))
+        if key not in self._lists:
+            require(value, name, self.device, (torch.int32,), (count,), 1)
+            self._lists[key] = True
         return value
 
     def _check_lists(self, counts: Optional[torch.Tensor], sequences: Optional[torch.Tensor], batch: int) -> None:
         if counts is not None:
-            require(counts, "counts", self.device, (torch.int32,), (batch,), 1)
+            self._list(counts, "counts", batch)
         if sequences is not None:
-            require(sequences, "sequences", self.device, (torch.int32,), (batch,), 1)
+            self._list(sequences, "sequences", batch)
         elif batch > self.sequences:
             raise ValueError(f"{batch} rows, and the cache has {self.sequences} sequences")
 
@@ -364,8 +368,10 @@ class PagedCache:
                                            source.shape[0], self._flag.data_ptr(), self._stream()), "cb_pages_copy")
 
     def _scratch(self, n: int) -> torch.Tensor:
-        size = self._lib.cb_pages_scratch(ctypes.byref(self._book_args), n)
-        return self._flag.new_empty((size + 3) // 4)
+        size = self._scratch_words.get(n)
+        if size is None:
+            size = self._scratch_words[n] = (self._lib.cb_pages_scratch(ctypes.byref(self._book_args), n) + 3) // 4
+        return self._flag.new_empty(size)
 
     # -- errors ------------------------------------------------------------
     def check_errors(self) -> None:
