@@ -30,38 +30,42 @@
 // are one sequence of tiles, cut into equal ranges for a grid that fills the
 // GPU once, whatever the lengths: each block finds its range from the lengths
 // on the device.  An item that a cut divides leaves partial results (maximum,
-// sum, weighted values), joined in a fixed order by a second kernel that is
-// launched along with the first (programmatic dependent launch).
+// sum, weighted values), which the block that finishes last joins in the order
+// of the keys: equal inputs give equal bits, and there is one launch.
 //
 // Within a tile each warp takes its own 16, 32 or 64 keys (4 KB for any head
 // size) with running maxima of its own, joined at the end of an item: no
 // block barrier inside the loop.  A warp copies its keys through shared memory
-// with 16-byte asynchronous copies, kStages - 1 steps ahead; keys beyond the
+// with 16-byte asynchronous copies, two or three steps ahead; keys beyond the
 // length are filled with zeros, whatever the page holds there.
 #include <type_traits>
 
 #include "paged.cuh"
+#include "sync.cuh"
 
 namespace cb {
 namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kStages = 4;
 constexpr int kStepBytes = 4096;                 // K and V of one warp's step
 constexpr int kHeadBytes = 64;                   // its scales: 4 of K, 4 of V
 constexpr int kSlotBytes = kStepBytes + kHeadBytes;
-constexpr int kRing = kWarps * kStages * kSlotBytes;
 
 // How the query rows fill the tensor core's 16-row tiles.
 enum { kPacked = 0, kOneTile = 1, kTwoTiles = 2 };
+// Resident blocks of an SM, and steps of a warp's ring: the registers (the
+// sums of 8, 16 or 32 rows) set the first, shared memory the second.
+__host__ __device__ constexpr int resident_of(int mode) { return mode == kPacked ? 4 : mode == kOneTile ? 3 : 2; }
+__host__ __device__ constexpr int stages_of(int mode) { return mode == kPacked ? 3 : 4; }
+__host__ __device__ constexpr int ring_bytes(int mode) { return kWarps * stages_of(mode) * kSlotBytes; }
 __host__ __device__ constexpr int rows_of(int mode) { return mode == kPacked ? 8 : 16 * mode; }
 __host__ __device__ constexpr int step_keys(int head_size) { return 2048 / head_size; }
 __host__ __device__ constexpr int tile_keys(int head_size) { return kWarps * step_keys(head_size); }
 
-// Shared memory of a block: the ring, and the queries that are not in registers.
+// Shared memory of a block: the ring, and the queries as the products read them.
 __host__ __device__ constexpr int shared_bytes(int head_size, int mode, int lo) {
-  return kRing + (mode == kPacked ? 0 : mode * (lo ? 2 : 1) * (head_size / 16) * 512);
+  return ring_bytes(mode) + (mode == kTwoTiles ? 2 : 1) * (lo ? 2 : 1) * (head_size / 16) * 512;
 }
 // Tiles' time that beginning an item costs (queries, first loads, joining the
 // warps): counted when the work is divided.
@@ -194,8 +198,9 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 struct Plan {  // of one launch
   cb_paged_attention_args a;
   int group, rows, blocks;  // query heads of a kv head, rows of a kv head, blocks of them
-  int4* cuts;               // scratch: for each block, the item that it begins and does not end
+  bool wide;                // queries can be read 16 bytes at a time
   float* partial;           // scratch: two partial results of each block
+  unsigned* arrived;        // for each block: parts of the item that it begins and does not end
 };
 
 struct Slot {
@@ -247,64 +252,100 @@ struct Sums {
   float m[kTiles][kHalves], l[kTiles][kHalves];
 };
 
+// Eight neighbouring elements of a query row.
+__device__ __forceinline__ void load_query(const Plan& p, const void* query, long long at, float* x) {
+  if (!p.wide) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = load_as_f32(query, at + i, p.a.dtype);
+  } else if (p.a.dtype == CB_F32) {
+    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(query) + at);
+    const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(query) + at + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  } else {
+    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(query) + at);
+    if (p.a.dtype == CB_BF16) {
+      unpack_bf16x8(w, x);
+    } else {
+      const __half2* h = reinterpret_cast<const __half2*>(&w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __low2float(h[i]);
+        x[2 * i + 1] = __high2float(h[i]);
+      }
+    }
+  }
+}
+
+// The block's query rows as the products read them: `queries` holds the 16-row
+// operands of each 16-element product, `factors` what turns a row's products
+// into scores in base 2.  SIZE / 8 neighbouring threads take a row; rows that
+// do not exist are zero.
+template <int SIZE, int MODE, int LO>
+__device__ __forceinline__ void load_queries(const Plan& p, const void* query, int count, int head, int first_row,
+                                             uint4* queries, float* factors) {
+  constexpr int kLanes = SIZE / 8, kDots = SIZE / 16, kParts = LO ? 2 : 1;
+  constexpr int kKeyWords = SIZE / 16 < 4 ? SIZE / 16 : 4;
+#pragma unroll
+  for (int first = 0; first < rows_of(MODE); first += kThreads / kLanes) {
+    const int row = first + static_cast<int>(threadIdx.x) / kLanes, d = static_cast<int>(threadIdx.x) % kLanes * 8;
+    const int r = first_row + row, t = r / p.group;
+    float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, largest = 0.0f;
+    if (row < rows_of(MODE) && r < p.rows && t < count)
+      load_query(p, query, t * p.a.q_strides[1] + (head * p.group + r % p.group) * p.a.q_strides[2] + d, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(x[i]));
+#pragma unroll
+    for (int o = 1; o < kLanes; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+    if (row >= rows_of(MODE)) continue;
+    // 2^e <= largest < 2^(e + 1); e in [-126, 127], and 2^-e is exact
+    const int e = min(max(static_cast<int>(__float_as_uint(largest) >> 23) - 127, -126), 127);
+    const float down = e == 127 ? 5.877471754111438e-39f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    if (d == 0)
+      factors[row] = p.a.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+    for (int word = 0; word < 2; ++word) {
+      const int at = d + 4 * word;  // of word `k` of read at / 64 of a key row, by the lanes of column `quad`
+      const int quad = at % 64 / (4 * kKeyWords), dot = at / 64 * kKeyWords + at % (4 * kKeyWords) / 4;
+      uint32_t* to = reinterpret_cast<uint32_t*>(queries + (row / 16 * kParts * kDots + dot) * 32 + row % 8 * 4 + quad);
+#pragma unroll
+      for (int pair = 0; pair < 2; ++pair) {
+        uint32_t hi, lo;
+        split(x[4 * word + 2 * pair] * down, x[4 * word + 2 * pair + 1] * down, hi, lo);
+        if (MODE == kPacked) {
+          to[2 * pair] = hi;
+          to[2 * pair + 1] = lo;
+        } else {
+          to[2 * pair + row / 8 % 2] = hi;
+          if (LO) to[kDots * 128 + 2 * pair + row / 8 % 2] = lo;
+        }
+      }
+    }
+  }
+}
+
 template <int SIZE, int STORAGE, int MODE, int LO>
-__device__ __forceinline__ void warp_item(const Plan& p, const void* query, const Slot& s, int head, int first_row, int tile, int tiles,
-                                          char* ring, uint4* queries, Sums<SIZE, MODE>& sums) {
+__device__ __forceinline__ void warp_item(const Plan& p, const void* query, const Slot& s, int head, int first_row,
+                                          int tile, int tiles, char* ring, uint4* queries, float* factors,
+                                          Sums<SIZE, MODE>& sums) {
   using S = Sums<SIZE, MODE>;
   constexpr int kKeys = step_keys(SIZE), kSubs = kKeys / 16;
   constexpr int kDots = SIZE / 16;                        // 16-element products of a score
   constexpr int kKeyWords = SIZE / 16 < 4 ? SIZE / 16 : 4;  // words of one read of a key row
   constexpr int kKeyReads = SIZE / 16 / kKeyWords;
   constexpr int kValueWords = SIZE / 32;
-  constexpr int kParts = LO ? 2 : 1;
+  constexpr int kParts = LO ? 2 : 1, kStages = stages_of(MODE);
   const cb_paged_cache& c = p.a.cache;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
 
   // limits: row r sees keys below limit[r]; all rows of the block see those below `common`
   int limit[S::kTiles][S::kHalves];
-  uint32_t q[kDots][4];  // a packed tile's queries; others lie in `queries`
-  float factor[S::kTiles][S::kHalves];
 #pragma unroll
   for (int mt = 0; mt < S::kTiles; ++mt) {
 #pragma unroll
     for (int half = 0; half < S::kHalves; ++half) {
       const int r = first_row + mt * 16 + half * 8 + g, t = r / p.group;
-      const bool real = r < p.rows && t < s.row.count;
-      limit[mt][half] = real ? s.row.length - s.row.count + t + 1 : 0;
-      const long long at = real ? t * p.a.q_strides[1] + (head * p.group + r % p.group) * p.a.q_strides[2] : 0;
-      float x[kDots][4], largest = 0.0f;
-#pragma unroll
-      for (int k = 0; k < kDots; ++k) {
-        // the elements of word k % kKeyWords of this lane's read k / kKeyWords of a key row
-        const int d = (k / kKeyWords) * 64 + quad * (4 * kKeyWords) + (k % kKeyWords) * 4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[k][i] = real ? load_as_f32(query, at + d + i, p.a.dtype) : 0.0f;
-          largest = fmaxf(largest, fabsf(x[k][i]));
-        }
-      }
-      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-      // 2^e <= largest < 2^(e + 1); e in [-126, 127], and 2^-e is exact
-      const int e = min(max(static_cast<int>(__float_as_uint(largest) >> 23) - 127, -126), 127);
-      const float down = e == 127 ? 5.877471754111438e-39f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      factor[mt][half] = p.a.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-#pragma unroll
-      for (int k = 0; k < kDots; ++k) {
-#pragma unroll
-        for (int pair = 0; pair < 2; ++pair) {
-          uint32_t hi, lo;
-          split(x[k][2 * pair] * down, x[k][2 * pair + 1] * down, hi, lo);
-          if (MODE == kPacked) {
-            q[k][2 * pair] = hi;
-            q[k][2 * pair + 1] = lo;
-          } else if (k % kWarps == warp) {  // every warp has them all; each stores a part
-            uint32_t* to = reinterpret_cast<uint32_t*>(queries + (mt * kParts * kDots + k) * 32 + lane);
-            to[2 * pair + half] = hi;
-            if (LO) to[kDots * 128 + 2 * pair + half] = lo;
-          }
-        }
-      }
+      limit[mt][half] = r < p.rows && t < s.row.count ? s.row.length - s.row.count + t + 1 : 0;
       sums.m[mt][half] = -INFINITY;
       sums.l[mt][half] = 0.0f;
 #pragma unroll
@@ -365,7 +406,13 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) prefetch(i);
 
-  if (MODE != kPacked) __syncthreads();
+  load_queries<SIZE, MODE, LO>(p, query, s.row.count, head, first_row, queries, factors);
+  __syncthreads();
+  float factor[S::kTiles][S::kHalves];
+#pragma unroll
+  for (int mt = 0; mt < S::kTiles; ++mt)
+#pragma unroll
+    for (int half = 0; half < S::kHalves; ++half) factor[mt][half] = factors[mt * 16 + half * 8 + g];
   for (int step = 0; step < tiles; ++step) {
     wait_groups<kStages - 2>();
     __syncwarp();  // every lane's copies of this step have landed; every lane has left the slot filled next
@@ -376,32 +423,31 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
 
     float score[S::kTiles][2 * kSubs][4];
 #pragma unroll
-    for (int n = 0; n < 2 * kSubs; ++n) {
-      const int row = n * 8 + key_of(g);
+    for (int r = 0; r < kKeyReads; ++r) {
+      uint32_t w[2 * kSubs][kKeyWords];
+      const int element = r * 64 + quad * (4 * kKeyWords);
 #pragma unroll
-      for (int r = 0; r < kKeyReads; ++r) {
-        uint32_t w[kKeyWords];
-        const int element = r * 64 + quad * (4 * kKeyWords);
-        read_words<kKeyWords>(slot + swizzled<SIZE>(row, element / 16) + element % 16, w);
+      for (int n = 0; n < 2 * kSubs; ++n)
+        read_words<kKeyWords>(slot + swizzled<SIZE>(n * 8 + key_of(g), element / 16) + element % 16, w[n]);
 #pragma unroll
-        for (int k = 0; k < kKeyWords; ++k) {
+      for (int k = 0; k < kKeyWords; ++k) {
+        const int dot = r * kKeyWords + k;
+        uint4 a[S::kTiles][kParts];
+#pragma unroll
+        for (int mt = 0; mt < S::kTiles; ++mt)
+#pragma unroll
+          for (int part = 0; part < kParts; ++part) a[mt][part] = queries[((mt * kParts + part) * kDots + dot) * 32 + lane];
+#pragma unroll
+        for (int n = 0; n < 2 * kSubs; ++n) {
           uint32_t b0, b1;
-          to_halves<STORAGE>(w[k], b0, b1);
+          to_halves<STORAGE>(w[n][k], b0, b1);
 #pragma unroll
           for (int mt = 0; mt < S::kTiles; ++mt) {
 #pragma unroll
             for (int part = 0; part < kParts; ++part) {
-              const int dot = r * kKeyWords + k;
-              uint32_t a[4];
-              if (MODE == kPacked) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = q[dot][i];
-              } else {
-                const uint4 v = queries[((mt * kParts + part) * kDots + dot) * 32 + lane];
-                a[0] = v.x; a[1] = v.y; a[2] = v.z; a[3] = v.w;
-              }
-              if (dot == 0 && part == 0) mma<true>(score[mt][n], a, b0, b1);
-              else mma<false>(score[mt][n], a, b0, b1);
+              const uint32_t row[4] = {a[mt][part].x, a[mt][part].y, a[mt][part].z, a[mt][part].w};
+              if (dot == 0 && part == 0) mma<true>(score[mt][n], row, b0, b1);
+              else mma<false>(score[mt][n], row, b0, b1);
             }
           }
         }
@@ -558,33 +604,65 @@ __device__ __forceinline__ void store4(const Plan& p, long long at, const float*
 template <int SIZE, int MODE>
 __host__ __device__ constexpr int partial_floats() { return rows_of(MODE) * (SIZE + 2); }
 
+// An item that a cut divided: its first part, then the first partial results of
+// the following blocks (`rest` + 2 k of them), in that order.
+template <int SIZE, int MODE>
+__device__ __forceinline__ void join(const Plan& p, long long b, int head, int first_row, int count, int parts,
+                                     const float* first, const float* rest) {
+  constexpr int kRows = rows_of(MODE), kFloats = partial_floats<SIZE, MODE>();
+  for (int i = threadIdx.x; i < kRows * SIZE / 4; i += kThreads) {
+    const int r = i / (SIZE / 4), d = i % (SIZE / 4) * 4, row = first_row + r;
+    if (row >= p.rows) continue;
+    float top = -INFINITY, sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+    for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg((k ? rest + 2LL * k * kFloats : first) + r));
+#pragma unroll 8
+    for (int k = 0; k < parts; ++k) {
+      const float* part = k ? rest + 2LL * k * kFloats : first;
+      const float most = __ldcg(part + r);
+      const float f = most == -INFINITY ? 0.0f : root2_of(most - top);
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(part + 2 * kRows + r * SIZE + d));
+      sum += f * __ldcg(part + kRows + r) * f;
+      v[0] += f * x.x * f; v[1] += f * x.y * f; v[2] += f * x.z * f; v[3] += f * x.w * f;
+    }
+    const bool real = row / p.group < count && sum != 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = real ? v[k] / sum : 0.0f;
+    store4(p, out_row<SIZE>(p, b, head, row) + d, v);
+  }
+}
+
 template <int SIZE, int STORAGE, int MODE, int LO>
-__global__ void __launch_bounds__(kThreads, MODE == kTwoTiles ? 2 : 3) attention_kernel(const __grid_constant__ Plan p) {
+__global__ void __launch_bounds__(kThreads, resident_of(MODE)) attention_kernel(const __grid_constant__ Plan p) {
   using S = Sums<SIZE, MODE>;
   constexpr int kRows = rows_of(MODE);
   extern __shared__ __align__(128) char shared[];
   __shared__ long long scan[kWarps];
-  __shared__ float most[kWarps][kRows], total[kWarps][kRows];
+  __shared__ float most[kWarps][kRows], total[kWarps][kRows], factors[kRows];
   __shared__ long long found[2];
   const long long batch = p.a.batch;
   const int items = p.a.cache.kv_heads * p.blocks;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  pdl_launch_dependents();
   // the tiles of all slots, and this block's range of them
   long long mine = 0, all;
-  for (long long b = threadIdx.x; b < batch; b += kThreads) mine += slot_of<SIZE>(p, b).tiles + kItemCost;
+  int span_first = 0;  // of slot threadIdx.x
+  for (long long b = threadIdx.x; b < batch; b += kThreads) {
+    const int span = slot_of<SIZE>(p, b).tiles + kItemCost;
+    if (b < kThreads) span_first = span;
+    mine += span;
+  }
   block_scan(mine, scan, &all);
   all *= items;
   const long long per = (all + gridDim.x - 1) / gridDim.x;
   long long at = per * blockIdx.x;
   const long long end = at + per < all ? at + per : all;
-  if (threadIdx.x == 0) p.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);
   if (at >= end) return;
   long long before = 0;
   for (long long first = 0; first < batch; first += kThreads) {
     const long long b = first + threadIdx.x;
-    const long long tiles = b < batch ? (slot_of<SIZE>(p, b).tiles + kItemCost) * static_cast<long long>(items) : 0;
+    const int span = first == 0 ? span_first : b < batch ? slot_of<SIZE>(p, b).tiles + kItemCost : 0;
+    const long long tiles = static_cast<long long>(span) * items;
     long long sum;
     const long long lower = before + block_scan(tiles, scan, &sum);
     if (lower <= at && at < lower + tiles) {
@@ -624,7 +702,8 @@ __global__ void __launch_bounds__(kThreads, MODE == kTwoTiles ? 2 : 3) attention
     Sums<SIZE, MODE> sums;
     const void* query = static_cast<const char*>(p.a.q) + b * p.a.q_strides[0] * (p.a.dtype == CB_F32 ? 4 : 2);
     warp_item<SIZE, STORAGE, MODE, LO>(p, query, s, head, first_row, tile, tiles,
-                                       shared + warp * kStages * kSlotBytes, reinterpret_cast<uint4*>(shared + kRing), sums);
+                                       shared + warp * stages_of(MODE) * kSlotBytes,
+                                       reinterpret_cast<uint4*>(shared + ring_bytes(MODE)), factors, sums);
 
     // join the warps
     __syncthreads();  // every warp is done with the ring
@@ -681,42 +760,23 @@ __global__ void __launch_bounds__(kThreads, MODE == kTwoTiles ? 2 : 3) attention
         }
       }
     }
-    if (!whole && tile == 0 && threadIdx.x == 0) {
-      const long long last = (item_at + span - 1) / per;  // block of the item's last tile
-      p.cuts[blockIdx.x] = make_int4(static_cast<int>(b), item, static_cast<int>(last), begins ? 0 : 1);
+    if (!whole) {
+      const long long from = (item_at + kItemCost) / per, last = (item_at + span - 1) / per;  // blocks of its tiles
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        const bool all_there = ticket_acq_rel(p.arrived + from) == static_cast<unsigned>(last - from);
+        if (all_there) p.arrived[from] = 0;
+        found[0] = all_there;
+      }
+      __syncthreads();
+      if (found[0]) {
+        const int own = item_at + kItemCost <= from * per ? 0 : 1;  // the first part's place
+        join<SIZE, MODE>(p, b, head, first_row, s.row.count, static_cast<int>(last - from) + 1,
+                         p.partial + (2 * from + own) * partial_floats<SIZE, MODE>(),
+                         p.partial + 2 * from * partial_floats<SIZE, MODE>());
+      }
     }
     __syncthreads();  // the joined rows are read; the ring is free again
-  }
-}
-
-// The items that were cut: one block for each block that began one.
-template <int SIZE, int MODE>
-__global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ Plan p) {
-  constexpr int kRows = rows_of(MODE), kFloats = partial_floats<SIZE, MODE>();
-  pdl_wait();
-  const int4 cut = p.cuts[blockIdx.x];
-  if (cut.x < 0) return;
-  const int head = cut.y / p.blocks, first_row = cut.y % p.blocks * kRows, parts = cut.z - static_cast<int>(blockIdx.x) + 1;
-  // its first part, then the first partial results of the following blocks
-  const float* first = p.partial + (2LL * blockIdx.x + cut.w) * kFloats;
-  const float* rest = p.partial + 2LL * blockIdx.x * kFloats;
-  const int count = p.a.counts != nullptr ? p.a.counts[cut.x] : static_cast<int>(p.a.tokens);
-  for (int i = threadIdx.x; i < kRows * SIZE / 4; i += kThreads) {
-    const int r = i / (SIZE / 4), d = i % (SIZE / 4) * 4, row = first_row + r;
-    if (row >= p.rows) continue;
-    float top = -INFINITY, sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k = 0; k < parts; ++k) top = fmaxf(top, (k ? rest + 2LL * k * kFloats : first)[r]);
-    for (int k = 0; k < parts; ++k) {
-      const float* part = k ? rest + 2LL * k * kFloats : first;
-      const float f = part[r] == -INFINITY ? 0.0f : root2_of(part[r] - top);
-      const float4 x = *reinterpret_cast<const float4*>(part + 2 * kRows + r * SIZE + d);
-      sum += f * part[kRows + r] * f;
-      v[0] += f * x.x * f; v[1] += f * x.y * f; v[2] += f * x.z * f; v[3] += f * x.w * f;
-    }
-    const bool real = row / p.group < count && sum != 0.0f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = real ? v[k] / sum : 0.0f;
-    store4(p, out_row<SIZE>(p, cut.x, head, row) + d, v);
   }
 }
 
@@ -794,38 +854,42 @@ long long cb_paged_attention_scratch(const cb_paged_attention_args* args) {
   if (args == nullptr || attention_check(*args) != CB_OK || args->batch == 0 || args->tokens == 0) return 0;
   return with_variant(*args, [&](auto size, auto storage, auto mode, auto lo) -> long long {
     const int per_sm = resident_blocks<size.value, storage.value, mode.value, lo.value>();
-    return grid_of<size.value, mode.value>(*args, per_sm) * (16 + 8LL * partial_floats<size.value, mode.value>());
+    return grid_of<size.value, mode.value>(*args, per_sm) * 8LL * partial_floats<size.value, mode.value>();
   });
 }
 
-int cb_paged_attention(const cb_paged_attention_args* args, void* scratch, cb_stream_t stream) {
+long long cb_paged_attention_counters(const cb_paged_attention_args* args) {
+  if (args == nullptr || attention_check(*args) != CB_OK) return 0;
+  return 8LL * sm_count();  // more than any launch has blocks
+}
+
+int cb_paged_attention(const cb_paged_attention_args* args, void* scratch, unsigned* counters, cb_stream_t stream) {
   CB_REQUIRE(args != nullptr, "cb_paged_attention: null arguments");
   const cb_paged_attention_args& a = *args;
   const int status = attention_check(a);
   if (status != CB_OK) return status;
   if (a.batch == 0 || a.tokens == 0) return CB_OK;
-  CB_REQUIRE(a.q != nullptr && a.out != nullptr && scratch != nullptr, "cb_paged_attention: a null pointer");
+  CB_REQUIRE(a.q != nullptr && a.out != nullptr && scratch != nullptr && counters != nullptr, "cb_paged_attention: a null pointer");
   CB_REQUIRE(reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && reinterpret_cast<uintptr_t>(scratch) % 16 == 0,
              "cb_paged_attention: out and scratch must be 16-byte aligned");
   return static_cast<int>(with_variant(a, [&](auto size, auto storage, auto mode, auto lo) -> long long {
     constexpr int SIZE = size.value, STORAGE = storage.value, MODE = mode.value, LO = lo.value;
     const int per_sm = resident_blocks<SIZE, STORAGE, MODE, LO>();
-    CB_REQUIRE(per_sm >= 1, "cb_paged_attention: the kernel does not fit this device");
+    CB_REQUIRE(per_sm >= 1 && per_sm <= 8, "cb_paged_attention: %d blocks of the kernel fit an SM", per_sm);
     const long long grid = grid_of<SIZE, MODE>(a, per_sm);
     Plan p;
     p.a = a;
     p.group = static_cast<int>(a.heads / a.cache.kv_heads);
     p.rows = static_cast<int>(a.tokens * p.group);
     p.blocks = (p.rows + rows_of(MODE) - 1) / rows_of(MODE);
-    p.cuts = static_cast<int4*>(scratch);
-    p.partial = reinterpret_cast<float*>(p.cuts + grid);
-    const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const dim3 blocks(static_cast<unsigned>(grid));
-    launch(attention_kernel<SIZE, STORAGE, MODE, LO>, blocks, dim3(kThreads), shared_bytes(SIZE, MODE, LO), s, false, p);
-    const int status = check_launch("cb_paged_attention");
-    if (status != CB_OK) return status;
-    launch(join_kernel<SIZE, MODE>, blocks, dim3(kThreads), 0, s, true, p);
-    return check_launch("cb_paged_attention: join");
+    const int item = a.dtype == CB_F32 ? 4 : 2;
+    p.wide = reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
+    for (int i = 0; i < 3; ++i) p.wide = p.wide && a.q_strides[i] * item % 16 == 0;
+    p.partial = static_cast<float*>(scratch);
+    p.arrived = counters;
+    launch(attention_kernel<SIZE, STORAGE, MODE, LO>, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
+           shared_bytes(SIZE, MODE, LO), static_cast<cudaStream_t>(stream), false, p);
+    return check_launch("cb_paged_attention");
   }));
 }
 

@@ -155,7 +155,7 @@ class PagedCache:
         p.page_bytes = self.kv_heads * self.page_size * self.head_size
         self._lib = _lib.load()
         self._attend_args, self._append_args, self._lists = Prepared(), Prepared(), Prepared()
-        self._scratch_words = Prepared()
+        self._scratch_words, self._counters = Prepared(), Prepared()
 
     @classmethod
     def allocate(cls, *, layers: int, pages: int, kv_heads: int, page_size: int, head_size: int, sequences: int,
@@ -285,14 +285,29 @@ class PagedCache:
             a.counts = counts.data_ptr()
         if sequences is not None:
             a.sequences = sequences.data_ptr()
-        scratch = self._flag.new_empty(known[1])
-        _lib.check(self._lib.cb_paged_attention(ctypes.byref(a), scratch.data_ptr(), self._stream()),
+        scratch, stream = self._flag.new_empty(known[1]), self._stream()
+        counters = self._counters_of(stream, known[2])
+        _lib.check(self._lib.cb_paged_attention(ctypes.byref(a), scratch.data_ptr(), counters.data_ptr(), stream),
                    "cb_paged_attention")
         return out
 
+    def _counters_of(self, stream: int, count: int) -> torch.Tensor:
+        """Zeroed counters for a call on ``stream``, which leaves them zero.
+
+        Calls of one stream follow one another and share theirs.  A captured
+        call may be replayed on any stream, so it has its own, cleared within
+        the graph.
+        """
+        if torch.cuda.is_current_stream_capturing():
+            return self._flag.new_zeros(count)
+        counters = self._counters.get(stream)
+        if counters is None or counters.shape[0] < count:
+            counters = self._counters[stream] = self._flag.new_zeros(count)
+        return counters
+
     def _prepare_attend(self, layer: int, q: torch.Tensor, counts: Optional[torch.Tensor],
                         sequences: Optional[torch.Tensor],
-                        scale: Optional[float]) -> Tuple[_lib.PagedAttentionArgs, int]:
+                        scale: Optional[float]) -> Tuple[_lib.PagedAttentionArgs, int, int]:
         require(q, "q", self.device, tuple(_VALUES), (None, None, None, self.head_size), 1)
         batch, tokens, heads = q.shape[:3]
         if heads == 0 or heads % self.kv_heads:
@@ -304,7 +319,8 @@ class PagedCache:
         a.q_strides[:] = q.stride()[:3]
         a.scale = 1.0 / math.sqrt(self.head_size) if scale is None else scale
         a.error_flag = self._flag.data_ptr()
-        return a, (self._lib.cb_paged_attention_scratch(ctypes.byref(a)) + 3) // 4
+        return (a, (self._lib.cb_paged_attention_scratch(ctypes.byref(a)) + 3) // 4,
+                self._lib.cb_paged_attention_counters(ctypes.byref(a)))
 
     # -- pages -------------------------------------------------------------
     def extend(self, counts: Any, *, sequences: Any = None) -> None:

@@ -820,7 +820,9 @@ CB_API int cb_paged_append(const cb_paged_append_args* args, cb_stream_t stream)
  * length - n + t), grouped kv heads, float32 softmax and sums.  A row that
  * sees no key gives zeros.  out: as q, contiguous, q's dtype.  Serves single
  * tokens, blocks of drafted tokens and short prompt chunks.  `scratch`:
- * cb_paged_attention_scratch bytes, 16-byte aligned. */
+ * cb_paged_attention_scratch bytes, 16-byte aligned; `counters`:
+ * cb_paged_attention_counters unsigned ints, zero before the first call (calls
+ * leave them zero, and may not share them while they overlap). */
 typedef struct {
   cb_paged_cache cache;
   const void* q; /* (batch, tokens, heads, head_size), head_size contiguous */
@@ -834,7 +836,9 @@ typedef struct {
   int* error_flag;
 } cb_paged_attention_args;
 CB_API long long cb_paged_attention_scratch(const cb_paged_attention_args* args);
-CB_API int cb_paged_attention(const cb_paged_attention_args* args, void* scratch, cb_stream_t stream);
+CB_API long long cb_paged_attention_counters(const cb_paged_attention_args* args);
+CB_API int cb_paged_attention(const cb_paged_attention_args* args, void* scratch, unsigned* counters,
+                              cb_stream_t stream);
 
 /* The book of a cache: who holds which page.  refs[p] slots hold page p;
  * free[0 .. *height) is a stack of the pages that none holds.  A slot of

@@ -39,7 +39,7 @@ def attend(c, **changes):
     a = _lib.PagedAttentionArgs(cache=c, q=16, out=16, dtype=_lib.F32, batch=1, tokens=1, heads=2, scale=1.0)
     for name, value in changes.items():
         setattr(a, name, value)
-    return _lib.call("cb_paged_attention", ctypes.byref(a), 16, None)
+    return _lib.call("cb_paged_attention", ctypes.byref(a), 16, 16, None)
 
 
 @pytest.mark.parametrize("change", [dict(storage=_lib.BF16), dict(head_size=48), dict(page=8), dict(page=24),
