@@ -240,6 +240,8 @@ __device__ __forceinline__ long long block_scan(long long v, long long* shared, 
   return before + incl - v;
 }
 
+constexpr float kSlack = 16.0f;
+
 // ---- one item ------------------------------------------------------------------
 
 // The sums of one warp: its rows g (and g + 8 of each 16-row tile), columns
@@ -462,6 +464,14 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
     for (int mt = 0; mt < S::kTiles; ++mt) {
 #pragma unroll
       for (int half = 0; half < S::kHalves; ++half) {
+        if (MODE == kTwoTiles && first_row + mt * 16 + half * 8 >= p.rows) {  // no such rows
+#pragma unroll
+          for (int n = 0; n < 2 * kSubs; ++n) weight[mt][0][n / 2][2 * (n & 1) + half] = 0u;
+#pragma unroll
+          for (int sub = 0; sub < kSubs; ++sub) fold[mt][half][sub] = 0.0f;
+          root[mt][half] = 1.0f;
+          continue;
+        }
         float x[2 * kSubs][2], most = -INFINITY;
 #pragma unroll
         for (int n = 0; n < 2 * kSubs; ++n) {
@@ -499,7 +509,10 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
             if (LO) weight[mt][kParts - 1][n / 2][2 * (n & 1) + half] = lo;
           }
         }
-        const float old = sums.m[mt][half], now = fmaxf(old, most);
+        // The sums are kept against a maximum that follows the running one only
+        // when that is 2^kSlack above it: float32 has room for such factors,
+        // and the sums are scaled once an item, not at every new maximum.
+        const float old = sums.m[mt][half], now = most > old + kSlack ? most : old;
         const float against = now == -INFINITY ? 0.0f : now;
         grows = grows || now > old;
         const float r = root2_of(old - against);
