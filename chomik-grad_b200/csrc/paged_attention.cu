@@ -19,12 +19,12 @@
 //     and the lo parts rows 8-15, at no cost.  16-bit queries in more than 8
 //     rows are used as they are (exact but for elements 2^-14 below the row's
 //     largest, whose error is below 2^-25 of that);
-//   - the probabilities of a step are taken against the step's own maximum and
-//     split the same way (16-bit outputs of more than 8 rows: hi only, a
-//     relative error of 2^-12 a weight, below the output's own rounding);
-//   - the step's product is then added to the float32 sums with the factor
-//     exp(step maximum - running maximum) * value scale, whose exponents are
-//     added first, so that neither over- nor underflows before the whole does.
+//   - what multiplies the value codes is the weight exp(s_j - m) times the
+//     page's value scale: the running maximum m is that of the scores plus the
+//     scales' exponents, so that these products stay within fp16 whatever the
+//     scales, and they are split the same way (16-bit outputs of more than 8
+//     rows: hi only, a relative error of 2^-12 a weight, below the output's own
+//     rounding).  The sum of the weights leaves the scale out again.
 //
 // How the work is laid out.  The keys of all (slot, kv head, block of rows)
 // are one sequence of tiles, cut into equal ranges for a grid that fills the
@@ -176,23 +176,6 @@ __device__ __forceinline__ float exp2_of(float x) {
 // kept where 2^x itself would be below float32's range.
 __device__ __forceinline__ float root2_of(float x) { return exp2_of(0.5f * x); }
 
-// Pairs of float32: two sums or products in one instruction.
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<unsigned long long&>(r))
-      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
-  return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(reinterpret_cast<unsigned long long&>(r))
-      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
-        "l"(reinterpret_cast<unsigned long long&>(c)));
-  return r;
-}
-
 // ---- division of the work ------------------------------------------------------
 
 struct Plan {  // of one launch
@@ -240,7 +223,9 @@ __device__ __forceinline__ long long block_scan(long long v, long long* shared, 
   return before + incl - v;
 }
 
-constexpr float kSlack = 16.0f;
+// Weights are at most 2^(kSlack + 1): far inside fp16, with its 11 (hi and lo:
+// 22) bits for all that are within 2^-14 of the largest.
+constexpr float kSlack = 8.0f;
 
 // ---- one item ------------------------------------------------------------------
 
@@ -250,7 +235,7 @@ template <int SIZE, int MODE>
 struct Sums {
   static constexpr int kTiles = MODE == kTwoTiles ? 2 : 1;
   static constexpr int kHalves = MODE == kPacked ? 1 : 2;
-  float2 o[kTiles][kHalves][SIZE / 8];
+  float o[kTiles][SIZE / 8][4];  // as the products leave them; packed: of the hi and the lo weights
   float m[kTiles][kHalves], l[kTiles][kHalves];
 };
 
@@ -350,10 +335,13 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
       limit[mt][half] = r < p.rows && t < s.row.count ? s.row.length - s.row.count + t + 1 : 0;
       sums.m[mt][half] = -INFINITY;
       sums.l[mt][half] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < SIZE / 8; ++j) sums.o[mt][half][j] = make_float2(0.0f, 0.0f);
     }
+#pragma unroll
+    for (int j = 0; j < SIZE / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sums.o[mt][j][i] = 0.0f;
   }
+  int last = 0;  // exponent of the value scale before
   const int common = s.row.length - s.row.count + first_row / p.group + 1;
   const int length = s.row.count > 0 ? s.row.length : 0;
 
@@ -456,10 +444,20 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
       }
     }
 
+    // value scales as 2^exponent * fraction; one that is zero takes the exponent
+    // before it, its weights count in the sum all the same
+    float exponent[kSubs], fraction[kSubs], undo[kSubs];
+#pragma unroll
+    for (int sub = 0; sub < kSubs; ++sub) {
+      const uint32_t word = __float_as_uint(scales[4 + sub]);
+      const int e = static_cast<int>(word >> 23 & 0xffu) - 127;
+      const bool normal = e > -127 && e < 127;
+      if (normal) last = e;
+      fraction[sub] = normal ? __uint_as_float((word & 0x807fffffu) | 0x3f800000u) : e < 0 ? 0.0f : NAN;
+      exponent[sub] = static_cast<float>(last);
+      undo[sub] = __uint_as_float(static_cast<uint32_t>(127 - last) << 23);
+    }
     uint32_t weight[S::kTiles][kParts][kSubs][4];
-    float fold[S::kTiles][S::kHalves][kSubs];
-    bool grows = false;
-    float root[S::kTiles][S::kHalves];
 #pragma unroll
     for (int mt = 0; mt < S::kTiles; ++mt) {
 #pragma unroll
@@ -467,9 +465,6 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
         if (MODE == kTwoTiles && first_row + mt * 16 + half * 8 >= p.rows) {  // no such rows
 #pragma unroll
           for (int n = 0; n < 2 * kSubs; ++n) weight[mt][0][n / 2][2 * (n & 1) + half] = 0u;
-#pragma unroll
-          for (int sub = 0; sub < kSubs; ++sub) fold[mt][half][sub] = 0.0f;
-          root[mt][half] = 1.0f;
           continue;
         }
         float x[2 * kSubs][2], most = -INFINITY;
@@ -478,8 +473,8 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
           const float f = factor[mt][half] * scales[n / 2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float v = MODE == kPacked ? score[mt][n][i] + score[mt][n][2 + i] : score[mt][n][2 * half + i];
-            x[n][i] = v * f;
+            const float v = MODE == kPacked ? score[mt][n][i] + score[mt][n][2 + i] : score[mt][n][2 * half + i];
+            x[n][i] = fmaf(v, f, exponent[n / 2]);
           }
         }
         if (key + kKeys > common) {  // (the same for the warp) columns 2 quad and 2 quad + 1
@@ -493,14 +488,33 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
         for (int n = 0; n < 2 * kSubs; ++n) most = fmaxf(most, fmaxf(x[n][0], x[n][1]));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const float base = most == -INFINITY ? 0.0f : most;
-        float sum = 0.0f;
+        // The sums are kept against a maximum that follows the running one only
+        // when that is 2^kSlack above it, so they are rarely scaled.
+        const float old = sums.m[mt][half];
+        if (__any_sync(0xffffffffu, most > old + kSlack)) {
+          const float now = most > old + kSlack ? most : old;
+          const float r = now == -INFINITY ? 1.0f : root2_of(old - now);
+          sums.m[mt][half] = now;
+          sums.l[mt][half] *= r * r;
+#pragma unroll
+          for (int j = 0; j < SIZE / 8; ++j) {
+            float* o = sums.o[mt][j];
+            if (MODE == kPacked) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[i] = o[i] * r * r;
+            } else {
+              o[2 * half] = o[2 * half] * r * r;
+              o[2 * half + 1] = o[2 * half + 1] * r * r;
+            }
+          }
+        }
+        const float against = sums.m[mt][half] == -INFINITY ? 0.0f : sums.m[mt][half];
 #pragma unroll
         for (int n = 0; n < 2 * kSubs; ++n) {
-          const float e0 = exp2_of(x[n][0] - base), e1 = exp2_of(x[n][1] - base);
-          sum += e0 + e1;
+          const float e0 = exp2_of(x[n][0] - against), e1 = exp2_of(x[n][1] - against);
+          sums.l[mt][half] = fmaf(e0 + e1, undo[n / 2], sums.l[mt][half]);
           uint32_t hi, lo;
-          split(e0, e1, hi, lo);
+          split(e0 * fraction[n / 2], e1 * fraction[n / 2], hi, lo);
           if (MODE == kPacked) {
             weight[mt][0][n / 2][2 * (n & 1)] = hi;
             weight[mt][0][n / 2][2 * (n & 1) + 1] = lo;
@@ -509,39 +523,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
             if (LO) weight[mt][kParts - 1][n / 2][2 * (n & 1) + half] = lo;
           }
         }
-        // The sums are kept against a maximum that follows the running one only
-        // when that is 2^kSlack above it: float32 has room for such factors,
-        // and the sums are scaled once an item, not at every new maximum.
-        const float old = sums.m[mt][half], now = most > old + kSlack ? most : old;
-        const float against = now == -INFINITY ? 0.0f : now;
-        grows = grows || now > old;
-        const float r = root2_of(old - against);
-        root[mt][half] = r;
-        sums.l[mt][half] = sums.l[mt][half] * r * r + sum * exp2_of(most - against);
-        sums.m[mt][half] = now;
-#pragma unroll
-        for (int sub = 0; sub < kSubs; ++sub) {
-          // exp2(most - now) * value scale = exp2(most - now + its exponent) * its fraction
-          const float vs = scales[4 + sub];
-          const uint32_t word = __float_as_uint(vs);
-          const int e = static_cast<int>(word >> 23 & 0xffu) - 127;
-          const bool normal = e > -127 && e < 128;
-          const float fraction = normal ? __uint_as_float((word & 0x807fffffu) | 0x3f800000u) : vs;
-          fold[mt][half][sub] = exp2_of(most - against + (normal ? static_cast<float>(e) : 0.0f)) * fraction;
-        }
       }
-    }
-    if (__any_sync(0xffffffffu, grows)) {
-#pragma unroll
-      for (int mt = 0; mt < S::kTiles; ++mt)
-#pragma unroll
-        for (int half = 0; half < S::kHalves; ++half)
-#pragma unroll
-          for (int j = 0; j < SIZE / 8; ++j) {
-            const float r = root[mt][half];
-            sums.o[mt][half][j].x = sums.o[mt][half][j].x * r * r;
-            sums.o[mt][half][j].y = sums.o[mt][half][j].y * r * r;
-          }
     }
 #pragma unroll
     for (int sub = 0; sub < kSubs; ++sub) {
@@ -560,25 +542,12 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
           to_halves<STORAGE>(__byte_perm(v[2 * pair][w], v[2 * pair + 1][w], 0x7362), b[2][pair], b[3][pair]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int mt = 0; mt < S::kTiles; ++mt) {
-            float t[4];
-            mma<true>(t, weight[mt][0][sub], b[i][0], b[i][1]);
-            if (LO) mma<false>(t, weight[mt][kParts - 1][sub], b[i][0], b[i][1]);
-            float2(*o)[SIZE / 8] = sums.o[mt];
-            const float f = fold[mt][0][sub], f8 = fold[mt][S::kHalves - 1][sub];
-            const float2 first = make_float2(t[0], t[1]), second = make_float2(t[2], t[3]);
-            float2& mine = o[0][w * 4 + i];
-            if (MODE == kPacked) {
-              mine = fma2(make_float2(f, f), add2(first, second), mine);
-            } else {
-              float2& other = o[S::kHalves - 1][w * 4 + i];
-              mine = fma2(make_float2(f, f), first, mine);
-              other = fma2(make_float2(f8, f8), second, other);
-            }
-          }
-        }
+          for (int mt = 0; mt < S::kTiles; ++mt)
+#pragma unroll
+            for (int part = 0; part < kParts; ++part)
+              mma<false>(sums.o[mt][w * 4 + i], weight[mt][part][sub], b[i][0], b[i][1]);
       }
     }
   }
@@ -733,12 +702,13 @@ __global__ void __launch_bounds__(kThreads, resident_of(MODE)) attention_kernel(
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           float* to = rows + (warp * kRows + r) * SIZE + element_of<SIZE>(2 * (lane & 3) + n);
-          const float2* o = sums.o[mt][half];
+          auto value = [&](int j) {
+            const float* o = sums.o[mt][j];
+            return MODE == kPacked ? o[n] + o[2 + n] : o[2 * half + n];
+          };
 #pragma unroll
           for (int j = 0; j < SIZE / 8; j += 4)
-            *reinterpret_cast<float4*>(to + j) =
-                make_float4(n ? o[j].y : o[j].x, n ? o[j + 1].y : o[j + 1].x, n ? o[j + 2].y : o[j + 2].x,
-                            n ? o[j + 3].y : o[j + 3].x);
+            *reinterpret_cast<float4*>(to + j) = make_float4(value(j), value(j + 1), value(j + 2), value(j + 3));
         }
       }
     __syncthreads();
