@@ -46,26 +46,30 @@
 namespace cb {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
-constexpr int kStepBytes = 4096;                 // K and V of one warp's step
+constexpr int kGroups = 4;                       // of keys, in a tile
+constexpr int kStepBytes = 4096;                 // K and V of a group's step
 constexpr int kHeadBytes = 64;                   // its scales: 4 of K, 4 of V
 constexpr int kSlotBytes = kStepBytes + kHeadBytes;
 
-// How the query rows fill the tensor core's 16-row tiles.
-enum { kPacked = 0, kOneTile = 1, kTwoTiles = 2 };
-// Resident blocks of an SM, and steps of a warp's ring: the registers (the
-// sums of 8, 16 or 32 rows) set the first, shared memory the second.
-__host__ __device__ constexpr int resident_of(int mode) { return mode == kPacked ? 4 : mode == kOneTile ? 3 : 2; }
-__host__ __device__ constexpr int stages_of(int mode) { return mode == kPacked ? 3 : 4; }
-__host__ __device__ constexpr int ring_bytes(int mode) { return kWarps * stages_of(mode) * kSlotBytes; }
+// How the query rows fill the tensor core's 16-row tiles: 8 of them with both
+// parts in one tile, or MODE tiles, each with warps of its own.
+enum { kPacked = 0 };
 __host__ __device__ constexpr int rows_of(int mode) { return mode == kPacked ? 8 : 16 * mode; }
+__host__ __device__ constexpr int tiles_of(int mode) { return mode == kPacked ? 1 : mode; }
+__host__ __device__ constexpr int warps_of(int mode) { return kGroups * tiles_of(mode); }
+__host__ __device__ constexpr int threads_of(int mode) { return 32 * warps_of(mode); }
+// Resident blocks of an SM: 16 warps of 128 registers, or, with the low parts of
+// float32 queries, 12 of 168.  The steps of a group's ring then follow from
+// shared memory, and from the joined rows that take its place.
+__host__ __device__ constexpr int resident_of(int mode, int lo) { return lo ? 3 : 4 / tiles_of(mode); }
+__host__ __device__ constexpr int stages_of(int mode, int lo) { return mode == 4 ? 8 : mode == 2 || lo ? 4 : 3; }
+__host__ __device__ constexpr int ring_bytes(int mode, int lo) { return kGroups * stages_of(mode, lo) * kSlotBytes; }
 __host__ __device__ constexpr int step_keys(int head_size) { return 2048 / head_size; }
-__host__ __device__ constexpr int tile_keys(int head_size) { return kWarps * step_keys(head_size); }
+__host__ __device__ constexpr int tile_keys(int head_size) { return kGroups * step_keys(head_size); }
 
 // Shared memory of a block: the ring, and the queries as the products read them.
 __host__ __device__ constexpr int shared_bytes(int head_size, int mode, int lo) {
-  return ring_bytes(mode) + (mode == kTwoTiles ? 2 : 1) * (lo ? 2 : 1) * (head_size / 16) * 512;
+  return ring_bytes(mode, lo) + tiles_of(mode) * (lo ? 2 : 1) * (head_size / 16) * 512;
 }
 // Tiles' time that beginning an item costs (queries, first loads, joining the
 // warps): counted when the work is divided.
@@ -79,10 +83,19 @@ __device__ __forceinline__ uint32_t shared_of(const void* p) {
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool real) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Barrier of the MODE warps that share a group's keys.
+template <int MODE>
+__device__ __forceinline__ void group_sync(int group) {
+  if (MODE <= 1) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * tiles_of(MODE)) : "memory");
+}
 template <int N>
 __device__ __forceinline__ void wait_groups() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -202,6 +215,7 @@ __device__ __forceinline__ Slot slot_of(const Plan& p, long long b) {
   return s;
 }
 
+template <int MODE>
 __device__ __forceinline__ long long block_scan(long long v, long long* shared, long long* total) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   long long incl = v;
@@ -215,7 +229,7 @@ __device__ __forceinline__ long long block_scan(long long v, long long* shared, 
   __syncthreads();
   long long before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < warps_of(MODE); ++w) {
     if (w == warp) before = all;
     all += shared[w];
   }
@@ -229,14 +243,13 @@ constexpr float kSlack = 8.0f;
 
 // ---- one item ------------------------------------------------------------------
 
-// The sums of one warp: its rows g (and g + 8 of each 16-row tile), columns
-// 2c and 2c + 1 of each value tile, g = lane / 4, c = lane % 4.
+// The sums of one warp: its rows g (and g + 8 of a 16-row tile), columns 2c and
+// 2c + 1 of each value tile, g = lane / 4, c = lane % 4.
 template <int SIZE, int MODE>
 struct Sums {
-  static constexpr int kTiles = MODE == kTwoTiles ? 2 : 1;
   static constexpr int kHalves = MODE == kPacked ? 1 : 2;
-  float o[kTiles][SIZE / 8][4];  // as the products leave them; packed: of the hi and the lo weights
-  float m[kTiles][kHalves], l[kTiles][kHalves];
+  float o[SIZE / 8][4];  // as the products leave them; packed: of the hi and the lo weights
+  float m[kHalves], l[kHalves];
 };
 
 // Eight neighbouring elements of a query row.
@@ -274,7 +287,7 @@ __device__ __forceinline__ void load_queries(const Plan& p, const void* query, i
   constexpr int kLanes = SIZE / 8, kDots = SIZE / 16, kParts = LO ? 2 : 1;
   constexpr int kKeyWords = SIZE / 16 < 4 ? SIZE / 16 : 4;
 #pragma unroll
-  for (int first = 0; first < rows_of(MODE); first += kThreads / kLanes) {
+  for (int first = 0; first < rows_of(MODE); first += threads_of(MODE) / kLanes) {
     const int row = first + static_cast<int>(threadIdx.x) / kLanes, d = static_cast<int>(threadIdx.x) % kLanes * 8;
     const int r = first_row + row, t = r / p.group;
     float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, largest = 0.0f;
@@ -312,43 +325,44 @@ __device__ __forceinline__ void load_queries(const Plan& p, const void* query, i
 }
 
 template <int SIZE, int STORAGE, int MODE, int LO>
-__device__ __forceinline__ void warp_item(const Plan& p, const void* query, const Slot& s, int head, int first_row,
-                                          int tile, int tiles, char* ring, uint4* queries, float* factors,
+__device__ __forceinline__ void warp_item(const Plan& p, const void* query, const Slot& s, int head, int block_row,
+                                          int tile, int tiles, char* shared, float* factors,
                                           Sums<SIZE, MODE>& sums) {
   using S = Sums<SIZE, MODE>;
-  constexpr int kKeys = step_keys(SIZE), kSubs = kKeys / 16;
-  constexpr int kDots = SIZE / 16;                        // 16-element products of a score
+  constexpr int kKeys = step_keys(SIZE), kSubs = kKeys / 16, kStages = stages_of(MODE, LO);
+  constexpr int kDots = SIZE / 16;                          // 16-element products of a score
   constexpr int kKeyWords = SIZE / 16 < 4 ? SIZE / 16 : 4;  // words of one read of a key row
   constexpr int kKeyReads = SIZE / 16 / kKeyWords;
   constexpr int kValueWords = SIZE / 32;
-  constexpr int kParts = LO ? 2 : 1, kStages = stages_of(MODE);
+  constexpr int kParts = LO ? 2 : 1;
   const cb_paged_cache& c = p.a.cache;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
+  const int group = warp % kGroups, rank = warp / kGroups;  // of keys; among the warps that share them
+  const int first_row = block_row + 16 * rank;
+  char* ring = shared + group * kStages * kSlotBytes;
+  uint4* queries = reinterpret_cast<uint4*>(shared + ring_bytes(MODE, LO));
 
-  // limits: row r sees keys below limit[r]; all rows of the block see those below `common`
-  int limit[S::kTiles][S::kHalves];
+  // limits: row r sees keys below limit[r]; all rows of the warp see those below `common`
+  int limit[S::kHalves];
 #pragma unroll
-  for (int mt = 0; mt < S::kTiles; ++mt) {
-#pragma unroll
-    for (int half = 0; half < S::kHalves; ++half) {
-      const int r = first_row + mt * 16 + half * 8 + g, t = r / p.group;
-      limit[mt][half] = r < p.rows && t < s.row.count ? s.row.length - s.row.count + t + 1 : 0;
-      sums.m[mt][half] = -INFINITY;
-      sums.l[mt][half] = 0.0f;
-    }
-#pragma unroll
-    for (int j = 0; j < SIZE / 8; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sums.o[mt][j][i] = 0.0f;
+  for (int half = 0; half < S::kHalves; ++half) {
+    const int r = first_row + half * 8 + g, t = r / p.group;
+    limit[half] = r < p.rows && t < s.row.count ? s.row.length - s.row.count + t + 1 : 0;
+    sums.m[half] = -INFINITY;
+    sums.l[half] = 0.0f;
   }
+#pragma unroll
+  for (int j = 0; j < SIZE / 8; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sums.o[j][i] = 0.0f;
   int last = 0;  // exponent of the value scale before
   const int common = s.row.length - s.row.count + first_row / p.group + 1;
-  const int length = s.row.count > 0 ? s.row.length : 0;
+  const int length = s.row.length;
 
-  // page ids: lane i of a batch holds that of the warp's 16-key piece 32 * batch + i
+  // page ids: lane i of a batch holds that of the group's 16-key piece 32 * batch + i
   const int shift = 31 - __clz(c.page);
   auto piece_key = [&](int piece) {
-    return (tile + piece / kSubs) * tile_keys(SIZE) + warp * kKeys + (piece % kSubs) * 16;
+    return (tile + piece / kSubs) * tile_keys(SIZE) + group * kKeys + (piece % kSubs) * 16;
   };
   auto ids_of = [&](int batch) {
     const int piece = batch * 32 + lane, key = piece_key(piece);
@@ -362,83 +376,102 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
   };
   int ids = ids_of(0), ids_next = ids_of(1), batch = 0;
 
+  // A step is eight copies of 32 x 16 bytes, four of K and four of V: a warp
+  // alone does all, one of two K or V, one of four half of those.
+  constexpr int kPools = tiles_of(MODE) == 1 ? 2 : 1, kCopies = 4 / (MODE == 4 ? 2 : 1), kRowCopies = SIZE / 32;
+  const int first_copy = MODE == 4 ? (rank >> 1) * 2 : 0;
+  const bool second = kPools == 1 && (rank & 1);  // copies V, not K
+  const uint32_t page_bytes = static_cast<uint32_t>(c.kv_heads) * c.page * SIZE;
+  const long long head_at = static_cast<long long>(head) * c.page * SIZE + lane * 16;
+  const char* k_pool = static_cast<const char*>(second ? c.v_pages : c.k_pages) + head_at;
+  const char* v_pool = static_cast<const char*>(c.v_pages) + head_at;
+  const float* scale_of = (second || (kPools == 2 && (lane & 1)) ? c.v_scale : c.k_scale) + head;
+  const uint32_t scale_to = kStepBytes + (second || (kPools == 2 && (lane & 1)) ? 16 : 0);
+  // the step's rows in 16-byte pieces, 32 a copy: the copies of one warp are
+  // 512 bytes apart, and odd ones of 128-byte rows are turned by half a line
+  const uint32_t to = swizzled<SIZE>(lane / (SIZE / 16), lane % (SIZE / 16)) + (second ? 2048 : 0);
   const uint32_t ring_at = shared_of(ring);
+  uint32_t fill = ring_at;  // slot that is filled next
   auto prefetch = [&](int step) {
     if (step < tiles) {
-      const uint32_t slot = ring_at + (step % kStages) * kSlotBytes;
       if (step * kSubs / 32 > batch) {
         ids = ids_next;
         ids_next = ids_of(++batch + 1);
       }
 #pragma unroll
-      for (int sub = 0; sub < kSubs; ++sub) {
-        const int piece = step * kSubs + sub, key = piece_key(piece);
+      for (int i = 0; i < kCopies; i += kRowCopies < kCopies ? kRowCopies : kCopies) {
+        const int sub = (first_copy + i) / kRowCopies, piece = step * kSubs + sub, key = piece_key(piece);
         const int page = __shfl_sync(0xffffffffu, ids, piece & 31);
-        const bool held = page >= 0;
-        const long long block = static_cast<long long>(held ? page : 0) * c.kv_heads + head;
-        const long long base = (block * c.page + (key & (c.page - 1))) * SIZE;
-        constexpr int kCopies = SIZE / 32;  // 16 rows of SIZE bytes by 32 lanes
-        const char* k = static_cast<const char*>(c.k_pages) + base + lane * 16;
-        const char* v = static_cast<const char*>(c.v_pages) + base + lane * 16;
-        const int rows = held ? length - key : 0;  // that exist
+        const int rows = page >= 0 ? length - key : 0;  // that exist
+        const long long from = static_cast<long long>(max(page, 0)) * page_bytes + (key & (c.page - 1)) * SIZE +
+                               (first_copy + i) % kRowCopies * 512;
+        const char *k = k_pool + from, *v = v_pool + from;
 #pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
-          const int row = (i * 32 + lane) / (SIZE / 16), part = lane % (SIZE / 16);
-          const uint32_t dst = slot + swizzled<SIZE>(sub * 16 + row, part);
-          copy16(dst, k + i * 512, row < rows);
-          copy16(dst + 2048, v + i * 512, row < rows);
+        for (int n = 0; n < kRowCopies && n < kCopies; ++n) {
+          const int at = first_copy + i + n;
+          const uint32_t dst = fill + ((SIZE == 128 && (n & 1) ? to ^ 64 : to) + at * 512);
+          if (rows >= 16) {
+            copy16(dst, k + n * 512);
+            if (kPools == 2) copy16(dst + 2048, v + n * 512);
+          } else {
+            const bool real = (at % kRowCopies * 512 + lane * 16) / SIZE < rows;
+            copy16(dst, k + n * 512, real);
+            if (kPools == 2) copy16(dst + 2048, v + n * 512, real);
+          }
         }
-        if (lane < 2) copy4(slot + kStepBytes + lane * 16 + sub * 4, (lane ? c.v_scale : c.k_scale) + block, held);
+        if (lane < kPools && (first_copy + i) % kRowCopies == 0)
+          copy4(fill + scale_to + sub * 4, scale_of + static_cast<long long>(max(page, 0)) * c.kv_heads, page >= 0);
       }
     }
     commit();
+    fill = fill + kSlotBytes == ring_at + kStages * kSlotBytes ? ring_at : fill + kSlotBytes;
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) prefetch(i);
 
-  load_queries<SIZE, MODE, LO>(p, query, s.row.count, head, first_row, queries, factors);
+  load_queries<SIZE, MODE, LO>(p, query, s.row.count, head, block_row, queries, factors);
   __syncthreads();
-  float factor[S::kTiles][S::kHalves];
+  float factor[S::kHalves];
 #pragma unroll
-  for (int mt = 0; mt < S::kTiles; ++mt)
-#pragma unroll
-    for (int half = 0; half < S::kHalves; ++half) factor[mt][half] = factors[mt * 16 + half * 8 + g];
+  for (int half = 0; half < S::kHalves; ++half) factor[half] = factors[16 * rank + half * 8 + g];
+  queries += rank * kParts * kDots * 32 + lane;
+  // where this lane reads: rows 8 n + key_of(g) of K, quad + 4 i of V.  The
+  // second half of a 128-byte key row, and every other row of V, lie half a line
+  // turned; the rest are constant distances.
+  const int key_at = swizzled<SIZE>(key_of(g), quad * kKeyWords / 4) + quad * kKeyWords * 4 % 16;
+  const int value_at = 2048 + swizzled<SIZE>(quad, element_of<SIZE>(g) / 16) + element_of<SIZE>(g) % 16;
+  const char* slot = ring;
   for (int step = 0; step < tiles; ++step) {
     wait_groups<kStages - 2>();
-    __syncwarp();  // every lane's copies of this step have landed; every lane has left the slot filled next
+    group_sync<MODE>(group);  // all copies of this step have landed; all warps have left the slot filled next
     prefetch(step + kStages - 1);
-    const char* slot = ring + (step % kStages) * kSlotBytes;
-    const int key = (tile + step) * tile_keys(SIZE) + warp * kKeys;
+    if (step > 0) slot = slot + kSlotBytes == ring + kStages * kSlotBytes ? ring : slot + kSlotBytes;
+    if (tiles_of(MODE) > 1 && first_row >= p.rows) continue;  // no such rows
+    const int key = (tile + step) * tile_keys(SIZE) + group * kKeys;
     const float* scales = reinterpret_cast<const float*>(slot + kStepBytes);
 
-    float score[S::kTiles][2 * kSubs][4];
+    float score[2 * kSubs][4];
 #pragma unroll
     for (int r = 0; r < kKeyReads; ++r) {
       uint32_t w[2 * kSubs][kKeyWords];
-      const int element = r * 64 + quad * (4 * kKeyWords);
+      const char* row = slot + (key_at ^ (r * 64));
 #pragma unroll
-      for (int n = 0; n < 2 * kSubs; ++n)
-        read_words<kKeyWords>(slot + swizzled<SIZE>(n * 8 + key_of(g), element / 16) + element % 16, w[n]);
+      for (int n = 0; n < 2 * kSubs; ++n) read_words<kKeyWords>(row + n * 8 * SIZE, w[n]);
 #pragma unroll
       for (int k = 0; k < kKeyWords; ++k) {
         const int dot = r * kKeyWords + k;
-        uint4 a[S::kTiles][kParts];
+        uint4 a[kParts];
 #pragma unroll
-        for (int mt = 0; mt < S::kTiles; ++mt)
-#pragma unroll
-          for (int part = 0; part < kParts; ++part) a[mt][part] = queries[((mt * kParts + part) * kDots + dot) * 32 + lane];
+        for (int part = 0; part < kParts; ++part) a[part] = queries[(part * kDots + dot) * 32];
 #pragma unroll
         for (int n = 0; n < 2 * kSubs; ++n) {
           uint32_t b0, b1;
           to_halves<STORAGE>(w[n][k], b0, b1);
 #pragma unroll
-          for (int mt = 0; mt < S::kTiles; ++mt) {
-#pragma unroll
-            for (int part = 0; part < kParts; ++part) {
-              const uint32_t row[4] = {a[mt][part].x, a[mt][part].y, a[mt][part].z, a[mt][part].w};
-              if (dot == 0 && part == 0) mma<true>(score[mt][n], row, b0, b1);
-              else mma<false>(score[mt][n], row, b0, b1);
-            }
+          for (int part = 0; part < kParts; ++part) {
+            const uint32_t row[4] = {a[part].x, a[part].y, a[part].z, a[part].w};
+            if (dot == 0 && part == 0) mma<true>(score[n], row, b0, b1);
+            else mma<false>(score[n], row, b0, b1);
           }
         }
       }
@@ -457,82 +490,66 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
       exponent[sub] = static_cast<float>(last);
       undo[sub] = __uint_as_float(static_cast<uint32_t>(127 - last) << 23);
     }
-    uint32_t weight[S::kTiles][kParts][kSubs][4];
+    uint32_t weight[kParts][kSubs][4];
 #pragma unroll
-    for (int mt = 0; mt < S::kTiles; ++mt) {
+    for (int half = 0; half < S::kHalves; ++half) {
+      float x[2 * kSubs][2], most = -INFINITY;
 #pragma unroll
-      for (int half = 0; half < S::kHalves; ++half) {
-        if (MODE == kTwoTiles && first_row + mt * 16 + half * 8 >= p.rows) {  // no such rows
+      for (int n = 0; n < 2 * kSubs; ++n) {
+        const float f = factor[half] * scales[n / 2];
 #pragma unroll
-          for (int n = 0; n < 2 * kSubs; ++n) weight[mt][0][n / 2][2 * (n & 1) + half] = 0u;
-          continue;
+        for (int i = 0; i < 2; ++i) {
+          const float v = MODE == kPacked ? score[n][i] + score[n][2 + i] : score[n][2 * half + i];
+          x[n][i] = fmaf(v, f, exponent[n / 2]);
         }
-        float x[2 * kSubs][2], most = -INFINITY;
+      }
+      if (key + kKeys > common) {  // (the same for the warp) columns 2 quad and 2 quad + 1
 #pragma unroll
-        for (int n = 0; n < 2 * kSubs; ++n) {
-          const float f = factor[mt][half] * scales[n / 2];
+        for (int n = 0; n < 2 * kSubs; ++n)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float v = MODE == kPacked ? score[mt][n][i] + score[mt][n][2 + i] : score[mt][n][2 * half + i];
-            x[n][i] = fmaf(v, f, exponent[n / 2]);
-          }
-        }
-        if (key + kKeys > common) {  // (the same for the warp) columns 2 quad and 2 quad + 1
+          for (int i = 0; i < 2; ++i)
+            if (key + n * 8 + quad + 4 * i >= limit[half]) x[n][i] = -INFINITY;
+      }
 #pragma unroll
-          for (int n = 0; n < 2 * kSubs; ++n)
+      for (int n = 0; n < 2 * kSubs; ++n) most = fmaxf(most, fmaxf(x[n][0], x[n][1]));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      // The sums are kept against a maximum that follows the running one only
+      // when that is 2^kSlack above it, so they are rarely scaled.
+      const float old = sums.m[half];
+      if (__any_sync(0xffffffffu, most > old + kSlack)) {
+        const float now = most > old + kSlack ? most : old;
+        const float r = now == -INFINITY ? 1.0f : root2_of(old - now);
+        sums.m[half] = now;
+        sums.l[half] *= r * r;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (key + n * 8 + quad + 4 * i >= limit[mt][half]) x[n][i] = -INFINITY;
-        }
+        for (int j = 0; j < SIZE / 8; ++j)
 #pragma unroll
-        for (int n = 0; n < 2 * kSubs; ++n) most = fmaxf(most, fmaxf(x[n][0], x[n][1]));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        // The sums are kept against a maximum that follows the running one only
-        // when that is 2^kSlack above it, so they are rarely scaled.
-        const float old = sums.m[mt][half];
-        if (__any_sync(0xffffffffu, most > old + kSlack)) {
-          const float now = most > old + kSlack ? most : old;
-          const float r = now == -INFINITY ? 1.0f : root2_of(old - now);
-          sums.m[mt][half] = now;
-          sums.l[mt][half] *= r * r;
+          for (int i = 0; i < 4; ++i)
+            if (MODE == kPacked || i / 2 == half) sums.o[j][i] = sums.o[j][i] * r * r;
+      }
+      const float against = sums.m[half] == -INFINITY ? 0.0f : sums.m[half];
 #pragma unroll
-          for (int j = 0; j < SIZE / 8; ++j) {
-            float* o = sums.o[mt][j];
-            if (MODE == kPacked) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) o[i] = o[i] * r * r;
-            } else {
-              o[2 * half] = o[2 * half] * r * r;
-              o[2 * half + 1] = o[2 * half + 1] * r * r;
-            }
-          }
-        }
-        const float against = sums.m[mt][half] == -INFINITY ? 0.0f : sums.m[mt][half];
-#pragma unroll
-        for (int n = 0; n < 2 * kSubs; ++n) {
-          const float e0 = exp2_of(x[n][0] - against), e1 = exp2_of(x[n][1] - against);
-          sums.l[mt][half] = fmaf(e0 + e1, undo[n / 2], sums.l[mt][half]);
-          uint32_t hi, lo;
-          split(e0 * fraction[n / 2], e1 * fraction[n / 2], hi, lo);
-          if (MODE == kPacked) {
-            weight[mt][0][n / 2][2 * (n & 1)] = hi;
-            weight[mt][0][n / 2][2 * (n & 1) + 1] = lo;
-          } else {
-            weight[mt][0][n / 2][2 * (n & 1) + half] = hi;
-            if (LO) weight[mt][kParts - 1][n / 2][2 * (n & 1) + half] = lo;
-          }
+      for (int n = 0; n < 2 * kSubs; ++n) {
+        const float e0 = exp2_of(x[n][0] - against), e1 = exp2_of(x[n][1] - against);
+        sums.l[half] = fmaf(e0 + e1, undo[n / 2], sums.l[half]);
+        uint32_t hi, lo;
+        split(e0 * fraction[n / 2], e1 * fraction[n / 2], hi, lo);
+        if (MODE == kPacked) {
+          weight[0][n / 2][2 * (n & 1)] = hi;
+          weight[0][n / 2][2 * (n & 1) + 1] = lo;
+        } else {
+          weight[0][n / 2][2 * (n & 1) + half] = hi;
+          if (LO) weight[kParts - 1][n / 2][2 * (n & 1) + half] = lo;
         }
       }
     }
 #pragma unroll
     for (int sub = 0; sub < kSubs; ++sub) {
       uint32_t v[4][kValueWords];
-      const int element = element_of<SIZE>(g);
 #pragma unroll
       for (int i = 0; i < 4; ++i)  // keys of columns 2 quad, 2 quad + 1 of both 8-key tiles
-        read_words<kValueWords>(slot + 2048 + swizzled<SIZE>(sub * 16 + quad + 4 * i, element / 16) + element % 16,
-                                v[i]);
+        read_words<kValueWords>(slot + (i & 1 ? value_at ^ 64 : value_at) + (sub * 16 + 4 * i) * SIZE, v[i]);
 #pragma unroll
       for (int w = 0; w < kValueWords; ++w) {
         uint32_t b[4][2];  // of the word's four elements: keys 0-7, keys 8-15
@@ -544,22 +561,17 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int mt = 0; mt < S::kTiles; ++mt)
-#pragma unroll
-            for (int part = 0; part < kParts; ++part)
-              mma<false>(sums.o[mt][w * 4 + i], weight[mt][part][sub], b[i][0], b[i][1]);
+          for (int part = 0; part < kParts; ++part) mma<false>(sums.o[w * 4 + i], weight[part][sub], b[i][0], b[i][1]);
       }
     }
   }
   wait_groups<0>();
 #pragma unroll
-  for (int mt = 0; mt < S::kTiles; ++mt)
-#pragma unroll
-    for (int half = 0; half < S::kHalves; ++half) {
-      float& l = sums.l[mt][half];
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-    }
+  for (int half = 0; half < S::kHalves; ++half) {
+    float& l = sums.l[half];
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+  }
 }
 
 // Where row r of an item goes; r past the item's rows: nowhere.
@@ -592,7 +604,7 @@ template <int SIZE, int MODE>
 __device__ __forceinline__ void join(const Plan& p, long long b, int head, int first_row, int count, int parts,
                                      const float* first, const float* rest) {
   constexpr int kRows = rows_of(MODE), kFloats = partial_floats<SIZE, MODE>();
-  for (int i = threadIdx.x; i < kRows * SIZE / 4; i += kThreads) {
+  for (int i = threadIdx.x; i < kRows * SIZE / 4; i += threads_of(MODE)) {
     const int r = i / (SIZE / 4), d = i % (SIZE / 4) * 4, row = first_row + r;
     if (row >= p.rows) continue;
     float top = -INFINITY, sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -615,16 +627,16 @@ __device__ __forceinline__ void join(const Plan& p, long long b, int head, int f
 }
 
 template <int SIZE, int STORAGE, int MODE, int LO>
-__global__ void __launch_bounds__(kThreads, resident_of(MODE)) attention_kernel(const __grid_constant__ Plan p) {
+__global__ void __launch_bounds__(threads_of(MODE), resident_of(MODE, LO)) attention_kernel(const __grid_constant__ Plan p) {
   using S = Sums<SIZE, MODE>;
-  constexpr int kRows = rows_of(MODE);
+  constexpr int kRows = rows_of(MODE), kThreads = threads_of(MODE);
   extern __shared__ __align__(128) char shared[];
-  __shared__ long long scan[kWarps];
-  __shared__ float most[kWarps][kRows], total[kWarps][kRows], factors[kRows];
+  __shared__ long long scan[warps_of(MODE)];
+  __shared__ float most[kGroups][kRows], total[kGroups][kRows], factors[kRows];
   __shared__ long long found[2];
   const long long batch = p.a.batch;
   const int items = p.a.cache.kv_heads * p.blocks;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = warp % kGroups, rank = warp / kGroups;
 
   // the tiles of all slots, and this block's range of them
   long long mine = 0, all;
@@ -634,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, resident_of(MODE)) attention_kernel(
     if (b < kThreads) span_first = span;
     mine += span;
   }
-  block_scan(mine, scan, &all);
+  block_scan<MODE>(mine, scan, &all);
   all *= items;
   const long long per = (all + gridDim.x - 1) / gridDim.x;
   long long at = per * blockIdx.x;
@@ -646,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, resident_of(MODE)) attention_kernel(
     const int span = first == 0 ? span_first : b < batch ? slot_of<SIZE>(p, b).tiles + kItemCost : 0;
     const long long tiles = static_cast<long long>(span) * items;
     long long sum;
-    const long long lower = before + block_scan(tiles, scan, &sum);
+    const long long lower = before + block_scan<MODE>(tiles, scan, &sum);
     if (lower <= at && at < lower + tiles) {
       found[0] = b;
       found[1] = lower;
@@ -683,34 +695,30 @@ __global__ void __launch_bounds__(kThreads, resident_of(MODE)) attention_kernel(
     }
     Sums<SIZE, MODE> sums;
     const void* query = static_cast<const char*>(p.a.q) + b * p.a.q_strides[0] * (p.a.dtype == CB_F32 ? 4 : 2);
-    warp_item<SIZE, STORAGE, MODE, LO>(p, query, s, head, first_row, tile, tiles,
-                                       shared + warp * stages_of(MODE) * kSlotBytes,
-                                       reinterpret_cast<uint4*>(shared + ring_bytes(MODE)), factors, sums);
+    warp_item<SIZE, STORAGE, MODE, LO>(p, query, s, head, first_row, tile, tiles, shared, factors, sums);
 
-    // join the warps
+    // join the groups
     __syncthreads();  // every warp is done with the ring
-    float* rows = reinterpret_cast<float*>(shared);  // (warps, kRows, SIZE)
+    float* rows = reinterpret_cast<float*>(shared);  // (groups, kRows, SIZE)
 #pragma unroll
-    for (int mt = 0; mt < S::kTiles; ++mt)
-#pragma unroll
-      for (int half = 0; half < S::kHalves; ++half) {
-        const int r = mt * 16 + half * 8 + (lane >> 2);
-        if ((lane & 3) == 0) {
-          most[warp][r] = sums.m[mt][half];
-          total[warp][r] = sums.l[mt][half];
-        }
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          float* to = rows + (warp * kRows + r) * SIZE + element_of<SIZE>(2 * (lane & 3) + n);
-          auto value = [&](int j) {
-            const float* o = sums.o[mt][j];
-            return MODE == kPacked ? o[n] + o[2 + n] : o[2 * half + n];
-          };
-#pragma unroll
-          for (int j = 0; j < SIZE / 8; j += 4)
-            *reinterpret_cast<float4*>(to + j) = make_float4(value(j), value(j + 1), value(j + 2), value(j + 3));
-        }
+    for (int half = 0; half < S::kHalves; ++half) {
+      const int r = rank * 16 + half * 8 + (lane >> 2);
+      if ((lane & 3) == 0) {
+        most[group][r] = sums.m[half];
+        total[group][r] = sums.l[half];
       }
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        float* to = rows + (group * kRows + r) * SIZE + element_of<SIZE>(2 * (lane & 3) + n);
+        auto value = [&](int j) {
+          const float* o = sums.o[j];
+          return MODE == kPacked ? o[n] + o[2 + n] : o[2 * half + n];
+        };
+#pragma unroll
+        for (int j = 0; j < SIZE / 8; j += 4)
+          *reinterpret_cast<float4*>(to + j) = make_float4(value(j), value(j + 1), value(j + 2), value(j + 3));
+      }
+    }
     __syncthreads();
     const bool whole = tile == 0 && tiles == s.tiles;
     const bool begins = item_at + kItemCost <= range;  // the item of the range's first tile: the first partial result
@@ -719,9 +727,9 @@ __global__ void __launch_bounds__(kThreads, resident_of(MODE)) attention_kernel(
       const int r = i / (SIZE / 4), d = i % (SIZE / 4) * 4;
       float top = -INFINITY, sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, most[w][r]);
+      for (int w = 0; w < kGroups; ++w) top = fmaxf(top, most[w][r]);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
+      for (int w = 0; w < kGroups; ++w) {
         const float f = most[w][r] == -INFINITY ? 0.0f : root2_of(most[w][r] - top);
         const float4 x = *reinterpret_cast<const float4*>(rows + (w * kRows + r) * SIZE + d);
         sum += f * total[w][r] * f;
@@ -787,25 +795,27 @@ int resident_blocks() {
     auto kernel = attention_kernel<SIZE, STORAGE, MODE, LO>;
     constexpr int kShared = shared_bytes(SIZE, MODE, LO);
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, kShared) != cudaSuccess)
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads_of(MODE), kShared) != cudaSuccess)
       per_sm = 0;
     device = per_sm > 0 ? now : -1;
   }
   return per_sm;
 }
 
-// Calls f with the template arguments of a launch: more rows than a packed tile
-// holds take 16- or 32-row tiles, float32 ones with their low parts.
+// Calls f with the template arguments of a launch: by the rows of a kv head 8
+// in one tile, or one, two or four 16-row tiles; float32 queries with their
+// low parts, in single tiles.
 template <typename F>
 long long with_variant(const cb_paged_attention_args& a, F f) {
   const long long rows = a.tokens * (a.heads / a.cache.kv_heads);
   auto by_rows = [&](auto size, auto storage) {
-    using Z = std::integral_constant<int, 0>;
-    using One = std::integral_constant<int, 1>;
-    using Two = std::integral_constant<int, kTwoTiles>;
-    if (rows <= 8) return f(size, storage, Z{}, Z{});
-    if (a.dtype == CB_F32) return f(size, storage, One{}, One{});
-    return rows <= 16 ? f(size, storage, One{}, Z{}) : f(size, storage, Two{}, Z{});
+    const auto zero = std::integral_constant<int, 0>{};
+    const auto one = std::integral_constant<int, 1>{};
+    if (rows <= 8) return f(size, storage, zero, zero);
+    if (a.dtype == CB_F32) return f(size, storage, one, one);
+    if (rows <= 16) return f(size, storage, one, zero);
+    if (rows <= 32) return f(size, storage, std::integral_constant<int, 2>{}, zero);
+    return f(size, storage, std::integral_constant<int, 4>{}, zero);
   };
   auto by_storage = [&](auto size) {
     return a.cache.storage == CB_I8 ? by_rows(size, std::integral_constant<int, CB_I8>{})
@@ -870,7 +880,7 @@ int cb_paged_attention(const cb_paged_attention_args* args, void* scratch, unsig
     for (int i = 0; i < 3; ++i) p.wide = p.wide && a.q_strides[i] * item % 16 == 0;
     p.partial = static_cast<float*>(scratch);
     p.arrived = counters;
-    launch(attention_kernel<SIZE, STORAGE, MODE, LO>, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
+    launch(attention_kernel<SIZE, STORAGE, MODE, LO>, dim3(static_cast<unsigned>(grid)), dim3(threads_of(MODE)),
            shared_bytes(SIZE, MODE, LO), static_cast<cudaStream_t>(stream), false, p);
     return check_launch("cb_paged_attention");
   }));
