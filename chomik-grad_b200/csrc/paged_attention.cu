@@ -50,6 +50,7 @@ constexpr int kGroups = 4;                       // of keys, in a tile
 constexpr int kStepBytes = 4096;                 // K and V of a group's step
 constexpr int kHeadBytes = 64;                   // its scales: 4 of K, 4 of V
 constexpr int kSlotBytes = kStepBytes + kHeadBytes;
+constexpr int kHalfBytes = 8192;                 // K and V of a step as fp16, where warps share them
 
 // How the query rows fill the tensor core's 16-row tiles: 8 of them with both
 // parts in one tile, or MODE tiles, each with warps of its own.
@@ -64,12 +65,15 @@ __host__ __device__ constexpr int threads_of(int mode) { return 32 * warps_of(mo
 __host__ __device__ constexpr int resident_of(int mode, int lo) { return lo ? 3 : 4 / tiles_of(mode); }
 __host__ __device__ constexpr int stages_of(int mode, int lo) { return mode == 4 ? 8 : mode == 2 || lo ? 4 : 3; }
 __host__ __device__ constexpr int ring_bytes(int mode, int lo) { return kGroups * stages_of(mode, lo) * kSlotBytes; }
+// Warps that share keys convert each of them once, into shared memory.
+__host__ __device__ constexpr bool shares(int mode) { return mode > 1; }
+__host__ __device__ constexpr int half_bytes(int mode) { return shares(mode) ? kGroups * kHalfBytes : 0; }
 __host__ __device__ constexpr int step_keys(int head_size) { return 2048 / head_size; }
 __host__ __device__ constexpr int tile_keys(int head_size) { return kGroups * step_keys(head_size); }
 
 // Shared memory of a block: the ring, and the queries as the products read them.
 __host__ __device__ constexpr int shared_bytes(int head_size, int mode, int lo) {
-  return ring_bytes(mode, lo) + tiles_of(mode) * (lo ? 2 : 1) * (head_size / 16) * 512;
+  return ring_bytes(mode, lo) + half_bytes(mode) + tiles_of(mode) * (lo ? 2 : 1) * (head_size / 16) * 512;
 }
 // Tiles' time that beginning an item costs (queries, first loads, joining the
 // warps): counted when the work is divided.
@@ -137,22 +141,63 @@ __device__ __forceinline__ void read_words(const char* p, uint32_t* w) {
 
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
-// Four codes -> two pairs of halves.  int8: the byte x + 128 under the exponent
-// of 1024 is the number 1152 + x.
+// Four codes -> two pairs of halves: of int8 elements 0, 2 and 1, 3, of e4m3
+// elements 0, 1 and 2, 3.  int8: the byte x + 128 (the sign bit turned) under
+// the exponent of 1024 is the number 1152 + x; one logic instruction makes two.
 template <int STORAGE>
 __device__ __forceinline__ void to_halves(uint32_t w, uint32_t& a, uint32_t& b) {
   if (STORAGE == CB_I8) {
-    w ^= 0x80808080u;
     const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-    const uint32_t lo = __byte_perm(w, 0x64646464u, 0x4140), hi = __byte_perm(w, 0x64646464u, 0x4342);
-    a = bits(__hsub2(*reinterpret_cast<const __half2*>(&lo), bias));
-    b = bits(__hsub2(*reinterpret_cast<const __half2*>(&hi), bias));
+    uint32_t even, odd;
+    asm("lop3.b32 %0, %1, 0x00ff00ff, 0x64806480, 0x6a;" : "=r"(even) : "r"(w));  // (w & mask) ^ bits
+    asm("lop3.b32 %0, %1, 0x00ff00ff, 0x64806480, 0x6a;" : "=r"(odd) : "r"(w >> 8));
+    a = bits(__hsub2(*reinterpret_cast<const __half2*>(&even), bias));
+    b = bits(__hsub2(*reinterpret_cast<const __half2*>(&odd), bias));
   } else {
     asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\t"
         "cvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
         : "=r"(a), "=r"(b)
         : "r"(w));
   }
+}
+// Four codes -> the pairs 0, 1 and 2, 3 whatever the storage.
+template <int STORAGE>
+__device__ __forceinline__ void to_halves_in_order(uint32_t w, uint32_t& a, uint32_t& b) {
+  if (STORAGE == CB_I8) {
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    w ^= 0x80808080u;
+    const uint32_t lo = __byte_perm(w, 0x64646464u, 0x4140), hi = __byte_perm(w, 0x64646464u, 0x4342);
+    a = bits(__hsub2(*reinterpret_cast<const __half2*>(&lo), bias));
+    b = bits(__hsub2(*reinterpret_cast<const __half2*>(&hi), bias));
+  } else {
+    to_halves<STORAGE>(w, a, b);
+  }
+}
+
+// Byte offset of 16-byte piece `piece` of fp16 row `row` (2 SIZE bytes): eight
+// rows of one piece, which a matrix load reads at once, lie in different banks.
+template <int SIZE>
+__device__ __forceinline__ int half_at(int row, int piece) {
+  const int at = row * (SIZE / 8) + piece, line = at >> 3;
+  const int turn = SIZE == 128 ? (line >> 1) & 7 : SIZE == 64 ? line & 7 : line & 3;
+  return (line << 7) + (((at & 7) ^ turn) << 4);
+}
+// Four 8x8 matrices of halves; lane l gives the address of row l % 8 of matrix l / 8.
+template <bool TURNED>
+__device__ __forceinline__ void load_matrices(uint32_t at, uint32_t* r) {
+  if (TURNED)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+
+// The words whose pairs are elements 2 i and 2 i + 1 of two rows, i = 0, 1.
+template <int STORAGE>
+__device__ __forceinline__ uint32_t interleave(uint32_t a, uint32_t b, int i) {
+  if (STORAGE == CB_I8) return __byte_perm(a, b, i ? 0x7632 : 0x5410);
+  return __byte_perm(a, b, i ? 0x7362 : 0x5140);
 }
 
 __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
@@ -281,7 +326,7 @@ __device__ __forceinline__ void load_query(const Plan& p, const void* query, lon
 // operands of each 16-element product, `factors` what turns a row's products
 // into scores in base 2.  SIZE / 8 neighbouring threads take a row; rows that
 // do not exist are zero.
-template <int SIZE, int MODE, int LO>
+template <int SIZE, int STORAGE, int MODE, int LO>
 __device__ __forceinline__ void load_queries(const Plan& p, const void* query, int count, int head, int first_row,
                                              uint4* queries, float* factors) {
   constexpr int kLanes = SIZE / 8, kDots = SIZE / 16, kParts = LO ? 2 : 1;
@@ -311,8 +356,15 @@ __device__ __forceinline__ void load_queries(const Plan& p, const void* query, i
 #pragma unroll
       for (int pair = 0; pair < 2; ++pair) {
         uint32_t hi, lo;
-        split(x[4 * word + 2 * pair] * down, x[4 * word + 2 * pair + 1] * down, hi, lo);
-        if (MODE == kPacked) {
+        const int first = 4 * word + (STORAGE == CB_I8 && !shares(MODE) ? pair : 2 * pair);
+        const int next = STORAGE == CB_I8 && !shares(MODE) ? 2 : 1;
+        split(x[first] * down, x[first + next] * down, hi, lo);  // in the pairs of to_halves
+        if (shares(MODE)) {  // elements 16 dot + 2 column + {0, 1}, and 8 further
+          const int pair_at = at + 2 * pair;
+          uint32_t* turned = reinterpret_cast<uint32_t*>(queries + (row / 16 * kDots + pair_at / 16) * 32 +
+                                                         row % 8 * 4 + pair_at % 8 / 2);
+          turned[2 * (pair_at / 8 % 2) + row / 8 % 2] = hi;
+        } else if (MODE == kPacked) {
           to[2 * pair] = hi;
           to[2 * pair + 1] = lo;
         } else {
@@ -340,7 +392,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
   const int group = warp % kGroups, rank = warp / kGroups;  // of keys; among the warps that share them
   const int first_row = block_row + 16 * rank;
   char* ring = shared + group * kStages * kSlotBytes;
-  uint4* queries = reinterpret_cast<uint4*>(shared + ring_bytes(MODE, LO));
+  uint4* queries = reinterpret_cast<uint4*>(shared + ring_bytes(MODE, LO) + half_bytes(MODE));
 
   // limits: row r sees keys below limit[r]; all rows of the warp see those below `common`
   int limit[S::kHalves];
@@ -389,7 +441,9 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
   const uint32_t scale_to = kStepBytes + (second || (kPools == 2 && (lane & 1)) ? 16 : 0);
   // the step's rows in 16-byte pieces, 32 a copy: the copies of one warp are
   // 512 bytes apart, and odd ones of 128-byte rows are turned by half a line
-  const uint32_t to = swizzled<SIZE>(lane / (SIZE / 16), lane % (SIZE / 16)) + (second ? 2048 : 0);
+  // (warps that share keys: a lane converts what it copied, in any place)
+  const uint32_t to = (shares(MODE) ? lane * 16 : swizzled<SIZE>(lane / (SIZE / 16), lane % (SIZE / 16))) +
+                      (second ? 2048 : 0);
   const uint32_t ring_at = shared_of(ring);
   uint32_t fill = ring_at;  // slot that is filled next
   auto prefetch = [&](int step) {
@@ -409,7 +463,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
 #pragma unroll
         for (int n = 0; n < kRowCopies && n < kCopies; ++n) {
           const int at = first_copy + i + n;
-          const uint32_t dst = fill + ((SIZE == 128 && (n & 1) ? to ^ 64 : to) + at * 512);
+          const uint32_t dst = fill + ((SIZE == 128 && !shares(MODE) && (n & 1) ? to ^ 64 : to) + at * 512);
           if (rows >= 16) {
             copy16(dst, k + n * 512);
             if (kPools == 2) copy16(dst + 2048, v + n * 512);
@@ -429,7 +483,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) prefetch(i);
 
-  load_queries<SIZE, MODE, LO>(p, query, s.row.count, head, block_row, queries, factors);
+  load_queries<SIZE, STORAGE, MODE, LO>(p, query, s.row.count, head, block_row, queries, factors);
   __syncthreads();
   float factor[S::kHalves];
 #pragma unroll
@@ -441,16 +495,59 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
   const int key_at = swizzled<SIZE>(key_of(g), quad * kKeyWords / 4) + quad * kKeyWords * 4 % 16;
   const int value_at = 2048 + swizzled<SIZE>(quad, element_of<SIZE>(g) / 16) + element_of<SIZE>(g) % 16;
   const char* slot = ring;
+  // the group's fp16 rows, and this lane's addresses in them for matrix loads: K
+  // rows of both 8-key tiles, 16 elements; V rows of 16 keys, two 8-element tiles
+  char* halves = shared + ring_bytes(MODE, LO) + group * kHalfBytes;
+  const uint32_t halves_at = shared_of(halves);
   for (int step = 0; step < tiles; ++step) {
     wait_groups<kStages - 2>();
-    group_sync<MODE>(group);  // all copies of this step have landed; all warps have left the slot filled next
-    prefetch(step + kStages - 1);
     if (step > 0) slot = slot + kSlotBytes == ring + kStages * kSlotBytes ? ring : slot + kSlotBytes;
+    if (shares(MODE)) {
+      uint32_t w[kCopies][8];
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        uint32_t raw[4];
+        read_words<4>(slot + to + (first_copy + i) * 512, raw);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) to_halves_in_order<STORAGE>(raw[k], w[i][2 * k], w[i][2 * k + 1]);
+      }
+      group_sync<MODE>(group);  // all warps are done with the step before
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int at = (first_copy + i) * 32 + lane, row = at / (SIZE / 16), piece = at % (SIZE / 16) * 2;
+        const bool odd = SIZE == 128 && piece >= 8;  // (the order keeps eight lanes in different banks)
+        char* base = halves + (second ? kHalfBytes / 2 : 0);
+        const uint4 lo = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]), hi = make_uint4(w[i][4], w[i][5], w[i][6], w[i][7]);
+        *reinterpret_cast<uint4*>(base + half_at<SIZE>(row, piece + (odd ? 1 : 0))) = odd ? hi : lo;
+        *reinterpret_cast<uint4*>(base + half_at<SIZE>(row, piece + (odd ? 0 : 1))) = odd ? lo : hi;
+      }
+    }
+    group_sync<MODE>(group);  // this step is complete; all warps have left the slot filled next
+    prefetch(step + kStages - 1);
     if (tiles_of(MODE) > 1 && first_row >= p.rows) continue;  // no such rows
     const int key = (tile + step) * tile_keys(SIZE) + group * kKeys;
     const float* scales = reinterpret_cast<const float*>(slot + kStepBytes);
 
     float score[2 * kSubs][4];
+    if constexpr (shares(MODE)) {
+#pragma unroll
+      for (int dot = 0; dot < kDots; ++dot) {
+        const uint4 a = queries[dot * 32];
+        const uint32_t row[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int sub = 0; sub < kSubs; ++sub) {
+          uint32_t b[4];  // elements 0-7 and 8-15 of keys 0-7, then of keys 8-15
+          load_matrices<false>(halves_at + half_at<SIZE>(sub * 16 + (lane & 7) + (lane & 16) / 2, dot * 2 + (lane >> 3 & 1)), b);
+          if (dot == 0) {
+            mma<true>(score[2 * sub], row, b[0], b[1]);
+            mma<true>(score[2 * sub + 1], row, b[2], b[3]);
+          } else {
+            mma<false>(score[2 * sub], row, b[0], b[1]);
+            mma<false>(score[2 * sub + 1], row, b[2], b[3]);
+          }
+        }
+      }
+    } else {
 #pragma unroll
     for (int r = 0; r < kKeyReads; ++r) {
       uint32_t w[2 * kSubs][kKeyWords];
@@ -475,6 +572,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
           }
         }
       }
+    }
     }
 
     // value scales as 2^exponent * fraction; one that is zero takes the exponent
@@ -508,7 +606,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
         for (int n = 0; n < 2 * kSubs; ++n)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            if (key + n * 8 + quad + 4 * i >= limit[half]) x[n][i] = -INFINITY;
+            if (key + n * 8 + (shares(MODE) ? 2 * quad + i : quad + 4 * i) >= limit[half]) x[n][i] = -INFINITY;
       }
 #pragma unroll
       for (int n = 0; n < 2 * kSubs; ++n) most = fmaxf(most, fmaxf(x[n][0], x[n][1]));
@@ -546,22 +644,32 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
     }
 #pragma unroll
     for (int sub = 0; sub < kSubs; ++sub) {
-      uint32_t v[4][kValueWords];
+      if constexpr (shares(MODE)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)  // keys of columns 2 quad, 2 quad + 1 of both 8-key tiles
-        read_words<kValueWords>(slot + (i & 1 ? value_at ^ 64 : value_at) + (sub * 16 + 4 * i) * SIZE, v[i]);
-#pragma unroll
-      for (int w = 0; w < kValueWords; ++w) {
-        uint32_t b[4][2];  // of the word's four elements: keys 0-7, keys 8-15
-#pragma unroll
-        for (int pair = 0; pair < 2; ++pair) {
-          to_halves<STORAGE>(__byte_perm(v[2 * pair][w], v[2 * pair + 1][w], 0x5140), b[0][pair], b[1][pair]);
-          to_halves<STORAGE>(__byte_perm(v[2 * pair][w], v[2 * pair + 1][w], 0x7362), b[2][pair], b[3][pair]);
+        for (int j = 0; j < SIZE / 8; j += 2) {
+          uint32_t b[4];  // keys 0-7 and 8-15 of tile j, then of tile j + 1
+          load_matrices<true>(halves_at + kHalfBytes / 2 + half_at<SIZE>(sub * 16 + (lane & 15), j + (lane >> 4)), b);
+          mma<false>(sums.o[j], weight[0][sub], b[0], b[1]);
+          mma<false>(sums.o[j + 1], weight[0][sub], b[2], b[3]);
         }
+      } else {
+        uint32_t v[4][kValueWords];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)  // keys of columns 2 quad, 2 quad + 1 of both 8-key tiles
+          read_words<kValueWords>(slot + (i & 1 ? value_at ^ 64 : value_at) + (sub * 16 + 4 * i) * SIZE, v[i]);
 #pragma unroll
-          for (int part = 0; part < kParts; ++part) mma<false>(sums.o[w * 4 + i], weight[part][sub], b[i][0], b[i][1]);
+        for (int w = 0; w < kValueWords; ++w) {
+          uint32_t b[4][2];  // of the word's four elements: keys 0-7, keys 8-15
+#pragma unroll
+          for (int pair = 0; pair < 2; ++pair) {
+            to_halves<STORAGE>(interleave<STORAGE>(v[2 * pair][w], v[2 * pair + 1][w], 0), b[0][pair], b[1][pair]);
+            to_halves<STORAGE>(interleave<STORAGE>(v[2 * pair][w], v[2 * pair + 1][w], 1), b[2][pair], b[3][pair]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) mma<false>(sums.o[w * 4 + i], weight[part][sub], b[i][0], b[i][1]);
+        }
       }
     }
   }
@@ -707,16 +815,23 @@ __global__ void __launch_bounds__(threads_of(MODE), resident_of(MODE, LO)) atten
         most[group][r] = sums.m[half];
         total[group][r] = sums.l[half];
       }
+      if constexpr (shares(MODE)) {  // columns 2 c and 2 c + 1 of tile j are those elements
+        float* to = rows + (group * kRows + r) * SIZE + 2 * (lane & 3);
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        float* to = rows + (group * kRows + r) * SIZE + element_of<SIZE>(2 * (lane & 3) + n);
-        auto value = [&](int j) {
-          const float* o = sums.o[j];
-          return MODE == kPacked ? o[n] + o[2 + n] : o[2 * half + n];
-        };
+        for (int j = 0; j < SIZE / 8; ++j)
+          *reinterpret_cast<float2*>(to + 8 * j) = make_float2(sums.o[j][2 * half], sums.o[j][2 * half + 1]);
+      } else {
 #pragma unroll
-        for (int j = 0; j < SIZE / 8; j += 4)
-          *reinterpret_cast<float4*>(to + j) = make_float4(value(j), value(j + 1), value(j + 2), value(j + 3));
+        for (int n = 0; n < 2; ++n) {
+          float* to = rows + (group * kRows + r) * SIZE + element_of<SIZE>(2 * (lane & 3) + n);
+          auto value = [&](int j) {
+            const float* o = sums.o[j];
+            return MODE == kPacked ? o[n] + o[2 + n] : o[2 * half + n];
+          };
+#pragma unroll
+          for (int j = 0; j < SIZE / 8; j += 4)
+            *reinterpret_cast<float4*>(to + j) = make_float4(value(j), value(j + 1), value(j + 2), value(j + 3));
+        }
       }
     }
     __syncthreads();
