@@ -78,6 +78,8 @@ __host__ __device__ constexpr int shared_bytes(int head_size, int mode, int lo) 
 // Tiles' time that beginning an item costs (queries, first loads, joining the
 // warps): counted when the work is divided.
 constexpr int kItemCost = 2;
+// Items of no more than six tiles are not cut: joining parts takes as long.
+constexpr int kSmallItem = kItemCost + 6;
 
 // ---- loads -------------------------------------------------------------------
 
@@ -249,30 +251,34 @@ struct Slot {
   int tiles;
 };
 template <int SIZE>
+__device__ __forceinline__ int tiles_of_slot(const PagedRow& row) {
+  const int keys = row.count > 0 ? row.length : 0;  // (an item without keys writes zeros)
+  return max(1, (keys + tile_keys(SIZE) - 1) / tile_keys(SIZE));
+}
+template <int SIZE>
 __device__ __forceinline__ Slot slot_of(const Plan& p, long long b) {
   Slot s;
   if (!paged_row(p.a.cache, p.a.sequences, p.a.counts, p.a.tokens, b, p.a.error_flag, &s.row)) {
     s.row.length = s.row.count = 0;
     s.row.table = p.a.cache.table;
   }
-  const int keys = s.row.count > 0 ? s.row.length : 0;  // (an item without keys writes zeros)
-  s.tiles = max(1, (keys + tile_keys(SIZE) - 1) / tile_keys(SIZE));
+  s.tiles = tiles_of_slot<SIZE>(s.row);
   return s;
 }
 
 template <int MODE>
-__device__ __forceinline__ long long block_scan(long long v, long long* shared, long long* total) {
+__device__ __forceinline__ int block_scan(int v, int* shared, int* total) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  long long incl = v;
+  int incl = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+    const int up = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += up;
   }
   __syncthreads();
   if (lane == 31) shared[warp] = incl;
   __syncthreads();
-  long long before = 0, all = 0;
+  int before = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < warps_of(MODE); ++w) {
     if (w == warp) before = all;
@@ -709,23 +715,39 @@ __host__ __device__ constexpr int partial_floats() { return rows_of(MODE) * (SIZ
 // An item that a cut divided: its first part, then the first partial results of
 // the following blocks (`rest` + 2 k of them), in that order.
 template <int SIZE, int MODE>
-__device__ __forceinline__ void join(const Plan& p, long long b, int head, int first_row, int count, int parts,
+__device__ __noinline__ void join(const Plan& p, long long b, int head, int first_row, int count, int parts,
                                      const float* first, const float* rest) {
   constexpr int kRows = rows_of(MODE), kFloats = partial_floats<SIZE, MODE>();
   for (int i = threadIdx.x; i < kRows * SIZE / 4; i += threads_of(MODE)) {
     const int r = i / (SIZE / 4), d = i % (SIZE / 4) * 4, row = first_row + r;
     if (row >= p.rows) continue;
     float top = -INFINITY, sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-    for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg((k ? rest + 2LL * k * kFloats : first) + r));
-#pragma unroll 8
-    for (int k = 0; k < parts; ++k) {
-      const float* part = k ? rest + 2LL * k * kFloats : first;
-      const float most = __ldcg(part + r);
-      const float f = most == -INFINITY ? 0.0f : root2_of(most - top);
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(part + 2 * kRows + r * SIZE + d));
-      sum += f * __ldcg(part + kRows + r) * f;
-      v[0] += f * x.x * f; v[1] += f * x.y * f; v[2] += f * x.z * f; v[3] += f * x.w * f;
+    constexpr int kBatch = 8;  // parts whose loads are in flight together
+    for (int from = 0; from < parts; from += kBatch) {
+      float m[kBatch], l[kBatch], now = top;
+      float4 x[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int at = from + k;
+        const float* part = at ? rest + 2LL * at * kFloats : first;
+        m[k] = at < parts ? __ldcg(part + r) : -INFINITY;
+        l[k] = at < parts ? __ldcg(part + kRows + r) : 0.0f;
+        x[k] = at < parts ? __ldcg(reinterpret_cast<const float4*>(part + 2 * kRows + r * SIZE + d))
+                          : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) now = fmaxf(now, m[k]);
+      const float keep = top == -INFINITY ? 0.0f : root2_of(top - now);
+      sum = sum * keep * keep;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = v[i] * keep * keep;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const float f = m[k] == -INFINITY ? 0.0f : root2_of(m[k] - now);
+        sum += f * l[k] * f;
+        v[0] += f * x[k].x * f; v[1] += f * x[k].y * f; v[2] += f * x[k].z * f; v[3] += f * x[k].w * f;
+      }
+      top = now;
     }
     const bool real = row / p.group < count && sum != 0.0f;
 #pragma unroll
@@ -739,57 +761,64 @@ __global__ void __launch_bounds__(threads_of(MODE), resident_of(MODE, LO)) atten
   using S = Sums<SIZE, MODE>;
   constexpr int kRows = rows_of(MODE), kThreads = threads_of(MODE);
   extern __shared__ __align__(128) char shared[];
-  __shared__ long long scan[warps_of(MODE)];
+  __shared__ int scan[warps_of(MODE)], found[5];
   __shared__ float most[kGroups][kRows], total[kGroups][kRows], factors[kRows];
-  __shared__ long long found[2];
-  const long long batch = p.a.batch;
-  const int items = p.a.cache.kv_heads * p.blocks;
+  const int batch = static_cast<int>(p.a.batch), items = p.a.cache.kv_heads * p.blocks;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = warp % kGroups, rank = warp / kGroups;
 
+  pdl_launch_dependents();
+  pdl_wait();
   // the tiles of all slots, and this block's range of them
-  long long mine = 0, all;
-  int span_first = 0;  // of slot threadIdx.x
-  for (long long b = threadIdx.x; b < batch; b += kThreads) {
-    const int span = slot_of<SIZE>(p, b).tiles + kItemCost;
-    if (b < kThreads) span_first = span;
-    mine += span;
+  Slot s;
+  s.tiles = -kItemCost;
+  int mine = 0, all;
+  for (int b = batch - 1 - (batch - 1 - static_cast<int>(threadIdx.x)) % kThreads; b >= 0 && b < batch; b -= kThreads) {
+    s = slot_of<SIZE>(p, b);  // (slot threadIdx.x last)
+    mine += s.tiles + kItemCost;
   }
   block_scan<MODE>(mine, scan, &all);
   all *= items;
-  const long long per = (all + gridDim.x - 1) / gridDim.x;
-  long long at = per * blockIdx.x;
-  const long long end = at + per < all ? at + per : all;
-  if (at >= end) return;
-  long long before = 0;
-  for (long long first = 0; first < batch; first += kThreads) {
-    const long long b = first + threadIdx.x;
-    const int span = first == 0 ? span_first : b < batch ? slot_of<SIZE>(p, b).tiles + kItemCost : 0;
-    const long long tiles = static_cast<long long>(span) * items;
-    long long sum;
-    const long long lower = before + block_scan<MODE>(tiles, scan, &sum);
-    if (lower <= at && at < lower + tiles) {
+  const int per = (all + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+  const int range = per * static_cast<int>(blockIdx.x), end = min(range + per, all);
+  if (range >= end) return;
+  int before = 0;
+  for (int first = 0; first < batch; first += kThreads) {
+    const int b = first + static_cast<int>(threadIdx.x);
+    if (first > 0) {
+      if (b < batch) s = slot_of<SIZE>(p, b);
+      else s.tiles = -kItemCost;
+    }
+    const int units = (s.tiles + kItemCost) * items;
+    int sum;
+    const int lower = before + block_scan<MODE>(units, scan, &sum);
+    if (lower <= range && range < lower + units) {
       found[0] = b;
       found[1] = lower;
+      found[2] = static_cast<int>((s.row.table - p.a.cache.table) / p.a.cache.columns);
+      found[3] = s.row.length;
+      found[4] = s.row.count;
     }
     before += sum;
-    if (before > at) break;
+    if (before > range) break;
   }
   __syncthreads();
-  long long b = found[0], origin = found[1];
-  Slot s = slot_of<SIZE>(p, b);
-  const long long range = at;
+  int b = found[0], origin = found[1], at = range;
+  s.row.table = p.a.cache.table + found[2] * p.a.cache.columns;
+  s.row.length = found[3];
+  s.row.count = found[4];
+  s.tiles = tiles_of_slot<SIZE>(s.row);
 
   while (at < end) {
     int span = s.tiles + kItemCost;
-    if (at - origin >= static_cast<long long>(span) * items) {
-      origin += static_cast<long long>(span) * items;
+    if (at - origin >= span * items) {
+      origin += span * items;
       s = slot_of<SIZE>(p, ++b);
       span = s.tiles + kItemCost;
     }
-    const int item = static_cast<int>((at - origin) / span);
-    const long long item_at = origin + static_cast<long long>(item) * span;  // its cost, then its tiles
-    const int tile = max(0, static_cast<int>(at - item_at) - kItemCost);
-    const int tiles = max(0, static_cast<int>(min(end - item_at, static_cast<long long>(span))) - kItemCost) - tile;
+    const int item = (at - origin) / span, item_at = origin + item * span;  // its cost, then its tiles
+    const bool small = span <= kSmallItem;  // belongs to the block in whose range it begins
+    const int tile = max(0, at - item_at - kItemCost);
+    const int tiles = small ? (at == item_at ? s.tiles : 0) : max(0, min(end - item_at, span) - kItemCost) - tile;
     at = item_at + span;
     if (tiles <= 0) continue;
     const int head = item / p.blocks, first_row = item % p.blocks * kRows;
@@ -802,7 +831,7 @@ __global__ void __launch_bounds__(threads_of(MODE), resident_of(MODE, LO)) atten
       continue;
     }
     Sums<SIZE, MODE> sums;
-    const void* query = static_cast<const char*>(p.a.q) + b * p.a.q_strides[0] * (p.a.dtype == CB_F32 ? 4 : 2);
+    const void* query = static_cast<const char*>(p.a.q) + static_cast<long long>(b) * p.a.q_strides[0] * (p.a.dtype == CB_F32 ? 4 : 2);
     warp_item<SIZE, STORAGE, MODE, LO>(p, query, s, head, first_row, tile, tiles, shared, factors, sums);
 
     // join the groups
@@ -867,7 +896,7 @@ __global__ void __launch_bounds__(threads_of(MODE), resident_of(MODE, LO)) atten
       }
     }
     if (!whole) {
-      const long long from = (item_at + kItemCost) / per, last = (item_at + span - 1) / per;  // blocks of its tiles
+      const int from = (item_at + kItemCost) / per, last = (item_at + span - 1) / per;  // blocks of its tiles
       __syncthreads();
       if (threadIdx.x == 0) {
         const bool all_there = ticket_acq_rel(p.arrived + from) == static_cast<unsigned>(last - from);
@@ -877,9 +906,9 @@ __global__ void __launch_bounds__(threads_of(MODE), resident_of(MODE, LO)) atten
       __syncthreads();
       if (found[0]) {
         const int own = item_at + kItemCost <= from * per ? 0 : 1;  // the first part's place
-        join<SIZE, MODE>(p, b, head, first_row, s.row.count, static_cast<int>(last - from) + 1,
-                         p.partial + (2 * from + own) * partial_floats<SIZE, MODE>(),
-                         p.partial + 2 * from * partial_floats<SIZE, MODE>());
+        join<SIZE, MODE>(p, b, head, first_row, s.row.count, last - from + 1,
+                         p.partial + (2LL * from + own) * partial_floats<SIZE, MODE>(),
+                         p.partial + 2LL * from * partial_floats<SIZE, MODE>());
       }
     }
     __syncthreads();  // the joined rows are read; the ring is free again
@@ -947,8 +976,11 @@ long long grid_of(const cb_paged_attention_args& a, int per_sm) {
   const long long rows = a.tokens * (a.heads / a.cache.kv_heads);
   const long long blocks = (rows + rows_of(MODE) - 1) / rows_of(MODE);
   const long long tiles = (a.cache.columns * a.cache.page + tile_keys(SIZE) - 1) / tile_keys(SIZE);
-  const long long most = a.batch * a.cache.kv_heads * blocks * (tiles + kItemCost), fill = 1LL * per_sm * sm_count();
-  return most < fill ? most : fill;
+  // in units of tiles; what a launch can have to divide is below 2^31 of them
+  const double most = static_cast<double>(a.batch) * a.cache.kv_heads * blocks * (tiles + kItemCost);
+  const long long fill = 1LL * per_sm * sm_count();
+  if (most >= 2147483648.0) return 0;
+  return most < fill ? static_cast<long long>(most) : fill;
 }
 
 }  // namespace
@@ -985,6 +1017,8 @@ int cb_paged_attention(const cb_paged_attention_args* args, void* scratch, unsig
     const int per_sm = resident_blocks<SIZE, STORAGE, MODE, LO>();
     CB_REQUIRE(per_sm >= 1 && per_sm <= 8, "cb_paged_attention: %d blocks of the kernel fit an SM", per_sm);
     const long long grid = grid_of<SIZE, MODE>(a, per_sm);
+    CB_REQUIRE(grid > 0, "cb_paged_attention: %lld rows of up to %lld keys are too many for one call",
+               a.batch * a.heads * a.tokens, a.cache.columns * a.cache.page);
     Plan p;
     p.a = a;
     p.group = static_cast<int>(a.heads / a.cache.kv_heads);
@@ -996,7 +1030,7 @@ int cb_paged_attention(const cb_paged_attention_args* args, void* scratch, unsig
     p.partial = static_cast<float*>(scratch);
     p.arrived = counters;
     launch(attention_kernel<SIZE, STORAGE, MODE, LO>, dim3(static_cast<unsigned>(grid)), dim3(threads_of(MODE)),
-           shared_bytes(SIZE, MODE, LO), static_cast<cudaStream_t>(stream), false, p);
+           shared_bytes(SIZE, MODE, LO), static_cast<cudaStream_t>(stream), true, p);
     return check_launch("cb_paged_attention");
   }));
 }
