@@ -127,6 +127,8 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* shared) {
 template <int DT, int STORAGE>
 __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ cb_paged_append_args a, bool wide) {
   __shared__ uint32_t shared[kThreads / 32];
+  pdl_launch_dependents();
+  pdl_wait();
   const cb_paged_cache& c = a.cache;
   const bool is_v = (blockIdx.x & 1) != 0;
   const int head = static_cast<int>(blockIdx.x >> 1), b = static_cast<int>(blockIdx.z);
@@ -225,8 +227,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
 
 template <int DT>
 int launch_append(const cb_paged_append_args& a, bool wide, dim3 grid, cudaStream_t stream) {
-  if (a.cache.storage == CB_I8) append_kernel<DT, CB_I8><<<grid, kThreads, 0, stream>>>(a, wide);
-  else append_kernel<DT, CB_E4M3><<<grid, kThreads, 0, stream>>>(a, wide);
+  if (a.cache.storage == CB_I8) launch(append_kernel<DT, CB_I8>, grid, dim3(kThreads), 0, stream, true, a, wide);
+  else launch(append_kernel<DT, CB_E4M3>, grid, dim3(kThreads), 0, stream, true, a, wide);
   return check_launch("cb_paged_append");
 }
 

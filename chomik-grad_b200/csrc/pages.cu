@@ -11,8 +11,8 @@
 // lists grow with the table and the pool, run as one cluster of up to eight
 // blocks that exchange their counts through distributed shared memory (64
 // slots of 128 pages: half released in 7 us; by one block 18).  The copies are
-// bound by memory: 8 loads of 16 bytes in flight for each thread of a grid that
-// fills the GPU, launched along with the book's kernel (programmatic dependent
+// bound by memory: a warp for a page of a layer, 8 loads of 16 bytes in flight for
+// each lane, a grid that fills the GPU, launched along with the book's kernel (programmatic dependent
 // launch), which leaves it the list.
 #include <cooperative_groups.h>
 
@@ -26,6 +26,7 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMostBlocks = 8;  // of a cluster: the portable limit
+constexpr long long kClusterCopy = 1LL << 20;  // bytes of pages
 
 // Exclusive prefix sum of v in thread order; *total receives the sum.
 __device__ __forceinline__ long long block_scan(long long v, long long* shared, long long* total) {
@@ -83,10 +84,53 @@ __host__ __device__ __forceinline__ Copies copies_of(void* scratch, long long n)
   return {p, p + 4, p + 4 + n, p + 4 + 2 * n};
 }
 
-__global__ void __launch_bounds__(kThreads) extend_kernel(cb_page_book k, const int* counts, const int* sequences,
-                                                          long long n, void* scratch, int* flag) {
+// Copies of whole pages: unit u = (copy, layer, K or V), taken in turn by the
+// callers' `warps`, each with kBatch 16-byte loads of a lane in flight.
+constexpr int kCopyThreads = 256;
+constexpr int kBatch = 8;
+
+__device__ __forceinline__ void copy_units(const cb_page_pools& p, const int* source, const int* target, int copies,
+                                           int warp, int warps, int* flag) {
+  const unsigned layers = static_cast<unsigned>(p.layers), lane = threadIdx.x & 31;
+  const int vectors = static_cast<int>(p.page_bytes / 16);
+  const unsigned long long units = 2ull * copies * layers;
+  for (unsigned long long u = warp; u < units; u += warps) {
+    const unsigned r = static_cast<unsigned>(u / (2 * layers)), rest = static_cast<unsigned>(u % (2 * layers));
+    const int from = __ldcg(source + r), to = __ldcg(target + r);
+    if (from < 0 || from >= p.pages || to < 0 || to >= p.pages) {
+      if (lane == 0) raise_flag(flag, CB_FLAG_BOOK);
+      continue;
+    }
+    const long long layer = rest >> 1;
+    const bool is_v = rest & 1;
+    char* pool = static_cast<char*>(is_v ? p.v_pages : p.k_pages) + layer * p.pages * p.page_bytes;
+    float* scale = (is_v ? p.v_scale : p.k_scale) + layer * p.pages * p.kv_heads;
+    const uint4* src = reinterpret_cast<const uint4*>(pool + from * p.page_bytes);
+    uint4* dst = reinterpret_cast<uint4*>(pool + to * p.page_bytes);
+    for (int at = lane; at < vectors; at += kBatch * 32) {
+      uint4 v[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (at + i * 32 < vectors) v[i] = __ldcs(src + at + i * 32);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (at + i * 32 < vectors) __stcs(dst + at + i * 32, v[i]);
+    }
+    for (int h = lane; h < p.kv_heads; h += 32)
+      scale[static_cast<long long>(to) * p.kv_heads + h] = scale[static_cast<long long>(from) * p.kv_heads + h];
+  }
+}
+
+__global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constant__ cb_page_pools p, const int* source,
+                                                            const int* target, const int* count, int n, int* flag) {
+  pdl_wait();
+  copy_units(p, source, target, count != nullptr ? *count : n, (blockIdx.x * kCopyThreads + threadIdx.x) / 32,
+             gridDim.x * (kCopyThreads / 32), flag);
+}
+
+__device__ __forceinline__ void extend_book(const cb_page_book& k, const int* counts, const int* sequences,
+                                            long long n, void* scratch, int* flag) {
   __shared__ long long shared[kWarps];
-  pdl_launch_dependents();
   const Copies copies = copies_of(scratch, n);
   int* tails = copies.more;      // open last page of each slot, or -1
   int* plan = copies.more + n;   // pages it takes, negative - 1 where the first of them is a copy
@@ -181,8 +225,24 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(cb_page_book k, const 
   }
 }
 
+// The first block of the cluster does the book; then, where there is more than
+// one, all of them the copies (else a kernel behind this one does).
+__global__ void __launch_bounds__(kThreads) extend_kernel(const __grid_constant__ cb_page_book k,
+                                                          const __grid_constant__ cb_page_pools p, const int* counts,
+                                                          const int* sequences, long long n, void* scratch, int* flag) {
+  pdl_launch_dependents();
+  pdl_wait();
+  if (blockIdx.x == 0) extend_book(k, counts, sequences, n, scratch, flag);
+  if (gridDim.x == 1) return;
+  cg::this_cluster().sync();
+  const Copies c = copies_of(scratch, n);
+  copy_units(p, c.source, c.target, __ldcg(c.count), blockIdx.x * kWarps + threadIdx.x / 32, gridDim.x * kWarps, flag);
+}
+
 __global__ void __launch_bounds__(256) fork_kernel(cb_page_book k, const int* parents, const int* children,
                                                    long long n, int* flag) {
+  pdl_launch_dependents();
+  pdl_wait();
   const long long i = blockIdx.x;
   const int parent = parents[i], child = children[i];
   bool bad = parent < 0 || parent >= k.slots || child < 0 || child >= k.slots;
@@ -217,6 +277,8 @@ __global__ void __launch_bounds__(kThreads) truncate_kernel(cb_page_book k, cons
                                                             int n, int* flag) {
   __shared__ long long shared[kWarps], first[kMostBlocks], second[kMostBlocks], third[kMostBlocks];
   cluster_begun();
+  pdl_launch_dependents();
+  pdl_wait();
   cg::cluster_group group = cg::this_cluster();
   const int blocks = static_cast<int>(group.num_blocks()), rank = static_cast<int>(group.block_rank());
   const int columns = static_cast<int>(k.columns), entries = n * columns;
@@ -314,6 +376,7 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(cb_page_book k, void*
   __shared__ long long shared[kWarps], first[kMostBlocks], second[kMostBlocks], third[kMostBlocks];
   cluster_begun();
   pdl_launch_dependents();
+  pdl_wait();
   cg::cluster_group group = cg::this_cluster();
   const int blocks = static_cast<int>(group.num_blocks()), rank = static_cast<int>(group.block_rank());
   const int pages = static_cast<int>(k.pages), thread = rank * kThreads + threadIdx.x, threads = blocks * kThreads;
@@ -367,41 +430,6 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(cb_page_book k, void*
   }
 }
 
-// Copies of whole pages: unit u = (copy, layer, K or V).
-constexpr int kCopyThreads = 256;
-constexpr int kBatch = 8;  // 16-byte loads a thread has in flight
-
-__global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constant__ cb_page_pools p, const int* source,
-                                                            const int* target, const int* count, int n, int* flag) {
-  pdl_wait();
-  const int copies = count != nullptr ? *count : n, layers = static_cast<int>(p.layers);
-  const long long units = 2LL * copies * layers;
-  const int vectors = static_cast<int>(p.page_bytes / 16);
-  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-    const int r = static_cast<int>(u / (2 * layers)), layer = static_cast<int>(u % (2 * layers)) >> 1;
-    const int from = source[r], to = target[r];
-    if (from < 0 || from >= p.pages || to < 0 || to >= p.pages) {
-      if (threadIdx.x == 0) raise_flag(flag, CB_FLAG_BOOK);
-      continue;
-    }
-    char* pool = static_cast<char*>(u % 2 ? p.v_pages : p.k_pages) + layer * p.pages * p.page_bytes;
-    float* scale = (u % 2 ? p.v_scale : p.k_scale) + layer * p.pages * p.kv_heads;
-    const uint4* src = reinterpret_cast<const uint4*>(pool + from * p.page_bytes);
-    uint4* dst = reinterpret_cast<uint4*>(pool + to * p.page_bytes);
-    for (int at = threadIdx.x; at < vectors; at += kBatch * kCopyThreads) {
-      uint4 v[kBatch];
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-        if (at + i * kCopyThreads < vectors) v[i] = __ldcs(src + at + i * kCopyThreads);
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-        if (at + i * kCopyThreads < vectors) __stcs(dst + at + i * kCopyThreads, v[i]);
-    }
-    for (int i = threadIdx.x; i < p.kv_heads; i += kCopyThreads)
-      scale[static_cast<long long>(to) * p.kv_heads + i] = scale[static_cast<long long>(from) * p.kv_heads + i];
-  }
-}
-
 int book_check(const cb_page_book* k, long long n, const char* who) {
   CB_REQUIRE(k != nullptr && k->table && k->lengths && k->refs && k->free_pages && k->height, "%s: a null pointer", who);
   CB_REQUIRE(k->slots >= 1 && k->columns >= 1 && k->pages >= 1 && k->page >= 1, "%s: an empty book", who);
@@ -423,8 +451,9 @@ int pools_check(const cb_page_pools* p, const char* who) {
 
 int launch_copies(const cb_page_pools& p, const int* source, const int* target, const int* count, long long most,
                   bool behind, int* flag, cudaStream_t stream) {
-  const long long units = most * p.layers * 2, cap = 1LL * (2048 / kCopyThreads) * sm_count();
-  launch(copy_kernel, dim3(static_cast<unsigned>(units < cap ? units : cap)), dim3(kCopyThreads), 0, stream, behind, p,
+  const long long blocks = (most * p.layers * 2 + kCopyThreads / 32 - 1) / (kCopyThreads / 32);
+  const long long cap = 1LL * (2048 / kCopyThreads) * sm_count();
+  launch(copy_kernel, dim3(static_cast<unsigned>(blocks < cap ? blocks : cap)), dim3(kCopyThreads), 0, stream, behind, p,
          source, target, count, static_cast<int>(most), flag);
   return check_launch("cb_pages: copies");
 }
@@ -439,12 +468,14 @@ int launch_cluster(void (*kernel)(Expected...), const char* what, long long work
   cfg.gridDim = dim3(blocks);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = blocks;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   cudaLaunchKernelEx(&cfg, kernel, static_cast<Expected>(args)...);
   return check_launch(what);
 }
@@ -472,9 +503,12 @@ int cb_pages_extend(const cb_page_book* book, const cb_page_pools* pools, const 
   CB_REQUIRE(pools->pages == book->pages, "cb_pages_extend: %lld pages in the pools, %lld in the book", pools->pages,
              book->pages);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  extend_kernel<<<1, kThreads, 0, s>>>(*book, counts, sequences, n, scratch, error_flag);
-  status = check_launch("cb_pages_extend");
-  if (status != CB_OK) return status;
+  // few bytes at most: one cluster does book and copies, in one launch; eight
+  // SMs copy at about 1 TB/s, so above kClusterCopy a grid of its own is faster
+  const bool together = 2LL * n * pools->layers * pools->page_bytes <= kClusterCopy;
+  status = launch_cluster(extend_kernel, "cb_pages_extend", together ? 1LL * kMostBlocks * kThreads : 1, s, *book, *pools,
+                          counts, sequences, n, scratch, error_flag);
+  if (status != CB_OK || together) return status;
   const Copies c = copies_of(scratch, n);
   return launch_copies(*pools, c.source, c.target, c.count, n, true, error_flag, s);
 }
@@ -485,8 +519,8 @@ int cb_pages_fork(const cb_page_book* book, const int* parents, const int* child
   if (status != CB_OK) return status;
   if (n == 0) return CB_OK;
   CB_REQUIRE(parents != nullptr && children != nullptr, "cb_pages_fork: a null pointer");
-  fork_kernel<<<static_cast<unsigned>(n), 256, 0, static_cast<cudaStream_t>(stream)>>>(*book, parents, children, n,
-                                                                                     error_flag);
+  launch(fork_kernel, dim3(static_cast<unsigned>(n)), dim3(256), 0, static_cast<cudaStream_t>(stream), true, *book,
+         parents, children, n, error_flag);
   return check_launch("cb_pages_fork");
 }
 

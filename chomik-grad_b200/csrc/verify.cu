@@ -22,15 +22,27 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMostBlocks = 8;  // of a cluster: the portable limit
 
 using u64 = unsigned long long;
 
+// trunc(min(max(x, 0), 1) * 2^40), NaN gives 0, as hi * 2^23 + lo: adding 2^23
+// with rounding toward zero leaves the integer part in the low bits of the sum
+// (float32 instructions only; a 64-bit conversion takes some ten times as long).
+// The bits of 2^23 itself are left in both for the caller to take off.
+constexpr uint32_t kBias = 0x4b000000u;
+__device__ __forceinline__ void fixed_parts(float x, uint32_t& hi, uint32_t& lo) {
+  const float big = 8388608.0f, y = fminf(fmaxf(x, 0.0f), 1.0f) * 131072.0f;
+  const float t = __fadd_rz(y, big);
+  hi = __float_as_uint(t);
+  lo = __float_as_uint(__fadd_rz((y - (t - big)) * big, big));
+}
 __device__ __forceinline__ u64 fixed_point(float x) {
-  // float -> integer conversion truncates; NaN and negative numbers weigh nothing
-  return x > 0.0f ? static_cast<u64>(fminf(x, 1.0f) * 1099511627776.0f) : 0ull;
+  uint32_t hi, lo;
+  fixed_parts(x, hi, lo);
+  return (static_cast<u64>(hi - kBias) << 23) + (lo - kBias);
 }
 
 __device__ __forceinline__ u64 warp_total(u64 v) {
@@ -44,25 +56,29 @@ struct Item {
   static constexpr int kPer = DT == CB_F32 ? 4 : 8;  // elements of 16 bytes
 };
 
+template <int DT>
+__device__ __forceinline__ void unpack(const uint4& w, float* x) {
+  if (DT == CB_F32) {
+    x[0] = __uint_as_float(w.x); x[1] = __uint_as_float(w.y);
+    x[2] = __uint_as_float(w.z); x[3] = __uint_as_float(w.w);
+  } else if (DT == CB_BF16) {
+    unpack_bf16x8(w, x);
+  } else {
+    const __half2* h = reinterpret_cast<const __half2*>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __low2float(h[i]);
+      x[2 * i + 1] = __high2float(h[i]);
+    }
+  }
+}
+
 // kPer probabilities from element j of a row of `vocab`; those past its end are 0.
 template <int DT>
 __device__ __forceinline__ void load_row(const char* row, long long j, long long vocab, bool wide, float* x) {
   constexpr int kPer = Item<DT>::kPer;
   if (wide && j + kPer <= vocab) {
-    const uint4 w = *reinterpret_cast<const uint4*>(row + j * (16 / kPer));
-    if (DT == CB_F32) {
-      x[0] = __uint_as_float(w.x); x[1] = __uint_as_float(w.y);
-      x[2] = __uint_as_float(w.z); x[3] = __uint_as_float(w.w);
-    } else if (DT == CB_BF16) {
-      unpack_bf16x8(w, x);
-    } else {
-      const __half2* h = reinterpret_cast<const __half2*>(&w);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[2 * i] = __low2float(h[i]);
-        x[2 * i + 1] = __high2float(h[i]);
-      }
-    }
+    unpack<DT>(*reinterpret_cast<const uint4*>(row + j * (16 / kPer)), x);
   } else {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) x[i] = j + i < vocab ? load_as_f32(row, j + i, DT) : 0.0f;
@@ -70,7 +86,7 @@ __device__ __forceinline__ void load_row(const char* row, long long j, long long
 }
 
 struct Sums {  // of one block
-  u64 rest, whole;
+  u64 weight;
   int nan;
 };
 
@@ -84,8 +100,10 @@ __host__ __device__ __forceinline__ long long run_of(long long vocab, int blocks
 template <int DT>
 __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant__ cb_verify_args a, int blocks) {
   constexpr int kPer = Item<DT>::kPer, kItem = 16 / kPer;
-  __shared__ Sums warps[kWarps], cluster[kMostBlocks];
+  __shared__ Sums warps[kWarps], cluster[2][kMostBlocks];
   cluster_begun();
+  pdl_launch_dependents();
+  pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = static_cast<int>(blockIdx.x) % blocks;
   const long long b = blockIdx.x / blocks;
   long long n = a.counts != nullptr ? a.counts[b] : a.tokens;
@@ -127,55 +145,87 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
   const long long from = (static_cast<long long>(rank) * kWarps + warp) * run;
   const long long to = from + run < a.vocab ? from + run : a.vocab;
 
-  // 1. sums of the runs
-  u64 rest = 0, whole = 0;
-  bool nan = false;
-#pragma unroll 4
-  for (long long j = from + lane * kPer; j < to; j += 32 * kPer) {
-    float p[kPer], q[kPer];
-    load_row<DT>(p_row, j, a.vocab, wide, p);
-    if (refused) load_row<DT>(q_row, j, a.vocab, wide, q);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const float other = refused ? q[i] : 0.0f;
-      nan = nan || p[i] != p[i] || other != other;
-      rest += fixed_point(p[i] - other);
-      whole += fixed_point(p[i]);
-    }
-  }
-  rest = warp_total(rest);
-  whole = warp_total(whole);
-  nan = __any_sync(0xffffffffu, nan);
-  if (lane == 0) warps[warp] = {rest, whole, nan};
-  __syncthreads();
+  // 1. sums of the runs.  The remainders p - q first; only where a refused
+  // draft leaves none, the target's own probabilities (`second`).
   cg::cluster_group group = cg::this_cluster();
-  cluster_all_begun();
-  if (static_cast<int>(threadIdx.x) < blocks) {  // a copy of the block's sums for each block of the cluster
-    Sums mine = {0, 0, 0};
+  u64 total = 0, before = 0;
+  bool second = false;
+  int bad = 0;
+  for (;;) {
+    const bool with_draft = refused && !second;
+    u64 sum = 0;
+    uint32_t hi = 0, lo = 0;
+    int held = 0;  // steps summed in hi and lo
+    bool nan = false;
+    auto flush = [&] {
+      const uint32_t bias = static_cast<uint32_t>(held) * kPer * kBias;
+      sum += (static_cast<u64>(hi - bias) << 23) + (lo - bias);
+      hi = lo = 0;
+      held = 0;
+    };
+    auto add = [&](const float* p, const float* q) {
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      mine.rest += warps[w].rest;
-      mine.whole += warps[w].whole;
-      mine.nan |= warps[w].nan;
+      for (int i = 0; i < kPer; ++i) {
+        const float other = with_draft ? q[i] : 0.0f;
+        nan = nan || p[i] != p[i] || other != other;
+        uint32_t h, l;
+        fixed_parts(p[i] - other, h, l);
+        hi += h;
+        lo += l;
+      }
+      if (++held == 32) flush();  // 32 steps of up to 8 weights below 2^23: their sum is below 2^32
+    };
+    constexpr int kStep = 32 * kPer, kBatch = 4;  // elements of a warp's loads; of them in flight
+    long long first = from;
+    for (; wide && first + kBatch * kStep <= to; first += kBatch * kStep) {
+      uint4 p[kBatch], q[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) p[i] = reinterpret_cast<const uint4*>(p_row)[(first + i * kStep) / kPer + lane];
+      if (with_draft) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) q[i] = reinterpret_cast<const uint4*>(q_row)[(first + i * kStep) / kPer + lane];
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        float x[kPer], y[kPer];
+        unpack<DT>(p[i], x);
+        if (with_draft) unpack<DT>(q[i], y);
+        add(x, y);
+      }
     }
-    *group.map_shared_rank(&cluster[rank], threadIdx.x) = mine;
+    for (; first < to; first += kStep) {
+      float x[kPer], y[kPer];
+      load_row<DT>(p_row, first + lane * kPer, a.vocab, wide, x);
+      if (with_draft) load_row<DT>(q_row, first + lane * kPer, a.vocab, wide, y);
+      add(x, y);
+    }
+    flush();
+    sum = warp_total(sum);
+    nan = __any_sync(0xffffffffu, nan);
+    if (lane == 0) warps[warp] = {sum, nan};
+    __syncthreads();
+    if (!second) cluster_all_begun();
+    if (static_cast<int>(threadIdx.x) < blocks) {  // a copy of the block's sums for each block of the cluster
+      Sums mine = {0, 0};
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        mine.weight += warps[w].weight;
+        mine.nan |= warps[w].nan;
+      }
+      *group.map_shared_rank(&cluster[second][rank], threadIdx.x) = mine;
+    }
+    group.sync();
+    total = 0;
+    for (int r = 0; r < blocks; ++r) {
+      if (r == rank) before = total;
+      total += cluster[second][r].weight;
+      bad |= cluster[second][r].nan;
+    }
+    if (total > 0 || !with_draft || bad) break;  // the same in every block
+    second = true;
   }
-  group.sync();
 
   // 2. the threshold, and the warp that holds it
-  u64 rest_total = 0, whole_total = 0, rest_before = 0, whole_before = 0;
-  int bad = 0;
-  for (int r = 0; r < blocks; ++r) {
-    if (r == rank) {
-      rest_before = rest_total;
-      whole_before = whole_total;
-    }
-    rest_total += cluster[r].rest;
-    whole_total += cluster[r].whole;
-    bad |= cluster[r].nan;
-  }
-  const bool from_rest = rest_total > 0;
-  const u64 total = from_rest ? rest_total : whole_total;
   bad |= total == 0;
   u64 bar = 0;
   if (!bad) {
@@ -192,32 +242,53 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
       if (t != accepted || bad) a.out[b * (a.tokens + 1) + t] = t < accepted ? drafted[t] : -1;
   }
   if (bad) return;
-  u64 before = from_rest ? rest_before : whole_before;
-  for (int w = 0; w < warp; ++w) before += from_rest ? warps[w].rest : warps[w].whole;
-  const u64 mine = from_rest ? warps[warp].rest : warps[warp].whole;
-  if (bar < before || bar >= before + mine) return;
+  for (int w = 0; w < warp; ++w) before += warps[w].weight;
+  if (bar < before || bar >= before + warps[warp].weight) return;
 
-  // 3. that warp's run once more, in order
-  for (long long first = from; first < to; first += 32 * kPer) {
+  // 3. that warp's run once more: each lane a contiguous part of it, then the
+  // part that holds the threshold, each lane kPer elements of it at a time
+  const bool with_draft = refused && !second;
+  auto weights = [&](long long j, u64* w) {
     float p[kPer], q[kPer];
-    load_row<DT>(p_row, first + lane * kPer, a.vocab, wide, p);
-    if (refused && from_rest) load_row<DT>(q_row, first + lane * kPer, a.vocab, wide, q);
+    load_row<DT>(p_row, j, a.vocab, wide, p);
+    if (with_draft) load_row<DT>(q_row, j, a.vocab, wide, q);
     u64 sum = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) sum += fixed_point(p[i] - (refused && from_rest ? q[i] : 0.0f));
-    u64 upto = sum;
+    for (int i = 0; i < kPer; ++i) {
+      w[i] = fixed_point(p[i] - (with_draft ? q[i] : 0.0f));
+      sum += w[i];
+    }
+    return sum;
+  };
+  auto upto_lane = [&](u64 v) {  // inclusive sum over the lanes
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const u64 up = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += up;
+      const u64 up = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += up;
     }
+    return v;
+  };
+  const long long part = run / 32;  // a multiple of kPer
+  u64 w[kPer], sum = 0;
+#pragma unroll 4
+  for (long long j = 0; j < part; j += kPer) sum += weights(from + lane * part + j, w);
+  u64 upto = upto_lane(sum);
+  const int holder = __ffs(__ballot_sync(0xffffffffu, bar < before + upto)) - 1;
+  before += __shfl_sync(0xffffffffu, upto - sum, holder);
+  const long long begin = from + holder * part;
+  for (long long first = begin; first < begin + part; first += 32 * kPer) {
+    const long long j = first + lane * kPer;
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) w[i] = 0;
+    if (j < begin + part) sum = weights(j, w);
+    upto = upto_lane(sum);
     u64 running = before + upto - sum;
     if (running <= bar && bar < before + upto) {  // one lane
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const u64 w = fixed_point(p[i] - (refused && from_rest ? q[i] : 0.0f));
-        if (running <= bar && bar < running + w) a.out[b * (a.tokens + 1) + accepted] = first + lane * kPer + i;
-        running += w;
+        if (running <= bar && bar < running + w[i]) a.out[b * (a.tokens + 1) + accepted] = j + i;
+        running += w[i];
       }
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
@@ -227,20 +298,21 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
 
 template <int DT>
 int launch_verify(const cb_verify_args& a, cudaStream_t stream) {
-  // blocks of a row: as few as leave a thread 16 elements (32000 of float32 by
-  // four blocks: 4.9 us; by one: 8.5, by eight: 5.0)
+  // blocks of a row: as few as leave a thread 16 elements
   int blocks = 1;
   while (blocks < kMostBlocks && a.vocab > 16LL * kThreads * blocks) blocks *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.batch * blocks));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = static_cast<unsigned>(blocks);
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   cudaLaunchKernelEx(&cfg, verify_kernel<DT>, a, blocks);
   return check_launch("cb_verify_draft");
 }

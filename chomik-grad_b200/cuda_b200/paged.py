@@ -73,8 +73,9 @@ def require(value: torch.Tensor, name: str, device: torch.device, dtypes, shape:
 
 def no_grad_needed(*values: torch.Tensor) -> None:
     """Refuse values that a gradient should flow through."""
-    if torch.is_grad_enabled() and any([v.requires_grad for v in values]):
-        raise ValueError("an argument requires grad: this operator has no backward pass")
+    for value in values:
+        if value.requires_grad and torch.is_grad_enabled():
+            raise ValueError("an argument requires grad: this operator has no backward pass")
 
 
 def current_stream(device: torch.device) -> int:
@@ -155,7 +156,7 @@ class PagedCache:
         p.page_bytes = self.kv_heads * self.page_size * self.head_size
         self._lib = _lib.load()
         self._attend_args, self._append_args, self._lists = Prepared(), Prepared(), Prepared()
-        self._scratch_words, self._counters = Prepared(), Prepared()
+        self._scratch_words, self._workspaces = Prepared(), Prepared()
 
     @classmethod
     def allocate(cls, *, layers: int, pages: int, kv_heads: int, page_size: int, head_size: int, sequences: int,
@@ -285,25 +286,26 @@ class PagedCache:
             a.counts = counts.data_ptr()
         if sequences is not None:
             a.sequences = sequences.data_ptr()
-        scratch, stream = self._flag.new_empty(known[1]), self._stream()
-        counters = self._counters_of(stream, known[2])
-        _lib.check(self._lib.cb_paged_attention(ctypes.byref(a), scratch.data_ptr(), counters.data_ptr(), stream),
-                   "cb_paged_attention")
+        stream = self._stream()
+        counters, scratch = self._workspace(stream, known[2], known[1])
+        _lib.check(self._lib.cb_paged_attention(ctypes.byref(a), scratch, counters, stream), "cb_paged_attention")
         return out
 
-    def _counters_of(self, stream: int, count: int) -> torch.Tensor:
-        """Zeroed counters for a call on ``stream``, which leaves them zero.
+    def _workspace(self, stream: int, counters: int, words: int) -> Tuple[int, int]:
+        """Addresses of zeroed counters, which a call leaves zero, and of scratch for a call on ``stream``.
 
         Calls of one stream follow one another and share theirs.  A captured
         call may be replayed on any stream, so it has its own, cleared within
         the graph.
         """
         if torch.cuda.is_current_stream_capturing():
-            return self._flag.new_zeros(count)
-        counters = self._counters.get(stream)
-        if counters is None or counters.shape[0] < count:
-            counters = self._counters[stream] = self._flag.new_zeros(count)
-        return counters
+            own = self._flag.new_empty(words)  # (the graph's memory pool keeps both)
+            return self._flag.new_zeros(counters).data_ptr(), own.data_ptr()
+        kept = self._workspaces.get(stream)
+        if kept is None or kept[0] < counters or kept[1] < words:
+            counts, scratch = self._flag.new_zeros(counters), self._flag.new_empty(words)
+            kept = self._workspaces[stream] = (counters, words, counts.data_ptr(), scratch.data_ptr(), counts, scratch)
+        return kept[2], kept[3]
 
     def _prepare_attend(self, layer: int, q: torch.Tensor, counts: Optional[torch.Tensor],
                         sequences: Optional[torch.Tensor],
