@@ -40,8 +40,7 @@
 // length are filled with zeros, whatever the page holds there.
 #include <type_traits>
 
-#include "paged.cuh"
-#include "sync.cuh"
+#include "paged_attention.cuh"
 
 namespace cb {
 namespace {
@@ -50,36 +49,26 @@ constexpr int kGroups = 4;                       // of keys, in a tile
 constexpr int kStepBytes = 4096;                 // K and V of a group's step
 constexpr int kHeadBytes = 64;                   // its scales: 4 of K, 4 of V
 constexpr int kSlotBytes = kStepBytes + kHeadBytes;
-constexpr int kHalfBytes = 8192;                 // K and V of a step as fp16, where warps share them
 
 // How the query rows fill the tensor core's 16-row tiles: 8 of them with both
-// parts in one tile, or MODE tiles, each with warps of its own.
+// parts in one tile, or MODE tiles of 16.
 enum { kPacked = 0 };
+__host__ __device__ constexpr int tiles_of_mode(int mode) { return mode == kPacked ? 1 : mode; }
 __host__ __device__ constexpr int rows_of(int mode) { return mode == kPacked ? 8 : 16 * mode; }
-__host__ __device__ constexpr int tiles_of(int mode) { return mode == kPacked ? 1 : mode; }
-__host__ __device__ constexpr int warps_of(int mode) { return kGroups * tiles_of(mode); }
-__host__ __device__ constexpr int threads_of(int mode) { return 32 * warps_of(mode); }
-// Resident blocks of an SM: 16 warps of 128 registers, or, with the low parts of
-// float32 queries, 12 of 168.  The steps of a group's ring then follow from
-// shared memory, and from the joined rows that take its place.
-__host__ __device__ constexpr int resident_of(int mode, int lo) { return lo ? 3 : 4 / tiles_of(mode); }
-__host__ __device__ constexpr int stages_of(int mode, int lo) { return mode == 4 ? 8 : mode == 2 || lo ? 4 : 3; }
+constexpr int kThreads = 32 * kGroups;
+// Resident blocks of an SM: 16 warps of 128 registers, with the low parts of
+// float32 queries 12 of 168, with two tiles' sums 8 of 255.  The steps of a
+// warp's ring then follow from shared memory.
+__host__ __device__ constexpr int resident_of(int mode, int lo) { return mode == 2 ? 2 : lo ? 3 : 4; }
+__host__ __device__ constexpr int stages_of(int mode, int lo) { return mode == 2 ? 5 : lo ? 4 : 3; }
 __host__ __device__ constexpr int ring_bytes(int mode, int lo) { return kGroups * stages_of(mode, lo) * kSlotBytes; }
-// Warps that share keys convert each of them once, into shared memory.
-__host__ __device__ constexpr bool shares(int mode) { return mode > 1; }
-__host__ __device__ constexpr int half_bytes(int mode) { return shares(mode) ? kGroups * kHalfBytes : 0; }
 __host__ __device__ constexpr int step_keys(int head_size) { return 2048 / head_size; }
 __host__ __device__ constexpr int tile_keys(int head_size) { return kGroups * step_keys(head_size); }
 
 // Shared memory of a block: the ring, and the queries as the products read them.
 __host__ __device__ constexpr int shared_bytes(int head_size, int mode, int lo) {
-  return ring_bytes(mode, lo) + half_bytes(mode) + tiles_of(mode) * (lo ? 2 : 1) * (head_size / 16) * 512;
+  return ring_bytes(mode, lo) + tiles_of_mode(mode) * (lo ? 2 : 1) * (head_size / 16) * 512;
 }
-// Tiles' time that beginning an item costs (queries, first loads, joining the
-// warps): counted when the work is divided.
-constexpr int kItemCost = 2;
-// Items of no more than six tiles are not cut: joining parts takes as long.
-constexpr int kSmallItem = kItemCost + 6;
 
 // ---- loads -------------------------------------------------------------------
 
@@ -96,12 +85,6 @@ __device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool real) 
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// Barrier of the MODE warps that share a group's keys.
-template <int MODE>
-__device__ __forceinline__ void group_sync(int group) {
-  if (MODE <= 1) __syncwarp();
-  else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * tiles_of(MODE)) : "memory");
-}
 template <int N>
 __device__ __forceinline__ void wait_groups() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -141,7 +124,6 @@ __device__ __forceinline__ void read_words(const char* p, uint32_t* w) {
 
 // ---- fp16 operands -------------------------------------------------------------
 
-__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
 // Four codes -> two pairs of halves: of int8 elements 0, 2 and 1, 3, of e4m3
 // elements 0, 1 and 2, 3.  int8: the byte x + 128 (the sign bit turned) under
@@ -162,39 +144,6 @@ __device__ __forceinline__ void to_halves(uint32_t w, uint32_t& a, uint32_t& b) 
         : "r"(w));
   }
 }
-// Four codes -> the pairs 0, 1 and 2, 3 whatever the storage.
-template <int STORAGE>
-__device__ __forceinline__ void to_halves_in_order(uint32_t w, uint32_t& a, uint32_t& b) {
-  if (STORAGE == CB_I8) {
-    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-    w ^= 0x80808080u;
-    const uint32_t lo = __byte_perm(w, 0x64646464u, 0x4140), hi = __byte_perm(w, 0x64646464u, 0x4342);
-    a = bits(__hsub2(*reinterpret_cast<const __half2*>(&lo), bias));
-    b = bits(__hsub2(*reinterpret_cast<const __half2*>(&hi), bias));
-  } else {
-    to_halves<STORAGE>(w, a, b);
-  }
-}
-
-// Byte offset of 16-byte piece `piece` of fp16 row `row` (2 SIZE bytes): eight
-// rows of one piece, which a matrix load reads at once, lie in different banks.
-template <int SIZE>
-__device__ __forceinline__ int half_at(int row, int piece) {
-  const int at = row * (SIZE / 8) + piece, line = at >> 3;
-  const int turn = SIZE == 128 ? (line >> 1) & 7 : SIZE == 64 ? line & 7 : line & 3;
-  return (line << 7) + (((at & 7) ^ turn) << 4);
-}
-// Four 8x8 matrices of halves; lane l gives the address of row l % 8 of matrix l / 8.
-template <bool TURNED>
-__device__ __forceinline__ void load_matrices(uint32_t at, uint32_t* r) {
-  if (TURNED)
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-  else
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-}
-
 // The words whose pairs are elements 2 i and 2 i + 1 of two rows, i = 0, 1.
 template <int STORAGE>
 __device__ __forceinline__ uint32_t interleave(uint32_t a, uint32_t b, int i) {
@@ -224,109 +173,16 @@ __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, ui
   }
 }
 
-// 2^x by the hardware's instruction: its relative error is below 2^-22, and
-// results below 2^-126 are zero (weights are at most one).
-__device__ __forceinline__ float exp2_of(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// 2^x as the square of this: a sum may be large enough that its share is
-// kept where 2^x itself would be below float32's range.
-__device__ __forceinline__ float root2_of(float x) { return exp2_of(0.5f * x); }
-
-// ---- division of the work ------------------------------------------------------
-
-struct Plan {  // of one launch
-  cb_paged_attention_args a;
-  int group, rows, blocks;  // query heads of a kv head, rows of a kv head, blocks of them
-  bool wide;                // queries can be read 16 bytes at a time
-  float* partial;           // scratch: two partial results of each block
-  unsigned* arrived;        // for each block: parts of the item that it begins and does not end
-};
-
-struct Slot {
-  PagedRow row;
-  int tiles;
-};
-template <int SIZE>
-__device__ __forceinline__ int tiles_of_slot(const PagedRow& row) {
-  const int keys = row.count > 0 ? row.length : 0;  // (an item without keys writes zeros)
-  return max(1, (keys + tile_keys(SIZE) - 1) / tile_keys(SIZE));
-}
-template <int SIZE>
-__device__ __forceinline__ Slot slot_of(const Plan& p, long long b) {
-  Slot s;
-  if (!paged_row(p.a.cache, p.a.sequences, p.a.counts, p.a.tokens, b, p.a.error_flag, &s.row)) {
-    s.row.length = s.row.count = 0;
-    s.row.table = p.a.cache.table;
-  }
-  s.tiles = tiles_of_slot<SIZE>(s.row);
-  return s;
-}
-
-template <int MODE>
-__device__ __forceinline__ int block_scan(int v, int* shared, int* total) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int incl = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += up;
-  }
-  __syncthreads();
-  if (lane == 31) shared[warp] = incl;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < warps_of(MODE); ++w) {
-    if (w == warp) before = all;
-    all += shared[w];
-  }
-  *total = all;
-  return before + incl - v;
-}
-
-// Weights are at most 2^(kSlack + 1): far inside fp16, with its 11 (hi and lo:
-// 22) bits for all that are within 2^-14 of the largest.
-constexpr float kSlack = 8.0f;
-
 // ---- one item ------------------------------------------------------------------
 
 // The sums of one warp: its rows g (and g + 8 of a 16-row tile), columns 2c and
 // 2c + 1 of each value tile, g = lane / 4, c = lane % 4.
 template <int SIZE, int MODE>
 struct Sums {
-  static constexpr int kHalves = MODE == kPacked ? 1 : 2;
-  float o[SIZE / 8][4];  // as the products leave them; packed: of the hi and the lo weights
-  float m[kHalves], l[kHalves];
+  static constexpr int kTiles = tiles_of_mode(MODE), kHalves = MODE == kPacked ? 1 : 2;
+  float o[kTiles][SIZE / 8][4];  // as the products leave them; packed: of the hi and the lo weights
+  float m[kTiles][kHalves], l[kTiles][kHalves];
 };
-
-// Eight neighbouring elements of a query row.
-__device__ __forceinline__ void load_query(const Plan& p, const void* query, long long at, float* x) {
-  if (!p.wide) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = load_as_f32(query, at + i, p.a.dtype);
-  } else if (p.a.dtype == CB_F32) {
-    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(query) + at);
-    const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(query) + at + 4);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  } else {
-    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(query) + at);
-    if (p.a.dtype == CB_BF16) {
-      unpack_bf16x8(w, x);
-    } else {
-      const __half2* h = reinterpret_cast<const __half2*>(&w);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[2 * i] = __low2float(h[i]);
-        x[2 * i + 1] = __high2float(h[i]);
-      }
-    }
-  }
-}
 
 // The block's query rows as the products read them: `queries` holds the 16-row
 // operands of each 16-element product, `factors` what turns a row's products
@@ -338,7 +194,7 @@ __device__ __forceinline__ void load_queries(const Plan& p, const void* query, i
   constexpr int kLanes = SIZE / 8, kDots = SIZE / 16, kParts = LO ? 2 : 1;
   constexpr int kKeyWords = SIZE / 16 < 4 ? SIZE / 16 : 4;
 #pragma unroll
-  for (int first = 0; first < rows_of(MODE); first += threads_of(MODE) / kLanes) {
+  for (int first = 0; first < rows_of(MODE); first += kThreads / kLanes) {
     const int row = first + static_cast<int>(threadIdx.x) / kLanes, d = static_cast<int>(threadIdx.x) % kLanes * 8;
     const int r = first_row + row, t = r / p.group;
     float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, largest = 0.0f;
@@ -362,15 +218,9 @@ __device__ __forceinline__ void load_queries(const Plan& p, const void* query, i
 #pragma unroll
       for (int pair = 0; pair < 2; ++pair) {
         uint32_t hi, lo;
-        const int first = 4 * word + (STORAGE == CB_I8 && !shares(MODE) ? pair : 2 * pair);
-        const int next = STORAGE == CB_I8 && !shares(MODE) ? 2 : 1;
+        const int first = 4 * word + (STORAGE == CB_I8 ? pair : 2 * pair), next = STORAGE == CB_I8 ? 2 : 1;
         split(x[first] * down, x[first + next] * down, hi, lo);  // in the pairs of to_halves
-        if (shares(MODE)) {  // elements 16 dot + 2 column + {0, 1}, and 8 further
-          const int pair_at = at + 2 * pair;
-          uint32_t* turned = reinterpret_cast<uint32_t*>(queries + (row / 16 * kDots + pair_at / 16) * 32 +
-                                                         row % 8 * 4 + pair_at % 8 / 2);
-          turned[2 * (pair_at / 8 % 2) + row / 8 % 2] = hi;
-        } else if (MODE == kPacked) {
+        if (MODE == kPacked) {
           to[2 * pair] = hi;
           to[2 * pair + 1] = lo;
         } else {
@@ -383,7 +233,7 @@ __device__ __forceinline__ void load_queries(const Plan& p, const void* query, i
 }
 
 template <int SIZE, int STORAGE, int MODE, int LO>
-__device__ __forceinline__ void warp_item(const Plan& p, const void* query, const Slot& s, int head, int block_row,
+__device__ __forceinline__ void warp_item(const Plan& p, const void* query, const Slot& s, int head, int first_row,
                                           int tile, int tiles, char* shared, float* factors,
                                           Sums<SIZE, MODE>& sums) {
   using S = Sums<SIZE, MODE>;
@@ -394,25 +244,26 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
   constexpr int kValueWords = SIZE / 32;
   constexpr int kParts = LO ? 2 : 1;
   const cb_paged_cache& c = p.a.cache;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
-  const int group = warp % kGroups, rank = warp / kGroups;  // of keys; among the warps that share them
-  const int first_row = block_row + 16 * rank;
+  const int group = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
   char* ring = shared + group * kStages * kSlotBytes;
-  uint4* queries = reinterpret_cast<uint4*>(shared + ring_bytes(MODE, LO) + half_bytes(MODE));
+  uint4* queries = reinterpret_cast<uint4*>(shared + ring_bytes(MODE, LO));
 
   // limits: row r sees keys below limit[r]; all rows of the warp see those below `common`
-  int limit[S::kHalves];
+  int limit[S::kTiles][S::kHalves];
 #pragma unroll
-  for (int half = 0; half < S::kHalves; ++half) {
-    const int r = first_row + half * 8 + g, t = r / p.group;
-    limit[half] = r < p.rows && t < s.row.count ? s.row.length - s.row.count + t + 1 : 0;
-    sums.m[half] = -INFINITY;
-    sums.l[half] = 0.0f;
+  for (int mt = 0; mt < S::kTiles; ++mt) {
+#pragma unroll
+    for (int half = 0; half < S::kHalves; ++half) {
+      const int r = first_row + mt * 16 + half * 8 + g, t = r / p.group;
+      limit[mt][half] = r < p.rows && t < s.row.count ? s.row.length - s.row.count + t + 1 : 0;
+      sums.m[mt][half] = -INFINITY;
+      sums.l[mt][half] = 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < SIZE / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sums.o[mt][j][i] = 0.0f;
   }
-#pragma unroll
-  for (int j = 0; j < SIZE / 8; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sums.o[j][i] = 0.0f;
   int last = 0;  // exponent of the value scale before
   const int common = s.row.length - s.row.count + first_row / p.group + 1;
   const int length = s.row.length;
@@ -434,22 +285,16 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
   };
   int ids = ids_of(0), ids_next = ids_of(1), batch = 0;
 
-  // A step is eight copies of 32 x 16 bytes, four of K and four of V: a warp
-  // alone does all, one of two K or V, one of four half of those.
-  constexpr int kPools = tiles_of(MODE) == 1 ? 2 : 1, kCopies = 4 / (MODE == 4 ? 2 : 1), kRowCopies = SIZE / 32;
-  const int first_copy = MODE == 4 ? (rank >> 1) * 2 : 0;
-  const bool second = kPools == 1 && (rank & 1);  // copies V, not K
+  // A step is four copies of 32 x 16 bytes of K and four of V, 512 bytes apart;
+  // odd ones of 128-byte rows are turned by half a line.
+  constexpr int kRowCopies = SIZE / 32;  // of 16 rows
   const uint32_t page_bytes = static_cast<uint32_t>(c.kv_heads) * c.page * SIZE;
   const long long head_at = static_cast<long long>(head) * c.page * SIZE + lane * 16;
-  const char* k_pool = static_cast<const char*>(second ? c.v_pages : c.k_pages) + head_at;
+  const char* k_pool = static_cast<const char*>(c.k_pages) + head_at;
   const char* v_pool = static_cast<const char*>(c.v_pages) + head_at;
-  const float* scale_of = (second || (kPools == 2 && (lane & 1)) ? c.v_scale : c.k_scale) + head;
-  const uint32_t scale_to = kStepBytes + (second || (kPools == 2 && (lane & 1)) ? 16 : 0);
-  // the step's rows in 16-byte pieces, 32 a copy: the copies of one warp are
-  // 512 bytes apart, and odd ones of 128-byte rows are turned by half a line
-  // (warps that share keys: a lane converts what it copied, in any place)
-  const uint32_t to = (shares(MODE) ? lane * 16 : swizzled<SIZE>(lane / (SIZE / 16), lane % (SIZE / 16))) +
-                      (second ? 2048 : 0);
+  const float* scale_of = (lane & 1 ? c.v_scale : c.k_scale) + head;
+  const uint32_t scale_to = kStepBytes + (lane & 1 ? 16 : 0);
+  const uint32_t to = swizzled<SIZE>(lane / (SIZE / 16), lane % (SIZE / 16));
   const uint32_t ring_at = shared_of(ring);
   uint32_t fill = ring_at;  // slot that is filled next
   auto prefetch = [&](int step) {
@@ -459,27 +304,25 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
         ids_next = ids_of(++batch + 1);
       }
 #pragma unroll
-      for (int i = 0; i < kCopies; i += kRowCopies < kCopies ? kRowCopies : kCopies) {
-        const int sub = (first_copy + i) / kRowCopies, piece = step * kSubs + sub, key = piece_key(piece);
+      for (int sub = 0; sub < kSubs; ++sub) {
+        const int piece = step * kSubs + sub, key = piece_key(piece);
         const int page = __shfl_sync(0xffffffffu, ids, piece & 31);
         const int rows = page >= 0 ? length - key : 0;  // that exist
-        const long long from = static_cast<long long>(max(page, 0)) * page_bytes + (key & (c.page - 1)) * SIZE +
-                               (first_copy + i) % kRowCopies * 512;
+        const long long from = static_cast<long long>(max(page, 0)) * page_bytes + (key & (c.page - 1)) * SIZE;
         const char *k = k_pool + from, *v = v_pool + from;
 #pragma unroll
-        for (int n = 0; n < kRowCopies && n < kCopies; ++n) {
-          const int at = first_copy + i + n;
-          const uint32_t dst = fill + ((SIZE == 128 && !shares(MODE) && (n & 1) ? to ^ 64 : to) + at * 512);
+        for (int n = 0; n < kRowCopies; ++n) {
+          const uint32_t dst = fill + ((SIZE == 128 && (n & 1) ? to ^ 64 : to) + (sub * kRowCopies + n) * 512);
           if (rows >= 16) {
             copy16(dst, k + n * 512);
-            if (kPools == 2) copy16(dst + 2048, v + n * 512);
+            copy16(dst + 2048, v + n * 512);
           } else {
-            const bool real = (at % kRowCopies * 512 + lane * 16) / SIZE < rows;
+            const bool real = (n * 512 + lane * 16) / SIZE < rows;
             copy16(dst, k + n * 512, real);
-            if (kPools == 2) copy16(dst + 2048, v + n * 512, real);
+            copy16(dst + 2048, v + n * 512, real);
           }
         }
-        if (lane < kPools && (first_copy + i) % kRowCopies == 0)
+        if (lane < 2)
           copy4(fill + scale_to + sub * 4, scale_of + static_cast<long long>(max(page, 0)) * c.kv_heads, page >= 0);
       }
     }
@@ -489,71 +332,29 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) prefetch(i);
 
-  load_queries<SIZE, STORAGE, MODE, LO>(p, query, s.row.count, head, block_row, queries, factors);
+  load_queries<SIZE, STORAGE, MODE, LO>(p, query, s.row.count, head, first_row, queries, factors);
   __syncthreads();
-  float factor[S::kHalves];
+  float factor[S::kTiles][S::kHalves];
 #pragma unroll
-  for (int half = 0; half < S::kHalves; ++half) factor[half] = factors[16 * rank + half * 8 + g];
-  queries += rank * kParts * kDots * 32 + lane;
+  for (int mt = 0; mt < S::kTiles; ++mt)
+#pragma unroll
+    for (int half = 0; half < S::kHalves; ++half) factor[mt][half] = factors[mt * 16 + half * 8 + g];
+  queries += lane;
   // where this lane reads: rows 8 n + key_of(g) of K, quad + 4 i of V.  The
   // second half of a 128-byte key row, and every other row of V, lie half a line
   // turned; the rest are constant distances.
   const int key_at = swizzled<SIZE>(key_of(g), quad * kKeyWords / 4) + quad * kKeyWords * 4 % 16;
   const int value_at = 2048 + swizzled<SIZE>(quad, element_of<SIZE>(g) / 16) + element_of<SIZE>(g) % 16;
   const char* slot = ring;
-  // the group's fp16 rows, and this lane's addresses in them for matrix loads: K
-  // rows of both 8-key tiles, 16 elements; V rows of 16 keys, two 8-element tiles
-  char* halves = shared + ring_bytes(MODE, LO) + group * kHalfBytes;
-  const uint32_t halves_at = shared_of(halves);
   for (int step = 0; step < tiles; ++step) {
     wait_groups<kStages - 2>();
-    if (step > 0) slot = slot + kSlotBytes == ring + kStages * kSlotBytes ? ring : slot + kSlotBytes;
-    if (shares(MODE)) {
-      uint32_t w[kCopies][8];
-#pragma unroll
-      for (int i = 0; i < kCopies; ++i) {
-        uint32_t raw[4];
-        read_words<4>(slot + to + (first_copy + i) * 512, raw);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) to_halves_in_order<STORAGE>(raw[k], w[i][2 * k], w[i][2 * k + 1]);
-      }
-      group_sync<MODE>(group);  // all warps are done with the step before
-#pragma unroll
-      for (int i = 0; i < kCopies; ++i) {
-        const int at = (first_copy + i) * 32 + lane, row = at / (SIZE / 16), piece = at % (SIZE / 16) * 2;
-        const bool odd = SIZE == 128 && piece >= 8;  // (the order keeps eight lanes in different banks)
-        char* base = halves + (second ? kHalfBytes / 2 : 0);
-        const uint4 lo = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]), hi = make_uint4(w[i][4], w[i][5], w[i][6], w[i][7]);
-        *reinterpret_cast<uint4*>(base + half_at<SIZE>(row, piece + (odd ? 1 : 0))) = odd ? hi : lo;
-        *reinterpret_cast<uint4*>(base + half_at<SIZE>(row, piece + (odd ? 0 : 1))) = odd ? lo : hi;
-      }
-    }
-    group_sync<MODE>(group);  // this step is complete; all warps have left the slot filled next
+    __syncwarp();  // all copies of this step have landed; all lanes have left the slot filled next
     prefetch(step + kStages - 1);
-    if (tiles_of(MODE) > 1 && first_row >= p.rows) continue;  // no such rows
+    if (step > 0) slot = slot + kSlotBytes == ring + kStages * kSlotBytes ? ring : slot + kSlotBytes;
     const int key = (tile + step) * tile_keys(SIZE) + group * kKeys;
     const float* scales = reinterpret_cast<const float*>(slot + kStepBytes);
 
-    float score[2 * kSubs][4];
-    if constexpr (shares(MODE)) {
-#pragma unroll
-      for (int dot = 0; dot < kDots; ++dot) {
-        const uint4 a = queries[dot * 32];
-        const uint32_t row[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int sub = 0; sub < kSubs; ++sub) {
-          uint32_t b[4];  // elements 0-7 and 8-15 of keys 0-7, then of keys 8-15
-          load_matrices<false>(halves_at + half_at<SIZE>(sub * 16 + (lane & 7) + (lane & 16) / 2, dot * 2 + (lane >> 3 & 1)), b);
-          if (dot == 0) {
-            mma<true>(score[2 * sub], row, b[0], b[1]);
-            mma<true>(score[2 * sub + 1], row, b[2], b[3]);
-          } else {
-            mma<false>(score[2 * sub], row, b[0], b[1]);
-            mma<false>(score[2 * sub + 1], row, b[2], b[3]);
-          }
-        }
-      }
-    } else {
+    float score[S::kTiles][2 * kSubs][4];
 #pragma unroll
     for (int r = 0; r < kKeyReads; ++r) {
       uint32_t w[2 * kSubs][kKeyWords];
@@ -563,22 +364,26 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
 #pragma unroll
       for (int k = 0; k < kKeyWords; ++k) {
         const int dot = r * kKeyWords + k;
-        uint4 a[kParts];
+        uint4 a[S::kTiles][kParts];
 #pragma unroll
-        for (int part = 0; part < kParts; ++part) a[part] = queries[(part * kDots + dot) * 32];
+        for (int mt = 0; mt < S::kTiles; ++mt)
+#pragma unroll
+          for (int part = 0; part < kParts; ++part) a[mt][part] = queries[((mt * kParts + part) * kDots + dot) * 32];
 #pragma unroll
         for (int n = 0; n < 2 * kSubs; ++n) {
           uint32_t b0, b1;
           to_halves<STORAGE>(w[n][k], b0, b1);
 #pragma unroll
-          for (int part = 0; part < kParts; ++part) {
-            const uint32_t row[4] = {a[part].x, a[part].y, a[part].z, a[part].w};
-            if (dot == 0 && part == 0) mma<true>(score[n], row, b0, b1);
-            else mma<false>(score[n], row, b0, b1);
+          for (int mt = 0; mt < S::kTiles; ++mt) {
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) {
+              const uint32_t rows[4] = {a[mt][part].x, a[mt][part].y, a[mt][part].z, a[mt][part].w};
+              if (dot == 0 && part == 0) mma<true>(score[mt][n], rows, b0, b1);
+              else mma<false>(score[mt][n], rows, b0, b1);
+            }
           }
         }
       }
-    }
     }
 
     // value scales as 2^exponent * fraction; one that is zero takes the exponent
@@ -594,16 +399,22 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
       exponent[sub] = static_cast<float>(last);
       undo[sub] = __uint_as_float(static_cast<uint32_t>(127 - last) << 23);
     }
-    uint32_t weight[kParts][kSubs][4];
+    uint32_t weight[S::kTiles][kParts][kSubs][4];
 #pragma unroll
-    for (int half = 0; half < S::kHalves; ++half) {
+    for (int at = 0; at < S::kTiles * S::kHalves; ++at) {
+      const int mt = at / S::kHalves, half = at % S::kHalves;
+      if (S::kTiles > 1 && first_row + at * 8 >= p.rows) {  // no such rows
+#pragma unroll
+        for (int n = 0; n < 2 * kSubs; ++n) weight[mt][0][n / 2][2 * (n & 1) + half] = 0u;
+        continue;
+      }
       float x[2 * kSubs][2], most = -INFINITY;
 #pragma unroll
       for (int n = 0; n < 2 * kSubs; ++n) {
-        const float f = factor[half] * scales[n / 2];
+        const float f = factor[mt][half] * scales[n / 2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float v = MODE == kPacked ? score[n][i] + score[n][2 + i] : score[n][2 * half + i];
+          const float v = MODE == kPacked ? score[mt][n][i] + score[mt][n][2 + i] : score[mt][n][2 * half + i];
           x[n][i] = fmaf(v, f, exponent[n / 2]);
         }
       }
@@ -612,7 +423,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
         for (int n = 0; n < 2 * kSubs; ++n)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            if (key + n * 8 + (shares(MODE) ? 2 * quad + i : quad + 4 * i) >= limit[half]) x[n][i] = -INFINITY;
+            if (key + n * 8 + quad + 4 * i >= limit[mt][half]) x[n][i] = -INFINITY;
       }
 #pragma unroll
       for (int n = 0; n < 2 * kSubs; ++n) most = fmaxf(most, fmaxf(x[n][0], x[n][1]));
@@ -620,209 +431,86 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
       // The sums are kept against a maximum that follows the running one only
       // when that is 2^kSlack above it, so they are rarely scaled.
-      const float old = sums.m[half];
+      const float old = sums.m[mt][half];
       if (__any_sync(0xffffffffu, most > old + kSlack)) {
         const float now = most > old + kSlack ? most : old;
         const float r = now == -INFINITY ? 1.0f : root2_of(old - now);
-        sums.m[half] = now;
-        sums.l[half] *= r * r;
+        sums.m[mt][half] = now;
+        sums.l[mt][half] *= r * r;
 #pragma unroll
         for (int j = 0; j < SIZE / 8; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (MODE == kPacked || i / 2 == half) sums.o[j][i] = sums.o[j][i] * r * r;
+            if (MODE == kPacked || i / 2 == half) sums.o[mt][j][i] = sums.o[mt][j][i] * r * r;
       }
-      const float against = sums.m[half] == -INFINITY ? 0.0f : sums.m[half];
+      const float against = sums.m[mt][half] == -INFINITY ? 0.0f : sums.m[mt][half];
 #pragma unroll
       for (int n = 0; n < 2 * kSubs; ++n) {
         const float e0 = exp2_of(x[n][0] - against), e1 = exp2_of(x[n][1] - against);
-        sums.l[half] = fmaf(e0 + e1, undo[n / 2], sums.l[half]);
+        sums.l[mt][half] = fmaf(e0 + e1, undo[n / 2], sums.l[mt][half]);
         uint32_t hi, lo;
         split(e0 * fraction[n / 2], e1 * fraction[n / 2], hi, lo);
         if (MODE == kPacked) {
-          weight[0][n / 2][2 * (n & 1)] = hi;
-          weight[0][n / 2][2 * (n & 1) + 1] = lo;
+          weight[mt][0][n / 2][2 * (n & 1)] = hi;
+          weight[mt][0][n / 2][2 * (n & 1) + 1] = lo;
         } else {
-          weight[0][n / 2][2 * (n & 1) + half] = hi;
-          if (LO) weight[kParts - 1][n / 2][2 * (n & 1) + half] = lo;
+          weight[mt][0][n / 2][2 * (n & 1) + half] = hi;
+          if (LO) weight[mt][kParts - 1][n / 2][2 * (n & 1) + half] = lo;
         }
       }
     }
 #pragma unroll
     for (int sub = 0; sub < kSubs; ++sub) {
-      if constexpr (shares(MODE)) {
+      uint32_t v[4][kValueWords];
 #pragma unroll
-        for (int j = 0; j < SIZE / 8; j += 2) {
-          uint32_t b[4];  // keys 0-7 and 8-15 of tile j, then of tile j + 1
-          load_matrices<true>(halves_at + kHalfBytes / 2 + half_at<SIZE>(sub * 16 + (lane & 15), j + (lane >> 4)), b);
-          mma<false>(sums.o[j], weight[0][sub], b[0], b[1]);
-          mma<false>(sums.o[j + 1], weight[0][sub], b[2], b[3]);
+      for (int i = 0; i < 4; ++i)  // keys of columns 2 quad, 2 quad + 1 of both 8-key tiles
+        read_words<kValueWords>(slot + (i & 1 ? value_at ^ 64 : value_at) + (sub * 16 + 4 * i) * SIZE, v[i]);
+#pragma unroll
+      for (int w = 0; w < kValueWords; ++w) {
+        uint32_t b[4][2];  // of the word's four elements: keys 0-7, keys 8-15
+#pragma unroll
+        for (int pair = 0; pair < 2; ++pair) {
+          to_halves<STORAGE>(interleave<STORAGE>(v[2 * pair][w], v[2 * pair + 1][w], 0), b[0][pair], b[1][pair]);
+          to_halves<STORAGE>(interleave<STORAGE>(v[2 * pair][w], v[2 * pair + 1][w], 1), b[2][pair], b[3][pair]);
         }
-      } else {
-        uint32_t v[4][kValueWords];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)  // keys of columns 2 quad, 2 quad + 1 of both 8-key tiles
-          read_words<kValueWords>(slot + (i & 1 ? value_at ^ 64 : value_at) + (sub * 16 + 4 * i) * SIZE, v[i]);
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int w = 0; w < kValueWords; ++w) {
-          uint32_t b[4][2];  // of the word's four elements: keys 0-7, keys 8-15
+          for (int mt = 0; mt < S::kTiles; ++mt)
 #pragma unroll
-          for (int pair = 0; pair < 2; ++pair) {
-            to_halves<STORAGE>(interleave<STORAGE>(v[2 * pair][w], v[2 * pair + 1][w], 0), b[0][pair], b[1][pair]);
-            to_halves<STORAGE>(interleave<STORAGE>(v[2 * pair][w], v[2 * pair + 1][w], 1), b[2][pair], b[3][pair]);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int part = 0; part < kParts; ++part) mma<false>(sums.o[w * 4 + i], weight[part][sub], b[i][0], b[i][1]);
-        }
+            for (int part = 0; part < kParts; ++part)
+              mma<false>(sums.o[mt][w * 4 + i], weight[mt][part][sub], b[i][0], b[i][1]);
       }
     }
   }
   wait_groups<0>();
 #pragma unroll
-  for (int half = 0; half < S::kHalves; ++half) {
-    float& l = sums.l[half];
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-  }
-}
-
-// Where row r of an item goes; r past the item's rows: nowhere.
-template <int SIZE>
-__device__ __forceinline__ long long out_row(const Plan& p, long long b, int head, int r) {
-  return ((b * p.a.tokens + r / p.group) * p.a.heads + head * p.group + r % p.group) * SIZE;
-}
-__device__ __forceinline__ void store4(const Plan& p, long long at, const float* v) {
-  if (p.a.dtype == CB_F32) {
-    *reinterpret_cast<float4*>(static_cast<float*>(p.a.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
-  } else {
-    uint2 w;
-    if (p.a.dtype == CB_BF16) {
-      __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
-      w = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
-    } else {
-      w = make_uint2(bits(__floats2half2_rn(v[0], v[1])), bits(__floats2half2_rn(v[2], v[3])));
+  for (int mt = 0; mt < S::kTiles; ++mt)
+#pragma unroll
+    for (int half = 0; half < S::kHalves; ++half) {
+      float& l = sums.l[mt][half];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
     }
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.a.out) + at) = w;
-  }
-}
-
-// Partial results: maxima and sums of the rows, then the rows.
-template <int SIZE, int MODE>
-__host__ __device__ constexpr int partial_floats() { return rows_of(MODE) * (SIZE + 2); }
-
-// An item that a cut divided: its first part, then the first partial results of
-// the following blocks (`rest` + 2 k of them), in that order.
-template <int SIZE, int MODE>
-__device__ __noinline__ void join(const Plan& p, long long b, int head, int first_row, int count, int parts,
-                                     const float* first, const float* rest) {
-  constexpr int kRows = rows_of(MODE), kFloats = partial_floats<SIZE, MODE>();
-  for (int i = threadIdx.x; i < kRows * SIZE / 4; i += threads_of(MODE)) {
-    const int r = i / (SIZE / 4), d = i % (SIZE / 4) * 4, row = first_row + r;
-    if (row >= p.rows) continue;
-    float top = -INFINITY, sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int kBatch = 8;  // parts whose loads are in flight together
-    for (int from = 0; from < parts; from += kBatch) {
-      float m[kBatch], l[kBatch], now = top;
-      float4 x[kBatch];
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int at = from + k;
-        const float* part = at ? rest + 2LL * at * kFloats : first;
-        m[k] = at < parts ? __ldcg(part + r) : -INFINITY;
-        l[k] = at < parts ? __ldcg(part + kRows + r) : 0.0f;
-        x[k] = at < parts ? __ldcg(reinterpret_cast<const float4*>(part + 2 * kRows + r * SIZE + d))
-                          : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      }
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) now = fmaxf(now, m[k]);
-      const float keep = top == -INFINITY ? 0.0f : root2_of(top - now);
-      sum = sum * keep * keep;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = v[i] * keep * keep;
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const float f = m[k] == -INFINITY ? 0.0f : root2_of(m[k] - now);
-        sum += f * l[k] * f;
-        v[0] += f * x[k].x * f; v[1] += f * x[k].y * f; v[2] += f * x[k].z * f; v[3] += f * x[k].w * f;
-      }
-      top = now;
-    }
-    const bool real = row / p.group < count && sum != 0.0f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = real ? v[k] / sum : 0.0f;
-    store4(p, out_row<SIZE>(p, b, head, row) + d, v);
-  }
 }
 
 template <int SIZE, int STORAGE, int MODE, int LO>
-__global__ void __launch_bounds__(threads_of(MODE), resident_of(MODE, LO)) attention_kernel(const __grid_constant__ Plan p) {
+__global__ void __launch_bounds__(kThreads, resident_of(MODE, LO)) attention_kernel(const __grid_constant__ Plan p) {
   using S = Sums<SIZE, MODE>;
-  constexpr int kRows = rows_of(MODE), kThreads = threads_of(MODE);
+  constexpr int kRows = rows_of(MODE);
   extern __shared__ __align__(128) char shared[];
-  __shared__ int scan[warps_of(MODE)], found[5];
+  __shared__ int scan[kGroups], found[5];
   __shared__ float most[kGroups][kRows], total[kGroups][kRows], factors[kRows];
-  const int batch = static_cast<int>(p.a.batch), items = p.a.cache.kv_heads * p.blocks;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = warp % kGroups, rank = warp / kGroups;
+  const int group = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   pdl_launch_dependents();
   pdl_wait();
-  // the tiles of all slots, and this block's range of them
-  Slot s;
-  s.tiles = -kItemCost;
-  int mine = 0, all;
-  for (int b = batch - 1 - (batch - 1 - static_cast<int>(threadIdx.x)) % kThreads; b >= 0 && b < batch; b -= kThreads) {
-    s = slot_of<SIZE>(p, b);  // (slot threadIdx.x last)
-    mine += s.tiles + kItemCost;
-  }
-  block_scan<MODE>(mine, scan, &all);
-  all *= items;
-  const int per = (all + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
-  const int range = per * static_cast<int>(blockIdx.x), end = min(range + per, all);
-  if (range >= end) return;
-  int before = 0;
-  for (int first = 0; first < batch; first += kThreads) {
-    const int b = first + static_cast<int>(threadIdx.x);
-    if (first > 0) {
-      if (b < batch) s = slot_of<SIZE>(p, b);
-      else s.tiles = -kItemCost;
-    }
-    const int units = (s.tiles + kItemCost) * items;
-    int sum;
-    const int lower = before + block_scan<MODE>(units, scan, &sum);
-    if (lower <= range && range < lower + units) {
-      found[0] = b;
-      found[1] = lower;
-      found[2] = static_cast<int>((s.row.table - p.a.cache.table) / p.a.cache.columns);
-      found[3] = s.row.length;
-      found[4] = s.row.count;
-    }
-    before += sum;
-    if (before > range) break;
-  }
-  __syncthreads();
-  int b = found[0], origin = found[1], at = range;
-  s.row.table = p.a.cache.table + found[2] * p.a.cache.columns;
-  s.row.length = found[3];
-  s.row.count = found[4];
-  s.tiles = tiles_of_slot<SIZE>(s.row);
-
-  while (at < end) {
-    int span = s.tiles + kItemCost;
-    if (at - origin >= span * items) {
-      origin += span * items;
-      s = slot_of<SIZE>(p, ++b);
-      span = s.tiles + kItemCost;
-    }
-    const int item = (at - origin) / span, item_at = origin + item * span;  // its cost, then its tiles
-    const bool small = span <= kSmallItem;  // belongs to the block in whose range it begins
-    const int tile = max(0, at - item_at - kItemCost);
-    const int tiles = small ? (at == item_at ? s.tiles : 0) : max(0, min(end - item_at, span) - kItemCost) - tile;
-    at = item_at + span;
-    if (tiles <= 0) continue;
-    const int head = item / p.blocks, first_row = item % p.blocks * kRows;
-    if (s.row.count == 0) {  // no rows: zeros, and no keys to read
+  Walk<tile_keys(SIZE)> walk;
+  if (!begin_walk<tile_keys(SIZE), kGroups>(p, scan, found, &walk)) return;
+  Segment seg;
+  while (walk.next(p, &seg)) {
+    const int b = seg.b, head = seg.item / p.blocks, first_row = seg.item % p.blocks * kRows;
+    if (seg.empty) {
       for (int i = threadIdx.x; i < kRows * SIZE / 4; i += kThreads) {
         const int row = first_row + i / (SIZE / 4);
         const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -832,41 +520,33 @@ __global__ void __launch_bounds__(threads_of(MODE), resident_of(MODE, LO)) atten
     }
     Sums<SIZE, MODE> sums;
     const void* query = static_cast<const char*>(p.a.q) + static_cast<long long>(b) * p.a.q_strides[0] * (p.a.dtype == CB_F32 ? 4 : 2);
-    warp_item<SIZE, STORAGE, MODE, LO>(p, query, s, head, first_row, tile, tiles, shared, factors, sums);
+    warp_item<SIZE, STORAGE, MODE, LO>(p, query, seg.s, head, first_row, seg.tile, seg.tiles, shared, factors, sums);
 
     // join the groups
     __syncthreads();  // every warp is done with the ring
-    float* rows = reinterpret_cast<float*>(shared);  // (groups, kRows, SIZE)
+    float* rows = reinterpret_cast<float*>(shared);  // (groups, kRows, kPitch)
+    constexpr int kPitch = SIZE + 8;                 // (rows begin in different banks)
 #pragma unroll
-    for (int half = 0; half < S::kHalves; ++half) {
-      const int r = rank * 16 + half * 8 + (lane >> 2);
+    for (int at = 0; at < S::kTiles * S::kHalves; ++at) {
+      const int mt = at / S::kHalves, half = at % S::kHalves, r = at * 8 + (lane >> 2);
       if ((lane & 3) == 0) {
-        most[group][r] = sums.m[half];
-        total[group][r] = sums.l[half];
+        most[group][r] = sums.m[mt][half];
+        total[group][r] = sums.l[mt][half];
       }
-      if constexpr (shares(MODE)) {  // columns 2 c and 2 c + 1 of tile j are those elements
-        float* to = rows + (group * kRows + r) * SIZE + 2 * (lane & 3);
 #pragma unroll
-        for (int j = 0; j < SIZE / 8; ++j)
-          *reinterpret_cast<float2*>(to + 8 * j) = make_float2(sums.o[j][2 * half], sums.o[j][2 * half + 1]);
-      } else {
+      for (int n = 0; n < 2; ++n) {
+        float* to = rows + (group * kRows + r) * kPitch + element_of<SIZE>(2 * (lane & 3) + n);
+        auto value = [&](int j) {
+          const float* o = sums.o[mt][j];
+          return MODE == kPacked ? o[n] + o[2 + n] : o[2 * half + n];
+        };
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          float* to = rows + (group * kRows + r) * SIZE + element_of<SIZE>(2 * (lane & 3) + n);
-          auto value = [&](int j) {
-            const float* o = sums.o[j];
-            return MODE == kPacked ? o[n] + o[2 + n] : o[2 * half + n];
-          };
-#pragma unroll
-          for (int j = 0; j < SIZE / 8; j += 4)
-            *reinterpret_cast<float4*>(to + j) = make_float4(value(j), value(j + 1), value(j + 2), value(j + 3));
-        }
+        for (int j = 0; j < SIZE / 8; j += 4)
+          *reinterpret_cast<float4*>(to + j) = make_float4(value(j), value(j + 1), value(j + 2), value(j + 3));
       }
     }
     __syncthreads();
-    const bool whole = tile == 0 && tiles == s.tiles;
-    const bool begins = item_at + kItemCost <= range;  // the item of the range's first tile: the first partial result
-    float* partial = p.partial + (2LL * blockIdx.x + (begins ? 0 : 1)) * partial_floats<SIZE, MODE>();
+    float* partial = part_of<SIZE, kRows>(p, blockIdx.x, seg.begins);
     for (int i = threadIdx.x; i < kRows * SIZE / 4; i += kThreads) {
       const int r = i / (SIZE / 4), d = i % (SIZE / 4) * 4;
       float top = -INFINITY, sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -875,14 +555,14 @@ __global__ void __launch_bounds__(threads_of(MODE), resident_of(MODE, LO)) atten
 #pragma unroll
       for (int w = 0; w < kGroups; ++w) {
         const float f = most[w][r] == -INFINITY ? 0.0f : root2_of(most[w][r] - top);
-        const float4 x = *reinterpret_cast<const float4*>(rows + (w * kRows + r) * SIZE + d);
+        const float4 x = *reinterpret_cast<const float4*>(rows + (w * kRows + r) * kPitch + d);
         sum += f * total[w][r] * f;
         v[0] += f * x.x * f; v[1] += f * x.y * f; v[2] += f * x.z * f; v[3] += f * x.w * f;
       }
       const int row = first_row + r;
-      if (whole) {
+      if (seg.whole) {
         if (row < p.rows) {
-          const bool real = row / p.group < s.row.count && sum != 0.0f;
+          const bool real = row / p.group < seg.s.row.count && sum != 0.0f;
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[k] = real ? v[k] / sum : 0.0f;
           store4(p, out_row<SIZE>(p, b, head, row) + d, v);
@@ -895,21 +575,14 @@ __global__ void __launch_bounds__(threads_of(MODE), resident_of(MODE, LO)) atten
         }
       }
     }
-    if (!whole) {
-      const int from = (item_at + kItemCost) / per, last = (item_at + span - 1) / per;  // blocks of its tiles
+    if (!seg.whole) {
       __syncthreads();
-      if (threadIdx.x == 0) {
-        const bool all_there = ticket_acq_rel(p.arrived + from) == static_cast<unsigned>(last - from);
-        if (all_there) p.arrived[from] = 0;
-        found[0] = all_there;
-      }
+      if (threadIdx.x == 0) found[0] = last_part(p, seg);
       __syncthreads();
-      if (found[0]) {
-        const int own = item_at + kItemCost <= from * per ? 0 : 1;  // the first part's place
-        join<SIZE, MODE>(p, b, head, first_row, s.row.count, last - from + 1,
-                         p.partial + (2LL * from + own) * partial_floats<SIZE, MODE>(),
-                         p.partial + 2LL * from * partial_floats<SIZE, MODE>());
-      }
+      if (found[0])  // (its first part is the first of its block's range, or the second)
+        join<SIZE, kRows>(p, b, head, first_row, seg.s.row.count, seg.last - seg.from + 1,
+                          part_of<SIZE, kRows>(p, seg.from, seg.from_begins), part_of<SIZE, kRows>(p, seg.from, true),
+                          threadIdx.x, kThreads);
     }
     __syncthreads();  // the joined rows are read; the ring is free again
   }
@@ -939,7 +612,7 @@ int resident_blocks() {
     auto kernel = attention_kernel<SIZE, STORAGE, MODE, LO>;
     constexpr int kShared = shared_bytes(SIZE, MODE, LO);
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads_of(MODE), kShared) != cudaSuccess)
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, kShared) != cudaSuccess)
       per_sm = 0;
     device = per_sm > 0 ? now : -1;
   }
@@ -947,8 +620,8 @@ int resident_blocks() {
 }
 
 // Calls f with the template arguments of a launch: by the rows of a kv head 8
-// in one tile, or one, two or four 16-row tiles; float32 queries with their
-// low parts, in single tiles.
+// in one tile, 16, or blocks of 32; float32 queries of more than 8 rows with
+// their low parts, in blocks of 16.
 template <typename F>
 long long with_variant(const cb_paged_attention_args& a, F f) {
   const long long rows = a.tokens * (a.heads / a.cache.kv_heads);
@@ -957,9 +630,7 @@ long long with_variant(const cb_paged_attention_args& a, F f) {
     const auto one = std::integral_constant<int, 1>{};
     if (rows <= 8) return f(size, storage, zero, zero);
     if (a.dtype == CB_F32) return f(size, storage, one, one);
-    if (rows <= 16) return f(size, storage, one, zero);
-    if (rows <= 32) return f(size, storage, std::integral_constant<int, 2>{}, zero);
-    return f(size, storage, std::integral_constant<int, 4>{}, zero);
+    return rows <= 16 ? f(size, storage, one, zero) : f(size, storage, std::integral_constant<int, 2>{}, zero);
   };
   auto by_storage = [&](auto size) {
     return a.cache.storage == CB_I8 ? by_rows(size, std::integral_constant<int, CB_I8>{})
@@ -968,19 +639,6 @@ long long with_variant(const cb_paged_attention_args& a, F f) {
   if (a.cache.head_size == 32) return by_storage(std::integral_constant<int, 32>{});
   if (a.cache.head_size == 64) return by_storage(std::integral_constant<int, 64>{});
   return by_storage(std::integral_constant<int, 128>{});
-}
-
-// Blocks that fill the GPU once, and no more than there can be tiles.
-template <int SIZE, int MODE>
-long long grid_of(const cb_paged_attention_args& a, int per_sm) {
-  const long long rows = a.tokens * (a.heads / a.cache.kv_heads);
-  const long long blocks = (rows + rows_of(MODE) - 1) / rows_of(MODE);
-  const long long tiles = (a.cache.columns * a.cache.page + tile_keys(SIZE) - 1) / tile_keys(SIZE);
-  // in units of tiles; what a launch can have to divide is below 2^31 of them
-  const double most = static_cast<double>(a.batch) * a.cache.kv_heads * blocks * (tiles + kItemCost);
-  const long long fill = 1LL * per_sm * sm_count();
-  if (most >= 2147483648.0) return 0;
-  return most < fill ? static_cast<long long>(most) : fill;
 }
 
 }  // namespace
@@ -994,7 +652,8 @@ long long cb_paged_attention_scratch(const cb_paged_attention_args* args) {
   if (args == nullptr || attention_check(*args) != CB_OK || args->batch == 0 || args->tokens == 0) return 0;
   return with_variant(*args, [&](auto size, auto storage, auto mode, auto lo) -> long long {
     const int per_sm = resident_blocks<size.value, storage.value, mode.value, lo.value>();
-    return grid_of<size.value, mode.value>(*args, per_sm) * 8LL * partial_floats<size.value, mode.value>();
+    return grid_of(*args, rows_of(mode.value), tile_keys(size.value), per_sm) * 8LL *
+           partial_floats(size.value, rows_of(mode.value));
   });
 }
 
@@ -1016,20 +675,11 @@ int cb_paged_attention(const cb_paged_attention_args* args, void* scratch, unsig
     constexpr int SIZE = size.value, STORAGE = storage.value, MODE = mode.value, LO = lo.value;
     const int per_sm = resident_blocks<SIZE, STORAGE, MODE, LO>();
     CB_REQUIRE(per_sm >= 1 && per_sm <= 8, "cb_paged_attention: %d blocks of the kernel fit an SM", per_sm);
-    const long long grid = grid_of<SIZE, MODE>(a, per_sm);
+    const long long grid = grid_of(a, rows_of(MODE), tile_keys(SIZE), per_sm);
     CB_REQUIRE(grid > 0, "cb_paged_attention: %lld rows of up to %lld keys are too many for one call",
                a.batch * a.heads * a.tokens, a.cache.columns * a.cache.page);
-    Plan p;
-    p.a = a;
-    p.group = static_cast<int>(a.heads / a.cache.kv_heads);
-    p.rows = static_cast<int>(a.tokens * p.group);
-    p.blocks = (p.rows + rows_of(MODE) - 1) / rows_of(MODE);
-    const int item = a.dtype == CB_F32 ? 4 : 2;
-    p.wide = reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
-    for (int i = 0; i < 3; ++i) p.wide = p.wide && a.q_strides[i] * item % 16 == 0;
-    p.partial = static_cast<float*>(scratch);
-    p.arrived = counters;
-    launch(attention_kernel<SIZE, STORAGE, MODE, LO>, dim3(static_cast<unsigned>(grid)), dim3(threads_of(MODE)),
+    const Plan p = plan_of(a, rows_of(MODE), scratch, counters);
+    launch(attention_kernel<SIZE, STORAGE, MODE, LO>, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
            shared_bytes(SIZE, MODE, LO), static_cast<cudaStream_t>(stream), true, p);
     return check_launch("cb_paged_attention");
   }));
