@@ -399,41 +399,49 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
       exponent[sub] = static_cast<float>(last);
       undo[sub] = __uint_as_float(static_cast<uint32_t>(127 - last) << 23);
     }
-    uint32_t weight[S::kTiles][kParts][kSubs][4];
+    // the rows' scores and their maxima; rows of a tile that do not exist are
+    // never above theirs
+    constexpr int kRowSets = S::kTiles * S::kHalves;
+    float x[kRowSets][2 * kSubs][2], most[kRowSets];
+    bool grows = false;
 #pragma unroll
-    for (int at = 0; at < S::kTiles * S::kHalves; ++at) {
+    for (int at = 0; at < kRowSets; ++at) {
       const int mt = at / S::kHalves, half = at % S::kHalves;
-      if (S::kTiles > 1 && first_row + at * 8 >= p.rows) {  // no such rows
-#pragma unroll
-        for (int n = 0; n < 2 * kSubs; ++n) weight[mt][0][n / 2][2 * (n & 1) + half] = 0u;
-        continue;
-      }
-      float x[2 * kSubs][2], most = -INFINITY;
+      most[at] = -INFINITY;
 #pragma unroll
       for (int n = 0; n < 2 * kSubs; ++n) {
         const float f = factor[mt][half] * scales[n / 2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float v = MODE == kPacked ? score[mt][n][i] + score[mt][n][2 + i] : score[mt][n][2 * half + i];
-          x[n][i] = fmaf(v, f, exponent[n / 2]);
+          x[at][n][i] = fmaf(v, f, exponent[n / 2]);
         }
       }
-      if (key + kKeys > common) {  // (the same for the warp) columns 2 quad and 2 quad + 1
+    }
+    if (key + kKeys > common) {  // (the same for the warp) columns 2 quad and 2 quad + 1
+#pragma unroll
+      for (int at = 0; at < kRowSets; ++at)
 #pragma unroll
         for (int n = 0; n < 2 * kSubs; ++n)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            if (key + n * 8 + quad + 4 * i >= limit[mt][half]) x[n][i] = -INFINITY;
-      }
+            if (key + n * 8 + quad + 4 * i >= limit[at / S::kHalves][at % S::kHalves]) x[at][n][i] = -INFINITY;
+    }
 #pragma unroll
-      for (int n = 0; n < 2 * kSubs; ++n) most = fmaxf(most, fmaxf(x[n][0], x[n][1]));
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      // The sums are kept against a maximum that follows the running one only
-      // when that is 2^kSlack above it, so they are rarely scaled.
-      const float old = sums.m[mt][half];
-      if (__any_sync(0xffffffffu, most > old + kSlack)) {
-        const float now = most > old + kSlack ? most : old;
+    for (int at = 0; at < kRowSets; ++at) {
+#pragma unroll
+      for (int n = 0; n < 2 * kSubs; ++n) most[at] = fmaxf(most[at], fmaxf(x[at][n][0], x[at][n][1]));
+      most[at] = fmaxf(most[at], __shfl_xor_sync(0xffffffffu, most[at], 1));
+      most[at] = fmaxf(most[at], __shfl_xor_sync(0xffffffffu, most[at], 2));
+      grows = grows || most[at] > sums.m[at / S::kHalves][at % S::kHalves] + kSlack;
+    }
+    // The sums are kept against a maximum that follows the running one only
+    // when that is 2^kSlack above it, so they are rarely scaled.
+    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+      for (int at = 0; at < kRowSets; ++at) {
+        const int mt = at / S::kHalves, half = at % S::kHalves;
+        const float old = sums.m[mt][half], now = most[at] > old + kSlack ? most[at] : old;
         const float r = now == -INFINITY ? 1.0f : root2_of(old - now);
         sums.m[mt][half] = now;
         sums.l[mt][half] *= r * r;
@@ -443,10 +451,15 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
           for (int i = 0; i < 4; ++i)
             if (MODE == kPacked || i / 2 == half) sums.o[mt][j][i] = sums.o[mt][j][i] * r * r;
       }
+    }
+    uint32_t weight[S::kTiles][kParts][kSubs][4];
+#pragma unroll
+    for (int at = 0; at < kRowSets; ++at) {
+      const int mt = at / S::kHalves, half = at % S::kHalves;
       const float against = sums.m[mt][half] == -INFINITY ? 0.0f : sums.m[mt][half];
 #pragma unroll
       for (int n = 0; n < 2 * kSubs; ++n) {
-        const float e0 = exp2_of(x[n][0] - against), e1 = exp2_of(x[n][1] - against);
+        const float e0 = exp2_of(x[at][n][0] - against), e1 = exp2_of(x[at][n][1] - against);
         sums.l[mt][half] = fmaf(e0 + e1, undo[n / 2], sums.l[mt][half]);
         uint32_t hi, lo;
         split(e0 * fraction[n / 2], e1 * fraction[n / 2], hi, lo);
