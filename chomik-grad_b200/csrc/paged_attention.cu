@@ -22,9 +22,9 @@
 //   - what multiplies the value codes is the weight exp(s_j - m) times the
 //     page's value scale: the running maximum m is that of the scores plus the
 //     scales' exponents, so that these products stay within fp16 whatever the
-//     scales, and they are split the same way (16-bit outputs of more than 8
-//     rows: hi only, a relative error of 2^-12 a weight, below the output's own
-//     rounding).  The sum of the weights leaves the scale out again.
+//     scales, and they are split the same way (bfloat16 outputs of more than 8
+//     rows: hi only, a relative error of 2^-12 a weight, a sixteenth of the
+//     output's own rounding).  The sum of the weights leaves the scale out again.
 //
 // How the work is laid out.  The keys of all (slot, kv head, block of rows)
 // are one sequence of tiles, cut into equal ranges for a grid that fills the
@@ -53,21 +53,24 @@ constexpr int kSlotBytes = kStepBytes + kHeadBytes;
 // How the query rows fill the tensor core's 16-row tiles: 8 of them with both
 // parts in one tile, or MODE tiles of 16.
 enum { kPacked = 0 };
+// Low parts of unpacked rows: none (bfloat16), of queries and weights (float32),
+// of the weights alone (float16, whose queries are exact).
+enum { kNoParts = 0, kBothParts = 1, kWeightParts = 2 };
 __host__ __device__ constexpr int tiles_of_mode(int mode) { return mode == kPacked ? 1 : mode; }
 __host__ __device__ constexpr int rows_of(int mode) { return mode == kPacked ? 8 : 16 * mode; }
 constexpr int kThreads = 32 * kGroups;
 // Resident blocks of an SM: 16 warps of 128 registers, with the low parts of
 // float32 queries 12 of 168, with two tiles' sums 8 of 255.  The steps of a
 // warp's ring then follow from shared memory.
-__host__ __device__ constexpr int resident_of(int mode, int lo) { return mode == 2 ? 2 : lo ? 3 : 4; }
-__host__ __device__ constexpr int stages_of(int mode, int lo) { return mode == 2 ? 5 : lo ? 4 : 3; }
+__host__ __device__ constexpr int resident_of(int mode, int lo) { return mode == 2 ? 2 : lo == kBothParts ? 3 : 4; }
+__host__ __device__ constexpr int stages_of(int mode, int lo) { return mode == 2 ? 5 : lo == kBothParts ? 4 : 3; }
 __host__ __device__ constexpr int ring_bytes(int mode, int lo) { return kGroups * stages_of(mode, lo) * kSlotBytes; }
 __host__ __device__ constexpr int step_keys(int head_size) { return 2048 / head_size; }
 __host__ __device__ constexpr int tile_keys(int head_size) { return kGroups * step_keys(head_size); }
 
 // Shared memory of a block: the ring, and the queries as the products read them.
 __host__ __device__ constexpr int shared_bytes(int head_size, int mode, int lo) {
-  return ring_bytes(mode, lo) + tiles_of_mode(mode) * (lo ? 2 : 1) * (head_size / 16) * 512;
+  return ring_bytes(mode, lo) + tiles_of_mode(mode) * (lo == kBothParts ? 2 : 1) * (head_size / 16) * 512;
 }
 
 // ---- loads -------------------------------------------------------------------
@@ -191,7 +194,7 @@ struct Sums {
 template <int SIZE, int STORAGE, int MODE, int LO>
 __device__ __forceinline__ void load_queries(const Plan& p, const void* query, int count, int head, int first_row,
                                              uint4* queries, float* factors) {
-  constexpr int kLanes = SIZE / 8, kDots = SIZE / 16, kParts = LO ? 2 : 1;
+  constexpr int kLanes = SIZE / 8, kDots = SIZE / 16, kParts = LO == kBothParts ? 2 : 1;
   constexpr int kKeyWords = SIZE / 16 < 4 ? SIZE / 16 : 4;
 #pragma unroll
   for (int first = 0; first < rows_of(MODE); first += kThreads / kLanes) {
@@ -225,7 +228,7 @@ __device__ __forceinline__ void load_queries(const Plan& p, const void* query, i
           to[2 * pair + 1] = lo;
         } else {
           to[2 * pair + row / 8 % 2] = hi;
-          if (LO) to[kDots * 128 + 2 * pair + row / 8 % 2] = lo;
+          if (LO == kBothParts) to[kDots * 128 + 2 * pair + row / 8 % 2] = lo;
         }
       }
     }
@@ -242,7 +245,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
   constexpr int kKeyWords = SIZE / 16 < 4 ? SIZE / 16 : 4;  // words of one read of a key row
   constexpr int kKeyReads = SIZE / 16 / kKeyWords;
   constexpr int kValueWords = SIZE / 32;
-  constexpr int kParts = LO ? 2 : 1;
+  constexpr int kParts = LO == kBothParts ? 2 : 1, kWeights = LO ? 2 : 1;  // parts of queries, of weights
   const cb_paged_cache& c = p.a.cache;
   const int group = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
   char* ring = shared + group * kStages * kSlotBytes;
@@ -452,7 +455,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
             if (MODE == kPacked || i / 2 == half) sums.o[mt][j][i] = sums.o[mt][j][i] * r * r;
       }
     }
-    uint32_t weight[S::kTiles][kParts][kSubs][4];
+    uint32_t weight[S::kTiles][kWeights][kSubs][4];
 #pragma unroll
     for (int at = 0; at < kRowSets; ++at) {
       const int mt = at / S::kHalves, half = at % S::kHalves;
@@ -468,7 +471,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
           weight[mt][0][n / 2][2 * (n & 1) + 1] = lo;
         } else {
           weight[mt][0][n / 2][2 * (n & 1) + half] = hi;
-          if (LO) weight[mt][kParts - 1][n / 2][2 * (n & 1) + half] = lo;
+          if (LO) weight[mt][kWeights - 1][n / 2][2 * (n & 1) + half] = lo;
         }
       }
     }
@@ -491,7 +494,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
 #pragma unroll
           for (int mt = 0; mt < S::kTiles; ++mt)
 #pragma unroll
-            for (int part = 0; part < kParts; ++part)
+            for (int part = 0; part < kWeights; ++part)
               mma<false>(sums.o[mt][w * 4 + i], weight[mt][part][sub], b[i][0], b[i][1]);
       }
     }
@@ -639,11 +642,15 @@ template <typename F>
 long long with_variant(const cb_paged_attention_args& a, F f) {
   const long long rows = a.tokens * (a.heads / a.cache.kv_heads);
   auto by_rows = [&](auto size, auto storage) {
-    const auto zero = std::integral_constant<int, 0>{};
     const auto one = std::integral_constant<int, 1>{};
-    if (rows <= 8) return f(size, storage, zero, zero);
-    if (a.dtype == CB_F32) return f(size, storage, one, one);
-    return rows <= 16 ? f(size, storage, one, zero) : f(size, storage, std::integral_constant<int, 2>{}, zero);
+    const auto none = std::integral_constant<int, kNoParts>{};
+    if (rows <= 8) return f(size, storage, std::integral_constant<int, kPacked>{}, none);
+    if (a.dtype == CB_F32) return f(size, storage, one, std::integral_constant<int, kBothParts>{});
+    auto by_type = [&](auto mode) {
+      return a.dtype == CB_F16 ? f(size, storage, mode, std::integral_constant<int, kWeightParts>{})
+                               : f(size, storage, mode, none);
+    };
+    return rows <= 16 ? by_type(one) : by_type(std::integral_constant<int, 2>{});
   };
   auto by_storage = [&](auto size) {
     return a.cache.storage == CB_I8 ? by_rows(size, std::integral_constant<int, CB_I8>{})
