@@ -48,8 +48,8 @@ def verify(target: Any, draft: Any, tokens: Any, uniforms: Any, *, counts: Any =
     if known is None:
         known = _VERIFY_ARGS[key] = _prepare(target, draft, tokens, uniforms, counts, error_flag)
     stream = current_stream(target.device)
-    emitted = uniforms.new_empty(uniforms.shape, dtype=torch.int64)
-    accepted = uniforms.new_empty(uniforms.shape[0], dtype=torch.int32)
+    emitted = torch.empty_like(uniforms, dtype=torch.int64)
+    accepted = torch.empty(target.shape[0], dtype=torch.int32, device=target.device)
     a = _lib.VerifyArgs.from_buffer_copy(known)
     a.target, a.draft, a.drafted, a.uniforms = (target.data_ptr(), draft.data_ptr(), tokens.data_ptr(),
                                                 uniforms.data_ptr())
