@@ -50,20 +50,24 @@ constexpr int kStepBytes = 4096;                 // K and V of a group's step
 constexpr int kHeadBytes = 64;                   // its scales: 4 of K, 4 of V
 constexpr int kSlotBytes = kStepBytes + kHeadBytes;
 
-// How the query rows fill the tensor core's 16-row tiles: 8 of them with both
-// parts in one tile, or MODE tiles of 16.
-enum { kPacked = 0 };
+// MODE is the number of 8-row sets that a block takes: one set with both parts
+// in one 16-row tile of the scores' products, or two to four, two to a tile.
+enum { kPacked = 1 };
 // Low parts of unpacked rows: none (bfloat16), of queries and weights (float32),
 // of the weights alone (float16, whose queries are exact).
 enum { kNoParts = 0, kBothParts = 1, kWeightParts = 2 };
-__host__ __device__ constexpr int tiles_of_mode(int mode) { return mode == kPacked ? 1 : mode; }
-__host__ __device__ constexpr int rows_of(int mode) { return mode == kPacked ? 8 : 16 * mode; }
+__host__ __device__ constexpr int tiles_of_mode(int mode) { return (mode + 1) / 2; }
+__host__ __device__ constexpr int rows_of(int mode) { return 8 * mode; }
 constexpr int kThreads = 32 * kGroups;
-// Resident blocks of an SM: 16 warps of 128 registers, with the low parts of
-// float32 queries 12 of 168, with two tiles' sums 8 of 255.  The steps of a
-// warp's ring then follow from shared memory.
-__host__ __device__ constexpr int resident_of(int mode, int lo) { return mode == 2 ? 2 : lo == kBothParts ? 3 : 4; }
-__host__ __device__ constexpr int stages_of(int mode, int lo) { return mode == 2 ? 5 : lo == kBothParts ? 4 : 3; }
+// Resident blocks of an SM: 16 warps of 128 registers; with the low parts of
+// float32 queries or three sets' sums 12 of 168, with four sets' 8 of 255.  The
+// steps of a warp's ring then follow from shared memory.
+__host__ __device__ constexpr int resident_of(int mode, int lo) {
+  return mode == 4 ? 2 : mode == 3 || lo == kBothParts ? 3 : 4;
+}
+__host__ __device__ constexpr int stages_of(int mode, int lo) {
+  return mode == 4 ? 5 : mode == 3 || lo == kBothParts ? 4 : 3;
+}
 __host__ __device__ constexpr int ring_bytes(int mode, int lo) { return kGroups * stages_of(mode, lo) * kSlotBytes; }
 __host__ __device__ constexpr int step_keys(int head_size) { return 2048 / head_size; }
 __host__ __device__ constexpr int tile_keys(int head_size) { return kGroups * step_keys(head_size); }
@@ -178,13 +182,17 @@ __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, ui
 
 // ---- one item ------------------------------------------------------------------
 
-// The sums of one warp: its rows g (and g + 8 of a 16-row tile), columns 2c and
-// 2c + 1 of each value tile, g = lane / 4, c = lane % 4.
+// The sums of one warp, g = lane / 4, c = lane % 4.  The maximum and the sum of
+// the weights are those of row g of each 8-row set.  The weighted values are
+// computed transposed, value elements as the products' 16 rows and the set as
+// their 8 columns: no row of a product is wasted, and the weights are its second
+// operand as the scores' products leave them.  o[set][j] holds elements 2 j (the
+// first two) and 2 j + 1 of column element_of(g), for rows 2 c and 2 c + 1.
 template <int SIZE, int MODE>
 struct Sums {
-  static constexpr int kTiles = tiles_of_mode(MODE), kHalves = MODE == kPacked ? 1 : 2;
-  float o[kTiles][SIZE / 8][4];  // as the products leave them; packed: of the hi and the lo weights
-  float m[kTiles][kHalves], l[kTiles][kHalves];
+  static constexpr int kTiles = tiles_of_mode(MODE);
+  float o[MODE][SIZE / 16][4];
+  float m[MODE], l[MODE];
 };
 
 // The block's query rows as the products read them: `queries` holds the 16-row
@@ -196,8 +204,9 @@ __device__ __forceinline__ void load_queries(const Plan& p, const void* query, i
                                              uint4* queries, float* factors) {
   constexpr int kLanes = SIZE / 8, kDots = SIZE / 16, kParts = LO == kBothParts ? 2 : 1;
   constexpr int kKeyWords = SIZE / 16 < 4 ? SIZE / 16 : 4;
+  constexpr int kAll = MODE == kPacked ? 8 : 16 * tiles_of_mode(MODE);  // rows of the operands
 #pragma unroll
-  for (int first = 0; first < rows_of(MODE); first += kThreads / kLanes) {
+  for (int first = 0; first < kAll; first += kThreads / kLanes) {
     const int row = first + static_cast<int>(threadIdx.x) / kLanes, d = static_cast<int>(threadIdx.x) % kLanes * 8;
     const int r = first_row + row, t = r / p.group;
     float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, largest = 0.0f;
@@ -207,11 +216,11 @@ __device__ __forceinline__ void load_queries(const Plan& p, const void* query, i
     for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(x[i]));
 #pragma unroll
     for (int o = 1; o < kLanes; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-    if (row >= rows_of(MODE)) continue;
+    if (row >= kAll) continue;
     // 2^e <= largest < 2^(e + 1); e in [-126, 127], and 2^-e is exact
     const int e = min(max(static_cast<int>(__float_as_uint(largest) >> 23) - 127, -126), 127);
     const float down = e == 127 ? 5.877471754111438e-39f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-    if (d == 0)
+    if (d == 0 && row < rows_of(MODE))
       factors[row] = p.a.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
     for (int word = 0; word < 2; ++word) {
@@ -245,27 +254,24 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
   constexpr int kKeyWords = SIZE / 16 < 4 ? SIZE / 16 : 4;  // words of one read of a key row
   constexpr int kKeyReads = SIZE / 16 / kKeyWords;
   constexpr int kValueWords = SIZE / 32;
-  constexpr int kParts = LO == kBothParts ? 2 : 1, kWeights = LO ? 2 : 1;  // parts of queries, of weights
+  constexpr int kParts = LO == kBothParts ? 2 : 1, kWeights = MODE == kPacked || LO ? 2 : 1;  // parts of queries, of weights
   const cb_paged_cache& c = p.a.cache;
   const int group = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
   char* ring = shared + group * kStages * kSlotBytes;
   uint4* queries = reinterpret_cast<uint4*>(shared + ring_bytes(MODE, LO));
 
   // limits: row r sees keys below limit[r]; all rows of the warp see those below `common`
-  int limit[S::kTiles][S::kHalves];
+  int limit[MODE];
 #pragma unroll
-  for (int mt = 0; mt < S::kTiles; ++mt) {
+  for (int at = 0; at < MODE; ++at) {
+    const int r = first_row + at * 8 + g, t = r / p.group;
+    limit[at] = r < p.rows && t < s.row.count ? s.row.length - s.row.count + t + 1 : 0;
+    sums.m[at] = -INFINITY;
+    sums.l[at] = 0.0f;
 #pragma unroll
-    for (int half = 0; half < S::kHalves; ++half) {
-      const int r = first_row + mt * 16 + half * 8 + g, t = r / p.group;
-      limit[mt][half] = r < p.rows && t < s.row.count ? s.row.length - s.row.count + t + 1 : 0;
-      sums.m[mt][half] = -INFINITY;
-      sums.l[mt][half] = 0.0f;
-    }
+    for (int j = 0; j < SIZE / 16; ++j)
 #pragma unroll
-    for (int j = 0; j < SIZE / 8; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sums.o[mt][j][i] = 0.0f;
+      for (int i = 0; i < 4; ++i) sums.o[at][j][i] = 0.0f;
   }
   int last = 0;  // exponent of the value scale before
   const int common = s.row.length - s.row.count + first_row / p.group + 1;
@@ -337,11 +343,9 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
 
   load_queries<SIZE, STORAGE, MODE, LO>(p, query, s.row.count, head, first_row, queries, factors);
   __syncthreads();
-  float factor[S::kTiles][S::kHalves];
+  float factor[MODE];
 #pragma unroll
-  for (int mt = 0; mt < S::kTiles; ++mt)
-#pragma unroll
-    for (int half = 0; half < S::kHalves; ++half) factor[mt][half] = factors[mt * 16 + half * 8 + g];
+  for (int at = 0; at < MODE; ++at) factor[at] = factors[at * 8 + g];
   queries += lane;
   // where this lane reads: rows 8 n + key_of(g) of K, quad + 4 i of V.  The
   // second half of a 128-byte key row, and every other row of V, lie half a line
@@ -402,77 +406,66 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
       exponent[sub] = static_cast<float>(last);
       undo[sub] = __uint_as_float(static_cast<uint32_t>(127 - last) << 23);
     }
-    // the rows' scores and their maxima; rows of a tile that do not exist are
-    // never above theirs
-    constexpr int kRowSets = S::kTiles * S::kHalves;
-    float x[kRowSets][2 * kSubs][2], most[kRowSets];
+    // the rows' scores and their maxima
+    float x[MODE][2 * kSubs][2], most[MODE];
     bool grows = false;
 #pragma unroll
-    for (int at = 0; at < kRowSets; ++at) {
-      const int mt = at / S::kHalves, half = at % S::kHalves;
-      most[at] = -INFINITY;
+    for (int at = 0; at < MODE; ++at) {
 #pragma unroll
       for (int n = 0; n < 2 * kSubs; ++n) {
-        const float f = factor[mt][half] * scales[n / 2];
+        const float f = factor[at] * scales[n / 2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float v = MODE == kPacked ? score[mt][n][i] + score[mt][n][2 + i] : score[mt][n][2 * half + i];
-          x[at][n][i] = fmaf(v, f, exponent[n / 2]);
+          const float* c = score[at / 2][n];
+          x[at][n][i] = fmaf(MODE == kPacked ? c[i] + c[2 + i] : c[at % 2 * 2 + i], f, exponent[n / 2]);
         }
       }
     }
     if (key + kKeys > common) {  // (the same for the warp) columns 2 quad and 2 quad + 1
 #pragma unroll
-      for (int at = 0; at < kRowSets; ++at)
+      for (int at = 0; at < MODE; ++at)
 #pragma unroll
         for (int n = 0; n < 2 * kSubs; ++n)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            if (key + n * 8 + quad + 4 * i >= limit[at / S::kHalves][at % S::kHalves]) x[at][n][i] = -INFINITY;
+            if (key + n * 8 + quad + 4 * i >= limit[at]) x[at][n][i] = -INFINITY;
     }
 #pragma unroll
-    for (int at = 0; at < kRowSets; ++at) {
+    for (int at = 0; at < MODE; ++at) {
+      most[at] = -INFINITY;
 #pragma unroll
       for (int n = 0; n < 2 * kSubs; ++n) most[at] = fmaxf(most[at], fmaxf(x[at][n][0], x[at][n][1]));
       most[at] = fmaxf(most[at], __shfl_xor_sync(0xffffffffu, most[at], 1));
       most[at] = fmaxf(most[at], __shfl_xor_sync(0xffffffffu, most[at], 2));
-      grows = grows || most[at] > sums.m[at / S::kHalves][at % S::kHalves] + kSlack;
+      grows = grows || most[at] > sums.m[at] + kSlack;
     }
     // The sums are kept against a maximum that follows the running one only
     // when that is 2^kSlack above it, so they are rarely scaled.
     if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-      for (int at = 0; at < kRowSets; ++at) {
-        const int mt = at / S::kHalves, half = at % S::kHalves;
-        const float old = sums.m[mt][half], now = most[at] > old + kSlack ? most[at] : old;
+      for (int at = 0; at < MODE; ++at) {
+        const float old = sums.m[at], now = most[at] > old + kSlack ? most[at] : old;
         const float r = now == -INFINITY ? 1.0f : root2_of(old - now);
-        sums.m[mt][half] = now;
-        sums.l[mt][half] *= r * r;
+        sums.m[at] = now;
+        sums.l[at] *= r * r;
+        const float r0 = __shfl_sync(0xffffffffu, r, quad * 8), r1 = __shfl_sync(0xffffffffu, r, quad * 8 + 4);
 #pragma unroll
-        for (int j = 0; j < SIZE / 8; ++j)
+        for (int j = 0; j < SIZE / 16; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (MODE == kPacked || i / 2 == half) sums.o[mt][j][i] = sums.o[mt][j][i] * r * r;
+          for (int i = 0; i < 4; ++i) sums.o[at][j][i] = sums.o[at][j][i] * (i & 1 ? r1 : r0) * (i & 1 ? r1 : r0);
       }
     }
-    uint32_t weight[S::kTiles][kWeights][kSubs][4];
+    uint32_t weight[MODE][kWeights][2 * kSubs];
 #pragma unroll
-    for (int at = 0; at < kRowSets; ++at) {
-      const int mt = at / S::kHalves, half = at % S::kHalves;
-      const float against = sums.m[mt][half] == -INFINITY ? 0.0f : sums.m[mt][half];
+    for (int at = 0; at < MODE; ++at) {
+      const float against = sums.m[at] == -INFINITY ? 0.0f : sums.m[at];
 #pragma unroll
       for (int n = 0; n < 2 * kSubs; ++n) {
         const float e0 = exp2_of(x[at][n][0] - against), e1 = exp2_of(x[at][n][1] - against);
-        sums.l[mt][half] = fmaf(e0 + e1, undo[n / 2], sums.l[mt][half]);
-        uint32_t hi, lo;
-        split(e0 * fraction[n / 2], e1 * fraction[n / 2], hi, lo);
-        if (MODE == kPacked) {
-          weight[mt][0][n / 2][2 * (n & 1)] = hi;
-          weight[mt][0][n / 2][2 * (n & 1) + 1] = lo;
-        } else {
-          weight[mt][0][n / 2][2 * (n & 1) + half] = hi;
-          if (LO) weight[mt][kWeights - 1][n / 2][2 * (n & 1) + half] = lo;
-        }
+        sums.l[at] = fmaf(e0 + e1, undo[n / 2], sums.l[at]);
+        uint32_t lo;
+        split(e0 * fraction[n / 2], e1 * fraction[n / 2], weight[at][0][n], lo);
+        if (kWeights == 2) weight[at][kWeights - 1][n] = lo;
       }
     }
 #pragma unroll
@@ -490,29 +483,27 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
           to_halves<STORAGE>(interleave<STORAGE>(v[2 * pair][w], v[2 * pair + 1][w], 1), b[2][pair], b[3][pair]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t values[4] = {b[2 * i][0], b[2 * i + 1][0], b[2 * i][1], b[2 * i + 1][1]};
 #pragma unroll
-          for (int mt = 0; mt < S::kTiles; ++mt)
+          for (int at = 0; at < MODE; ++at)
 #pragma unroll
             for (int part = 0; part < kWeights; ++part)
-              mma<false>(sums.o[mt][w * 4 + i], weight[mt][part][sub], b[i][0], b[i][1]);
+              mma<false>(sums.o[at][w * 2 + i], values, weight[at][part][2 * sub], weight[at][part][2 * sub + 1]);
+        }
       }
     }
   }
   wait_groups<0>();
 #pragma unroll
-  for (int mt = 0; mt < S::kTiles; ++mt)
-#pragma unroll
-    for (int half = 0; half < S::kHalves; ++half) {
-      float& l = sums.l[mt][half];
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-    }
+  for (int at = 0; at < MODE; ++at) {
+    sums.l[at] += __shfl_xor_sync(0xffffffffu, sums.l[at], 1);
+    sums.l[at] += __shfl_xor_sync(0xffffffffu, sums.l[at], 2);
+  }
 }
 
 template <int SIZE, int STORAGE, int MODE, int LO>
 __global__ void __launch_bounds__(kThreads, resident_of(MODE, LO)) attention_kernel(const __grid_constant__ Plan p) {
-  using S = Sums<SIZE, MODE>;
   constexpr int kRows = rows_of(MODE);
   extern __shared__ __align__(128) char shared[];
   __shared__ int scan[kGroups], found[5];
@@ -541,24 +532,20 @@ __global__ void __launch_bounds__(kThreads, resident_of(MODE, LO)) attention_ker
     // join the groups
     __syncthreads();  // every warp is done with the ring
     float* rows = reinterpret_cast<float*>(shared);  // (groups, kRows, kPitch)
-    constexpr int kPitch = SIZE + 8;                 // (rows begin in different banks)
+    constexpr int kPitch = SIZE + 4;                 // (neighbouring rows begin in different banks)
 #pragma unroll
-    for (int at = 0; at < S::kTiles * S::kHalves; ++at) {
-      const int mt = at / S::kHalves, half = at % S::kHalves, r = at * 8 + (lane >> 2);
+    for (int at = 0; at < MODE; ++at) {
       if ((lane & 3) == 0) {
-        most[group][r] = sums.m[mt][half];
-        total[group][r] = sums.l[mt][half];
+        most[group][at * 8 + (lane >> 2)] = sums.m[at];
+        total[group][at * 8 + (lane >> 2)] = sums.l[at];
       }
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        float* to = rows + (group * kRows + r) * kPitch + element_of<SIZE>(2 * (lane & 3) + n);
-        auto value = [&](int j) {
-          const float* o = sums.o[mt][j];
-          return MODE == kPacked ? o[n] + o[2 + n] : o[2 * half + n];
-        };
+        float* to = rows + (group * kRows + at * 8 + 2 * (lane & 3) + n) * kPitch + element_of<SIZE>(lane >> 2);
 #pragma unroll
-        for (int j = 0; j < SIZE / 8; j += 4)
-          *reinterpret_cast<float4*>(to + j) = make_float4(value(j), value(j + 1), value(j + 2), value(j + 3));
+        for (int j = 0; j < SIZE / 16; j += 2)
+          *reinterpret_cast<float4*>(to + 2 * j) =
+              make_float4(sums.o[at][j][n], sums.o[at][j][2 + n], sums.o[at][j + 1][n], sums.o[at][j + 1][2 + n]);
       }
     }
     __syncthreads();
@@ -635,22 +622,24 @@ int resident_blocks() {
   return per_sm;
 }
 
-// Calls f with the template arguments of a launch: by the rows of a kv head 8
-// in one tile, 16, or blocks of 32; float32 queries of more than 8 rows with
-// their low parts, in blocks of 16.
+// Calls f with the template arguments of a launch: blocks of 8 rows, 16, 24 or
+// 32 by the rows of a kv head, of 24 or 32 those that need fewer blocks;
+// float32 queries of more than 8 rows with their low parts, in blocks of 16.
 template <typename F>
 long long with_variant(const cb_paged_attention_args& a, F f) {
   const long long rows = a.tokens * (a.heads / a.cache.kv_heads);
   auto by_rows = [&](auto size, auto storage) {
-    const auto one = std::integral_constant<int, 1>{};
+    const auto two = std::integral_constant<int, 2>{};
     const auto none = std::integral_constant<int, kNoParts>{};
     if (rows <= 8) return f(size, storage, std::integral_constant<int, kPacked>{}, none);
-    if (a.dtype == CB_F32) return f(size, storage, one, std::integral_constant<int, kBothParts>{});
+    if (a.dtype == CB_F32) return f(size, storage, two, std::integral_constant<int, kBothParts>{});
     auto by_type = [&](auto mode) {
       return a.dtype == CB_F16 ? f(size, storage, mode, std::integral_constant<int, kWeightParts>{})
                                : f(size, storage, mode, none);
     };
-    return rows <= 16 ? by_type(one) : by_type(std::integral_constant<int, 2>{});
+    if (rows <= 16) return by_type(two);
+    if ((rows + 23) / 24 == (rows + 31) / 32) return by_type(std::integral_constant<int, 3>{});
+    return by_type(std::integral_constant<int, 4>{});
   };
   auto by_storage = [&](auto size) {
     return a.cache.storage == CB_I8 ? by_rows(size, std::integral_constant<int, CB_I8>{})
