@@ -59,22 +59,24 @@ enum { kNoParts = 0, kBothParts = 1, kWeightParts = 2 };
 __host__ __device__ constexpr int tiles_of_mode(int mode) { return (mode + 1) / 2; }
 __host__ __device__ constexpr int rows_of(int mode) { return 8 * mode; }
 constexpr int kThreads = 32 * kGroups;
-// Resident blocks of an SM: 16 warps of 128 registers; with the low parts of
-// float32 queries or three sets' sums 12 of 168, with four sets' 8 of 255.  The
-// steps of a warp's ring then follow from shared memory.
-__host__ __device__ constexpr int resident_of(int mode, int lo) {
-  return mode == 4 ? 2 : mode == 3 || lo == kBothParts ? 3 : 4;
+// Resident blocks of an SM by the registers of the sums: 16 warps of 128 for one
+// set, 12 of 168 for two (47 us against 53 with 16 warps that spill, 12 rows,
+// 16 x 5100 keys on average, 8 kv heads of 128, bfloat16), 8 of 255 for three
+// and four (62 against 70 with 12 warps, 20 rows).  The steps of a warp's ring
+// then follow from shared memory.
+__host__ __device__ constexpr int resident_of(int mode) {
+  return mode >= 3 ? 2 : mode == 2 ? 3 : 4;
 }
-__host__ __device__ constexpr int stages_of(int mode, int lo) {
-  return mode == 4 ? 5 : mode == 3 || lo == kBothParts ? 4 : 3;
+__host__ __device__ constexpr int stages_of(int mode) {
+  return mode >= 3 ? 5 : mode == 2 ? 4 : 3;
 }
-__host__ __device__ constexpr int ring_bytes(int mode, int lo) { return kGroups * stages_of(mode, lo) * kSlotBytes; }
+__host__ __device__ constexpr int ring_bytes(int mode) { return kGroups * stages_of(mode) * kSlotBytes; }
 __host__ __device__ constexpr int step_keys(int head_size) { return 2048 / head_size; }
 __host__ __device__ constexpr int tile_keys(int head_size) { return kGroups * step_keys(head_size); }
 
 // Shared memory of a block: the ring, and the queries as the products read them.
 __host__ __device__ constexpr int shared_bytes(int head_size, int mode, int lo) {
-  return ring_bytes(mode, lo) + tiles_of_mode(mode) * (lo == kBothParts ? 2 : 1) * (head_size / 16) * 512;
+  return ring_bytes(mode) + tiles_of_mode(mode) * (lo == kBothParts ? 2 : 1) * (head_size / 16) * 512;
 }
 
 // ---- loads -------------------------------------------------------------------
@@ -249,7 +251,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
                                           int tile, int tiles, char* shared, float* factors,
                                           Sums<SIZE, MODE>& sums) {
   using S = Sums<SIZE, MODE>;
-  constexpr int kKeys = step_keys(SIZE), kSubs = kKeys / 16, kStages = stages_of(MODE, LO);
+  constexpr int kKeys = step_keys(SIZE), kSubs = kKeys / 16, kStages = stages_of(MODE);
   constexpr int kDots = SIZE / 16;                          // 16-element products of a score
   constexpr int kKeyWords = SIZE / 16 < 4 ? SIZE / 16 : 4;  // words of one read of a key row
   constexpr int kKeyReads = SIZE / 16 / kKeyWords;
@@ -258,7 +260,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
   const cb_paged_cache& c = p.a.cache;
   const int group = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
   char* ring = shared + group * kStages * kSlotBytes;
-  uint4* queries = reinterpret_cast<uint4*>(shared + ring_bytes(MODE, LO));
+  uint4* queries = reinterpret_cast<uint4*>(shared + ring_bytes(MODE));
 
   // limits: row r sees keys below limit[r]; all rows of the warp see those below `common`
   int limit[MODE];
@@ -503,7 +505,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
 }
 
 template <int SIZE, int STORAGE, int MODE, int LO>
-__global__ void __launch_bounds__(kThreads, resident_of(MODE, LO)) attention_kernel(const __grid_constant__ Plan p) {
+__global__ void __launch_bounds__(kThreads, resident_of(MODE)) attention_kernel(const __grid_constant__ Plan p) {
   constexpr int kRows = rows_of(MODE);
   extern __shared__ __align__(128) char shared[];
   __shared__ int scan[kGroups], found[5];
