@@ -36,7 +36,7 @@
 // Within a tile each warp takes its own 16, 32 or 64 keys (4 KB for any head
 // size) with running maxima of its own, joined at the end of an item: no
 // block barrier inside the loop.  A warp copies its keys through shared memory
-// with 16-byte asynchronous copies, two or three steps ahead; keys beyond the
+// with 16-byte asynchronous copies, one to three steps ahead; keys beyond the
 // length are filled with zeros, whatever the page holds there.
 #include <type_traits>
 
@@ -59,16 +59,19 @@ enum { kNoParts = 0, kBothParts = 1, kWeightParts = 2 };
 __host__ __device__ constexpr int tiles_of_mode(int mode) { return (mode + 1) / 2; }
 __host__ __device__ constexpr int rows_of(int mode) { return 8 * mode; }
 constexpr int kThreads = 32 * kGroups;
-// Resident blocks of an SM by the registers of the sums: 16 warps of 128 for one
-// set, 12 of 168 for two (47 us against 53 with 16 warps that spill, 12 rows,
-// 16 x 5100 keys on average, 8 kv heads of 128, bfloat16), 8 of 255 for three
-// and four (62 against 70 with 12 warps, 20 rows).  The steps of a warp's ring
-// then follow from shared memory.
+// Resident blocks of an SM by the registers of a warp's sums: 12 warps of 168
+// for one set (its queries stay in registers too: 97 us against 102 with 16
+// warps at two sequences of 131,067 keys, 8 kv heads of 128) and two (47 us
+// against 53 with 16 warps that spill, 12 rows, 16 x 5100 keys on average,
+// bfloat16), 8 of 255 for three and four (62 against 70 with 12 warps, 20 rows).
+// The steps of a warp's ring: as few as the join at an item's end leaves (two
+// against four: 94 us and 97 at the long sequences, 45.6 and 47.4 with 12 rows;
+// 8 KB a warp in flight are 96 KB an SM).
 __host__ __device__ constexpr int resident_of(int mode) {
-  return mode >= 3 ? 2 : mode == 2 ? 3 : 4;
+  return mode >= 3 ? 2 : 3;
 }
 __host__ __device__ constexpr int stages_of(int mode) {
-  return mode >= 3 ? 5 : mode == 2 ? 4 : 3;
+  return mode == 4 ? 4 : mode == 3 ? 3 : 2;
 }
 __host__ __device__ constexpr int ring_bytes(int mode) { return kGroups * stages_of(mode) * kSlotBytes; }
 __host__ __device__ constexpr int step_keys(int head_size) { return 2048 / head_size; }
@@ -349,6 +352,9 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
 #pragma unroll
   for (int at = 0; at < MODE; ++at) factor[at] = factors[at * 8 + g];
   queries += lane;
+  uint4 held[MODE == kPacked ? kDots : 1];  // packed queries stay in registers
+#pragma unroll
+  for (int dot = 0; dot < (MODE == kPacked ? kDots : 0); ++dot) held[dot] = queries[dot * 32];
   // where this lane reads: rows 8 n + key_of(g) of K, quad + 4 i of V.  The
   // second half of a 128-byte key row, and every other row of V, lie half a line
   // turned; the rest are constant distances.
@@ -377,7 +383,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
 #pragma unroll
         for (int mt = 0; mt < S::kTiles; ++mt)
 #pragma unroll
-          for (int part = 0; part < kParts; ++part) a[mt][part] = queries[((mt * kParts + part) * kDots + dot) * 32];
+          for (int part = 0; part < kParts; ++part) a[mt][part] = MODE == kPacked ? held[dot] : queries[((mt * kParts + part) * kDots + dot) * 32];
 #pragma unroll
         for (int n = 0; n < 2 * kSubs; ++n) {
           uint32_t b0, b1;
@@ -535,6 +541,7 @@ __global__ void __launch_bounds__(kThreads, resident_of(MODE)) attention_kernel(
     __syncthreads();  // every warp is done with the ring
     float* rows = reinterpret_cast<float*>(shared);  // (groups, kRows, kPitch)
     constexpr int kPitch = SIZE + 4;                 // (neighbouring rows begin in different banks)
+    static_assert(kGroups * kRows * kPitch * 4 <= shared_bytes(SIZE, MODE, LO), "the rows to join fit the ring");
 #pragma unroll
     for (int at = 0; at < MODE; ++at) {
       if ((lane & 3) == 0) {
@@ -625,8 +632,7 @@ int resident_blocks() {
 }
 
 // Calls f with the template arguments of a launch: blocks of 8 rows, 16, 24 or
-// 32 by the rows of a kv head, of 24 or 32 those that need fewer blocks;
-// float32 queries of more than 8 rows with their low parts, in blocks of 16.
+// 32 by the rows of a kv head, of 24 or 32 those that need fewer blocks.
 template <typename F>
 long long with_variant(const cb_paged_attention_args& a, F f) {
   const long long rows = a.tokens * (a.heads / a.cache.kv_heads);
@@ -634,10 +640,10 @@ long long with_variant(const cb_paged_attention_args& a, F f) {
     const auto two = std::integral_constant<int, 2>{};
     const auto none = std::integral_constant<int, kNoParts>{};
     if (rows <= 8) return f(size, storage, std::integral_constant<int, kPacked>{}, none);
-    if (a.dtype == CB_F32) return f(size, storage, two, std::integral_constant<int, kBothParts>{});
     auto by_type = [&](auto mode) {
-      return a.dtype == CB_F16 ? f(size, storage, mode, std::integral_constant<int, kWeightParts>{})
-                               : f(size, storage, mode, none);
+      if (a.dtype == CB_F32) return f(size, storage, mode, std::integral_constant<int, kBothParts>{});
+      if (a.dtype == CB_F16) return f(size, storage, mode, std::integral_constant<int, kWeightParts>{});
+      return f(size, storage, mode, none);
     };
     if (rows <= 16) return by_type(two);
     if ((rows + 23) / 24 == (rows + 31) / 32) return by_type(std::integral_constant<int, 3>{});

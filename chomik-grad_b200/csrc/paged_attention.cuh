@@ -10,7 +10,7 @@ namespace {
 
 // Tiles' time that beginning an item costs (queries, first loads, joining the
 // warps): counted when the work is divided.
-constexpr int kItemCost = 3;
+constexpr int kItemCost = 4;
 // Items of no more than six tiles are not cut: joining parts takes as long.
 constexpr int kSmallItem = kItemCost + 6;
 
