@@ -17,14 +17,16 @@
 //   - a query row is scaled by a power of two to below 2 and split into
 //     hi + lo (22 bits); up to 8 rows, the hi parts are rows 0-7 of the tile
 //     and the lo parts rows 8-15, at no cost.  16-bit queries in more than 8
-//     rows are used as they are (exact but for elements 2^-14 below the row's
+//     rows take the hi part alone (exact but for elements 2^-14 below the row's
 //     largest, whose error is below 2^-25 of that);
 //   - what multiplies the value codes is the weight exp(s_j - m) times the
 //     page's value scale: the running maximum m is that of the scores plus the
 //     scales' exponents, so that these products stay within fp16 whatever the
 //     scales, and they are split the same way (bfloat16 outputs of more than 8
 //     rows: hi only, a relative error of 2^-12 a weight, a sixteenth of the
-//     output's own rounding).  The sum of the weights leaves the scale out again.
+//     output's own rounding; float16 outputs keep both, for an error of 2.1e-4
+//     against 2.9e-4 and 9 us of 69 in blocks of 20 rows).  The sum of the
+//     weights leaves the scale out again.
 //
 // How the work is laid out.  The keys of all (slot, kv head, block of rows)
 // are one sequence of tiles, cut into equal ranges for a grid that fills the
@@ -38,6 +40,14 @@
 // block barrier inside the loop.  A warp copies its keys through shared memory
 // with 16-byte asynchronous copies, one to three steps ahead; keys beyond the
 // length are filled with zeros, whatever the page holds there.
+//
+// Measured, one B200, 8 kv heads of 128: two sequences of 131,067 keys, e4m3,
+// 4 rows: 94 us, 5.7 TB/s (88% of the measured copy); 32 ragged sequences of up
+// to 4096, int8, 4 rows: 39 us, 4.1 TB/s (3 us until the first products, 5.7
+// TB/s after that, blocks' ends 28 to 41 us apart by their share of begins,
+// ends and joins); 16 ragged ones of up to 8191, int8, float16, 20 rows: 69 us,
+// 2.5 TB/s, where 8 warps an SM leave the latency of the instructions open (IPC
+// 1.65, tensor pipe 41%).  One sequence of 384 keys: 7 us of dependent loads.
 #include <type_traits>
 
 #include "paged_attention.cuh"

