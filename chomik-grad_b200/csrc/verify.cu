@@ -9,13 +9,13 @@
 // One cluster of blocks per sequence, one launch.  A row is read once: a warp
 // owns a contiguous run of it, the warps' sums are joined over the block, and
 // the blocks' over the cluster through distributed shared memory; then the
-// warp whose run holds the threshold reads its run again (some KB, from L2) to
-// find the token.  What bounds it: one target row and, where a draft was
+// block that holds the threshold reads the run that does again (some KB, from
+// L2) to find the token.  What bounds it: one target row and, where a draft was
 // refused, one draft row per sequence; in small batches the chain of dependent
 // loads (drafted token, its probabilities, the rows).  Measured: 64 rows of 7
-// drafts and 128,256 float32 probabilities 18.3 us (3.4 TB/s: the chain before
-// the rows, the exchange and the second read take half of it), one row of 4
-// drafts and 32,000 4.7 us.
+// drafts and 128,256 float32 probabilities 18.2 us (2 us until the rows, which
+// take until 9 to 14, the exchange until 13 to 15, the second read 1.5), one
+// row of 4 drafts and 32,000 4.6 us.
 #include <cooperative_groups.h>
 
 #include "paged.cuh"
@@ -104,6 +104,7 @@ template <int DT>
 __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant__ cb_verify_args a, int blocks) {
   constexpr int kPer = Item<DT>::kPer, kItem = 16 / kPer;
   __shared__ Sums warps[kWarps], cluster[2][kMostBlocks];
+  __shared__ u64 parts[kWarps];
   cluster_begun();
   pdl_launch_dependents();
   pdl_wait();
@@ -244,12 +245,12 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
     for (long long t = threadIdx.x; t <= a.tokens; t += kThreads)
       if (t != accepted || bad) a.out[b * (a.tokens + 1) + t] = t < accepted ? drafted[t] : -1;
   }
-  if (bad) return;
-  for (int w = 0; w < warp; ++w) before += warps[w].weight;
-  if (bar < before || bar >= before + warps[warp].weight) return;
+  if (bad || bar < before || bar >= before + cluster[second][rank].weight) return;  // the same in the block
 
-  // 3. that warp's run once more: each lane a contiguous part of it, then the
-  // part that holds the threshold, each lane kPer elements of it at a time
+  // 3. the block that holds it reads that warp's run once more, each thread a
+  // contiguous part, and the thread whose part holds it finds the token
+  int holder = 0;
+  while (bar >= before + warps[holder].weight) before += warps[holder++].weight;
   const bool with_draft = refused && !second;
   auto weights = [&](long long j, u64* w) {
     float p[kPer], q[kPer];
@@ -263,39 +264,30 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
     }
     return sum;
   };
-  auto upto_lane = [&](u64 v) {  // inclusive sum over the lanes
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 up = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += up;
-    }
-    return v;
-  };
-  const long long part = run / 32;  // a multiple of kPer
+  const long long start = (static_cast<long long>(rank) * kWarps + holder) * run;
+  const long long part = (run / kPer + kThreads - 1) / kThreads * kPer;
+  const long long begin = start + threadIdx.x * part, end = begin + part < start + run ? begin + part : start + run;
   u64 w[kPer], sum = 0;
 #pragma unroll 4
-  for (long long j = 0; j < part; j += kPer) sum += weights(from + lane * part + j, w);
-  u64 upto = upto_lane(sum);
-  const int holder = __ffs(__ballot_sync(0xffffffffu, bar < before + upto)) - 1;
-  before += __shfl_sync(0xffffffffu, upto - sum, holder);
-  const long long begin = from + holder * part;
-  for (long long first = begin; first < begin + part; first += 32 * kPer) {
-    const long long j = first + lane * kPer;
-    sum = 0;
+  for (long long j = begin; j < end; j += kPer) sum += weights(j, w);
+  u64 upto = sum;  // inclusive sum over the lanes
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) w[i] = 0;
-    if (j < begin + part) sum = weights(j, w);
-    upto = upto_lane(sum);
-    u64 running = before + upto - sum;
-    if (running <= bar && bar < before + upto) {  // one lane
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 up = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += up;
+  }
+  if (lane == 31) parts[warp] = upto;
+  __syncthreads();
+  u64 running = before + upto - sum;
+  for (int p = 0; p < warp; ++p) running += parts[p];
+  if (bar < running || bar >= running + sum) return;
+  for (long long j = begin; j < end; j += kPer) {  // one thread
+    weights(j, w);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        if (running <= bar && bar < running + w[i]) a.out[b * (a.tokens + 1) + accepted] = j + i;
-        running += w[i];
-      }
+    for (int i = 0; i < kPer; ++i) {
+      if (running <= bar && bar < running + w[i]) a.out[b * (a.tokens + 1) + accepted] = j + i;
+      running += w[i];
     }
-    before += __shfl_sync(0xffffffffu, upto, 31);
-    if (before > bar) return;
   }
 }
 
