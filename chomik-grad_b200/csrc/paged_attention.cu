@@ -269,7 +269,8 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
   constexpr int kKeyWords = SIZE / 16 < 4 ? SIZE / 16 : 4;  // words of one read of a key row
   constexpr int kKeyReads = SIZE / 16 / kKeyWords;
   constexpr int kValueWords = SIZE / 32;
-  constexpr int kParts = LO == kBothParts ? 2 : 1, kWeights = MODE == kPacked || LO ? 2 : 1;  // parts of queries, of weights
+  constexpr int kParts = LO == kBothParts ? 2 : 1;          // of the queries
+  constexpr int kWeights = MODE == kPacked || LO ? 2 : 1;   // parts of the weights
   const cb_paged_cache& c = p.a.cache;
   const int group = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
   char* ring = shared + group * kStages * kSlotBytes;
@@ -393,7 +394,8 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
 #pragma unroll
         for (int mt = 0; mt < S::kTiles; ++mt)
 #pragma unroll
-          for (int part = 0; part < kParts; ++part) a[mt][part] = MODE == kPacked ? held[dot] : queries[((mt * kParts + part) * kDots + dot) * 32];
+          for (int part = 0; part < kParts; ++part)
+            a[mt][part] = MODE == kPacked ? held[dot] : queries[((mt * kParts + part) * kDots + dot) * 32];
 #pragma unroll
         for (int n = 0; n < 2 * kSubs; ++n) {
           uint32_t b0, b1;
@@ -544,7 +546,8 @@ __global__ void __launch_bounds__(kThreads, resident_of(MODE)) attention_kernel(
       continue;
     }
     Sums<SIZE, MODE> sums;
-    const void* query = static_cast<const char*>(p.a.q) + static_cast<long long>(b) * p.a.q_strides[0] * (p.a.dtype == CB_F32 ? 4 : 2);
+    const int item = p.a.dtype == CB_F32 ? 4 : 2;
+    const void* query = static_cast<const char*>(p.a.q) + static_cast<long long>(b) * p.a.q_strides[0] * item;
     warp_item<SIZE, STORAGE, MODE, LO>(p, query, seg.s, head, first_row, seg.tile, seg.tiles, shared, factors, sums);
 
     // join the groups
@@ -642,7 +645,10 @@ int resident_blocks() {
 }
 
 // Calls f with the template arguments of a launch: blocks of 8 rows, 16, 24 or
-// 32 by the rows of a kv head, of 24 or 32 those that need fewer blocks.
+// 32 by the rows of a kv head, of 24 or 32 those that need fewer blocks (16 x
+// 5100 keys on average, int8, bfloat16: 8 rows 41 us, 12 and 16 45 and 46; 20
+// rows 60 in one block of 24 and 68 in one of 32; 40 rows 102 in two of 24 and
+// 118 in two of 32).
 template <typename F>
 long long with_variant(const cb_paged_attention_args& a, F f) {
   const long long rows = a.tokens * (a.heads / a.cache.kv_heads);
@@ -695,7 +701,8 @@ int cb_paged_attention(const cb_paged_attention_args* args, void* scratch, unsig
   const int status = attention_check(a);
   if (status != CB_OK) return status;
   if (a.batch == 0 || a.tokens == 0) return CB_OK;
-  CB_REQUIRE(a.q != nullptr && a.out != nullptr && scratch != nullptr && counters != nullptr, "cb_paged_attention: a null pointer");
+  CB_REQUIRE(a.q != nullptr && a.out != nullptr && scratch != nullptr && counters != nullptr,
+             "cb_paged_attention: a null pointer");
   CB_REQUIRE(reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && reinterpret_cast<uintptr_t>(scratch) % 16 == 0,
              "cb_paged_attention: out and scratch must be 16-byte aligned");
   return static_cast<int>(with_variant(a, [&](auto size, auto storage, auto mode, auto lo) -> long long {
