@@ -20,13 +20,16 @@
 //     rows take the hi part alone (exact but for elements 2^-14 below the row's
 //     largest, whose error is below 2^-25 of that);
 //   - what multiplies the value codes is the weight exp(s_j - m) times the
-//     page's value scale: the running maximum m is that of the scores plus the
-//     scales' exponents, so that these products stay within fp16 whatever the
-//     scales, and they are split the same way (bfloat16 outputs of more than 8
-//     rows: hi only, a relative error of 2^-12 a weight, a sixteenth of the
+//     page's value scale, against that of the warp's first page whose scale is
+//     not zero: the running maximum m is that of the scores plus the scales'
+//     exponents relative to it, so that these products stay within fp16 whatever
+//     the scales, and they are split the same way (bfloat16 outputs of more than
+//     8 rows: hi only, a relative error of 2^-12 a weight, a sixteenth of the
 //     output's own rounding; float16 outputs keep both, for an error of 2.1e-4
 //     against 2.9e-4 and 9 us of 69 in blocks of 20 rows).  The sum of the
-//     weights leaves the scale out again.
+//     weights leaves the scale out again.  Pages of zero values (scale 0) belong
+//     to that sum alone: they stand 2^-64 below the first scale, so that they do
+//     not set m.
 //
 // How the work is laid out.  The keys of all (slot, kv head, block of rows)
 // are one sequence of tiles, cut into equal ranges for a grid that fills the
@@ -289,7 +292,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
 #pragma unroll
       for (int i = 0; i < 4; ++i) sums.o[at][j][i] = 0.0f;
   }
-  int last = 0;  // exponent of the value scale before
+  int base = 0;  // exponent field of the first value scale that is not zero; 0 before it
   const int common = s.row.length - s.row.count + first_row / p.group + 1;
   const int length = s.row.length;
 
@@ -413,18 +416,42 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
       }
     }
 
-    // value scales as 2^exponent * fraction; one that is zero takes the exponent
-    // before it, its weights count in the sum all the same
+    // value scales as 2^(base + exponent) * fraction
     float exponent[kSubs], fraction[kSubs], undo[kSubs];
+    int field[kSubs], largest = 0;  // exponent fields; 0 for a scale of zero
 #pragma unroll
     for (int sub = 0; sub < kSubs; ++sub) {
       const uint32_t word = __float_as_uint(scales[4 + sub]);
-      const int e = static_cast<int>(word >> 23 & 0xffu) - 127;
-      const bool normal = e > -127 && e < 127;
-      if (normal) last = e;
-      fraction[sub] = normal ? __uint_as_float((word & 0x807fffffu) | 0x3f800000u) : e < 0 ? 0.0f : NAN;
-      exponent[sub] = static_cast<float>(last);
-      undo[sub] = __uint_as_float(static_cast<uint32_t>(127 - last) << 23);
+      field[sub] = static_cast<int>(word >> 23 & 0xffu);
+      fraction[sub] = field[sub] == 0 ? 0.0f : field[sub] == 255 ? NAN : __uint_as_float((word & 0x807fffffu) | 0x3f800000u);
+      if (field[sub] == 255) field[sub] = 0;  // (an infinity or NaN)
+      largest = max(largest, field[sub]);
+    }
+    if (base == 0) {
+      base = largest;
+    } else if (largest > base + kMostAbove) {  // (the same for the warp) the sums in larger units
+      const int up = largest - base - kMostAbove, lower = min(up, kMostLower), down = up - lower;
+      const float grow = power2(lower), shrink0 = power2(-(down >> 1)), shrink1 = power2((down >> 1) - down);
+      base += up;
+#pragma unroll
+      for (int at = 0; at < MODE; ++at) {
+        sums.m[at] -= lower;
+        sums.l[at] *= grow;
+#pragma unroll
+        for (int j = 0; j < SIZE / 16; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sums.o[at][j][i] = sums.o[at][j][i] * shrink0 * shrink1;
+      }
+    }
+#pragma unroll
+    for (int sub = 0; sub < kSubs; ++sub) {
+      int e = field[sub] > 0 ? field[sub] - base : -kZeroBelow;
+      if (e < -kZeroBelow) {
+        fraction[sub] *= power2(max(e + kZeroBelow, -126));
+        e = -kZeroBelow;
+      }
+      exponent[sub] = static_cast<float>(e);
+      undo[sub] = power2(-e);
     }
     // the rows' scores and their maxima
     float x[MODE][2 * kSubs][2], most[MODE];
@@ -515,10 +542,21 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
     }
   }
   wait_groups<0>();
+  // From units of 2^base to ones, which other warps and blocks have too: most of
+  // it moves the maximum, what could leave the range of the sum of the weights
+  // scales the values.
+  const int unit = base > 0 ? base - 127 : 0, fold = max(unit - 10, -10);
+  const float to_l = power2(-fold), to_o = power2(unit - fold);
 #pragma unroll
   for (int at = 0; at < MODE; ++at) {
+    sums.m[at] += fold;
     sums.l[at] += __shfl_xor_sync(0xffffffffu, sums.l[at], 1);
     sums.l[at] += __shfl_xor_sync(0xffffffffu, sums.l[at], 2);
+    sums.l[at] *= to_l;
+#pragma unroll
+    for (int j = 0; j < SIZE / 16; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sums.o[at][j][i] *= to_o;
   }
 }
 

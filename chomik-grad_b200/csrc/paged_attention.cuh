@@ -31,6 +31,15 @@ __device__ __forceinline__ float root2_of(float x) { return exp2_of(0.5f * x); }
 // 22) bits for all that are within 2^-14 of the largest.
 constexpr float kSlack = 8.0f;
 
+// Value scales are exponents relative to the first that is not zero.  Those
+// from 2^-kZeroBelow (which zeros count as) to 2^kMostAbove of it keep both
+// sums within float32; a larger one moves the reference, and of that up to
+// 2^kMostLower the maximum, the rest the weighted values.
+constexpr int kZeroBelow = 64, kMostAbove = 100, kMostLower = 24;
+
+// 2^e, e in [-126, 127]
+__device__ __forceinline__ float power2(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
 struct Plan {  // of one launch
