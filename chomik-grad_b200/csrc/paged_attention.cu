@@ -19,17 +19,14 @@
 //     and the lo parts rows 8-15, at no cost.  16-bit queries in more than 8
 //     rows take the hi part alone (exact but for elements 2^-14 below the row's
 //     largest, whose error is below 2^-25 of that);
-//   - what multiplies the value codes is the weight exp(s_j - m) times the
-//     page's value scale, against that of the warp's first page whose scale is
-//     not zero: the running maximum m is that of the scores plus the scales'
-//     exponents relative to it, so that these products stay within fp16 whatever
-//     the scales, and they are split the same way (bfloat16 outputs of more than
-//     8 rows: hi only, a relative error of 2^-12 a weight, a sixteenth of the
-//     output's own rounding; float16 outputs keep both, for an error of 2.1e-4
-//     against 2.9e-4 and 9 us of 69 in blocks of 20 rows).  The sum of the
-//     weights leaves the scale out again.  Pages of zero values (scale 0) belong
-//     to that sum alone: they stand 2^-64 below the first scale, so that they do
-//     not set m.
+//   - what multiplies the value codes is the weight 2^(x - c) times the page's
+//     value scale, both against references that follow the keys (see
+//     paged_attention.cuh), so that these products stay within fp16 and keep their
+//     bits however far apart scores and scales are.  They are split the same way
+//     (bfloat16 outputs of more than 8 rows: hi only, a relative error of 2^-12 a
+//     weight, a sixteenth of the output's own rounding; float16 outputs keep both,
+//     for an error of 2.1e-4 against 2.9e-4 and 9 us of 69 in blocks of 20 rows).
+//     The sum of the weights leaves the scale out.
 //
 // How the work is laid out.  The keys of all (slot, kv head, block of rows)
 // are one sequence of tiles, cut into equal ranges for a grid that fills the
@@ -285,14 +282,16 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
   for (int at = 0; at < MODE; ++at) {
     const int r = first_row + at * 8 + g, t = r / p.group;
     limit[at] = r < p.rows && t < s.row.count ? s.row.length - s.row.count + t + 1 : 0;
-    sums.m[at] = -INFINITY;
+    sums.m[at] = kUnset;
     sums.l[at] = 0.0f;
 #pragma unroll
     for (int j = 0; j < SIZE / 16; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) sums.o[at][j][i] = 0.0f;
   }
-  int base = 0;  // exponent field of the first value scale that is not zero; 0 before it
+  uint32_t least = kNoScale;  // bits of 2^(base - kScales), once there is a scale
+  float unit = 1.0f;          // 2^(kLift - base)
+  int far = 0;                // the largest scale's exponent, where it is above base
   const int common = s.row.length - s.row.count + first_row / p.group + 1;
   const int length = s.row.length;
 
@@ -416,46 +415,59 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
       }
     }
 
-    // value scales as 2^(base + exponent) * fraction
-    float exponent[kSubs], fraction[kSubs], undo[kSubs];
-    int field[kSubs], largest = 0;  // exponent fields; 0 for a scale of zero
+    // value scales as 2^(base + exponent) * value
+    float value[kSubs], exponent[kSubs], undo[kSubs];
+    bool near = true;
 #pragma unroll
     for (int sub = 0; sub < kSubs; ++sub) {
-      const uint32_t word = __float_as_uint(scales[4 + sub]);
-      field[sub] = static_cast<int>(word >> 23 & 0xffu);
-      fraction[sub] = field[sub] == 0 ? 0.0f : field[sub] == 255 ? NAN : __uint_as_float((word & 0x807fffffu) | 0x3f800000u);
-      if (field[sub] == 255) field[sub] = 0;  // (an infinity or NaN)
-      largest = max(largest, field[sub]);
+      value[sub] = scales[4 + sub] * unit;
+      exponent[sub] = 0.0f;
+      undo[sub] = 1.0f;
+      near = near && __float_as_uint(scales[4 + sub]) - least < (kScales + 1u) << 23;
     }
-    if (base == 0) {
-      base = largest;
-    } else if (largest > base + kMostAbove) {  // (the same for the warp) the sums in larger units
-      const int up = largest - base - kMostAbove, lower = min(up, kMostLower), down = up - lower;
-      const float grow = power2(lower), shrink0 = power2(-(down >> 1)), shrink1 = power2((down >> 1) - down);
-      base += up;
+    if (!near) {  // (the same for the warp) the first scale, zeros, scales far from the first, infinities
+      int field[kSubs], largest = 0;
 #pragma unroll
-      for (int at = 0; at < MODE; ++at) {
-        sums.m[at] -= lower;
-        sums.l[at] *= grow;
-#pragma unroll
-        for (int j = 0; j < SIZE / 16; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sums.o[at][j][i] = sums.o[at][j][i] * shrink0 * shrink1;
+      for (int sub = 0; sub < kSubs; ++sub) {
+        field[sub] = static_cast<int>(__float_as_uint(scales[4 + sub]) >> 23 & 0xffu);
+        if (field[sub] < 255) largest = max(largest, field[sub]);
       }
-    }
+      int base = least == kNoScale ? min(max(largest + 1, kLeastField), 254) : static_cast<int>(least >> 23) + kScales;
+      if (largest > base + kMostAbove) {
+        const int up = largest - base - kMostAbove, lower = min(up, kMostLower) & ~1, less = up - lower;
+        const float by0 = power2(-(less >> 1)), by1 = power2((less >> 1) - less);
+        base += up;
 #pragma unroll
-    for (int sub = 0; sub < kSubs; ++sub) {
-      int e = field[sub] > 0 ? field[sub] - base : -kZeroBelow;
-      if (e < -kZeroBelow) {
-        fraction[sub] *= power2(max(e + kZeroBelow, -126));
-        e = -kZeroBelow;
+        for (int at = 0; at < MODE; ++at) {
+          sums.m[at] -= lower;
+          sums.l[at] *= power2(lower);
+#pragma unroll
+          for (int j = 0; j < SIZE / 16; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sums.o[at][j][i] = sums.o[at][j][i] * by0 * by1;
+        }
       }
-      exponent[sub] = static_cast<float>(e);
-      undo[sub] = power2(-e);
+      far = max(far, largest - base);
+      if (largest > 0) least = static_cast<uint32_t>(base - kScales) << 23;
+      unit = power2(127 - base + kLift);
+#pragma unroll
+      for (int sub = 0; sub < kSubs; ++sub) {
+        const int e = field[sub] - base;
+        value[sub] = scales[4 + sub] * unit;
+        if (field[sub] == 0 || field[sub] == 255) {
+          value[sub] = field[sub] == 0 ? 0.0f : NAN;
+          exponent[sub] = -kZeroBelow;
+        } else if (e > 0 || e < -kScales) {
+          value[sub] = __uint_as_float((__float_as_uint(scales[4 + sub]) & 0x807fffffu) | (127u + kLift) << 23);
+          if (e < -kZeroBelow) value[sub] *= power2(max(e + kZeroBelow, -126));
+          exponent[sub] = static_cast<float>(max(e, -kZeroBelow));
+        }
+        undo[sub] = power2(-static_cast<int>(exponent[sub]));
+      }
     }
     // the rows' scores and their maxima
     float x[MODE][2 * kSubs][2], most[MODE];
-    bool grows = false;
+    bool moves = false;
 #pragma unroll
     for (int at = 0; at < MODE; ++at) {
 #pragma unroll
@@ -484,15 +496,18 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
       for (int n = 0; n < 2 * kSubs; ++n) most[at] = fmaxf(most[at], fmaxf(x[at][n][0], x[at][n][1]));
       most[at] = fmaxf(most[at], __shfl_xor_sync(0xffffffffu, most[at], 1));
       most[at] = fmaxf(most[at], __shfl_xor_sync(0xffffffffu, most[at], 2));
-      grows = grows || most[at] > sums.m[at] + kSlack;
+      moves = moves || fabsf(most[at] - sums.m[at]) > kWindow;
     }
-    // The sums are kept against a maximum that follows the running one only
-    // when that is 2^kSlack above it, so they are rarely scaled.
-    if (__any_sync(0xffffffffu, grows)) {
+    if (__any_sync(0xffffffffu, moves)) {
+      const float room = power2(kRoom - far);  // (the weighted values are at most 2^(far + 14) times the weights' sum)
 #pragma unroll
       for (int at = 0; at < MODE; ++at) {
-        const float old = sums.m[at], now = most[at] > old + kSlack ? most[at] : old;
-        const float r = now == -INFINITY ? 1.0f : root2_of(old - now);
+        const float old = sums.m[at], next = 2.0f * ceilf(0.5f * most[at]) - kAbove;
+        float held = fmaxf(sums.l[at], __shfl_xor_sync(0xffffffffu, sums.l[at], 1));
+        held = fmaxf(held, __shfl_xor_sync(0xffffffffu, held, 2));
+        const bool falls = most[at] < old - kWindow && most[at] > -INFINITY && held < room;
+        const float now = most[at] > old + kWindow ? next : falls ? fmaxf(next, old - kDown) : old;
+        const float r = now == old ? 1.0f : power2(max(static_cast<int>(0.5f * (old - now)), -126));
         sums.m[at] = now;
         sums.l[at] *= r * r;
         const float r0 = __shfl_sync(0xffffffffu, r, quad * 8), r1 = __shfl_sync(0xffffffffu, r, quad * 8 + 4);
@@ -505,13 +520,12 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
     uint32_t weight[MODE][kWeights][2 * kSubs];
 #pragma unroll
     for (int at = 0; at < MODE; ++at) {
-      const float against = sums.m[at] == -INFINITY ? 0.0f : sums.m[at];
 #pragma unroll
       for (int n = 0; n < 2 * kSubs; ++n) {
-        const float e0 = exp2_of(x[at][n][0] - against), e1 = exp2_of(x[at][n][1] - against);
+        const float e0 = exp2_of(x[at][n][0] - sums.m[at]), e1 = exp2_of(x[at][n][1] - sums.m[at]);
         sums.l[at] = fmaf(e0 + e1, undo[n / 2], sums.l[at]);
         uint32_t lo;
-        split(e0 * fraction[n / 2], e1 * fraction[n / 2], weight[at][0][n], lo);
+        split(e0 * value[n / 2], e1 * value[n / 2], weight[at][0][n], lo);
         if (kWeights == 2) weight[at][kWeights - 1][n] = lo;
       }
     }
@@ -542,11 +556,11 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
     }
   }
   wait_groups<0>();
-  // From units of 2^base to ones, which other warps and blocks have too: most of
-  // it moves the maximum, what could leave the range of the sum of the weights
-  // scales the values.
-  const int unit = base > 0 ? base - 127 : 0, fold = max(unit - 10, -10);
-  const float to_l = power2(-fold), to_o = power2(unit - fold);
+  // From units of 2^(base - kLift) to ones, which other warps and blocks have
+  // too: most of it moves the reference, what could leave the range of the sum of
+  // the weights scales the values.
+  const int base = least == kNoScale ? 0 : static_cast<int>(least >> 23) + kScales - 127, fold = max(base - 10, -10);
+  const float to_l = power2(-fold), to_o = power2(base - kLift - fold);
 #pragma unroll
   for (int at = 0; at < MODE; ++at) {
     sums.m[at] += fold;

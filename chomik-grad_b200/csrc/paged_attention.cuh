@@ -27,15 +27,27 @@ __device__ __forceinline__ float exp2_of(float x) {
 // kept where 2^x itself would be below float32's range.
 __device__ __forceinline__ float root2_of(float x) { return exp2_of(0.5f * x); }
 
-// Weights are at most 2^(kSlack + 1): far inside fp16, with its 11 (hi and lo:
-// 22) bits for all that are within 2^-14 of the largest.
-constexpr float kSlack = 8.0f;
+// Value scales are taken against 2^base, twice the power of two of the first that
+// is not zero.  One from 2^-kScales of it to less than twice goes into the weights as it is; others
+// leave their exponent e, against base, to the score, and 2^-e to the weight's
+// share in the sum of the weights.  From -kZeroBelow (which zeros count as: they
+// belong to that sum alone) to kMostAbove both sums stay within float32; a larger
+// scale moves base, and of that up to kMostLower the scores' reference, the rest
+// the weighted values.
+constexpr int kScales = 5, kZeroBelow = 64, kMostAbove = 100, kMostLower = 24, kLeastField = 7;
+constexpr uint32_t kNoScale = 0xfc000000u;  // (of no scale but those below -2^121)
 
-// Value scales are exponents relative to the first that is not zero.  Those
-// from 2^-kZeroBelow (which zeros count as) to 2^kMostAbove of it keep both
-// sums within float32; a larger one moves the reference, and of that up to
-// 2^kMostLower the maximum, the rest the weighted values.
-constexpr int kZeroBelow = 64, kMostAbove = 100, kMostLower = 24;
+// The sums are kept against a reference c: a score x, its scale's exponent
+// included, weighs 2^(x - c), and 2^kLift times that in fp16.  A step whose
+// largest x is more than kWindow from c moves c to kAbove below it, up or down
+// (by an even number: sums move by exact powers of two).  So the largest weight
+// of a step, with a scale like the first, lies between 2^-7 and 2^15, where two
+// fp16 parts hold it to 18 bits at worst and to 22 in the upper half, and the
+// step's others to 2^-25: keys far below one that was seen before keep their
+// bits.  Down by at most kDown at
+// a time, and not where the sums would come near float32's end.
+constexpr float kWindow = 10.0f, kAbove = 4.0f, kDown = 50.0f, kUnset = -1e30f;
+constexpr int kLift = 4, kRoom = 20;
 
 // 2^e, e in [-126, 127]
 __device__ __forceinline__ float power2(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }

@@ -1,9 +1,13 @@
-"""cb_paged_attention where value scales lie far apart or are zero, against a float64 softmax.
+"""cb_paged_attention where value scales or weights lie far apart, against a float64 softmax.
 
-Bound, from the formula: an output is sum w v / sum w, and an error e of the
-weights (relative) moves it by at most 2 e max|v|.  e is that of the other
-tests of this entry point: scores below 64 in base 2 of numbers held to 22 bits
-or more give 2^-16, weights rounded to 11 bits (16-bit types) 2^-11 more.
+Bound, from the formula: an output is sum w v / sum w.  An error e of the
+weights (relative) moves it by at most 2 e max|v|, and where keys whose values
+are zero hold most of the weight, by at most 2 e max|v| times the share f of
+the others.  e is that of the other tests of this entry point: scores below 64
+in base 2 of numbers held to 22 bits or more give 2^-16, weights rounded to 11
+bits (16-bit types) 2^-11 more.  Weights are rounded against the largest of
+their step of 2048 / head_size keys, whose low parts end 2^-30 below it, so the
+keys of the step that holds a dominant one may be off by that each.
 """
 
 from __future__ import annotations
@@ -22,10 +26,10 @@ pytestmark = pytest.mark.gpu
 WEIGHTS = {"f32": 2.0 ** -16, "bf16": 2.0 ** -16 + 2.0 ** -11, "f16": 2.0 ** -16 + 2.0 ** -11}
 
 
-def compare(got, want, largest, dtype):
-    """``largest``: of the values."""
+def compare(got, want, largest, dtype, share=1.0, lost=0.0):
+    """``largest``: of the values; ``share``: of the weights that count (broadcasts); ``lost``: absolute, of largest."""
     info = torch.finfo(DTYPE[dtype])
-    bound = 2 * WEIGHTS[dtype] * largest + info.eps / 2 * np.abs(want) + info.tiny * info.eps / 2
+    bound = (2 * WEIGHTS[dtype] * share + lost) * largest + info.eps / 2 * np.abs(want) + info.tiny * info.eps / 2
     got = wide(got)
     assert np.isfinite(got).all()
     assert (np.abs(got - want) <= bound).all(), float(np.max(np.abs(got - want) / bound))
@@ -121,3 +125,86 @@ def test_a_large_scale_that_earlier_rows_do_not_see():
     want, got = expected(host, q, [0], 0.1)[0], to_device(host).attend(0, q, scale=0.1)[0]
     compare(got[:2], want[:2], 127 * 2.0 ** -100, "f32")
     compare(got[2:], want[2:], 127 * 2.0 ** 27, "f32")
+
+
+def scored(rng, lengths, codes, size, page, dtype, tokens, heads, scale_exponent=-6):
+    """A cache and queries whose scores are codes / 4 (natural logarithm); sinks (codes above 16) have zero values."""
+    host = filled(rng, lengths, kv_heads=1, head_size=size, page=page, spare=0, garbage=False)
+    host.scales[0][:] = 0.25
+    host.scales[1][:] = 2.0 ** scale_exponent
+    host.pools[0][:] = 0
+    for slot, length in enumerate(lengths):
+        at = np.arange(length)
+        pages, rows = host.table[slot, at // page], at % page
+        host.pools[0][0, pages, 0, rows, 0] = codes[slot]
+        values = rng.integers(64, 128, (length, size)).astype(np.int8)  # one sign: nothing cancels
+        values[codes[slot] > 16] = 0
+        host.pools[1][0, pages, 0, rows] = values
+    q = torch.zeros(len(lengths), tokens, heads, size, device="cuda", dtype=DTYPE[dtype])
+    q[..., 0] = 1.0
+    return host, q
+
+
+def shares(codes, tokens):
+    """The weights' share that is not the sinks', for each token of a block."""
+    out = []
+    for t in range(tokens):
+        seen = codes[:len(codes) - tokens + t + 1].astype(np.float64) / 4
+        w = np.exp(seen - seen.max())
+        out.append(w[codes[:len(seen)] <= 16].sum() / w.sum())
+    return np.array(out)[:, None, None]
+
+
+@pytest.mark.parametrize("dtype", list(DTYPE))
+@pytest.mark.parametrize("size, page, tokens, heads", [(128, 64, 1, 4), (64, 16, 1, 8), (32, 32, 1, 1), (128, 32, 3, 4),
+                                                       (64, 64, 5, 4), (128, 16, 8, 4), (32, 128, 8, 4)])
+@pytest.mark.parametrize("gap", [40, 56, 64, 68, 80, 100])
+def test_one_key_takes_the_weight(dtype, size, page, tokens, heads, gap):
+    """A dominant key with zero values (10 to 25 nats above) before, amid and behind a tail of 8,192 that carries the result."""
+    rng = np.random.default_rng(gap)
+    n = 8192
+    codes = [rng.integers(-2, 3, n) for _ in range(4)]
+    codes[0][:] = 0                       # equal weights: their roundings add up
+    for slot, place in enumerate([0, 5, n // 2, n - tokens]):
+        codes[slot][place] = gap
+    host, q = scored(rng, [n] * 4, codes, size, page, dtype, tokens, heads)
+    cache = to_device(host)
+    got = cache.attend(0, q, scale=1.0)
+    cache.check_errors()
+    want = expected(host, q, range(4), 1.0)
+    for b in range(4):
+        compare(got[b], want[b], 127 * 2.0 ** -6, dtype, shares(codes[b], tokens), 2.0 ** -30 * 2048 / size)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("size, tokens, heads", [(128, 1, 4), (64, 3, 4), (32, 5, 4)])
+def test_scores_that_swing(dtype, size, tokens, heads):
+    """Runs of keys whose scores jump up and down by up to 20 nats, in runs around a step's keys."""
+    rng = np.random.default_rng(size)
+    codes = []
+    for run in (7, 16, 64, 300):
+        codes.append(np.repeat(rng.integers(-64, 17, 5000 // run + 1), run)[:5000])
+    host, q = scored(rng, [5000] * 4, codes, size, 64, dtype, tokens, heads)
+    cache = to_device(host)
+    got = cache.attend(0, q, scale=1.0)
+    cache.check_errors()
+    compare(got, expected(host, q, range(4), 1.0), 127 * 2.0 ** -6, dtype)
+
+
+def test_zero_values_hold_the_weight():
+    """Whole pages of zero values, up to 40 nats above the pages that carry the result, before and behind them."""
+    rng = np.random.default_rng(3)
+    for gap in (20, 60, 100, 127):
+        codes = [rng.integers(-1, 2, 2048) for _ in range(3)]
+        codes[0][:256] = gap
+        codes[1][1024:1280] = gap
+        codes[2][-256:] = gap
+        host, q = scored(rng, [2048] * 3, codes, 128, 64, "f32", 1, 4)
+        for slot in range(3):
+            for column in range(32):
+                page = host.table[slot, column]
+                if not host.pools[1][0, page].any():
+                    host.scales[1][0, page] = 0
+        got, want = to_device(host).attend(0, q, scale=1.0), expected(host, q, range(3), 1.0)
+        for b in range(3):
+            compare(got[b], want[b], 127 * 2.0 ** -6, "f32", shares(codes[b], 1))
