@@ -11,10 +11,17 @@ __device__ __forceinline__ void raise_flag(int* flag, int code) {
   if (flag != nullptr) atomicMax(flag, code);
 }
 
+// Cluster barriers without .aligned: threads of a warp may come to them one by
+// one, out of loops and branches that ended at different times.
+//
 // A cluster's blocks write to one another's shared memory only once all have
 // begun: each arrives first thing, and waits before its first such write.
-__device__ __forceinline__ void cluster_begun() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_all_begun() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_begun() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void cluster_all_begun() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
+// Orders the memory of all threads of the cluster, as __syncthreads that of a block.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
 
 inline int paged_cache_check(const cb_paged_cache& c, const char* who) {
   CB_REQUIRE(c.storage == CB_I8 || c.storage == CB_E4M3, "%s: storage must be int8 or e4m3 (got code %d)", who,

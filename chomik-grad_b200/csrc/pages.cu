@@ -63,7 +63,7 @@ __device__ __forceinline__ long long cluster_scan(long long v, long long* slots,
   cg::cluster_group group = cg::this_cluster();
   const int blocks = static_cast<int>(group.num_blocks()), rank = static_cast<int>(group.block_rank());
   if (static_cast<int>(threadIdx.x) < blocks) *group.map_shared_rank(slots + rank, threadIdx.x) = v;
-  group.sync();
+  cluster_sync();
   long long before = 0, all = 0;
   for (int r = 0; r < blocks; ++r) {
     if (r == rank) before = all;
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(const __grid_constant_
   pdl_wait();
   if (blockIdx.x == 0) extend_book(k, counts, sequences, n, scratch, flag);
   if (gridDim.x == 1) return;
-  cg::this_cluster().sync();
+  cluster_sync();
   const Copies c = copies_of(scratch, n);
   copy_units(p, c.source, c.target, __ldcg(c.count), blockIdx.x * kWarps + threadIdx.x / 32, gridDim.x * kWarps, flag);
 }
@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(kThreads) truncate_kernel(cb_page_book k, cons
     }
     pushed += sum;
   }
-  group.sync();  // every block has used the lengths
+  cluster_sync();  // every block has used the lengths
   if (rank == 0) {
     for (int i = threadIdx.x; i < n; i += kThreads) {
       const int slot = sequences != nullptr ? sequences[i] : i;
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(cb_page_book k, void*
     k.refs[target] = k.refs[source];
     k.refs[source] = 0;
   }
-  group.sync();
+  cluster_sync();
   for (long long e = thread; e < k.slots * k.columns; e += threads) {
     const int page = k.table[e];
     if (page >= pages) raise_flag(flag, CB_FLAG_BOOK);

@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
       }
       *group.map_shared_rank(&cluster[second][rank], threadIdx.x) = mine;
     }
-    group.sync();
+    cluster_sync();
     total = 0;
     for (int r = 0; r < blocks; ++r) {
       if (r == rank) before = total;
