@@ -155,6 +155,8 @@ __device__ __forceinline__ void extend_book(const cb_page_book& k, const int* co
     }
     tails[i] = tail;
   }
+  const int height = *k.height;
+  bad = bad || height < 0 || height > k.pages;
   bool outgrown = false;
   if (__syncthreads_or(bad)) {
     if (threadIdx.x == 0) raise_flag(flag, CB_FLAG_BOOK);
@@ -188,13 +190,26 @@ __device__ __forceinline__ void extend_book(const cb_page_book& k, const int* co
     taken_before += total & 0xffffffffll;
     copied_before += total >> 32;
   }
-  const int height = *k.height;
   // __syncthreads_or also orders the lists above before their use below
-  if (__syncthreads_or(outgrown || taken_before > height || height > k.pages)) {
+  if (__syncthreads_or(outgrown || taken_before > height)) {
     if (threadIdx.x == 0) raise_flag(flag, CB_FLAG_PAGES);
     return;
   }
+  // the pages to take have to be free ones of the pool, each on the stack once:
+  // each is marked, before anything else changes
   const int lane = threadIdx.x & 31;
+  for (long long r = threadIdx.x; r < taken_before; r += kThreads) {
+    const int page = k.free_pages[height - 1 - r];
+    bad = bad || page < 0 || page >= k.pages || atomicCAS(&k.refs[page], 0, -1) != 0;
+  }
+  if (__syncthreads_or(bad)) {
+    if (threadIdx.x == 0) raise_flag(flag, CB_FLAG_BOOK);
+    for (long long r = threadIdx.x; r < taken_before; r += kThreads) {
+      const int page = k.free_pages[height - 1 - r];
+      if (page >= 0 && page < k.pages) atomicCAS(&k.refs[page], -1, 0);
+    }
+    return;
+  }
   for (long long i = threadIdx.x >> 5; i < n; i += kWarps) {
     const long long slot = sequences != nullptr ? sequences[i] : i;
     const bool copied = plan[i] < 0;
@@ -202,10 +217,6 @@ __device__ __forceinline__ void extend_book(const cb_page_book& k, const int* co
     const int base = (k.lengths[slot] + k.page - 1) / k.page - (copied ? 1 : 0);
     for (int m = lane; m < taken; m += 32) {
       const int page = k.free_pages[height - 1 - firsts[i] - m];
-      if (page < 0 || page >= k.pages) {
-        raise_flag(flag, CB_FLAG_BOOK);
-        continue;
-      }
       k.table[slot * k.columns + base + m] = page;
       k.refs[page] = 1;
     }

@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import numpy as np
 import pytest
+import torch
 
 from paged_helpers import filled, same_book, same_pools, to_device
 
@@ -32,3 +33,29 @@ def test_entries_that_end_inside_a_warp(slots, columns):
     cache.check_errors()
     same_book(cache, host)
     same_pools(cache, host)
+
+
+def refused(cache, call):
+    """``call`` raises IndexError at the check and leaves book and pools as they are."""
+    whole = (cache.book, cache.k_pages, cache.k_scale.view(torch.int32))  # (bits: what no slot holds is NaN)
+    before = [t.clone() for t in whole]
+    call()
+    with pytest.raises(IndexError):
+        cache.check_errors()
+    for now, was in zip(whole, before):
+        assert torch.equal(now, was)
+
+
+@pytest.mark.parametrize("bad", ["beyond", "negative", "held", "twice"])
+@pytest.mark.parametrize("depth", [0, 2])
+def test_extend_checks_the_free_stack_first(bad, depth):
+    """An id on the stack that is no free page: as a slot's next page, and as the target of a copy on write."""
+    host = filled(np.random.default_rng(5), [20, 33, 0, 0], spare=8, columns=4)
+    cache = to_device(host)
+    cache.fork([0], [3])  # slot 0's and 3's open page is shared: the first of them to grow copies it
+    height = int(cache.height)
+    cache.free[height - 1 - depth] = {"beyond": cache.pages, "negative": -1, "held": int(cache.table[1, 0]),
+                                      "twice": int(cache.free[height - 2])}[bad]
+    refused(cache, lambda: cache.extend([1, 20, 5, 1]))
+    cache.extend([1, 0, 0, 0][:1 + depth // 2] if depth else [0])  # what takes no page from there goes on
+    cache.check_errors()
