@@ -295,7 +295,8 @@ __global__ void __launch_bounds__(kThreads) truncate_kernel(cb_page_book k, cons
   cg::cluster_group group = cg::this_cluster();
   const int blocks = static_cast<int>(group.num_blocks()), rank = static_cast<int>(group.block_rank());
   const int columns = static_cast<int>(k.columns), entries = n * columns;
-  bool bad = false;
+  const int height = *k.height;
+  bool bad = height < 0 || height > k.pages;
   for (int i = threadIdx.x; i < n; i += kThreads) {  // every block for itself
     const int slot = sequences != nullptr ? sequences[i] : i;
     if (slot < 0 || slot >= k.slots) {
@@ -326,7 +327,6 @@ __global__ void __launch_bounds__(kThreads) truncate_kernel(cb_page_book k, cons
     if (threadIdx.x == 0) raise_flag(flag, CB_FLAG_BOOK);
     return;
   }
-  const int height = *k.height;
   int pages[kKept];
   for (int it = 0, f = begin + threadIdx.x; f < end; ++it, f += kThreads) {
     const int page = page_of(f);

@@ -59,3 +59,13 @@ def test_extend_checks_the_free_stack_first(bad, depth):
     refused(cache, lambda: cache.extend([1, 20, 5, 1]))
     cache.extend([1, 0, 0, 0][:1 + depth // 2] if depth else [0])  # what takes no page from there goes on
     cache.check_errors()
+
+
+@pytest.mark.parametrize("height", [-1, -7, "beyond"])
+def test_heights_outside_the_stack(height):
+    host = filled(np.random.default_rng(6), [40, 33, 0, 0], spare=8, columns=4)
+    cache = to_device(host)
+    cache.height.fill_(cache.pages + 1 if height == "beyond" else height)
+    refused(cache, lambda: cache.extend([30, 1]))
+    refused(cache, lambda: cache.truncate([17, 3]))
+    refused(cache, lambda: cache.release([0, 1]))
