@@ -252,6 +252,7 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(const __grid_constant_
   copy_units(p, c.source, c.target, __ldcg(c.count), blockIdx.x * kWarps + threadIdx.x / 32, gridDim.x * kWarps, flag);
 }
 
+// Each pair by itself: all of it, or where it is refused none.
 __global__ void __launch_bounds__(256) fork_kernel(cb_page_book k, const int* parents, const int* children,
                                                    long long n, int* flag) {
   pdl_launch_dependents();
@@ -261,19 +262,20 @@ __global__ void __launch_bounds__(256) fork_kernel(cb_page_book k, const int* pa
   bool bad = parent < 0 || parent >= k.slots || child < 0 || child >= k.slots;
   for (long long j = threadIdx.x; j < n; j += blockDim.x)
     bad = bad || (j != i && children[j] == child) || parents[j] == child;
-  if (!bad) bad = k.lengths[child] != 0 || k.lengths[parent] < 0 || k.lengths[parent] > k.columns * k.page;
+  const int length = bad ? 0 : k.lengths[parent];
+  if (!bad) bad = k.lengths[child] != 0 || length < 0 || length > k.columns * k.page;
+  for (long long m = threadIdx.x; !bad && m * k.page < length; m += blockDim.x) {
+    const int page = k.table[parent * k.columns + m];
+    bad = page < 0 || page >= k.pages;
+  }
   if (__syncthreads_or(bad)) {
     if (threadIdx.x == 0) raise_flag(flag, CB_FLAG_BOOK);
     return;
   }
-  const int length = k.lengths[parent];
   for (long long m = threadIdx.x; m < k.columns; m += blockDim.x) {
     const int page = k.table[parent * k.columns + m];
     k.table[child * k.columns + m] = page;
-    if (m * k.page < length) {
-      if (page >= 0 && page < k.pages) atomicAdd(&k.refs[page], 1);
-      else raise_flag(flag, CB_FLAG_BOOK);
-    }
+    if (m * k.page < length) atomicAdd(&k.refs[page], 1);
   }
   __syncthreads();  // every thread has seen the child empty
   if (threadIdx.x == 0) k.lengths[child] = length;

@@ -342,7 +342,10 @@ class PagedCache:
             self._stream()), "cb_pages_extend")
 
     def fork(self, parents: Any, children: Any) -> None:
-        """Slot ``children[i]``, which has to be empty, continues slot ``parents[i]`` and shares its pages."""
+        """Slot ``children[i]``, which has to be empty, continues slot ``parents[i]`` and shares its pages.
+
+        Each pair by itself: one that is refused changes nothing, the others are done.
+        """
         parents = self._list(parents, "parents", None)
         n = parents.shape[0]
         children = self._list(children, "children", n)

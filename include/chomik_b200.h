@@ -873,13 +873,18 @@ CB_API long long cb_pages_scratch(const cb_page_book* book, long long n);
 CB_API int cb_pages_extend(const cb_page_book* book, const cb_page_pools* pools, const int* counts,
                            const int* sequences, long long n, void* scratch, int* error_flag, cb_stream_t stream);
 /* Slot children[i], which has to be empty, becomes a copy of slot parents[i]
- * that shares its pages. */
+ * that shares its pages.  Each pair by itself: one that names a slot outside the
+ * table, a child of another pair as its parent, a child twice or one that holds
+ * tokens, or a parent whose row names what is no page, changes nothing and sets
+ * CB_FLAG_BOOK; the call's other pairs are done. */
 CB_API int cb_pages_fork(const cb_page_book* book, const int* parents, const int* children, long long n,
                          int* error_flag, cb_stream_t stream);
 /* The last counts[i] tokens (NULL: all) of slot sequences[i] (NULL: slot i)
  * are dropped, and the pages that hold none of the rest let go: a page that no
  * slot holds any more is pushed, in the reverse order of the last of its
- * dropped table entries.  (So a release undoes the pops of an extend.) */
+ * dropped table entries.  (So a release undoes the pops of an extend.)  Slots,
+ * counts, lengths and a stack height outside their ranges set CB_FLAG_BOOK and
+ * change nothing; a dropped entry that names no page sets it and lets nothing go. */
 CB_API int cb_pages_truncate(const cb_page_book* book, const int* counts, const int* sequences, long long n,
                              int* error_flag, cb_stream_t stream);
 /* The n held pages become pages 0 .. n-1: in ascending order, those beyond

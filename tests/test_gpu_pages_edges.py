@@ -69,3 +69,26 @@ def test_heights_outside_the_stack(height):
     refused(cache, lambda: cache.extend([30, 1]))
     refused(cache, lambda: cache.truncate([17, 3]))
     refused(cache, lambda: cache.release([0, 1]))
+
+
+@pytest.mark.parametrize("page", ["beyond", -1, -5])
+def test_fork_checks_the_parents_pages_first(page):
+    """A row that names a page outside the pool: neither the child's row nor a count changes."""
+    host = filled(np.random.default_rng(7), [40, 33, 0, 0], spare=8, columns=4)
+    cache = to_device(host)
+    cache.table[0, 2] = cache.pages if page == "beyond" else page
+    refused(cache, lambda: cache.fork([0], [2]))
+
+
+def test_fork_decides_for_each_pair():
+    """A pair that is refused leaves the others of the call as they are."""
+    host = filled(np.random.default_rng(8), [40, 33, 0, 0, 0], spare=8, columns=4)
+    for parents, children in (([0, 1], [1, 3]), ([9, 1], [2, 3]), ([1, 0], [3, -1])):
+        cache = to_device(host)
+        cache.fork(parents, children)
+        with pytest.raises(IndexError):
+            cache.check_errors()
+        want = to_device(host)
+        want.fork([1], [3])
+        want.check_errors()
+        assert torch.equal(cache.book, want.book)
