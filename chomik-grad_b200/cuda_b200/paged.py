@@ -32,6 +32,7 @@ import math
 from typing import Any, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -72,10 +73,12 @@ def require(value: torch.Tensor, name: str, device: torch.device, dtypes, shape:
 
 
 def no_grad_needed(*values: torch.Tensor) -> None:
-    """Refuse values that a gradient should flow through."""
+    """Refuse values that a gradient should flow through, backward or as a forward-mode tangent."""
     for value in values:
         if value.requires_grad and torch.is_grad_enabled():
             raise ValueError("an argument requires grad: this operator has no backward pass")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(value).tangent is not None:
+            raise ValueError("an argument has a tangent: this operator has no forward-mode derivative")
 
 
 def current_stream(device: torch.device) -> int:
@@ -280,6 +283,9 @@ class PagedCache:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
             require(out, "out", self.device, (q.dtype,), tuple(q.shape), 4)
+            no_grad_needed(out)
+            if not out.is_inference():  # a backward pass that kept what it held notices
+                torch.autograd.graph.increment_version(out)
         a = _lib.PagedAttentionArgs.from_buffer_copy(known[0])
         a.q, a.out = q.data_ptr(), out.data_ptr()
         if counts is not None:

@@ -1,0 +1,47 @@
+"""Checks of the paged cache's host side on the device."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from cuda_b200 import speculative
+from paged_helpers import filled, to_device
+
+pytestmark = pytest.mark.gpu
+
+
+def test_derivatives_are_refused():
+    cache = to_device(filled(np.random.default_rng(0), [20, 20]))
+    q, rows = torch.randn(2, 1, 4, 64, device="cuda"), torch.randn(2, 1, 2, 64, device="cuda")
+    p = torch.full((1, 2, 4), 0.25, device="cuda")
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(q, torch.ones_like(q))
+        with pytest.raises(ValueError):
+            cache.attend(0, dual)
+        with pytest.raises(ValueError):
+            cache.append(0, rows, forward_ad.make_dual(rows, rows))
+        with pytest.raises(ValueError):
+            speculative.verify(forward_ad.make_dual(p, p), p[:, :1], torch.zeros(1, 1, dtype=torch.int64, device="cuda"),
+                               torch.zeros(1, 2, dtype=torch.float64, device="cuda"))
+    out = torch.zeros_like(q)
+    for bad in (out.clone().requires_grad_(), out.clone().requires_grad_() * 1):
+        with pytest.raises(ValueError):
+            cache.attend(0, q, out=bad)
+    with torch.no_grad():
+        cache.attend(0, q, out=out.clone().requires_grad_())
+
+
+def test_a_kept_activation_that_is_overwritten_is_noticed():
+    """``out`` counts as written in place for a backward pass that kept it."""
+    cache = to_device(filled(np.random.default_rng(0), [20, 20]))
+    q = torch.randn(2, 1, 4, 64, device="cuda")
+    out, weight = cache.attend(0, q), torch.ones(64, device="cuda", requires_grad=True)
+    loss = (out * weight).sum()  # keeps out
+    cache.attend(0, 2 * q, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        cache.attend(0, q, out=torch.empty_like(q))
