@@ -17,12 +17,14 @@ one float32 scale for each page and kv head, and pages can be shared:
     cache.compact()                           # move the held pages to the front of the pools
 
 Values are CUDA ``torch.Tensor`` or the device's ``DeviceArray``.  Every call
-runs on the current stream and reads lengths and tables on the device, with no
-host synchronisation, so a step can be captured in a CUDA graph.  Arguments
-that the host can see are checked at the call (``TypeError``, ``ValueError``);
-what only the device sees (a slot, page, length or count outside its range,
-too few free pages) sets the cache's error flag, which ``check_errors`` reads
-and raises.  There is no backward pass.
+runs on the current stream and reads lengths and tables on the device.  Counts
+and slots are int32 tensors on the device, or lists: a list is copied there
+first, which waits for the host's copy.  With tensors no call synchronises with
+the host, and a step can be captured in a CUDA graph (lists are refused then).
+Arguments that the host can see are checked at the call (``TypeError``,
+``ValueError``); what only the device sees (a slot, page, length or count
+outside its range, too few free pages) sets the cache's error flag, which
+``check_errors`` reads and raises.  There is no backward pass.
 """
 
 from __future__ import annotations
@@ -201,6 +203,8 @@ class PagedCache:
         if value is None or isinstance(value, torch.Tensor):
             return value
         if isinstance(value, (list, tuple)):
+            if torch.cuda.is_current_stream_capturing():
+                raise ValueError("counts and slots have to be int32 tensors on the device while a graph is captured")
             return torch.tensor(value, dtype=torch.int32, device=self.device)
         return tensor_of(value)
 

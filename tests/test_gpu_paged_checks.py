@@ -45,3 +45,28 @@ def test_a_kept_activation_that_is_overwritten_is_noticed():
         loss.backward()
     with torch.inference_mode():
         cache.attend(0, q, out=torch.empty_like(q))
+
+
+def test_lists_are_refused_in_a_capture():
+    """A host list would be copied by the host; the same step with tensors is captured and replayed."""
+    cache = to_device(filled(np.random.default_rng(0), [20, 20], spare=8))
+    rows, q = torch.randn(2, 1, 2, 64, device="cuda"), torch.randn(2, 1, 4, 64, device="cuda")
+    ones, slots = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([1, 1], [0, 1]))
+    out, graph = torch.empty_like(q), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: cache.extend([1, 1]), lambda: cache.append(0, rows, rows, counts=(1, 1)),
+                     lambda: cache.attend(0, q, sequences=[0, 1]), lambda: cache.truncate([1, 1]),
+                     lambda: cache.release([0]), lambda: cache.fork([0], [1]), lambda: cache.copy_pages([0], [1])):
+            with pytest.raises(ValueError, match="captured"):
+                call()
+        cache.extend(ones, sequences=slots)
+        cache.append(0, rows, rows, sequences=slots)
+        cache.attend(0, q, sequences=slots, out=out)
+        cache.truncate(ones, sequences=slots)
+    for _ in range(2):
+        graph.replay()
+    cache.check_errors()
+    assert cache.lengths.tolist() == [20, 20]
+    cache.extend([1, 1])
+    cache.append(0, rows, rows)
+    assert torch.equal(out, cache.attend(0, q))
