@@ -503,6 +503,7 @@ using namespace cb;
 extern "C" {
 
 long long cb_pages_scratch(const cb_page_book* book, long long n) {
+  if (book_check(book, n, "cb_pages_scratch") != CB_OK) return 0;
   // extend: five lists of n; compact: three of the pages
   const long long extend = 5 * n, compact = 3 * book->pages;
   return 4 * (4 + (extend > compact ? extend : compact));

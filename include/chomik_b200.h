@@ -868,7 +868,8 @@ typedef struct {
  * its holders in this call keeps the page itself).  All or nothing: where
  * pages or columns do not suffice, *error_flag is CB_FLAG_PAGES and nothing
  * changes; so too (CB_FLAG_BOOK) where the stack's top holds what is no free
- * page of the pool, or one twice.  scratch: cb_pages_scratch(book, n) bytes. */
+ * page of the pool, or one twice.  scratch: cb_pages_scratch(book, n) bytes
+ * (0 for a book or n that the calls refuse). */
 CB_API long long cb_pages_scratch(const cb_page_book* book, long long n);
 CB_API int cb_pages_extend(const cb_page_book* book, const cb_page_pools* pools, const int* counts,
                            const int* sequences, long long n, void* scratch, int* error_flag, cb_stream_t stream);

@@ -2,11 +2,13 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
-from cuda_b200 import paged
+from cuda_b200 import _lib, paged
 
 
 def test_tangents_are_refused():
@@ -21,3 +23,15 @@ def test_tangents_are_refused():
     with pytest.raises(ValueError, match="tangent"):
         torch.func.jvp(lambda v: paged.no_grad_needed(v) or v, (x,), (torch.ones(3),))
     paged.no_grad_needed(x)
+
+
+def test_scratch_of_no_book_is_nothing():
+    """A size has no error: 0 for books that every call refuses, a null pointer among them."""
+    book = _lib.PageBook(table=16, lengths=16, refs=16, free_pages=16, height=16, slots=4, columns=4, pages=8, page=16)
+    scratch = _lib.load().cb_pages_scratch
+    assert scratch(ctypes.byref(book), 4) == 4 * (4 + 24) and scratch(None, 1) == 0
+    assert scratch(ctypes.byref(book), 5) == 0 and scratch(ctypes.byref(book), -1) == 0
+    for name, value in (("pages", 0), ("pages", 2 ** 31), ("slots", 2 ** 30), ("table", None)):
+        bad = _lib.PageBook.from_buffer_copy(book)
+        setattr(bad, name, value)
+        assert scratch(ctypes.byref(bad), 0) == 0
