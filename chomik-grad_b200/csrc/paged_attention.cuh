@@ -77,13 +77,14 @@ inline Plan plan_of(const cb_paged_attention_args& a, int block_rows, void* scra
 }
 
 // Blocks that fill the GPU once, and no more than there can be tiles; 0 where a
-// launch could have 2^31 units of work to divide.
+// launch could have more units of work than can be divided in 32 bits (they are
+// rounded up to a multiple of the blocks).
 inline long long grid_of(const cb_paged_attention_args& a, int block_rows, int tile, int per_sm) {
   const long long rows = a.tokens * (a.heads / a.cache.kv_heads), blocks = (rows + block_rows - 1) / block_rows;
   const long long tiles = (a.cache.columns * a.cache.page + tile - 1) / tile;
   const double most = static_cast<double>(a.batch) * a.cache.kv_heads * blocks * (tiles + kItemCost);
   const long long fill = 1LL * per_sm * sm_count();
-  if (most >= 2147483648.0) return 0;
+  if (most + static_cast<double>(fill) >= 2147483648.0) return 0;
   return most < fill ? static_cast<long long>(most) : fill;
 }
 
