@@ -136,9 +136,9 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
   PagedRow row;
   if (!paged_row(c, a.sequences, a.counts, a.tokens, b, a.error_flag, &row)) return;
   const int start = row.length - row.count;
-  const int column = start / c.page + static_cast<int>(blockIdx.y);
-  const int first = column * c.page;
-  if (row.count == 0 || first >= row.length) return;
+  const long long column = start / c.page + static_cast<long long>(blockIdx.y);
+  if (row.count == 0 || column * c.page >= row.length) return;
+  const int first = static_cast<int>(column) * c.page;
   const int page = row.table[column];
   if (page < 0 || page >= c.pages) {
     raise_flag(a.error_flag, CB_FLAG_BOOK);

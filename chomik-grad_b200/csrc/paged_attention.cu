@@ -301,8 +301,10 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
     return (tile + piece / kSubs) * tile_keys(SIZE) + group * kKeys + (piece % kSubs) * 16;
   };
   auto ids_of = [&](int batch) {
-    const int piece = batch * 32 + lane, key = piece_key(piece);
-    if (piece >= tiles * kSubs || key >= length) return -1;
+    const int piece = batch * 32 + lane;
+    if (piece >= tiles * kSubs) return -1;
+    const int key = piece_key(piece);
+    if (key >= length) return -1;
     const int page = s.row.table[key >> shift];
     if (page < 0 || page >= c.pages) {
       raise_flag(p.a.error_flag, CB_FLAG_BOOK);
@@ -480,7 +482,7 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
         }
       }
     }
-    if (key + kKeys > common) {  // (the same for the warp) columns 2 quad and 2 quad + 1
+    if (key > common - kKeys) {  // (the same for the warp) columns 2 quad and 2 quad + 1
 #pragma unroll
       for (int at = 0; at < MODE; ++at)
 #pragma unroll

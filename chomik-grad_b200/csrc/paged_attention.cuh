@@ -94,8 +94,8 @@ struct Slot {
 };
 template <int TILE>
 __device__ __forceinline__ int tiles_of(const PagedRow& row) {
-  const int keys = row.count > 0 ? row.length : 0;  // (an item without keys writes zeros)
-  return max(1, (keys + TILE - 1) / TILE);
+  const int keys = row.count > 0 ? row.length : 1;  // (an item without keys writes zeros)
+  return (keys - 1) / TILE + 1;                     // (no sum that passes 2^31)
 }
 template <int TILE>
 __device__ __forceinline__ Slot slot_of(const Plan& p, long long b) {
