@@ -448,7 +448,10 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(cb_page_book k, void*
 int book_check(const cb_page_book* k, long long n, const char* who) {
   CB_REQUIRE(k != nullptr && k->table && k->lengths && k->refs && k->free_pages && k->height, "%s: a null pointer", who);
   CB_REQUIRE(k->slots >= 1 && k->columns >= 1 && k->pages >= 1 && k->page >= 1, "%s: an empty book", who);
-  CB_REQUIRE(k->pages < (1LL << 31) && k->columns * k->page < (1LL << 31) && k->slots * k->columns < (1LL << 31),
+  // (entries are counted in 32 bits and rounded up to a multiple of a cluster's threads)
+  CB_REQUIRE(k->columns * k->page < (1LL << 31) &&
+                 k->slots * k->columns <= (1LL << 31) - kMostBlocks * kThreads * 2 &&
+                 k->pages <= (1LL << 31) - kMostBlocks * kThreads * 2,
              "%s: %lld slots of %lld columns, %lld pages", who, k->slots, k->columns, k->pages);
   CB_REQUIRE(n >= 0 && n <= k->slots, "%s: %lld of %lld slots", who, n, k->slots);
   return CB_OK;

@@ -35,3 +35,13 @@ def test_scratch_of_no_book_is_nothing():
         bad = _lib.PageBook.from_buffer_copy(book)
         setattr(bad, name, value)
         assert scratch(ctypes.byref(bad), 0) == 0
+
+
+@pytest.mark.parametrize("change", [dict(slots=16, columns=2 ** 27 - 100), dict(pages=2 ** 31 - 1024)])
+def test_tables_whose_rounded_entries_pass_32_bits(change):
+    book = _lib.PageBook(table=16, lengths=16, refs=16, free_pages=16, height=16, slots=4, columns=4, pages=8, page=16)
+    for name, value in change.items():
+        setattr(book, name, value)
+    assert _lib.load().cb_pages_scratch(ctypes.byref(book), 1) == 0
+    book.slots, book.pages = min(book.slots, 8), min(book.pages, 2 ** 30)
+    assert _lib.load().cb_pages_scratch(ctypes.byref(book), 1) > 0
