@@ -755,8 +755,7 @@ int cb_paged_attention(const cb_paged_attention_args* args, void* scratch, unsig
   const int status = attention_check(a);
   if (status != CB_OK) return status;
   if (a.batch == 0 || a.tokens == 0) return CB_OK;
-  CB_REQUIRE(a.q != nullptr && a.out != nullptr && scratch != nullptr && counters != nullptr,
-             "cb_paged_attention: a null pointer");
+  CB_REQUIRE(a.q != nullptr && a.out != nullptr && counters != nullptr, "cb_paged_attention: a null pointer");
   CB_REQUIRE(reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && reinterpret_cast<uintptr_t>(scratch) % 16 == 0,
              "cb_paged_attention: out and scratch must be 16-byte aligned");
   return static_cast<int>(with_variant(a, [&](auto size, auto storage, auto mode, auto lo) -> long long {
@@ -766,6 +765,7 @@ int cb_paged_attention(const cb_paged_attention_args* args, void* scratch, unsig
     const long long grid = grid_of(a, rows_of(MODE), tile_keys(SIZE), per_sm);
     CB_REQUIRE(grid > 0, "cb_paged_attention: %lld rows of up to %lld keys are too many for one call",
                a.batch * a.heads * a.tokens, a.cache.columns * a.cache.page);
+    CB_REQUIRE(scratch != nullptr, "cb_paged_attention: a null pointer");
     const Plan p = plan_of(a, rows_of(MODE), scratch, counters);
     launch(attention_kernel<SIZE, STORAGE, MODE, LO>, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
            shared_bytes(SIZE, MODE, LO), static_cast<cudaStream_t>(stream), true, p);

@@ -74,6 +74,12 @@ def require(value: torch.Tensor, name: str, device: torch.device, dtypes, shape:
         step *= value.shape[at]
 
 
+def aligned(value: torch.Tensor, name: str) -> None:
+    """Check that a tensor begins on 16 bytes, as the kernels' wide accesses need it."""
+    if value.data_ptr() % 16:
+        raise ValueError(f"{name} has to begin on a multiple of 16 bytes")
+
+
 def no_grad_needed(*values: torch.Tensor) -> None:
     """Refuse values that a gradient should flow through, backward or as a forward-mode tangent."""
     for value in values:
@@ -142,6 +148,8 @@ class PagedCache:
             raise ValueError("a sequence holds fewer than 2**31 tokens")
         require(k_pages, "k_pages", self.device, tuple(_STORAGE), tuple(k_pages.shape), 5)
         require(v_pages, "v_pages", self.device, (k_pages.dtype,), tuple(k_pages.shape), 5)
+        aligned(k_pages, "k_pages")
+        aligned(v_pages, "v_pages")
         for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
             require(scale, name, self.device, (torch.float32,), tuple(k_pages.shape[:3]), 3)
         rows = self.sequences * self.pages_per_sequence
@@ -287,6 +295,7 @@ class PagedCache:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
             require(out, "out", self.device, (q.dtype,), tuple(q.shape), 4)
+            aligned(out, "out")
             no_grad_needed(out)
             if not out.is_inference():  # a backward pass that kept what it held notices
                 torch.autograd.graph.increment_version(out)

@@ -7,7 +7,8 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from cuda_b200 import speculative
+from cuda_b200 import _lib, speculative
+from cuda_b200.paged import PagedCache
 from paged_helpers import filled, to_device
 
 pytestmark = pytest.mark.gpu
@@ -70,3 +71,26 @@ def test_lists_are_refused_in_a_capture():
     cache.extend([1, 1])
     cache.append(0, rows, rows)
     assert torch.equal(out, cache.attend(0, q))
+
+
+def test_addresses_off_16_bytes_are_value_errors():
+    cache = to_device(filled(np.random.default_rng(0), [20, 20]))
+    q = torch.randn(2, 1, 4, 64, device="cuda")
+    store = torch.zeros(2 * 4 * 64 + 1, device="cuda")
+    with pytest.raises(ValueError, match="16 bytes"):
+        cache.attend(0, q, out=store[1:].view(2, 1, 4, 64))
+    pools = [torch.zeros(cache.k_pages.numel() + 8, dtype=torch.int8, device="cuda")[8:].view(cache.k_pages.shape)
+             for _ in range(2)]
+    for k, v in ((pools[0], cache.v_pages), (cache.k_pages, pools[1])):
+        with pytest.raises(ValueError, match="16 bytes"):
+            PagedCache(k, v, cache.k_scale, cache.v_scale, cache.book, sequences=cache.sequences,
+                       pages_per_sequence=cache.pages_per_sequence)
+
+
+def test_too_much_work_for_one_call_says_so():
+    """Lengths that a table of this many columns could hold, for this many rows: refused before any launch."""
+    cache = PagedCache.allocate(layers=1, pages=1, kv_heads=1, page_size=16, head_size=128, sequences=1,
+                                pages_per_sequence=131_072)
+    q = torch.zeros(65_535, 1, 1, 128, device="cuda")
+    with pytest.raises(_lib.KernelError, match="too many for one call"):
+        cache.attend(0, q, sequences=torch.zeros(65_535, dtype=torch.int32, device="cuda"))
