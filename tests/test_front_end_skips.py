@@ -48,3 +48,6 @@ def test_only_the_missing_front_end_skips(tmp_path):
     child = "def test_it():\n    raise RuntimeError(\"ModuleNotFoundError: No module named 'chomikgrad'\")\n"
     assert outcomes(tmp_path, child).startswith("1 skipped")
     assert outcomes(tmp_path, "import other_chomikgrad\n").startswith("1 error")
+    rank = "def test_it():\n    got = repr(ModuleNotFoundError(\"No module named '{}'\"))\n    assert not got, got\n"
+    assert outcomes(tmp_path, rank.format("chomikgrad")).startswith("1 skipped")
+    assert outcomes(tmp_path, rank.format("whole")).startswith("1 failed")
