@@ -8,10 +8,11 @@
 // is a reduction over the block, so no scale is shared between blocks and no
 // atomics are needed.  What bounds it: the rows are read once and a quarter or
 // half of their bytes written (8 prompts of 2048 tokens, 8 kv heads of 128,
-// bfloat16 to e4m3: 101 MB in 19.8 us, 5.1 TB/s, 79% of the measured copy, with
-// 78% of the issue slots taken; one token of 32 sequences 3.6 us).  The rows stay in registers between the two
-// passes (the largest value, then the codes) up to 8192 elements, which is a
-// page of 64 tokens and a head of 128; beyond that they are read again from L2.
+// bfloat16 to e4m3: 101 MB in 19.9 us, 5.1 TB/s, 78% of the measured copy, with
+// 78% of the issue slots taken; one token of 32 sequences 3.8 us).  The rows stay
+// in registers between the two passes (the largest value, then the codes) up to
+// 8192 elements, which is a page of 64 tokens and a head of 128; beyond that they
+// are read again from L2.
 // The codes take few instructions: without infinities and NaN no clamp is
 // needed (|x| * (1 / s') rounds to at most top), and int8 rounds by adding
 // 1.5 * 2^23, whose low byte is then the code.

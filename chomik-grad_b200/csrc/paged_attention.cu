@@ -6,7 +6,7 @@
 //   out = sum_j exp(s_j - m) vs[page(j), g] vq[j, :] / sum_j exp(s_j - m)
 //
 // What bounds it: the cache is read once, 2 * head_size bytes a key and kv
-// head, for 4 flops a byte and query row.  The rows that share a kv head
+// head, for 2 flops a byte and query row.  The rows that share a kv head
 // (tokens * heads / kv_heads of them) are multiplied together, so that the
 // bytes stay the bound up to about 32 rows; with 8 rows the multiply-adds
 // alone (184 a clock and SM at the measured 6.47 TB/s) are beyond the FP32
@@ -31,23 +31,25 @@
 // How the work is laid out.  The keys of all (slot, kv head, block of rows)
 // are one sequence of tiles, cut into equal ranges for a grid that fills the
 // GPU once, whatever the lengths: each block finds its range from the lengths
-// on the device.  An item that a cut divides leaves partial results (maximum,
+// on the device.  An item that a cut divides leaves partial results (reference,
 // sum, weighted values), which the block that finishes last joins in the order
 // of the keys: equal inputs give equal bits, and there is one launch.
 //
 // Within a tile each warp takes its own 16, 32 or 64 keys (4 KB for any head
-// size) with running maxima of its own, joined at the end of an item: no
+// size) with references of its own, joined at the end of an item: no
 // block barrier inside the loop.  A warp copies its keys through shared memory
 // with 16-byte asynchronous copies, one to three steps ahead; keys beyond the
 // length are filled with zeros, whatever the page holds there.
 //
 // Measured, one B200, 8 kv heads of 128: two sequences of 131,067 keys, e4m3,
-// 4 rows: 94 us, 5.7 TB/s (88% of the measured copy); 32 ragged sequences of up
-// to 4096, int8, 4 rows: 39 us, 4.1 TB/s (3 us until the first products, 5.7
+// 4 rows: 94.5 us, 5.7 TB/s (88% of the measured copy); 32 ragged sequences of up
+// to 4096, int8, 4 rows: 39.5 us, 4.1 TB/s (3 us until the first products, 5.7
 // TB/s after that, blocks' ends 28 to 41 us apart by their share of begins,
-// ends and joins); 16 ragged ones of up to 8191, int8, float16, 20 rows: 69 us,
-// 2.5 TB/s, where 8 warps an SM leave the latency of the instructions open (IPC
-// 1.65, tensor pipe 41%).  One sequence of 384 keys: 7 us of dependent loads.
+// ends and joins); 16 ragged ones of up to 8191, int8, float16, 20 rows: 69 to 72
+// us by where the pool lies in memory, 2.4 TB/s, where 8 warps an SM leave the
+// latency of the instructions open (IPC 1.67, tensor pipe 40%).  One sequence of
+// 384 keys: 7.4 us of dependent loads.  References that follow scores and scales
+// cost 0.4 us of these at the long ones, 0.9 at the batch, 3 in the drafted blocks.
 #include <type_traits>
 
 #include "paged_attention.cuh"

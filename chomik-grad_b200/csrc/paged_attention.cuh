@@ -44,8 +44,9 @@ constexpr uint32_t kNoScale = 0xfc000000u;  // (of no scale but those below -2^1
 // of a step, with a scale like the first, lies between 2^-7 and 2^15, where two
 // fp16 parts hold it to 18 bits at worst and to 22 in the upper half, and the
 // step's others to 2^-25: keys far below one that was seen before keep their
-// bits.  Down by at most kDown at
-// a time, and not where the sums would come near float32's end.
+// bits, and only those that share their step of 2048 / head_size keys with a far
+// heavier one are off, by up to 2^-30 of its weight each.  Down by at most kDown
+// at a time, and not where the sums would come near float32's end.
 constexpr float kWindow = 10.0f, kAbove = 4.0f, kDown = 50.0f, kUnset = -1e30f;
 constexpr int kLift = 4, kRoom = 20;
 

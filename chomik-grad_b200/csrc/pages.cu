@@ -10,12 +10,13 @@
 // of dependent steps, so their time is latency; truncate and compact, whose
 // lists grow with the table and the pool, run as one cluster of up to eight
 // blocks that exchange their counts through distributed shared memory (64
-// slots of 128 pages, half of them released: 12 us; by one block 19).  The
-// copies are bound by memory: a warp for a page of a layer, 8 loads of 16 bytes
-// in flight for each lane, a grid that fills the GPU, launched along with the
-// book's kernel (programmatic dependent launch), which leaves it the list (32
-// sequences compacted, 16 layers, 1.07 GB read and written: 181 us, of which the
-// copies 163 at 6.1 TB/s).
+// slots of 128 pages, half of them released: 13 us; by one block 19).  That the
+// slots of a call differ is found by comparing all pairs, n^2 / 1024 of them a
+// thread.  The copies are bound by memory: a warp for a page of a layer, 8 loads
+// of 16 bytes in flight for each lane, a grid that fills the GPU, launched along
+// with the book's kernel (programmatic dependent launch), which leaves it the
+// list (32 sequences compacted, 16 layers, 1.07 GB read and written: 186 us, of
+// which the copies 163 at 6.1 TB/s).
 #include <cooperative_groups.h>
 
 #include "paged.cuh"
@@ -523,9 +524,9 @@ int cb_pages_extend(const cb_page_book* book, const cb_page_pools* pools, const 
              book->pages);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   // few bytes at most: one cluster does book and copies, in one launch (2.7 us
-  // less for the host).  Its eight SMs copy at about 1 TB/s: 16 slots' open pages
-  // of 22 layers (5.8 MB read and written) took 16 us that way and 10 by a grid
-  // of their own, so that takes over at kClusterCopy.
+  // less for the host).  Its eight SMs copy at about 1 TB/s: with 16 slots' open
+  // pages of 22 layers (5.8 MB read and written) fork and extend took 19.2 us that
+  // way and 12.5 by a grid of their own, so that takes over at kClusterCopy.
   const bool together = 2LL * n * pools->layers * pools->page_bytes <= kClusterCopy;
   status = launch_cluster(extend_kernel, "cb_pages_extend", together ? 1LL * kMostBlocks * kThreads : 1, s, *book, *pools,
                           counts, sequences, n, scratch, error_flag);

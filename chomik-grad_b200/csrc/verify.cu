@@ -13,7 +13,7 @@
 // L2) to find the token.  What bounds it: one target row and, where a draft was
 // refused, one draft row per sequence; in small batches the chain of dependent
 // loads (drafted token, its probabilities, the rows).  Measured: 64 rows of 7
-// drafts and 128,256 float32 probabilities 18.2 us (2 us until the rows, which
+// drafts and 128,256 float32 probabilities 18.0 us (2 us until the rows, which
 // take until 9 to 14, the exchange until 13 to 15, the second read 1.5), one
 // row of 4 drafts and 32,000 4.6 us.
 #include <cooperative_groups.h>

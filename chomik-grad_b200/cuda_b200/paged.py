@@ -284,6 +284,14 @@ class PagedCache:
         ``sequences`` as in ``append``; rows past ``counts[b]`` and rows that
         see nothing give zeros).  ``scale`` is 1/sqrt(head_size) without one.
         Returns (batch, tokens, heads, head_size) of q's dtype.
+
+        Queries and weights go to the tensor cores as fp16 in two parts (22
+        bits) with float32 sums; where more than 8 rows share a kv head,
+        bfloat16 outputs take one part (11 bits) of both and float16 outputs one
+        of the queries.  A key whose weight is below 2^-30 of another's within
+        the same 2048 / head_size keys may be left out.  Every block of rows of a
+        slot walks the slot's whole length, also those past ``counts[b]``: one
+        long chunk with many single tokens costs less in a call of its own.
         """
         q, counts, sequences = tensor_of(q), self._ints(counts), self._ints(sequences)
         no_grad_needed(q)

@@ -160,7 +160,7 @@ def shares(codes, tokens):
                                                        (64, 64, 5, 4), (128, 16, 8, 4), (32, 128, 8, 4)])
 @pytest.mark.parametrize("gap", [40, 56, 64, 68, 80, 100])
 def test_one_key_takes_the_weight(dtype, size, page, tokens, heads, gap):
-    """A dominant key with zero values (10 to 25 nats above) before, amid and behind a tail of 8,192 that carries the result."""
+    """A dominant key of zero values, 10 to 25 nats above 8,192 others that carry the result: first, amid them, last."""
     rng = np.random.default_rng(gap)
     n = 8192
     codes = [rng.integers(-2, 3, n) for _ in range(4)]

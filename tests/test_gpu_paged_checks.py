@@ -25,8 +25,9 @@ def test_derivatives_are_refused():
         with pytest.raises(ValueError):
             cache.append(0, rows, forward_ad.make_dual(rows, rows))
         with pytest.raises(ValueError):
-            speculative.verify(forward_ad.make_dual(p, p), p[:, :1], torch.zeros(1, 1, dtype=torch.int64, device="cuda"),
-                               torch.zeros(1, 2, dtype=torch.float64, device="cuda"))
+            tokens, uniforms = (torch.zeros(1, n, dtype=t, device="cuda") for n, t in ((1, torch.int64),
+                                                                                     (2, torch.float64)))
+            speculative.verify(forward_ad.make_dual(p, p), p[:, :1], tokens, uniforms)
     out = torch.zeros_like(q)
     for bad in (out.clone().requires_grad_(), out.clone().requires_grad_() * 1):
         with pytest.raises(ValueError):
