@@ -1,0 +1,495 @@
+// Products with 4-bit weights and group scales: cb_weights4_linear, and what makes
+// and unmakes such weights (cb_weights4_quantise, _pack, _dequantise).
+//
+//   y[m, n] = sum over groups g of s[n, g] * sum_{k in g} q[n, k] x[m, k],  q in [-8, 7]
+//
+// What bounds it: the weights are read once, half a byte each and 2 bytes for a
+// group's scale, 2 flops a weight and row.  At the measured 6.46 TB/s an SM gets 23
+// bytes a clock, 46 weights: with scalar multiply-adds that would be 46 conversions
+// and as many products for each row, so the products go to the tensor cores
+// (m16n8k16, float32 sums) with the weights as the 16-row operand: up to 8 rows of
+// x cost the same.  The codes are exact in fp16 and bfloat16, so x stays in its own
+// type, and a group's scale multiplies the group's float32 sum.  float32 x is split
+// into three bfloat16 parts (24 bits) that are columns of their own.
+//
+// Layout.  The operand's order of k is free as long as x has the same, so weights
+// are kept as a lane reads them: a block of 16 outputs x 64 inputs is 512 bytes, 16
+// for each lane (row g = lane / 4 and g + 8, c = lane % 4), one word for each
+// product: word s of lane (g, c) holds inputs k = 32 (s / 2) + 8 c + 4 (s % 2) + 0 .. 3
+// of both rows.  Lane (g, c) so needs x[g][32 h + 8 c + 0 .. 7], 16 neighbouring bytes,
+// which come straight from L1: no staging, no barrier before the products.  Code
+// q + 8 of pair i (row g, inputs 0 and 1; row g + 8, the same; row g, inputs 2 and
+// 3; row g + 8) is nibbles i and i + 4: one logic instruction makes two operands of
+// them (see halves_of).
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace cb {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kBlockBytes = 512;   // 16 outputs x 64 inputs
+constexpr int kColumnTiles = 4;    // most of 8 columns that a launch's block takes
+
+__host__ __device__ constexpr long long tiles_of(long long outputs) { return (outputs + 15) / 16; }
+__host__ __device__ constexpr long long chunks_of(long long inputs) { return (inputs + 63) / 64; }
+// Scales of a tile: by chunk (two chunks, for groups of 128), row g, group within the chunk, rows g and g + 8.
+__host__ __device__ constexpr long long tile_scales(long long inputs, int group) {
+  return group == 128 ? (chunks_of(inputs) + 1) / 2 * 16 : chunks_of(inputs) * (64 / group) * 16;
+}
+__host__ __device__ constexpr long long scale_at(long long inputs, int group, long long n, long long at) {
+  const long long tile = n / 16 * tile_scales(inputs, group), row = n % 16;
+  if (group == 32) return tile + at / 2 * 32 + row % 8 * 4 + at % 2 * 2 + row / 8;
+  return tile + at * 16 + row % 8 * 2 + row / 8;
+}
+
+__device__ __forceinline__ float scale_of(uint32_t bits, int dtype) {
+  return dtype == CB_BF16 ? bf16_bits_to_f32(static_cast<uint16_t>(bits))
+                          : __half2float(__ushort_as_half(static_cast<uint16_t>(bits)));
+}
+
+// Pair i of a word as two numbers of the products' type.  bfloat16: the code under
+// the exponent of 128 is 128 + code; fp16: under that of 1024, where the next
+// nibble is in reach too, as 1024 + 16 * code.
+template <bool HALF>
+__device__ __forceinline__ void halves_of(uint32_t w, uint32_t* a) {
+  if (HALF) {
+    const __half2 low = __half2half2(__ushort_as_half(0x6408));                  // 1032
+    const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00)), high = __half2half2(__ushort_as_half(0xd480));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t v = i ? w >> 8 : w;
+      uint32_t x, y;
+      asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(x) : "r"(v));  // (v & mask) | bits
+      asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(y) : "r"(v));
+      __half2 p = __hsub2(*reinterpret_cast<__half2*>(&x), low);
+      __half2 q = __hfma2(*reinterpret_cast<__half2*>(&y), sixteenth, high);     // (1024 + 16 code) / 16 - 72
+      a[2 * i] = *reinterpret_cast<uint32_t*>(&p);
+      a[2 * i + 1] = *reinterpret_cast<uint32_t*>(&q);
+    }
+  } else {
+    const __nv_bfloat162 bias = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));  // 136
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t x;
+      asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(x) : "r"(w >> 4 * i));
+      __nv_bfloat162 p = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&x), bias);
+      a[i] = *reinterpret_cast<uint32_t*>(&p);
+    }
+  }
+}
+
+template <bool HALF>
+__device__ __forceinline__ void product(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if (HALF) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+
+struct LinearPlan {
+  cb_weights4 w;
+  const void* x;  // 16-bit rows, 16-byte aligned
+  long long ld;   // elements between them
+  int rows;       // of x, of all launches' blocks
+  int parts;      // rows of x that a row of y is the sum of: part p of row r is row p * (rows / parts) + r
+  void* out;
+  int out_dtype;
+  long long out_ld;
+  int per;  // rows of y that a block takes
+};
+
+// A block takes one tile of 16 outputs and `per` rows of y.  Its warps take the
+// chunks of 64 inputs in turn and are joined in shared memory, in their order.
+template <bool HALF, int GROUP, int COLUMNS>
+__global__ void __launch_bounds__(kThreads) linear_kernel(const __grid_constant__ LinearPlan p) {
+  constexpr int kScaleWords = GROUP == 32 ? 2 : 1;  // of a lane, for a chunk
+  __shared__ float sums[kWarps][16][8 * COLUMNS + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const long long tile = blockIdx.x;
+  const int chunks = static_cast<int>(chunks_of(p.w.inputs));
+  const int all = p.rows / p.parts, first = static_cast<int>(blockIdx.y) * p.per, mine = min(p.per, all - first);
+  const uint4* codes = static_cast<const uint4*>(p.w.codes) + tile * chunks * 32 + lane;
+  const uint32_t* scales = static_cast<const uint32_t*>(p.w.scales) + tile * tile_scales(p.w.inputs, GROUP) / 2;
+  pdl_launch_dependents();
+  if (mine <= 0) return;
+
+  // column j of the block's: part j / mine of row first + j % mine
+  const uint16_t* x[COLUMNS];
+#pragma unroll
+  for (int t = 0; t < COLUMNS; ++t) {
+    const int j = t * 8 + g;
+    x[t] = j < mine * p.parts
+               ? static_cast<const uint16_t*>(p.x) + (static_cast<long long>(j / mine) * all + first + j % mine) * p.ld + c * 8
+               : nullptr;
+  }
+  float total[COLUMNS][4], sum[COLUMNS][4];
+#pragma unroll
+  for (int t = 0; t < COLUMNS; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) total[t][i] = sum[t][i] = 0.0f;
+  pdl_wait();
+  // groups of 128: a warp takes both chunks of one
+  constexpr int kTogether = GROUP == 128 ? 2 : 1;
+  for (int from = warp * kTogether; from < chunks; from += kWarps * kTogether) {
+#pragma unroll
+    for (int part = 0; part < kTogether; ++part) {
+      const int chunk = from + part;
+      if (chunk >= chunks) break;
+      const uint4 w4 = __ldcs(codes + static_cast<long long>(chunk) * 32);
+      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+      uint32_t s[kScaleWords];
+      if (GROUP == 128) s[0] = __ldg(scales + static_cast<long long>(chunk / 2) * 8 + g);
+      if (GROUP == 64) s[0] = __ldg(scales + static_cast<long long>(chunk) * 8 + g);
+      if (GROUP == 32) {
+        const uint2 two = __ldg(reinterpret_cast<const uint2*>(scales) + static_cast<long long>(chunk) * 8 + g);
+        s[0] = two.x;
+        s[kScaleWords - 1] = two.y;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint4 b[COLUMNS];
+        const long long k = static_cast<long long>(chunk) * 64 + h * 32;
+#pragma unroll
+        for (int t = 0; t < COLUMNS; ++t)
+          b[t] = x[t] != nullptr && k + c * 8 < p.w.inputs ? *reinterpret_cast<const uint4*>(x[t] + k)
+                                                           : make_uint4(0, 0, 0, 0);
+        uint32_t a[4];
+        halves_of<HALF>(w[2 * h], a);
+#pragma unroll
+        for (int t = 0; t < COLUMNS; ++t) product<HALF>(sum[t], a, b[t].x, b[t].y);
+        halves_of<HALF>(w[2 * h + 1], a);
+#pragma unroll
+        for (int t = 0; t < COLUMNS; ++t) product<HALF>(sum[t], a, b[t].z, b[t].w);
+        const bool ends = GROUP == 32 || (h == 1 && (GROUP == 64 || part == 1 || chunk + 1 == chunks));
+        if (ends) {
+          const uint32_t both = s[GROUP == 32 ? h * (kScaleWords - 1) : 0];
+          const float low = scale_of(both & 0xffffu, p.w.scale_dtype), high = scale_of(both >> 16, p.w.scale_dtype);
+#pragma unroll
+          for (int t = 0; t < COLUMNS; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              total[t][i] = fmaf(i < 2 ? low : high, sum[t][i], total[t][i]);
+              sum[t][i] = 0.0f;
+            }
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < COLUMNS; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sums[warp][g + i / 2 * 8][t * 8 + 2 * c + i % 2] = total[t][i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * mine; i += kThreads) {
+    const int n = i % 16, r = i / 16;
+    float y = 0.0f;
+    for (int part = 0; part < p.parts; ++part)
+#pragma unroll
+      for (int v = 0; v < kWarps; ++v) y += sums[v][n][part * mine + r];
+    if (tile * 16 + n < p.w.outputs)
+      store_from_f32(p.out, (first + r) * p.out_ld + tile * 16 + n, p.out_dtype, y);
+  }
+}
+
+// x in a form that the products can read: float32 as three bfloat16 parts, 16-bit
+// rows that do not lie on 16 bytes as they are, in rows of ld elements.
+__global__ void __launch_bounds__(256) arrange_kernel(const void* x, int dtype, long long ld, long long rows,
+                                                      long long inputs, uint16_t* to, long long to_ld) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long at = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= rows * inputs) return;
+  const long long r = at / inputs, k = at % inputs;
+  if (dtype == CB_F32) {
+    float v = static_cast<const float*>(x)[r * ld + k];
+#pragma unroll
+    for (int part = 0; part < 3; ++part) {
+      const __nv_bfloat16 h = __float2bfloat16_rz(v);  // (towards zero: 8 bits each, and nothing becomes infinite)
+      to[(part * rows + r) * to_ld + k] = __bfloat16_as_ushort(h);
+      v -= __bfloat162float(h);
+      if (!isfinite(__bfloat162float(h))) v = 0.0f;  // an infinity or NaN is in the first part alone
+    }
+  } else {
+    to[r * to_ld + k] = static_cast<const uint16_t*>(x)[r * ld + k];
+  }
+}
+
+// ---- making and unmaking weights -----------------------------------------------
+
+// One word of a lane for each thread; outputs and inputs beyond the last have code 8, zero.
+__global__ void __launch_bounds__(256) pack_kernel(const uint8_t* codes, const uint16_t* scales, const cb_weights4 w) {
+  const long long chunks = chunks_of(w.inputs), words = tiles_of(w.outputs) * chunks * 128;
+  const long long at = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (at < words) {
+    const int s = at % 4, lane = at / 4 % 32;
+    const long long tile = at / 128 / chunks, chunk = at / 128 % chunks;
+    const long long k = chunk * 64 + s / 2 * 32 + lane % 4 * 8 + s % 2 * 4;
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long n = tile * 16 + lane / 4 + i % 2 * 8, from = k + i / 2 * 2;
+      const uint32_t byte = n < w.outputs && from < w.inputs ? codes[n * (w.inputs / 2) + from / 2] : 0x88u;
+      word |= (byte & 15u) << 4 * i | byte >> 4 << (16 + 4 * i);
+    }
+    const_cast<uint32_t*>(static_cast<const uint32_t*>(w.codes))[at] = word;
+  }
+  // scales of outputs and groups that do not exist are zero
+  const long long per = tile_scales(w.inputs, w.group), all = tiles_of(w.outputs) * per;
+  const long long groups = w.inputs / w.group;
+  for (long long i = at; i < all; i += static_cast<long long>(gridDim.x) * 256) {
+    const long long tile = i / per, in = i % per;
+    const long long row = w.group == 32 ? in % 32 / 4 + in % 2 * 8 : in % 16 / 2 + in % 2 * 8;
+    const long long group = w.group == 32 ? in / 32 * 2 + in % 4 / 2 : in / 16, n = tile * 16 + row;
+    const_cast<uint16_t*>(static_cast<const uint16_t*>(w.scales))[i] =
+        n < w.outputs && group < groups ? scales[n * groups + group] : 0;
+  }
+}
+
+// A warp to 16 outputs x 64 inputs.
+template <int ITEM>
+__global__ void __launch_bounds__(256) dequantise_kernel(const cb_weights4 w, void* out, int dtype, long long ld,
+                                                         int wide) {
+  const long long chunks = chunks_of(w.inputs);
+  const long long block = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (block >= tiles_of(w.outputs) * chunks) return;
+  const int lane = threadIdx.x & 31;
+  const long long tile = block / chunks, chunk = block % chunks;
+  const uint4 w4 = __ldcs(static_cast<const uint4*>(w.codes) + block * 32 + lane);
+  const uint32_t words[4] = {w4.x, w4.y, w4.z, w4.w};
+  const uint16_t* scales = static_cast<const uint16_t*>(w.scales);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const long long k = chunk * 64 + half * 32 + lane % 4 * 8;
+    if (k >= w.inputs) break;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      const long long n = tile * 16 + lane / 4 + which * 8;
+      if (n >= w.outputs) continue;
+      const float s = scale_of(scales[scale_at(w.inputs, w.group, n, k / w.group)], w.scale_dtype);
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t word = words[2 * half + i / 4];
+        const int pair = i % 4 / 2 * 2 + which;
+        v[i] = (static_cast<float>(word >> (4 * pair + i % 2 * 16) & 15u) - 8.0f) * s;
+      }
+      const long long at = n * ld + k;
+      if (!wide) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) store_from_f32(out, at + i, dtype, v[i]);
+      } else if (ITEM == 4) {
+        float4* to = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
+        to[0] = make_float4(v[0], v[1], v[2], v[3]);
+        to[1] = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (dtype == CB_BF16) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            h[i] = *reinterpret_cast<const uint32_t*>(&b);
+          } else {
+            const __half2 b = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            h[i] = *reinterpret_cast<const uint32_t*>(&b);
+          }
+        }
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+    }
+  }
+}
+
+// A warp to a group: s = rn(max |w| / 7), q = rne(w / s) within [-8, 7].
+__global__ void __launch_bounds__(256) quantise_kernel(const void* weight, int dtype, long long ld, const cb_weights4 w,
+                                                       uint8_t* codes, uint16_t* scales) {
+  const long long groups = w.inputs / w.group;
+  const long long at = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (at >= w.outputs * groups) return;
+  const int lane = threadIdx.x & 31;
+  const long long n = at / groups, k = at % groups * w.group;
+  float largest = 0.0f;
+  bool fine = true;
+  for (int i = lane; i < w.group; i += 32) {
+    const float v = load_as_f32(weight, n * ld + k + i, dtype);
+    fine = fine && isfinite(v);
+    largest = fmaxf(largest, fabsf(v));
+  }
+  largest = warp_max(largest);
+  fine = __all_sync(0xffffffffu, fine);
+  // (a group with an infinity or a NaN has a NaN scale: its products are NaN, not wrong)
+  const float s = round_to(fine ? largest / 7.0f : NAN, w.scale_dtype);
+  if (lane == 0)
+    scales[at] = w.scale_dtype == CB_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(s))
+                                          : __half_as_ushort(__float2half_rn(s));
+  for (int i = 2 * lane; i < w.group; i += 64) {
+    uint32_t byte = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float v = load_as_f32(weight, n * ld + k + i + j, dtype);
+      const float q = s > 0.0f && fine ? fminf(fmaxf(rintf(v / s), -8.0f), 7.0f) : 0.0f;
+      byte |= static_cast<uint32_t>(static_cast<int>(q) + 8) << 4 * j;
+    }
+    codes[n * (w.inputs / 2) + (k + i) / 2] = static_cast<uint8_t>(byte);
+  }
+}
+
+int weights_check(const cb_weights4& w, const char* who) {
+  CB_REQUIRE(w.group == 32 || w.group == 64 || w.group == 128, "%s: groups of 32, 64 or 128 (got %d)", who, w.group);
+  CB_REQUIRE(w.scale_dtype == CB_BF16 || w.scale_dtype == CB_F16, "%s: scales must be bfloat16 or float16", who);
+  CB_REQUIRE(w.outputs >= 1 && w.inputs >= w.group && w.inputs % w.group == 0 && w.outputs < (1LL << 31) &&
+                 w.inputs < (1LL << 31) && tiles_of(w.outputs) * chunks_of(w.inputs) < (1LL << 31),
+             "%s: %lld outputs of %lld inputs in groups of %d", who, w.outputs, w.inputs, w.group);
+  return CB_OK;
+}
+
+int weights_and_pools_check(const cb_weights4& w, const char* who) {
+  const int status = weights_check(w, who);
+  if (status != CB_OK) return status;
+  CB_REQUIRE(w.codes != nullptr && w.scales != nullptr && reinterpret_cast<uintptr_t>(w.codes) % 16 == 0 &&
+                 reinterpret_cast<uintptr_t>(w.scales) % 16 == 0,
+             "%s: codes and scales must be given, aligned to 16 bytes", who);
+  return CB_OK;
+}
+
+bool needs_arranging(const cb_linear4_args& a) {
+  return a.dtype == CB_F32 || reinterpret_cast<uintptr_t>(a.x) % 16 != 0 || (a.rows > 1 && a.ld % 8 != 0);
+}
+
+template <typename F>
+int with_columns(int columns, F f) {
+  if (columns <= 1) return f(std::integral_constant<int, 1>{});
+  if (columns == 2) return f(std::integral_constant<int, 2>{});
+  if (columns == 3) return f(std::integral_constant<int, 3>{});
+  return f(std::integral_constant<int, 4>{});
+}
+
+}  // namespace
+}  // namespace cb
+
+using namespace cb;
+
+extern "C" {
+
+long long cb_weights4_code_bytes(const cb_weights4* weights) {
+  if (weights == nullptr || weights_check(*weights, "cb_weights4_code_bytes") != CB_OK) return 0;
+  return tiles_of(weights->outputs) * chunks_of(weights->inputs) * kBlockBytes;
+}
+
+long long cb_weights4_scale_bytes(const cb_weights4* weights) {
+  if (weights == nullptr || weights_check(*weights, "cb_weights4_scale_bytes") != CB_OK) return 0;
+  return tiles_of(weights->outputs) * tile_scales(weights->inputs, weights->group) * 2;
+}
+
+int cb_weights4_quantise(const cb_weights4* weights, const void* weight, int dtype, long long ld, void* codes,
+                         void* scales, cb_stream_t stream) {
+  CB_REQUIRE(weights != nullptr, "cb_weights4_quantise: null arguments");
+  const cb_weights4& w = *weights;
+  const int status = weights_check(w, "cb_weights4_quantise");
+  if (status != CB_OK) return status;
+  CB_REQUIRE(dtype == CB_F32 || dtype == CB_BF16 || dtype == CB_F16,
+             "cb_weights4_quantise: weights must be float32, bfloat16 or float16");
+  CB_REQUIRE(weight != nullptr && codes != nullptr && scales != nullptr, "cb_weights4_quantise: a null pointer");
+  const long long blocks = (w.outputs * (w.inputs / w.group) + 7) / 8;
+  CB_REQUIRE(blocks < (1LL << 31), "cb_weights4_quantise: %lld outputs of %lld inputs", w.outputs, w.inputs);
+  quantise_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      weight, dtype, ld, w, static_cast<uint8_t*>(codes), static_cast<uint16_t*>(scales));
+  return check_launch("cb_weights4_quantise");
+}
+
+int cb_weights4_pack(const cb_weights4* weights, const void* codes, const void* scales, cb_stream_t stream) {
+  CB_REQUIRE(weights != nullptr, "cb_weights4_pack: null arguments");
+  const cb_weights4& w = *weights;
+  const int status = weights_and_pools_check(w, "cb_weights4_pack");
+  if (status != CB_OK) return status;
+  CB_REQUIRE(codes != nullptr && scales != nullptr, "cb_weights4_pack: a null pointer");
+  const long long blocks = (tiles_of(w.outputs) * chunks_of(w.inputs) * 128 + 255) / 256;
+  CB_REQUIRE(blocks < (1LL << 31), "cb_weights4_pack: %lld outputs of %lld inputs", w.outputs, w.inputs);
+  pack_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint8_t*>(codes), static_cast<const uint16_t*>(scales), w);
+  return check_launch("cb_weights4_pack");
+}
+
+int cb_weights4_dequantise(const cb_weights4* weights, void* out, int dtype, long long ld, cb_stream_t stream) {
+  CB_REQUIRE(weights != nullptr, "cb_weights4_dequantise: null arguments");
+  const cb_weights4& w = *weights;
+  const int status = weights_and_pools_check(w, "cb_weights4_dequantise");
+  if (status != CB_OK) return status;
+  CB_REQUIRE(dtype == CB_F32 || dtype == CB_BF16 || dtype == CB_F16,
+             "cb_weights4_dequantise: out must be float32, bfloat16 or float16");
+  CB_REQUIRE(out != nullptr && ld >= w.inputs, "cb_weights4_dequantise: rows of %lld elements", ld);
+  const int item = dtype == CB_F32 ? 4 : 2;
+  const int wide = reinterpret_cast<uintptr_t>(out) % 16 == 0 && ld * item % 16 == 0;
+  const unsigned blocks = static_cast<unsigned>((tiles_of(w.outputs) * chunks_of(w.inputs) + 7) / 8);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (item == 4) dequantise_kernel<4><<<blocks, 256, 0, s>>>(w, out, dtype, ld, wide);
+  else dequantise_kernel<2><<<blocks, 256, 0, s>>>(w, out, dtype, ld, wide);
+  return check_launch("cb_weights4_dequantise");
+}
+
+long long cb_linear4_scratch(const cb_linear4_args* args) {
+  if (args == nullptr || args->rows <= 0 || !needs_arranging(*args)) return 0;
+  return args->rows * (args->dtype == CB_F32 ? 3 : 1) * args->weights.inputs * 2;
+}
+
+int cb_linear4(const cb_linear4_args* args, void* scratch, cb_stream_t stream) {
+  CB_REQUIRE(args != nullptr, "cb_linear4: null arguments");
+  const cb_linear4_args& a = *args;
+  const int status = weights_and_pools_check(a.weights, "cb_linear4");
+  if (status != CB_OK) return status;
+  CB_REQUIRE(a.dtype == CB_F32 || a.dtype == CB_BF16 || a.dtype == CB_F16,
+             "cb_linear4: x must be float32, bfloat16 or float16");
+  CB_REQUIRE(a.rows >= 0 && a.rows < (1LL << 24), "cb_linear4: %lld rows", a.rows);
+  if (a.rows == 0) return CB_OK;
+  CB_REQUIRE(a.x != nullptr && a.out != nullptr, "cb_linear4: a null pointer");
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  LinearPlan p = {};
+  p.w = a.weights;
+  p.x = a.x;
+  p.ld = a.ld;
+  p.parts = a.dtype == CB_F32 ? 3 : 1;
+  p.rows = static_cast<int>(a.rows * p.parts);
+  p.out = a.out;
+  p.out_dtype = a.dtype;
+  p.out_ld = a.out_ld;
+  if (needs_arranging(a)) {
+    CB_REQUIRE(scratch != nullptr && reinterpret_cast<uintptr_t>(scratch) % 16 == 0,
+               "cb_linear4: %lld bytes of scratch are needed, aligned to 16", cb_linear4_scratch(args));
+    const long long blocks = (a.rows * a.weights.inputs + 255) / 256;
+    CB_REQUIRE(blocks < (1LL << 31), "cb_linear4: %lld rows of %lld", a.rows, a.weights.inputs);
+    launch(arrange_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, true, a.x, a.dtype, a.ld, a.rows,
+           a.weights.inputs, static_cast<uint16_t*>(scratch), a.weights.inputs);
+    const int arranged = check_launch("cb_linear4");
+    if (arranged != CB_OK) return arranged;
+    p.x = scratch;
+    p.ld = a.weights.inputs;
+  }
+  const int most = kColumnTiles * 8 / p.parts;
+  const int launches = static_cast<int>((a.rows + most - 1) / most);
+  CB_REQUIRE(launches <= 65535, "cb_linear4: %lld rows", a.rows);
+  p.per = static_cast<int>((a.rows + launches - 1) / launches);
+  return with_columns((p.per * p.parts + 7) / 8, [&](auto columns) {
+    constexpr int C = columns.value;
+    const dim3 grid(static_cast<unsigned>(tiles_of(a.weights.outputs)), static_cast<unsigned>(launches));
+    auto go = [&](auto kernel) {
+      launch(kernel, grid, dim3(kThreads), 0, s, true, p);
+      return check_launch("cb_linear4");
+    };
+    const bool half = a.dtype == CB_F16;
+    if (a.weights.group == 32) return half ? go(linear_kernel<true, 32, C>) : go(linear_kernel<false, 32, C>);
+    if (a.weights.group == 64) return half ? go(linear_kernel<true, 64, C>) : go(linear_kernel<false, 64, C>);
+    return half ? go(linear_kernel<true, 128, C>) : go(linear_kernel<false, 128, C>);
+  });
+}
+
+}  // extern "C"

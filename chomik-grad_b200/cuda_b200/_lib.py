@@ -283,6 +283,34 @@ class VerifyArgs(ctypes.Structure):
     ]
 
 
+class Weights4Args(ctypes.Structure):
+    _fields_ = [
+        ("codes", c_void_p), ("scales", c_void_p), ("scale_dtype", c_int), ("group", c_int),
+        ("outputs", c_longlong), ("inputs", c_longlong),
+    ]
+
+
+class Linear4Args(ctypes.Structure):
+    _fields_ = [
+        ("weights", Weights4Args), ("x", c_void_p), ("dtype", c_int), ("rows", c_longlong), ("ld", c_longlong),
+        ("out", c_void_p), ("out_ld", c_longlong),
+    ]
+
+
+class AdjustArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", c_void_p), ("dtype", c_int), ("rows", c_longlong), ("vocab", c_longlong), ("ld", c_longlong),
+        ("out", c_void_p), ("out_ld", c_longlong),
+        ("tokens", c_void_p), ("token_dtype", c_int), ("history", c_longlong), ("token_ld", c_longlong),
+        ("lengths", c_void_p), ("prompts", c_void_p),
+        ("repetitions", c_void_p), ("frequencies", c_void_p), ("presences", c_void_p),
+        ("repetition", c_float), ("frequency", c_float), ("presence", c_float),
+        ("bias_tokens", c_void_p), ("bias_token_dtype", c_int), ("bias", c_void_p),
+        ("biases", c_longlong), ("bias_token_ld", c_longlong), ("bias_ld", c_longlong),
+        ("allowed", c_void_p), ("allowed_ld", c_longlong), ("error_flag", c_void_p),
+    ]
+
+
 class KernelError(RuntimeError):
     """A libchomik_b200 entry point returned a non-zero status."""
 
@@ -362,6 +390,14 @@ _SIGNATURES = {
                                      c_void_p, c_void_p, c_void_p, c_void_p], c_int),
     "cb_sgd_update": ([c_void_p, c_void_p], c_int),
     "cb_sample_rows": ([c_void_p, c_void_p], c_int),
+    "cb_weights4_code_bytes": ([POINTER(Weights4Args)], c_longlong),
+    "cb_weights4_scale_bytes": ([POINTER(Weights4Args)], c_longlong),
+    "cb_weights4_quantise": ([POINTER(Weights4Args), c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_void_p], c_int),
+    "cb_weights4_pack": ([POINTER(Weights4Args), c_void_p, c_void_p, c_void_p], c_int),
+    "cb_weights4_dequantise": ([POINTER(Weights4Args), c_void_p, c_int, c_longlong, c_void_p], c_int),
+    "cb_linear4_scratch": ([POINTER(Linear4Args)], c_longlong),
+    "cb_linear4": ([POINTER(Linear4Args), c_void_p, c_void_p], c_int),
+    "cb_adjust_logits": ([POINTER(AdjustArgs), c_void_p], c_int),
     "cb_paged_append": ([POINTER(PagedAppendArgs), c_void_p], c_int),
     "cb_paged_attention_scratch": ([POINTER(PagedAttentionArgs)], c_longlong),
     "cb_paged_attention_counters": ([POINTER(PagedAttentionArgs)], c_longlong),
@@ -406,6 +442,7 @@ FLAG_WAIT_DATA, FLAG_WAIT_SLOT, FLAG_WAIT_DRAIN, FLAG_WAIT_PHASE = 4, 5, 6, 7
 FLAG_NAN = 8
 FLAG_WAIT_PEER = 9
 FLAG_PAGES, FLAG_BOOK = 10, 11
+FLAG_HISTORY = 12
 
 
 def flag_error(value: int) -> Exception:
@@ -422,6 +459,8 @@ def flag_error(value: int) -> Exception:
         return MemoryError("the cache has too few free pages, or a sequence would outgrow its table row")
     if value == FLAG_BOOK:
         return IndexError("a sequence, page, length or count of the paged cache is outside its range")
+    if value == FLAG_HISTORY:
+        return IndexError("a length of the token history is outside its range")
     waits = {FLAG_WAIT_DATA: "a consumer waiting for weight data",
              FLAG_WAIT_SLOT: "a producer waiting for a free ring slot",
              FLAG_WAIT_DRAIN: "the end-of-kernel drain of bulk copies",

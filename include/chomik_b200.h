@@ -45,7 +45,8 @@ enum {
   CB_FLAG_NAN = 8,        /* cb_sample_rows: NaN probabilities */
   CB_FLAG_WAIT_PEER = 9,  /* cb_peer_all_reduce: a rank of the group did not arrive in time */
   CB_FLAG_PAGES = 10,     /* cb_pages_extend: the free pages or a table row's columns do not suffice */
-  CB_FLAG_BOOK = 11       /* cb_paged_*, cb_pages_*: a slot, page, length or count outside its range */
+  CB_FLAG_BOOK = 11,      /* cb_paged_*, cb_pages_*: a slot, page, length or count outside its range */
+  CB_FLAG_HISTORY = 12    /* cb_adjust_logits: a length of a row's history outside its range */
 };
 
 #define CB_MAX_DIMS 8
@@ -762,6 +763,88 @@ typedef struct {
   int* error_flag;             /* optional: CB_FLAG_NAN */
 } cb_sample_args;
 CB_API int cb_sample_rows(const cb_sample_args* a, cb_stream_t stream);
+
+/* ---- 4-bit weights with group scales ----------------------------------------
+ * The Linear of the graphs, inputs @ weight.T (chomikgrad/llama.py:275-277),
+ * with weights of 4 bits: w[n][k] = scale[n][k / group] * q[n][k], q in [-8, 7].
+ * `codes` and `scales` hold them in the order in which the products read them
+ * (cb_weights4_code_bytes and cb_weights4_scale_bytes of them, 16-byte aligned);
+ * the plain form, which cb_weights4_quantise writes and cb_weights4_pack takes, is
+ * (outputs, inputs / 2) bytes, input 2 i in the low half of byte i and 2 i + 1 in the
+ * high one, each as q + 8, and (outputs, inputs / group) scales. */
+typedef struct {
+  const void* codes;
+  const void* scales;
+  int scale_dtype; /* CB_BF16 or CB_F16 */
+  int group;       /* 32, 64 or 128 inputs */
+  long long outputs, inputs; /* inputs: a multiple of the group */
+} cb_weights4;
+CB_API long long cb_weights4_code_bytes(const cb_weights4* weights);
+CB_API long long cb_weights4_scale_bytes(const cb_weights4* weights);
+/* The plain form of weights (float32, bfloat16 or float16, rows of ld elements):
+ * scale = max |w| / 7 over a group, rounded to its type, q = w / scale rounded to
+ * the nearest (ties to even) within [-8, 7]; of a group with an infinity or a NaN
+ * the scale is NaN.  The pointers in `weights` are not read. */
+CB_API int cb_weights4_quantise(const cb_weights4* weights, const void* weight, int dtype, long long ld, void* codes,
+                                void* scales, cb_stream_t stream);
+/* The plain form into weights->codes and weights->scales. */
+CB_API int cb_weights4_pack(const cb_weights4* weights, const void* codes, const void* scales, cb_stream_t stream);
+/* The weights as (outputs, inputs) numbers, each rounded once, in rows of ld elements. */
+CB_API int cb_weights4_dequantise(const cb_weights4* weights, void* out, int dtype, long long ld, cb_stream_t stream);
+
+/* out[r] = x[r] @ weights.T: rows of x and out have ld and out_ld elements and
+ * one type, CB_F32, CB_BF16 or CB_F16; sums are float32, rounded once.  Up to 8
+ * rows cost about what one costs, and every 32 rows (10 of float32) read the
+ * weights again.  `scratch`: cb_linear4_scratch bytes (0 for 16-bit rows that
+ * lie on 16 bytes), 16-byte aligned. */
+typedef struct {
+  cb_weights4 weights;
+  const void* x;
+  int dtype;
+  long long rows, ld;
+  void* out;
+  long long out_ld;
+} cb_linear4_args;
+CB_API long long cb_linear4_scratch(const cb_linear4_args* args);
+CB_API int cb_linear4(const cb_linear4_args* args, void* scratch, cb_stream_t stream);
+
+/* ---- penalties, biases and masks on logits ---------------------------------
+ * What a sampler applies to logit rows before cb_sample_rows chooses (not in
+ * the reference, whose sampler has temperature and top-k only,
+ * examples/generate_tinyllama.py:124-143).  With c and d the times that token v
+ * occurs in the row's first lengths[row] history tokens, and among those from
+ * prompts[row] on:
+ *   x = logits[v], times (where it is above 0: divided by) the repetition if c > 0
+ *   x = x - (frequency * d + presence * [d > 0]) + the biases listed for v
+ *   x = -inf where bit v % 32 of allowed[v / 32] is clear
+ * in float32, rounded once.  History tokens and biases of tokens outside the
+ * vocabulary are passed over (a -1 pads a list); a token listed twice gets the sum, in
+ * the list's order.  A length outside [0, history] or a prompt outside [0,
+ * length] is taken as the nearest end, with CB_FLAG_HISTORY.  A row whose mask
+ * leaves nothing is -inf throughout.  out may be logits (with out_ld == ld);
+ * other overlaps are not allowed. */
+typedef struct {
+  const void* logits; /* rows of ld elements, CB_F32, CB_BF16 or CB_F16 */
+  int dtype;
+  long long rows, vocab, ld;
+  void* out; /* the same type, rows of out_ld elements */
+  long long out_ld;
+  const void* tokens; /* optional history: rows of token_ld elements, CB_I32 or CB_I64 */
+  int token_dtype;
+  long long history, token_ld;
+  const int* lengths; /* optional, one for each row: history without */
+  const int* prompts; /* optional, one for each row: 0 without */
+  const float *repetitions, *frequencies, *presences; /* optional, one for each row */
+  float repetition, frequency, presence;              /* of all rows without */
+  const void* bias_tokens; /* rows of bias_token_ld elements, CB_I32 or CB_I64 */
+  int bias_token_dtype;
+  const float* bias; /* rows of bias_ld elements */
+  long long biases, bias_token_ld, bias_ld; /* at most 1024 to a row */
+  const int* allowed; /* optional: rows of allowed_ld words, ceil(vocab / 32) of them used */
+  long long allowed_ld;
+  int* error_flag; /* optional */
+} cb_adjust_args;
+CB_API int cb_adjust_logits(const cb_adjust_args* args, cb_stream_t stream);
 
 /* ---- paged 8-bit KV cache --------------------------------------------------
  * The cache of a serving program: sequences of unlike lengths, each a row of
