@@ -578,7 +578,8 @@ __device__ __forceinline__ void warp_item(const Plan& p, const void* query, cons
   }
 }
 
-template <int SIZE, int STORAGE, int MODE, int LO>
+// SHARED: of the keys behind those that all sequences have in common, whose sums are joined at the end.
+template <int SIZE, int STORAGE, int MODE, int LO, bool SHARED>
 __global__ void __launch_bounds__(kThreads, resident_of(MODE)) attention_kernel(const __grid_constant__ Plan p) {
   constexpr int kRows = rows_of(MODE);
   extern __shared__ __align__(128) char shared[];
@@ -588,8 +589,10 @@ __global__ void __launch_bounds__(kThreads, resident_of(MODE)) attention_kernel(
 
   pdl_launch_dependents();
   pdl_wait();
+  const int pages = SHARED ? common_pages(p.shared, p.a.batch, found) : 0;
+  if (SHARED) __syncthreads();  // (found is used again)
   Walk<tile_keys(SIZE)> walk;
-  if (!begin_walk<tile_keys(SIZE), kGroups>(p, scan, found, &walk)) return;
+  if (!begin_walk<tile_keys(SIZE), kGroups>(p, pages, scan, found, &walk)) return;
   Segment seg;
   while (walk.next(p, &seg)) {
     const int b = seg.b, head = seg.item / p.blocks, first_row = seg.item % p.blocks * kRows;
@@ -643,6 +646,8 @@ __global__ void __launch_bounds__(kThreads, resident_of(MODE)) attention_kernel(
       const int row = first_row + r;
       if (seg.whole) {
         if (row < p.rows) {
+          if (SHARED && pages > 0 && row / p.group < seg.s.row.count)
+            add_shared<SIZE>(p, pages, static_cast<long long>(b) * p.rows + row, head, d, &top, &sum, v);
           const bool real = row / p.group < seg.s.row.count && sum != 0.0f;
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[k] = real ? v[k] / sum : 0.0f;
@@ -661,9 +666,9 @@ __global__ void __launch_bounds__(kThreads, resident_of(MODE)) attention_kernel(
       if (threadIdx.x == 0) found[0] = last_part(p, seg);
       __syncthreads();
       if (found[0])  // (its first part is the first of its block's range, or the second)
-        join<SIZE, kRows>(p, b, head, first_row, seg.s.row.count, seg.last - seg.from + 1,
-                          part_of<SIZE, kRows>(p, seg.from, seg.from_begins), part_of<SIZE, kRows>(p, seg.from, true),
-                          threadIdx.x, kThreads);
+        join<SIZE, kRows, SHARED>(p, b, head, first_row, seg.s.row.count, seg.last - seg.from + 1,
+                                  part_of<SIZE, kRows>(p, seg.from, seg.from_begins),
+                                  part_of<SIZE, kRows>(p, seg.from, true), pages, threadIdx.x, kThreads);
     }
     __syncthreads();  // the joined rows are read; the ring is free again
   }
@@ -671,26 +676,13 @@ __global__ void __launch_bounds__(kThreads, resident_of(MODE)) attention_kernel(
 
 // ---- launch --------------------------------------------------------------------
 
-int attention_check(const cb_paged_attention_args& a) {
-  const int status = paged_cache_check(a.cache, "cb_paged_attention");
-  if (status != CB_OK) return status;
-  CB_REQUIRE(a.dtype == CB_F32 || a.dtype == CB_BF16 || a.dtype == CB_F16,
-             "cb_paged_attention: q must be float32, bfloat16 or float16");
-  CB_REQUIRE(a.heads >= 1 && a.heads <= (1 << 20) && a.heads % a.cache.kv_heads == 0,
-             "cb_paged_attention: %lld heads for %d kv heads", a.heads, a.cache.kv_heads);
-  CB_REQUIRE(a.batch >= 0 && a.batch <= 65535 && a.tokens >= 0 && a.tokens <= 65535 &&
-                 a.tokens * (a.heads / a.cache.kv_heads) < (1LL << 30),
-             "cb_paged_attention: %lld sequences of %lld tokens", a.batch, a.tokens);
-  return CB_OK;
-}
-
-template <int SIZE, int STORAGE, int MODE, int LO>
+template <int SIZE, int STORAGE, int MODE, int LO, bool SHARED>
 int resident_blocks() {
   static thread_local int device = -1, per_sm = 0;
   int now = 0;
   cudaGetDevice(&now);
   if (now != device) {
-    auto kernel = attention_kernel<SIZE, STORAGE, MODE, LO>;
+    auto kernel = attention_kernel<SIZE, STORAGE, MODE, LO, SHARED>;
     constexpr int kShared = shared_bytes(SIZE, MODE, LO);
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared) != cudaSuccess ||
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, kShared) != cudaSuccess)
@@ -731,6 +723,42 @@ long long with_variant(const cb_paged_attention_args& a, F f) {
 }
 
 }  // namespace
+
+long long attention_scratch(const cb_paged_attention_args& a, bool shared) {
+  if (a.batch == 0 || a.tokens == 0) return 0;
+  return with_variant(a, [&](auto size, auto storage, auto mode, auto lo) -> long long {
+    const int per_sm = shared ? resident_blocks<size.value, storage.value, mode.value, lo.value, true>()
+                              : resident_blocks<size.value, storage.value, mode.value, lo.value, false>();
+    return grid_of(a, rows_of(mode.value), tile_keys(size.value), per_sm) * 8LL *
+           partial_floats(size.value, rows_of(mode.value));
+  });
+}
+
+int launch_attention(const cb_paged_attention_args& a, const SharedKeys* shared, void* scratch, unsigned* counters,
+                     cudaStream_t stream) {
+  const char* who = shared != nullptr ? "cb_paged_attention_shared" : "cb_paged_attention";
+  CB_REQUIRE(a.q != nullptr && a.out != nullptr && counters != nullptr, "%s: a null pointer", who);
+  CB_REQUIRE(reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && reinterpret_cast<uintptr_t>(scratch) % 16 == 0,
+             "%s: out and scratch must be 16-byte aligned", who);
+  return static_cast<int>(with_variant(a, [&](auto size, auto storage, auto mode, auto lo) -> long long {
+    constexpr int SIZE = size.value, STORAGE = storage.value, MODE = mode.value, LO = lo.value;
+    auto go = [&](auto kernel, int per_sm) -> int {
+      CB_REQUIRE(per_sm >= 1 && per_sm <= 8, "%s: %d blocks of the kernel fit an SM", who, per_sm);
+      const long long grid = grid_of(a, rows_of(MODE), tile_keys(SIZE), per_sm);
+      CB_REQUIRE(grid > 0, "%s: %lld rows of up to %lld keys are too many for one call", who,
+                 a.batch * a.heads * a.tokens, a.cache.columns * a.cache.page);
+      CB_REQUIRE(scratch != nullptr, "%s: a null pointer", who);
+      Plan p = plan_of(a, rows_of(MODE), scratch, counters);
+      p.shared = shared != nullptr ? *shared : SharedKeys{};
+      launch(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), shared_bytes(SIZE, MODE, LO), stream, true, p);
+      return check_launch(who);
+    };
+    if (shared != nullptr)
+      return go(attention_kernel<SIZE, STORAGE, MODE, LO, true>, resident_blocks<SIZE, STORAGE, MODE, LO, true>());
+    return go(attention_kernel<SIZE, STORAGE, MODE, LO, false>, resident_blocks<SIZE, STORAGE, MODE, LO, false>());
+  }));
+}
+
 }  // namespace cb
 
 using namespace cb;
@@ -738,41 +766,21 @@ using namespace cb;
 extern "C" {
 
 long long cb_paged_attention_scratch(const cb_paged_attention_args* args) {
-  if (args == nullptr || attention_check(*args) != CB_OK || args->batch == 0 || args->tokens == 0) return 0;
-  return with_variant(*args, [&](auto size, auto storage, auto mode, auto lo) -> long long {
-    const int per_sm = resident_blocks<size.value, storage.value, mode.value, lo.value>();
-    return grid_of(*args, rows_of(mode.value), tile_keys(size.value), per_sm) * 8LL *
-           partial_floats(size.value, rows_of(mode.value));
-  });
+  if (args == nullptr || attention_check(*args, "cb_paged_attention") != CB_OK) return 0;
+  return attention_scratch(*args, false);
 }
 
 long long cb_paged_attention_counters(const cb_paged_attention_args* args) {
-  if (args == nullptr || attention_check(*args) != CB_OK) return 0;
+  if (args == nullptr || attention_check(*args, "cb_paged_attention") != CB_OK) return 0;
   return 8LL * sm_count();  // more than any launch has blocks
 }
 
 int cb_paged_attention(const cb_paged_attention_args* args, void* scratch, unsigned* counters, cb_stream_t stream) {
   CB_REQUIRE(args != nullptr, "cb_paged_attention: null arguments");
-  const cb_paged_attention_args& a = *args;
-  const int status = attention_check(a);
+  const int status = attention_check(*args, "cb_paged_attention");
   if (status != CB_OK) return status;
-  if (a.batch == 0 || a.tokens == 0) return CB_OK;
-  CB_REQUIRE(a.q != nullptr && a.out != nullptr && counters != nullptr, "cb_paged_attention: a null pointer");
-  CB_REQUIRE(reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && reinterpret_cast<uintptr_t>(scratch) % 16 == 0,
-             "cb_paged_attention: out and scratch must be 16-byte aligned");
-  return static_cast<int>(with_variant(a, [&](auto size, auto storage, auto mode, auto lo) -> long long {
-    constexpr int SIZE = size.value, STORAGE = storage.value, MODE = mode.value, LO = lo.value;
-    const int per_sm = resident_blocks<SIZE, STORAGE, MODE, LO>();
-    CB_REQUIRE(per_sm >= 1 && per_sm <= 8, "cb_paged_attention: %d blocks of the kernel fit an SM", per_sm);
-    const long long grid = grid_of(a, rows_of(MODE), tile_keys(SIZE), per_sm);
-    CB_REQUIRE(grid > 0, "cb_paged_attention: %lld rows of up to %lld keys are too many for one call",
-               a.batch * a.heads * a.tokens, a.cache.columns * a.cache.page);
-    CB_REQUIRE(scratch != nullptr, "cb_paged_attention: a null pointer");
-    const Plan p = plan_of(a, rows_of(MODE), scratch, counters);
-    launch(attention_kernel<SIZE, STORAGE, MODE, LO>, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
-           shared_bytes(SIZE, MODE, LO), static_cast<cudaStream_t>(stream), true, p);
-    return check_launch("cb_paged_attention");
-  }));
+  if (args->batch == 0 || args->tokens == 0) return CB_OK;
+  return launch_attention(*args, nullptr, scratch, counters, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

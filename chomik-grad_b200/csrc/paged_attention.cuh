@@ -1,11 +1,47 @@
-// Shared by the kernels of cb_paged_attention: the division of the work over a
-// launch's blocks, and the results that several blocks join.
+// Shared by the kernels of cb_paged_attention and cb_paged_attention_shared: the
+// division of the work over a launch's blocks, and the results that several
+// blocks join.
 #pragma once
+
+#include <climits>
 
 #include "paged.cuh"
 #include "sync.cuh"
 
 namespace cb {
+
+// The first keys of all sequences of a call, computed apart (paged_shared.cu).
+// `common`: for each sequence the whole pages that it has in common with the
+// call's first; INT_MAX where it takes no part.  The rows of a kv head, those
+// of all sequences, go in blocks of `block_rows`, and the keys of all (kv head,
+// block of rows) in tiles of kSharedTile are cut into equal ranges.  Range c's
+// part of item i is parts (i + c) * ways .. + ways - 1: references of block_rows
+// rows, their sums, then the rows.
+constexpr int kSharedTile = 64;
+struct SharedKeys {
+  const int* common;  // and behind them the slot of the first sequence that takes part
+  const float* parts;
+  int block_rows, ways, ranges, least;  // tiles of a range: `least` or more
+};
+// cb_paged_attention's launch, of the keys behind the shared ones where `shared` is given.
+int launch_attention(const cb_paged_attention_args& a, const SharedKeys* shared, void* scratch, unsigned* counters,
+                     cudaStream_t stream);
+// Bytes of scratch that it needs.
+long long attention_scratch(const cb_paged_attention_args& a, bool shared);
+
+inline int attention_check(const cb_paged_attention_args& a, const char* who) {
+  const int status = paged_cache_check(a.cache, who);
+  if (status != CB_OK) return status;
+  CB_REQUIRE(a.dtype == CB_F32 || a.dtype == CB_BF16 || a.dtype == CB_F16,
+             "%s: q must be float32, bfloat16 or float16", who);
+  CB_REQUIRE(a.heads >= 1 && a.heads <= (1 << 20) && a.heads % a.cache.kv_heads == 0,
+             "%s: %lld heads for %d kv heads", who, a.heads, a.cache.kv_heads);
+  CB_REQUIRE(a.batch >= 0 && a.batch <= 65535 && a.tokens >= 0 && a.tokens <= 65535 &&
+                 a.tokens * (a.heads / a.cache.kv_heads) < (1LL << 30),
+             "%s: %lld sequences of %lld tokens", who, a.batch, a.tokens);
+  return CB_OK;
+}
+
 namespace {
 
 // Tiles' time that beginning an item costs (queries, first loads, joining the
@@ -61,7 +97,30 @@ struct Plan {  // of one launch
   bool wide;                // queries can be read 16 bytes at a time
   float* partial;           // scratch: two partial results of each block
   unsigned* arrived;        // for each block: parts of the item that it begins and does not end
+  SharedKeys shared;
 };
+
+// Pages that all sequences of the call have in common; every thread of the block calls this.
+__device__ __forceinline__ int common_pages(const SharedKeys& shared, long long batch, int* found) {
+  if (threadIdx.x == 0) *found = INT_MAX;
+  __syncthreads();
+  int least = INT_MAX;
+  for (int b = threadIdx.x; b < batch; b += blockDim.x) least = min(least, __ldcg(shared.common + b));
+  least = __reduce_min_sync(0xffffffffu, least);
+  if ((threadIdx.x & 31) == 0 && least != INT_MAX) atomicMin(found, least);
+  __syncthreads();
+  return *found == INT_MAX ? 0 : *found;
+}
+// The division of the shared keys: tiles of an item, and of a range.
+struct SharedCut {
+  int tiles, per;
+};
+__device__ __forceinline__ SharedCut shared_cut(const SharedKeys& s, int items, int keys) {
+  SharedCut cut;
+  cut.tiles = (keys + kSharedTile - 1) / kSharedTile;
+  cut.per = max(s.least, (items * cut.tiles + s.ranges - 1) / s.ranges);
+  return cut;
+}
 
 inline Plan plan_of(const cb_paged_attention_args& a, int block_rows, void* scratch, unsigned* counters) {
   Plan p;
@@ -98,12 +157,17 @@ __device__ __forceinline__ int tiles_of(const PagedRow& row) {
   const int keys = row.count > 0 ? row.length : 1;  // (an item without keys writes zeros)
   return (keys - 1) / TILE + 1;                     // (no sum that passes 2^31)
 }
+// `skip`: columns of the table that are left out (at least one key of each row is not among them).
 template <int TILE>
-__device__ __forceinline__ Slot slot_of(const Plan& p, long long b) {
+__device__ __forceinline__ Slot slot_of(const Plan& p, long long b, int skip) {
   Slot s;
   if (!paged_row(p.a.cache, p.a.sequences, p.a.counts, p.a.tokens, b, p.a.error_flag, &s.row)) {
     s.row.length = s.row.count = 0;
     s.row.table = p.a.cache.table;
+  }
+  if (s.row.count > 0) {
+    s.row.table += skip;
+    s.row.length -= skip * p.a.cache.page;
   }
   s.tiles = tiles_of<TILE>(s.row);
   return s;
@@ -146,14 +210,14 @@ struct Segment {
 template <int TILE>
 struct Walk {
   Slot s;
-  int b, origin, at, range, end, per, items;
+  int b, origin, at, range, end, per, items, skip;
 
   __device__ __forceinline__ bool next(const Plan& p, Segment* g) {
     while (at < end) {
       int span = s.tiles + kItemCost;
       if (at - origin >= span * items) {
         origin += span * items;
-        s = slot_of<TILE>(p, ++b);
+        s = slot_of<TILE>(p, ++b, skip);
         span = s.tiles + kItemCost;
       }
       const int item = (at - origin) / span, item_at = origin + item * span;
@@ -179,14 +243,14 @@ struct Walk {
 
 // Finds the block's range; every thread of it calls this.  False: none.
 template <int TILE, int WARPS>
-__device__ __forceinline__ bool begin_walk(const Plan& p, int* scan, int* found, Walk<TILE>* walk) {
+__device__ __forceinline__ bool begin_walk(const Plan& p, int skip, int* scan, int* found, Walk<TILE>* walk) {
   constexpr int kBlock = 32 * WARPS;
   const int batch = static_cast<int>(p.a.batch), items = p.a.cache.kv_heads * p.blocks;
   Slot s;
   s.tiles = -kItemCost;
   int mine = 0, all;
   for (int b = batch - 1 - (batch - 1 - static_cast<int>(threadIdx.x)) % kBlock; b >= 0 && b < batch; b -= kBlock) {
-    s = slot_of<TILE>(p, b);  // (slot threadIdx.x last)
+    s = slot_of<TILE>(p, b, skip);  // (slot threadIdx.x last)
     mine += s.tiles + kItemCost;
   }
   block_scan<WARPS>(mine, scan, &all);
@@ -198,7 +262,7 @@ __device__ __forceinline__ bool begin_walk(const Plan& p, int* scan, int* found,
   for (int first = 0; first < batch; first += kBlock) {
     const int b = first + static_cast<int>(threadIdx.x);
     if (first > 0) {
-      if (b < batch) s = slot_of<TILE>(p, b);
+      if (b < batch) s = slot_of<TILE>(p, b, skip);
       else s.tiles = -kItemCost;
     }
     const int units = (s.tiles + kItemCost) * items;
@@ -217,7 +281,7 @@ __device__ __forceinline__ bool begin_walk(const Plan& p, int* scan, int* found,
   __syncthreads();
   walk->b = found[0];
   walk->origin = found[1];
-  walk->s.row.table = p.a.cache.table + found[2] * p.a.cache.columns;
+  walk->s.row.table = p.a.cache.table + found[2] * p.a.cache.columns + (found[4] > 0 ? skip : 0);
   walk->s.row.length = found[3];
   walk->s.row.count = found[4];
   walk->s.tiles = tiles_of<TILE>(walk->s.row);
@@ -225,6 +289,7 @@ __device__ __forceinline__ bool begin_walk(const Plan& p, int* scan, int* found,
   walk->end = end;
   walk->per = per;
   walk->items = items;
+  walk->skip = skip;
   return true;
 }
 
@@ -276,11 +341,58 @@ __device__ __forceinline__ void store4(const Plan& p, long long at, const float*
 // Partial results: maxima and sums of the rows, then the rows.
 __host__ __device__ constexpr int partial_floats(int size, int rows) { return rows * (size + 2); }
 
+// Weighted values v of a row's elements d .. d + 3 and the sum of its weights
+// against the reference `top`, with those of the shared keys added in the order of
+// the ranges.  `row` counts those of the kv head in all sequences.
+template <int SIZE>
+__device__ __noinline__ void add_shared(const Plan& p, int pages, long long row, int head, int d, float* top_,
+                                        float* sum_, float* v) {
+  const SharedKeys& s = p.shared;
+  const int blocks = static_cast<int>((p.a.batch * p.rows + s.block_rows - 1) / s.block_rows);
+  const SharedCut cut = shared_cut(s, p.a.cache.kv_heads * blocks, pages * p.a.cache.page);
+  const int item = head * blocks + static_cast<int>(row / s.block_rows), r = static_cast<int>(row % s.block_rows);
+  const int from = item * cut.tiles / cut.per, last = ((item + 1) * cut.tiles - 1) / cut.per;
+  const long long floats = static_cast<long long>(s.block_rows) * (SIZE + 2);
+  const float* parts = s.parts + static_cast<long long>(item + from) * s.ways * floats;
+  const int count = (last - from + 1) * s.ways;
+  float top = *top_, sum = *sum_;
+  constexpr int kBatch = 8;  // parts whose loads are in flight together
+  for (int at = 0; at < count; at += kBatch) {
+    float m[kBatch], l[kBatch], now = top;
+    float4 x[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const float* part = parts + (at + k) * floats;
+      m[k] = at + k < count ? __ldcg(part + r) : -INFINITY;
+      l[k] = at + k < count ? __ldcg(part + s.block_rows + r) : 0.0f;
+      x[k] = at + k < count
+                 ? __ldcg(reinterpret_cast<const float4*>(part + 2 * s.block_rows + static_cast<long long>(r) * SIZE + d))
+                 : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) now = fmaxf(now, m[k]);
+    if (now == -INFINITY) continue;  // nothing yet
+    const float keep = top == -INFINITY ? 0.0f : root2_of(top - now);
+    sum = sum * keep * keep;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = v[i] * keep * keep;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const float f = m[k] == -INFINITY ? 0.0f : root2_of(m[k] - now);
+      sum += f * l[k] * f;
+      v[0] += f * x[k].x * f; v[1] += f * x[k].y * f; v[2] += f * x[k].z * f; v[3] += f * x[k].w * f;
+    }
+    top = now;
+  }
+  *top_ = top;
+  *sum_ = sum;
+}
+
 // An item that a cut divided: its first part, then the first partial results of
 // the following blocks (`rest` + 2 k of them), in that order.
-template <int SIZE, int ROWS>
+template <int SIZE, int ROWS, bool SHARED>
 __device__ __noinline__ void join(const Plan& p, long long b, int head, int first_row, int count, int parts,
-                                  const float* first, const float* rest, int thread, int threads) {
+                                  const float* first, const float* rest, int pages, int thread, int threads) {
   constexpr int kRows = ROWS, kFloats = partial_floats(SIZE, ROWS);
   for (int i = thread; i < kRows * SIZE / 4; i += threads) {
     const int r = i / (SIZE / 4), d = i % (SIZE / 4) * 4, row = first_row + r;
@@ -313,6 +425,7 @@ __device__ __noinline__ void join(const Plan& p, long long b, int head, int firs
       }
       top = now;
     }
+    if (SHARED && pages > 0 && row / p.group < count) add_shared<SIZE>(p, pages, b * p.rows + row, head, d, &top, &sum, v);
     const bool real = row / p.group < count && sum != 0.0f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = real ? v[k] / sum : 0.0f;

@@ -12,6 +12,7 @@ one float32 scale for each page and kv head, and pages can be shared:
         cache.append(layer, k, v, counts=counts)        # quantise them into their pages
         out = cache.attend(layer, q, counts=counts)     # attention of the same tokens
     cache.fork([0, 0], [5, 6])                # slots 5 and 6 continue slot 0, sharing its pages
+    out = cache.attend_shared(layer, q)       # attend, with the pages that all slots share read once
     cache.truncate(refused)                   # drop the last refused[b] tokens
     cache.release([6])                        # all of slot 6
     cache.compact()                           # move the held pages to the front of the pools
@@ -293,12 +294,28 @@ class PagedCache:
         slot walks the slot's whole length, also those past ``counts[b]``: one
         long chunk with many single tokens costs less in a call of its own.
         """
+        return self._attend("cb_paged_attention", layer, q, counts, sequences, scale, out)
+
+    def attend_shared(self, layer: int, q: Any, *, counts: Any = None, sequences: Any = None,
+                      scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``attend`` for sequences that begin alike, as ``fork`` leaves them.
+
+        The leading pages that all sequences of the call hold in common (those
+        with a count of 0 aside) are found on the device, and read and multiplied
+        once with the rows of all of them; each sequence's other keys are its own,
+        as in ``attend``.  Any sequences may be given: where they share nothing the
+        call takes little longer than ``attend``'s.
+        """
+        return self._attend("cb_paged_attention_shared", layer, q, counts, sequences, scale, out)
+
+    def _attend(self, entry: str, layer: int, q: Any, counts: Any, sequences: Any, scale: Optional[float],
+                out: Optional[torch.Tensor]) -> torch.Tensor:
         q, counts, sequences = tensor_of(q), self._ints(counts), self._ints(sequences)
         no_grad_needed(q)
-        key = (layer, signature(q), signature(counts), signature(sequences), scale)
+        key = (entry, layer, signature(q), signature(counts), signature(sequences), scale)
         known = self._attend_args.get(key)
         if known is None:
-            known = self._attend_args[key] = self._prepare_attend(layer, q, counts, sequences, scale)
+            known = self._attend_args[key] = self._prepare_attend(entry, layer, q, counts, sequences, scale)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
@@ -315,7 +332,7 @@ class PagedCache:
             a.sequences = sequences.data_ptr()
         stream = self._stream()
         counters, scratch = self._workspace(stream, known[2], known[1])
-        _lib.check(self._lib.cb_paged_attention(ctypes.byref(a), scratch, counters, stream), "cb_paged_attention")
+        _lib.check(getattr(self._lib, entry)(ctypes.byref(a), scratch, counters, stream), entry)
         return out
 
     def _workspace(self, stream: int, counters: int, words: int) -> Tuple[int, int]:
@@ -334,7 +351,7 @@ class PagedCache:
             kept = self._workspaces[stream] = (counters, words, counts.data_ptr(), scratch.data_ptr(), counts, scratch)
         return kept[2], kept[3]
 
-    def _prepare_attend(self, layer: int, q: torch.Tensor, counts: Optional[torch.Tensor],
+    def _prepare_attend(self, entry: str, layer: int, q: torch.Tensor, counts: Optional[torch.Tensor],
                         sequences: Optional[torch.Tensor],
                         scale: Optional[float]) -> Tuple[_lib.PagedAttentionArgs, int, int]:
         require(q, "q", self.device, tuple(_VALUES), (None, None, None, self.head_size), 1)
@@ -348,7 +365,7 @@ class PagedCache:
         a.q_strides[:] = q.stride()[:3]
         a.scale = 1.0 / math.sqrt(self.head_size) if scale is None else scale
         a.error_flag = self._flag.data_ptr()
-        return (a, (self._lib.cb_paged_attention_scratch(ctypes.byref(a)) + 3) // 4,
+        return (a, (getattr(self._lib, entry + "_scratch")(ctypes.byref(a)) + 3) // 4,
                 self._lib.cb_paged_attention_counters(ctypes.byref(a)))
 
     # -- pages -------------------------------------------------------------

@@ -923,6 +923,17 @@ CB_API long long cb_paged_attention_counters(const cb_paged_attention_args* args
 CB_API int cb_paged_attention(const cb_paged_attention_args* args, void* scratch, unsigned* counters,
                               cb_stream_t stream);
 
+/* cb_paged_attention for sequences that begin alike, as cb_pages_fork leaves them:
+ * the leading pages that the tables of all sequences with a count name alike, as
+ * far as they are whole and leave each row a key of its own, are found on the
+ * device, and read and multiplied once with the rows of all of them.  Any
+ * sequences may be given; those that share nothing take the time of
+ * cb_paged_attention and of two short launches.  `scratch`:
+ * cb_paged_attention_shared_scratch bytes; `counters` as there. */
+CB_API long long cb_paged_attention_shared_scratch(const cb_paged_attention_args* args);
+CB_API int cb_paged_attention_shared(const cb_paged_attention_args* args, void* scratch, unsigned* counters,
+                                     cb_stream_t stream);
+
 /* The book of a cache: who holds which page.  refs[p] slots hold page p;
  * free[0 .. *height) is a stack of the pages that none holds.  A slot of
  * length n holds ceil(n / page) pages, its other columns are -1. */

@@ -127,3 +127,41 @@ def test_rows():
     assert quantized._rows(x[0, :1].expand(5, 32)) == (5, 0)
     with pytest.raises(ValueError):
         quantized._rows(x[:, :3])
+
+
+def cache(**changes):
+    c = _lib.PagedCacheArgs(k_pages=16, v_pages=16, k_scale=16, v_scale=16, storage=_lib.I8, kv_heads=2, page=16,
+                            head_size=64, pages=8, table=16, lengths=16, slots=2, columns=4)
+    for name, value in changes.items():
+        setattr(c, name, value)
+    return c
+
+
+def shared(c, scratch=16, counters=16, **changes):
+    a = _lib.PagedAttentionArgs(cache=c, q=16, out=16, dtype=_lib.F32, batch=1, tokens=1, heads=2, scale=1.0)
+    for name, value in changes.items():
+        setattr(a, name, value)
+    return _lib.call("cb_paged_attention_shared", ctypes.byref(a), scratch, counters, None)
+
+
+@pytest.mark.parametrize("change", [dict(storage=_lib.BF16), dict(head_size=48), dict(page=24), dict(kv_heads=0),
+                                    dict(columns=2 ** 31 // 16), dict(k_pages=None), dict(v_pages=8)])
+def test_shared_cache_refusals(change):
+    with pytest.raises(_lib.KernelError):
+        shared(cache(**change))
+
+
+@pytest.mark.parametrize("change", [dict(dtype=_lib.I64), dict(heads=3), dict(heads=0), dict(out=None), dict(q=None),
+                                    dict(batch=65536), dict(tokens=-1), dict(out=8), dict(scratch=None),
+                                    dict(scratch=8), dict(counters=None)])
+def test_shared_call_refusals(change):
+    with pytest.raises(_lib.KernelError):
+        shared(cache(), **change)
+
+
+def test_shared_calls_with_too_much_work():
+    """Rows and keys whose division would pass 32 bits, and empty calls, which do nothing."""
+    with pytest.raises(_lib.KernelError, match="too many"):
+        shared(cache(columns=2 ** 26), batch=65535, tokens=64)
+    shared(cache(), batch=0)
+    shared(cache(), tokens=0)
