@@ -148,26 +148,6 @@ __device__ __forceinline__ void read_words(const char* p, uint32_t* w) {
 
 // ---- fp16 operands -------------------------------------------------------------
 
-
-// Four codes -> two pairs of halves: of int8 elements 0, 2 and 1, 3, of e4m3
-// elements 0, 1 and 2, 3.  int8: the byte x + 128 (the sign bit turned) under
-// the exponent of 1024 is the number 1152 + x; one logic instruction makes two.
-template <int STORAGE>
-__device__ __forceinline__ void to_halves(uint32_t w, uint32_t& a, uint32_t& b) {
-  if (STORAGE == CB_I8) {
-    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-    uint32_t even, odd;
-    asm("lop3.b32 %0, %1, 0x00ff00ff, 0x64806480, 0x6a;" : "=r"(even) : "r"(w));  // (w & mask) ^ bits
-    asm("lop3.b32 %0, %1, 0x00ff00ff, 0x64806480, 0x6a;" : "=r"(odd) : "r"(w >> 8));
-    a = bits(__hsub2(*reinterpret_cast<const __half2*>(&even), bias));
-    b = bits(__hsub2(*reinterpret_cast<const __half2*>(&odd), bias));
-  } else {
-    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\t"
-        "cvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
-        : "=r"(a), "=r"(b)
-        : "r"(w));
-  }
-}
 // The words whose pairs are elements 2 i and 2 i + 1 of two rows, i = 0, 1.
 template <int STORAGE>
 __device__ __forceinline__ uint32_t interleave(uint32_t a, uint32_t b, int i) {

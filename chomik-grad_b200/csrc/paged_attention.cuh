@@ -16,13 +16,19 @@ namespace cb {
 // of all sequences, go in blocks of `block_rows`, and the keys of all (kv head,
 // block of rows) in tiles of kSharedTile are cut into equal ranges.  Range c's
 // part of item i is parts (i + c) * ways .. + ways - 1: references of block_rows
-// rows, their sums, then the rows.
+// rows, their sums, then the rows' elements (see shared_at).
 constexpr int kSharedTile = 64;
 struct SharedKeys {
   const int* common;  // and behind them the slot of the first sequence that takes part
   const float* parts;
   int block_rows, ways, ranges, least;  // tiles of a range: `least` or more
 };
+// Of element d of row r behind a part's references and sums: eight neighbouring
+// elements of a row together, so that the rows that write them and the elements that
+// read them touch whole sectors.
+__host__ __device__ constexpr long long shared_at(int block_rows, int r, int d) {
+  return (static_cast<long long>(d / 8) * block_rows + r) * 8 + d % 8;
+}
 // cb_paged_attention's launch, of the keys behind the shared ones where `shared` is given.
 int launch_attention(const cb_paged_attention_args& a, const SharedKeys* shared, void* scratch, unsigned* counters,
                      cudaStream_t stream);
@@ -91,6 +97,25 @@ __device__ __forceinline__ float power2(int e) { return __uint_as_float(static_c
 
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
+// Four codes -> two pairs of halves: of int8 elements 0, 2 and 1, 3, of e4m3
+// elements 0, 1 and 2, 3.  int8: the byte x + 128 (the sign bit turned) under
+// the exponent of 1024 is the number 1152 + x; one logic instruction makes two.
+template <int STORAGE>
+__device__ __forceinline__ void to_halves(uint32_t w, uint32_t& a, uint32_t& b) {
+  if (STORAGE == CB_I8) {
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    uint32_t even, odd;
+    asm("lop3.b32 %0, %1, 0x00ff00ff, 0x64806480, 0x6a;" : "=r"(even) : "r"(w));  // (w & mask) ^ bits
+    asm("lop3.b32 %0, %1, 0x00ff00ff, 0x64806480, 0x6a;" : "=r"(odd) : "r"(w >> 8));
+    a = bits(__hsub2(*reinterpret_cast<const __half2*>(&even), bias));
+    b = bits(__hsub2(*reinterpret_cast<const __half2*>(&odd), bias));
+  } else {
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+        : "=r"(a), "=r"(b)
+        : "r"(w));
+  }
+}
 struct Plan {  // of one launch
   cb_paged_attention_args a;
   int group, rows, blocks;  // query heads of a kv head, rows of a kv head, blocks of them
@@ -366,7 +391,7 @@ __device__ __noinline__ void add_shared(const Plan& p, int pages, long long row,
       m[k] = at + k < count ? __ldcg(part + r) : -INFINITY;
       l[k] = at + k < count ? __ldcg(part + s.block_rows + r) : 0.0f;
       x[k] = at + k < count
-                 ? __ldcg(reinterpret_cast<const float4*>(part + 2 * s.block_rows + static_cast<long long>(r) * SIZE + d))
+                 ? __ldcg(reinterpret_cast<const float4*>(part + 2 * s.block_rows + shared_at(s.block_rows, r, d)))
                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
 #pragma unroll

@@ -8,6 +8,7 @@
 #include <type_traits>
 
 #include "paged_attention.cuh"
+#include "tc_core.cuh"
 
 namespace cb {
 namespace {
@@ -64,84 +65,573 @@ __global__ void __launch_bounds__(kCommonThreads) common_kernel(const cb_paged_a
 struct SharedPlan {
   cb_paged_attention_args a;
   int group, rows;  // query heads of a kv head; rows of a kv head in a sequence
+  bool wide;        // queries can be read 16 bytes at a time
   SharedKeys shared;
   float* parts;
 };
 
-constexpr int kSimpleThreads = 256;
+// ---- the shared keys -------------------------------------------------------------
 
-// A warp to a row.
+constexpr int kRowLanes = 128;  // rows of a product: lanes of the tensor memory
+constexpr int kSetThreads = 128;
+constexpr int kKeyWarp = 8, kValueWarp = 12, kIssueWarp = 16;  // warps 0-7: two sets of rows
+constexpr int kSharedThreads = 32 * (kIssueWarp + 1);
+constexpr int kStages = 3;
+constexpr int kChunkBytes = kSharedTile * 128;  // 64 keys of 64 fp16 elements
+// Columns of the tensor memory: weighted values and scores of both sets, queries
+// (of both sets, or their high and low parts).  The weights take the place of the scores.
+constexpr int kValuesAt = 0, kScoresAt = 256, kQueriesAt = 384, kColumns = 512;
+
+// Per stage: scales of the tile's four runs of 16 keys.
+struct __align__(16) Scales {
+  float key[4], log[4], inverse[4], factor[4];  // of values: log2, 2^-log2, what the logarithm leaves
+  int irregular, pad[3];
+};
+
 template <int SIZE>
-__global__ void __launch_bounds__(kSimpleThreads) shared_kernel(const __grid_constant__ SharedPlan p) {
-  __shared__ int found;
-  constexpr int kEach = SIZE / 32;
-  const cb_paged_cache& c = p.a.cache;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_launch_dependents();
-  pdl_wait();
-  const int pages = common_pages(p.shared, p.a.batch, &found);
-  if (pages == 0) return;
-  const long long all_rows = p.a.batch * p.rows;
-  const int blocks = static_cast<int>((all_rows + p.shared.block_rows - 1) / p.shared.block_rows);
-  const int items = c.kv_heads * blocks, keys = pages * c.page;
-  const SharedCut cut = shared_cut(p.shared, items, keys);
-  const int* table = c.table + __ldcg(p.shared.common + p.a.batch) * c.columns;
-  const int range = blockIdx.x, end = min((range + 1) * cut.per, items * cut.tiles);
-  for (int at = range * cut.per; at < end;) {
-    const int item = at / cut.tiles, tile = at % cut.tiles, tiles = min(cut.tiles - tile, end - at);
-    const int head = item / blocks;
-    float* part = p.parts + static_cast<long long>(item + range) * p.shared.ways * p.shared.block_rows * (SIZE + 2);
-    for (int r = warp; r < p.shared.block_rows; r += kSimpleThreads / 32) {
-      const long long row = static_cast<long long>(item % blocks) * p.shared.block_rows + r;
-      if (row >= all_rows) break;
-      const long long b = row / p.rows, t = row % p.rows / p.group, h = head * p.group + row % p.group;
-      const long long from = b * p.a.q_strides[0] + t * p.a.q_strides[1] + h * p.a.q_strides[2];
-      float q[kEach], o[kEach], m = -INFINITY, l = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        q[i] = load_as_f32(p.a.q, from + lane + 32 * i, p.a.dtype);
-        o[i] = 0.0f;
-      }
-      for (int key = tile * kSharedTile; key < min(keys, (tile + tiles) * kSharedTile); ++key) {
-        const int page = table[key / c.page];
-        if (page < 0 || page >= c.pages) {
-          raise_flag(p.a.error_flag, CB_FLAG_BOOK);
-          continue;
-        }
-        const long long at_page = static_cast<long long>(page) * c.kv_heads + head;
-        const long long line = (at_page * c.page + key % c.page) * SIZE;
-        float dot = 0.0f, v[kEach];
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-          float k;
-          if (c.storage == CB_I8) {
-            k = static_cast<const int8_t*>(c.k_pages)[line + lane + 32 * i];
-            v[i] = static_cast<const int8_t*>(c.v_pages)[line + lane + 32 * i];
-          } else {
-            k = static_cast<float>(static_cast<const __nv_fp8_e4m3*>(c.k_pages)[line + lane + 32 * i]);
-            v[i] = static_cast<float>(static_cast<const __nv_fp8_e4m3*>(c.v_pages)[line + lane + 32 * i]);
-          }
-          dot = fmaf(q[i], k, dot);
-        }
-        const float x = warp_sum(dot) * (c.k_scale[at_page] * (p.a.scale * 1.4426950408889634f));
-        const float now = fmaxf(m, x), keep = exp2f(m - now), w = exp2f(x - now), scaled = w * c.v_scale[at_page];
-        l = fmaf(l, keep, w);
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) o[i] = fmaf(o[i], keep, scaled * v[i]);
-        m = now;
-      }
-      if (lane == 0) {
-        part[r] = m;
-        part[p.shared.block_rows + r] = l;
-      }
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) part[2 * p.shared.block_rows + r * SIZE + lane + 32 * i] = o[i];
-    }
-    at += tiles;
-  }
+struct SharedShape {
+  static constexpr int kChunks = SIZE == 128 ? 2 : 1;
+  static constexpr int kStageBytes = 2 * kChunks * kChunkBytes;  // keys, then values
+  static constexpr int kBytes = kStages * kStageBytes + 1024;    // (the tiles begin on 1024)
+  static constexpr int kWide = SIZE < 64 ? 64 : SIZE;            // columns of the weighted values
+};
+
+// fp16 x fp16 -> float32, 128 x n; the second operand with its contraction along (K) or across its rows.
+__host__ __device__ constexpr uint32_t idesc_f16(int n, bool across) {
+  return (1u << 4) | (across ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (128u >> 4 << 24);
+}
+// A tile of rows of 128 bytes whose contraction runs across them: 64 columns to a
+// chunk, chunks kChunkBytes apart, 8 rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t across_desc(const void* tile) {
+  return ((static_cast<uint64_t>(smem_addr(tile)) >> 4) & 0x3FFFull) |
+         (static_cast<uint64_t>(kChunkBytes >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void multiply(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void store8(uint32_t at, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 
-constexpr int kBlockRows = 128;
+// Eight neighbouring elements of a query row.
+__device__ __forceinline__ void load_row8(const SharedPlan& p, long long at, float* x) {
+  if (!p.wide) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = load_as_f32(p.a.q, at + i, p.a.dtype);
+  } else if (p.a.dtype == CB_F32) {
+    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p.a.q) + at);
+    const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p.a.q) + at + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  } else {
+    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.a.q) + at);
+    if (p.a.dtype == CB_BF16) {
+      unpack_bf16x8(w, x);
+    } else {
+      const __half2* h = reinterpret_cast<const __half2*>(&w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __low2float(h[i]);
+        x[2 * i + 1] = __high2float(h[i]);
+      }
+    }
+  }
+}
+// Eight float32 columns of this thread's lane of the tensor memory (warp-wide).
+__device__ __forceinline__ void load8(uint32_t at, float* out) {
+  uint32_t v[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(at));
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7])
+               :
+               : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) out[i] = __uint_as_float(v[i]);
+}
+
+// What a role of the block walks: its range of units, item by item.
+struct SharedWalk {
+  int blocks, keys, range, begin, end;
+  SharedCut cut;
+  const int* table;
+};
+
+// Barriers of a block.  Sets and stages count their phases apart.
+struct SharedSync {
+  uint64_t key_full[kStages], key_free[kStages], value_full[kStages], value_free[kStages];
+  uint64_t query_full, query_free, score_full[2], weight_full[2], value_done[2], all_done;
+  uint32_t tmem;
+  int abort, found;
+};
+
+// Keys (or values) of the range's tiles: codes to fp16 in shared memory, rows of 64
+// elements on 128 bytes, their 16-byte pieces exchanged as the products read them.  The
+// loads of kAhead tiles are in flight.
+template <int SIZE, int STORAGE, bool VALUES>
+__device__ __forceinline__ bool convert(const SharedPlan& p, const SharedWalk& w, char* tiles, Scales* scales,
+                                        SharedSync& sync) {
+  constexpr int kPieces = SIZE / 16, kLoads = kSharedTile * kPieces / kSetThreads, kAhead = 3;
+  const cb_paged_cache& c = p.a.cache;
+  const int thread = threadIdx.x - 32 * (VALUES ? kValueWarp : kKeyWarp);
+  const int piece = thread % kPieces, row = thread / kPieces;
+  const int shift = 31 - __clz(c.page), count = w.end - w.begin;
+  const char* pool = static_cast<const char*>(VALUES ? c.v_pages : c.k_pages);
+  uint4 codes[kAhead][kLoads];
+  int pages[kLoads], scale_page;  // of the tile that is loaded next, found one earlier
+  float key_scale[kAhead], value_scale[kAhead];
+  bool there[kAhead];
+
+  // the tile whose pages are looked up next, and the one that is loaded next
+  int look = 0, look_tile = w.begin % w.cut.tiles;
+  int load_tile = look_tile, load_item = w.begin / w.cut.tiles;
+  auto page_of = [&](int r) {  // of row r: -1 where there is none
+    const int key = look < count ? look_tile * kSharedTile + r : w.keys;
+    if (key >= w.keys) return -1;
+    const int page = w.table[key >> shift];
+    if (page < 0 || page >= c.pages) {
+      raise_flag(p.a.error_flag, CB_FLAG_BOOK);
+      return -1;
+    }
+    return page;
+  };
+  auto look_up = [&] {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) pages[i] = page_of(row + i * (kSetThreads / kPieces));
+    if (VALUES) scale_page = page_of((thread & 3) * 16);
+    ++look;
+    if (++look_tile == w.cut.tiles) look_tile = 0;
+  };
+  auto load = [&](int slot) {  // and looks up the next tile's pages
+    const int head = min(load_item / w.blocks, c.kv_heads - 1);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int key = load_tile * kSharedTile + row + i * (kSetThreads / kPieces);
+      codes[slot][i] = make_uint4(0, 0, 0, 0);
+      if (pages[i] >= 0)
+        codes[slot][i] = __ldg(reinterpret_cast<const uint4*>(
+            pool + ((static_cast<long long>(pages[i]) * c.kv_heads + head) * c.page + (key & (c.page - 1))) * SIZE +
+            piece * 16));
+    }
+    if (VALUES) {
+      there[slot] = scale_page >= 0;
+      const long long line = static_cast<long long>(max(scale_page, 0)) * c.kv_heads + head;
+      key_scale[slot] = scale_page >= 0 ? __ldg(c.k_scale + line) : 0.0f;
+      value_scale[slot] = scale_page >= 0 ? __ldg(c.v_scale + line) : 0.0f;
+    }
+    if (++load_tile == w.cut.tiles) {
+      load_tile = 0;
+      ++load_item;
+    }
+    look_up();
+  };
+  if (VALUES && SIZE == 32) {  // the columns that no element has
+    for (int i = thread; i < kStages * kSharedTile * 4; i += kSetThreads)
+      *reinterpret_cast<uint4*>(tiles + i / (kSharedTile * 4) * SharedShape<SIZE>::kStageBytes +
+                                tc::swizzle_offset(i / 4 % kSharedTile, 4 + i % 4)) = make_uint4(0, 0, 0, 0);
+  }
+  look_up();
+#pragma unroll
+  for (int n = 0; n < kAhead; ++n) load(n);
+  bool ok = true;
+  for (int n = 0; n < count; n += kAhead) {
+#pragma unroll
+    for (int slot = 0; slot < kAhead; ++slot) {
+      const int at = n + slot;
+      if (at >= count) break;
+      const int stage = at % kStages, turn = at / kStages;
+      uint64_t* free = (VALUES ? sync.value_free : sync.key_free) + stage;
+      if (turn > 0 && ok) ok = tc::wait_or_abort(free, static_cast<uint32_t>((turn - 1) & 1), &sync.abort);
+      char* to = tiles + stage * SharedShape<SIZE>::kStageBytes;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int r = row + i * (kSetThreads / kPieces), first = piece % 4 * 2;
+        const uint32_t word[4] = {codes[slot][i].x, codes[slot][i].y, codes[slot][i].z, codes[slot][i].w};
+        uint32_t h[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) to_halves<STORAGE>(word[k], h[2 * k], h[2 * k + 1]);
+        char* line = to + piece / 4 * kChunkBytes;
+        const uint4 low = make_uint4(h[0], h[1], h[2], h[3]), high = make_uint4(h[4], h[5], h[6], h[7]);
+        const bool turned = piece >= 4;  // (so that both chunks' pieces of a row touch different banks)
+        *reinterpret_cast<uint4*>(line + tc::swizzle_offset(r, first + turned)) = turned ? high : low;
+        *reinterpret_cast<uint4*>(line + tc::swizzle_offset(r, first + !turned)) = turned ? low : high;
+      }
+      if (VALUES && thread < 32) {
+        const float v = value_scale[slot], k = key_scale[slot];
+        const bool real = there[slot];
+        const bool regular = !real || (v >= 9.3e-10f && v <= 1.07e9f && k >= 0.0f);  // 2^-30 .. 2^30
+        float log = -INFINITY, inverse = 0.0f, factor = 1.0f;
+        if (real) {
+          const float size = fabsf(v);
+          log = isfinite(v) ? fmaxf(log2f(size), -100.0f) : 0.0f;
+          inverse = exp2f(-log);
+          factor = !isfinite(v) ? NAN : size < 7.9e-31f ? v * 1.2676506002282294e30f : v < 0.0f ? -1.0f : 1.0f;  // 2^-100, 2^100
+        }
+        const bool odd = __any_sync(0xffffffffu, !regular);
+        if (thread < 4) {
+          Scales& s = scales[stage];
+          s.key[thread] = real ? k : 0.0f;
+          s.log[thread] = log;
+          s.inverse[thread] = inverse;
+          s.factor[thread] = factor;
+          if (thread == 0) s.irregular = odd;
+        }
+      }
+      tc::fence_async_shared();
+      mbar_arrive((VALUES ? sync.value_full : sync.key_full) + stage);
+      load(slot);
+    }
+  }
+  return ok;
+}
+
+// Issues the products of the block's range; one thread.  A job is a tile of one set:
+// both sets take every tile (SETS 2: their own rows) or every other one (1: the same rows).
+template <int SIZE, int SETS, bool LO>
+__device__ __forceinline__ bool issue(const SharedWalk& w, const char* keys, const char* values, SharedSync& sync) {
+  using S = SharedShape<SIZE>;
+  constexpr uint32_t kScoreDesc = idesc_f16(kSharedTile, false), kValueDesc = idesc_f16(S::kWide, true);
+  volatile int* abort = &sync.abort;
+  const uint32_t tmem = sync.tmem;
+  int done[2] = {0, 0}, segment = 0, before = 0;  // iterations of the sets; tiles before the segment
+  for (int at = w.begin; at < w.end; ++segment) {
+    const int tiles = min(w.cut.tiles - at % w.cut.tiles, w.end - at), jobs = SETS * tiles;
+    if (!tc::wait_or_abort(&sync.query_full, static_cast<uint32_t>(segment & 1), abort)) return false;
+    tc::fence_after();
+    auto scores = [&](int job) {
+      const int set = job & 1, n = before + (SETS == 2 ? job / 2 : job), stage = n % kStages;
+      if (!tc::wait_or_abort(sync.key_full + stage, static_cast<uint32_t>(n / kStages & 1), abort)) return false;
+      tc::fence_after();
+      const char* tile = keys + stage * S::kStageBytes;
+      const uint32_t d = tmem + kScoresAt + set * kSharedTile;
+      const uint32_t q = tmem + kQueriesAt + (SETS == 2 ? set * 64 : 0);
+#pragma unroll
+      for (int part = 0; part < (LO ? 2 : 1); ++part)
+#pragma unroll
+        for (int k = 0; k < SIZE / 16; ++k)
+          multiply(d, q + part * 64 + k * 8, tc::sw128_desc(tile + k / 4 * kChunkBytes + k % 4 * 32), kScoreDesc,
+                   part + k > 0 ? 1u : 0u);
+      tc::umma_commit(sync.score_full + set);
+      if (SETS == 1 || set == 1) tc::umma_commit(sync.key_free + stage);
+      if (job + 1 == jobs) tc::umma_commit(&sync.query_free);
+      return true;
+    };
+    for (int job = 0; job < min(2, jobs); ++job)
+      if (!scores(job)) return false;
+    for (int job = 0; job < jobs; ++job) {
+      const int set = job & 1, n = before + (SETS == 2 ? job / 2 : job), stage = n % kStages;
+      if (!tc::wait_or_abort(sync.weight_full + set, static_cast<uint32_t>(done[set] & 1), abort)) return false;
+      ++done[set];
+      if (!tc::wait_or_abort(sync.value_full + stage, static_cast<uint32_t>(n / kStages & 1), abort)) return false;
+      tc::fence_after();
+      const char* tile = values + stage * S::kStageBytes;
+      const uint32_t d = tmem + kValuesAt + set * 128, a = tmem + kScoresAt + set * kSharedTile;
+#pragma unroll
+      for (int part = 0; part < (LO ? 2 : 1); ++part)
+#pragma unroll
+        for (int k = 0; k < kSharedTile / 16; ++k)
+          multiply(d, a + part * 32 + k * 8, across_desc(tile + k * 2048), kValueDesc, job >= 2 || part + k > 0 ? 1u : 0u);
+      tc::umma_commit(sync.value_done + set);
+      if (SETS == 1 || set == 1) tc::umma_commit(sync.value_free + stage);
+      if (job + 2 < jobs && !scores(job + 2)) return false;
+    }
+    at += tiles;
+    before += tiles;
+  }
+  return true;
+}
+
+// The references follow the scores and value scales (their logarithms included) as
+// in paged_attention.cuh: what multiplies the value codes is 2^(y - c), y a key's
+// score plus the logarithm of its value scale.  A tile whose largest is more
+// than kRise above c or kFall below it moves c to kRest below it.
+constexpr float kRise = 13.0f, kFall = 6.0f, kRest = 5.0f, kFarBelow = 60.0f, kHeld = 1.2676506002282294e30f;  // 2^100
+
+// A set of 128 rows, a thread each.
+template <int SIZE, int STORAGE, int SETS, bool LO>
+__device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, const Scales* scales, SharedSync& sync) {
+  const int set = threadIdx.x / kSetThreads, r = threadIdx.x % kSetThreads;
+  const int local = SETS == 2 ? threadIdx.x : r;
+  volatile int* abort = &sync.abort;
+  const uint32_t lanes = sync.tmem + (static_cast<uint32_t>(threadIdx.x / 32 % 4 * 32) << 16);
+  const uint32_t scores = lanes + kScoresAt + set * kSharedTile, sums = lanes + kValuesAt + set * 128;
+  const long long all_rows = p.a.batch * p.rows;
+  int iteration = 0, segment = 0, before = 0;
+  for (int at = w.begin; at < w.end; ++segment) {
+    const int item = at / w.cut.tiles, tiles = min(w.cut.tiles - at % w.cut.tiles, w.end - at);
+    const int head = item / w.blocks;
+    const long long row = static_cast<long long>(item % w.blocks) * p.shared.block_rows + local;
+    const bool real = row < all_rows, any = __any_sync(0xffffffffu, real);  // (rows of no warp are skipped)
+
+    // the row's queries, scaled to below 2, in the order of the codes' halves
+    float factor;
+    {
+      long long from = 0;
+      if (real) {
+        const long long b = row / p.rows, t = row % p.rows / p.group, h = head * p.group + row % p.group;
+        from = b * p.a.q_strides[0] + t * p.a.q_strides[1] + h * p.a.q_strides[2];
+      }
+      float largest = 0.0f;
+#pragma unroll 4
+      for (int d = 0; d < SIZE; d += 8) {
+        float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (real) load_row8(p, from + d, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(x[i]));
+      }
+      const int e = min(max(static_cast<int>(__float_as_uint(largest) >> 23) - 127, -126), 127);
+      const float down = e == 127 ? 5.877471754111438e-39f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      const float sign = p.a.scale < 0.0f ? -down : down;
+      factor = fabsf(p.a.scale) * 1.4426950408889634f * power2(e);
+      if (segment > 0 &&
+          !__all_sync(0xffffffffu, tc::wait_or_abort(&sync.query_free, static_cast<uint32_t>((segment - 1) & 1), abort)))
+        return false;
+      tc::fence_after();
+      const bool writes = SETS == 2 || LO || set == 0;
+#pragma unroll 1
+      for (int d = 0; writes && d < SIZE; d += 16) {
+        uint32_t hi[8], lo[8];
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+        if (real) {
+          load_row8(p, from + d, x);
+          load_row8(p, from + d + 8, x + 8);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int first = STORAGE == CB_I8 ? i / 2 * 4 + i % 2 : 2 * i, second = STORAGE == CB_I8 ? first + 2 : first + 1;
+          const float a = x[first] * sign, b = x[second] * sign;
+          const __half2 h = __floats2half2_rn(a, b);
+          hi[i] = bits(h);
+          lo[i] = bits(__floats2half2_rn(a - __low2float(h), b - __high2float(h)));
+        }
+        const bool second = LO && set == 1;
+        store8(lanes + kQueriesAt + (SETS == 2 || LO ? set * 64 : 0) + d / 2, second ? lo : hi);
+      }
+      tc::tmem_wait_st();
+      tc::fence_before();
+      mbar_arrive(&sync.query_full);
+    }
+
+    float c = 0.0f, l = 0.0f, sum = 0.0f;  // reference, sum of the weights, and of what multiplied the codes
+    bool first = true;
+    for (int tile = SETS == 2 ? 0 : set; tile < tiles; tile += SETS == 2 ? 1 : 2, ++iteration) {
+      const int n = before + tile, stage = n % kStages;
+      if (!__all_sync(0xffffffffu, tc::wait_or_abort(sync.score_full + set, static_cast<uint32_t>(iteration & 1), abort) &&
+                                       tc::wait_or_abort(sync.value_full + stage, static_cast<uint32_t>(n / kStages & 1), abort)))
+        return false;
+      tc::fence_after();
+      if (any) {
+        float s[kSharedTile];
+        tc::tmem_load32_nowait(scores, s);
+        tc::tmem_load32_nowait(scores + 32, s + 32);
+        const Scales& at_stage = scales[stage];
+        float by[4], log[4], inverse[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          by[i] = factor * at_stage.key[i];
+          log[i] = at_stage.log[i];
+          inverse[i] = at_stage.inverse[i];
+        }
+        const bool irregular = at_stage.irregular != 0;
+        tc::tmem_wait_ld();
+        tc::reg_fence<kSharedTile>(s);
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float most = s[16 * i], least = s[16 * i];
+#pragma unroll
+          for (int k = 1; k < 16; ++k) most = fmaxf(most, s[16 * i + k]);
+          if (irregular) {
+#pragma unroll
+            for (int k = 1; k < 16; ++k) least = fminf(least, s[16 * i + k]);
+          }
+          top = fmaxf(top, fmaf(by[i] < 0.0f ? least : most, by[i], log[i]));
+        }
+        const bool moves = first || top > c + kRise || top < c - kFall;
+        if (__any_sync(0xffffffffu, moves)) {
+          const float next = floorf(top) - kRest;
+          float now = c;
+          if (first) now = top > -INFINITY ? next : 0.0f;
+          else if (top > c + kRise) now = next;
+          else if (top < c - kFall && top > -INFINITY) {
+            now = fmaxf(next, c - 50.0f);
+            if (fmaxf(sum, l) * exp2_of(c - now) > kHeld) now = c;
+          }
+          if (!first) {
+            const float scale = exp2_of(c - now);
+            l *= scale;
+            sum *= scale;
+            if (!__all_sync(0xffffffffu, tc::wait_or_abort(sync.value_done + set, static_cast<uint32_t>((iteration - 1) & 1), abort)))
+              return false;
+            tc::fence_after();
+#pragma unroll 1
+            for (int d = 0; d < SharedShape<SIZE>::kWide; d += 8) {
+              float o[8];
+              load8(sums + d, o);
+              uint32_t v[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(o[i] * scale);
+              store8(sums + d, v);
+            }
+          }
+          c = now;
+        }
+        first = false;
+        const bool slow = irregular || __any_sync(0xffffffffu, top < c - kFarBelow);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float* x = s + 16 * i;
+          const float shift = log[i] - c;
+          float run[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          if (!slow) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              x[k] = exp2_of(fmaf(x[k], by[i], shift));
+              run[k & 3] += x[k];
+            }
+            const float all = (run[0] + run[1]) + (run[2] + run[3]);
+            l = fmaf(all, inverse[i], l);
+            sum += all;
+          } else {  // scales of any sign and size: weights by themselves
+            const float kept = at_stage.factor[i];
+            float weights = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const float score = x[k] * by[i];
+              weights += exp2_of(score - c);
+              x[k] = exp2_of(score + shift);
+              run[k & 3] += x[k];
+              x[k] *= kept;
+            }
+            if (inverse[i] != 0.0f) l += weights;
+            sum += (run[0] + run[1]) + (run[2] + run[3]);
+          }
+          uint32_t hi[8], lo[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const __half2 h = __floats2half2_rn(x[2 * k], x[2 * k + 1]);
+            hi[k] = bits(h);
+            if (LO) lo[k] = bits(__floats2half2_rn(x[2 * k] - __low2float(h), x[2 * k + 1] - __high2float(h)));
+          }
+          store8(scores + i * 8, hi);
+          if (LO) store8(scores + 32 + i * 8, lo);
+        }
+        tc::tmem_wait_st();
+      }
+      tc::fence_before();
+      mbar_arrive(sync.weight_full + set);
+    }
+    // the part of this set
+    const bool some = SETS == 2 || tiles > set;
+    if (some && !__all_sync(0xffffffffu, tc::wait_or_abort(sync.value_done + set, static_cast<uint32_t>((iteration - 1) & 1), abort)))
+      return false;
+    tc::fence_after();
+    if (any) {
+      const int rows = p.shared.block_rows;
+      float* part = p.parts + ((item + w.range) * static_cast<long long>(p.shared.ways) + (SETS == 2 ? 0 : set)) * rows * (SIZE + 2);
+      if (real) {
+        part[local] = some ? c : -INFINITY;
+        part[rows + local] = l;
+      }
+#pragma unroll 1
+      for (int d = 0; d < SIZE; d += 8) {
+        float o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (some) load8(sums + d, o);
+        if (real) {
+          float4* to = reinterpret_cast<float4*>(part + 2 * rows + shared_at(rows, local, d));
+          constexpr int b = STORAGE == CB_I8 ? 2 : 1, e = STORAGE == CB_I8 ? 1 : 2;  // (the order of the codes' halves)
+          to[0] = make_float4(o[0], o[b], o[e], o[3]);
+          to[1] = make_float4(o[4], o[4 + b], o[4 + e], o[7]);
+        }
+      }
+      tc::fence_before();
+    }
+    at += tiles;
+    before += tiles;
+  }
+  return true;
+}
+
+template <int SIZE, int STORAGE, int SETS, bool LO>
+__global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_constant__ SharedPlan p) {
+  using S = SharedShape<SIZE>;
+  extern __shared__ char memory[];
+  __shared__ SharedSync sync;
+  __shared__ Scales scales[kStages];
+  char* tiles = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(memory) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_launch_dependents();
+  if (warp == kIssueWarp) tc::tmem_alloc(&sync.tmem, kColumns);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(sync.key_full + i, kSetThreads);
+      mbar_init(sync.value_full + i, kSetThreads);
+      mbar_init(sync.key_free + i, 1);
+      mbar_init(sync.value_free + i, 1);
+    }
+    mbar_init(&sync.query_full, 2 * kSetThreads);
+    mbar_init(&sync.query_free, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(sync.score_full + i, 1);
+      mbar_init(sync.weight_full + i, kSetThreads);
+      mbar_init(sync.value_done + i, 1);
+    }
+    mbar_init(&sync.all_done, 1);
+    mbar_fence_init();
+    sync.abort = 0;
+  }
+  tc::fence_before();
+  pdl_wait();
+  const int pages = common_pages(p.shared, p.a.batch, &sync.found);  // (barriers of the block)
+  tc::fence_after();
+  SharedWalk w;
+  w.blocks = static_cast<int>((p.a.batch * p.rows + p.shared.block_rows - 1) / p.shared.block_rows);
+  w.keys = pages * p.a.cache.page;
+  w.cut = shared_cut(p.shared, p.a.cache.kv_heads * w.blocks, w.keys);
+  w.range = blockIdx.x;
+  const long long begin = static_cast<long long>(blockIdx.x) * w.cut.per, all = 1LL * p.a.cache.kv_heads * w.blocks * w.cut.tiles;
+  w.begin = static_cast<int>(min(begin, all));
+  w.end = static_cast<int>(min(begin + w.cut.per, all));
+  w.table = p.a.cache.table + __ldcg(p.shared.common + p.a.batch) * p.a.cache.columns;
+  const char* values = tiles + S::kChunks * kChunkBytes;
+  bool ok = true;
+  if (w.begin < w.end) {
+    if (warp < kKeyWarp) {
+      ok = weigh<SIZE, STORAGE, SETS, LO>(p, w, scales, sync);
+    } else if (warp < kValueWarp) {
+      ok = convert<SIZE, STORAGE, false>(p, w, tiles, scales, sync);
+    } else if (warp < kIssueWarp) {
+      ok = convert<SIZE, STORAGE, true>(p, w, tiles + S::kChunks * kChunkBytes, scales, sync);
+    } else if (lane == 0) {
+      ok = issue<SIZE, SETS, LO>(w, tiles, values, sync);
+      tc::umma_commit(&sync.all_done);  // arrives once every product issued above has completed
+    }
+    if (!ok) {
+      raise_flag(p.a.error_flag, CB_FLAG_WAIT_DATA);
+      sync.abort = 1;
+    }
+  } else if (threadIdx.x == 32 * kIssueWarp) {
+    tc::umma_commit(&sync.all_done);
+  }
+  __syncwarp();
+  tc::fence_before();
+  __syncthreads();
+  if (warp == kIssueWarp) {
+    // the tensor memory is freed only after the products that write it have completed
+    if (!tc::wait_short(&sync.all_done, 0u) && lane == 0) raise_flag(p.a.error_flag, CB_FLAG_WAIT_DRAIN);
+    tc::fence_after();
+    tc::tmem_dealloc(sync.tmem, kColumns);
+  }
+}
 
 // Where the pieces of the scratch lie.
 struct SharedScratch {
@@ -157,12 +647,19 @@ SharedScratch scratch_of(const cb_paged_attention_args& a, const SharedKeys& sha
                           (a.cache.head_size + 2) * 4LL;
   return s;
 }
+// More than 128 rows of 16-bit queries: two sets of them to a block, which share
+// the tiles; float32, whose queries and weights take two parts, and fewer rows: both
+// sets are the same rows, and take the tiles in turn.
+bool two_sets(const cb_paged_attention_args& a) {
+  return a.dtype != CB_F32 && a.batch * a.tokens * (a.heads / a.cache.kv_heads) > kRowLanes;
+}
 SharedKeys shared_of(const cb_paged_attention_args& a) {
+  const bool two = two_sets(a);
   SharedKeys s = {};
-  s.block_rows = kBlockRows;
-  s.ways = 1;
+  s.block_rows = two ? 2 * kRowLanes : kRowLanes;
+  s.ways = two ? 1 : 2;
   s.ranges = sm_count();
-  s.least = 1;
+  s.least = 4;
   return s;
 }
 
@@ -171,11 +668,28 @@ int shared_check(const cb_paged_attention_args& a) {
   if (status != CB_OK) return status;
   const long long rows = a.batch * a.tokens * (a.heads / a.cache.kv_heads);
   const long long tiles = (a.cache.columns * a.cache.page + kSharedTile - 1) / kSharedTile;
-  const double units = static_cast<double>((rows + kBlockRows - 1) / kBlockRows) * a.cache.kv_heads * tiles;
+  const double units = static_cast<double>((rows + kRowLanes - 1) / kRowLanes) * a.cache.kv_heads * tiles;
   CB_REQUIRE(units + (1 << 20) < 2147483648.0,
              "cb_paged_attention_shared: %lld rows of up to %lld keys are too many for one call", rows,
              a.cache.columns * a.cache.page);
   return CB_OK;
+}
+
+template <typename F>
+int with_shape(const cb_paged_attention_args& a, F f) {
+  auto by_rows = [&](auto size, auto storage) {
+    using one = std::integral_constant<int, 1>;
+    if (a.dtype == CB_F32) return f(size, storage, one{}, std::true_type{});
+    if (two_sets(a)) return f(size, storage, std::integral_constant<int, 2>{}, std::false_type{});
+    return f(size, storage, one{}, std::false_type{});
+  };
+  auto by_storage = [&](auto size) {
+    return a.cache.storage == CB_I8 ? by_rows(size, std::integral_constant<int, CB_I8>{})
+                                    : by_rows(size, std::integral_constant<int, CB_E4M3>{});
+  };
+  if (a.cache.head_size == 32) return by_storage(std::integral_constant<int, 32>{});
+  if (a.cache.head_size == 64) return by_storage(std::integral_constant<int, 64>{});
+  return by_storage(std::integral_constant<int, 128>{});
 }
 
 }  // namespace
@@ -216,12 +730,24 @@ int cb_paged_attention_shared(const cb_paged_attention_args* args, void* scratch
   launch(common_kernel, dim3(static_cast<unsigned>(a.batch)), dim3(kCommonThreads), 0, s, true, a, common);
   int done = check_launch("cb_paged_attention_shared");
   if (done != CB_OK) return done;
-  auto go = [&](auto kernel) {
-    launch(kernel, dim3(static_cast<unsigned>(p.shared.ranges)), dim3(kSimpleThreads), 0, s, true, p);
+  const int item = a.dtype == CB_F32 ? 4 : 2;
+  p.wide = reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
+  for (int i = 0; i < 3; ++i) p.wide = p.wide && a.q_strides[i] * item % 16 == 0;
+  done = with_shape(a, [&](auto size, auto storage, auto sets, auto lo) -> int {
+    constexpr int SIZE = size.value;
+    auto kernel = shared_kernel<SIZE, storage.value, sets.value, lo.value>;
+    static thread_local int device = -1;
+    int now = 0;
+    cudaGetDevice(&now);
+    if (now != device) {
+      const cudaError_t e =
+          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SharedShape<SIZE>::kBytes);
+      CB_REQUIRE(e == cudaSuccess, "cb_paged_attention_shared: %s", cudaGetErrorString(e));
+      device = now;
+    }
+    launch(kernel, dim3(static_cast<unsigned>(p.shared.ranges)), dim3(kSharedThreads), SharedShape<SIZE>::kBytes, s, true, p);
     return check_launch("cb_paged_attention_shared");
-  };
-  done = a.cache.head_size == 32 ? go(shared_kernel<32>) : a.cache.head_size == 64 ? go(shared_kernel<64>)
-                                                                                    : go(shared_kernel<128>);
+  });
   if (done != CB_OK) return done;
   return launch_attention(a, &p.shared, base + at.attention, counters, s);
 }
