@@ -74,13 +74,17 @@ struct SharedPlan {
 
 constexpr int kRowLanes = 128;  // rows of a product: lanes of the tensor memory
 constexpr int kSetThreads = 128;
-constexpr int kKeyWarp = 8, kValueWarp = 12, kIssueWarp = 16;  // warps 0-7: two sets of rows
-constexpr int kSharedThreads = 32 * (kIssueWarp + 1);
-constexpr int kStages = 3;
+constexpr int kKeyWarp = 8, kValueWarp = 12, kIssueWarp = 16;  // warps 0-7: two sets of rows; 16 and 17 issue theirs
+constexpr int kSharedThreads = 32 * (kIssueWarp + 4);
+// Registers of a thread: as launched (the converting warps keep them), of the
+// warps that weigh, of the issuing warp and the three beside it (61440 at the
+// launch and after).
+constexpr int kWeighRegisters = 128, kIssueRegisters = 32;
+constexpr int kStages = 3, kAhead = 4;  // tiles as fp16, and tiles whose codes are on their way
 constexpr int kChunkBytes = kSharedTile * 128;  // 64 keys of 64 fp16 elements
-// Columns of the tensor memory: weighted values and scores of both sets, queries
-// (of both sets, or their high and low parts).  The weights take the place of the scores.
-constexpr int kValuesAt = 0, kScoresAt = 256, kQueriesAt = 384, kColumns = 512;
+// Columns of the tensor memory: weighted values of both sets, then their scores, two
+// tiles each.  The weights of 16 keys take the place of their scores, high parts first.
+constexpr int kValuesAt = 0, kScoresAt = 256, kColumns = 512;
 
 // Per stage: scales of the tile's four runs of 16 keys.
 struct __align__(16) Scales {
@@ -92,7 +96,10 @@ template <int SIZE>
 struct SharedShape {
   static constexpr int kChunks = SIZE == 128 ? 2 : 1;
   static constexpr int kStageBytes = 2 * kChunks * kChunkBytes;  // keys, then values
-  static constexpr int kBytes = kStages * kStageBytes + 1024;    // (the tiles begin on 1024)
+  static constexpr int kCodeBytes = 2 * kSharedTile * SIZE;      // of a tile on its way
+  static constexpr int kQueryBytes = kChunks * kRowLanes * 128;  // of a set, or of one part
+  // (the tiles begin on 1024)
+  static constexpr int kBytes = kStages * kStageBytes + 2 * kQueryBytes + kAhead * kCodeBytes + 1024;
   static constexpr int kWide = SIZE < 64 ? 64 : SIZE;            // columns of the weighted values
 };
 
@@ -113,17 +120,65 @@ __device__ __forceinline__ void multiply(uint32_t d, uint32_t a, uint64_t b, uin
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
 }
+// The same with its first operand in shared memory.
+__device__ __forceinline__ void multiply_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
 __device__ __forceinline__ void store8(uint32_t at, const uint32_t* v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), "r"(v[0]),
                "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
 }
 
+// Every lane of the warp waits for a phase, one of them looks: at most kPolls
+// times, without the clock, a read of which takes longer than most of these waits.
+// QUICK: by mbarrier.test_wait, which does not suspend the thread; a try_wait that
+// began well before its phase ends returns about a thousand cycles after it.
+constexpr uint32_t kPolls = 1u << 24;
+template <bool QUICK = true>
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, const volatile int* abort) {
+  bool there = true;
+  if ((threadIdx.x & 31) == 0) {
+    for (uint32_t i = 0;; ++i) {
+      if (QUICK) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(smem_addr(bar)), "r"(parity)
+            : "memory");
+        if (done != 0) break;
+      } else if (mbar_try_wait_short(bar, parity)) {
+        break;
+      }
+      if (i == kPolls || ((i & 255u) == 255u && *abort != 0)) {
+        there = false;
+        break;
+      }
+    }
+  }
+  return __all_sync(0xffffffffu, there);
+}
+__device__ __forceinline__ bool elected() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+
+__device__ __noinline__ void load_row8_scalar(const void* q, long long at, int dtype, float* x) {
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) x[i] = load_as_f32(q, at + i, dtype);
+}
 // Eight neighbouring elements of a query row.
 __device__ __forceinline__ void load_row8(const SharedPlan& p, long long at, float* x) {
   if (!p.wide) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = load_as_f32(p.a.q, at + i, p.a.dtype);
+    load_row8_scalar(p.a.q, at, p.a.dtype, x);
   } else if (p.a.dtype == CB_F32) {
     const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p.a.q) + at);
     const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p.a.q) + at + 4);
@@ -167,105 +222,107 @@ struct SharedWalk {
 // Barriers of a block.  Sets and stages count their phases apart.
 struct SharedSync {
   uint64_t key_full[kStages], key_free[kStages], value_full[kStages], value_free[kStages];
-  uint64_t query_full, query_free, score_full[2], weight_full[2], value_done[2], all_done;
+  uint64_t query_full, query_free, score_full[2][2], weight_full[2][2], value_done[2], all_done;  // [set][tile % 2]
   uint32_t tmem;
   int abort, found;
 };
 
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
+}
+
 // Keys (or values) of the range's tiles: codes to fp16 in shared memory, rows of 64
 // elements on 128 bytes, their 16-byte pieces exchanged as the products read them.  The
-// loads of kAhead tiles are in flight.
-template <int SIZE, int STORAGE, bool VALUES>
-__device__ __forceinline__ bool convert(const SharedPlan& p, const SharedWalk& w, char* tiles, Scales* scales,
-                                        SharedSync& sync) {
-  constexpr int kPieces = SIZE / 16, kLoads = kSharedTile * kPieces / kSetThreads, kAhead = 3;
+// codes of the next kAhead tiles are copied to shared memory meanwhile; a thread
+// converts what it copied, so nothing but its own copies has to be waited for.  One
+// copy of this code serves both, in rolled loops: what the roles run by turns has to
+// fit the instruction cache (with 80 KB of unrolled code a tile took 5900 cycles).
+template <int SIZE, int STORAGE>
+__device__ __forceinline__ bool convert(const SharedPlan& p, const SharedWalk& w, bool values, char* tiles, char* codes,
+                                        Scales* scales, float (*raw)[12], SharedSync& sync) {
+  constexpr int kPieces = SIZE / 16, kLoads = kSharedTile * kPieces / kSetThreads, kRows = kSetThreads / kPieces;
+  constexpr int kNoPage = INT_MIN;
   const cb_paged_cache& c = p.a.cache;
-  const int thread = threadIdx.x - 32 * (VALUES ? kValueWarp : kKeyWarp);
+  const int thread = threadIdx.x % kSetThreads, lane = threadIdx.x & 31;
   const int piece = thread % kPieces, row = thread / kPieces;
   const int shift = 31 - __clz(c.page), count = w.end - w.begin;
-  const char* pool = static_cast<const char*>(VALUES ? c.v_pages : c.k_pages);
-  uint4 codes[kAhead][kLoads];
-  int pages[kLoads], scale_page;  // of the tile that is loaded next, found one earlier
-  float key_scale[kAhead], value_scale[kAhead];
-  bool there[kAhead];
+  const char* pool = static_cast<const char*>(values ? c.v_pages : c.k_pages) + piece * 16;
 
-  // the tile whose pages are looked up next, and the one that is loaded next
-  int look = 0, look_tile = w.begin % w.cut.tiles;
+  // the page of keys 16 (lane % 4) .. + 15 of the tile that is copied next, found one earlier
+  int look = 0, look_tile = w.begin % w.cut.tiles, found = kNoPage;
   int load_tile = look_tile, load_item = w.begin / w.cut.tiles;
-  auto page_of = [&](int r) {  // of row r: -1 where there is none
-    const int key = look < count ? look_tile * kSharedTile + r : w.keys;
-    if (key >= w.keys) return -1;
-    const int page = w.table[key >> shift];
-    if (page < 0 || page >= c.pages) {
-      raise_flag(p.a.error_flag, CB_FLAG_BOOK);
-      return -1;
-    }
-    return page;
-  };
   auto look_up = [&] {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) pages[i] = page_of(row + i * (kSetThreads / kPieces));
-    if (VALUES) scale_page = page_of((thread & 3) * 16);
+    const int key = look_tile * kSharedTile + (lane & 3) * 16;
+    found = look < count && key < w.keys ? __ldg(w.table + (key >> shift)) : kNoPage;
     ++look;
     if (++look_tile == w.cut.tiles) look_tile = 0;
   };
-  auto load = [&](int slot) {  // and looks up the next tile's pages
+  const uint32_t codes_at = smem_addr(codes) + thread * 16;
+  auto copy = [&](int slot) {  // and looks up the next tile's pages
     const int head = min(load_item / w.blocks, c.kv_heads - 1);
-#pragma unroll
+    bool real = static_cast<unsigned>(found) < static_cast<unsigned>(c.pages);
+    if (!real && found != kNoPage) raise_flag(p.a.error_flag, CB_FLAG_BOOK);
+    const int page = real ? found : -1;
+#pragma unroll 1
     for (int i = 0; i < kLoads; ++i) {
-      const int key = load_tile * kSharedTile + row + i * (kSetThreads / kPieces);
-      codes[slot][i] = make_uint4(0, 0, 0, 0);
-      if (pages[i] >= 0)
-        codes[slot][i] = __ldg(reinterpret_cast<const uint4*>(
-            pool + ((static_cast<long long>(pages[i]) * c.kv_heads + head) * c.page + (key & (c.page - 1))) * SIZE +
-            piece * 16));
+      const int r = row + i * kRows, at = __shfl_sync(0xffffffffu, page, r / 16);
+      const int in = (load_tile * kSharedTile + r) & (c.page - 1);
+      const long long line = (static_cast<long long>(max(at, 0)) * c.kv_heads + head) * c.page + in;
+      copy16(codes_at + slot * SharedShape<SIZE>::kCodeBytes + i * kSetThreads * 16, pool + line * SIZE, at >= 0);
     }
-    if (VALUES) {
-      there[slot] = scale_page >= 0;
-      const long long line = static_cast<long long>(max(scale_page, 0)) * c.kv_heads + head;
-      key_scale[slot] = scale_page >= 0 ? __ldg(c.k_scale + line) : 0.0f;
-      value_scale[slot] = scale_page >= 0 ? __ldg(c.v_scale + line) : 0.0f;
+    if (values && thread < 4) {
+      const long long line = static_cast<long long>(max(page, 0)) * c.kv_heads + head;
+      copy4(smem_addr(raw[slot] + thread), c.k_scale + line, real);
+      copy4(smem_addr(raw[slot] + 4 + thread), c.v_scale + line, real);
+      raw[slot][8 + thread] = real ? 1.0f : 0.0f;
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
     if (++load_tile == w.cut.tiles) {
       load_tile = 0;
       ++load_item;
     }
     look_up();
   };
-  if (VALUES && SIZE == 32) {  // the columns that no element has
+  if (values && SIZE == 32) {  // the columns that no element has
     for (int i = thread; i < kStages * kSharedTile * 4; i += kSetThreads)
       *reinterpret_cast<uint4*>(tiles + i / (kSharedTile * 4) * SharedShape<SIZE>::kStageBytes +
                                 tc::swizzle_offset(i / 4 % kSharedTile, 4 + i % 4)) = make_uint4(0, 0, 0, 0);
   }
   look_up();
-#pragma unroll
-  for (int n = 0; n < kAhead; ++n) load(n);
+  uint64_t* const free = values ? sync.value_free : sync.key_free;
+  uint64_t* const full = values ? sync.value_full : sync.key_full;
   bool ok = true;
-  for (int n = 0; n < count; n += kAhead) {
-#pragma unroll
-    for (int slot = 0; slot < kAhead; ++slot) {
-      const int at = n + slot;
-      if (at >= count) break;
-      const int stage = at % kStages, turn = at / kStages;
-      uint64_t* free = (VALUES ? sync.value_free : sync.key_free) + stage;
-      if (turn > 0 && ok) ok = tc::wait_or_abort(free, static_cast<uint32_t>((turn - 1) & 1), &sync.abort);
-      char* to = tiles + stage * SharedShape<SIZE>::kStageBytes;
-#pragma unroll
+  int stage = 0, turn = 0, slot = 0;
+#pragma unroll 1
+  for (int n = -kAhead; n < count; ++n) {
+    if (n >= 0) {
+      if (turn > 0 && ok) ok = wait_warp<false>(free + stage, static_cast<uint32_t>((turn - 1) & 1), &sync.abort);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+      const int first = piece % 4 * 2;
+      const bool turned = piece >= 4;  // (so that both chunks' pieces of a row touch different banks)
+      char* to = tiles + stage * SharedShape<SIZE>::kStageBytes + piece / 4 * kChunkBytes;
+      const char* from = codes + slot * SharedShape<SIZE>::kCodeBytes + thread * 16;
+#pragma unroll 1
       for (int i = 0; i < kLoads; ++i) {
-        const int r = row + i * (kSetThreads / kPieces), first = piece % 4 * 2;
-        const uint32_t word[4] = {codes[slot][i].x, codes[slot][i].y, codes[slot][i].z, codes[slot][i].w};
-        uint32_t h[8];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) to_halves<STORAGE>(word[k], h[2 * k], h[2 * k + 1]);
-        char* line = to + piece / 4 * kChunkBytes;
-        const uint4 low = make_uint4(h[0], h[1], h[2], h[3]), high = make_uint4(h[4], h[5], h[6], h[7]);
-        const bool turned = piece >= 4;  // (so that both chunks' pieces of a row touch different banks)
-        *reinterpret_cast<uint4*>(line + tc::swizzle_offset(r, first + turned)) = turned ? high : low;
-        *reinterpret_cast<uint4*>(line + tc::swizzle_offset(r, first + !turned)) = turned ? low : high;
+        const int r = row + i * kRows;
+        const uint2 v = *reinterpret_cast<const uint2*>(from + i * kSetThreads * 16 + 8 * turned);
+        const uint2 u = *reinterpret_cast<const uint2*>(from + i * kSetThreads * 16 + 8 * !turned);
+        uint4 h;
+        to_halves<STORAGE>(v.x, h.x, h.y);
+        to_halves<STORAGE>(v.y, h.z, h.w);
+        *reinterpret_cast<uint4*>(to + tc::swizzle_offset(r, first + turned)) = h;
+        to_halves<STORAGE>(u.x, h.x, h.y);
+        to_halves<STORAGE>(u.y, h.z, h.w);
+        *reinterpret_cast<uint4*>(to + tc::swizzle_offset(r, first + !turned)) = h;
       }
-      if (VALUES && thread < 32) {
-        const float v = value_scale[slot], k = key_scale[slot];
-        const bool real = there[slot];
+      if (values && thread < 32) {
+        const int run = thread & 3;
+        __syncwarp();  // (what lanes 0-3 copied)
+        const float k = raw[slot][run], v = raw[slot][4 + run];
+        const bool real = raw[slot][8 + run] != 0.0f;
         const bool regular = !real || (v >= 9.3e-10f && v <= 1.07e9f && k >= 0.0f);  // 2^-30 .. 2^30
         float log = -INFINITY, inverse = 0.0f, factor = 1.0f;
         if (real) {
@@ -283,65 +340,84 @@ __device__ __forceinline__ bool convert(const SharedPlan& p, const SharedWalk& w
           s.factor[thread] = factor;
           if (thread == 0) s.irregular = odd;
         }
+        __syncwarp();  // (before lanes 0-3 copy into the slot again)
       }
       tc::fence_async_shared();
-      mbar_arrive((VALUES ? sync.value_full : sync.key_full) + stage);
-      load(slot);
+      mbar_arrive(full + stage);
+      if (++stage == kStages) {
+        stage = 0;
+        ++turn;
+      }
     }
+    copy(slot);
+    if (++slot == kAhead) slot = 0;
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   return ok;
 }
 
-// Issues the products of the block's range; one thread.  A job is a tile of one set:
-// both sets take every tile (SETS 2: their own rows) or every other one (1: the same rows).
+// Issues the products of a set over the block's range: a warp, so that what it computes
+// is uniform, and one lane of it.  Both sets take every tile (SETS 2: their own rows)
+// or every other one (1: the same rows).  The scores of two tiles are under way, so
+// that the set weighs one while the other is multiplied.  (While warps take
+// exponentials, a look at a barrier can wait for hundreds of cycles, so there are as
+// few as possible: that a tile's values are there is known from its weights.)
 template <int SIZE, int SETS, bool LO>
-__device__ __forceinline__ bool issue(const SharedWalk& w, const char* keys, const char* values, SharedSync& sync) {
+__device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* keys, const char* values,
+                                      const char* queries, SharedSync& sync) {
   using S = SharedShape<SIZE>;
   constexpr uint32_t kScoreDesc = idesc_f16(kSharedTile, false), kValueDesc = idesc_f16(S::kWide, true);
   volatile int* abort = &sync.abort;
-  const uint32_t tmem = sync.tmem;
-  int done[2] = {0, 0}, segment = 0, before = 0;  // iterations of the sets; tiles before the segment
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sync.tmem, 0);
+  const bool leads = elected();
+  const uint64_t query = tc::sw128_desc(queries + (SETS == 2 ? set * S::kQueryBytes : 0));
+  int iteration = 0, segment = 0, before = 0;  // tiles of the set; tiles before the segment
+#pragma unroll 1
   for (int at = w.begin; at < w.end; ++segment) {
-    const int tiles = min(w.cut.tiles - at % w.cut.tiles, w.end - at), jobs = SETS * tiles;
-    if (!tc::wait_or_abort(&sync.query_full, static_cast<uint32_t>(segment & 1), abort)) return false;
+    const int tiles = min(w.cut.tiles - at % w.cut.tiles, w.end - at), jobs = SETS == 2 ? tiles : (tiles - set + 1) / 2;
+    if (!wait_warp(&sync.query_full, static_cast<uint32_t>(segment & 1), abort)) return false;
     tc::fence_after();
-    auto scores = [&](int job) {
-      const int set = job & 1, n = before + (SETS == 2 ? job / 2 : job), stage = n % kStages;
-      if (!tc::wait_or_abort(sync.key_full + stage, static_cast<uint32_t>(n / kStages & 1), abort)) return false;
-      tc::fence_after();
-      const char* tile = keys + stage * S::kStageBytes;
-      const uint32_t d = tmem + kScoresAt + set * kSharedTile;
-      const uint32_t q = tmem + kQueriesAt + (SETS == 2 ? set * 64 : 0);
+#pragma unroll 1
+    for (int job = -2; job < jobs; ++job) {
+      if (job >= 0) {  // the weighted values of tile `job`
+        const int n = before + (SETS == 2 ? job : 2 * job + set), now = iteration + job, buffer = now & 1;
+        if (!wait_warp(sync.weight_full[set] + buffer, static_cast<uint32_t>(now / 2 & 1), abort)) return false;
+        tc::fence_after();
+        const uint64_t tile = across_desc(values + n % kStages * S::kStageBytes);
+        const uint32_t d = tmem + kValuesAt + set * 128, a = tmem + kScoresAt + (set * 2 + buffer) * kSharedTile;
+        if (leads) {
 #pragma unroll
-      for (int part = 0; part < (LO ? 2 : 1); ++part)
+          for (int part = 0; part < (LO ? 2 : 1); ++part)
 #pragma unroll
-        for (int k = 0; k < SIZE / 16; ++k)
-          multiply(d, q + part * 64 + k * 8, tc::sw128_desc(tile + k / 4 * kChunkBytes + k % 4 * 32), kScoreDesc,
-                   part + k > 0 ? 1u : 0u);
-      tc::umma_commit(sync.score_full + set);
-      if (SETS == 1 || set == 1) tc::umma_commit(sync.key_free + stage);
-      if (job + 1 == jobs) tc::umma_commit(&sync.query_free);
-      return true;
-    };
-    for (int job = 0; job < min(2, jobs); ++job)
-      if (!scores(job)) return false;
-    for (int job = 0; job < jobs; ++job) {
-      const int set = job & 1, n = before + (SETS == 2 ? job / 2 : job), stage = n % kStages;
-      if (!tc::wait_or_abort(sync.weight_full + set, static_cast<uint32_t>(done[set] & 1), abort)) return false;
-      ++done[set];
-      if (!tc::wait_or_abort(sync.value_full + stage, static_cast<uint32_t>(n / kStages & 1), abort)) return false;
-      tc::fence_after();
-      const char* tile = values + stage * S::kStageBytes;
-      const uint32_t d = tmem + kValuesAt + set * 128, a = tmem + kScoresAt + set * kSharedTile;
+            for (int k = 0; k < kSharedTile / 16; ++k)
+              multiply(d, a + k * 16 + part * 8, tile + k * 2048 / 16, kValueDesc, job > 0 || part + k > 0);
+          tc::umma_commit(sync.value_done + set);
+          tc::umma_commit(sync.value_free + n % kStages);
+        }
+        __syncwarp();
+      }
+      if (job + 2 < jobs) {  // the scores of the tile after the next
+        const int n = before + (SETS == 2 ? job + 2 : 2 * (job + 2) + set), buffer = (iteration + job) & 1;
+        if (!wait_warp(sync.key_full + n % kStages, static_cast<uint32_t>(n / kStages & 1), abort)) return false;
+        tc::fence_after();
+        const uint64_t tile = tc::sw128_desc(keys + n % kStages * S::kStageBytes);
+        const uint32_t d = tmem + kScoresAt + (set * 2 + buffer) * kSharedTile;
+        if (leads) {
 #pragma unroll
-      for (int part = 0; part < (LO ? 2 : 1); ++part)
+          for (int part = 0; part < (LO ? 2 : 1); ++part)
 #pragma unroll
-        for (int k = 0; k < kSharedTile / 16; ++k)
-          multiply(d, a + part * 32 + k * 8, across_desc(tile + k * 2048), kValueDesc, job >= 2 || part + k > 0 ? 1u : 0u);
-      tc::umma_commit(sync.value_done + set);
-      if (SETS == 1 || set == 1) tc::umma_commit(sync.value_free + stage);
-      if (job + 2 < jobs && !scores(job + 2)) return false;
+            for (int k = 0; k < SIZE / 16; ++k)
+              multiply_shared(d, query + (part * S::kQueryBytes + k / 4 * kRowLanes * 128 + k % 4 * 32) / 16,
+                              tile + (k / 4 * kChunkBytes + k % 4 * 32) / 16, kScoreDesc, part + k > 0);
+          tc::umma_commit(sync.score_full[set] + buffer);
+          tc::umma_commit(sync.key_free + n % kStages);
+        }
+        __syncwarp();
+      }
     }
+    if (leads) tc::umma_commit(&sync.query_free);
+    __syncwarp();
+    iteration += jobs;
     at += tiles;
     before += tiles;
   }
@@ -351,23 +427,41 @@ __device__ __forceinline__ bool issue(const SharedWalk& w, const char* keys, con
 // The references follow the scores and value scales (their logarithms included) as
 // in paged_attention.cuh: what multiplies the value codes is 2^(y - c), y a key's
 // score plus the logarithm of its value scale.  A tile whose largest is more
-// than kRise above c or kFall below it moves c to kRest below it.
-constexpr float kRise = 13.0f, kFall = 6.0f, kRest = 5.0f, kFarBelow = 60.0f, kHeld = 1.2676506002282294e30f;  // 2^100
+// than kRise above c or `fall` below it moves c to kRest below it: it is rounded to
+// 2^-24 of 2^(y - c), so the largest of every tile keeps 9 bits, of two parts
+// (float32) 22.  Moving takes a pass over the sums; the wide range makes it rare.
+constexpr float kRise = 15.0f, kRest = 2.0f, kFarBelow = 60.0f, kHeld = 1.2676506002282294e30f;  // 2^100
+__host__ __device__ constexpr float fall_of(bool lo) { return lo ? 2.0f : 15.0f; }
+
+// Sixteen weights as fp16, and what is left of them.
+template <bool LO>
+__device__ __forceinline__ void store_weights(uint32_t at, const float* x) {
+  uint32_t hi[8], lo[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const __half2 h = __floats2half2_rn(x[2 * k], x[2 * k + 1]);
+    hi[k] = bits(h);
+    if (LO) lo[k] = bits(__floats2half2_rn(x[2 * k] - __low2float(h), x[2 * k + 1] - __high2float(h)));
+  }
+  store8(at, hi);
+  if (LO) store8(at + 8, lo);
+}
 
 // A set of 128 rows, a thread each.
 template <int SIZE, int STORAGE, int SETS, bool LO>
-__device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, const Scales* scales, SharedSync& sync) {
+__device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, char* queries, const Scales* scales,
+                                      SharedSync& sync) {
   const int set = threadIdx.x / kSetThreads, r = threadIdx.x % kSetThreads;
   const int local = SETS == 2 ? threadIdx.x : r;
   volatile int* abort = &sync.abort;
   const uint32_t lanes = sync.tmem + (static_cast<uint32_t>(threadIdx.x / 32 % 4 * 32) << 16);
-  const uint32_t scores = lanes + kScoresAt + set * kSharedTile, sums = lanes + kValuesAt + set * 128;
-  const long long all_rows = p.a.batch * p.rows;
+  const uint32_t sums = lanes + kValuesAt + set * 128;
+  const int all_rows = static_cast<int>(p.a.batch) * p.rows;
   int iteration = 0, segment = 0, before = 0;
   for (int at = w.begin; at < w.end; ++segment) {
     const int item = at / w.cut.tiles, tiles = min(w.cut.tiles - at % w.cut.tiles, w.end - at);
     const int head = item / w.blocks;
-    const long long row = static_cast<long long>(item % w.blocks) * p.shared.block_rows + local;
+    const int row = item % w.blocks * p.shared.block_rows + local;
     const bool real = row < all_rows, any = __any_sync(0xffffffffu, real);  // (rows of no warp are skipped)
 
     // the row's queries, scaled to below 2, in the order of the codes' halves
@@ -375,11 +469,11 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
     {
       long long from = 0;
       if (real) {
-        const long long b = row / p.rows, t = row % p.rows / p.group, h = head * p.group + row % p.group;
+        const int b = row / p.rows, t = row % p.rows / p.group, h = head * p.group + row % p.group;
         from = b * p.a.q_strides[0] + t * p.a.q_strides[1] + h * p.a.q_strides[2];
       }
       float largest = 0.0f;
-#pragma unroll 4
+#pragma unroll 2
       for (int d = 0; d < SIZE; d += 8) {
         float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         if (real) load_row8(p, from + d, x);
@@ -390,34 +484,25 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
       const float down = e == 127 ? 5.877471754111438e-39f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
       const float sign = p.a.scale < 0.0f ? -down : down;
       factor = fabsf(p.a.scale) * 1.4426950408889634f * power2(e);
-      if (segment > 0 &&
-          !__all_sync(0xffffffffu, tc::wait_or_abort(&sync.query_free, static_cast<uint32_t>((segment - 1) & 1), abort)))
-        return false;
-      tc::fence_after();
+      if (segment > 0 && !wait_warp(&sync.query_free, static_cast<uint32_t>((segment - 1) & 1), abort)) return false;
       const bool writes = SETS == 2 || LO || set == 0;
+      char* to = queries + (SETS == 2 || LO ? set * SharedShape<SIZE>::kQueryBytes : 0);
 #pragma unroll 1
-      for (int d = 0; writes && d < SIZE; d += 16) {
-        uint32_t hi[8], lo[8];
-        float x[16];
+      for (int d = 0; writes && d < SIZE; d += 8) {
+        uint32_t h[4];
+        float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (real) load_row8(p, from + d, x);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = 0.0f;
-        if (real) {
-          load_row8(p, from + d, x);
-          load_row8(p, from + d + 8, x + 8);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
           const int first = STORAGE == CB_I8 ? i / 2 * 4 + i % 2 : 2 * i, second = STORAGE == CB_I8 ? first + 2 : first + 1;
           const float a = x[first] * sign, b = x[second] * sign;
-          const __half2 h = __floats2half2_rn(a, b);
-          hi[i] = bits(h);
-          lo[i] = bits(__floats2half2_rn(a - __low2float(h), b - __high2float(h)));
+          const __half2 hi = __floats2half2_rn(a, b);
+          h[i] = LO && set == 1 ? bits(__floats2half2_rn(a - __low2float(hi), b - __high2float(hi))) : bits(hi);
         }
-        const bool second = LO && set == 1;
-        store8(lanes + kQueriesAt + (SETS == 2 || LO ? set * 64 : 0) + d / 2, second ? lo : hi);
+        *reinterpret_cast<uint4*>(to + d / 64 * kRowLanes * 128 + tc::swizzle_offset(r, d % 64 / 8)) =
+            make_uint4(h[0], h[1], h[2], h[3]);
       }
-      tc::tmem_wait_st();
-      tc::fence_before();
+      tc::fence_async_shared();
       mbar_arrive(&sync.query_full);
     }
 
@@ -425,44 +510,51 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
     bool first = true;
     for (int tile = SETS == 2 ? 0 : set; tile < tiles; tile += SETS == 2 ? 1 : 2, ++iteration) {
       const int n = before + tile, stage = n % kStages;
-      if (!__all_sync(0xffffffffu, tc::wait_or_abort(sync.score_full + set, static_cast<uint32_t>(iteration & 1), abort) &&
-                                       tc::wait_or_abort(sync.value_full + stage, static_cast<uint32_t>(n / kStages & 1), abort)))
+      const int buffer = iteration & 1;
+      const uint32_t scores = lanes + kScoresAt + (set * 2 + buffer) * kSharedTile;
+      if (!wait_warp(sync.value_full + stage, static_cast<uint32_t>(n / kStages & 1), abort) ||
+          !wait_warp(sync.score_full[set] + buffer, static_cast<uint32_t>(iteration / 2 & 1), abort))
         return false;
       tc::fence_after();
       if (any) {
-        float s[kSharedTile];
-        tc::tmem_load32_nowait(scores, s);
-        tc::tmem_load32_nowait(scores + 32, s + 32);
+        float s[kSharedTile], by[4], log[4], inverse[4];
         const Scales& at_stage = scales[stage];
-        float by[4], log[4], inverse[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          by[i] = factor * at_stage.key[i];
-          log[i] = at_stage.log[i];
-          inverse[i] = at_stage.inverse[i];
-        }
         const bool irregular = at_stage.irregular != 0;
-        tc::tmem_wait_ld();
-        tc::reg_fence<kSharedTile>(s);
         float top = -INFINITY;
+        if (__builtin_expect(!irregular, 1)) {
+          tc::tmem_load32_nowait(scores, s);
+          tc::tmem_load32_nowait(scores + 32, s + 32);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float most = s[16 * i], least = s[16 * i];
-#pragma unroll
-          for (int k = 1; k < 16; ++k) most = fmaxf(most, s[16 * i + k]);
-          if (irregular) {
-#pragma unroll
-            for (int k = 1; k < 16; ++k) least = fminf(least, s[16 * i + k]);
+          for (int i = 0; i < 4; ++i) {
+            by[i] = factor * at_stage.key[i];
+            log[i] = at_stage.log[i];
+            inverse[i] = at_stage.inverse[i];
           }
-          top = fmaxf(top, fmaf(by[i] < 0.0f ? least : most, by[i], log[i]));
+          tc::tmem_wait_ld();
+          tc::reg_fence<kSharedTile>(s);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float most = s[16 * i];
+#pragma unroll
+            for (int k = 1; k < 16; ++k) most = fmaxf(most, s[16 * i + k]);
+            top = fmaxf(top, fmaf(most, by[i], log[i]));
+          }
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) {
+            float x[16];
+            tc::tmem_load16(scores + i * 16, x);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) top = fmaxf(top, fmaf(x[k], factor * at_stage.key[i], at_stage.log[i]));
+          }
         }
-        const bool moves = first || top > c + kRise || top < c - kFall;
+        const bool moves = first || top > c + kRise || top < c - fall_of(LO);
         if (__any_sync(0xffffffffu, moves)) {
           const float next = floorf(top) - kRest;
           float now = c;
           if (first) now = top > -INFINITY ? next : 0.0f;
           else if (top > c + kRise) now = next;
-          else if (top < c - kFall && top > -INFINITY) {
+          else if (top < c - fall_of(LO) && top > -INFINITY) {
             now = fmaxf(next, c - 50.0f);
             if (fmaxf(sum, l) * exp2_of(c - now) > kHeld) now = c;
           }
@@ -470,29 +562,32 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
             const float scale = exp2_of(c - now);
             l *= scale;
             sum *= scale;
-            if (!__all_sync(0xffffffffu, tc::wait_or_abort(sync.value_done + set, static_cast<uint32_t>((iteration - 1) & 1), abort)))
-              return false;
+            if (!wait_warp(sync.value_done + set, static_cast<uint32_t>((iteration - 1) & 1), abort)) return false;
             tc::fence_after();
 #pragma unroll 1
-            for (int d = 0; d < SharedShape<SIZE>::kWide; d += 8) {
-              float o[8];
-              load8(sums + d, o);
-              uint32_t v[8];
+            for (int d = 0; d < SharedShape<SIZE>::kWide; d += 32) {
+              float o[32];
+              tc::tmem_load32_nowait(sums + d, o);
+              tc::tmem_wait_ld();
+              tc::reg_fence<32>(o);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(o[i] * scale);
-              store8(sums + d, v);
+              for (int i = 0; i < 32; i += 8) {
+                uint32_t v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = __float_as_uint(o[i + k] * scale);
+                store8(sums + d + i, v);
+              }
             }
           }
           c = now;
         }
         first = false;
-        const bool slow = irregular || __any_sync(0xffffffffu, top < c - kFarBelow);
+        if (__builtin_expect(!irregular && !__any_sync(0xffffffffu, top < c - kFarBelow), 1)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float* x = s + 16 * i;
-          const float shift = log[i] - c;
-          float run[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          if (!slow) {
+          for (int i = 0; i < 4; ++i) {
+            float* x = s + 16 * i;
+            const float shift = log[i] - c;
+            float run[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               x[k] = exp2_of(fmaf(x[k], by[i], shift));
@@ -501,39 +596,34 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
             const float all = (run[0] + run[1]) + (run[2] + run[3]);
             l = fmaf(all, inverse[i], l);
             sum += all;
-          } else {  // scales of any sign and size: weights by themselves
-            const float kept = at_stage.factor[i];
-            float weights = 0.0f;
+            store_weights<LO>(scores + i * 16, x);
+          }
+        } else {  // value scales of any sign and size, or all far below c: the weights by themselves
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) {
+            const float by_i = factor * at_stage.key[i], shift = at_stage.log[i] - c, kept = at_stage.factor[i];
+            float x[16], weights = 0.0f;
+            tc::tmem_load16(scores + i * 16, x);
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-              const float score = x[k] * by[i];
+              const float score = x[k] * by_i;
               weights += exp2_of(score - c);
               x[k] = exp2_of(score + shift);
-              run[k & 3] += x[k];
+              sum += x[k];
               x[k] *= kept;
             }
-            if (inverse[i] != 0.0f) l += weights;
-            sum += (run[0] + run[1]) + (run[2] + run[3]);
+            if (at_stage.inverse[i] != 0.0f) l += weights;
+            store_weights<LO>(scores + i * 16, x);
           }
-          uint32_t hi[8], lo[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const __half2 h = __floats2half2_rn(x[2 * k], x[2 * k + 1]);
-            hi[k] = bits(h);
-            if (LO) lo[k] = bits(__floats2half2_rn(x[2 * k] - __low2float(h), x[2 * k + 1] - __high2float(h)));
-          }
-          store8(scores + i * 8, hi);
-          if (LO) store8(scores + 32 + i * 8, lo);
         }
         tc::tmem_wait_st();
       }
       tc::fence_before();
-      mbar_arrive(sync.weight_full + set);
+      mbar_arrive(sync.weight_full[set] + buffer);
     }
     // the part of this set
     const bool some = SETS == 2 || tiles > set;
-    if (some && !__all_sync(0xffffffffu, tc::wait_or_abort(sync.value_done + set, static_cast<uint32_t>((iteration - 1) & 1), abort)))
-      return false;
+    if (some && !wait_warp(sync.value_done + set, static_cast<uint32_t>((iteration - 1) & 1), abort)) return false;
     tc::fence_after();
     if (any) {
       const int rows = p.shared.block_rows;
@@ -567,6 +657,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
   extern __shared__ char memory[];
   __shared__ SharedSync sync;
   __shared__ Scales scales[kStages];
+  __shared__ float raw[kAhead][12];  // scales on their way: of keys, of values, whether there are any
   char* tiles = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(memory) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
@@ -575,17 +666,19 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
     for (int i = 0; i < kStages; ++i) {
       mbar_init(sync.key_full + i, kSetThreads);
       mbar_init(sync.value_full + i, kSetThreads);
-      mbar_init(sync.key_free + i, 1);
-      mbar_init(sync.value_free + i, 1);
+      mbar_init(sync.key_free + i, SETS);
+      mbar_init(sync.value_free + i, SETS);
     }
     mbar_init(&sync.query_full, 2 * kSetThreads);
-    mbar_init(&sync.query_free, 1);
+    mbar_init(&sync.query_free, 2);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(sync.score_full + i, 1);
-      mbar_init(sync.weight_full + i, kSetThreads);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(sync.score_full[i] + k, 1);
+        mbar_init(sync.weight_full[i] + k, kSetThreads);
+      }
       mbar_init(sync.value_done + i, 1);
     }
-    mbar_init(&sync.all_done, 1);
+    mbar_init(&sync.all_done, 2);
     mbar_fence_init();
     sync.abort = 0;
   }
@@ -603,25 +696,29 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
   w.end = static_cast<int>(min(begin + w.cut.per, all));
   w.table = p.a.cache.table + __ldcg(p.shared.common + p.a.batch) * p.a.cache.columns;
   const char* values = tiles + S::kChunks * kChunkBytes;
+  char* queries = tiles + kStages * S::kStageBytes;
+  char* codes = queries + 2 * S::kQueryBytes;
   bool ok = true;
   if (w.begin < w.end) {
-    if (warp < kKeyWarp) {
-      ok = weigh<SIZE, STORAGE, SETS, LO>(p, w, scales, sync);
-    } else if (warp < kValueWarp) {
-      ok = convert<SIZE, STORAGE, false>(p, w, tiles, scales, sync);
-    } else if (warp < kIssueWarp) {
-      ok = convert<SIZE, STORAGE, true>(p, w, tiles + S::kChunks * kChunkBytes, scales, sync);
-    } else if (lane == 0) {
-      ok = issue<SIZE, SETS, LO>(w, tiles, values, sync);
-      tc::umma_commit(&sync.all_done);  // arrives once every product issued above has completed
+    if (warp >= kIssueWarp) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegisters));
+      if (warp < kIssueWarp + 2) ok = issue<SIZE, SETS, LO>(w, warp - kIssueWarp, tiles, values, queries, sync);
+    } else if (warp < kKeyWarp) {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWeighRegisters));
+      ok = weigh<SIZE, STORAGE, SETS, LO>(p, w, queries, scales, sync);
+    } else {
+      const bool is_value = warp >= kValueWarp;
+      ok = convert<SIZE, STORAGE>(p, w, is_value, is_value ? tiles + S::kChunks * kChunkBytes : tiles,
+                                  is_value ? codes + S::kCodeBytes / 2 : codes, scales, raw, sync);
     }
     if (!ok) {
       raise_flag(p.a.error_flag, CB_FLAG_WAIT_DATA);
       sync.abort = 1;
     }
-  } else if (threadIdx.x == 32 * kIssueWarp) {
-    tc::umma_commit(&sync.all_done);
   }
+  __syncwarp();
+  // (arrives once every product that was issued has completed; the lanes that issued them)
+  if ((warp == kIssueWarp || warp == kIssueWarp + 1) && elected()) tc::umma_commit(&sync.all_done);
   __syncwarp();
   tc::fence_before();
   __syncthreads();
@@ -669,7 +766,7 @@ int shared_check(const cb_paged_attention_args& a) {
   const long long rows = a.batch * a.tokens * (a.heads / a.cache.kv_heads);
   const long long tiles = (a.cache.columns * a.cache.page + kSharedTile - 1) / kSharedTile;
   const double units = static_cast<double>((rows + kRowLanes - 1) / kRowLanes) * a.cache.kv_heads * tiles;
-  CB_REQUIRE(units + (1 << 20) < 2147483648.0,
+  CB_REQUIRE(units + (1 << 20) < 2147483648.0 && rows < (1LL << 31) - 2 * kRowLanes,
              "cb_paged_attention_shared: %lld rows of up to %lld keys are too many for one call", rows,
              a.cache.columns * a.cache.page);
   return CB_OK;
