@@ -74,21 +74,26 @@ struct SharedPlan {
 
 constexpr int kRowLanes = 128;  // rows of a product: lanes of the tensor memory
 constexpr int kSetThreads = 128;
-constexpr int kKeyWarp = 8, kValueWarp = 12, kIssueWarp = 16;  // warps 0-7: two sets of rows; 16 and 17 issue theirs
+// warps 0-7: two sets of rows; 16 and 17 issue theirs; 18 looks up pages and scales
+constexpr int kKeyWarp = 8, kValueWarp = 12, kIssueWarp = 16, kLookWarp = 18;
 constexpr int kSharedThreads = 32 * (kIssueWarp + 4);
 // Registers of a thread: as launched (the converting warps keep them), of the
 // warps that weigh, of the issuing warp and the three beside it (61440 at the
 // launch and after).
 constexpr int kWeighRegisters = 128, kIssueRegisters = 32;
-constexpr int kStages = 3, kAhead = 4;  // tiles as fp16, and tiles whose codes are on their way
+constexpr int kStages = 3, kAhead = 3;  // tiles as fp16, and tiles whose codes are on their way
 constexpr int kChunkBytes = kSharedTile * 128;  // 64 keys of 64 fp16 elements
 // Columns of the tensor memory: weighted values of both sets, then their scores, two
 // tiles each.  The weights of 16 keys take the place of their scores, high parts first.
 constexpr int kValuesAt = 0, kScoresAt = 256, kColumns = 512;
 
-// Per stage: scales of the tile's four runs of 16 keys.
-struct __align__(16) Scales {
-  float key[4], log[4], inverse[4], factor[4];  // of values: log2, 2^-log2, what the logarithm leaves
+// Of a tile's four runs of 16 keys: the line of each in the pools (page and kv head; -1:
+// none), and its scales, of values as log2, 2^-log2 and what the logarithm leaves.
+// They are looked up for eight tiles at a time, a lane to a run.
+constexpr int kBatch = 8, kBatches = 3;
+struct __align__(16) Runs {
+  long long line[4];
+  float key[4], log[4], inverse[4], factor[4];
   int irregular, pad[3];
 };
 
@@ -198,18 +203,58 @@ __device__ __forceinline__ void load_row8(const SharedPlan& p, long long at, flo
     }
   }
 }
-// Eight float32 columns of this thread's lane of the tensor memory (warp-wide).
+// 8, 32 and 64 float32 columns of this thread's lane of the tensor memory (warp-wide).
+// The load and the wait for it are one statement: between two, the compiler could
+// move registers that are not written yet.
 __device__ __forceinline__ void load8(uint32_t at, float* out) {
   uint32_t v[8];
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-               : "r"(at));
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7])
-               :
-               : "memory");
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7"
+      "}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+      : "r"(at)
+      : "memory");
 #pragma unroll
   for (int i = 0; i < 8; ++i) out[i] = __uint_as_float(v[i]);
+}
+__device__ __forceinline__ void load32(uint32_t at, float* out) {
+  uint32_t v[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31"
+      "}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(at)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) out[i] = __uint_as_float(v[i]);
+}
+__device__ __forceinline__ void load64(uint32_t at, float* out) {
+  uint32_t v[64];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, "
+      "%40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, "
+      "%59, %60, %61, %62, %63"
+      "}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]),
+        "=r"(v[32]), "=r"(v[33]), "=r"(v[34]), "=r"(v[35]), "=r"(v[36]), "=r"(v[37]), "=r"(v[38]), "=r"(v[39]),
+        "=r"(v[40]), "=r"(v[41]), "=r"(v[42]), "=r"(v[43]), "=r"(v[44]), "=r"(v[45]), "=r"(v[46]), "=r"(v[47]),
+        "=r"(v[48]), "=r"(v[49]), "=r"(v[50]), "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]),
+        "=r"(v[56]), "=r"(v[57]), "=r"(v[58]), "=r"(v[59]), "=r"(v[60]), "=r"(v[61]), "=r"(v[62]), "=r"(v[63])
+      : "r"(at)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) out[i] = __uint_as_float(v[i]);
 }
 
 // What a role of the block walks: its range of units, item by item.
@@ -222,7 +267,8 @@ struct SharedWalk {
 // Barriers of a block.  Sets and stages count their phases apart.
 struct SharedSync {
   uint64_t key_full[kStages], key_free[kStages], value_full[kStages], value_free[kStages];
-  uint64_t query_full, query_free, score_full[2][2], weight_full[2][2], value_done[2], all_done;  // [set][tile % 2]
+  uint64_t batch_full[kBatches], batch_free[kBatches], query_full, query_free, all_done;
+  uint64_t score_full[2][2], weight_full[2][2], value_done[2][2];  // [set][tile % 2]: no two phases are open at once
   uint32_t tmem;
   int abort, found;
 };
@@ -230,72 +276,70 @@ struct SharedSync {
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
+
+// Looks up the runs of the range's tiles.
+__device__ __forceinline__ bool look_up(const SharedPlan& p, const SharedWalk& w, Runs* runs, SharedSync& sync) {
+  const cb_paged_cache& c = p.a.cache;
+  const int lane = threadIdx.x & 31, run = lane & 3, count = w.end - w.begin, shift = 31 - __clz(c.page);
+#pragma unroll 1
+  for (int batch = 0; batch * kBatch < count; ++batch) {
+    const int n = batch * kBatch + lane / 4, at = w.begin + n, key = at % w.cut.tiles * kSharedTile + run * 16;
+    const int head = at / w.cut.tiles / w.blocks, slot = batch % kBatches;
+    long long line = -1;
+    if (n < count && key < w.keys) {
+      const int page = __ldg(w.table + (key >> shift));
+      if (static_cast<unsigned>(page) < static_cast<unsigned>(c.pages)) line = static_cast<long long>(page) * c.kv_heads + head;
+      else raise_flag(p.a.error_flag, CB_FLAG_BOOK);
+    }
+    const bool real = line >= 0;
+    const float k = real ? __ldg(c.k_scale + line) : 0.0f, v = real ? __ldg(c.v_scale + line) : 1.0f;
+    float log = -INFINITY, inverse = 0.0f, factor = 1.0f;
+    if (real) {  // (an error of the logarithm moves the weights and their sum alike)
+      const float size = fabsf(v);
+      log = isfinite(v) ? fmaxf(__log2f(size), -100.0f) : 0.0f;
+      inverse = exp2_of(-log);
+      factor = !isfinite(v) ? NAN : size < 7.9e-31f ? v * 1.2676506002282294e30f : v < 0.0f ? -1.0f : 1.0f;  // 2^-100, 2^100
+    }
+    const unsigned regular = __ballot_sync(0xffffffffu, v >= 9.3e-10f && v <= 1.07e9f && k >= 0.0f);  // 2^-30 .. 2^30
+    if (batch >= kBatches && !wait_warp<false>(sync.batch_free + slot, static_cast<uint32_t>((batch / kBatches - 1) & 1), &sync.abort))
+      return false;
+    Runs& to = runs[slot * kBatch + lane / 4];
+    to.line[run] = line;
+    to.key[run] = k;
+    to.log[run] = log;
+    to.inverse[run] = inverse;
+    to.factor[run] = factor;
+    if (run == 0) to.irregular = (regular >> lane & 15u) != 15u;
+    mbar_arrive(sync.batch_full + slot);
+  }
+  return true;
 }
 
 // Keys (or values) of the range's tiles: codes to fp16 in shared memory, rows of 64
 // elements on 128 bytes, their 16-byte pieces exchanged as the products read them.  The
 // codes of the next kAhead tiles are copied to shared memory meanwhile; a thread
 // converts what it copied, so nothing but its own copies has to be waited for.  One
-// copy of this code serves both, in rolled loops: what the roles run by turns has to
-// fit the instruction cache (with 80 KB of unrolled code a tile took 5900 cycles).
+// copy of this code serves both: what the roles run by turns has to fit the
+// instruction cache (with 80 KB of unrolled code a tile took 5900 cycles).
 template <int SIZE, int STORAGE>
 __device__ __forceinline__ bool convert(const SharedPlan& p, const SharedWalk& w, bool values, char* tiles, char* codes,
-                                        Scales* scales, float (*raw)[12], SharedSync& sync) {
+                                        const Runs* runs, SharedSync& sync) {
   constexpr int kPieces = SIZE / 16, kLoads = kSharedTile * kPieces / kSetThreads, kRows = kSetThreads / kPieces;
-  constexpr int kNoPage = INT_MIN;
   const cb_paged_cache& c = p.a.cache;
-  const int thread = threadIdx.x % kSetThreads, lane = threadIdx.x & 31;
-  const int piece = thread % kPieces, row = thread / kPieces;
-  const int shift = 31 - __clz(c.page), count = w.end - w.begin;
+  const int thread = threadIdx.x % kSetThreads, piece = thread % kPieces, row = thread / kPieces;
+  const int count = w.end - w.begin;
   const char* pool = static_cast<const char*>(values ? c.v_pages : c.k_pages) + piece * 16;
-
-  // the page of keys 16 (lane % 4) .. + 15 of the tile that is copied next, found one earlier
-  int look = 0, look_tile = w.begin % w.cut.tiles, found = kNoPage;
-  int load_tile = look_tile, load_item = w.begin / w.cut.tiles;
-  auto look_up = [&] {
-    const int key = look_tile * kSharedTile + (lane & 3) * 16;
-    found = look < count && key < w.keys ? __ldg(w.table + (key >> shift)) : kNoPage;
-    ++look;
-    if (++look_tile == w.cut.tiles) look_tile = 0;
-  };
   const uint32_t codes_at = smem_addr(codes) + thread * 16;
-  auto copy = [&](int slot) {  // and looks up the next tile's pages
-    const int head = min(load_item / w.blocks, c.kv_heads - 1);
-    bool real = static_cast<unsigned>(found) < static_cast<unsigned>(c.pages);
-    if (!real && found != kNoPage) raise_flag(p.a.error_flag, CB_FLAG_BOOK);
-    const int page = real ? found : -1;
-#pragma unroll 1
-    for (int i = 0; i < kLoads; ++i) {
-      const int r = row + i * kRows, at = __shfl_sync(0xffffffffu, page, r / 16);
-      const int in = (load_tile * kSharedTile + r) & (c.page - 1);
-      const long long line = (static_cast<long long>(max(at, 0)) * c.kv_heads + head) * c.page + in;
-      copy16(codes_at + slot * SharedShape<SIZE>::kCodeBytes + i * kSetThreads * 16, pool + line * SIZE, at >= 0);
-    }
-    if (values && thread < 4) {
-      const long long line = static_cast<long long>(max(page, 0)) * c.kv_heads + head;
-      copy4(smem_addr(raw[slot] + thread), c.k_scale + line, real);
-      copy4(smem_addr(raw[slot] + 4 + thread), c.v_scale + line, real);
-      raw[slot][8 + thread] = real ? 1.0f : 0.0f;
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    if (++load_tile == w.cut.tiles) {
-      load_tile = 0;
-      ++load_item;
-    }
-    look_up();
-  };
   if (values && SIZE == 32) {  // the columns that no element has
     for (int i = thread; i < kStages * kSharedTile * 4; i += kSetThreads)
       *reinterpret_cast<uint4*>(tiles + i / (kSharedTile * 4) * SharedShape<SIZE>::kStageBytes +
                                 tc::swizzle_offset(i / 4 % kSharedTile, 4 + i % 4)) = make_uint4(0, 0, 0, 0);
   }
-  look_up();
   uint64_t* const free = values ? sync.value_free : sync.key_free;
   uint64_t* const full = values ? sync.value_full : sync.key_full;
   bool ok = true;
   int stage = 0, turn = 0, slot = 0;
+  int next = 0, next_tile = w.begin % w.cut.tiles, batch = 0, batch_turn = 0;  // what is copied next
 #pragma unroll 1
   for (int n = -kAhead; n < count; ++n) {
     if (n >= 0) {
@@ -305,42 +349,22 @@ __device__ __forceinline__ bool convert(const SharedPlan& p, const SharedWalk& w
       const bool turned = piece >= 4;  // (so that both chunks' pieces of a row touch different banks)
       char* to = tiles + stage * SharedShape<SIZE>::kStageBytes + piece / 4 * kChunkBytes;
       const char* from = codes + slot * SharedShape<SIZE>::kCodeBytes + thread * 16;
-#pragma unroll 1
+      uint2 v[kLoads], u[kLoads];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        v[i] = *reinterpret_cast<const uint2*>(from + i * kSetThreads * 16 + 8 * turned);
+        u[i] = *reinterpret_cast<const uint2*>(from + i * kSetThreads * 16 + 8 * !turned);
+      }
+#pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int r = row + i * kRows;
-        const uint2 v = *reinterpret_cast<const uint2*>(from + i * kSetThreads * 16 + 8 * turned);
-        const uint2 u = *reinterpret_cast<const uint2*>(from + i * kSetThreads * 16 + 8 * !turned);
         uint4 h;
-        to_halves<STORAGE>(v.x, h.x, h.y);
-        to_halves<STORAGE>(v.y, h.z, h.w);
+        to_halves<STORAGE>(v[i].x, h.x, h.y);
+        to_halves<STORAGE>(v[i].y, h.z, h.w);
         *reinterpret_cast<uint4*>(to + tc::swizzle_offset(r, first + turned)) = h;
-        to_halves<STORAGE>(u.x, h.x, h.y);
-        to_halves<STORAGE>(u.y, h.z, h.w);
+        to_halves<STORAGE>(u[i].x, h.x, h.y);
+        to_halves<STORAGE>(u[i].y, h.z, h.w);
         *reinterpret_cast<uint4*>(to + tc::swizzle_offset(r, first + !turned)) = h;
-      }
-      if (values && thread < 32) {
-        const int run = thread & 3;
-        __syncwarp();  // (what lanes 0-3 copied)
-        const float k = raw[slot][run], v = raw[slot][4 + run];
-        const bool real = raw[slot][8 + run] != 0.0f;
-        const bool regular = !real || (v >= 9.3e-10f && v <= 1.07e9f && k >= 0.0f);  // 2^-30 .. 2^30
-        float log = -INFINITY, inverse = 0.0f, factor = 1.0f;
-        if (real) {
-          const float size = fabsf(v);
-          log = isfinite(v) ? fmaxf(log2f(size), -100.0f) : 0.0f;
-          inverse = exp2f(-log);
-          factor = !isfinite(v) ? NAN : size < 7.9e-31f ? v * 1.2676506002282294e30f : v < 0.0f ? -1.0f : 1.0f;  // 2^-100, 2^100
-        }
-        const bool odd = __any_sync(0xffffffffu, !regular);
-        if (thread < 4) {
-          Scales& s = scales[stage];
-          s.key[thread] = real ? k : 0.0f;
-          s.log[thread] = log;
-          s.inverse[thread] = inverse;
-          s.factor[thread] = factor;
-          if (thread == 0) s.irregular = odd;
-        }
-        __syncwarp();  // (before lanes 0-3 copy into the slot again)
       }
       tc::fence_async_shared();
       mbar_arrive(full + stage);
@@ -349,7 +373,27 @@ __device__ __forceinline__ bool convert(const SharedPlan& p, const SharedWalk& w
         ++turn;
       }
     }
-    copy(slot);
+    if (next < count) {
+      if (next % kBatch == 0 && ok) ok = wait_warp<false>(sync.batch_full + batch, static_cast<uint32_t>(batch_turn & 1), &sync.abort);
+      const Runs& tile = runs[batch * kBatch + next % kBatch];
+      long long line[kLoads];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) line[i] = tile.line[(row + i * kRows) / 16];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int in = (next_tile * kSharedTile + row + i * kRows) & (c.page - 1);
+        const bool real = ok && line[i] >= 0;
+        copy16(codes_at + slot * SharedShape<SIZE>::kCodeBytes + i * kSetThreads * 16,
+               pool + (real ? (line[i] * c.page + in) * SIZE : 0), real);
+      }
+      ++next;
+      if (++next_tile == w.cut.tiles) next_tile = 0;
+      if (next % kBatch == 0 && ++batch == kBatches) {
+        batch = 0;
+        ++batch_turn;
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
     if (++slot == kAhead) slot = 0;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -358,10 +402,10 @@ __device__ __forceinline__ bool convert(const SharedPlan& p, const SharedWalk& w
 
 // Issues the products of a set over the block's range: a warp, so that what it computes
 // is uniform, and one lane of it.  Both sets take every tile (SETS 2: their own rows)
-// or every other one (1: the same rows).  The scores of two tiles are under way, so
-// that the set weighs one while the other is multiplied.  (While warps take
-// exponentials, a look at a barrier can wait for hundreds of cycles, so there are as
-// few as possible: that a tile's values are there is known from its weights.)
+// or every other one (1: the same rows).  A tile's scores are computed while the set
+// weighs the one before.  (While warps take
+// exponentials, a look at a barrier can wait for hundreds of cycles: those for the
+// tiles come before the one for the weights.)
 template <int SIZE, int SETS, bool LO>
 __device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* keys, const char* values,
                                       const char* queries, SharedSync& sync) {
@@ -378,27 +422,14 @@ __device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* 
     if (!wait_warp(&sync.query_full, static_cast<uint32_t>(segment & 1), abort)) return false;
     tc::fence_after();
 #pragma unroll 1
-    for (int job = -2; job < jobs; ++job) {
-      if (job >= 0) {  // the weighted values of tile `job`
-        const int n = before + (SETS == 2 ? job : 2 * job + set), now = iteration + job, buffer = now & 1;
-        if (!wait_warp(sync.weight_full[set] + buffer, static_cast<uint32_t>(now / 2 & 1), abort)) return false;
-        tc::fence_after();
-        const uint64_t tile = across_desc(values + n % kStages * S::kStageBytes);
-        const uint32_t d = tmem + kValuesAt + set * 128, a = tmem + kScoresAt + (set * 2 + buffer) * kSharedTile;
-        if (leads) {
-#pragma unroll
-          for (int part = 0; part < (LO ? 2 : 1); ++part)
-#pragma unroll
-            for (int k = 0; k < kSharedTile / 16; ++k)
-              multiply(d, a + k * 16 + part * 8, tile + k * 2048 / 16, kValueDesc, job > 0 || part + k > 0);
-          tc::umma_commit(sync.value_done + set);
-          tc::umma_commit(sync.value_free + n % kStages);
-        }
-        __syncwarp();
-      }
-      if (job + 2 < jobs) {  // the scores of the tile after the next
-        const int n = before + (SETS == 2 ? job + 2 : 2 * (job + 2) + set), buffer = (iteration + job) & 1;
-        if (!wait_warp(sync.key_full + n % kStages, static_cast<uint32_t>(n / kStages & 1), abort)) return false;
+    for (int job = -1; job < jobs; ++job) {
+      if (job + 1 < jobs) {  // the scores of the next tile
+        const int n = before + (SETS == 2 ? job + 1 : 2 * (job + 1) + set), buffer = (iteration + job + 1) & 1;
+        // (where the weights of the tile before `job` were: products of another shape
+        // need not follow those in order)
+        if (!wait_warp(sync.key_full + n % kStages, static_cast<uint32_t>(n / kStages & 1), abort) ||
+            (job > 0 && !wait_warp(sync.value_done[set] + buffer, static_cast<uint32_t>((iteration + job - 1) / 2 & 1), abort)))
+          return false;
         tc::fence_after();
         const uint64_t tile = tc::sw128_desc(keys + n % kStages * S::kStageBytes);
         const uint32_t d = tmem + kScoresAt + (set * 2 + buffer) * kSharedTile;
@@ -411,6 +442,25 @@ __device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* 
                               tile + (k / 4 * kChunkBytes + k % 4 * 32) / 16, kScoreDesc, part + k > 0);
           tc::umma_commit(sync.score_full[set] + buffer);
           tc::umma_commit(sync.key_free + n % kStages);
+        }
+        __syncwarp();
+      }
+      if (job >= 0) {  // the weighted values of tile `job`
+        const int n = before + (SETS == 2 ? job : 2 * job + set), now = iteration + job, buffer = now & 1;
+        if (!wait_warp(sync.value_full + n % kStages, static_cast<uint32_t>(n / kStages & 1), abort) ||
+            !wait_warp(sync.weight_full[set] + buffer, static_cast<uint32_t>(now / 2 & 1), abort))
+          return false;
+        tc::fence_after();
+        const uint64_t tile = across_desc(values + n % kStages * S::kStageBytes);
+        const uint32_t d = tmem + kValuesAt + set * 128, a = tmem + kScoresAt + (set * 2 + buffer) * kSharedTile;
+        if (leads) {
+#pragma unroll
+          for (int part = 0; part < (LO ? 2 : 1); ++part)
+#pragma unroll
+            for (int k = 0; k < kSharedTile / 16; ++k)
+              multiply(d, a + k * 16 + part * 8, tile + k * 2048 / 16, kValueDesc, job > 0 || part + k > 0);
+          tc::umma_commit(sync.value_done[set] + buffer);
+          tc::umma_commit(sync.value_free + n % kStages);
         }
         __syncwarp();
       }
@@ -449,7 +499,7 @@ __device__ __forceinline__ void store_weights(uint32_t at, const float* x) {
 
 // A set of 128 rows, a thread each.
 template <int SIZE, int STORAGE, int SETS, bool LO>
-__device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, char* queries, const Scales* scales,
+__device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, char* queries, const Runs* runs,
                                       SharedSync& sync) {
   const int set = threadIdx.x / kSetThreads, r = threadIdx.x % kSetThreads;
   const int local = SETS == 2 ? threadIdx.x : r;
@@ -457,6 +507,17 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
   const uint32_t lanes = sync.tmem + (static_cast<uint32_t>(threadIdx.x / 32 % 4 * 32) << 16);
   const uint32_t sums = lanes + kValuesAt + set * 128;
   const int all_rows = static_cast<int>(p.a.batch) * p.rows;
+  // every warp takes every batch of runs and leaves it, whether it weighs a tile of it or not
+  int batch = -1;
+  auto reach = [&](int n) {  // the batch of the range's tile n
+    while (batch < n / kBatch) {
+      __syncwarp();
+      if (batch >= 0 && (threadIdx.x & 31) == 0) mbar_arrive(sync.batch_free + batch % kBatches);
+      ++batch;
+      if (!wait_warp(sync.batch_full + batch % kBatches, static_cast<uint32_t>(batch / kBatches & 1), abort)) return false;
+    }
+    return true;
+  };
   int iteration = 0, segment = 0, before = 0;
   for (int at = w.begin; at < w.end; ++segment) {
     const int item = at / w.cut.tiles, tiles = min(w.cut.tiles - at % w.cut.tiles, w.end - at);
@@ -473,7 +534,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
         from = b * p.a.q_strides[0] + t * p.a.q_strides[1] + h * p.a.q_strides[2];
       }
       float largest = 0.0f;
-#pragma unroll 2
+#pragma unroll 8
       for (int d = 0; d < SIZE; d += 8) {
         float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         if (real) load_row8(p, from + d, x);
@@ -487,7 +548,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
       if (segment > 0 && !wait_warp(&sync.query_free, static_cast<uint32_t>((segment - 1) & 1), abort)) return false;
       const bool writes = SETS == 2 || LO || set == 0;
       char* to = queries + (SETS == 2 || LO ? set * SharedShape<SIZE>::kQueryBytes : 0);
-#pragma unroll 1
+#pragma unroll 2
       for (int d = 0; writes && d < SIZE; d += 8) {
         uint32_t h[4];
         float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
@@ -509,29 +570,26 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
     float c = 0.0f, l = 0.0f, sum = 0.0f;  // reference, sum of the weights, and of what multiplied the codes
     bool first = true;
     for (int tile = SETS == 2 ? 0 : set; tile < tiles; tile += SETS == 2 ? 1 : 2, ++iteration) {
-      const int n = before + tile, stage = n % kStages;
+      const int n = before + tile;
       const int buffer = iteration & 1;
       const uint32_t scores = lanes + kScoresAt + (set * 2 + buffer) * kSharedTile;
-      if (!wait_warp(sync.value_full + stage, static_cast<uint32_t>(n / kStages & 1), abort) ||
+      if (!reach(n) ||
           !wait_warp(sync.score_full[set] + buffer, static_cast<uint32_t>(iteration / 2 & 1), abort))
         return false;
       tc::fence_after();
       if (any) {
         float s[kSharedTile], by[4], log[4], inverse[4];
-        const Scales& at_stage = scales[stage];
-        const bool irregular = at_stage.irregular != 0;
+        const Runs& tile_runs = runs[batch % kBatches * kBatch + n % kBatch];
+        const bool irregular = tile_runs.irregular != 0;
         float top = -INFINITY;
         if (__builtin_expect(!irregular, 1)) {
-          tc::tmem_load32_nowait(scores, s);
-          tc::tmem_load32_nowait(scores + 32, s + 32);
+          load64(scores, s);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            by[i] = factor * at_stage.key[i];
-            log[i] = at_stage.log[i];
-            inverse[i] = at_stage.inverse[i];
+            by[i] = factor * tile_runs.key[i];
+            log[i] = tile_runs.log[i];
+            inverse[i] = tile_runs.inverse[i];
           }
-          tc::tmem_wait_ld();
-          tc::reg_fence<kSharedTile>(s);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float most = s[16 * i];
@@ -545,7 +603,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
             float x[16];
             tc::tmem_load16(scores + i * 16, x);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) top = fmaxf(top, fmaf(x[k], factor * at_stage.key[i], at_stage.log[i]));
+            for (int k = 0; k < 16; ++k) top = fmaxf(top, fmaf(x[k], factor * tile_runs.key[i], tile_runs.log[i]));
           }
         }
         const bool moves = first || top > c + kRise || top < c - fall_of(LO);
@@ -562,14 +620,13 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
             const float scale = exp2_of(c - now);
             l *= scale;
             sum *= scale;
-            if (!wait_warp(sync.value_done + set, static_cast<uint32_t>((iteration - 1) & 1), abort)) return false;
+            if (!wait_warp(sync.value_done[set] + (buffer ^ 1), static_cast<uint32_t>((iteration - 1) / 2 & 1), abort))
+              return false;
             tc::fence_after();
 #pragma unroll 1
             for (int d = 0; d < SharedShape<SIZE>::kWide; d += 32) {
               float o[32];
-              tc::tmem_load32_nowait(sums + d, o);
-              tc::tmem_wait_ld();
-              tc::reg_fence<32>(o);
+              load32(sums + d, o);
 #pragma unroll
               for (int i = 0; i < 32; i += 8) {
                 uint32_t v[8];
@@ -601,7 +658,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
         } else {  // value scales of any sign and size, or all far below c: the weights by themselves
 #pragma unroll 1
           for (int i = 0; i < 4; ++i) {
-            const float by_i = factor * at_stage.key[i], shift = at_stage.log[i] - c, kept = at_stage.factor[i];
+            const float by_i = factor * tile_runs.key[i], shift = tile_runs.log[i] - c, kept = tile_runs.factor[i];
             float x[16], weights = 0.0f;
             tc::tmem_load16(scores + i * 16, x);
 #pragma unroll
@@ -612,7 +669,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
               sum += x[k];
               x[k] *= kept;
             }
-            if (at_stage.inverse[i] != 0.0f) l += weights;
+            if (tile_runs.inverse[i] != 0.0f) l += weights;
             store_weights<LO>(scores + i * 16, x);
           }
         }
@@ -623,7 +680,8 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
     }
     // the part of this set
     const bool some = SETS == 2 || tiles > set;
-    if (some && !wait_warp(sync.value_done + set, static_cast<uint32_t>((iteration - 1) & 1), abort)) return false;
+    if (some && !wait_warp(sync.value_done[set] + ((iteration - 1) & 1), static_cast<uint32_t>((iteration - 1) / 2 & 1), abort))
+      return false;
     tc::fence_after();
     if (any) {
       const int rows = p.shared.block_rows;
@@ -647,6 +705,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
     }
     at += tiles;
     before += tiles;
+    if (at < w.end && !reach(before)) return false;
   }
   return true;
 }
@@ -656,8 +715,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
   using S = SharedShape<SIZE>;
   extern __shared__ char memory[];
   __shared__ SharedSync sync;
-  __shared__ Scales scales[kStages];
-  __shared__ float raw[kAhead][12];  // scales on their way: of keys, of values, whether there are any
+  __shared__ Runs runs[kBatches * kBatch];
   char* tiles = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(memory) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
@@ -669,14 +727,18 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
       mbar_init(sync.key_free + i, SETS);
       mbar_init(sync.value_free + i, SETS);
     }
+    for (int i = 0; i < kBatches; ++i) {
+      mbar_init(sync.batch_full + i, 32);
+      mbar_init(sync.batch_free + i, 2 * kSetThreads / 32);
+    }
     mbar_init(&sync.query_full, 2 * kSetThreads);
     mbar_init(&sync.query_free, 2);
     for (int i = 0; i < 2; ++i) {
       for (int k = 0; k < 2; ++k) {
         mbar_init(sync.score_full[i] + k, 1);
         mbar_init(sync.weight_full[i] + k, kSetThreads);
+        mbar_init(sync.value_done[i] + k, 1);
       }
-      mbar_init(sync.value_done + i, 1);
     }
     mbar_init(&sync.all_done, 2);
     mbar_fence_init();
@@ -703,13 +765,14 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
     if (warp >= kIssueWarp) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegisters));
       if (warp < kIssueWarp + 2) ok = issue<SIZE, SETS, LO>(w, warp - kIssueWarp, tiles, values, queries, sync);
+      if (warp == kLookWarp) ok = look_up(p, w, runs, sync);
     } else if (warp < kKeyWarp) {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWeighRegisters));
-      ok = weigh<SIZE, STORAGE, SETS, LO>(p, w, queries, scales, sync);
+      ok = weigh<SIZE, STORAGE, SETS, LO>(p, w, queries, runs, sync);
     } else {
       const bool is_value = warp >= kValueWarp;
       ok = convert<SIZE, STORAGE>(p, w, is_value, is_value ? tiles + S::kChunks * kChunkBytes : tiles,
-                                  is_value ? codes + S::kCodeBytes / 2 : codes, scales, raw, sync);
+                                  is_value ? codes + S::kCodeBytes / 2 : codes, runs, sync);
     }
     if (!ok) {
       raise_flag(p.a.error_flag, CB_FLAG_WAIT_DATA);
