@@ -77,15 +77,16 @@ constexpr int kSetThreads = 128;
 // warps 0-7: two sets of rows; 16 and 17 issue theirs; 18 looks up pages and scales
 constexpr int kKeyWarp = 8, kValueWarp = 12, kIssueWarp = 16, kLookWarp = 18;
 constexpr int kSharedThreads = 32 * (kIssueWarp + 4);
-// Registers of a thread: as launched (the converting warps keep them), of the
-// warps that weigh, of the issuing warp and the three beside it (61440 at the
-// launch and after).
-constexpr int kWeighRegisters = 128, kIssueRegisters = 32;
+// Registers of a thread, 96 at the launch: of the warps that weigh, of those that
+// convert, and of the four that issue and look up (61440 of a block, before and after).
+constexpr int kWeighRegisters = 152, kConvertRegisters = 72, kIssueRegisters = 32;
 constexpr int kStages = 3, kAhead = 3;  // tiles as fp16, and tiles whose codes are on their way
 constexpr int kChunkBytes = kSharedTile * 128;  // 64 keys of 64 fp16 elements
-// Columns of the tensor memory: weighted values of both sets, then their scores, two
-// tiles each.  The weights of 16 keys take the place of their scores, high parts first.
-constexpr int kValuesAt = 0, kScoresAt = 256, kColumns = 512;
+// Columns of the tensor memory: weighted values of both sets; then, for each set, the
+// scores of a tile and behind them its weights as fp16: of two tiles by turns, or high
+// and low parts of one, 16 keys of each together.
+constexpr int kValuesAt = 0, kScoresAt = 256, kSetColumns = 128, kWeightsAt = 64, kColumns = 512;
+__host__ __device__ constexpr int weights_at(bool lo, int tile) { return kWeightsAt + (lo ? 0 : (tile & 1) * 32); }
 
 // Of a tile's four runs of 16 keys: the line of each in the pools (page and kv head; -1:
 // none), and its scales, of values as log2, 2^-log2 and what the logarithm leaves.
@@ -176,34 +177,41 @@ __device__ __forceinline__ bool elected() {
   return one != 0;
 }
 
-__device__ __noinline__ void load_row8_scalar(const void* q, long long at, int dtype, float* x) {
-#pragma unroll 1
-  for (int i = 0; i < 8; ++i) x[i] = load_as_f32(q, at + i, dtype);
-}
-// Eight neighbouring elements of a query row.
+// Eight neighbouring elements of a query row: float32 (WIDE), or of 16 bits.
+template <bool WIDE>
 __device__ __forceinline__ void load_row8(const SharedPlan& p, long long at, float* x) {
-  if (!p.wide) {
-    load_row8_scalar(p.a.q, at, p.a.dtype, x);
-  } else if (p.a.dtype == CB_F32) {
-    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p.a.q) + at);
-    const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p.a.q) + at + 4);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  } else {
-    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.a.q) + at);
-    if (p.a.dtype == CB_BF16) {
-      unpack_bf16x8(w, x);
-    } else {
-      const __half2* h = reinterpret_cast<const __half2*>(&w);
+  if (WIDE) {
+    const float* from = static_cast<const float*>(p.a.q) + at;
+    if (p.wide) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[2 * i] = __low2float(h[i]);
-        x[2 * i + 1] = __high2float(h[i]);
+      for (int i = 0; i < 8; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(from + i);
+        x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = from[i];
+    }
+  } else {
+    const uint16_t* from = static_cast<const uint16_t*>(p.a.q) + at;
+    uint32_t w[4];
+    if (p.wide) {
+      const uint4 v = *reinterpret_cast<const uint4*>(from);
+      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = from[2 * i] | static_cast<uint32_t>(from[2 * i + 1]) << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = *reinterpret_cast<const __half2*>(w + i);
+      const bool brain = p.a.dtype == CB_BF16;
+      x[2 * i] = brain ? __uint_as_float(w[i] << 16) : __low2float(h);
+      x[2 * i + 1] = brain ? __uint_as_float(w[i] & 0xffff0000u) : __high2float(h);
     }
   }
 }
-// 8, 32 and 64 float32 columns of this thread's lane of the tensor memory (warp-wide).
+// 8 and 32 float32 columns of this thread's lane of the tensor memory (warp-wide).
 // The load and the wait for it are one statement: between two, the compiler could
 // move registers that are not written yet.
 __device__ __forceinline__ void load8(uint32_t at, float* out) {
@@ -234,28 +242,6 @@ __device__ __forceinline__ void load32(uint32_t at, float* out) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) out[i] = __uint_as_float(v[i]);
 }
-__device__ __forceinline__ void load64(uint32_t at, float* out) {
-  uint32_t v[64];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
-      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
-      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, "
-      "%40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, "
-      "%59, %60, %61, %62, %63"
-      "}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]),
-        "=r"(v[32]), "=r"(v[33]), "=r"(v[34]), "=r"(v[35]), "=r"(v[36]), "=r"(v[37]), "=r"(v[38]), "=r"(v[39]),
-        "=r"(v[40]), "=r"(v[41]), "=r"(v[42]), "=r"(v[43]), "=r"(v[44]), "=r"(v[45]), "=r"(v[46]), "=r"(v[47]),
-        "=r"(v[48]), "=r"(v[49]), "=r"(v[50]), "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]),
-        "=r"(v[56]), "=r"(v[57]), "=r"(v[58]), "=r"(v[59]), "=r"(v[60]), "=r"(v[61]), "=r"(v[62]), "=r"(v[63])
-      : "r"(at)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 64; ++i) out[i] = __uint_as_float(v[i]);
-}
 
 // What a role of the block walks: its range of units, item by item.
 struct SharedWalk {
@@ -268,7 +254,8 @@ struct SharedWalk {
 struct SharedSync {
   uint64_t key_full[kStages], key_free[kStages], value_full[kStages], value_free[kStages];
   uint64_t batch_full[kBatches], batch_free[kBatches], query_full, query_free, all_done;
-  uint64_t score_full[2][2], weight_full[2][2], value_done[2][2];  // [set][tile % 2]: no two phases are open at once
+  uint64_t score_full[2], score_free[2];
+  uint64_t weight_full[2][2], value_done[2][2];  // [set][tile % 2]: a set is up to two tiles ahead of its products
   uint32_t tmem;
   int abort, found;
 };
@@ -402,8 +389,8 @@ __device__ __forceinline__ bool convert(const SharedPlan& p, const SharedWalk& w
 
 // Issues the products of a set over the block's range: a warp, so that what it computes
 // is uniform, and one lane of it.  Both sets take every tile (SETS 2: their own rows)
-// or every other one (1: the same rows).  A tile's scores are computed while the set
-// weighs the one before.  (While warps take
+// or every other one (1: the same rows).  A tile's scores are computed as soon as those
+// of the one before are in registers, while the set weighs it.  (While warps take
 // exponentials, a look at a barrier can wait for hundreds of cycles: those for the
 // tiles come before the one for the weights.)
 template <int SIZE, int SETS, bool LO>
@@ -424,15 +411,13 @@ __device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* 
 #pragma unroll 1
     for (int job = -1; job < jobs; ++job) {
       if (job + 1 < jobs) {  // the scores of the next tile
-        const int n = before + (SETS == 2 ? job + 1 : 2 * (job + 1) + set), buffer = (iteration + job + 1) & 1;
-        // (where the weights of the tile before `job` were: products of another shape
-        // need not follow those in order)
+        const int n = before + (SETS == 2 ? job + 1 : 2 * (job + 1) + set), now = iteration + job + 1;
         if (!wait_warp(sync.key_full + n % kStages, static_cast<uint32_t>(n / kStages & 1), abort) ||
-            (job > 0 && !wait_warp(sync.value_done[set] + buffer, static_cast<uint32_t>((iteration + job - 1) / 2 & 1), abort)))
+            (now > 0 && !wait_warp(sync.score_free + set, static_cast<uint32_t>((now - 1) & 1), abort)))
           return false;
         tc::fence_after();
         const uint64_t tile = tc::sw128_desc(keys + n % kStages * S::kStageBytes);
-        const uint32_t d = tmem + kScoresAt + (set * 2 + buffer) * kSharedTile;
+        const uint32_t d = tmem + kScoresAt + set * kSetColumns;
         if (leads) {
 #pragma unroll
           for (int part = 0; part < (LO ? 2 : 1); ++part)
@@ -440,7 +425,7 @@ __device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* 
             for (int k = 0; k < SIZE / 16; ++k)
               multiply_shared(d, query + (part * S::kQueryBytes + k / 4 * kRowLanes * 128 + k % 4 * 32) / 16,
                               tile + (k / 4 * kChunkBytes + k % 4 * 32) / 16, kScoreDesc, part + k > 0);
-          tc::umma_commit(sync.score_full[set] + buffer);
+          tc::umma_commit(sync.score_full + set);
           tc::umma_commit(sync.key_free + n % kStages);
         }
         __syncwarp();
@@ -452,13 +437,13 @@ __device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* 
           return false;
         tc::fence_after();
         const uint64_t tile = across_desc(values + n % kStages * S::kStageBytes);
-        const uint32_t d = tmem + kValuesAt + set * 128, a = tmem + kScoresAt + (set * 2 + buffer) * kSharedTile;
+        const uint32_t d = tmem + kValuesAt + set * 128, a = tmem + kScoresAt + set * kSetColumns + weights_at(LO, now);
         if (leads) {
 #pragma unroll
           for (int part = 0; part < (LO ? 2 : 1); ++part)
 #pragma unroll
             for (int k = 0; k < kSharedTile / 16; ++k)
-              multiply(d, a + k * 16 + part * 8, tile + k * 2048 / 16, kValueDesc, job > 0 || part + k > 0);
+              multiply(d, a + k * (LO ? 16 : 8) + part * 8, tile + k * 2048 / 16, kValueDesc, job > 0 || part + k > 0);
           tc::umma_commit(sync.value_done[set] + buffer);
           tc::umma_commit(sync.value_free + n % kStages);
         }
@@ -483,6 +468,69 @@ __device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* 
 constexpr float kRise = 15.0f, kRest = 2.0f, kFarBelow = 60.0f, kHeld = 1.2676506002282294e30f;  // 2^100
 __host__ __device__ constexpr float fall_of(bool lo) { return lo ? 2.0f : 15.0f; }
 
+// Two float32 numbers in a 64-bit register, for the instructions that take both.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void split_pair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+// x = 2^(x * by + shift) of 16 numbers, and their sum.  Half of them for 16-bit
+// outputs are computed on the multiply-add units (the special function unit would take
+// 512 cycles for a warp's tile, and two warps share it): 2^e = 2^n 2^f with n the
+// nearest whole number to e (added to 1.5 * 2^23, whose low bits it becomes), and 2^f,
+// |f| <= 1/2, by its Taylor polynomial of degree 5: (f ln 2)^6 / 720 < 2.5e-6, a
+// hundredth of the weights' rounding to 11 bits.
+template <bool LO>
+__device__ __forceinline__ float exponentials(float* x, float by, float shift) {
+  const uint64_t by2 = pair_of(by, by), shift2 = pair_of(shift, shift);
+  uint64_t run[2] = {0, 0};
+  constexpr float kMagic = 12582912.0f, kLn2 = 0.6931471805599453f;
+  const uint64_t magic = pair_of(kMagic, kMagic), back = pair_of(-kMagic, -kMagic), minus = pair_of(-1.0f, -1.0f);
+#pragma unroll
+  for (int k = 0; k < 16; k += 2) {
+    uint64_t e = fma2(pair_of(x[k], x[k + 1]), by2, shift2);
+    float a, b;
+    split_pair(e, a, b);
+    if (LO || k % 4 == 0) {
+      x[k] = exp2_of(a);
+      x[k + 1] = exp2_of(b);
+    } else {
+      asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(a));  // -126
+      asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(b));
+      e = pair_of(a, b);
+      const uint64_t n = add2(e, magic), f = fma2(add2(n, back), minus, e);
+      constexpr float c1 = kLn2, c2 = kLn2 * kLn2 / 2, c3 = c2 * kLn2 / 3, c4 = c3 * kLn2 / 4, c5 = c4 * kLn2 / 5;
+      uint64_t y = fma2(pair_of(c5, c5), f, pair_of(c4, c4));
+      y = fma2(y, f, pair_of(c3, c3));
+      y = fma2(y, f, pair_of(c2, c2));
+      y = fma2(y, f, pair_of(c1, c1));
+      y = fma2(y, f, pair_of(1.0f, 1.0f));
+      float n0, n1;
+      split_pair(n, n0, n1);
+      split_pair(y, a, b);
+      x[k] = __uint_as_float(__float_as_uint(a) + (__float_as_uint(n0) << 23));
+      x[k + 1] = __uint_as_float(__float_as_uint(b) + (__float_as_uint(n1) << 23));
+    }
+    run[k / 2 & 1] = add2(run[k / 2 & 1], pair_of(x[k], x[k + 1]));
+  }
+  float a, b;
+  split_pair(add2(run[0], run[1]), a, b);
+  return a + b;
+}
+
 // Sixteen weights as fp16, and what is left of them.
 template <bool LO>
 __device__ __forceinline__ void store_weights(uint32_t at, const float* x) {
@@ -499,13 +547,13 @@ __device__ __forceinline__ void store_weights(uint32_t at, const float* x) {
 
 // A set of 128 rows, a thread each.
 template <int SIZE, int STORAGE, int SETS, bool LO>
-__device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, char* queries, const Runs* runs,
-                                      SharedSync& sync) {
+__device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, char* queries, float* factors, long long* offsets,
+                                      const Runs* runs, SharedSync& sync) {
   const int set = threadIdx.x / kSetThreads, r = threadIdx.x % kSetThreads;
   const int local = SETS == 2 ? threadIdx.x : r;
   volatile int* abort = &sync.abort;
   const uint32_t lanes = sync.tmem + (static_cast<uint32_t>(threadIdx.x / 32 % 4 * 32) << 16);
-  const uint32_t sums = lanes + kValuesAt + set * 128;
+  const uint32_t sums = lanes + kValuesAt + set * 128, scores = lanes + kScoresAt + set * kSetColumns;
   const int all_rows = static_cast<int>(p.a.batch) * p.rows;
   // every warp takes every batch of runs and leaves it, whether it weighs a tile of it or not
   int batch = -1;
@@ -525,34 +573,38 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
     const int row = item % w.blocks * p.shared.block_rows + local;
     const bool real = row < all_rows, any = __any_sync(0xffffffffu, real);  // (rows of no warp are skipped)
 
-    // the row's queries, scaled to below 2, in the order of the codes' halves
-    float factor;
+    // the warp's rows of queries, SIZE / 8 lanes to a row, scaled to below 2, in the
+    // order of the codes' halves
+    long long from = -1;
+    if (real) {
+      const int b = row / p.rows, t = row % p.rows / p.group, h = head * p.group + row % p.group;
+      from = b * p.a.q_strides[0] + t * p.a.q_strides[1] + h * p.a.q_strides[2];
+    }
+    offsets[threadIdx.x] = from;
+    __syncwarp();
+    if (segment > 0 && !wait_warp(&sync.query_free, static_cast<uint32_t>((segment - 1) & 1), abort)) return false;
     {
-      long long from = 0;
-      if (real) {
-        const int b = row / p.rows, t = row % p.rows / p.group, h = head * p.group + row % p.group;
-        from = b * p.a.q_strides[0] + t * p.a.q_strides[1] + h * p.a.q_strides[2];
-      }
-      float largest = 0.0f;
-#pragma unroll 8
-      for (int d = 0; d < SIZE; d += 8) {
-        float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (real) load_row8(p, from + d, x);
+      constexpr int kLanes = SIZE / 8;
+      const int lane = threadIdx.x & 31, d = lane % kLanes * 8;
+      const bool writes = SETS == 2 || LO || set == 0;
+      char* to = queries + (SETS == 2 || LO ? set * SharedShape<SIZE>::kQueryBytes : 0) + d / 64 * kRowLanes * 128;
+#pragma unroll 4
+      for (int step = 0; step < kLanes; ++step) {
+        const int from_lane = step * (32 / kLanes) + lane / kLanes;
+        const long long at_row = offsets[threadIdx.x / 32 * 32 + from_lane];
+        const bool there = at_row >= 0;
+        float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, largest = 0.0f;
+        if (there) load_row8<LO>(p, at_row + d, x);
 #pragma unroll
         for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(x[i]));
-      }
-      const int e = min(max(static_cast<int>(__float_as_uint(largest) >> 23) - 127, -126), 127);
-      const float down = e == 127 ? 5.877471754111438e-39f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      const float sign = p.a.scale < 0.0f ? -down : down;
-      factor = fabsf(p.a.scale) * 1.4426950408889634f * power2(e);
-      if (segment > 0 && !wait_warp(&sync.query_free, static_cast<uint32_t>((segment - 1) & 1), abort)) return false;
-      const bool writes = SETS == 2 || LO || set == 0;
-      char* to = queries + (SETS == 2 || LO ? set * SharedShape<SIZE>::kQueryBytes : 0);
-#pragma unroll 2
-      for (int d = 0; writes && d < SIZE; d += 8) {
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+        const int e = min(max(static_cast<int>(__float_as_uint(largest) >> 23) - 127, -126), 127);
+        const float down = e == 127 ? 5.877471754111438e-39f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        const float sign = p.a.scale < 0.0f ? -down : down;
+        const int local_row = threadIdx.x % kSetThreads / 32 * 32 + from_lane;
+        if (d == 0) factors[set * kSetThreads + local_row] = fabsf(p.a.scale) * 1.4426950408889634f * power2(e);
         uint32_t h[4];
-        float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (real) load_row8(p, from + d, x);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int first = STORAGE == CB_I8 ? i / 2 * 4 + i % 2 : 2 * i, second = STORAGE == CB_I8 ? first + 2 : first + 1;
@@ -560,30 +612,43 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
           const __half2 hi = __floats2half2_rn(a, b);
           h[i] = LO && set == 1 ? bits(__floats2half2_rn(a - __low2float(hi), b - __high2float(hi))) : bits(hi);
         }
-        *reinterpret_cast<uint4*>(to + d / 64 * kRowLanes * 128 + tc::swizzle_offset(r, d % 64 / 8)) =
-            make_uint4(h[0], h[1], h[2], h[3]);
+        if (writes)
+          *reinterpret_cast<uint4*>(to + tc::swizzle_offset(local_row, d % 64 / 8)) = make_uint4(h[0], h[1], h[2], h[3]);
       }
       tc::fence_async_shared();
       mbar_arrive(&sync.query_full);
+      __syncwarp();
     }
+    const float factor = factors[threadIdx.x];
 
     float c = 0.0f, l = 0.0f, sum = 0.0f;  // reference, sum of the weights, and of what multiplied the codes
     bool first = true;
     for (int tile = SETS == 2 ? 0 : set; tile < tiles; tile += SETS == 2 ? 1 : 2, ++iteration) {
       const int n = before + tile;
       const int buffer = iteration & 1;
-      const uint32_t scores = lanes + kScoresAt + (set * 2 + buffer) * kSharedTile;
+      const uint32_t weights = scores + weights_at(LO, iteration);
       if (!reach(n) ||
-          !wait_warp(sync.score_full[set] + buffer, static_cast<uint32_t>(iteration / 2 & 1), abort))
+          !wait_warp(sync.score_full + set, static_cast<uint32_t>(iteration & 1), abort))
         return false;
       tc::fence_after();
+      auto leave_scores = [&] {  // they are read: the next tile's may take their place
+        tc::fence_before();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(sync.score_free + set);
+      };
+      // (low parts leave no room for the weights of two tiles)
+      if (LO && iteration > 0 &&
+          !wait_warp(sync.value_done[set] + (buffer ^ 1), static_cast<uint32_t>((iteration - 1) / 2 & 1), abort))
+        return false;
+      if (!any) leave_scores();
       if (any) {
         float s[kSharedTile], by[4], log[4], inverse[4];
         const Runs& tile_runs = runs[batch % kBatches * kBatch + n % kBatch];
         const bool irregular = tile_runs.irregular != 0;
         float top = -INFINITY;
         if (__builtin_expect(!irregular, 1)) {
-          load64(scores, s);
+          load32(scores, s);
+          load32(scores + 32, s + 32);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             by[i] = factor * tile_runs.key[i];
@@ -640,38 +705,32 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
         }
         first = false;
         if (__builtin_expect(!irregular && !__any_sync(0xffffffffu, top < c - kFarBelow), 1)) {
+          leave_scores();
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float* x = s + 16 * i;
-            const float shift = log[i] - c;
-            float run[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              x[k] = exp2_of(fmaf(x[k], by[i], shift));
-              run[k & 3] += x[k];
-            }
-            const float all = (run[0] + run[1]) + (run[2] + run[3]);
+            const float all = exponentials<LO>(s + 16 * i, by[i], log[i] - c);
             l = fmaf(all, inverse[i], l);
             sum += all;
-            store_weights<LO>(scores + i * 16, x);
+            store_weights<LO>(weights + i * (LO ? 16 : 8), s + 16 * i);
           }
         } else {  // value scales of any sign and size, or all far below c: the weights by themselves
 #pragma unroll 1
           for (int i = 0; i < 4; ++i) {
             const float by_i = factor * tile_runs.key[i], shift = tile_runs.log[i] - c, kept = tile_runs.factor[i];
-            float x[16], weights = 0.0f;
+            float x[16], all = 0.0f;
             tc::tmem_load16(scores + i * 16, x);
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               const float score = x[k] * by_i;
-              weights += exp2_of(score - c);
+              all += exp2_of(score - c);
               x[k] = exp2_of(score + shift);
               sum += x[k];
               x[k] *= kept;
             }
-            if (tile_runs.inverse[i] != 0.0f) l += weights;
-            store_weights<LO>(scores + i * 16, x);
+            if (tile_runs.inverse[i] != 0.0f) l += all;
+            store_weights<LO>(weights + i * (LO ? 16 : 8), x);
           }
+          leave_scores();
         }
         tc::tmem_wait_st();
       }
@@ -716,6 +775,8 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
   extern __shared__ char memory[];
   __shared__ SharedSync sync;
   __shared__ Runs runs[kBatches * kBatch];
+  __shared__ float factors[2 * kSetThreads];  // what turns a row's products into scores in base 2
+  __shared__ long long offsets[2 * kSetThreads];  // of the rows' queries, -1: none
   char* tiles = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(memory) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
@@ -734,8 +795,9 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
     mbar_init(&sync.query_full, 2 * kSetThreads);
     mbar_init(&sync.query_free, 2);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(sync.score_full + i, 1);
+      mbar_init(sync.score_free + i, kSetThreads / 32);
       for (int k = 0; k < 2; ++k) {
-        mbar_init(sync.score_full[i] + k, 1);
         mbar_init(sync.weight_full[i] + k, kSetThreads);
         mbar_init(sync.value_done[i] + k, 1);
       }
@@ -768,9 +830,10 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
       if (warp == kLookWarp) ok = look_up(p, w, runs, sync);
     } else if (warp < kKeyWarp) {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWeighRegisters));
-      ok = weigh<SIZE, STORAGE, SETS, LO>(p, w, queries, runs, sync);
+      ok = weigh<SIZE, STORAGE, SETS, LO>(p, w, queries, factors, offsets, runs, sync);
     } else {
       const bool is_value = warp >= kValueWarp;
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegisters));
       ok = convert<SIZE, STORAGE>(p, w, is_value, is_value ? tiles + S::kChunks * kChunkBytes : tiles,
                                   is_value ? codes + S::kCodeBytes / 2 : codes, runs, sync);
     }
