@@ -74,9 +74,10 @@ struct SharedPlan {
 
 constexpr int kRowLanes = 128;  // rows of a product: lanes of the tensor memory
 constexpr int kSetThreads = 128;
-// warps 0-7: two sets of rows; 16 and 17 issue theirs; 18 looks up pages and scales
-constexpr int kKeyWarp = 8, kValueWarp = 12, kIssueWarp = 16, kLookWarp = 18;
-constexpr int kSharedThreads = 32 * (kIssueWarp + 4);
+// Warps 0 and 1 issue the products of the two sets of rows, 2 looks up pages and scales:
+// first, since a scheduler prefers its older warps, and these wait most and do least.
+constexpr int kIssueWarp = 0, kLookWarp = 2, kWeighWarp = 4, kKeyWarp = 12, kValueWarp = 16;
+constexpr int kSharedThreads = 32 * (kValueWarp + 4);
 // Registers of a thread, 96 at the launch: of the warps that weigh, of those that
 // convert, and of the four that issue and look up (61440 of a block, before and after).
 constexpr int kWeighRegisters = 152, kConvertRegisters = 72, kIssueRegisters = 32;
@@ -549,10 +550,10 @@ __device__ __forceinline__ void store_weights(uint32_t at, const float* x) {
 template <int SIZE, int STORAGE, int SETS, bool LO>
 __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, char* queries, float* factors, long long* offsets,
                                       const Runs* runs, SharedSync& sync) {
-  const int set = threadIdx.x / kSetThreads, r = threadIdx.x % kSetThreads;
-  const int local = SETS == 2 ? threadIdx.x : r;
+  const int thread = threadIdx.x - 32 * kWeighWarp, set = thread / kSetThreads, r = thread % kSetThreads;
+  const int local = SETS == 2 ? thread : r;
   volatile int* abort = &sync.abort;
-  const uint32_t lanes = sync.tmem + (static_cast<uint32_t>(threadIdx.x / 32 % 4 * 32) << 16);
+  const uint32_t lanes = sync.tmem + (static_cast<uint32_t>(r / 32 * 32) << 16);
   const uint32_t sums = lanes + kValuesAt + set * 128, scores = lanes + kScoresAt + set * kSetColumns;
   const int all_rows = static_cast<int>(p.a.batch) * p.rows;
   // every warp takes every batch of runs and leaves it, whether it weighs a tile of it or not
@@ -580,7 +581,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
       const int b = row / p.rows, t = row % p.rows / p.group, h = head * p.group + row % p.group;
       from = b * p.a.q_strides[0] + t * p.a.q_strides[1] + h * p.a.q_strides[2];
     }
-    offsets[threadIdx.x] = from;
+    offsets[thread] = from;
     __syncwarp();
     if (segment > 0 && !wait_warp(&sync.query_free, static_cast<uint32_t>((segment - 1) & 1), abort)) return false;
     {
@@ -591,7 +592,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
 #pragma unroll 4
       for (int step = 0; step < kLanes; ++step) {
         const int from_lane = step * (32 / kLanes) + lane / kLanes;
-        const long long at_row = offsets[threadIdx.x / 32 * 32 + from_lane];
+        const long long at_row = offsets[thread / 32 * 32 + from_lane];
         const bool there = at_row >= 0;
         float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, largest = 0.0f;
         if (there) load_row8<LO>(p, at_row + d, x);
@@ -602,7 +603,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
         const int e = min(max(static_cast<int>(__float_as_uint(largest) >> 23) - 127, -126), 127);
         const float down = e == 127 ? 5.877471754111438e-39f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
         const float sign = p.a.scale < 0.0f ? -down : down;
-        const int local_row = threadIdx.x % kSetThreads / 32 * 32 + from_lane;
+        const int local_row = r / 32 * 32 + from_lane;
         if (d == 0) factors[set * kSetThreads + local_row] = fabsf(p.a.scale) * 1.4426950408889634f * power2(e);
         uint32_t h[4];
 #pragma unroll
@@ -619,7 +620,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
       mbar_arrive(&sync.query_full);
       __syncwarp();
     }
-    const float factor = factors[threadIdx.x];
+    const float factor = factors[thread];
 
     float c = 0.0f, l = 0.0f, sum = 0.0f;  // reference, sum of the weights, and of what multiplied the codes
     bool first = true;
@@ -824,7 +825,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
   char* codes = queries + 2 * S::kQueryBytes;
   bool ok = true;
   if (w.begin < w.end) {
-    if (warp >= kIssueWarp) {
+    if (warp < kWeighWarp) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegisters));
       if (warp < kIssueWarp + 2) ok = issue<SIZE, SETS, LO>(w, warp - kIssueWarp, tiles, values, queries, sync);
       if (warp == kLookWarp) ok = look_up(p, w, runs, sync);
