@@ -13,15 +13,15 @@ namespace cb {
 // The first keys of all sequences of a call, computed apart (paged_shared.cu).
 // `common`: for each sequence the whole pages that it has in common with the
 // call's first; INT_MAX where it takes no part.  The rows of a kv head, those
-// of all sequences, go in blocks of `block_rows`, and the keys of all (kv head,
-// block of rows) in tiles of kSharedTile are cut into equal ranges.  Range c's
-// part of item i is parts (i + c) * ways .. + ways - 1: references of block_rows
-// rows, their sums, then the rows' elements (see shared_at).
+// of all sequences, go in blocks of `block_rows`; an item is a kv head and a block
+// of rows, and its keys, in tiles of kSharedTile, are cut into `splits` pieces (see
+// shared_cut).  Piece s of item i is parts (i * splits + s) * ways .. + ways - 1:
+// references of block_rows rows, their sums, then the rows' elements (see shared_at).
 constexpr int kSharedTile = 64;
 struct SharedKeys {
   const int* common;  // and behind them the slot of the first sequence that takes part
   const float* parts;
-  int block_rows, ways, ranges, least;  // tiles of a range: `least` or more
+  int block_rows, ways, blocks, least;  // blocks of the grid; tiles of a piece: `least` or more, or all
 };
 // Of element d of row r behind a part's references and sums: eight neighbouring
 // elements of a row together, so that the rows that write them and the elements that
@@ -136,14 +136,18 @@ __device__ __forceinline__ int common_pages(const SharedKeys& shared, long long 
   __syncthreads();
   return *found == INT_MAX ? 0 : *found;
 }
-// The division of the shared keys: tiles of an item, and of a range.
+// The division of the shared keys: tiles of an item and of a piece, pieces of an item.
+// No block takes pieces of two items while there are more blocks than items, since
+// beginning and ending one takes as long as several tiles.
 struct SharedCut {
-  int tiles, per;
+  int tiles, per, splits;
 };
 __device__ __forceinline__ SharedCut shared_cut(const SharedKeys& s, int items, int keys) {
   SharedCut cut;
   cut.tiles = (keys + kSharedTile - 1) / kSharedTile;
-  cut.per = max(s.least, (items * cut.tiles + s.ranges - 1) / s.ranges);
+  const int splits = max(1, min(s.blocks / items, (cut.tiles + s.least - 1) / s.least));
+  cut.per = (cut.tiles + splits - 1) / splits;
+  cut.splits = cut.per > 0 ? (cut.tiles + cut.per - 1) / cut.per : 1;
   return cut;
 }
 
@@ -376,10 +380,9 @@ __device__ __noinline__ void add_shared(const Plan& p, int pages, long long row,
   const int blocks = static_cast<int>((p.a.batch * p.rows + s.block_rows - 1) / s.block_rows);
   const SharedCut cut = shared_cut(s, p.a.cache.kv_heads * blocks, pages * p.a.cache.page);
   const int item = head * blocks + static_cast<int>(row / s.block_rows), r = static_cast<int>(row % s.block_rows);
-  const int from = item * cut.tiles / cut.per, last = ((item + 1) * cut.tiles - 1) / cut.per;
   const long long floats = static_cast<long long>(s.block_rows) * (SIZE + 2);
-  const float* parts = s.parts + static_cast<long long>(item + from) * s.ways * floats;
-  const int count = (last - from + 1) * s.ways;
+  const float* parts = s.parts + static_cast<long long>(item) * cut.splits * s.ways * floats;
+  const int count = cut.splits * s.ways;
   float top = *top_, sum = *sum_;
   constexpr int kBatch = 8;  // parts whose loads are in flight together
   for (int at = 0; at < count; at += kBatch) {

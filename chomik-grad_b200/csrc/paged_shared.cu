@@ -244,9 +244,9 @@ __device__ __forceinline__ void load32(uint32_t at, float* out) {
   for (int i = 0; i < 32; ++i) out[i] = __uint_as_float(v[i]);
 }
 
-// What a role of the block walks: its range of units, item by item.
+// What the roles of a block walk: `count` tiles from tile `first` of each of its items.
 struct SharedWalk {
-  int blocks, keys, range, begin, end;
+  int blocks, keys, item, step, items, first, tiles, count;  // step: to the block's next item; count: of all its tiles
   SharedCut cut;
   const int* table;
 };
@@ -268,11 +268,11 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real)
 // Looks up the runs of the range's tiles.
 __device__ __forceinline__ bool look_up(const SharedPlan& p, const SharedWalk& w, Runs* runs, SharedSync& sync) {
   const cb_paged_cache& c = p.a.cache;
-  const int lane = threadIdx.x & 31, run = lane & 3, count = w.end - w.begin, shift = 31 - __clz(c.page);
+  const int lane = threadIdx.x & 31, run = lane & 3, count = w.count, shift = 31 - __clz(c.page);
 #pragma unroll 1
   for (int batch = 0; batch * kBatch < count; ++batch) {
-    const int n = batch * kBatch + lane / 4, at = w.begin + n, key = at % w.cut.tiles * kSharedTile + run * 16;
-    const int head = at / w.cut.tiles / w.blocks, slot = batch % kBatches;
+    const int n = batch * kBatch + lane / 4, key = (w.first + n % w.tiles) * kSharedTile + run * 16;
+    const int head = (w.item + n / w.tiles * w.step) / w.blocks, slot = batch % kBatches;
     long long line = -1;
     if (n < count && key < w.keys) {
       const int page = __ldg(w.table + (key >> shift));
@@ -315,7 +315,7 @@ __device__ __forceinline__ bool convert(const SharedPlan& p, const SharedWalk& w
   constexpr int kPieces = SIZE / 16, kLoads = kSharedTile * kPieces / kSetThreads, kRows = kSetThreads / kPieces;
   const cb_paged_cache& c = p.a.cache;
   const int thread = threadIdx.x % kSetThreads, piece = thread % kPieces, row = thread / kPieces;
-  const int count = w.end - w.begin;
+  const int count = w.count;
   const char* pool = static_cast<const char*>(values ? c.v_pages : c.k_pages) + piece * 16;
   const uint32_t codes_at = smem_addr(codes) + thread * 16;
   if (values && SIZE == 32) {  // the columns that no element has
@@ -327,7 +327,7 @@ __device__ __forceinline__ bool convert(const SharedPlan& p, const SharedWalk& w
   uint64_t* const full = values ? sync.value_full : sync.key_full;
   bool ok = true;
   int stage = 0, turn = 0, slot = 0;
-  int next = 0, next_tile = w.begin % w.cut.tiles, batch = 0, batch_turn = 0;  // what is copied next
+  int next = 0, next_tile = 0, batch = 0, batch_turn = 0;  // what is copied next
 #pragma unroll 1
   for (int n = -kAhead; n < count; ++n) {
     if (n >= 0) {
@@ -369,13 +369,13 @@ __device__ __forceinline__ bool convert(const SharedPlan& p, const SharedWalk& w
       for (int i = 0; i < kLoads; ++i) line[i] = tile.line[(row + i * kRows) / 16];
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int in = (next_tile * kSharedTile + row + i * kRows) & (c.page - 1);
+        const int in = ((w.first + next_tile) * kSharedTile + row + i * kRows) & (c.page - 1);
         const bool real = ok && line[i] >= 0;
         copy16(codes_at + slot * SharedShape<SIZE>::kCodeBytes + i * kSetThreads * 16,
                pool + (real ? (line[i] * c.page + in) * SIZE : 0), real);
       }
       ++next;
-      if (++next_tile == w.cut.tiles) next_tile = 0;
+      if (++next_tile == w.tiles) next_tile = 0;
       if (next % kBatch == 0 && ++batch == kBatches) {
         batch = 0;
         ++batch_turn;
@@ -405,8 +405,8 @@ __device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* 
   const uint64_t query = tc::sw128_desc(queries + (SETS == 2 ? set * S::kQueryBytes : 0));
   int iteration = 0, segment = 0, before = 0;  // tiles of the set; tiles before the segment
 #pragma unroll 1
-  for (int at = w.begin; at < w.end; ++segment) {
-    const int tiles = min(w.cut.tiles - at % w.cut.tiles, w.end - at), jobs = SETS == 2 ? tiles : (tiles - set + 1) / 2;
+  for (int item = w.item; item < w.items; item += w.step, ++segment) {
+    const int jobs = SETS == 2 ? w.tiles : (w.tiles - set + 1) / 2;
     if (!wait_warp(&sync.query_full, static_cast<uint32_t>(segment & 1), abort)) return false;
     tc::fence_after();
 #pragma unroll 1
@@ -454,8 +454,7 @@ __device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* 
     if (leads) tc::umma_commit(&sync.query_free);
     __syncwarp();
     iteration += jobs;
-    at += tiles;
-    before += tiles;
+    before += w.tiles;
   }
   return true;
 }
@@ -568,9 +567,9 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
     return true;
   };
   int iteration = 0, segment = 0, before = 0;
-  for (int at = w.begin; at < w.end; ++segment) {
-    const int item = at / w.cut.tiles, tiles = min(w.cut.tiles - at % w.cut.tiles, w.end - at);
-    const int head = item / w.blocks;
+#pragma unroll 1
+  for (int item = w.item; item < w.items; item += w.step, ++segment) {
+    const int tiles = w.tiles, head = item / w.blocks;
     const int row = item % w.blocks * p.shared.block_rows + local;
     const bool real = row < all_rows, any = __any_sync(0xffffffffu, real);  // (rows of no warp are skipped)
 
@@ -589,7 +588,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
       const int lane = threadIdx.x & 31, d = lane % kLanes * 8;
       const bool writes = SETS == 2 || LO || set == 0;
       char* to = queries + (SETS == 2 || LO ? set * SharedShape<SIZE>::kQueryBytes : 0) + d / 64 * kRowLanes * 128;
-#pragma unroll 4
+#pragma unroll 8
       for (int step = 0; step < kLanes; ++step) {
         const int from_lane = step * (32 / kLanes) + lane / kLanes;
         const long long at_row = offsets[thread / 32 * 32 + from_lane];
@@ -745,27 +744,35 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
     tc::fence_after();
     if (any) {
       const int rows = p.shared.block_rows;
-      float* part = p.parts + ((item + w.range) * static_cast<long long>(p.shared.ways) + (SETS == 2 ? 0 : set)) * rows * (SIZE + 2);
+      const long long piece = static_cast<long long>(item) * w.cut.splits + w.first / w.cut.per;
+      float* part = p.parts + (piece * p.shared.ways + (SETS == 2 ? 0 : set)) * rows * (SIZE + 2);
       if (real) {
         part[local] = some ? c : -INFINITY;
         part[rows + local] = l;
       }
 #pragma unroll 1
-      for (int d = 0; d < SIZE; d += 8) {
-        float o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (some) load8(sums + d, o);
+      for (int d = 0; d < SIZE; d += 32) {
+        float o[32];
+        if (some) {
+          load32(sums + d, o);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+        }
         if (real) {
-          float4* to = reinterpret_cast<float4*>(part + 2 * rows + shared_at(rows, local, d));
-          constexpr int b = STORAGE == CB_I8 ? 2 : 1, e = STORAGE == CB_I8 ? 1 : 2;  // (the order of the codes' halves)
-          to[0] = make_float4(o[0], o[b], o[e], o[3]);
-          to[1] = make_float4(o[4], o[4 + b], o[4 + e], o[7]);
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            float4* to = reinterpret_cast<float4*>(part + 2 * rows + shared_at(rows, local, d + i));
+            constexpr int b = STORAGE == CB_I8 ? 2 : 1, e = STORAGE == CB_I8 ? 1 : 2;  // (the order of the codes' halves)
+            to[0] = make_float4(o[i], o[i + b], o[i + e], o[i + 3]);
+            to[1] = make_float4(o[i + 4], o[i + 4 + b], o[i + 4 + e], o[i + 7]);
+          }
         }
       }
       tc::fence_before();
     }
-    at += tiles;
     before += tiles;
-    if (at < w.end && !reach(before)) return false;
+    if (before < w.count && !reach(before)) return false;
   }
   return true;
 }
@@ -814,17 +821,20 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
   SharedWalk w;
   w.blocks = static_cast<int>((p.a.batch * p.rows + p.shared.block_rows - 1) / p.shared.block_rows);
   w.keys = pages * p.a.cache.page;
-  w.cut = shared_cut(p.shared, p.a.cache.kv_heads * w.blocks, w.keys);
-  w.range = blockIdx.x;
-  const long long begin = static_cast<long long>(blockIdx.x) * w.cut.per, all = 1LL * p.a.cache.kv_heads * w.blocks * w.cut.tiles;
-  w.begin = static_cast<int>(min(begin, all));
-  w.end = static_cast<int>(min(begin + w.cut.per, all));
+  const int all = p.a.cache.kv_heads * w.blocks, block = static_cast<int>(blockIdx.x);
+  w.cut = shared_cut(p.shared, all, w.keys);
+  w.item = block / w.cut.splits;
+  w.step = w.cut.splits > 1 ? all : static_cast<int>(gridDim.x);
+  w.first = block % w.cut.splits * w.cut.per;
+  w.tiles = min(w.cut.per, w.cut.tiles - w.first);
+  w.items = w.keys > 0 ? all : 0;
+  w.count = w.item < w.items ? ((w.items - 1 - w.item) / w.step + 1) * w.tiles : 0;
   w.table = p.a.cache.table + __ldcg(p.shared.common + p.a.batch) * p.a.cache.columns;
   const char* values = tiles + S::kChunks * kChunkBytes;
   char* queries = tiles + kStages * S::kStageBytes;
   char* codes = queries + 2 * S::kQueryBytes;
   bool ok = true;
-  if (w.begin < w.end) {
+  if (w.count > 0) {
     if (warp < kWeighWarp) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegisters));
       if (warp < kIssueWarp + 2) ok = issue<SIZE, SETS, LO>(w, warp - kIssueWarp, tiles, values, queries, sync);
@@ -867,8 +877,8 @@ SharedScratch scratch_of(const cb_paged_attention_args& a, const SharedKeys& sha
   s.common = 0;
   s.attention = ((a.batch + 1) * 4 + 15) / 16 * 16;
   s.parts = s.attention + (attention_scratch(a, true) + 15) / 16 * 16;
-  s.bytes = s.parts + (a.cache.kv_heads * blocks + shared.ranges - 1) * shared.ways * shared.block_rows *
-                          (a.cache.head_size + 2) * 4LL;
+  const long long items = a.cache.kv_heads * blocks, pieces = items > shared.blocks ? items : shared.blocks;
+  s.bytes = s.parts + pieces * shared.ways * shared.block_rows * (a.cache.head_size + 2) * 4LL;
   return s;
 }
 // More than 128 rows of 16-bit queries: two sets of them to a block, which share
@@ -882,7 +892,7 @@ SharedKeys shared_of(const cb_paged_attention_args& a) {
   SharedKeys s = {};
   s.block_rows = two ? 2 * kRowLanes : kRowLanes;
   s.ways = two ? 1 : 2;
-  s.ranges = sm_count();
+  s.blocks = sm_count();
   s.least = 4;
   return s;
 }
@@ -969,7 +979,7 @@ int cb_paged_attention_shared(const cb_paged_attention_args* args, void* scratch
       CB_REQUIRE(e == cudaSuccess, "cb_paged_attention_shared: %s", cudaGetErrorString(e));
       device = now;
     }
-    launch(kernel, dim3(static_cast<unsigned>(p.shared.ranges)), dim3(kSharedThreads), SharedShape<SIZE>::kBytes, s, true, p);
+    launch(kernel, dim3(static_cast<unsigned>(p.shared.blocks)), dim3(kSharedThreads), SharedShape<SIZE>::kBytes, s, true, p);
     return check_launch("cb_paged_attention_shared");
   });
   if (done != CB_OK) return done;
