@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, resident_of(MODE)) attention_kernel(
 
   pdl_launch_dependents();
   pdl_wait();
-  const int pages = SHARED ? common_pages(p.shared, p.a.batch, found) : 0;
+  const int pages = SHARED ? common_pages(p.a, p.shared, found) : 0;
   if (SHARED) __syncthreads();  // (found is used again)
   Walk<tile_keys(SIZE)> walk;
   if (!begin_walk<tile_keys(SIZE), kGroups>(p, pages, scan, found, &walk)) return;

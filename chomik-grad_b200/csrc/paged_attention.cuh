@@ -10,6 +10,16 @@
 
 namespace cb {
 
+// Keys are computed apart where every sequence's reading them would be 128 MB or more:
+// beginning, ending and joining their parts takes 25 to 30 us, in which the other
+// kernel reads that from L2 (8 kv heads of 128, 64 sequences, 4 rows: 1024 keys 59 us
+// apart and 43 not, 8192 keys 78 and 189; 16 sequences, 20 rows: 1024 keys 65 and 29,
+// 16350 keys 115 and 158).
+constexpr long long kSharedBytes = 1LL << 27;
+__host__ __device__ inline long long shared_bytes_of(const cb_paged_attention_args& a, long long sequences, long long keys) {
+  return (sequences - 1) * keys * a.cache.kv_heads * a.cache.head_size * 2;
+}
+
 // The first keys of all sequences of a call, computed apart (paged_shared.cu).
 // `common`: for each sequence the whole pages that it has in common with the
 // call's first; INT_MAX where it takes no part.  The rows of a kv head, those
@@ -22,10 +32,10 @@ struct SharedKeys {
   const int* common;  // and behind them the slot of the first sequence that takes part
   const float* parts;
   int block_rows, ways, blocks, least;  // blocks of the grid; tiles of a piece: `least` or more, or all
+  long long least_bytes;                // see kSharedBytes
 };
-// Of element d of row r behind a part's references and sums: eight neighbouring
-// elements of a row together, so that the rows that write them and the elements that
-// read them touch whole sectors.
+// Of element d of row r behind a part's references and sums: eight elements of all rows
+// together, a sector each.
 __host__ __device__ constexpr long long shared_at(int block_rows, int r, int d) {
   return (static_cast<long long>(d / 8) * block_rows + r) * 8 + d % 8;
 }
@@ -125,16 +135,30 @@ struct Plan {  // of one launch
   SharedKeys shared;
 };
 
-// Pages that all sequences of the call have in common; every thread of the block calls this.
-__device__ __forceinline__ int common_pages(const SharedKeys& shared, long long batch, int* found) {
-  if (threadIdx.x == 0) *found = INT_MAX;
+// Pages that all sequences of the call have in common, 0 where it is not worth their
+// being computed apart; every thread of the block calls this.
+__device__ __forceinline__ int common_pages(const cb_paged_attention_args& a, const SharedKeys& shared, int* found) {
+  if (threadIdx.x == 0) {
+    found[0] = INT_MAX;
+    found[1] = 0;
+  }
   __syncthreads();
-  int least = INT_MAX;
-  for (int b = threadIdx.x; b < batch; b += blockDim.x) least = min(least, __ldcg(shared.common + b));
+  int least = INT_MAX, there = 0;
+  for (int b = threadIdx.x; b < a.batch; b += blockDim.x) {
+    const int pages = __ldcg(shared.common + b);
+    least = min(least, pages);
+    there += pages != INT_MAX;
+  }
   least = __reduce_min_sync(0xffffffffu, least);
-  if ((threadIdx.x & 31) == 0 && least != INT_MAX) atomicMin(found, least);
+  there = __reduce_add_sync(0xffffffffu, there);
+  if ((threadIdx.x & 31) == 0 && there > 0) {
+    atomicMin(found, least);
+    atomicAdd(found + 1, there);
+  }
   __syncthreads();
-  return *found == INT_MAX ? 0 : *found;
+  if (found[1] == 0) return 0;
+  const long long keys = static_cast<long long>(found[0]) * a.cache.page;
+  return shared_bytes_of(a, found[1], keys) >= shared.least_bytes ? found[0] : 0;
 }
 // The division of the shared keys: tiles of an item and of a piece, pieces of an item.
 // No block takes pieces of two items while there are more blocks than items, since

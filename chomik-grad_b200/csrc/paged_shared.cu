@@ -141,7 +141,7 @@ __device__ __forceinline__ void store8(uint32_t at, const uint32_t* v) {
                : "memory");
 }
 
-// Every lane of the warp waits for a phase, one of them looks: at most kPolls
+// Every lane of the warp waits for a phase and looks at most kPolls
 // times, without the clock, a read of which takes longer than most of these waits.
 // QUICK: by mbarrier.test_wait, which does not suspend the thread; a try_wait that
 // began well before its phase ends returns about a thousand cycles after it.
@@ -149,25 +149,23 @@ constexpr uint32_t kPolls = 1u << 24;
 template <bool QUICK = true>
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, const volatile int* abort) {
   bool there = true;
-  if ((threadIdx.x & 31) == 0) {
-    for (uint32_t i = 0;; ++i) {
-      if (QUICK) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(smem_addr(bar)), "r"(parity)
-            : "memory");
-        if (done != 0) break;
-      } else if (mbar_try_wait_short(bar, parity)) {
-        break;
-      }
-      if (i == kPolls || ((i & 255u) == 255u && *abort != 0)) {
-        there = false;
-        break;
-      }
+  for (uint32_t i = 0;; ++i) {
+    if (QUICK) {
+      uint32_t done;
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(done)
+          : "r"(smem_addr(bar)), "r"(parity)
+          : "memory");
+      if (done != 0) break;
+    } else if (mbar_try_wait_short(bar, parity)) {
+      break;
+    }
+    if (i == kPolls || ((i & 255u) == 255u && *abort != 0)) {
+      there = false;
+      break;
     }
   }
   return __all_sync(0xffffffffu, there);
@@ -178,6 +176,16 @@ __device__ __forceinline__ bool elected() {
   return one != 0;
 }
 
+__device__ __forceinline__ void unpack_row8(const SharedPlan& p, const uint4& v, float* x) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = *reinterpret_cast<const __half2*>(w + i);
+    const bool brain = p.a.dtype == CB_BF16;
+    x[2 * i] = brain ? __uint_as_float(w[i] << 16) : __low2float(h);
+    x[2 * i + 1] = brain ? __uint_as_float(w[i] & 0xffff0000u) : __high2float(h);
+  }
+}
 // Eight neighbouring elements of a query row: float32 (WIDE), or of 16 bits.
 template <bool WIDE>
 __device__ __forceinline__ void load_row8(const SharedPlan& p, long long at, float* x) {
@@ -196,37 +204,14 @@ __device__ __forceinline__ void load_row8(const SharedPlan& p, long long at, flo
   } else {
     const uint16_t* from = static_cast<const uint16_t*>(p.a.q) + at;
     uint32_t w[4];
-    if (p.wide) {
-      const uint4 v = *reinterpret_cast<const uint4*>(from);
-      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = from[2 * i] | static_cast<uint32_t>(from[2 * i + 1]) << 16;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __half2 h = *reinterpret_cast<const __half2*>(w + i);
-      const bool brain = p.a.dtype == CB_BF16;
-      x[2 * i] = brain ? __uint_as_float(w[i] << 16) : __low2float(h);
-      x[2 * i + 1] = brain ? __uint_as_float(w[i] & 0xffff0000u) : __high2float(h);
-    }
+    for (int i = 0; i < 4; ++i) w[i] = from[2 * i] | static_cast<uint32_t>(from[2 * i + 1]) << 16;
+    unpack_row8(p, make_uint4(w[0], w[1], w[2], w[3]), x);
   }
 }
-// 8 and 32 float32 columns of this thread's lane of the tensor memory (warp-wide).
+// 32 float32 columns of this thread's lane of the tensor memory (warp-wide).
 // The load and the wait for it are one statement: between two, the compiler could
 // move registers that are not written yet.
-__device__ __forceinline__ void load8(uint32_t at, float* out) {
-  uint32_t v[8];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {"
-      "%0, %1, %2, %3, %4, %5, %6, %7"
-      "}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-      : "r"(at)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 8; ++i) out[i] = __uint_as_float(v[i]);
-}
 __device__ __forceinline__ void load32(uint32_t at, float* out) {
   uint32_t v[32];
   asm volatile(
@@ -258,7 +243,7 @@ struct SharedSync {
   uint64_t score_full[2], score_free[2];
   uint64_t weight_full[2][2], value_done[2][2];  // [set][tile % 2]: a set is up to two tiles ahead of its products
   uint32_t tmem;
-  int abort, found;
+  int abort, found[2];
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
@@ -583,18 +568,32 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
     offsets[thread] = from;
     __syncwarp();
     if (segment > 0 && !wait_warp(&sync.query_free, static_cast<uint32_t>((segment - 1) & 1), abort)) return false;
-    {
+    const uint32_t turn_of_queries = static_cast<uint32_t>(segment & 1);
+    if (SETS == 2 || LO || set == 0) {
+      // 16-bit rows are copied to where they will be first; the loops are rolled, since
+      // code that runs once costs its way to the instruction cache
       constexpr int kLanes = SIZE / 8;
       const int lane = threadIdx.x & 31, d = lane % kLanes * 8;
-      const bool writes = SETS == 2 || LO || set == 0;
       char* to = queries + (SETS == 2 || LO ? set * SharedShape<SIZE>::kQueryBytes : 0) + d / 64 * kRowLanes * 128;
-#pragma unroll 8
+      const bool copied = !LO && p.wide;
+      if (copied) {
+#pragma unroll 1
+        for (int step = 0; step < kLanes; ++step) {
+          const int from_lane = step * (32 / kLanes) + lane / kLanes;
+          const long long at_row = offsets[thread / 32 * 32 + from_lane];
+          copy16(smem_addr(to + tc::swizzle_offset(r / 32 * 32 + from_lane, d % 64 / 8)),
+                 static_cast<const uint16_t*>(p.a.q) + (at_row >= 0 ? at_row + d : 0), at_row >= 0);
+        }
+        asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+      }
+#pragma unroll 1
       for (int step = 0; step < kLanes; ++step) {
-        const int from_lane = step * (32 / kLanes) + lane / kLanes;
+        const int from_lane = step * (32 / kLanes) + lane / kLanes, local_row = r / 32 * 32 + from_lane;
         const long long at_row = offsets[thread / 32 * 32 + from_lane];
-        const bool there = at_row >= 0;
+        uint4* place = reinterpret_cast<uint4*>(to + tc::swizzle_offset(local_row, d % 64 / 8));
         float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, largest = 0.0f;
-        if (there) load_row8<LO>(p, at_row + d, x);
+        if (copied) unpack_row8(p, *place, x);
+        else if (at_row >= 0) load_row8<LO>(p, at_row + d, x);
 #pragma unroll
         for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(x[i]));
 #pragma unroll
@@ -602,7 +601,6 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
         const int e = min(max(static_cast<int>(__float_as_uint(largest) >> 23) - 127, -126), 127);
         const float down = e == 127 ? 5.877471754111438e-39f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
         const float sign = p.a.scale < 0.0f ? -down : down;
-        const int local_row = r / 32 * 32 + from_lane;
         if (d == 0) factors[set * kSetThreads + local_row] = fabsf(p.a.scale) * 1.4426950408889634f * power2(e);
         uint32_t h[4];
 #pragma unroll
@@ -612,14 +610,16 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
           const __half2 hi = __floats2half2_rn(a, b);
           h[i] = LO && set == 1 ? bits(__floats2half2_rn(a - __low2float(hi), b - __high2float(hi))) : bits(hi);
         }
-        if (writes)
-          *reinterpret_cast<uint4*>(to + tc::swizzle_offset(local_row, d % 64 / 8)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *place = make_uint4(h[0], h[1], h[2], h[3]);
       }
       tc::fence_async_shared();
-      mbar_arrive(&sync.query_full);
-      __syncwarp();
     }
-    const float factor = factors[thread];
+    mbar_arrive(&sync.query_full);
+    __syncwarp();
+    // (one part of one set of rows: the other set has its factors from there)
+    const bool other = SETS == 1 && !LO && set == 1;
+    if (other && !wait_warp(&sync.query_full, turn_of_queries, abort)) return false;
+    const float factor = factors[other ? r : thread];
 
     float c = 0.0f, l = 0.0f, sum = 0.0f;  // reference, sum of the weights, and of what multiplied the codes
     bool first = true;
@@ -649,6 +649,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
         if (__builtin_expect(!irregular, 1)) {
           load32(scores, s);
           load32(scores + 32, s + 32);
+          leave_scores();
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             by[i] = factor * tile_runs.key[i];
@@ -704,16 +705,22 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
           c = now;
         }
         first = false;
-        if (__builtin_expect(!irregular && !__any_sync(0xffffffffu, top < c - kFarBelow), 1)) {
-          leave_scores();
+        if (__builtin_expect(!irregular, 1)) {
+          // all far below c: the weights by themselves, since 2^(y - c) may not be there
+          const bool far = __any_sync(0xffffffffu, top < c - kFarBelow);
+          if (__builtin_expect(far, 0)) {
+#pragma unroll
+            for (int k = 0; k < kSharedTile; ++k)
+              l += inverse[k / 16] != 0.0f ? exp2_of(fmaf(s[k], by[k / 16], -c)) : 0.0f;
+          }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float all = exponentials<LO>(s + 16 * i, by[i], log[i] - c);
-            l = fmaf(all, inverse[i], l);
+            if (!far) l = fmaf(all, inverse[i], l);
             sum += all;
             store_weights<LO>(weights + i * (LO ? 16 : 8), s + 16 * i);
           }
-        } else {  // value scales of any sign and size, or all far below c: the weights by themselves
+        } else {  // value scales of any sign and size: the weights by themselves
 #pragma unroll 1
           for (int i = 0; i < 4; ++i) {
             const float by_i = factor * tile_runs.key[i], shift = tile_runs.log[i] - c, kept = tile_runs.factor[i];
@@ -762,10 +769,11 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
         if (real) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
-            float4* to = reinterpret_cast<float4*>(part + 2 * rows + shared_at(rows, local, d + i));
+            float* to = part + 2 * rows + shared_at(rows, local, d + i);
             constexpr int b = STORAGE == CB_I8 ? 2 : 1, e = STORAGE == CB_I8 ? 1 : 2;  // (the order of the codes' halves)
-            to[0] = make_float4(o[i], o[i + b], o[i + e], o[i + 3]);
-            to[1] = make_float4(o[i + 4], o[i + 4 + b], o[i + 4 + e], o[i + 7]);
+            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "f"(o[i]), "f"(o[i + b]),
+                         "f"(o[i + e]), "f"(o[i + 3]), "f"(o[i + 4]), "f"(o[i + 4 + b]), "f"(o[i + 4 + e]), "f"(o[i + 7])
+                         : "memory");
           }
         }
       }
@@ -816,7 +824,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
   }
   tc::fence_before();
   pdl_wait();
-  const int pages = common_pages(p.shared, p.a.batch, &sync.found);  // (barriers of the block)
+  const int pages = common_pages(p.a, p.shared, sync.found);  // (barriers of the block)
   tc::fence_after();
   SharedWalk w;
   w.blocks = static_cast<int>((p.a.batch * p.rows + p.shared.block_rows - 1) / p.shared.block_rows);
@@ -875,8 +883,8 @@ SharedScratch scratch_of(const cb_paged_attention_args& a, const SharedKeys& sha
   const long long blocks = (a.batch * a.tokens * (a.heads / a.cache.kv_heads) + shared.block_rows - 1) / shared.block_rows;
   SharedScratch s;
   s.common = 0;
-  s.attention = ((a.batch + 1) * 4 + 15) / 16 * 16;
-  s.parts = s.attention + (attention_scratch(a, true) + 15) / 16 * 16;
+  s.attention = ((a.batch + 1) * 4 + 31) / 32 * 32;
+  s.parts = s.attention + (attention_scratch(a, true) + 31) / 32 * 32;
   const long long items = a.cache.kv_heads * blocks, pieces = items > shared.blocks ? items : shared.blocks;
   s.bytes = s.parts + pieces * shared.ways * shared.block_rows * (a.cache.head_size + 2) * 4LL;
   return s;
@@ -887,13 +895,14 @@ SharedScratch scratch_of(const cb_paged_attention_args& a, const SharedKeys& sha
 bool two_sets(const cb_paged_attention_args& a) {
   return a.dtype != CB_F32 && a.batch * a.tokens * (a.heads / a.cache.kv_heads) > kRowLanes;
 }
-SharedKeys shared_of(const cb_paged_attention_args& a) {
+SharedKeys shared_of(const cb_paged_attention_args& a, long long least_bytes) {
   const bool two = two_sets(a);
   SharedKeys s = {};
   s.block_rows = two ? 2 * kRowLanes : kRowLanes;
   s.ways = two ? 1 : 2;
   s.blocks = sm_count();
   s.least = 4;
+  s.least_bytes = least_bytes;
   return s;
 }
 
@@ -907,6 +916,11 @@ int shared_check(const cb_paged_attention_args& a) {
              "cb_paged_attention_shared: %lld rows of up to %lld keys are too many for one call", rows,
              a.cache.columns * a.cache.page);
   return CB_OK;
+}
+
+// Whether the sequences could hold enough keys in common for these to be computed apart.
+bool may_share(const cb_paged_attention_args& a, long long least_bytes) {
+  return shared_bytes_of(a, a.batch, a.cache.columns * a.cache.page) >= least_bytes;
 }
 
 template <typename F>
@@ -933,28 +947,32 @@ using namespace cb;
 
 extern "C" {
 
-long long cb_paged_attention_shared_scratch(const cb_paged_attention_args* args) {
+long long cb_paged_attention_shared_scratch(const cb_paged_attention_args* args, long long least_bytes) {
+  if (least_bytes < 0) least_bytes = kSharedBytes;
   if (args == nullptr || shared_check(*args) != CB_OK || args->batch == 0 || args->tokens == 0) return 0;
-  return scratch_of(*args, shared_of(*args)).bytes;
+  if (!may_share(*args, least_bytes)) return attention_scratch(*args, false);
+  return scratch_of(*args, shared_of(*args, least_bytes)).bytes;
 }
 
-int cb_paged_attention_shared(const cb_paged_attention_args* args, void* scratch, unsigned* counters,
-                              cb_stream_t stream) {
+int cb_paged_attention_shared(const cb_paged_attention_args* args, long long least_bytes, void* scratch,
+                              unsigned* counters, cb_stream_t stream) {
+  if (least_bytes < 0) least_bytes = kSharedBytes;
   CB_REQUIRE(args != nullptr, "cb_paged_attention_shared: null arguments");
   const cb_paged_attention_args& a = *args;
   const int status = shared_check(a);
   if (status != CB_OK) return status;
   if (a.batch == 0 || a.tokens == 0) return CB_OK;
+  if (!may_share(a, least_bytes)) return launch_attention(a, nullptr, scratch, counters, static_cast<cudaStream_t>(stream));
   CB_REQUIRE(a.q != nullptr && a.out != nullptr && counters != nullptr && scratch != nullptr,
              "cb_paged_attention_shared: a null pointer");
-  CB_REQUIRE(reinterpret_cast<uintptr_t>(scratch) % 16 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0,
-             "cb_paged_attention_shared: out and scratch must be 16-byte aligned");
+  CB_REQUIRE(reinterpret_cast<uintptr_t>(scratch) % 32 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0,
+             "cb_paged_attention_shared: out must be 16-byte aligned, scratch 32");
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   SharedPlan p = {};
   p.a = a;
   p.group = static_cast<int>(a.heads / a.cache.kv_heads);
   p.rows = static_cast<int>(a.tokens * p.group);
-  p.shared = shared_of(a);
+  p.shared = shared_of(a, least_bytes);
   const SharedScratch at = scratch_of(a, p.shared);
   char* base = static_cast<char*>(scratch);
   int* common = reinterpret_cast<int*>(base + at.common);

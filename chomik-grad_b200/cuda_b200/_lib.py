@@ -402,8 +402,8 @@ _SIGNATURES = {
     "cb_paged_attention_scratch": ([POINTER(PagedAttentionArgs)], c_longlong),
     "cb_paged_attention_counters": ([POINTER(PagedAttentionArgs)], c_longlong),
     "cb_paged_attention": ([POINTER(PagedAttentionArgs), c_void_p, c_void_p, c_void_p], c_int),
-    "cb_paged_attention_shared_scratch": ([POINTER(PagedAttentionArgs)], c_longlong),
-    "cb_paged_attention_shared": ([POINTER(PagedAttentionArgs), c_void_p, c_void_p, c_void_p], c_int),
+    "cb_paged_attention_shared_scratch": ([POINTER(PagedAttentionArgs), c_longlong], c_longlong),
+    "cb_paged_attention_shared": ([POINTER(PagedAttentionArgs), c_longlong, c_void_p, c_void_p, c_void_p], c_int),
     "cb_pages_scratch": ([POINTER(PageBook), c_longlong], c_longlong),
     "cb_pages_extend": ([POINTER(PageBook), POINTER(PagePools), c_void_p, c_void_p, c_longlong, c_void_p, c_void_p,
                          c_void_p], c_int),

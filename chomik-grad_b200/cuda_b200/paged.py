@@ -41,6 +41,7 @@ from . import _lib
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 HEAD_SIZES = (32, 64, 128)
+SHARED_BYTES = 2 ** 27  # of ``attend_shared``: from where reading shared keys once pays
 _VALUES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _STORAGE = {torch.int8: _lib.I8, torch.float8_e4m3fn: _lib.E4M3}
 
@@ -294,28 +295,36 @@ class PagedCache:
         slot walks the slot's whole length, also those past ``counts[b]``: one
         long chunk with many single tokens costs less in a call of its own.
         """
-        return self._attend("cb_paged_attention", layer, q, counts, sequences, scale, out)
+        return self._attend(layer, q, counts, sequences, scale, out, None)
 
     def attend_shared(self, layer: int, q: Any, *, counts: Any = None, sequences: Any = None,
-                      scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                      scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                      least_bytes: int = SHARED_BYTES) -> torch.Tensor:
         """``attend`` for sequences that begin alike, as ``fork`` leaves them.
 
         The leading pages that all sequences of the call hold in common (those
-        with a count of 0 aside) are found on the device, and read and multiplied
-        once with the rows of all of them; each sequence's other keys are its own,
-        as in ``attend``.  Any sequences may be given: where they share nothing the
-        call takes little longer than ``attend``'s.
-        """
-        return self._attend("cb_paged_attention_shared", layer, q, counts, sequences, scale, out)
+        with a count of 0 aside) are found on the device.  Where the sequences'
+        reading them one by one would be ``least_bytes`` more than once, they are read
+        and multiplied once with the rows of all; each sequence's other keys are
+        its own.  Any sequences may be given, and a cache whose tables cannot hold that
+        much is read as by ``attend``.
 
-    def _attend(self, entry: str, layer: int, q: Any, counts: Any, sequences: Any, scale: Optional[float],
-                out: Optional[torch.Tensor]) -> torch.Tensor:
+        Queries and weights of these keys go to the tensor cores as fp16 with float32
+        sums, of float32 queries in two parts (22 bits).  Within 64 keys, one whose
+        weight is below 2^-9 (float32: 2^-22) of the largest of them may be rounded
+        to that, and one below 2^-10 (2^-23) of it left out, where another tile's
+        is 2^15 (2^2) times larger still.
+        """
+        return self._attend(layer, q, counts, sequences, scale, out, int(least_bytes))
+
+    def _attend(self, layer: int, q: Any, counts: Any, sequences: Any, scale: Optional[float],
+                out: Optional[torch.Tensor], least_bytes: Optional[int]) -> torch.Tensor:
         q, counts, sequences = tensor_of(q), self._ints(counts), self._ints(sequences)
         no_grad_needed(q)
-        key = (entry, layer, signature(q), signature(counts), signature(sequences), scale)
+        key = (layer, signature(q), signature(counts), signature(sequences), scale, least_bytes)
         known = self._attend_args.get(key)
         if known is None:
-            known = self._attend_args[key] = self._prepare_attend(entry, layer, q, counts, sequences, scale)
+            known = self._attend_args[key] = self._prepare_attend(layer, q, counts, sequences, scale, least_bytes)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
@@ -332,7 +341,11 @@ class PagedCache:
             a.sequences = sequences.data_ptr()
         stream = self._stream()
         counters, scratch = self._workspace(stream, known[2], known[1])
-        _lib.check(getattr(self._lib, entry)(ctypes.byref(a), scratch, counters, stream), entry)
+        if least_bytes is None:
+            _lib.check(self._lib.cb_paged_attention(ctypes.byref(a), scratch, counters, stream), "cb_paged_attention")
+        else:
+            _lib.check(self._lib.cb_paged_attention_shared(ctypes.byref(a), least_bytes, scratch, counters, stream),
+                       "cb_paged_attention_shared")
         return out
 
     def _workspace(self, stream: int, counters: int, words: int) -> Tuple[int, int]:
@@ -351,9 +364,11 @@ class PagedCache:
             kept = self._workspaces[stream] = (counters, words, counts.data_ptr(), scratch.data_ptr(), counts, scratch)
         return kept[2], kept[3]
 
-    def _prepare_attend(self, entry: str, layer: int, q: torch.Tensor, counts: Optional[torch.Tensor],
-                        sequences: Optional[torch.Tensor],
-                        scale: Optional[float]) -> Tuple[_lib.PagedAttentionArgs, int, int]:
+    def _prepare_attend(self, layer: int, q: torch.Tensor, counts: Optional[torch.Tensor],
+                        sequences: Optional[torch.Tensor], scale: Optional[float],
+                        least_bytes: Optional[int]) -> Tuple[_lib.PagedAttentionArgs, int, int]:
+        if least_bytes is not None and not 0 <= least_bytes < 2 ** 63:
+            raise ValueError(f"least_bytes is {least_bytes}, expected 0 or more")
         require(q, "q", self.device, tuple(_VALUES), (None, None, None, self.head_size), 1)
         batch, tokens, heads = q.shape[:3]
         if heads == 0 or heads % self.kv_heads:
@@ -365,7 +380,11 @@ class PagedCache:
         a.q_strides[:] = q.stride()[:3]
         a.scale = 1.0 / math.sqrt(self.head_size) if scale is None else scale
         a.error_flag = self._flag.data_ptr()
-        return (a, (getattr(self._lib, entry + "_scratch")(ctypes.byref(a)) + 3) // 4,
+        if least_bytes is None:
+            size = self._lib.cb_paged_attention_scratch(ctypes.byref(a))
+        else:
+            size = self._lib.cb_paged_attention_shared_scratch(ctypes.byref(a), least_bytes)
+        return (a, (size + 3) // 4,
                 self._lib.cb_paged_attention_counters(ctypes.byref(a)))
 
     # -- pages -------------------------------------------------------------

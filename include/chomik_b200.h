@@ -926,13 +926,16 @@ CB_API int cb_paged_attention(const cb_paged_attention_args* args, void* scratch
 /* cb_paged_attention for sequences that begin alike, as cb_pages_fork leaves them:
  * the leading pages that the tables of all sequences with a count name alike, as
  * far as they are whole and leave each row a key of its own, are found on the
- * device, and read and multiplied once with the rows of all of them.  Any
- * sequences may be given; those that share nothing take the time of
- * cb_paged_attention and of two short launches.  `scratch`:
- * cb_paged_attention_shared_scratch bytes; `counters` as there. */
-CB_API long long cb_paged_attention_shared_scratch(const cb_paged_attention_args* args);
-CB_API int cb_paged_attention_shared(const cb_paged_attention_args* args, void* scratch, unsigned* counters,
-                                     cb_stream_t stream);
+ * device.  Where the sequences' reading them one by one would be `least_bytes` more
+ * than once (below 0: 128 MB, from where it pays), they are read and
+ * multiplied once, with the rows of all.  Any sequences may be given; where the table's
+ * columns cannot hold that much this is cb_paged_attention.  `scratch`:
+ * cb_paged_attention_shared_scratch bytes for the same arguments, 32-byte aligned;
+ * `counters` as there.  A bounded wait that gives up sets CB_FLAG_WAIT_DATA or
+ * CB_FLAG_WAIT_DRAIN. */
+CB_API long long cb_paged_attention_shared_scratch(const cb_paged_attention_args* args, long long least_bytes);
+CB_API int cb_paged_attention_shared(const cb_paged_attention_args* args, long long least_bytes, void* scratch,
+                                     unsigned* counters, cb_stream_t stream);
 
 /* The book of a cache: who holds which page.  refs[p] slots hold page p;
  * free[0 .. *height) is a stack of the pages that none holds.  A slot of

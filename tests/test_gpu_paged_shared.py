@@ -53,7 +53,7 @@ def check(host, q, counts, slots, dtype, scale=None, **call):
     given = {"counts": torch.tensor(counts, dtype=torch.int32, device="cuda")}
     if slots is not None:
         given["sequences"] = torch.tensor(slots, dtype=torch.int32, device="cuda")
-    got = cache.attend_shared(0, q, scale=scale, **given, **call)
+    got = cache.attend_shared(0, q, least_bytes=0, scale=scale, **given, **call)
     cache.check_errors()
     size = q.shape[-1]
     want = expected(host, q, counts, range(q.shape[0]) if slots is None else slots,
@@ -105,7 +105,7 @@ def test_many_rows_and_long_prefixes(batch, prefix, dtype):
     q = queries(rng, batch, 1, 8, 64, dtype)
     cache, got = check(host, q, [1] * batch, None, dtype)
     for _ in range(3):
-        assert torch.equal(got, cache.attend_shared(0, q))
+        assert torch.equal(got, cache.attend_shared(0, q, least_bytes=0))
 
 
 def test_whole_sequences_shared():
@@ -157,7 +157,7 @@ def test_queries_of_any_size(size, dtype):
     q = queries(rng, 2, 1, 4, 128, dtype) * size
     cache = to_device(host)
     want = expected(host, q, [1, 1], range(2), 1 / math.sqrt(128))
-    got = wide(cache.attend_shared(0, q))
+    got = wide(cache.attend_shared(0, q, least_bytes=0))
     cache.check_errors()
     values = max(float(np.abs(host.read(0, 1, s)).max()) for s in range(2))
     # scores of thousands in base 2 move by their own float32 rounding: 2^-22 of them
@@ -204,12 +204,12 @@ def test_captured_on_other_streams():
     cache = to_device(host)
     q = queries(rng, 3, 1, 8, 64, "bf16")
     counts = torch.ones(3, dtype=torch.int32, device="cuda")
-    cache.attend_shared(0, q, counts=counts)
+    cache.attend_shared(0, q, least_bytes=0, counts=counts)
     graphs, outs = [], []
     for _ in range(2):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            outs.append(cache.attend_shared(0, q, counts=counts))
+            outs.append(cache.attend_shared(0, q, least_bytes=0, counts=counts))
         graphs.append(graph)
     host.truncate([3, 30, 8], [0, 1, 2])
     cache.truncate([3, 30, 8])
@@ -225,7 +225,7 @@ def test_captured_on_other_streams():
     for out in outs:
         compare(out, expected(host, q, [1] * 3, range(3), 0.125), host, "bf16")
     with torch.cuda.stream(streams[0]):
-        assert torch.equal(cache.attend_shared(0, q, counts=counts), outs[0])
+        assert torch.equal(cache.attend_shared(0, q, least_bytes=0, counts=counts), outs[0])
     torch.cuda.synchronize()
 
 
@@ -237,21 +237,21 @@ def test_bad_books_are_flagged():
     for bad in (len(host.refs), -1, 2 ** 31 - 1):
         cache = to_device(host)
         cache.table[:, 2] = bad
-        cache.attend_shared(0, q)
+        cache.attend_shared(0, q, least_bytes=0)
         with pytest.raises(IndexError):
             cache.check_errors()
     cache = to_device(host)
     ones = torch.ones(3, dtype=torch.int32, device="cuda")
     for call in (dict(sequences=2 * ones), dict(counts=3 * ones), dict(counts=-ones),
                  dict(sequences=torch.tensor([3, 0, 1], dtype=torch.int32, device="cuda"))):
-        got = cache.attend_shared(0, q, **call)
+        got = cache.attend_shared(0, q, least_bytes=0, **call)
         if "sequences" in call and int(call["sequences"][0]) == 2:
             cache.check_errors()  # (one slot three times is a call of its own)
             continue
         with pytest.raises(IndexError):
             cache.check_errors()
         assert torch.isfinite(got).all()
-    compare(cache.attend_shared(0, q), expected(host, q, [1] * 3, range(3), 0.125), host, "f32")
+    compare(cache.attend_shared(0, q, least_bytes=0), expected(host, q, [1] * 3, range(3), 0.125), host, "f32")
     cache.check_errors()
 
 
@@ -265,5 +265,7 @@ def test_refusals():
             cache.attend_shared(**{"layer": 0, **call})
     with pytest.raises(TypeError):
         cache.attend_shared(0, q.double())
+    with pytest.raises(ValueError):
+        cache.attend_shared(0, q, least_bytes=-1)
     with pytest.raises(ValueError):
         cache.attend_shared(0, q.requires_grad_())

@@ -141,7 +141,7 @@ def shared(c, scratch=16, counters=16, **changes):
     a = _lib.PagedAttentionArgs(cache=c, q=16, out=16, dtype=_lib.F32, batch=1, tokens=1, heads=2, scale=1.0)
     for name, value in changes.items():
         setattr(a, name, value)
-    return _lib.call("cb_paged_attention_shared", ctypes.byref(a), scratch, counters, None)
+    return _lib.call("cb_paged_attention_shared", ctypes.byref(a), 0, scratch, counters, None)
 
 
 @pytest.mark.parametrize("change", [dict(storage=_lib.BF16), dict(head_size=48), dict(page=24), dict(kv_heads=0),
