@@ -31,6 +31,7 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kBlockBytes = 512;   // 16 outputs x 64 inputs
+constexpr int kTwoFrom = 6;        // tiles to an SM from which a block takes two
 constexpr int kColumnTiles = 4;    // most of 8 columns that a launch's block takes
 
 __host__ __device__ constexpr long long tiles_of(long long outputs) { return (outputs + 15) / 16; }
@@ -108,18 +109,88 @@ struct LinearPlan {
   int per;  // rows of y that a block takes
 };
 
-// A block takes one tile of 16 outputs and `per` rows of y.  Its warps take the
-// chunks of 64 inputs in turn and are joined in shared memory, in their order.
-template <bool HALF, int GROUP, int COLUMNS>
-__global__ void __launch_bounds__(kThreads) linear_kernel(const __grid_constant__ LinearPlan p) {
-  constexpr int kScaleWords = GROUP == 32 ? 2 : 1;  // of a lane, for a chunk
-  __shared__ float sums[kWarps][16][8 * COLUMNS + 1];
+// A unit of a warp: 16 outputs x 128 inputs, and their scales.
+template <int GROUP>
+struct Unit {
+  static constexpr int kWords = GROUP == 32 ? 4 : GROUP == 64 ? 2 : 1;
+  uint4 codes[2];
+  uint32_t scales[kWords];
+};
+// WHOLE: both of its chunks are there.
+template <int GROUP, bool WHOLE>
+__device__ __forceinline__ void load_unit(Unit<GROUP>& u, const uint4* codes, const uint32_t* scales) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const bool real = WHOLE || i == 0;
+    u.codes[i] = real ? __ldcs(codes + i * 32) : make_uint4(0, 0, 0, 0);
+    if (GROUP == 64) u.scales[i % Unit<GROUP>::kWords] = real ? __ldcs(scales + i * 8) : 0;
+    if (GROUP == 32) {
+      const uint2 two = real ? __ldcs(reinterpret_cast<const uint2*>(scales) + i * 8) : make_uint2(0, 0);
+      u.scales[2 * i % Unit<GROUP>::kWords] = two.x;
+      u.scales[(2 * i + 1) % Unit<GROUP>::kWords] = two.y;
+    }
+  }
+  if (GROUP == 128) u.scales[0] = __ldcs(scales);
+}
+
+// The products of TILES units with the same x.  `left`: inputs from this lane's first on
+// (all of a whole unit's are there).
+template <bool HALF, int GROUP, int COLUMNS, int TILES, bool WHOLE>
+__device__ __forceinline__ void multiply_units(const Unit<GROUP>* u, const uint16_t* const* x, long long k, long long left,
+                                               int scale_dtype, float (*total)[COLUMNS][4]) {
+  float sum[TILES][COLUMNS][4];
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = part * 64 + h * 32;
+      uint4 b[COLUMNS];
+#pragma unroll
+      for (int t = 0; t < COLUMNS; ++t)
+        b[t] = WHOLE || at < left ? *reinterpret_cast<const uint4*>(x[t] + k + at) : make_uint4(0, 0, 0, 0);
+      const bool begins = GROUP == 32 || (h == 0 && (GROUP == 64 || part == 0));
+      const bool ends = GROUP == 32 || (h == 1 && (GROUP == 64 || part == 1));
+#pragma unroll
+      for (int n = 0; n < TILES; ++n) {
+        const uint32_t w[4] = {u[n].codes[part].x, u[n].codes[part].y, u[n].codes[part].z, u[n].codes[part].w};
+        uint32_t a[4];
+        halves_of<HALF>(w[2 * h], a);
+#pragma unroll
+        for (int t = 0; t < COLUMNS; ++t) {
+          if (begins) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[n][t][i] = 0.0f;
+          }
+          product<HALF>(sum[n][t], a, b[t].x, b[t].y);
+        }
+        halves_of<HALF>(w[2 * h + 1], a);
+#pragma unroll
+        for (int t = 0; t < COLUMNS; ++t) product<HALF>(sum[n][t], a, b[t].z, b[t].w);
+        if (ends) {
+          const uint32_t both = u[n].scales[GROUP == 32 ? 2 * part + h : GROUP == 64 ? part : 0];
+          const float low = scale_of(both & 0xffffu, scale_dtype), high = scale_of(both >> 16, scale_dtype);
+#pragma unroll
+          for (int t = 0; t < COLUMNS; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) total[n][t][i] = fmaf(i < 2 ? low : high, sum[n][t][i], total[n][t][i]);
+        }
+      }
+    }
+  }
+}
+
+// A block takes TILES tiles of 16 outputs and `per` rows of y.  Its warps take the
+// units of the tiles in turn, the loads of the next under way, and are joined in
+// shared memory, in their order.  Columns that no row of x belongs to are computed
+// like row `first` and not stored.
+template <bool HALF, int GROUP, int COLUMNS, int TILES>
+__global__ void __launch_bounds__(kThreads, TILES * COLUMNS <= 2 ? 3 : 2) linear_kernel(const __grid_constant__ LinearPlan p) {
+  __shared__ float sums[kWarps][16 * TILES][8 * COLUMNS + 1];
+  constexpr int kScaleWords = 8 * Unit<GROUP>::kWords;  // of a unit's tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const long long tile = blockIdx.x;
-  const int chunks = static_cast<int>(chunks_of(p.w.inputs));
+  const int chunks = static_cast<int>(chunks_of(p.w.inputs)), units = (chunks + 1) / 2;
   const int all = p.rows / p.parts, first = static_cast<int>(blockIdx.y) * p.per, mine = min(p.per, all - first);
-  const uint4* codes = static_cast<const uint4*>(p.w.codes) + tile * chunks * 32 + lane;
-  const uint32_t* scales = static_cast<const uint32_t*>(p.w.scales) + tile * tile_scales(p.w.inputs, GROUP) / 2;
+  const long long tile = static_cast<long long>(blockIdx.x) * TILES, last = tiles_of(p.w.outputs) - 1;
   pdl_launch_dependents();
   if (mine <= 0) return;
 
@@ -127,78 +198,72 @@ __global__ void __launch_bounds__(kThreads) linear_kernel(const __grid_constant_
   const uint16_t* x[COLUMNS];
 #pragma unroll
   for (int t = 0; t < COLUMNS; ++t) {
-    const int j = t * 8 + g;
-    x[t] = j < mine * p.parts
-               ? static_cast<const uint16_t*>(p.x) + (static_cast<long long>(j / mine) * all + first + j % mine) * p.ld + c * 8
-               : nullptr;
+    const int j = t * 8 + g, row = j < mine * p.parts ? j / mine * all + first + j % mine : first;
+    x[t] = static_cast<const uint16_t*>(p.x) + static_cast<long long>(row) * p.ld + c * 8;
   }
-  float total[COLUMNS][4], sum[COLUMNS][4];
+  const uint4* codes[TILES];
+  const uint32_t* scales[TILES];
 #pragma unroll
-  for (int t = 0; t < COLUMNS; ++t)
+  for (int n = 0; n < TILES; ++n) {
+    const long long at = min(tile + n, last);  // (one that is not there is computed like the last and not stored)
+    codes[n] = static_cast<const uint4*>(p.w.codes) + at * chunks * 32 + lane;
+    scales[n] = static_cast<const uint32_t*>(p.w.scales) + at * tile_scales(p.w.inputs, GROUP) / 2 +
+                g * (GROUP == 32 ? 2 : 1);
+  }
+  float total[TILES][COLUMNS][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) total[t][i] = sum[t][i] = 0.0f;
+  for (int n = 0; n < TILES; ++n)
+#pragma unroll
+    for (int t = 0; t < COLUMNS; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) total[n][t][i] = 0.0f;
   pdl_wait();
-  // groups of 128: a warp takes both chunks of one
-  constexpr int kTogether = GROUP == 128 ? 2 : 1;
-  for (int from = warp * kTogether; from < chunks; from += kWarps * kTogether) {
+  const int whole = static_cast<int>(p.w.inputs / 128);  // units that are
+  Unit<GROUP> ring[2][TILES];
+  auto load = [&](Unit<GROUP>* u, int unit) {
+    if (unit < whole) {
 #pragma unroll
-    for (int part = 0; part < kTogether; ++part) {
-      const int chunk = from + part;
-      if (chunk >= chunks) break;
-      const uint4 w4 = __ldcs(codes + static_cast<long long>(chunk) * 32);
-      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-      uint32_t s[kScaleWords];
-      if (GROUP == 128) s[0] = __ldg(scales + static_cast<long long>(chunk / 2) * 8 + g);
-      if (GROUP == 64) s[0] = __ldg(scales + static_cast<long long>(chunk) * 8 + g);
-      if (GROUP == 32) {
-        const uint2 two = __ldg(reinterpret_cast<const uint2*>(scales) + static_cast<long long>(chunk) * 8 + g);
-        s[0] = two.x;
-        s[kScaleWords - 1] = two.y;
-      }
+      for (int n = 0; n < TILES; ++n)
+        load_unit<GROUP, true>(u[n], codes[n] + static_cast<long long>(unit) * 64,
+                               scales[n] + static_cast<long long>(unit) * kScaleWords);
+    }
+  };
+  load(ring[0], warp);
+  int unit = warp;
+  for (; unit < whole; unit += 2 * kWarps) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint4 b[COLUMNS];
-        const long long k = static_cast<long long>(chunk) * 64 + h * 32;
-#pragma unroll
-        for (int t = 0; t < COLUMNS; ++t)
-          b[t] = x[t] != nullptr && k + c * 8 < p.w.inputs ? *reinterpret_cast<const uint4*>(x[t] + k)
-                                                           : make_uint4(0, 0, 0, 0);
-        uint32_t a[4];
-        halves_of<HALF>(w[2 * h], a);
-#pragma unroll
-        for (int t = 0; t < COLUMNS; ++t) product<HALF>(sum[t], a, b[t].x, b[t].y);
-        halves_of<HALF>(w[2 * h + 1], a);
-#pragma unroll
-        for (int t = 0; t < COLUMNS; ++t) product<HALF>(sum[t], a, b[t].z, b[t].w);
-        const bool ends = GROUP == 32 || (h == 1 && (GROUP == 64 || part == 1 || chunk + 1 == chunks));
-        if (ends) {
-          const uint32_t both = s[GROUP == 32 ? h * (kScaleWords - 1) : 0];
-          const float low = scale_of(both & 0xffffu, p.w.scale_dtype), high = scale_of(both >> 16, p.w.scale_dtype);
-#pragma unroll
-          for (int t = 0; t < COLUMNS; ++t) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              total[t][i] = fmaf(i < 2 ? low : high, sum[t][i], total[t][i]);
-              sum[t][i] = 0.0f;
-            }
-          }
-        }
-      }
+    for (int slot = 0; slot < 2; ++slot) {
+      const int now = unit + slot * kWarps;
+      if (now >= whole) break;
+      load(ring[slot ^ 1], now + kWarps);
+      multiply_units<HALF, GROUP, COLUMNS, TILES, true>(ring[slot], x, now * 128LL, 0, p.w.scale_dtype, total);
     }
   }
+  if (whole < units && whole % kWarps == warp) {  // less than a unit is left
+    const long long k = whole * 128LL;
 #pragma unroll
-  for (int t = 0; t < COLUMNS; ++t)
+    for (int n = 0; n < TILES; ++n) {
+      const uint4* from = codes[n] + static_cast<long long>(whole) * 64;
+      const uint32_t* by = scales[n] + static_cast<long long>(whole) * kScaleWords;
+      if (2 * whole + 1 < chunks) load_unit<GROUP, true>(ring[0][n], from, by);
+      else load_unit<GROUP, false>(ring[0][n], from, by);
+    }
+    multiply_units<HALF, GROUP, COLUMNS, TILES, false>(ring[0], x, k, p.w.inputs - k - c * 8, p.w.scale_dtype, total);
+  }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sums[warp][g + i / 2 * 8][t * 8 + 2 * c + i % 2] = total[t][i];
+  for (int n = 0; n < TILES; ++n)
+#pragma unroll
+    for (int t = 0; t < COLUMNS; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sums[warp][n * 16 + g + i / 2 * 8][t * 8 + 2 * c + i % 2] = total[n][t][i];
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * mine; i += kThreads) {
-    const int n = i % 16, r = i / 16;
+  for (int i = threadIdx.x; i < 16 * TILES * mine; i += kThreads) {
+    const int n = i % (16 * TILES), r = i / (16 * TILES);
     float y = 0.0f;
     for (int part = 0; part < p.parts; ++part)
 #pragma unroll
       for (int v = 0; v < kWarps; ++v) y += sums[v][n][part * mine + r];
-    if (tile * 16 + n < p.w.outputs)
-      store_from_f32(p.out, (first + r) * p.out_ld + tile * 16 + n, p.out_dtype, y);
+    if (tile * 16 + n < p.w.outputs) store_from_f32(p.out, (first + r) * p.out_ld + tile * 16 + n, p.out_dtype, y);
   }
 }
 
@@ -480,15 +545,23 @@ int cb_linear4(const cb_linear4_args* args, void* scratch, cb_stream_t stream) {
   p.per = static_cast<int>((a.rows + launches - 1) / launches);
   return with_columns((p.per * p.parts + 7) / 8, [&](auto columns) {
     constexpr int C = columns.value;
-    const dim3 grid(static_cast<unsigned>(tiles_of(a.weights.outputs)), static_cast<unsigned>(launches));
-    auto go = [&](auto kernel) {
-      launch(kernel, grid, dim3(kThreads), 0, s, true, p);
+    const long long tiles = tiles_of(a.weights.outputs);
+    auto go = [&](auto group, auto count) {
+      constexpr int T = count.value;
+      const dim3 grid(static_cast<unsigned>((tiles + T - 1) / T), static_cast<unsigned>(launches));
+      if (a.dtype == CB_F16)
+        launch(linear_kernel<true, group.value, C, T>, grid, dim3(kThreads), 0, s, true, p);
+      else
+        launch(linear_kernel<false, group.value, C, T>, grid, dim3(kThreads), 0, s, true, p);
       return check_launch("cb_linear4");
     };
-    const bool half = a.dtype == CB_F16;
-    if (a.weights.group == 32) return half ? go(linear_kernel<true, 32, C>) : go(linear_kernel<false, 32, C>);
-    if (a.weights.group == 64) return half ? go(linear_kernel<true, 64, C>) : go(linear_kernel<false, 64, C>);
-    return half ? go(linear_kernel<true, 128, C>) : go(linear_kernel<false, 128, C>);
+    auto by_tiles = [&](auto group) {
+      return tiles >= kTwoFrom * sm_count() ? go(group, std::integral_constant<int, 2>{})
+                                      : go(group, std::integral_constant<int, 1>{});
+    };
+    if (a.weights.group == 32) return by_tiles(std::integral_constant<int, 32>{});
+    if (a.weights.group == 64) return by_tiles(std::integral_constant<int, 64>{});
+    return by_tiles(std::integral_constant<int, 128>{});
   });
 }
 
