@@ -31,7 +31,13 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kBlockBytes = 512;   // 16 outputs x 64 inputs
-constexpr int kTwoFrom = 6;        // tiles to an SM from which a block takes two
+// Tiles to an SM: up to kFewTo one wave of blocks with 80 registers, whose loads reach
+// further ahead (256 tiles of 14336 inputs 11.4 us, with 64 registers 15.0); above, four
+// blocks an SM (896 tiles of 4096 inputs 9.9 us, three 12.5); from kTwoFrom on a block
+// takes two tiles, which share the rows of x (8016 tiles: 60.6 us and 64.2 for one
+// row, 91 and 110 for 16; of more columns than two the sums do not fit the
+// registers: 32 rows 35 us with two tiles, 31 with one).
+constexpr int kFewTo = 3, kTwoFrom = 16;
 constexpr int kColumnTiles = 4;    // most of 8 columns that a launch's block takes
 
 __host__ __device__ constexpr long long tiles_of(long long outputs) { return (outputs + 15) / 16; }
@@ -40,12 +46,6 @@ __host__ __device__ constexpr long long chunks_of(long long inputs) { return (in
 __host__ __device__ constexpr long long tile_scales(long long inputs, int group) {
   return group == 128 ? (chunks_of(inputs) + 1) / 2 * 16 : chunks_of(inputs) * (64 / group) * 16;
 }
-__host__ __device__ constexpr long long scale_at(long long inputs, int group, long long n, long long at) {
-  const long long tile = n / 16 * tile_scales(inputs, group), row = n % 16;
-  if (group == 32) return tile + at / 2 * 32 + row % 8 * 4 + at % 2 * 2 + row / 8;
-  return tile + at * 16 + row % 8 * 2 + row / 8;
-}
-
 __device__ __forceinline__ float scale_of(uint32_t bits, int dtype) {
   return dtype == CB_BF16 ? bf16_bits_to_f32(static_cast<uint16_t>(bits))
                           : __half2float(__ushort_as_half(static_cast<uint16_t>(bits)));
@@ -183,8 +183,8 @@ __device__ __forceinline__ void multiply_units(const Unit<GROUP>* u, const uint1
 // units of the tiles in turn, the loads of the next under way, and are joined in
 // shared memory, in their order.  Columns that no row of x belongs to are computed
 // like row `first` and not stored.
-template <bool HALF, int GROUP, int COLUMNS, int TILES>
-__global__ void __launch_bounds__(kThreads, TILES * COLUMNS <= 2 ? 3 : 2) linear_kernel(const __grid_constant__ LinearPlan p) {
+template <bool HALF, int GROUP, int COLUMNS, int TILES, int RESIDENT>
+__global__ void __launch_bounds__(kThreads, RESIDENT) linear_kernel(const __grid_constant__ LinearPlan p) {
   __shared__ float sums[kWarps][16 * TILES][8 * COLUMNS + 1];
   constexpr int kScaleWords = 8 * Unit<GROUP>::kWords;  // of a unit's tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -321,42 +321,57 @@ __global__ void __launch_bounds__(256) pack_kernel(const uint8_t* codes, const u
   }
 }
 
-// A warp to 16 outputs x 64 inputs.
-template <int ITEM>
+// A warp to 16 outputs x 64 inputs.  Bound by its instructions before its stores: the
+// codes come out of a word as bytes, by whose place a float's bits are made (2^23 + code),
+// and the group and the strides are known when it is compiled or computed once.
+template <int GROUP, int ITEM>
 __global__ void __launch_bounds__(256) dequantise_kernel(const cb_weights4 w, void* out, int dtype, long long ld,
                                                          int wide) {
-  const long long chunks = chunks_of(w.inputs);
+  const int chunks = static_cast<int>(chunks_of(w.inputs));
   const long long block = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (block >= tiles_of(w.outputs) * chunks) return;
-  const int lane = threadIdx.x & 31;
-  const long long tile = block / chunks, chunk = block % chunks;
+  const int lane = threadIdx.x & 31, g = lane / 4, c = lane % 4;
+  const int tile = static_cast<int>(static_cast<unsigned>(block) / static_cast<unsigned>(chunks));
+  const int chunk = static_cast<int>(block) - tile * chunks;
   const uint4 w4 = __ldcs(static_cast<const uint4*>(w.codes) + block * 32 + lane);
   const uint32_t words[4] = {w4.x, w4.y, w4.z, w4.w};
-  const uint16_t* scales = static_cast<const uint16_t*>(w.scales);
+  const uint32_t* from = static_cast<const uint32_t*>(w.scales) + tile * tile_scales(w.inputs, GROUP) / 2;
+  uint32_t both[2];
+  if (GROUP == 32) {
+    const uint2 two = __ldg(reinterpret_cast<const uint2*>(from) + chunk * 8LL + g);
+    both[0] = two.x;
+    both[1] = two.y;
+  } else {
+    both[0] = both[1] = __ldg(from + (GROUP == 128 ? chunk / 2 : chunk) * 8LL + g);
+  }
+  const long long k = chunk * 64LL + c * 8, n = tile * 16LL + g;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const long long k = chunk * 64 + half * 32 + lane % 4 * 8;
-    if (k >= w.inputs) break;
+    if (k + half * 32 >= w.inputs) break;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-      const long long n = tile * 16 + lane / 4 + which * 8;
-      if (n >= w.outputs) continue;
-      const float s = scale_of(scales[scale_at(w.inputs, w.group, n, k / w.group)], w.scale_dtype);
+      if (n + which * 8 >= w.outputs) continue;
+      const float s = scale_of(both[half] >> (16 * which) & 0xffffu, w.scale_dtype);
+      // pairs `which` and `which` + 2 of both words: even elements in the low halves
       float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t word = words[2 * half + i / 4];
-        const int pair = i % 4 / 2 * 2 + which;
-        v[i] = (static_cast<float>(word >> (4 * pair + i % 2 * 16) & 15u) - 8.0f) * s;
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t word = words[2 * half + i] >> (4 * which);
+#pragma unroll
+        for (int pair = 0; pair < 2; ++pair) {
+          const uint32_t two = word >> (8 * pair) & 0x000f000fu;
+          v[4 * i + 2 * pair] = (__uint_as_float((two & 0xffffu) | 0x4b000000u) - 8388616.0f) * s;
+          v[4 * i + 2 * pair + 1] = (__uint_as_float(two >> 16 | 0x4b000000u) - 8388616.0f) * s;
+        }
       }
-      const long long at = n * ld + k;
+      const long long at = (n + which * 8) * ld + k + half * 32;
       if (!wide) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) store_from_f32(out, at + i, dtype, v[i]);
       } else if (ITEM == 4) {
-        float4* to = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
-        to[0] = make_float4(v[0], v[1], v[2], v[3]);
-        to[1] = make_float4(v[4], v[5], v[6], v[7]);
+        float* to = static_cast<float*>(out) + at;
+        __stcs(reinterpret_cast<float4*>(to), make_float4(v[0], v[1], v[2], v[3]));
+        __stcs(reinterpret_cast<float4*>(to) + 1, make_float4(v[4], v[5], v[6], v[7]));
       } else {
         uint32_t h[4];
 #pragma unroll
@@ -369,7 +384,7 @@ __global__ void __launch_bounds__(256) dequantise_kernel(const cb_weights4 w, vo
             h[i] = *reinterpret_cast<const uint32_t*>(&b);
           }
         }
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) = make_uint4(h[0], h[1], h[2], h[3]);
+        __stcs(reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at), make_uint4(h[0], h[1], h[2], h[3]));
       }
     }
   }
@@ -497,8 +512,13 @@ int cb_weights4_dequantise(const cb_weights4* weights, void* out, int dtype, lon
   const int wide = reinterpret_cast<uintptr_t>(out) % 16 == 0 && ld * item % 16 == 0;
   const unsigned blocks = static_cast<unsigned>((tiles_of(w.outputs) * chunks_of(w.inputs) + 7) / 8);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (item == 4) dequantise_kernel<4><<<blocks, 256, 0, s>>>(w, out, dtype, ld, wide);
-  else dequantise_kernel<2><<<blocks, 256, 0, s>>>(w, out, dtype, ld, wide);
+  auto go = [&](auto group) {
+    if (item == 4) dequantise_kernel<group.value, 4><<<blocks, 256, 0, s>>>(w, out, dtype, ld, wide);
+    else dequantise_kernel<group.value, 2><<<blocks, 256, 0, s>>>(w, out, dtype, ld, wide);
+  };
+  if (w.group == 32) go(std::integral_constant<int, 32>{});
+  else if (w.group == 64) go(std::integral_constant<int, 64>{});
+  else go(std::integral_constant<int, 128>{});
   return check_launch("cb_weights4_dequantise");
 }
 
@@ -546,18 +566,27 @@ int cb_linear4(const cb_linear4_args* args, void* scratch, cb_stream_t stream) {
   return with_columns((p.per * p.parts + 7) / 8, [&](auto columns) {
     constexpr int C = columns.value;
     const long long tiles = tiles_of(a.weights.outputs);
-    auto go = [&](auto group, auto count) {
-      constexpr int T = count.value;
+    auto go = [&](auto group, auto count, auto resident) {
+      constexpr int T = count.value, RESIDENT = resident.value;
       const dim3 grid(static_cast<unsigned>((tiles + T - 1) / T), static_cast<unsigned>(launches));
       if (a.dtype == CB_F16)
-        launch(linear_kernel<true, group.value, C, T>, grid, dim3(kThreads), 0, s, true, p);
+        launch(linear_kernel<true, group.value, C, T, RESIDENT>, grid, dim3(kThreads), 0, s, true, p);
       else
-        launch(linear_kernel<false, group.value, C, T>, grid, dim3(kThreads), 0, s, true, p);
+        launch(linear_kernel<false, group.value, C, T, RESIDENT>, grid, dim3(kThreads), 0, s, true, p);
       return check_launch("cb_linear4");
     };
     auto by_tiles = [&](auto group) {
-      return tiles >= kTwoFrom * sm_count() ? go(group, std::integral_constant<int, 2>{})
-                                      : go(group, std::integral_constant<int, 1>{});
+      using one = std::integral_constant<int, 1>;
+      using two = std::integral_constant<int, 2>;
+      using three = std::integral_constant<int, 3>;
+      if constexpr (C > 2) {
+        return go(group, one{}, two{});
+      } else {
+        const long long all = tiles * launches;
+        if (all >= 1LL * kTwoFrom * sm_count()) return go(group, two{}, std::integral_constant<int, C == 1 ? 3 : 2>{});
+        if (C == 1 && all > 1LL * kFewTo * sm_count()) return go(group, one{}, std::integral_constant<int, C == 1 ? 4 : 3>{});
+        return go(group, one{}, three{});
+      }
     };
     if (a.weights.group == 32) return by_tiles(std::integral_constant<int, 32>{});
     if (a.weights.group == 64) return by_tiles(std::integral_constant<int, 64>{});
