@@ -23,7 +23,7 @@ from . import _lib
 from .paged import _VALUES, Prepared, current_stream, no_grad_needed, require, signature, tensor_of
 
 _INDICES = {torch.int32: _lib.I32, torch.int64: _lib.I64}
-MAX_BIASES = 1024
+MAX_BIASES, MAX_HISTORY = 1023, 2 ** 20 - 1
 _ADJUST_ARGS = Prepared()
 
 
@@ -33,7 +33,7 @@ def adjust(logits: Any, *, tokens: Any = None, lengths: Any = None, prompts: Any
            out: Optional[torch.Tensor] = None, error_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The rows of ``logits`` (rows, vocab) with penalties, biases and a mask applied, in that order.
 
-    ``tokens`` (rows, n) int32 or int64 is each row's history, of which
+    ``tokens`` (rows, n) int32 or int64, n < 2**20, is each row's history, of which
     ``lengths[row]`` tokens count (all without) and the first ``prompts[row]``
     were given rather than made (none without); both int32.  With c the times
     that a token is among them and d those from ``prompts[row]`` on, its logit is
@@ -42,7 +42,7 @@ def adjust(logits: Any, *, tokens: Any = None, lengths: Any = None, prompts: Any
     three is a number or a float32 tensor (rows).
 
     ``bias`` (rows, m) float32 is added to the logits of ``bias_tokens`` (rows,
-    m) int32 or int64, at most 1024 to a row; a token that is listed twice gets
+    m) int32 or int64, at most 1023 to a row; a token that is listed twice gets
     both.  Tokens outside the vocabulary are passed over in both lists, so a -1
     pads them.  ``allowed`` (rows, ceil(vocab / 32)) int32 holds a bit for each
     token, the lowest first: a token whose bit is clear becomes -inf, and a row
@@ -110,6 +110,8 @@ def _prepare(logits: torch.Tensor, out: torch.Tensor, values, numbers,
         raise ValueError(f"logits are on {device}, expected a CUDA device")
     require(logits, "logits", device, tuple(_VALUES), (None, None), 1)
     rows, vocab = logits.shape
+    if vocab >= 2 ** 30:
+        raise ValueError(f"a vocabulary of {vocab} tokens, fewer than 2**30 are taken")
     require(out, "out", device, (logits.dtype,), (rows, vocab), 1)
     if rows > 1 and vocab and abs(out.stride(0)) < vocab:
         raise ValueError("the rows of out share memory")
@@ -118,6 +120,8 @@ def _prepare(logits: torch.Tensor, out: torch.Tensor, values, numbers,
     if "tokens" in values:
         tokens = values["tokens"]
         require(tokens, "tokens", device, tuple(_INDICES), (rows, None), 1)
+        if tokens.shape[1] > MAX_HISTORY:
+            raise ValueError(f"a history of {tokens.shape[1]} tokens, at most {MAX_HISTORY} are taken")
         a.token_dtype, a.history, a.token_ld = _INDICES[tokens.dtype], tokens.shape[1], tokens.stride(0)
     for name, number, neutral in zip(_FIELDS, numbers, (1.0, 0.0, 0.0)):
         if name in values:

@@ -831,7 +831,7 @@ typedef struct {
   long long out_ld;
   const void* tokens; /* optional history: rows of token_ld elements, CB_I32 or CB_I64 */
   int token_dtype;
-  long long history, token_ld;
+  long long history, token_ld; /* fewer than 2^20 tokens */
   const int* lengths; /* optional, one for each row: history without */
   const int* prompts; /* optional, one for each row: 0 without */
   const float *repetitions, *frequencies, *presences; /* optional, one for each row */
@@ -839,7 +839,7 @@ typedef struct {
   const void* bias_tokens; /* rows of bias_token_ld elements, CB_I32 or CB_I64 */
   int bias_token_dtype;
   const float* bias; /* rows of bias_ld elements */
-  long long biases, bias_token_ld, bias_ld; /* at most 1024 to a row */
+  long long biases, bias_token_ld, bias_ld; /* at most 1023 to a row */
   const int* allowed; /* optional: rows of allowed_ld words, ceil(vocab / 32) of them used */
   long long allowed_ld;
   int* error_flag; /* optional */

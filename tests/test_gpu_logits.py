@@ -85,7 +85,7 @@ def test_everything_together(dtype, vocab):
     close(operators.adjust(x, **call), wide(x), given)
 
 
-@pytest.mark.parametrize("what", [{}, {"history": 1}, {"history": 1500}, {"biases": 1}, {"biases": 1024},
+@pytest.mark.parametrize("what", [{}, {"history": 1}, {"history": 1500}, {"biases": 1}, {"biases": 1023},
                                   {"grammar": True}, {"history": 40, "grammar": True}, {"history": 9, "biases": 700}])
 def test_one_at_a_time(what):
     rng = np.random.default_rng(len(str(what)))
@@ -207,8 +207,8 @@ def test_refusals():
            dict(bias_tokens=tokens), dict(bias_tokens=tokens, bias=bias[:, :2]),
            dict(allowed=torch.zeros(4, 3, dtype=torch.int32, device="cuda")), dict(out=x[:, 1:]),
            dict(out=torch.zeros(64, device="cuda").expand(4, 64)), dict(tokens=tokens.cpu()),
-           dict(bias_tokens=torch.zeros(4, 1025, dtype=torch.int32, device="cuda"),
-                bias=torch.zeros(4, 1025, device="cuda"))]
+           dict(bias_tokens=torch.zeros(4, 1024, dtype=torch.int32, device="cuda"),
+                bias=torch.zeros(4, 1024, device="cuda"))]
     for call in bad:
         with pytest.raises(ValueError):
             operators.adjust(x, **call)

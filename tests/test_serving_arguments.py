@@ -25,11 +25,11 @@ def adjust(**changes):
     _lib.call("cb_adjust_logits", ctypes.byref(a), None)
 
 
-@pytest.mark.parametrize("change", [dict(dtype=_lib.I32), dict(rows=-1), dict(vocab=2 ** 31), dict(logits=None),
+@pytest.mark.parametrize("change", [dict(dtype=_lib.I32), dict(rows=-1), dict(vocab=2 ** 30), dict(logits=None),
                                     dict(out=None), dict(out=18), dict(tokens=16, token_dtype=_lib.F32, history=2),
-                                    dict(history=2), dict(biases=1025), dict(biases=1), dict(history=-1),
+                                    dict(history=2), dict(tokens=16, token_dtype=_lib.I32, history=2 ** 20), dict(biases=1024), dict(biases=1), dict(history=-1),
                                     dict(biases=2, bias=16, bias_tokens=16, bias_token_dtype=_lib.BF16),
-                                    dict(rows=2 ** 31 - 1, vocab=2 ** 31 - 1)])
+                                    dict(rows=2 ** 31 - 1, vocab=2 ** 30 - 1)])
 def test_adjust_refusals(change):
     with pytest.raises(_lib.KernelError):
         adjust(**change)
