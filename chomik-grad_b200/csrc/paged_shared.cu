@@ -448,10 +448,12 @@ __device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* 
 // in paged_attention.cuh: what multiplies the value codes is 2^(y - c), y a key's
 // score plus the logarithm of its value scale.  A tile whose largest is more
 // than kRise above c or `fall` below it moves c to kRest below it: it is rounded to
-// 2^-24 of 2^(y - c), so the largest of every tile keeps 9 bits, of two parts
-// (float32) 22.  Moving takes a pass over the sums; the wide range makes it rare.
+// 2^-24 of 2^(y - c), so the largest of every tile keeps 11 bits, and those 2^5 below it,
+// of two parts (float32) 22.  Moving takes a pass over the sums (2000 cycles); the range
+// makes it rare (rises of 15 and falls of 6: most tiles of some row, 137 us for 64
+// samples of 16384 keys; falls of 8 or 15: the same 81 us).
 constexpr float kRise = 15.0f, kRest = 2.0f, kFarBelow = 60.0f, kHeld = 1.2676506002282294e30f;  // 2^100
-__host__ __device__ constexpr float fall_of(bool lo) { return lo ? 2.0f : 15.0f; }
+__host__ __device__ constexpr float fall_of(bool lo) { return lo ? 2.0f : 8.0f; }
 
 // Two float32 numbers in a 64-bit register, for the instructions that take both.
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
@@ -514,6 +516,13 @@ __device__ __forceinline__ float exponentials(float* x, float by, float shift) {
   float a, b;
   split_pair(add2(run[0], run[1]), a, b);
   return a + b;
+}
+
+// 2^a, also where it is below the least normal number: a row's sum of weights is
+// against a reference that holds the value scale, up to 2^127, and keeps what is far
+// below its largest.
+__device__ __forceinline__ float weight_of(float a) {
+  return a < 0.0f ? exp2_of(a + 64.0f) * 5.421010862427522e-20f : exp2_of(a);  // 2^-64
 }
 
 // Sixteen weights as fp16, and what is left of them.
@@ -683,9 +692,10 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
             if (fmaxf(sum, l) * exp2_of(c - now) > kHeld) now = c;
           }
           if (!first) {
-            const float scale = exp2_of(c - now);
-            l *= scale;
-            sum *= scale;
+            // (in two steps: the sum of the weights may be large while c falls by more than 126)
+            const float first_step = rintf(0.5f * (c - now)), by0 = exp2_of(first_step), by1 = exp2_of(c - now - first_step);
+            l = l * by0 * by1;
+            sum = sum * by0 * by1;
             if (!wait_warp(sync.value_done[set] + (buffer ^ 1), static_cast<uint32_t>((iteration - 1) / 2 & 1), abort))
               return false;
             tc::fence_after();
@@ -697,7 +707,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
               for (int i = 0; i < 32; i += 8) {
                 uint32_t v[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = __float_as_uint(o[i + k] * scale);
+                for (int k = 0; k < 8; ++k) v[k] = __float_as_uint(o[i + k] * by0 * by1);
                 store8(sums + d + i, v);
               }
             }
@@ -711,7 +721,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
           if (__builtin_expect(far, 0)) {
 #pragma unroll
             for (int k = 0; k < kSharedTile; ++k)
-              l += inverse[k / 16] != 0.0f ? exp2_of(fmaf(s[k], by[k / 16], -c)) : 0.0f;
+              l += inverse[k / 16] != 0.0f ? weight_of(fmaf(s[k], by[k / 16], -c)) : 0.0f;
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -729,7 +739,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               const float score = x[k] * by_i;
-              all += exp2_of(score - c);
+              all += weight_of(score - c);
               x[k] = exp2_of(score + shift);
               sum += x[k];
               x[k] *= kept;
@@ -912,7 +922,7 @@ int shared_check(const cb_paged_attention_args& a) {
   const long long rows = a.batch * a.tokens * (a.heads / a.cache.kv_heads);
   const long long tiles = (a.cache.columns * a.cache.page + kSharedTile - 1) / kSharedTile;
   const double units = static_cast<double>((rows + kRowLanes - 1) / kRowLanes) * a.cache.kv_heads * tiles;
-  CB_REQUIRE(units + (1 << 20) < 2147483648.0 && rows < (1LL << 31) - 2 * kRowLanes,
+  CB_REQUIRE(units + (1 << 20) < 2147483648.0 && a.cache.columns * a.cache.page < (1LL << 31) - 4096 && rows < (1LL << 31) - 2 * kRowLanes,
              "cb_paged_attention_shared: %lld rows of up to %lld keys are too many for one call", rows,
              a.cache.columns * a.cache.page);
   return CB_OK;

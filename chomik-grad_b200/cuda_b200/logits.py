@@ -54,42 +54,53 @@ def adjust(logits: Any, *, tokens: Any = None, lengths: Any = None, prompts: Any
     its ends and set ``error_flag`` (an int32 of the caller's, read with
     ``speculative.check``).
     """
-    logits = tensor_of(logits)
-    given = {"tokens": tokens, "lengths": lengths, "prompts": prompts, "repetition": repetition,
-             "frequency": frequency, "presence": presence, "bias_tokens": bias_tokens, "bias": bias,
-             "allowed": allowed}
-    numbers = []
-    for name in ("repetition", "frequency", "presence"):
-        if isinstance(given[name], (int, float)):
-            numbers.append(float(given[name]))
-            given[name] = None
-        else:
+    if type(logits) is not torch.Tensor:
+        logits = tensor_of(logits)
+    numbers, pointers, values, key = [], [], {}, [signature(logits), signature(error_flag)]
+    for name, value in (("repetition", repetition), ("frequency", frequency), ("presence", presence),
+                        ("bias", bias), ("tokens", tokens), ("lengths", lengths), ("prompts", prompts),
+                        ("bias_tokens", bias_tokens), ("allowed", allowed)):
+        if name in _FIELDS and isinstance(value, (int, float)):
+            numbers.append(float(value))
+            continue
+        if value is None and name not in _FIELDS:
+            continue
+        if type(value) is not torch.Tensor:
+            value = tensor_of(value)
+        if name in _FIELDS:
             numbers.append(None)
-    values = {name: tensor_of(value) for name, value in given.items() if value is not None}
-    no_grad_needed(logits, *(v for v in values.values() if v.is_floating_point()))
-    if out is None:
+        values[name] = value
+        key.append(name)
+        key.append(signature(value))
+        pointers.append((_FIELDS.get(name, name), value.data_ptr()))
+    no_grad_needed(logits, *(values[name] for name in _FLOATS if name in values))
+    fresh = out is None
+    if fresh:
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     else:
         no_grad_needed(out)
-    key = (signature(logits), signature(out), *numbers, signature(error_flag),
-           *((name, signature(v)) for name, v in values.items()))
+        key.append(signature(out))
+    key.extend(numbers)
+    key = tuple(key)
     known = _ADJUST_ARGS.get(key)
     if known is None:
         known = _ADJUST_ARGS[key] = _prepare(logits, out, values, numbers, error_flag)
-    apart(logits, out)
     stream = current_stream(logits.device)
-    if not out.is_inference():  # a backward pass that kept what it held notices
-        torch.autograd.graph.increment_version(out)
+    if not fresh:
+        apart(logits, out)
+        if not out.is_inference():  # a backward pass that kept what it held notices
+            torch.autograd.graph.increment_version(out)
     a = _lib.AdjustArgs.from_buffer_copy(known)
     a.logits, a.out = logits.data_ptr(), out.data_ptr()
-    for name, value in values.items():
-        setattr(a, _FIELDS.get(name, name), value.data_ptr())
+    for name, pointer in pointers:
+        setattr(a, name, pointer)
     if error_flag is not None:
         a.error_flag = error_flag.data_ptr()
     _lib.check(_lib.load().cb_adjust_logits(ctypes.byref(a), stream), "cb_adjust_logits")
     return out
 
 
+_FLOATS = ("repetition", "frequency", "presence", "bias")
 _FIELDS = {"repetition": "repetitions", "frequency": "frequencies", "presence": "presences"}
 
 

@@ -309,11 +309,9 @@ class PagedCache:
         its own.  Any sequences may be given, and a cache whose tables cannot hold that
         much is read as by ``attend``.
 
-        Queries and weights of these keys go to the tensor cores as fp16 with float32
-        sums, of float32 queries in two parts (22 bits).  Within 64 keys, one whose
-        weight is below 2^-9 (float32: 2^-22) of the largest of them may be rounded
-        to that, and one below 2^-10 (2^-23) of it left out, where another tile's
-        is 2^15 (2^2) times larger still.
+        Queries and weights of these keys go to the tensor cores as fp16 (11 bits)
+        with float32 sums, of float32 queries in two parts (22 bits).  Of 64 keys, one whose
+        weight is below 2^-17 (float32: 2^-23) of the largest of them may be left out.
         """
         return self._attend(layer, q, counts, sequences, scale, out, int(least_bytes))
 
