@@ -442,6 +442,8 @@ int weights_and_pools_check(const cb_weights4& w, const char* who) {
   return CB_OK;
 }
 
+bool on_its_type(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype == CB_F32 ? 4 : 2) == 0; }
+
 bool needs_arranging(const cb_linear4_args& a) {
   return a.dtype == CB_F32 || reinterpret_cast<uintptr_t>(a.x) % 16 != 0 || (a.rows > 1 && a.ld % 8 != 0);
 }
@@ -480,6 +482,8 @@ int cb_weights4_quantise(const cb_weights4* weights, const void* weight, int dty
   CB_REQUIRE(dtype == CB_F32 || dtype == CB_BF16 || dtype == CB_F16,
              "cb_weights4_quantise: weights must be float32, bfloat16 or float16");
   CB_REQUIRE(weight != nullptr && codes != nullptr && scales != nullptr, "cb_weights4_quantise: a null pointer");
+  CB_REQUIRE(on_its_type(weight, dtype) && on_its_type(scales, w.scale_dtype),
+             "cb_weights4_quantise: weight and scales must be aligned to their types");
   const long long blocks = (w.outputs * (w.inputs / w.group) + 7) / 8;
   CB_REQUIRE(blocks < (1LL << 31), "cb_weights4_quantise: %lld outputs of %lld inputs", w.outputs, w.inputs);
   quantise_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
@@ -493,6 +497,7 @@ int cb_weights4_pack(const cb_weights4* weights, const void* codes, const void* 
   const int status = weights_and_pools_check(w, "cb_weights4_pack");
   if (status != CB_OK) return status;
   CB_REQUIRE(codes != nullptr && scales != nullptr, "cb_weights4_pack: a null pointer");
+  CB_REQUIRE(on_its_type(scales, w.scale_dtype), "cb_weights4_pack: scales must be aligned to their type");
   const long long blocks = (tiles_of(w.outputs) * chunks_of(w.inputs) * 128 + 255) / 256;
   CB_REQUIRE(blocks < (1LL << 31), "cb_weights4_pack: %lld outputs of %lld inputs", w.outputs, w.inputs);
   pack_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
@@ -508,6 +513,7 @@ int cb_weights4_dequantise(const cb_weights4* weights, void* out, int dtype, lon
   CB_REQUIRE(dtype == CB_F32 || dtype == CB_BF16 || dtype == CB_F16,
              "cb_weights4_dequantise: out must be float32, bfloat16 or float16");
   CB_REQUIRE(out != nullptr && ld >= w.inputs, "cb_weights4_dequantise: rows of %lld elements", ld);
+  CB_REQUIRE(on_its_type(out, dtype), "cb_weights4_dequantise: out must be aligned to its type");
   const int item = dtype == CB_F32 ? 4 : 2;
   const int wide = reinterpret_cast<uintptr_t>(out) % 16 == 0 && ld * item % 16 == 0;
   const unsigned blocks = static_cast<unsigned>((tiles_of(w.outputs) * chunks_of(w.inputs) + 7) / 8);
@@ -537,6 +543,8 @@ int cb_linear4(const cb_linear4_args* args, void* scratch, cb_stream_t stream) {
   CB_REQUIRE(a.rows >= 0 && a.rows < (1LL << 24), "cb_linear4: %lld rows", a.rows);
   if (a.rows == 0) return CB_OK;
   CB_REQUIRE(a.x != nullptr && a.out != nullptr, "cb_linear4: a null pointer");
+  CB_REQUIRE(on_its_type(a.x, a.dtype) && on_its_type(a.out, a.dtype),
+             "cb_linear4: x and out must be aligned to their type");
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   LinearPlan p = {};
   p.w = a.weights;

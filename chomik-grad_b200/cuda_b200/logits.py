@@ -20,7 +20,7 @@ from typing import Any, Optional, Union
 import torch
 
 from . import _lib
-from .paged import _VALUES, Prepared, current_stream, no_grad_needed, require, signature, tensor_of
+from .paged import _VALUES, Prepared, current_stream, no_grad_needed, overlap, require, signature, tensor_of
 
 _INDICES = {torch.int32: _lib.I32, torch.int64: _lib.I64}
 MAX_BIASES, MAX_HISTORY = 1023, 2 ** 20 - 1
@@ -106,11 +106,9 @@ _FIELDS = {"repetition": "repetitions", "frequency": "frequencies", "presence": 
 
 def apart(logits: torch.Tensor, out: torch.Tensor) -> None:
     """Refuse an ``out`` that shares part of its memory with ``logits``: it is the same rows, or none of them."""
-    begin, other = logits.data_ptr(), out.data_ptr()
-    if begin == other and (logits.stride(0) == out.stride(0) or logits.shape[0] <= 1):
+    if logits.data_ptr() == out.data_ptr() and (logits.stride(0) == out.stride(0) or logits.shape[0] <= 1):
         return
-    size = [(t.shape[0] - 1) * t.stride(0) + t.shape[1] if t.numel() else 0 for t in (logits, out)]
-    if begin < other + size[1] * out.element_size() and other < begin + size[0] * logits.element_size():
+    if overlap(logits, out):
         raise ValueError("out has to be logits itself, or memory of its own")
 
 
@@ -137,9 +135,11 @@ def _prepare(logits: torch.Tensor, out: torch.Tensor, values, numbers,
     for name, number, neutral in zip(_FIELDS, numbers, (1.0, 0.0, 0.0)):
         if name in values:
             require(values[name], name, device, (torch.float32,), (rows,), 1)
-        elif not math.isfinite(number) or (name == "repetition" and number <= 0.0):
-            raise ValueError(f"{name} is {number}, expected a finite number"
-                             + (" above 0" if name == "repetition" else ""))
+        else:
+            single = ctypes.c_float(number).value  # as the kernel has it
+            if not math.isfinite(single) or (name == "repetition" and single <= 0.0):
+                raise ValueError(f"{name} is {number}, expected a finite float32"
+                                 + (" above 0" if name == "repetition" else ""))
         if "tokens" not in values and (name in values or number != neutral):
             raise ValueError(f"{name} needs the tokens of a history")
     a.repetition, a.frequency, a.presence = (0.0 if n is None else n for n in numbers)

@@ -101,6 +101,13 @@ def current_stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the spans of memory that ``a`` and ``b`` reach over meet."""
+    ends = [t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+            for t in (a, b)]
+    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < ends[1] and b.data_ptr() < ends[0]
+
+
 def signature(value: Optional[torch.Tensor]):
     """What the checks of an argument look at: equal signatures pass or fail alike."""
     return None if value is None else (value.shape, value.stride(), value.dtype, value.device)

@@ -22,7 +22,7 @@ from typing import Any, Optional
 import torch
 
 from . import _lib
-from .paged import _VALUES, Prepared, aligned, current_stream, no_grad_needed, require, signature, tensor_of
+from .paged import _VALUES, Prepared, aligned, current_stream, no_grad_needed, overlap, require, signature, tensor_of
 
 GROUPS = (32, 64, 128)
 _SCALES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
@@ -82,7 +82,7 @@ class Weights4:
 
         A group's scale is its largest magnitude / 7, rounded to the type
         ``scales``; codes are rounded to the nearest.  The products of a group that
-        holds an infinity or a NaN are NaN.
+        holds an infinity or a NaN, or whose scale is beyond the type, are NaN.
         """
         return cls.pack(*quantise(weight, group=group, scales=scales))
 
@@ -99,8 +99,8 @@ class Weights4:
         Products are exact and sums float32.  Up to 8 rows cost about what one
         costs; every 32 rows (10 of float32) read the weights again, so a prompt's rows
         are better multiplied with ``dequantise``'s.  float32 rows, and 16-bit rows
-        that do not begin on 16 bytes, are first copied to a workspace.  ``out`` may
-        not overlap x.
+        that do not begin on 16 bytes, are first copied to a workspace.  ``out`` is
+        contiguous and shares no memory with x.
         """
         x = tensor_of(x)
         no_grad_needed(x)
@@ -113,6 +113,8 @@ class Weights4:
             out = x.new_empty(shape)
         else:
             require(out, "out", self.device, (x.dtype,), shape, len(shape))
+            if overlap(out, x):
+                raise ValueError("out shares memory with x")
             no_grad_needed(out)
             if not out.is_inference():  # a backward pass that kept what it held notices
                 torch.autograd.graph.increment_version(out)

@@ -10,6 +10,7 @@ import torch
 
 import test_abi
 from cuda_b200 import _lib, logits, quantized
+from cuda_b200.paged import overlap
 
 
 def test_structures_match_the_header(tmp_path, monkeypatch):
@@ -165,3 +166,23 @@ def test_shared_calls_with_too_much_work():
         shared(cache(columns=2 ** 26), batch=65535, tokens=64)
     shared(cache(), batch=0)
     shared(cache(), tokens=0)
+
+
+def test_alignment():
+    """Values that do not lie on multiples of their type."""
+    ref, w = ctypes.byref, weights()
+    for change in (dict(x=17), dict(out=17), dict(out=18, dtype=_lib.F32)):
+        with pytest.raises(_lib.KernelError, match="aligned"):
+            linear(**change)
+    for name, args in (("cb_weights4_quantise", (18, _lib.F32, 128, 16, 16)),
+                       ("cb_weights4_quantise", (16, _lib.F32, 128, 16, 17)), ("cb_weights4_pack", (16, 17)),
+                       ("cb_weights4_dequantise", (18, _lib.F32, 128))):
+        with pytest.raises(_lib.KernelError, match="aligned"):
+            _lib.call(name, ref(w), *args, None)
+
+
+def test_overlap():
+    room = torch.zeros(4, 64)
+    assert overlap(room, room[3, 63:]) and overlap(room[:2], room[1:])
+    assert not overlap(room[:2], room[2:]) and not overlap(room, room[:0])
+    assert overlap(room[:, :8], room[:, 8:])  # (spans, not elements)
