@@ -5,6 +5,28 @@
 // the same pages from their beginning on; what they all hold is read and
 // multiplied once, with the rows of all sequences together, and each
 // sequence's own keys by cb_paged_attention's kernel, which joins both.
+//
+// For row r (a sequence's query, one of a kv head's group) and the keys j of P, the
+// common pages, and T, the sequence's own:
+//   y_j = scale log2(e) ks_j (q_r . kq_j) + log2 vs_j
+//   O = sum_j 2^(y_j - c) vq_j,  l = sum_j 2^(y_j - c) / vs_j    over P, and over T
+//   out = (2^(c_P - m) O_P + 2^(c_T - m) O_T) / (2^(c_P - m) l_P + 2^(c_T - m) l_T)
+// Whether a value scale is part of the weight or of the values is a matter of
+// notation, so O needs no scaled copy of the codes.
+//
+// What bounds it: with R rows to a key the products are 2 R flops a byte (64 samples
+// of 4 rows to a kv head, or 16 blocks of 20: 256 and 320 rows), so they go to
+// tcgen05: 128-row products of fp16 (codes are exact in it) with float32 sums in
+// tensor memory.  A tile of 64 keys of 128 elements then takes a set of 128 rows 640
+// cycles on the tensor cores (scores 8 x 48, values 4 x 64), but 8192 exponentials with their
+// conversions about 1700 cycles on the four schedulers: that, and the hand-offs
+// between warps that it delays, is what is left (2600 to 2900 cycles a tile of two
+// sets; 64 samples of 16384 keys 81 us on the device, 16 blocks of 5 tokens at 32700
+// keys 150; by cb_paged_attention, each sequence for itself, 351 and 292).
+//
+// Three launches, each begun while the one before ends: the common pages of each
+// sequence; the shared keys, a block to an SM, whose warps are divided by what they
+// do (two sets of 128 rows share a tile of keys and values, 20 warps); the tails.
 #include <type_traits>
 
 #include "paged_attention.cuh"
@@ -806,6 +828,8 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
   char* tiles = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(memory) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
+  // (all of the tensor memory, before the kernels ahead have ended: none of theirs that
+  // takes some fits an SM beside this block's shared memory)
   if (warp == kIssueWarp) tc::tmem_alloc(&sync.tmem, kColumns);
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {

@@ -11,8 +11,8 @@ instantiates it.  After that, the reference's graphs select it by name::
                                        dynamic_inputs=...)
 
 The plugin has no front-end of its own: its graphs need an importable
-``chomikgrad``.  The serving operators (``paged``, ``speculative``) and the C
-binding (``_lib``) take tensors, so without it the package still imports, with
+``chomikgrad``.  The serving operators (``paged``, ``speculative``,
+``logits``, ``quantized``) and the C binding (``_lib``) take tensors, so without it the package still imports, with
 nothing registered, and ``install`` raises.
 """
 
