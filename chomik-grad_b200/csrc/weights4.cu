@@ -18,10 +18,9 @@
 // product: word s of lane (g, c) holds inputs k = 32 (s / 2) + 8 c + 4 (s % 2) + 0 .. 3
 // of both rows.  Lane (g, c) so needs x[g][32 h + 8 c + 0 .. 7], 16 neighbouring bytes,
 // which come straight from L1: no staging, no barrier before the products.  Measured:
-// 16 rows by 4096 x 128256, 91 us (3.0 TB/s: 16 warps an SM do not cover the loads of
-// x and the conversions, issue slots 45%, L1 52%), one row 60.6 (4.5 TB/s); one row by
-// 4096 x 14336 9.8, by 2048 x 2048 2.9, of which about 2.5 are the launch and one
-// chain of loads, products and sums.  Code
+// 16 rows by 4096 x 128256, 77 us (3.6 TB/s: 16 warps an SM do not cover the loads of
+// x and the conversions), one row 55 (5.0 TB/s); one row by 4096 x 14336 8.9, by 2048 x
+// 2048 2.2, a launch and one chain of loads, products and sums.  Code
 // q + 8 of pair i (row g, inputs 0 and 1; row g + 8, the same; row g, inputs 2 and
 // 3; row g + 8) is nibbles i and i + 4: one logic instruction makes two operands of
 // them (see halves_of).
@@ -32,16 +31,7 @@
 namespace cb {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = 32 * kWarps;
 constexpr int kBlockBytes = 512;   // 16 outputs x 64 inputs
-// Tiles to an SM: up to kFewTo one wave of blocks with 80 registers, whose loads reach
-// further ahead (256 tiles of 14336 inputs 11.4 us, with 64 registers 15.0); above, four
-// blocks an SM (896 tiles of 4096 inputs 9.9 us, three 12.5); from kTwoFrom on a block
-// takes two tiles, which share the rows of x (8016 tiles: 60.6 us and 64.2 for one
-// row, 91 and 110 for 16; of more columns than two the sums do not fit the
-// registers: 32 rows 35 us with two tiles, 31 with one).
-constexpr int kFewTo = 3, kTwoFrom = 16;
 constexpr int kColumnTiles = 4;    // most of 8 columns that a launch's block takes
 
 __host__ __device__ constexpr long long tiles_of(long long outputs) { return (outputs + 15) / 16; }
@@ -183,13 +173,13 @@ __device__ __forceinline__ void multiply_units(const Unit<GROUP>* u, const uint1
   }
 }
 
-// A block takes TILES tiles of 16 outputs and `per` rows of y.  Its warps take the
+// A block takes TILES tiles of 16 outputs and `per` rows of y.  Its WARPS warps take the
 // units of the tiles in turn, the loads of the next under way, and are joined in
 // shared memory, in their order.  Columns that no row of x belongs to are computed
 // like row `first` and not stored.
-template <bool HALF, int GROUP, int COLUMNS, int TILES, int RESIDENT>
-__global__ void __launch_bounds__(kThreads, RESIDENT) linear_kernel(const __grid_constant__ LinearPlan p) {
-  __shared__ float sums[kWarps][16 * TILES][8 * COLUMNS + 1];
+template <bool HALF, int GROUP, int COLUMNS, int TILES, int WARPS, int RESIDENT>
+__global__ void __launch_bounds__(32 * WARPS, RESIDENT) linear_kernel(const __grid_constant__ LinearPlan p) {
+  __shared__ float sums[WARPS][16 * TILES][8 * COLUMNS + 1];
   constexpr int kScaleWords = 8 * Unit<GROUP>::kWords;  // of a unit's tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int chunks = static_cast<int>(chunks_of(p.w.inputs)), units = (chunks + 1) / 2;
@@ -234,16 +224,16 @@ __global__ void __launch_bounds__(kThreads, RESIDENT) linear_kernel(const __grid
   };
   load(ring[0], warp);
   int unit = warp;
-  for (; unit < whole; unit += 2 * kWarps) {
+  for (; unit < whole; unit += 2 * WARPS) {
 #pragma unroll
     for (int slot = 0; slot < 2; ++slot) {
-      const int now = unit + slot * kWarps;
+      const int now = unit + slot * WARPS;
       if (now >= whole) break;
-      load(ring[slot ^ 1], now + kWarps);
+      load(ring[slot ^ 1], now + WARPS);
       multiply_units<HALF, GROUP, COLUMNS, TILES, true>(ring[slot], x, now * 128LL, 0, p.w.scale_dtype, total);
     }
   }
-  if (whole < units && whole % kWarps == warp) {  // less than a unit is left
+  if (whole < units && whole % WARPS == warp) {  // less than a unit is left
     const long long k = whole * 128LL;
 #pragma unroll
     for (int n = 0; n < TILES; ++n) {
@@ -261,12 +251,12 @@ __global__ void __launch_bounds__(kThreads, RESIDENT) linear_kernel(const __grid
 #pragma unroll
       for (int i = 0; i < 4; ++i) sums[warp][n * 16 + g + i / 2 * 8][t * 8 + 2 * c + i % 2] = total[n][t][i];
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * TILES * mine; i += kThreads) {
+  for (int i = threadIdx.x; i < 16 * TILES * mine; i += 32 * WARPS) {
     const int n = i % (16 * TILES), r = i / (16 * TILES);
     float y = 0.0f;
     for (int part = 0; part < p.parts; ++part)
 #pragma unroll
-      for (int v = 0; v < kWarps; ++v) y += sums[v][n][part * mine + r];
+      for (int v = 0; v < WARPS; ++v) y += sums[v][n][part * mine + r];
     if (tile * 16 + n < p.w.outputs) store_from_f32(p.out, (first + r) * p.out_ld + tile * 16 + n, p.out_dtype, y);
   }
 }
@@ -453,12 +443,15 @@ bool needs_arranging(const cb_linear4_args& a) {
   return a.dtype == CB_F32 || reinterpret_cast<uintptr_t>(a.x) % 16 != 0 || (a.rows > 1 && a.ld % 8 != 0);
 }
 
+template <int N>
+using is = std::integral_constant<int, N>;
+
 template <typename F>
 int with_columns(int columns, F f) {
-  if (columns <= 1) return f(std::integral_constant<int, 1>{});
-  if (columns == 2) return f(std::integral_constant<int, 2>{});
-  if (columns == 3) return f(std::integral_constant<int, 3>{});
-  return f(std::integral_constant<int, 4>{});
+  if (columns <= 1) return f(is<1>{});
+  if (columns == 2) return f(is<2>{});
+  if (columns == 3) return f(is<3>{});
+  return f(is<4>{});
 }
 
 }  // namespace
@@ -579,31 +572,48 @@ int cb_linear4(const cb_linear4_args* args, void* scratch, cb_stream_t stream) {
   return with_columns((p.per * p.parts + 7) / 8, [&](auto columns) {
     constexpr int C = columns.value;
     const long long tiles = tiles_of(a.weights.outputs);
-    auto go = [&](auto group, auto count, auto resident) {
-      constexpr int T = count.value, RESIDENT = resident.value;
+    // The form of a block: its tiles, its warps, and how many are on an SM.  Few tiles
+    // have many warps each, so that each chain of loads and products is short (tiles of
+    // 5632 inputs on 128 SMs, 15 columns: 16 warps 7.0 us, 8 warps 9.7; 256 tiles of 14336
+    // inputs, one column: 8.9 and 11.4); many have few, which wait for few others (896
+    // tiles of 4096 inputs, one column: 4 warps, 7 blocks an SM 8.9, 8 warps, 4 blocks 9.9),
+    // and from there on two tiles share the rows of x as long as their sums fit the
+    // registers (8016 tiles: one column 55 us and 60 with 8 warps, 16 columns 77 and 91;
+    // one tile to a block 56 and 99).
+    auto go = [&](auto group, auto count, auto warps, auto resident) {
+      constexpr int T = count.value, WARPS = warps.value, RESIDENT = resident.value;
       const dim3 grid(static_cast<unsigned>((tiles + T - 1) / T), static_cast<unsigned>(launches));
       if (a.dtype == CB_F16)
-        launch(linear_kernel<true, group.value, C, T, RESIDENT>, grid, dim3(kThreads), 0, s, true, p);
+        launch(linear_kernel<true, group.value, C, T, WARPS, RESIDENT>, grid, dim3(32 * WARPS), 0, s, true, p);
       else
-        launch(linear_kernel<false, group.value, C, T, RESIDENT>, grid, dim3(kThreads), 0, s, true, p);
+        launch(linear_kernel<false, group.value, C, T, WARPS, RESIDENT>, grid, dim3(32 * WARPS), 0, s, true, p);
       return check_launch("cb_linear4");
     };
     auto by_tiles = [&](auto group) {
-      using one = std::integral_constant<int, 1>;
-      using two = std::integral_constant<int, 2>;
-      using three = std::integral_constant<int, 3>;
-      if constexpr (C > 2) {
-        return go(group, one{}, two{});
+      const long long all = tiles * launches, sms = sm_count();
+      if (all <= sms) return go(group, is<1>{}, is<16>{}, is<1>{});
+      if constexpr (C > 2) {  // (32 rows: 896 tiles 26 us, with 8 warps 30; 256 tiles are not a wave of these)
+        if (all <= 2 * sms) return go(group, is<1>{}, is<8>{}, is<2>{});
+        return go(group, is<1>{}, is<4>{}, is<4>{});
       } else {
-        const long long all = tiles * launches;
-        if (all >= 1LL * kTwoFrom * sm_count()) return go(group, two{}, std::integral_constant<int, C == 1 ? 3 : 2>{});
-        if (C == 1 && all > 1LL * kFewTo * sm_count()) return go(group, one{}, std::integral_constant<int, C == 1 ? 4 : 3>{});
-        return go(group, one{}, three{});
+        if (all <= 2 * sms) return go(group, is<1>{}, is<16>{}, is<2>{});
+        if (all <= 3 * sms) return go(group, is<1>{}, is<8>{}, is<3>{});
+        if constexpr (C == 2) {  // (563 tiles: one to a block 10.0 us, two 12.7; 896 tiles: 18.3 and 13.1)
+          if (all <= 5 * sms) return go(group, is<1>{}, is<4>{}, is<5>{});
+          return go(group, is<2>{}, is<4>{}, is<4>{});
+        } else {
+          if (all <= 4 * sms) return go(group, is<1>{}, is<8>{}, is<4>{});
+          if (all >= 16 * sms) return go(group, is<2>{}, is<4>{}, is<6>{});
+          // seven blocks an SM have more registers, eight may save a wave (1184 tiles of 3584 inputs: 12.1 and
+          // 9.1 us; 896 of 4096: 8.9 and 10.0)
+          const bool saves = (all + 7 * sms - 1) / (7 * sms) > (all + 8 * sms - 1) / (8 * sms);
+          return saves ? form(is<1>{}, is<4>{}, is<8>{}) : go(group, is<1>{}, is<4>{}, is<7>{});
+        }
       }
     };
-    if (a.weights.group == 32) return by_tiles(std::integral_constant<int, 32>{});
-    if (a.weights.group == 64) return by_tiles(std::integral_constant<int, 64>{});
-    return by_tiles(std::integral_constant<int, 128>{});
+    if (a.weights.group == 32) return by_tiles(is<32>{});
+    if (a.weights.group == 64) return by_tiles(is<64>{});
+    return by_tiles(is<128>{});
   });
 }
 

@@ -115,3 +115,24 @@ def test_little_shared_is_attend():
     assert torch.equal(cache.attend_shared(0, q[:1], sequences=[2], least_bytes=0), cache.attend_shared(0, q[:1], sequences=[3],
                                                                                                      least_bytes=0))
     cache.check_errors()
+
+
+@pytest.mark.parametrize("dtype", list(DTYPE.values()))
+@pytest.mark.parametrize("outputs", [2367, 2370, 4750, 7150, 9500, 11900, 16600, 18900, 37900])
+@pytest.mark.parametrize("group, inputs", [(32, 96), (64, 704), (128, 1152)])
+def test_many_outputs(dtype, outputs, group, inputs):
+    """As many tiles of 16 outputs as change a block's form: warps, tiles and blocks an SM.
+
+    A group's products are added within 2^-22 of what its terms add up to for each product of 16 inputs (of three parts
+    for float32); then a warp of at least four adds its groups, and up to 16 warps are joined, each float32.
+    """
+    torch.manual_seed(outputs)
+    weights = quantized.Weights4.quantise(torch.randn(outputs, inputs, device="cuda"), group=group)
+    w = weights.dequantise(torch.float32).double()
+    for rows in (1, 5, 9, 16, 27):
+        x = torch.randn(rows, inputs, device="cuda", dtype=dtype)
+        got = weights.linear(x).double()
+        want, size = x.double() @ w.T, x.double().abs() @ w.abs().T
+        steps = group / 16 * (3 if dtype == torch.float32 else 1)
+        error = (steps * 2.0 ** -22 + (inputs / group / 4 + 20) * 2.0 ** -24) * size
+        assert ((got - want).abs() <= error + torch.finfo(dtype).eps / 2 * (want.abs() + error)).all()
