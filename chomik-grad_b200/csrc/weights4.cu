@@ -607,7 +607,7 @@ int cb_linear4(const cb_linear4_args* args, void* scratch, cb_stream_t stream) {
           // seven blocks an SM have more registers, eight may save a wave (1184 tiles of 3584 inputs: 12.1 and
           // 9.1 us; 896 of 4096: 8.9 and 10.0)
           const bool saves = (all + 7 * sms - 1) / (7 * sms) > (all + 8 * sms - 1) / (8 * sms);
-          return saves ? form(is<1>{}, is<4>{}, is<8>{}) : go(group, is<1>{}, is<4>{}, is<7>{});
+          return saves ? go(group, is<1>{}, is<4>{}, is<8>{}) : go(group, is<1>{}, is<4>{}, is<7>{});
         }
       }
     };
