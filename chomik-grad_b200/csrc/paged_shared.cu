@@ -115,6 +115,10 @@ __host__ __device__ constexpr int weights_at(bool lo, int tile) { return kWeight
 // none), and its scales, of values as log2, 2^-log2 and what the logarithm leaves.
 // They are looked up for eight tiles at a time, a lane to a run.
 constexpr int kBatch = 8, kBatches = 3;
+// Warps that read a batch, and arrive when they have left it: those that weigh and those
+// that convert.  (Neither follows from the other: with one set of rows, whose tiles are
+// weighed by turns, the values may be converted eight tiles behind the scores.)
+constexpr int kBatchReaders = kValueWarp + 4 - kWeighWarp;
 struct __align__(16) Runs {
   long long line[4];
   float key[4], log[4], inverse[4], factor[4];
@@ -383,9 +387,13 @@ __device__ __forceinline__ bool convert(const SharedPlan& p, const SharedWalk& w
       }
       ++next;
       if (++next_tile == w.tiles) next_tile = 0;
-      if (next % kBatch == 0 && ++batch == kBatches) {
-        batch = 0;
-        ++batch_turn;
+      if (next % kBatch == 0) {
+        __syncwarp();  // (every lane has its lines of the batch, which may be looked up anew from here on)
+        if ((threadIdx.x & 31) == 0) mbar_arrive(sync.batch_free + batch);
+        if (++batch == kBatches) {
+          batch = 0;
+          ++batch_turn;
+        }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -840,7 +848,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
     }
     for (int i = 0; i < kBatches; ++i) {
       mbar_init(sync.batch_full + i, 32);
-      mbar_init(sync.batch_free + i, 2 * kSetThreads / 32);
+      mbar_init(sync.batch_free + i, kBatchReaders);
     }
     mbar_init(&sync.query_full, 2 * kSetThreads);
     mbar_init(&sync.query_free, 2);
