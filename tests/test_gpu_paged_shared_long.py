@@ -81,3 +81,43 @@ def test_many_tiles_of_few_rows(dtype, storage, keys):
 def test_many_tiles_of_many_rows(dtype, storage, keys):
     """The same with two sets of rows, the second with a few."""
     run(np.random.default_rng(keys + 1), dtype, storage, keys, [1 + b % 5 for b in range(17)], sms() // 2 + 6, 8)
+
+
+def several(more):
+    """``more`` kv heads than there are SMs (a few blocks take two items), or fewer than twice as many (a few take one)."""
+    return more + sms() * (2 if more < 0 else 1)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPE))
+@pytest.mark.parametrize("storage", ["int8", "e4m3"])
+@pytest.mark.parametrize("keys", [64, 130, 208, 320, 900])
+@pytest.mark.parametrize("more", [13, -9])
+def test_several_items_of_few_rows(dtype, storage, keys, more):
+    """1, 2, 4 (the last of 16 keys), 5 and 14 tiles of each item: one set has fewer tiles than the other or none, and
+    tiles that are looked up together belong to two or more items."""
+    run(np.random.default_rng(keys + more), dtype, storage, keys, [1, 7, 18], several(more), 1)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("storage", ["int8", "e4m3"])
+@pytest.mark.parametrize("keys", [64, 130, 320, 900])
+def test_several_items_of_many_rows(dtype, storage, keys):
+    run(np.random.default_rng(keys), dtype, storage, keys, [1 + b % 4 for b in range(18)], several(13), 8)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPE))
+def test_several_items_of_blocks(dtype):
+    """Items that are blocks of rows as well as heads: 90 sequences of 5 tokens (fewer in some, none in one) on 80 kv
+    heads; 450 rows a head are four blocks of 128, or two of 256."""
+    rng = np.random.default_rng(90)
+    tails = [0 if b == 7 else 5 + b % 3 for b in range(90)]
+    counts = [0 if b == 7 else 5 - b % 4 for b in range(90)]
+    run(rng, dtype, "int8", 700, tails, sms() // 2 + 6, 1, tokens=5, counts=counts)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPE))
+def test_three_items_and_more(dtype):
+    """Five items to a block, of 7 and 25 tiles."""
+    rng = np.random.default_rng(5)
+    for keys in (440, 1600):
+        run(rng, dtype, "e4m3", keys, [1, 3], 4 * sms() + 5, 1)
