@@ -1,0 +1,73 @@
+"""attend_shared where the device decides whether shared keys are computed apart: from ``least_bytes``
+of repeated reads on, counted over the sequences that take part and the whole pages that all of
+them hold, in caches whose tables have room for more."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from paged_helpers import DTYPE, to_device
+from test_gpu_paged_attention import compare, expected, queries
+from test_gpu_paged_shared import family
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", list(DTYPE))
+@pytest.mark.parametrize("storage, page, kv_heads, size, tokens", [("int8", 16, 2, 64, 1), ("e4m3", 64, 1, 128, 3),
+                                                                  ("int8", 32, 3, 32, 5)])
+@pytest.mark.parametrize("idle", [(), (0,), (2, 5)])
+def test_the_border(dtype, storage, page, kv_heads, size, tokens, idle):
+    rng = np.random.default_rng(page + len(idle))
+    prefix, tails = 10 * page + 3, [tokens, tokens + 9, 2 * page, 40, tokens + 1, 70, tokens]
+    host = family(rng, prefix, tails, kv_heads=kv_heads, head_size=size, page=page, storage=storage, room=50)
+    cache = to_device(host)
+    counts = [0 if b in idle else tokens for b in range(len(tails))]
+    given = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    q = queries(rng, len(tails), tokens, 4 * kv_heads, size, dtype)
+
+    def call(least_bytes):
+        got = cache.attend_shared(0, q, counts=given, least_bytes=least_bytes)
+        cache.check_errors()
+        return got
+
+    # ten whole pages are common to all; the first rows of a block see keys of their own from there on
+    border = (len(tails) - len(idle) - 1) * 10 * page * kv_heads * size * 2
+    apart, whole = call(0), cache.attend(0, q, counts=given)
+    want = expected(host, q, counts, range(len(tails)), 1 / math.sqrt(size))
+    compare(apart, want, host, dtype)
+    compare(whole, want, host, dtype)
+    if dtype == "f32":  # (so that equal bits say which way a call went)
+        assert not torch.equal(apart, whole)
+    assert torch.equal(call(border - 1), apart) and torch.equal(call(border), apart)
+    assert torch.equal(call(border + 1), whole)
+    assert torch.equal(call(border + page * kv_heads * size * 2), whole)
+
+
+def test_the_border_follows_the_tables():
+    """The same call before and after a sequence leaves the family, and while one that never belonged takes part."""
+    rng = np.random.default_rng(8)
+    host = family(rng, 320, [1, 1, 1, 1], kv_heads=2, head_size=64, page=16, room=30)
+    q = queries(rng, 4, 1, 8, 64, "f32")
+    cache = to_device(host)
+    unit = 20 * 16 * 2 * 64 * 2  # a repeated read of the twenty pages
+    ones = torch.ones(4, dtype=torch.int32, device="cuda")
+    apart, whole = cache.attend_shared(0, q, least_bytes=0), cache.attend(0, q)
+    assert not torch.equal(apart, whole)
+    assert torch.equal(cache.attend_shared(0, q, least_bytes=3 * unit), apart)
+    ones[3] = 0  # three are left: two repeated reads
+    three = cache.attend_shared(0, q, counts=ones, least_bytes=2 * unit)
+    assert torch.equal(three, cache.attend_shared(0, q, counts=ones, least_bytes=0))
+    assert torch.equal(cache.attend_shared(0, q, counts=ones, least_bytes=2 * unit + 1), cache.attend(0, q, counts=ones))
+    cache.release([3])
+    cache.extend([0, 0, 0, 40])
+    zeros = torch.zeros(1, 40, 2, 64, device="cuda")
+    cache.append(0, zeros, zeros, sequences=[3])
+    cache.check_errors()
+    assert torch.equal(cache.attend_shared(0, q, least_bytes=1), cache.attend(0, q))  # nothing is common to all four
+    assert torch.equal(cache.attend_shared(0, q, counts=ones, least_bytes=2 * unit), three)
+    cache.check_errors()
