@@ -499,6 +499,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
   return v;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t v;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
@@ -509,7 +514,8 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // 512 cycles for a warp's tile, and two warps share it): 2^e = 2^n 2^f with n the
 // nearest whole number to e (added to 1.5 * 2^23, whose low bits it becomes), and 2^f,
 // |f| <= 1/2, by its Taylor polynomial of degree 5: (f ln 2)^6 / 720 < 2.5e-6, a
-// hundredth of the weights' rounding to 11 bits.
+// hundredth of the weights' rounding to 11 bits.  (2^n is multiplied: added to the
+// exponent's bits it would make a number of a NaN.)
 template <bool LO>
 __device__ __forceinline__ float exponentials(float* x, float by, float shift) {
   const uint64_t by2 = pair_of(by, by), shift2 = pair_of(shift, shift);
@@ -535,11 +541,10 @@ __device__ __forceinline__ float exponentials(float* x, float by, float shift) {
       y = fma2(y, f, pair_of(c2, c2));
       y = fma2(y, f, pair_of(c1, c1));
       y = fma2(y, f, pair_of(1.0f, 1.0f));
-      float n0, n1;
-      split_pair(n, n0, n1);
-      split_pair(y, a, b);
-      x[k] = __uint_as_float(__float_as_uint(a) + (__float_as_uint(n0) << 23));
-      x[k + 1] = __uint_as_float(__float_as_uint(b) + (__float_as_uint(n1) << 23));
+      split_pair(n, a, b);
+      const uint64_t power = pair_of(__uint_as_float((__float_as_uint(a) << 23) + 0x3f800000u),
+                                     __uint_as_float((__float_as_uint(b) << 23) + 0x3f800000u));
+      split_pair(mul2(y, power), x[k], x[k + 1]);
     }
     run[k / 2 & 1] = add2(run[k / 2 & 1], pair_of(x[k], x[k + 1]));
   }
