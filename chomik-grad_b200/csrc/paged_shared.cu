@@ -751,12 +751,13 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
         }
         first = false;
         if (__builtin_expect(!irregular, 1)) {
-          // all far below c: the weights by themselves, since 2^(y - c) may not be there
-          const bool far = __any_sync(0xffffffffu, top < c - kFarBelow);
-          if (__builtin_expect(far, 0)) {
+          // all of a row's far below c: its weights by themselves, since 2^(y - c) may not
+          // be there (of that row alone: no bit of a row depends on the rows beside it)
+          const bool far = top < c - kFarBelow;
+          if (__builtin_expect(__any_sync(0xffffffffu, far), 0)) {
 #pragma unroll
             for (int k = 0; k < kSharedTile; ++k)
-              l += inverse[k / 16] != 0.0f ? weight_of(fmaf(s[k], by[k / 16], -c)) : 0.0f;
+              l += far && inverse[k / 16] != 0.0f ? weight_of(fmaf(s[k], by[k / 16], -c)) : 0.0f;
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {

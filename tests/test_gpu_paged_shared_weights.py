@@ -41,3 +41,30 @@ def test_nan_codes(dtype, sequences, larger):
             else:
                 assert torch.isnan(got[..., 7]).all(), row
                 assert torch.equal(got[..., :7], clean[..., :7]) and torch.equal(got[..., 8:], clean[..., 8:])
+
+
+@pytest.mark.parametrize("dtype", list(DTYPE))
+@pytest.mark.parametrize("storage", ["int8", "e4m3"])
+@pytest.mark.parametrize("sequences", [3, 40])
+def test_rows_by_themselves(dtype, storage, sequences):
+    """What the queries past a count hold, and those of other sequences, does not move a bit of a row."""
+    rng = np.random.default_rng(2)
+    tails = [5 + b % 3 for b in range(sequences)]
+    counts = [5 - b % 4 for b in range(sequences)]
+    host = family(rng, 1000, tails, kv_heads=2, head_size=64, storage=storage)
+    cache = to_device(host)
+    given = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    q = queries(rng, sequences, 5, 8, 64, dtype)
+    for b, n in enumerate(counts):
+        q[b, n:] = 0
+    want = cache.attend_shared(0, q, counts=given, least_bytes=0)
+    for size in (3.0, 100.0, 3000.0, math.inf, math.nan):
+        other = q.clone()
+        for b, n in enumerate(counts):
+            other[b, n:] = (size * torch.from_numpy(rng.normal(0, 1, (5 - n, 8, 64)).astype(np.float32))).to(q.dtype).cuda()
+        assert torch.equal(cache.attend_shared(0, other, counts=given, least_bytes=0), want), size
+        other = q.clone()
+        other[1] *= size
+        got = cache.attend_shared(0, other, counts=given, least_bytes=0)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[2:], want[2:]), size
+    cache.check_errors()
