@@ -482,8 +482,13 @@ __device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* 
 // of two parts (float32) 22.  Moving takes a pass over the sums (2000 cycles); the range
 // makes it rare (rises of 15 and falls of 6: most tiles of some row, 137 us for 64
 // samples of 16384 keys; falls of 8 or 15: the same 81 us).
-constexpr float kRise = 15.0f, kRest = 2.0f, kFarBelow = 60.0f, kHeld = 1.2676506002282294e30f;  // 2^100
+// It falls as far as the sums against it stay below 2^kHeldExponent: keys below about
+// 2^-100 of all the weights before them may be lost.
+constexpr float kRise = 15.0f, kRest = 2.0f, kFarBelow = 60.0f;
+constexpr int kHeldExponent = 100;
 __host__ __device__ constexpr float fall_of(bool lo) { return lo ? 2.0f : 8.0f; }
+// e of 2^e <= x < 2^(e + 1); -127 of zero, 128 of infinity and NaN
+__device__ __forceinline__ int exponent_of(float x) { return static_cast<int>(__float_as_uint(x) >> 23) - 127; }
 
 // Two float32 numbers in a 64-bit register, for the instructions that take both.
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
@@ -716,16 +721,15 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
             for (int k = 0; k < 16; ++k) top = fmaxf(top, fmaf(x[k], factor * tile_runs.key[i], tile_runs.log[i]));
           }
         }
-        const bool moves = first || top > c + kRise || top < c - fall_of(LO);
-        if (__any_sync(0xffffffffu, moves)) {
+        float now = c;
+        if (__any_sync(0xffffffffu, first || top > c + kRise || top < c - fall_of(LO))) {
           const float next = floorf(top) - kRest;
-          float now = c;
           if (first) now = top > -INFINITY ? next : 0.0f;
           else if (top > c + kRise) now = next;
-          else if (top < c - fall_of(LO) && top > -INFINITY) {
-            now = fmaxf(next, c - 50.0f);
-            if (fmaxf(sum, l) * exp2_of(c - now) > kHeld) now = c;
-          }
+          else if (top < c - fall_of(LO) && top > -INFINITY)  // (the sums stay below 2^kHeldExponent)
+            now = fmaxf(next, c - static_cast<float>(max(kHeldExponent - 1 - exponent_of(fmaxf(sum, l)), 0)));
+        }
+        if (__any_sync(0xffffffffu, first || now != c)) {
           if (!first) {
             // (in two steps: the sum of the weights may be large while c falls by more than 126)
             const float first_step = rintf(0.5f * (c - now)), by0 = exp2_of(first_step), by1 = exp2_of(c - now - first_step);

@@ -318,7 +318,8 @@ class PagedCache:
 
         Queries and weights of these keys go to the tensor cores as fp16 (11 bits)
         with float32 sums, of float32 queries in two parts (22 bits).  Of 64 keys, one whose
-        weight is below 2^-17 (float32: 2^-23) of the largest of them may be left out.
+        weight is below 2^-17 (float32: 2^-23) of the largest of them, or 2^-90 of the
+        row's, may be left out.
         """
         return self._attend(layer, q, counts, sequences, scale, out, int(least_bytes))
 

@@ -68,3 +68,55 @@ def test_rows_by_themselves(dtype, storage, sequences):
         got = cache.attend_shared(0, other, counts=given, least_bytes=0)
         assert torch.equal(got[0], want[0]) and torch.equal(got[2:], want[2:]), size
     cache.check_errors()
+
+
+@pytest.mark.parametrize("dtype", list(DTYPE))
+@pytest.mark.parametrize("sequences", [3, 40])
+@pytest.mark.parametrize("above", [5, 12, 20, 40, 60, 90])
+@pytest.mark.parametrize("where", [0, 700, 1279])
+def test_what_a_heavy_key_leaves(dtype, sequences, above, where):
+    """One key outweighs each of the others by 2^above and has a value of zero: the others are the result, all tiles
+    but its own to their full bits.
+
+    With s the others' share of the weights, largest the largest value: an error e of the weights moves an output
+    by 2 e s largest; a tile's weights are rounded to 2^-25 (in two parts of float32: 2^-23 of the largest at worst) of
+    what its own largest is above, 2^-8 (2^-2), and the heavy key's tile to 2^-27 of the heavy weight, where no key
+    loses more than itself.
+    """
+    rng = np.random.default_rng(above + where)
+    size, prefix = 64, 1280
+    host = family(rng, prefix, [1 + 4 * b % 9 for b in range(sequences)], kv_heads=1, head_size=size, page=64)
+    host.scales[0][np.isfinite(host.scales[0])] = 0.25
+    host.scales[1][np.isfinite(host.scales[1])] = 2.0 ** -6
+    for slot in range(sequences):
+        for at in range(host.held(int(host.lengths[slot]))):
+            page = int(host.table[slot, at])
+            rows = min(64, int(host.lengths[slot]) - 64 * at)
+            if at < prefix // 64 and slot > 0:
+                continue
+            host.pools[0][0, page, 0, :rows] = 0
+            host.pools[0][0, page, 0, :rows, 0] = rng.integers(-4, 5, rows)
+            host.pools[1][0, page, 0, :rows] = rng.integers(64, 128, (rows, size))  # one sign: nothing cancels
+    page, row = int(host.table[0, where // 64]), where % 64
+    host.pools[0][0, page, 0, row, 0] = 127
+    host.pools[1][0, page, 0, row] = 0
+    q = torch.zeros(sequences, 1, 4, size, device="cuda", dtype=DTYPE[dtype])
+    q[..., 0] = above * math.log(2.0) / (0.25 * 127)
+    cache = to_device(host)
+    got = wide(cache.attend_shared(0, q, scale=1.0, least_bytes=0))
+    cache.check_errors()
+    want = expected(host, q, [1] * sequences, range(sequences), 1.0)
+    info, largest = torch.finfo(DTYPE[dtype]), 127 * 2.0 ** -6
+    score = 0.25 * float(q[0, 0, 0, 0])
+    tile = slice(where // 64 * 64, where // 64 * 64 + 64)
+    for b in range(sequences):
+        weight = np.exp(score * (host.read(0, 0, b)[:, 0, 0] / 0.25 - 127))  # of the heavy one
+        total = weight.sum()
+        others = np.delete(weight, where) / total
+        share, mine = others.sum(), np.delete(weight[tile], where % 64) / total
+        part = 2.0 ** -23 if dtype == "f32" else 2.0 ** -17
+        bound = (2 * (WEIGHTS[dtype] + part * math.exp(8 * score)) * share + np.minimum(mine, 2.0 ** -27).sum()) * largest
+        bound = bound + info.eps / 2 * np.abs(want[b]) + info.tiny * info.eps / 2
+        if np.abs(want[b]).min() > 4 * info.tiny * info.eps:  # (what the type holds)
+            assert (np.abs(want[b]) > bound).all()  # zeros would not do
+        assert (np.abs(got[b] - want[b]) <= bound).all(), float(np.max(np.abs(got[b] - want[b]) / bound))
