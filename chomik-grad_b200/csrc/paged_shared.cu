@@ -136,6 +136,15 @@ struct SharedShape {
   static constexpr int kWide = SIZE < 64 ? 64 : SIZE;            // columns of the weighted values
 };
 
+// What has a second fp16 part, of what the first leaves: nothing (bfloat16), the weights
+// (float16, whose queries are exact in one), queries and weights (float32).  One part of
+// the weights would do for 11-bit outputs but for an error as large as their rounding:
+// 2.9e-4 of the result against 2.1e-4, and 152 us against 176 for 16 blocks of 5 tokens at
+// 32700 keys, 81 against 89 for 64 samples of 16384.
+enum { kOnePart = 0, kWeightParts = 1, kBothParts = 2 };
+__host__ __device__ constexpr bool low_queries(int parts) { return parts == kBothParts; }
+__host__ __device__ constexpr bool low_weights(int parts) { return parts != kOnePart; }
+
 // fp16 x fp16 -> float32, 128 x n; the second operand with its contraction along (K) or across its rows.
 __host__ __device__ constexpr uint32_t idesc_f16(int n, bool across) {
   return (1u << 4) | (across ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (128u >> 4 << 24);
@@ -409,7 +418,7 @@ __device__ __forceinline__ bool convert(const SharedPlan& p, const SharedWalk& w
 // of the one before are in registers, while the set weighs it.  (While warps take
 // exponentials, a look at a barrier can wait for hundreds of cycles: those for the
 // tiles come before the one for the weights.)
-template <int SIZE, int SETS, bool LO>
+template <int SIZE, int SETS, int PARTS>
 __device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* keys, const char* values,
                                       const char* queries, SharedSync& sync) {
   using S = SharedShape<SIZE>;
@@ -436,7 +445,7 @@ __device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* 
         const uint32_t d = tmem + kScoresAt + set * kSetColumns;
         if (leads) {
 #pragma unroll
-          for (int part = 0; part < (LO ? 2 : 1); ++part)
+          for (int part = 0; part < (low_queries(PARTS) ? 2 : 1); ++part)
 #pragma unroll
             for (int k = 0; k < SIZE / 16; ++k)
               multiply_shared(d, query + (part * S::kQueryBytes + k / 4 * kRowLanes * 128 + k % 4 * 32) / 16,
@@ -453,13 +462,13 @@ __device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* 
           return false;
         tc::fence_after();
         const uint64_t tile = across_desc(values + n % kStages * S::kStageBytes);
-        const uint32_t d = tmem + kValuesAt + set * 128, a = tmem + kScoresAt + set * kSetColumns + weights_at(LO, now);
+        const uint32_t d = tmem + kValuesAt + set * 128, a = tmem + kScoresAt + set * kSetColumns + weights_at(low_weights(PARTS), now);
         if (leads) {
 #pragma unroll
-          for (int part = 0; part < (LO ? 2 : 1); ++part)
+          for (int part = 0; part < (low_weights(PARTS) ? 2 : 1); ++part)
 #pragma unroll
             for (int k = 0; k < kSharedTile / 16; ++k)
-              multiply(d, a + k * (LO ? 16 : 8) + part * 8, tile + k * 2048 / 16, kValueDesc, job > 0 || part + k > 0);
+              multiply(d, a + k * (low_weights(PARTS) ? 16 : 8) + part * 8, tile + k * 2048 / 16, kValueDesc, job > 0 || part + k > 0);
           tc::umma_commit(sync.value_done[set] + buffer);
           tc::umma_commit(sync.value_free + n % kStages);
         }
@@ -478,15 +487,15 @@ __device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* 
 // in paged_attention.cuh: what multiplies the value codes is 2^(y - c), y a key's
 // score plus the logarithm of its value scale.  A tile whose largest is more
 // than kRise above c or `fall` below it moves c to kRest below it: it is rounded to
-// 2^-24 of 2^(y - c), so the largest of every tile keeps 11 bits, and those 2^5 below it,
-// of two parts (float32) 22.  Moving takes a pass over the sums (2000 cycles); the range
+// 2^-24 of 2^(y - c), so the largest of every tile keeps 11 bits, and those 2^5 below it;
+// of two parts it keeps 16 (float16) and 22 (float32, which falls earlier).  Moving takes a pass over the sums (2000 cycles); the range
 // makes it rare (rises of 15 and falls of 6: most tiles of some row, 137 us for 64
 // samples of 16384 keys; falls of 8 or 15: the same 81 us).
 // It falls as far as the sums against it stay below 2^kHeldExponent: keys below about
 // 2^-100 of all the weights before them may be lost.
 constexpr float kRise = 15.0f, kRest = 2.0f, kFarBelow = 60.0f;
 constexpr int kHeldExponent = 100;
-__host__ __device__ constexpr float fall_of(bool lo) { return lo ? 2.0f : 8.0f; }
+__host__ __device__ constexpr float fall_of(bool close) { return close ? 2.0f : 8.0f; }
 // e of 2^e <= x < 2^(e + 1); -127 of zero, 128 of infinity and NaN
 __device__ __forceinline__ int exponent_of(float x) { return static_cast<int>(__float_as_uint(x) >> 23) - 127; }
 
@@ -521,7 +530,7 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // |f| <= 1/2, by its Taylor polynomial of degree 5: (f ln 2)^6 / 720 < 2.5e-6, a
 // hundredth of the weights' rounding to 11 bits.  (2^n is multiplied: added to the
 // exponent's bits it would make a number of a NaN.)
-template <bool LO>
+template <bool CLOSE>
 __device__ __forceinline__ float exponentials(float* x, float by, float shift) {
   const uint64_t by2 = pair_of(by, by), shift2 = pair_of(shift, shift);
   uint64_t run[2] = {0, 0};
@@ -532,7 +541,7 @@ __device__ __forceinline__ float exponentials(float* x, float by, float shift) {
     uint64_t e = fma2(pair_of(x[k], x[k + 1]), by2, shift2);
     float a, b;
     split_pair(e, a, b);
-    if (LO || k % 4 == 0) {
+    if (CLOSE || k % 4 == 0) {
       x[k] = exp2_of(a);
       x[k + 1] = exp2_of(b);
     } else {
@@ -580,7 +589,7 @@ __device__ __forceinline__ void store_weights(uint32_t at, const float* x) {
 }
 
 // A set of 128 rows, a thread each.
-template <int SIZE, int STORAGE, int SETS, bool LO>
+template <int SIZE, int STORAGE, int SETS, int PARTS>
 __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, char* queries, float* factors, long long* offsets,
                                       const Runs* runs, SharedSync& sync) {
   const int thread = threadIdx.x - 32 * kWeighWarp, set = thread / kSetThreads, r = thread % kSetThreads;
@@ -618,13 +627,13 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
     __syncwarp();
     if (segment > 0 && !wait_warp(&sync.query_free, static_cast<uint32_t>((segment - 1) & 1), abort)) return false;
     const uint32_t turn_of_queries = static_cast<uint32_t>(segment & 1);
-    if (SETS == 2 || LO || set == 0) {
+    if (SETS == 2 || low_queries(PARTS) || set == 0) {
       // 16-bit rows are copied to where they will be first; the loops are rolled, since
       // code that runs once costs its way to the instruction cache
       constexpr int kLanes = SIZE / 8;
       const int lane = threadIdx.x & 31, d = lane % kLanes * 8;
-      char* to = queries + (SETS == 2 || LO ? set * SharedShape<SIZE>::kQueryBytes : 0) + d / 64 * kRowLanes * 128;
-      const bool copied = !LO && p.wide;
+      char* to = queries + (SETS == 2 || low_queries(PARTS) ? set * SharedShape<SIZE>::kQueryBytes : 0) + d / 64 * kRowLanes * 128;
+      const bool copied = !low_queries(PARTS) && p.wide;
       if (copied) {
 #pragma unroll 1
         for (int step = 0; step < kLanes; ++step) {
@@ -642,7 +651,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
         uint4* place = reinterpret_cast<uint4*>(to + tc::swizzle_offset(local_row, d % 64 / 8));
         float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, largest = 0.0f;
         if (copied) unpack_row8(p, *place, x);
-        else if (at_row >= 0) load_row8<LO>(p, at_row + d, x);
+        else if (at_row >= 0) load_row8<low_queries(PARTS)>(p, at_row + d, x);
 #pragma unroll
         for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(x[i]));
 #pragma unroll
@@ -657,7 +666,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
           const int first = STORAGE == CB_I8 ? i / 2 * 4 + i % 2 : 2 * i, second = STORAGE == CB_I8 ? first + 2 : first + 1;
           const float a = x[first] * sign, b = x[second] * sign;
           const __half2 hi = __floats2half2_rn(a, b);
-          h[i] = LO && set == 1 ? bits(__floats2half2_rn(a - __low2float(hi), b - __high2float(hi))) : bits(hi);
+          h[i] = low_queries(PARTS) && set == 1 ? bits(__floats2half2_rn(a - __low2float(hi), b - __high2float(hi))) : bits(hi);
         }
         *place = make_uint4(h[0], h[1], h[2], h[3]);
       }
@@ -666,7 +675,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
     mbar_arrive(&sync.query_full);
     __syncwarp();
     // (one part of one set of rows: the other set has its factors from there)
-    const bool other = SETS == 1 && !LO && set == 1;
+    const bool other = SETS == 1 && !low_queries(PARTS) && set == 1;
     if (other && !wait_warp(&sync.query_full, turn_of_queries, abort)) return false;
     const float factor = factors[other ? r : thread];
 
@@ -675,7 +684,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
     for (int tile = SETS == 2 ? 0 : set; tile < tiles; tile += SETS == 2 ? 1 : 2, ++iteration) {
       const int n = before + tile;
       const int buffer = iteration & 1;
-      const uint32_t weights = scores + weights_at(LO, iteration);
+      const uint32_t weights = scores + weights_at(low_weights(PARTS), iteration);
       if (!reach(n) ||
           !wait_warp(sync.score_full + set, static_cast<uint32_t>(iteration & 1), abort))
         return false;
@@ -685,10 +694,6 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
         __syncwarp();
         if ((threadIdx.x & 31) == 0) mbar_arrive(sync.score_free + set);
       };
-      // (low parts leave no room for the weights of two tiles)
-      if (LO && iteration > 0 &&
-          !wait_warp(sync.value_done[set] + (buffer ^ 1), static_cast<uint32_t>((iteration - 1) / 2 & 1), abort))
-        return false;
       if (!any) leave_scores();
       if (any) {
         float s[kSharedTile], by[4], log[4], inverse[4];
@@ -722,11 +727,11 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
           }
         }
         float now = c;
-        if (__any_sync(0xffffffffu, first || top > c + kRise || top < c - fall_of(LO))) {
+        if (__any_sync(0xffffffffu, first || top > c + kRise || top < c - fall_of(low_queries(PARTS)))) {
           const float next = floorf(top) - kRest;
           if (first) now = top > -INFINITY ? next : 0.0f;
           else if (top > c + kRise) now = next;
-          else if (top < c - fall_of(LO) && top > -INFINITY)  // (the sums stay below 2^kHeldExponent)
+          else if (top < c - fall_of(low_queries(PARTS)) && top > -INFINITY)  // (the sums stay below 2^kHeldExponent)
             now = fmaxf(next, c - static_cast<float>(max(kHeldExponent - 1 - exponent_of(fmaxf(sum, l)), 0)));
         }
         if (__any_sync(0xffffffffu, first || now != c)) {
@@ -754,6 +759,10 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
           c = now;
         }
         first = false;
+        // (low parts leave no room for the weights of two tiles)
+        if (low_weights(PARTS) && iteration > 0 &&
+            !wait_warp(sync.value_done[set] + (buffer ^ 1), static_cast<uint32_t>((iteration - 1) / 2 & 1), abort))
+          return false;
         if (__builtin_expect(!irregular, 1)) {
           // all of a row's far below c: its weights by themselves, since 2^(y - c) may not
           // be there (of that row alone: no bit of a row depends on the rows beside it)
@@ -765,10 +774,10 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float all = exponentials<LO>(s + 16 * i, by[i], log[i] - c);
+            const float all = exponentials<low_queries(PARTS)>(s + 16 * i, by[i], log[i] - c);
             if (!far) l = fmaf(all, inverse[i], l);
             sum += all;
-            store_weights<LO>(weights + i * (LO ? 16 : 8), s + 16 * i);
+            store_weights<low_weights(PARTS)>(weights + i * (low_weights(PARTS) ? 16 : 8), s + 16 * i);
           }
         } else {  // value scales of any sign and size: the weights by themselves
 #pragma unroll 1
@@ -785,7 +794,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
               x[k] *= kept;
             }
             if (tile_runs.inverse[i] != 0.0f) l += all;
-            store_weights<LO>(weights + i * (LO ? 16 : 8), x);
+            store_weights<low_weights(PARTS)>(weights + i * (low_weights(PARTS) ? 16 : 8), x);
           }
           leave_scores();
         }
@@ -835,7 +844,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
   return true;
 }
 
-template <int SIZE, int STORAGE, int SETS, bool LO>
+template <int SIZE, int STORAGE, int SETS, int PARTS>
 __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_constant__ SharedPlan p) {
   using S = SharedShape<SIZE>;
   extern __shared__ char memory[];
@@ -897,11 +906,11 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
   if (w.count > 0) {
     if (warp < kWeighWarp) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegisters));
-      if (warp < kIssueWarp + 2) ok = issue<SIZE, SETS, LO>(w, warp - kIssueWarp, tiles, values, queries, sync);
+      if (warp < kIssueWarp + 2) ok = issue<SIZE, SETS, PARTS>(w, warp - kIssueWarp, tiles, values, queries, sync);
       if (warp == kLookWarp) ok = look_up(p, w, runs, sync);
     } else if (warp < kKeyWarp) {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWeighRegisters));
-      ok = weigh<SIZE, STORAGE, SETS, LO>(p, w, queries, factors, offsets, runs, sync);
+      ok = weigh<SIZE, STORAGE, SETS, PARTS>(p, w, queries, factors, offsets, runs, sync);
     } else {
       const bool is_value = warp >= kValueWarp;
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegisters));
@@ -978,10 +987,14 @@ bool may_share(const cb_paged_attention_args& a, long long least_bytes) {
 template <typename F>
 int with_shape(const cb_paged_attention_args& a, F f) {
   auto by_rows = [&](auto size, auto storage) {
-    using one = std::integral_constant<int, 1>;
-    if (a.dtype == CB_F32) return f(size, storage, one{}, std::true_type{});
-    if (two_sets(a)) return f(size, storage, std::integral_constant<int, 2>{}, std::false_type{});
-    return f(size, storage, one{}, std::false_type{});
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    if (a.dtype == CB_F32) return f(size, storage, one, std::integral_constant<int, kBothParts>{});
+    auto by_type = [&](auto sets) {
+      if (a.dtype == CB_F16) return f(size, storage, sets, std::integral_constant<int, kWeightParts>{});
+      return f(size, storage, sets, std::integral_constant<int, kOnePart>{});
+    };
+    return two_sets(a) ? by_type(two) : by_type(one);
   };
   auto by_storage = [&](auto size) {
     return a.cache.storage == CB_I8 ? by_rows(size, std::integral_constant<int, CB_I8>{})
@@ -1037,9 +1050,9 @@ int cb_paged_attention_shared(const cb_paged_attention_args* args, long long lea
   const int item = a.dtype == CB_F32 ? 4 : 2;
   p.wide = reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
   for (int i = 0; i < 3; ++i) p.wide = p.wide && a.q_strides[i] * item % 16 == 0;
-  done = with_shape(a, [&](auto size, auto storage, auto sets, auto lo) -> int {
+  done = with_shape(a, [&](auto size, auto storage, auto sets, auto parts) -> int {
     constexpr int SIZE = size.value;
-    auto kernel = shared_kernel<SIZE, storage.value, sets.value, lo.value>;
+    auto kernel = shared_kernel<SIZE, storage.value, sets.value, parts.value>;
     static thread_local int device = -1;
     int now = 0;
     cudaGetDevice(&now);

@@ -316,8 +316,9 @@ class PagedCache:
         its own.  Any sequences may be given, and a cache whose tables cannot hold that
         much is read as by ``attend``.
 
-        Queries and weights of these keys go to the tensor cores as fp16 (11 bits)
-        with float32 sums, of float32 queries in two parts (22 bits).  Of 64 keys, one whose
+        Queries and weights of these keys go to the tensor cores as fp16 with float32
+        sums: one part (11 bits) of both for bfloat16, two (22 bits) of both for float32 and
+        of the weights for float16, whose queries are exact in one. Of 64 keys, one whose
         weight is below 2^-17 (float32: 2^-23) of the largest of them, or 2^-90 of the
         row's, may be left out.
         """

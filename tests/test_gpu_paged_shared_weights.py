@@ -120,3 +120,24 @@ def test_what_a_heavy_key_leaves(dtype, sequences, above, where):
         if np.abs(want[b]).min() > 4 * info.tiny * info.eps:  # (what the type holds)
             assert (np.abs(want[b]) > bound).all()  # zeros would not do
         assert (np.abs(got[b] - want[b]) <= bound).all(), float(np.max(np.abs(got[b] - want[b]) / bound))
+
+
+@pytest.mark.parametrize("storage", ["int8", "e4m3"])
+@pytest.mark.parametrize("sequences, tokens, size", [(3, 1, 64), (40, 1, 128), (9, 5, 32)])
+def test_float16_keeps_its_bits(storage, sequences, tokens, size):
+    """float16 outputs are as near as their own rounding: weights and queries are held to more than its 11 bits.
+
+    In the 2-norm, over the result's: rounding to 11 bits moves float16 numbers by 1.9e-4 to 2.4e-4 (what `floor` is
+    here); weights held to 2^-16 (scores below 64 in base 2 of 22 bits, exponentials to 2.5e-6, two parts) move the
+    result by 3.1e-5 before that at most, 0.15 of it.
+    """
+    rng = np.random.default_rng(size)
+    tails = [tokens + b % 3 for b in range(sequences)]
+    host = family(rng, 1280, tails, kv_heads=1, head_size=size, storage=storage)
+    q = queries(rng, sequences, tokens, 4, size, "f16")
+    cache = to_device(host)
+    got = wide(cache.attend_shared(0, q, least_bytes=0))
+    cache.check_errors()
+    want = expected(host, q, [tokens] * sequences, range(sequences), 1 / math.sqrt(size))
+    floor = np.linalg.norm(want.astype(np.float16).astype(np.float64) - want)
+    assert np.linalg.norm(got - want) <= 1.15 * floor, float(np.linalg.norm(got - want) / floor)
