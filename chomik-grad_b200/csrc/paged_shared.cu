@@ -101,8 +101,11 @@ constexpr int kSetThreads = 128;
 constexpr int kIssueWarp = 0, kLookWarp = 2, kWeighWarp = 4, kKeyWarp = 12, kValueWarp = 16;
 constexpr int kSharedThreads = 32 * (kValueWarp + 4);
 // Registers of a thread, 96 at the launch: of the warps that weigh, of those that
-// convert, and of the four that issue and look up (61440 of a block, before and after).
+// convert, and of the four that issue and look up (61440 of a block, before and after;
+// the launch checks that they were there before, since a raise waits for them).
 constexpr int kWeighRegisters = 152, kConvertRegisters = 72, kIssueRegisters = 32;
+constexpr int kBlockRegisters =
+    32 * (8 * kWeighRegisters + 8 * kConvertRegisters + 4 * kIssueRegisters);
 constexpr int kStages = 3, kAhead = 3;  // tiles as fp16, and tiles whose codes are on their way
 constexpr int kChunkBytes = kSharedTile * 128;  // 64 keys of 64 fp16 elements
 // Columns of the tensor memory: weighted values of both sets; then, for each set, the
@@ -135,6 +138,11 @@ struct SharedShape {
   static constexpr int kBytes = kStages * kStageBytes + 2 * kQueryBytes + kAhead * kCodeBytes + 1024;
   static constexpr int kWide = SIZE < 64 ? 64 : SIZE;            // columns of the weighted values
 };
+// Every block asks for the shared memory of the largest, so that no other that takes
+// tensor memory fits beside it: it takes all of that before the kernels ahead have ended,
+// and one of theirs, or of those behind, that waited for some on the same SM would keep both.
+constexpr int kBlockBytes = SharedShape<128>::kBytes;
+static_assert(kBlockBytes >= SharedShape<64>::kBytes && kBlockBytes >= SharedShape<32>::kBytes, "the largest");
 
 // What has a second fp16 part, of what the first leaves: nothing (bfloat16), the weights
 // (float16, whose queries are exact in one), queries and weights (float32).  One part of
@@ -855,8 +863,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1) shared_kernel(const __grid_
   char* tiles = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(memory) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
-  // (all of the tensor memory, before the kernels ahead have ended: none of theirs that
-  // takes some fits an SM beside this block's shared memory)
+  // (all of the tensor memory, before the kernels ahead have ended: see kBlockBytes)
   if (warp == kIssueWarp) tc::tmem_alloc(&sync.tmem, kColumns);
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -1044,25 +1051,28 @@ int cb_paged_attention_shared(const cb_paged_attention_args* args, long long lea
   p.shared.common = common;
   p.parts = reinterpret_cast<float*>(base + at.parts);
   p.shared.parts = p.parts;
-  launch(common_kernel, dim3(static_cast<unsigned>(a.batch)), dim3(kCommonThreads), 0, s, true, a, common);
-  int done = check_launch("cb_paged_attention_shared");
-  if (done != CB_OK) return done;
   const int item = a.dtype == CB_F32 ? 4 : 2;
   p.wide = reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
   for (int i = 0; i < 3; ++i) p.wide = p.wide && a.q_strides[i] * item % 16 == 0;
-  done = with_shape(a, [&](auto size, auto storage, auto sets, auto parts) -> int {
+  const int done = with_shape(a, [&](auto size, auto storage, auto sets, auto parts) -> int {
     constexpr int SIZE = size.value;
     auto kernel = shared_kernel<SIZE, storage.value, sets.value, parts.value>;
     static thread_local int device = -1;
     int now = 0;
     cudaGetDevice(&now);
     if (now != device) {
-      const cudaError_t e =
-          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SharedShape<SIZE>::kBytes);
+      cudaFuncAttributes attributes;
+      cudaError_t e = cudaFuncGetAttributes(&attributes, kernel);
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBlockBytes);
       CB_REQUIRE(e == cudaSuccess, "cb_paged_attention_shared: %s", cudaGetErrorString(e));
+      CB_REQUIRE(attributes.numRegs * kSharedThreads >= kBlockRegisters,
+                 "cb_paged_attention_shared: built with %d registers a thread, too few to be divided", attributes.numRegs);
       device = now;
     }
-    launch(kernel, dim3(static_cast<unsigned>(p.shared.blocks)), dim3(kSharedThreads), SharedShape<SIZE>::kBytes, s, true, p);
+    launch(common_kernel, dim3(static_cast<unsigned>(a.batch)), dim3(kCommonThreads), 0, s, true, a, common);
+    const int found = check_launch("cb_paged_attention_shared");
+    if (found != CB_OK) return found;
+    launch(kernel, dim3(static_cast<unsigned>(p.shared.blocks)), dim3(kSharedThreads), kBlockBytes, s, true, p);
     return check_launch("cb_paged_attention_shared");
   });
   if (done != CB_OK) return done;
