@@ -1039,6 +1039,9 @@ int cb_paged_attention_shared(const cb_paged_attention_args* args, long long lea
              "cb_paged_attention_shared: a null pointer");
   CB_REQUIRE(reinterpret_cast<uintptr_t>(scratch) % 32 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0,
              "cb_paged_attention_shared: out must be 16-byte aligned, scratch 32");
+  // (what launch_attention would refuse, before anything is launched)
+  CB_REQUIRE(attention_scratch(a, true) > 0, "cb_paged_attention_shared: %lld rows of up to %lld keys are too many for one call",
+             a.batch * a.heads * a.tokens, a.cache.columns * a.cache.page);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   SharedPlan p = {};
   p.a = a;

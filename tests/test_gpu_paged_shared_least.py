@@ -10,6 +10,8 @@ import numpy as np
 import pytest
 import torch
 
+from cuda_b200 import _lib
+from cuda_b200.paged import PagedCache
 from paged_helpers import DTYPE, to_device
 from test_gpu_paged_attention import compare, expected, queries
 from test_gpu_paged_shared import family
@@ -71,3 +73,15 @@ def test_the_border_follows_the_tables():
     assert torch.equal(cache.attend_shared(0, q, least_bytes=1), cache.attend(0, q))  # nothing is common to all four
     assert torch.equal(cache.attend_shared(0, q, counts=ones, least_bytes=2 * unit), three)
     cache.check_errors()
+
+
+def test_too_many_for_one_call():
+    """What the kernel of the sequences' own keys cannot divide is refused before a kernel of the call runs."""
+    cache = PagedCache.allocate(layers=1, pages=8, kv_heads=8, page_size=16, head_size=32, sequences=2,
+                                pages_per_sequence=2 ** 16)
+    slots = torch.zeros(65535, dtype=torch.int32, device="cuda")
+    q = torch.zeros(65535, 1, 8, 32, device="cuda")
+    for call in (dict(least_bytes=0), dict()):
+        with pytest.raises(_lib.KernelError, match="too many"):
+            cache.attend_shared(0, q, sequences=slots, **call)
+    cache.check_errors()  # (a kernel would have found that slot 0 holds no token)
