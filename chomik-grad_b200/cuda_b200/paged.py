@@ -32,6 +32,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 from typing import Any, Optional, Tuple
 
 import torch
@@ -178,7 +179,7 @@ class PagedCache:
         p.page_bytes = self.kv_heads * self.page_size * self.head_size
         self._lib = _lib.load()
         self._attend_args, self._append_args, self._lists = Prepared(), Prepared(), Prepared()
-        self._scratch_words, self._workspaces = Prepared(), Prepared()
+        self._scratch_words, self._workspaces, self._calls = Prepared(), Prepared(), threading.Lock()
 
     @classmethod
     def allocate(cls, *, layers: int, pages: int, kv_heads: int, page_size: int, head_size: int, sequences: int,
@@ -347,12 +348,14 @@ class PagedCache:
         if sequences is not None:
             a.sequences = sequences.data_ptr()
         stream = self._stream()
-        counters, scratch = self._workspace(stream, known[2], known[1])
-        if least_bytes is None:
-            _lib.check(self._lib.cb_paged_attention(ctypes.byref(a), scratch, counters, stream), "cb_paged_attention")
-        else:
-            _lib.check(self._lib.cb_paged_attention_shared(ctypes.byref(a), least_bytes, scratch, counters, stream),
-                       "cb_paged_attention_shared")
+        with self._calls:  # (a call's launches share its workspace: none of another thread's come between)
+            counters, scratch = self._workspace(stream, known[2], known[1])
+            if least_bytes is None:
+                _lib.check(self._lib.cb_paged_attention(ctypes.byref(a), scratch, counters, stream),
+                           "cb_paged_attention")
+            else:
+                _lib.check(self._lib.cb_paged_attention_shared(ctypes.byref(a), least_bytes, scratch, counters, stream),
+                           "cb_paged_attention_shared")
         return out
 
     def _workspace(self, stream: int, counters: int, words: int) -> Tuple[int, int]:

@@ -931,7 +931,8 @@ CB_API int cb_paged_attention(const cb_paged_attention_args* args, void* scratch
  * multiplied once, with the rows of all.  Any sequences may be given; where the table's
  * columns cannot hold that much this is cb_paged_attention.  `scratch`:
  * cb_paged_attention_shared_scratch bytes for the same arguments, 32-byte aligned;
- * `counters` as there.  A bounded wait that gives up sets CB_FLAG_WAIT_DATA or
+ * `counters` as there; a call is several launches, so calls of threads that share
+ * scratch and a stream must not meet.  A bounded wait that gives up sets CB_FLAG_WAIT_DATA or
  * CB_FLAG_WAIT_DRAIN. */
 CB_API long long cb_paged_attention_shared_scratch(const cb_paged_attention_args* args, long long least_bytes);
 CB_API int cb_paged_attention_shared(const cb_paged_attention_args* args, long long least_bytes, void* scratch,
