@@ -15,12 +15,12 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Any, Optional, Union
+from typing import Any, Dict, Optional, Tuple, Union
 
 import torch
 
 from . import _lib
-from .paged import _VALUES, Prepared, current_stream, no_grad_needed, overlap, require, signature, tensor_of
+from .paged import _VALUES, Prepared, current_stream, meet, no_grad_needed, reach, require, signature, tensor_of
 
 _INDICES = {torch.int32: _lib.I32, torch.int64: _lib.I64}
 MAX_BIASES, MAX_HISTORY = 1023, 2 ** 20 - 1
@@ -50,9 +50,9 @@ def adjust(logits: Any, *, tokens: Any = None, lengths: Any = None, prompts: Any
 
     float32, bfloat16 or float16 with rows of any stride (a history, bias or mask
     that all rows share can be expanded).  The sums are float32 and rounded once.
-    ``out`` may be ``logits`` itself.  Lengths outside the history are taken as
-    its ends and set ``error_flag`` (an int32 of the caller's, read with
-    ``speculative.check``).
+    ``out`` may be ``logits`` itself; it shares no memory with another argument.
+    Lengths outside the history are taken as its ends and set ``error_flag`` (an
+    int32 of the caller's, read with ``speculative.check``).
     """
     if type(logits) is not torch.Tensor:
         logits = tensor_of(logits)
@@ -86,11 +86,12 @@ def adjust(logits: Any, *, tokens: Any = None, lengths: Any = None, prompts: Any
     if known is None:
         known = _ADJUST_ARGS[key] = _prepare(logits, out, values, numbers, error_flag)
     stream = current_stream(logits.device)
+    a, spans = known
     if not fresh:
-        apart(logits, out)
+        apart(logits, out, spans, pointers, error_flag)
         if not out.is_inference():  # a backward pass that kept what it held notices
             torch.autograd.graph.increment_version(out)
-    a = _lib.AdjustArgs.from_buffer_copy(known)
+    a = _lib.AdjustArgs.from_buffer_copy(a)
     a.logits, a.out = logits.data_ptr(), out.data_ptr()
     for name, pointer in pointers:
         setattr(a, name, pointer)
@@ -104,16 +105,22 @@ _FLOATS = ("repetition", "frequency", "presence", "bias")
 _FIELDS = {"repetition": "repetitions", "frequency": "frequencies", "presence": "presences"}
 
 
-def apart(logits: torch.Tensor, out: torch.Tensor) -> None:
-    """Refuse an ``out`` that shares part of its memory with ``logits``: it is the same rows, or none of them."""
-    if logits.data_ptr() == out.data_ptr() and (logits.stride(0) == out.stride(0) or logits.shape[0] <= 1):
-        return
-    if overlap(logits, out):
+def apart(logits: torch.Tensor, out: torch.Tensor, spans, pointers, error_flag: Optional[torch.Tensor]) -> None:
+    """Refuse an ``out`` that shares memory with an argument, but for ``logits``' own rows: blocks write it while
+    others read.  ``spans``: the bytes that each argument reaches over, by its name."""
+    at, size = out.data_ptr(), spans["out"]
+    same = logits.data_ptr() == at and (logits.stride(0) == out.stride(0) or logits.shape[0] <= 1)
+    if not same and meet(at, size, logits.data_ptr(), spans["logits"]):
         raise ValueError("out has to be logits itself, or memory of its own")
+    for name, pointer in pointers:
+        if meet(at, size, pointer, spans[name]):
+            raise ValueError(f"out shares memory with {name}")
+    if error_flag is not None and meet(at, size, error_flag.data_ptr(), 4):
+        raise ValueError("out shares memory with error_flag")
 
 
 def _prepare(logits: torch.Tensor, out: torch.Tensor, values, numbers,
-             error_flag: Optional[torch.Tensor]) -> _lib.AdjustArgs:
+             error_flag: Optional[torch.Tensor]) -> Tuple[_lib.AdjustArgs, Dict[str, int]]:
     device = logits.device
     if device.type != "cuda":
         raise ValueError(f"logits are on {device}, expected a CUDA device")
@@ -163,4 +170,5 @@ def _prepare(logits: torch.Tensor, out: torch.Tensor, values, numbers,
         a.allowed_ld = values["allowed"].stride(0)
     if error_flag is not None:
         require(error_flag, "error_flag", device, (torch.int32,), (1,), 1)
-    return a
+    return a, {_FIELDS.get(name, name): reach(value)
+               for name, value in (("logits", logits), ("out", out), *values.items())}

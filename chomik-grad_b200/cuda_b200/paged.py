@@ -102,11 +102,21 @@ def current_stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def reach(value: torch.Tensor) -> int:
+    """Bytes of memory from a tensor's first element to behind its last."""
+    if value.numel() == 0:
+        return 0
+    return (1 + sum((n - 1) * s for n, s in zip(value.shape, value.stride()))) * value.element_size()
+
+
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether the spans of memory that ``a`` and ``b`` reach over meet."""
-    ends = [t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
-            for t in (a, b)]
-    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < ends[1] and b.data_ptr() < ends[0]
+    return meet(a.data_ptr(), reach(a), b.data_ptr(), reach(b))
+
+
+def meet(a: int, a_bytes: int, b: int, b_bytes: int) -> bool:
+    """Whether two spans of memory, each an address and its bytes, have a byte in common."""
+    return a_bytes > 0 and b_bytes > 0 and a < b + b_bytes and b < a + a_bytes
 
 
 def signature(value: Optional[torch.Tensor]):

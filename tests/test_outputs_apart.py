@@ -1,0 +1,55 @@
+"""An ``out`` that lies over an argument is refused: other blocks read that while it is written."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from cuda_b200 import logits
+from cuda_b200.paged import meet, reach
+
+
+def test_spans():
+    room = torch.zeros(4, 64)
+    assert reach(room) == 1024 and reach(room[:, :8]) == 3 * 256 + 32 and reach(room[:0]) == 0
+    assert reach(room[0].expand(9, 64)) == 256 and reach(room.bfloat16()[1:, ::2]) == 2 * 128 + 63 * 2
+    assert meet(100, 10, 109, 1) and not meet(100, 10, 110, 5) and not meet(110, 5, 100, 10)
+    assert not meet(100, 10, 100, 0) and not meet(100, 0, 90, 100)
+
+
+def test_adjust_apart():
+    """The check by itself, on host memory: which arguments an out may lie over."""
+    room = torch.zeros(3, 64)
+    rows, flag = room[:, :40], torch.zeros(1, dtype=torch.int32)
+    tokens, allowed = room.view(torch.int32)[:, 48:], torch.zeros(3, 2, dtype=torch.int32)
+
+    def check(out, source=rows, **more):
+        spans = {"logits": reach(source), "out": reach(out)} | {name: reach(t) for name, t in more.items()}
+        logits.apart(source, out, spans, [(name, t.data_ptr()) for name, t in more.items()], flag)
+
+    check(rows)
+    check(torch.zeros(3, 40), tokens=tokens, allowed=allowed)
+    check(rows, allowed=allowed)
+    for out, more in ((room[:, 1:41], {}), (rows, {"tokens": tokens}), (allowed.view(torch.float32), {"allowed": allowed}),
+                      (flag.view(torch.float32).expand(1, 1), {})):
+        with pytest.raises(ValueError, match="out "):
+            check(out, **more)
+
+
+@pytest.mark.gpu
+def test_adjust_refuses():
+    room = torch.zeros(8, 64, device="cuda")
+    words = room.view(torch.int32)
+    x = torch.zeros(4, 64, device="cuda")
+    for name, more in (("tokens", dict(tokens=words[3:7, :9])), ("bias", dict(bias_tokens=words[4:, :9].clone(), bias=room[3:7, :9])),
+                       ("bias_tokens", dict(bias_tokens=words[3:7, :9], bias=room[4:, :9].clone())),
+                       ("allowed", dict(allowed=words[3:7, :2])), ("lengths", dict(tokens=words[4:], lengths=words[0, :4])),
+                       ("presences", dict(tokens=words[4:], presence=room[1, 3:7])), ("error_flag", dict(error_flag=words[3, 63:]))):
+        with pytest.raises(ValueError, match=name):
+            logits.adjust(x, out=room[:4], **more)
+    rows = torch.randn(4, 64, device="cuda")
+    words.zero_()
+    want = logits.adjust(rows, tokens=words[4:], presence=0.5)
+    assert logits.adjust(rows, tokens=words[4:], presence=0.5, out=room[:4]) is not want
+    assert torch.equal(room[:4], want)
+    assert torch.equal(logits.adjust(rows, tokens=words[4:], presence=0.5, out=rows), want)
