@@ -22,7 +22,8 @@ from typing import Any, Optional
 import torch
 
 from . import _lib
-from .paged import _VALUES, Prepared, aligned, current_stream, no_grad_needed, overlap, require, signature, tensor_of
+from .paged import (_VALUES, Prepared, aligned, current_stream, meet, no_grad_needed, reach, require, signature,
+                    tensor_of)
 
 GROUPS = (32, 64, 128)
 _SCALES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
@@ -100,7 +101,7 @@ class Weights4:
         costs; every 32 rows (10 of float32) read the weights again, so a prompt's rows
         are better multiplied with ``dequantise``'s.  float32 rows, and 16-bit rows
         that do not begin on 16 bytes, are first copied to a workspace.  ``out`` is
-        contiguous and shares no memory with x.
+        contiguous and shares no memory with x or the weights.
         """
         x = tensor_of(x)
         no_grad_needed(x)
@@ -113,8 +114,7 @@ class Weights4:
             out = x.new_empty(shape)
         else:
             require(out, "out", self.device, (x.dtype,), shape, len(shape))
-            if overlap(out, x):
-                raise ValueError("out shares memory with x")
+            self._apart(out, x)
             no_grad_needed(out)
             if not out.is_inference():  # a backward pass that kept what it held notices
                 torch.autograd.graph.increment_version(out)
@@ -127,6 +127,13 @@ class Weights4:
         _lib.check(self._lib.cb_linear4(ctypes.byref(a), None if scratch is None else scratch.data_ptr(), stream),
                    "cb_linear4")
         return out
+
+    def _apart(self, out: torch.Tensor, x: Optional[torch.Tensor] = None) -> None:
+        """Refuse an ``out`` over x or the weights: other blocks read those while it is written."""
+        at, size = out.data_ptr(), reach(out)
+        for name, value in (("x", x), ("codes", self.codes), ("scales", self.scales)):
+            if value is not None and meet(at, size, value.data_ptr(), reach(value)):
+                raise ValueError(f"out shares memory with {name}")
 
     def _prepare_linear(self, x: torch.Tensor):
         if x.ndim < 1:
@@ -149,6 +156,7 @@ class Weights4:
             require(out, "out", self.device, tuple(_VALUES), (self.outputs, self.inputs), 1)
             if self.outputs > 1 and out.stride(0) < self.inputs:
                 raise ValueError("the rows of out share memory")
+            self._apart(out)
             no_grad_needed(out)
             if not out.is_inference():
                 torch.autograd.graph.increment_version(out)

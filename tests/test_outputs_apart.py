@@ -7,6 +7,7 @@ import torch
 
 from cuda_b200 import logits
 from cuda_b200.paged import meet, reach
+from cuda_b200.quantized import Weights4
 
 
 def test_spans():
@@ -53,3 +54,23 @@ def test_adjust_refuses():
     assert logits.adjust(rows, tokens=words[4:], presence=0.5, out=room[:4]) is not want
     assert torch.equal(room[:4], want)
     assert torch.equal(logits.adjust(rows, tokens=words[4:], presence=0.5, out=rows), want)
+
+
+@pytest.mark.gpu
+def test_weights_refuse():
+    weights = Weights4.quantise(torch.randn(64, 128, device="cuda"), group=32)
+    x = torch.randn(2, 128, device="cuda")
+    codes, scales = weights.codes.clone(), weights.scales.clone()
+    for name, out in (("codes", weights.codes[:512].view(torch.float32).view(2, 64)),
+                      ("scales", weights.scales.view(torch.float32)[:128].view(2, 64)), ("x", x.view(-1)[64:192].view(2, 64))):
+        with pytest.raises(ValueError, match=name):
+            weights.linear(x, out=out)
+    room = torch.zeros(64 * 64 * 2 + 64 * 128 * 2, dtype=torch.uint8, device="cuda")
+    with pytest.raises(ValueError, match="codes"):  # the last of the codes, in a buffer that holds both
+        over = Weights4(room[:weights.codes.numel()], weights.scales, outputs=64, inputs=128, group=32)
+        over.dequantise(out=room[weights.codes.numel() - 16:][:64 * 128 * 2].view(torch.bfloat16).view(64, 128))
+    assert torch.equal(weights.codes, codes) and torch.equal(weights.scales, scales)
+    over = Weights4(room[:weights.codes.numel()], weights.scales, outputs=64, inputs=128, group=32)
+    over.codes.copy_(codes)
+    behind = room[weights.codes.numel():][:64 * 128 * 2].view(torch.bfloat16).view(64, 128)
+    assert torch.equal(over.dequantise(out=behind), weights.dequantise(torch.bfloat16))
