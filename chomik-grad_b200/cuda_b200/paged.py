@@ -177,6 +177,9 @@ class PagedCache:
         self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.book = k_pages, v_pages, k_scale, v_scale, book
         self.table, self.lengths, self.refs, self.free, self.height = self.split(book)
         self._flag = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._spans = [(name, t.data_ptr(), reach(t)) for name, t in (
+            ("k_pages", k_pages), ("v_pages", v_pages), ("k_scale", k_scale), ("v_scale", v_scale), ("the book", book),
+            ("the error flag", self._flag))]
         self._layer_args = [self._args_of(layer) for layer in range(self.layers)]
         self._book_args, self._pool_args = _lib.PageBook(), _lib.PagePools()
         b, p = self._book_args, self._pool_args
@@ -303,7 +306,8 @@ class PagedCache:
         Each token sees its slot's keys up to its own (``counts`` and
         ``sequences`` as in ``append``; rows past ``counts[b]`` and rows that
         see nothing give zeros).  ``scale`` is 1/sqrt(head_size) without one.
-        Returns (batch, tokens, heads, head_size) of q's dtype.
+        Returns (batch, tokens, heads, head_size) of q's dtype; ``out`` may be a
+        contiguous ``q`` itself and lies over nothing else that the call reads.
 
         Queries and weights go to the tensor cores as fp16 in two parts (22
         bits) with float32 sums; where more than 8 rows share a kv head,
@@ -348,6 +352,7 @@ class PagedCache:
         else:
             require(out, "out", self.device, (q.dtype,), tuple(q.shape), 4)
             aligned(out, "out")
+            self._apart(out, q, counts, sequences)
             no_grad_needed(out)
             if not out.is_inference():  # a backward pass that kept what it held notices
                 torch.autograd.graph.increment_version(out)
@@ -367,6 +372,19 @@ class PagedCache:
                 _lib.check(self._lib.cb_paged_attention_shared(ctypes.byref(a), least_bytes, scratch, counters, stream),
                            "cb_paged_attention_shared")
         return out
+
+    def _apart(self, out: torch.Tensor, q: torch.Tensor, counts: Optional[torch.Tensor],
+               sequences: Optional[torch.Tensor]) -> None:
+        """Refuse an ``out`` over what other blocks read while it is written; it may be ``q`` itself, row by row."""
+        at, size = out.data_ptr(), reach(out)
+        for name, pointer, held in self._spans:
+            if meet(at, size, pointer, held):
+                raise ValueError(f"out shares memory with {name}")
+        for name, value in (("q", q), ("counts", counts), ("sequences", sequences)):
+            if value is None or (value is q and q.data_ptr() == at and q.is_contiguous()):
+                continue
+            if meet(at, size, value.data_ptr(), reach(value)):
+                raise ValueError(f"out shares memory with {name}")
 
     def _workspace(self, stream: int, counters: int, words: int) -> Tuple[int, int]:
         """Addresses of zeroed counters, which a call leaves zero, and of scratch for a call on ``stream``.

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from cuda_b200 import logits
-from cuda_b200.paged import meet, reach
+from cuda_b200.paged import PagedCache, meet, reach
 from cuda_b200.quantized import Weights4
 
 
@@ -74,3 +74,41 @@ def test_weights_refuse():
     over.codes.copy_(codes)
     behind = room[weights.codes.numel():][:64 * 128 * 2].view(torch.bfloat16).view(64, 128)
     assert torch.equal(over.dequantise(out=behind), weights.dequantise(torch.bfloat16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["attend", "attend_shared"])
+def test_attention_refuses(name):
+    """Pools, scales and book in one buffer with the output, queries that it partly covers; the queries' own place."""
+    q = torch.randn(2, 3, 4, 64, device="cuda")
+    sizes = [1 * 8 * 2 * 16 * 64] * 2 + [4 * 16] * 2 + [4 * (2 * 4 + 2 + 16 + 1)]
+    room = torch.zeros(sum(sizes) + 16 * 1024, dtype=torch.uint8, device="cuda")
+    starts = [0, sizes[0], sum(sizes[:2]), sum(sizes[:3]), sum(sizes[:4])]
+    parts = [room[a:a + n] for a, n in zip(starts, sizes)]
+    pools = [p.view(torch.int8).view(1, 8, 2, 16, 64) for p in parts[:2]]
+    scales = [p.view(torch.float32).view(1, 8, 2) for p in parts[2:4]]
+    book = parts[4].view(torch.int32)
+    book[:8].fill_(-1)
+    book[10 + 8:10 + 16] = torch.arange(8, device="cuda")
+    book[-1] = 8
+    cache = PagedCache(*pools, *scales, book, sequences=2, pages_per_sequence=4)
+    cache.extend([20, 30])
+    for at, what in ((0, "k_pages"), (sizes[0] + 16, "v_pages"), (starts[2], "k_scale"), (starts[3], "v_scale"),
+                     (starts[4] // 16 * 16 + 16, "the book")):
+        out = room[at:at + 2 * 3 * 4 * 64 * 4].view(torch.float32).view(2, 3, 4, 64)
+        with pytest.raises(ValueError, match=what):
+            getattr(cache, name)(0, q, out=out)
+    wide = torch.randn(3, 3, 4, 64, device="cuda")
+    with pytest.raises(ValueError, match="q"):
+        getattr(cache, name)(0, wide[:2], out=wide[1:])
+    words = torch.ones(3 * 3 * 4 * 64, dtype=torch.int32, device="cuda")
+    for more in ("counts", "sequences"):
+        with pytest.raises(ValueError, match=more):
+            getattr(cache, name)(0, q, out=words[4:].view(torch.float32)[:2 * 3 * 4 * 64].view(2, 3, 4, 64),
+                                 **{more: words[8:10]})
+    rows = torch.randn(2, 50, 2, 64, device="cuda")
+    cache.append(0, rows[:, :20], rows[:, 20:40], counts=[20, 20])
+    more = {"least_bytes": 0} if name == "attend_shared" else {}
+    want = getattr(cache, name)(0, q, **more)
+    assert getattr(cache, name)(0, q, out=q, **more) is q and torch.equal(q, want)
+    cache.check_errors()
