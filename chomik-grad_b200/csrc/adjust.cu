@@ -34,7 +34,7 @@ constexpr int kBiasAt = 20;
 
 struct AdjustPlan {
   cb_adjust_args a;
-  int slices, slice;  // of a row, and their tokens
+  int slices;         // of a row
   int has_history;    // tokens, or lengths to be checked
   int shared_lead;    // logits and out lie alike to 16 bytes in every row: wide accesses
 };
@@ -301,7 +301,6 @@ int run_adjust(AdjustPlan p, cudaStream_t stream) {
   const long long item = sizeof(T);
   const uintptr_t in = reinterpret_cast<uintptr_t>(p.a.logits), out = reinterpret_cast<uintptr_t>(p.a.out);
   p.shared_lead = (in - out) % 16 == 0 && (p.a.rows == 1 || (p.a.ld - p.a.out_ld) * item % 16 == 0);
-  p.slice = kSlice;
   const long long slices = (p.a.vocab + 7 + kSlice - 1) / kSlice;
   CB_REQUIRE(slices * p.a.rows < (1LL << 31), "cb_adjust_logits: %lld rows of %lld", p.a.rows, p.a.vocab);
   p.slices = static_cast<int>(slices);
@@ -357,6 +356,8 @@ int cb_adjust_logits(const cb_adjust_args* args, cb_stream_t stream) {
   const int item = a.dtype == CB_F32 ? 4 : 2;
   CB_REQUIRE(reinterpret_cast<uintptr_t>(a.logits) % item == 0 && reinterpret_cast<uintptr_t>(a.out) % item == 0,
              "cb_adjust_logits: logits and out must be aligned to their type");
+  CB_REQUIRE(a.rows == 1 || a.out_ld >= a.vocab || -a.out_ld >= a.vocab,
+             "cb_adjust_logits: rows of %lld tokens, %lld apart, share memory", a.vocab, a.out_ld);
   CB_REQUIRE(a.tokens == nullptr || a.token_dtype == CB_I32 || a.token_dtype == CB_I64,
              "cb_adjust_logits: tokens must be int32 or int64");
   CB_REQUIRE(a.tokens != nullptr || a.history == 0, "cb_adjust_logits: a history without tokens");

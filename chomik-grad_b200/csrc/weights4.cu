@@ -543,6 +543,8 @@ int cb_linear4(const cb_linear4_args* args, void* scratch, cb_stream_t stream) {
   CB_REQUIRE(a.x != nullptr && a.out != nullptr, "cb_linear4: a null pointer");
   CB_REQUIRE(on_its_type(a.x, a.dtype) && on_its_type(a.out, a.dtype),
              "cb_linear4: x and out must be aligned to their type");
+  CB_REQUIRE(a.rows == 1 || a.out_ld >= a.weights.outputs || -a.out_ld >= a.weights.outputs,
+             "cb_linear4: rows of %lld outputs, %lld apart, share memory", a.weights.outputs, a.out_ld);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   LinearPlan p = {};
   p.w = a.weights;
