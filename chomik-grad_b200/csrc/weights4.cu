@@ -7,10 +7,12 @@
 // group's scale, 2 flops a weight and row.  At the measured 6.46 TB/s an SM gets 23
 // bytes a clock, 46 weights: with scalar multiply-adds that would be 46 conversions
 // and as many products for each row, so the products go to the tensor cores
-// (m16n8k16, float32 sums) with the weights as the 16-row operand: up to 8 rows of
-// x cost the same.  The codes are exact in fp16 and bfloat16, so x stays in its own
-// type, and a group's scale multiplies the group's float32 sum.  float32 x is split
-// into three bfloat16 parts (24 bits) that are columns of their own.
+// (m16n8k16, float32 sums) with the weights as the 16-row operand: up to 8 columns
+// cost the same.  The codes are exact in fp16 and bfloat16, so x stays in its own
+// type, and a group's scale multiplies the group's float32 sum, which has to be within
+// float32 before that.  float32 x is split into three bfloat16 parts that are columns of
+// their own (24 bits; of numbers below 2^-110 what is above 2^-133), so 2 rows of it cost
+// what one does.
 //
 // Layout.  The operand's order of k is free as long as x has the same, so weights
 // are kept as a lane reads them: a block of 16 outputs x 64 inputs is 512 bytes, 16
@@ -538,7 +540,9 @@ int cb_linear4(const cb_linear4_args* args, void* scratch, cb_stream_t stream) {
   if (status != CB_OK) return status;
   CB_REQUIRE(a.dtype == CB_F32 || a.dtype == CB_BF16 || a.dtype == CB_F16,
              "cb_linear4: x must be float32, bfloat16 or float16");
-  CB_REQUIRE(a.rows >= 0 && a.rows < (1LL << 24), "cb_linear4: %lld rows", a.rows);
+  const int parts = a.dtype == CB_F32 ? 3 : 1, most = kColumnTiles * 8 / parts;  // rows that a block can take
+  CB_REQUIRE(a.rows >= 0 && a.rows <= 65535LL * most, "cb_linear4: %lld rows, at most %lld are taken", a.rows,
+             65535LL * most);
   if (a.rows == 0) return CB_OK;
   CB_REQUIRE(a.x != nullptr && a.out != nullptr, "cb_linear4: a null pointer");
   CB_REQUIRE(on_its_type(a.x, a.dtype) && on_its_type(a.out, a.dtype),
@@ -550,7 +554,7 @@ int cb_linear4(const cb_linear4_args* args, void* scratch, cb_stream_t stream) {
   p.w = a.weights;
   p.x = a.x;
   p.ld = a.ld;
-  p.parts = a.dtype == CB_F32 ? 3 : 1;
+  p.parts = parts;
   p.rows = static_cast<int>(a.rows * p.parts);
   p.out = a.out;
   p.out_dtype = a.dtype;
@@ -567,9 +571,7 @@ int cb_linear4(const cb_linear4_args* args, void* scratch, cb_stream_t stream) {
     p.x = scratch;
     p.ld = a.weights.inputs;
   }
-  const int most = kColumnTiles * 8 / p.parts;
   const int launches = static_cast<int>((a.rows + most - 1) / most);
-  CB_REQUIRE(launches <= 65535, "cb_linear4: %lld rows", a.rows);
   p.per = static_cast<int>((a.rows + launches - 1) / launches);
   return with_columns((p.per * p.parts + 7) / 8, [&](auto columns) {
     constexpr int C = columns.value;

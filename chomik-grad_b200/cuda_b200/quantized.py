@@ -97,11 +97,13 @@ class Weights4:
     def linear(self, x: Any, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``x @ weight.T`` for x (..., inputs) in float32, bfloat16 or float16: (..., outputs) of x's type.
 
-        Products are exact and sums float32.  Up to 8 rows cost about what one
+        Products are exact and sums float32 (those of a group's codes and x, before its
+        scale, have to be within it).  Up to 8 rows (2 of float32) cost about what one
         costs; every 32 rows (10 of float32) read the weights again, so a prompt's rows
         are better multiplied with ``dequantise``'s.  float32 rows, and 16-bit rows
-        that do not begin on 16 bytes, are first copied to a workspace.  ``out`` is
-        contiguous and shares no memory with x or the weights.
+        that do not begin on 16 bytes, are first copied to a workspace.  At most
+        2,097,120 rows are taken (655,350 of float32).  ``out`` is contiguous and
+        shares no memory with x or the weights.
         """
         x = tensor_of(x)
         no_grad_needed(x)

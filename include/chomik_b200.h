@@ -793,9 +793,10 @@ CB_API int cb_weights4_pack(const cb_weights4* weights, const void* codes, const
 CB_API int cb_weights4_dequantise(const cb_weights4* weights, void* out, int dtype, long long ld, cb_stream_t stream);
 
 /* out[r] = x[r] @ weights.T: rows of x and out have ld and out_ld elements and
- * one type, CB_F32, CB_BF16 or CB_F16; sums are float32, rounded once.  Up to 8
- * rows cost about what one costs, and every 32 rows (10 of float32) read the
- * weights again.  `scratch`: cb_linear4_scratch bytes (0 for 16-bit rows that
+ * one type, CB_F32, CB_BF16 or CB_F16; sums are float32, rounded once (those of a
+ * group's codes and x, before its scale, have to be within float32).  Up to 8 rows (2 of
+ * float32) cost about what one costs, and every 32 rows (10 of float32) read the
+ * weights again; at most 2,097,120 rows (655,350) are taken.  `scratch`: cb_linear4_scratch bytes (0 for 16-bit rows that
  * lie on 16 bytes), 16-byte aligned. */
 typedef struct {
   cb_weights4 weights;
