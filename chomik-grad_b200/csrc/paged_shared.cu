@@ -293,7 +293,8 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real)
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
 
-// Looks up the runs of the range's tiles.
+// Looks up the runs of the range's tiles.  (Through L2: the kernels ahead may have written
+// the table and the scales after this one began, so they are no read-only data of it.)
 __device__ __forceinline__ bool look_up(const SharedPlan& p, const SharedWalk& w, Runs* runs, SharedSync& sync) {
   const cb_paged_cache& c = p.a.cache;
   const int lane = threadIdx.x & 31, run = lane & 3, count = w.count, shift = 31 - __clz(c.page);
@@ -303,12 +304,12 @@ __device__ __forceinline__ bool look_up(const SharedPlan& p, const SharedWalk& w
     const int head = (w.item + n / w.tiles * w.step) / w.blocks, slot = batch % kBatches;
     long long line = -1;
     if (n < count && key < w.keys) {
-      const int page = __ldg(w.table + (key >> shift));
+      const int page = __ldcg(w.table + (key >> shift));
       if (static_cast<unsigned>(page) < static_cast<unsigned>(c.pages)) line = static_cast<long long>(page) * c.kv_heads + head;
       else raise_flag(p.a.error_flag, CB_FLAG_BOOK);
     }
     const bool real = line >= 0;
-    const float k = real ? __ldg(c.k_scale + line) : 0.0f, v = real ? __ldg(c.v_scale + line) : 1.0f;
+    const float k = real ? __ldcg(c.k_scale + line) : 0.0f, v = real ? __ldcg(c.v_scale + line) : 1.0f;
     float log = -INFINITY, inverse = 0.0f, factor = 1.0f;
     if (real) {  // (an error of the logarithm moves the weights and their sum alike)
       const float size = fabsf(v);
