@@ -21,8 +21,10 @@
 // cycles on the tensor cores (scores 8 x 48, values 4 x 64), but 8192 exponentials with their
 // conversions about 1700 cycles on the four schedulers: that, and the hand-offs
 // between warps that it delays, is what is left (2600 to 2900 cycles a tile of two
-// sets; 64 samples of 16384 keys 81 us on the device, 16 blocks of 5 tokens at 32700
-// keys 150; by cb_paged_attention, each sequence for itself, 351 and 292).
+// sets, 3400 where the weights have two parts; 64 samples of 16384 keys 82 us on the
+// device, 90 in float16 and 95 in float32, 16 blocks of 5 tokens at 32700 keys 151 and
+// 176 in float16, by cb_paged_attention, each sequence for itself, 351 and 292; 8
+// samples of 32768 keys, both sets the same rows, 65 and 71).
 //
 // Three launches, each begun while the one before ends: the common pages of each
 // sequence; the shared keys, a block to an SM, whose warps are divided by what they
@@ -147,8 +149,8 @@ static_assert(kBlockBytes >= SharedShape<64>::kBytes && kBlockBytes >= SharedSha
 // What has a second fp16 part, of what the first leaves: nothing (bfloat16), the weights
 // (float16, whose queries are exact in one), queries and weights (float32).  One part of
 // the weights would do for 11-bit outputs but for an error as large as their rounding:
-// 2.9e-4 of the result against 2.1e-4, and 152 us against 176 for 16 blocks of 5 tokens at
-// 32700 keys, 81 against 89 for 64 samples of 16384.
+// 2.9e-4 of the result against 2.1e-4 (152 us against 176 for 16 blocks of 5 tokens at
+// 32700 keys, 81 against 90 for 64 samples of 16384).
 enum { kOnePart = 0, kWeightParts = 1, kBothParts = 2 };
 __host__ __device__ constexpr bool low_queries(int parts) { return parts == kBothParts; }
 __host__ __device__ constexpr bool low_weights(int parts) { return parts != kOnePart; }
@@ -499,7 +501,7 @@ __device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* 
 // 2^-24 of 2^(y - c), so the largest of every tile keeps 11 bits, and those 2^5 below it;
 // of two parts it keeps 16 (float16) and 22 (float32, which falls earlier).  Moving takes a pass over the sums (2000 cycles); the range
 // makes it rare (rises of 15 and falls of 6: most tiles of some row, 137 us for 64
-// samples of 16384 keys; falls of 8 or 15: the same 81 us).
+// samples of 16384 keys; falls of 8 or 15: the same 82 us).
 // It falls as far as the sums against it stay below 2^kHeldExponent: keys below about
 // 2^-100 of all the weights before them may be lost.
 constexpr float kRise = 15.0f, kRest = 2.0f, kFarBelow = 60.0f;

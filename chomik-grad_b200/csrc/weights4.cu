@@ -21,8 +21,10 @@
 // of both rows.  Lane (g, c) so needs x[g][32 h + 8 c + 0 .. 7], 16 neighbouring bytes,
 // which come straight from L1: no staging, no barrier before the products.  Measured:
 // 16 rows by 4096 x 128256, 77 us (3.6 TB/s: 16 warps an SM do not cover the loads of
-// x and the conversions), one row 55 (5.0 TB/s); one row by 4096 x 14336 8.9, by 2048 x
-// 2048 2.2, a launch and one chain of loads, products and sums.  Code
+// x and the conversions), one row 55 (5.0 TB/s); one row by 4096 x 14336 8.2, by 2048 x
+// 2048 2.2, a launch and one chain of loads, products and sums.  Above 16 rows a block has
+// one tile and loads all of them from L1 for it, and above 32 the weights are read and
+// converted again: 24, 32, 64 and 80 rows by 4096 x 128256 take 134, 179, 354 and 498 us.  Code
 // q + 8 of pair i (row g, inputs 0 and 1; row g + 8, the same; row g, inputs 2 and
 // 3; row g + 8) is nibbles i and i + 4: one logic instruction makes two operands of
 // them (see halves_of).
@@ -49,7 +51,8 @@ __device__ __forceinline__ float scale_of(uint32_t bits, int dtype) {
 
 // Pair i of a word as two numbers of the products' type.  bfloat16: the code under
 // the exponent of 128 is 128 + code; fp16: under that of 1024, where the next
-// nibble is in reach too, as 1024 + 16 * code.
+// nibble is in reach too, as 1024 + 16 * code.  (The method: Kim, Henry, Fahim and Awadalla,
+// "Who Says Elephants Can't Run", 2022.)
 template <bool HALF>
 __device__ __forceinline__ void halves_of(uint32_t w, uint32_t* a) {
   if (HALF) {
