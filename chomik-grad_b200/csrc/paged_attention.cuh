@@ -10,16 +10,6 @@
 
 namespace cb {
 
-// Keys are computed apart where every sequence's reading them would be 128 MB or more:
-// beginning, ending and joining their parts takes 25 to 30 us, in which the other
-// kernel reads that from L2 (8 kv heads of 128, 64 sequences, 4 rows: 1024 keys 59 us
-// apart and 43 not, 8192 keys 78 and 189; 16 sequences, 20 rows: 1024 keys 65 and 29,
-// 16350 keys 115 and 158).
-constexpr long long kSharedBytes = 1LL << 27;
-__host__ __device__ inline long long shared_bytes_of(const cb_paged_attention_args& a, long long sequences, long long keys) {
-  return (sequences - 1) * keys * a.cache.kv_heads * a.cache.head_size * 2;
-}
-
 // The first keys of all sequences of a call, computed apart (paged_shared.cu).
 // `common`: for each sequence the whole pages that it has in common with the
 // call's first; INT_MAX where it takes no part.  The rows of a kv head, those
@@ -32,8 +22,27 @@ struct SharedKeys {
   const int* common;  // and behind them the slot of the first sequence that takes part
   const float* parts;
   int block_rows, ways, blocks, least;  // blocks of the grid; tiles of a piece: `least` or more, or all
-  long long least_bytes;                // see kSharedBytes
+  long long least_bytes;                // of reads that are repeated; below 0: see worth_sharing
 };
+// Whether `keys` that `sequences` hold in common are computed apart.  Where the caller leaves
+// it open, from 192 MB on that all but three of the sequences would read: beginning, ending
+// and joining the parts takes 25 to 30 us, and a pass of the shared kernel about as long as
+// three sequences' reads by the other one (8 kv heads of 128; apart and not: 64 sequences of
+// one token, 1024 keys 42 us and 38, 2048 43 and 58, 16384 69 and 356; 16 of 5 tokens, 4400
+// keys 66 and 53, 8192 77 and 82; 8 of one token, 8192 keys 43 and 33, 16384 51 and 53; 4, 65536
+// keys 103 and 101; 2, 131072 keys 160 and 101).  And items for a 32nd of the SMs: of fewer
+// each is cut in so many pieces that joining them takes longer than the reads (one kv head,
+// 32 rows, 16 sequences of 65536 keys: 74 pieces, 191 us and 105).
+constexpr int kSharedReads = 3, kSharedPieces = 32;
+constexpr long long kSharedBytes = 192LL << 20;
+__host__ __device__ inline bool worth_sharing(const cb_paged_attention_args& a, const SharedKeys& s, long long sequences,
+                                              long long keys) {
+  const long long each = keys * a.cache.kv_heads * a.cache.head_size * 2;
+  if (s.least_bytes >= 0) return (sequences - 1) * each >= s.least_bytes;
+  const long long rows = a.batch * a.tokens * (a.heads / a.cache.kv_heads);
+  const long long items = a.cache.kv_heads * ((rows + s.block_rows - 1) / s.block_rows);
+  return (sequences - kSharedReads) * each >= kSharedBytes && items * kSharedPieces >= s.blocks;
+}
 // Of element d of row r behind a part's references and sums: eight elements of all rows
 // together, a sector each.
 __host__ __device__ constexpr long long shared_at(int block_rows, int r, int d) {
@@ -159,7 +168,7 @@ __device__ __forceinline__ int common_pages(const cb_paged_attention_args& a, co
   __syncthreads();
   if (found[1] == 0) return 0;
   const long long keys = static_cast<long long>(found[0]) * a.cache.page;
-  return shared_bytes_of(a, found[1], keys) >= shared.least_bytes ? found[0] : 0;
+  return worth_sharing(a, shared, found[1], keys) ? found[0] : 0;
 }
 // The division of the shared keys: tiles of an item and of a piece, pieces of an item.
 // No block takes pieces of two items while there are more blocks than items, since

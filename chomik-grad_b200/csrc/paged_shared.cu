@@ -990,8 +990,8 @@ int shared_check(const cb_paged_attention_args& a) {
 }
 
 // Whether the sequences could hold enough keys in common for these to be computed apart.
-bool may_share(const cb_paged_attention_args& a, long long least_bytes) {
-  return shared_bytes_of(a, a.batch, a.cache.columns * a.cache.page) >= least_bytes;
+bool may_share(const cb_paged_attention_args& a, const SharedKeys& shared) {
+  return worth_sharing(a, shared, a.batch, a.cache.columns * a.cache.page);
 }
 
 template <typename F>
@@ -1023,21 +1023,20 @@ using namespace cb;
 extern "C" {
 
 long long cb_paged_attention_shared_scratch(const cb_paged_attention_args* args, long long least_bytes) {
-  if (least_bytes < 0) least_bytes = kSharedBytes;
   if (args == nullptr || shared_check(*args) != CB_OK || args->batch == 0 || args->tokens == 0) return 0;
-  if (!may_share(*args, least_bytes)) return attention_scratch(*args, false);
-  return scratch_of(*args, shared_of(*args, least_bytes)).bytes;
+  const SharedKeys shared = shared_of(*args, least_bytes);
+  return may_share(*args, shared) ? scratch_of(*args, shared).bytes : attention_scratch(*args, false);
 }
 
 int cb_paged_attention_shared(const cb_paged_attention_args* args, long long least_bytes, void* scratch,
                               unsigned* counters, cb_stream_t stream) {
-  if (least_bytes < 0) least_bytes = kSharedBytes;
   CB_REQUIRE(args != nullptr, "cb_paged_attention_shared: null arguments");
   const cb_paged_attention_args& a = *args;
   const int status = shared_check(a);
   if (status != CB_OK) return status;
   if (a.batch == 0 || a.tokens == 0) return CB_OK;
-  if (!may_share(a, least_bytes)) return launch_attention(a, nullptr, scratch, counters, static_cast<cudaStream_t>(stream));
+  const SharedKeys shared = shared_of(a, least_bytes);
+  if (!may_share(a, shared)) return launch_attention(a, nullptr, scratch, counters, static_cast<cudaStream_t>(stream));
   CB_REQUIRE(a.q != nullptr && a.out != nullptr && counters != nullptr && scratch != nullptr,
              "cb_paged_attention_shared: a null pointer");
   CB_REQUIRE(reinterpret_cast<uintptr_t>(scratch) % 32 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0,
@@ -1050,7 +1049,7 @@ int cb_paged_attention_shared(const cb_paged_attention_args* args, long long lea
   p.a = a;
   p.group = static_cast<int>(a.heads / a.cache.kv_heads);
   p.rows = static_cast<int>(a.tokens * p.group);
-  p.shared = shared_of(a, least_bytes);
+  p.shared = shared;
   const SharedScratch at = scratch_of(a, p.shared);
   char* base = static_cast<char*>(scratch);
   int* common = reinterpret_cast<int*>(base + at.common);

@@ -42,7 +42,6 @@ from . import _lib
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 HEAD_SIZES = (32, 64, 128)
-SHARED_BYTES = 2 ** 27  # of ``attend_shared``: from where reading shared keys once pays
 _VALUES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _STORAGE = {torch.int8: _lib.I8, torch.float8_e4m3fn: _lib.E4M3}
 
@@ -321,15 +320,16 @@ class PagedCache:
 
     def attend_shared(self, layer: int, q: Any, *, counts: Any = None, sequences: Any = None,
                       scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
-                      least_bytes: int = SHARED_BYTES) -> torch.Tensor:
+                      least_bytes: Optional[int] = None) -> torch.Tensor:
         """``attend`` for sequences that begin alike, as ``fork`` leaves them.
 
         The leading pages that all sequences of the call hold in common (those
-        with a count of 0 aside) are found on the device.  Where the sequences'
-        reading them one by one would be ``least_bytes`` more than once, they are read
-        and multiplied once with the rows of all; each sequence's other keys are
-        its own.  Any sequences may be given, and a cache whose tables cannot hold that
-        much is read as by ``attend``.
+        with a count of 0 aside) are found on the device.  Where it pays, they are
+        read and multiplied once with the rows of all, each sequence's other keys by
+        themselves; elsewhere all is read as by ``attend``, so any sequences may be
+        given.  It pays from 192 MB on that all but three of the sequences would read,
+        with kv heads and blocks of rows for a part of the GPU; with ``least_bytes``
+        the keys are read once wherever that saves so many bytes of reads.
 
         Queries and weights of these keys go to the tensor cores as fp16 with float32
         sums: one part (11 bits) of both for bfloat16, two (22 bits) of both for float32 and
@@ -337,7 +337,10 @@ class PagedCache:
         weight is below 2^-17 (float32: 2^-23) of the largest of them, or 2^-90 of the
         row's, may be left out.
         """
-        return self._attend(layer, q, counts, sequences, scale, out, int(least_bytes))
+        least = -1 if least_bytes is None else int(least_bytes)  # (below 0: by the library's rule)
+        if least_bytes is not None and not 0 <= least < 2 ** 63:
+            raise ValueError(f"least_bytes is {least_bytes}, expected 0 or more")
+        return self._attend(layer, q, counts, sequences, scale, out, least)
 
     def _attend(self, layer: int, q: Any, counts: Any, sequences: Any, scale: Optional[float],
                 out: Optional[torch.Tensor], least_bytes: Optional[int]) -> torch.Tensor:
@@ -405,8 +408,6 @@ class PagedCache:
     def _prepare_attend(self, layer: int, q: torch.Tensor, counts: Optional[torch.Tensor],
                         sequences: Optional[torch.Tensor], scale: Optional[float],
                         least_bytes: Optional[int]) -> Tuple[_lib.PagedAttentionArgs, int, int]:
-        if least_bytes is not None and not 0 <= least_bytes < 2 ** 63:
-            raise ValueError(f"least_bytes is {least_bytes}, expected 0 or more")
         require(q, "q", self.device, tuple(_VALUES), (None, None, None, self.head_size), 1)
         batch, tokens, heads = q.shape[:3]
         if heads == 0 or heads % self.kv_heads:

@@ -928,7 +928,8 @@ CB_API int cb_paged_attention(const cb_paged_attention_args* args, void* scratch
  * the leading pages that the tables of all sequences with a count name alike, as
  * far as they are whole and leave each row a key of its own, are found on the
  * device.  Where the sequences' reading them one by one would be `least_bytes` more
- * than once (below 0: 128 MB, from where it pays), they are read and
+ * than once (below 0: where it pays, from 192 MB on that all but three of the sequences
+ * would read, with kv heads times blocks of rows for a 32nd of the SMs), they are read and
  * multiplied once, with the rows of all.  Any sequences may be given; where the table's
  * columns cannot hold that much this is cb_paged_attention.  `scratch`:
  * cb_paged_attention_shared_scratch bytes for the same arguments, 32-byte aligned;

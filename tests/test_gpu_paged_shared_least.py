@@ -85,3 +85,37 @@ def test_too_many_for_one_call():
         with pytest.raises(_lib.KernelError, match="too many"):
             cache.attend_shared(0, q, sequences=slots, **call)
     cache.check_errors()  # (a kernel would have found that slot 0 holds no token)
+
+
+# heads and kv heads of 128, sequences, tokens, dtype; keys in common from which they are computed apart by
+# themselves (None: at no length that is tried)
+RULE = [(32, 8, 64, 1, "bf16", 1664), (32, 8, 64, 1, "f32", 1664), (32, 8, 16, 5, "f16", 7616), (32, 8, 8, 1, "bf16", 19712),
+        (32, 8, 4, 1, "bf16", 98304), (32, 8, 3, 1, "bf16", None), (32, 8, 2, 1, "f32", None), (32, 1, 16, 1, "bf16", None),
+        (32, 1, 64, 1, "bf16", 12928)]
+
+
+@pytest.mark.parametrize("heads, kv_heads, batch, tokens, dtype, keys", RULE)
+def test_the_rule_by_itself(heads, kv_heads, batch, tokens, dtype, keys):
+    """Without least_bytes: 192 MB that all but three of the sequences would read, items for a 32nd of the SMs, and one
+    page less is attend's, bit for bit."""
+    if torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        pytest.skip("the borders are those of 148 SMs")
+    page, size = 64, 128
+    most = (200_000 if keys is None else keys) // page * page
+    cache = PagedCache.allocate(layers=1, pages=most // page + 2 * batch, kv_heads=kv_heads, page_size=page, head_size=size,
+                                sequences=batch, pages_per_sequence=most // page + 3)
+    gen = torch.Generator(device="cuda").manual_seed(keys or 1)
+    cache.k_pages.copy_(torch.randint(-90, 91, cache.k_pages.shape, device="cuda", generator=gen, dtype=torch.int8))
+    cache.v_pages.copy_(torch.randint(-90, 91, cache.v_pages.shape, device="cuda", generator=gen, dtype=torch.int8))
+    cache.k_scale.fill_(0.01), cache.v_scale.fill_(0.02)
+    q = torch.randn(batch, tokens, heads, size, device="cuda", generator=gen).to(DTYPE[dtype])
+    for length in ([most] if keys is None else [most - page, most]):
+        cache.release(list(range(batch)))
+        cache.extend([length], sequences=[0])
+        cache.fork([0] * (batch - 1), list(range(1, batch)))
+        cache.extend([tokens] * batch)
+        got, whole = cache.attend_shared(0, q), cache.attend(0, q)
+        apart = cache.attend_shared(0, q, least_bytes=0)
+        cache.check_errors()
+        assert not torch.equal(apart, whole)  # (so that equal bits say which way a call went)
+        assert torch.equal(got, apart if length == keys else whole)
