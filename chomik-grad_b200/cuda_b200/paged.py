@@ -327,7 +327,7 @@ class PagedCache:
         with a count of 0 aside) are found on the device.  Where it pays, they are
         read and multiplied once with the rows of all, each sequence's other keys by
         themselves; elsewhere all is read as by ``attend``, so any sequences may be
-        given.  It pays from 192 MB on that all but three of the sequences would read,
+        given (looking costs 6 to 8 us where the tables could hold as much).  It pays from 192 MB on that all but three of the sequences would read,
         with kv heads and blocks of rows for a part of the GPU; with ``least_bytes``
         the keys are read once wherever that saves so many bytes of reads.
 
