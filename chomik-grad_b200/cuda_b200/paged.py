@@ -42,6 +42,7 @@ from . import _lib
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 HEAD_SIZES = (32, 64, 128)
+SHARED_BYTES = 2 ** 27  # of reads that are repeated: a border for ``attend_shared``'s ``least_bytes``
 _VALUES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _STORAGE = {torch.int8: _lib.I8, torch.float8_e4m3fn: _lib.E4M3}
 
@@ -176,7 +177,7 @@ class PagedCache:
         self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.book = k_pages, v_pages, k_scale, v_scale, book
         self.table, self.lengths, self.refs, self.free, self.height = self.split(book)
         self._flag = torch.zeros(1, dtype=torch.int32, device=self.device)
-        self._spans = [(name, t.data_ptr(), reach(t)) for name, t in (
+        self._spans = [(name, t.data_ptr(), t.data_ptr() + t.nbytes) for name, t in (
             ("k_pages", k_pages), ("v_pages", v_pages), ("k_scale", k_scale), ("v_scale", v_scale), ("the book", book),
             ("the error flag", self._flag))]
         self._layer_args = [self._args_of(layer) for layer in range(self.layers)]
@@ -378,10 +379,10 @@ class PagedCache:
 
     def _apart(self, out: torch.Tensor, q: torch.Tensor, counts: Optional[torch.Tensor],
                sequences: Optional[torch.Tensor]) -> None:
-        """Refuse an ``out`` over what other blocks read while it is written; it may be ``q`` itself, row by row."""
-        at, size = out.data_ptr(), reach(out)
-        for name, pointer, held in self._spans:
-            if meet(at, size, pointer, held):
+        """Refuse an ``out`` (contiguous) over what other blocks read while it is written; it may be ``q`` itself."""
+        at, size = out.data_ptr(), out.nbytes
+        for name, start, end in self._spans:
+            if start < at + size and at < end and size:
                 raise ValueError(f"out shares memory with {name}")
         for name, value in (("q", q), ("counts", counts), ("sequences", sequences)):
             if value is None or (value is q and q.data_ptr() == at and q.is_contiguous()):

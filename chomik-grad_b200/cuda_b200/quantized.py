@@ -49,6 +49,7 @@ class Weights4:
         aligned(codes, "codes")
         aligned(scales, "scales")
         self.codes, self.scales = codes, scales
+        self._spans = [("codes", codes.data_ptr(), codes.nbytes), ("scales", scales.data_ptr(), scales.nbytes)]
         args.codes, args.scales = codes.data_ptr(), scales.data_ptr()
         self._args = args
         self._linear_args = Prepared()
@@ -133,9 +134,11 @@ class Weights4:
     def _apart(self, out: torch.Tensor, x: Optional[torch.Tensor] = None) -> None:
         """Refuse an ``out`` over x or the weights: other blocks read those while it is written."""
         at, size = out.data_ptr(), reach(out)
-        for name, value in (("x", x), ("codes", self.codes), ("scales", self.scales)):
-            if value is not None and meet(at, size, value.data_ptr(), reach(value)):
+        for name, start, held in self._spans:
+            if meet(at, size, start, held):
                 raise ValueError(f"out shares memory with {name}")
+        if x is not None and meet(at, size, x.data_ptr(), reach(x)):
+            raise ValueError("out shares memory with x")
 
     def _prepare_linear(self, x: torch.Tensor):
         if x.ndim < 1:

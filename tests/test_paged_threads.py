@@ -82,3 +82,36 @@ def test_a_call_that_fails_lets_others_in(cache):
         cache.attend(0, q)
     cache.attend_shared(0, q)
     assert library.most == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("streams", [1, 2])
+def test_threads_on_the_device(streams):
+    """Threads of one stream, or of two, with calls of other sizes and sequences: each gets its own results."""
+    cache = paged.PagedCache.allocate(layers=1, pages=300, kv_heads=2, page_size=16, head_size=64, sequences=12,
+                                      pages_per_sequence=60)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for parent, length in ((0, 500), (4, 700), (8, 90)):
+        cache.extend([length], sequences=[parent])
+        k, v = (torch.randn(1, length, 2, 64, device="cuda", generator=gen) for _ in range(2))
+        cache.append(0, k, v, sequences=[parent])
+        cache.fork([parent] * 3, [parent + i for i in (1, 2, 3)])
+    calls = []
+    for i in range(6):
+        slots = torch.arange(i % 3 * 4, i % 3 * 4 + 4 - i % 2, device="cuda").int()
+        q = torch.randn(len(slots), 1 + i, 8, 64, device="cuda", generator=gen)
+        calls.append((q, slots, cache.attend_shared(0, q, sequences=slots, least_bytes=0)))
+    cache.check_errors()
+    torch.cuda.synchronize()
+    used = [torch.cuda.Stream() for _ in range(streams)]
+
+    def work(i):
+        q, slots, want = calls[i]
+        with torch.cuda.stream(used[i % streams]):
+            got = [cache.attend_shared(0, q, sequences=slots, least_bytes=0) for _ in range(40)]
+        torch.cuda.synchronize()
+        return all(torch.equal(g, want) for g in got)
+
+    with ThreadPoolExecutor(6) as pool:
+        assert all(pool.map(work, range(6)))
+    cache.check_errors()
