@@ -505,7 +505,7 @@ __device__ __forceinline__ bool issue(const SharedWalk& w, int set, const char* 
 // It falls as far as the sums against it stay below 2^kHeldExponent: keys below about
 // 2^-100 of all the weights before them may be lost.
 constexpr float kRise = 15.0f, kRest = 2.0f, kFarBelow = 60.0f;
-constexpr int kHeldExponent = 100;
+constexpr int kHeldExponent = 100, kLargeExponent = 112;
 __host__ __device__ constexpr float fall_of(bool close) { return close ? 2.0f : 8.0f; }
 // e of 2^e <= x < 2^(e + 1); -127 of zero, 128 of infinity and NaN
 __device__ __forceinline__ int exponent_of(float x) { return static_cast<int>(__float_as_uint(x) >> 23) - 127; }
@@ -691,6 +691,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
     const float factor = factors[other ? r : thread];
 
     float c = 0.0f, l = 0.0f, sum = 0.0f;  // reference, sum of the weights, and of what multiplied the codes
+    float ceiling = 0.0f;                  // a tile whose largest is above it moves c
     bool first = true;
     for (int tile = SETS == 2 ? 0 : set; tile < tiles; tile += SETS == 2 ? 1 : 2, ++iteration) {
       const int n = before + tile;
@@ -738,10 +739,10 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
           }
         }
         float now = c;
-        if (__any_sync(0xffffffffu, first || top > c + kRise || top < c - fall_of(low_queries(PARTS)))) {
+        if (__any_sync(0xffffffffu, first || top > ceiling || top < c - fall_of(low_queries(PARTS)))) {
           const float next = floorf(top) - kRest;
           if (first) now = top > -INFINITY ? next : 0.0f;
-          else if (top > c + kRise) now = next;
+          else if (top > ceiling) now = next;
           else if (top < c - fall_of(low_queries(PARTS)) && top > -INFINITY)  // (the sums stay below 2^kHeldExponent)
             now = fmaxf(next, c - static_cast<float>(max(kHeldExponent - 1 - exponent_of(fmaxf(sum, l)), 0)));
         }
@@ -768,6 +769,7 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
             }
           }
           c = now;
+          ceiling = c + kRise;
         }
         first = false;
         // (low parts leave no room for the weights of two tiles)
@@ -807,6 +809,9 @@ __device__ __forceinline__ bool weigh(const SharedPlan& p, const SharedWalk& w, 
             if (tile_runs.inverse[i] != 0.0f) l += all;
             store_weights<low_weights(PARTS)>(weights + i * (low_weights(PARTS) ? 16 : 8), x);
           }
+          // (the weights by themselves are against 2^c over the value scale: up to 2^115 for a key
+          // whose values are zero or tiny.  What comes to more lets no tile stay above c.)
+          if (exponent_of(l) >= kLargeExponent) ceiling = c + kRest;
           leave_scores();
         }
         tc::tmem_wait_st();

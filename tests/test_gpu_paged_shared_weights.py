@@ -141,3 +141,35 @@ def test_float16_keeps_its_bits(storage, sequences, tokens, size):
     want = expected(host, q, [tokens] * sequences, range(sequences), 1 / math.sqrt(size))
     floor = np.linalg.norm(want.astype(np.float16).astype(np.float64) - want)
     assert np.linalg.norm(got - want) <= 1.15 * floor, float(np.linalg.norm(got - want) / floor)
+
+
+@pytest.mark.parametrize("dtype, sequences, pages", [("f32", 2, 290), ("bf16", 2, 290), ("f16", 2, 290), ("bf16", 150, 145),
+                                                    ("f16", 150, 145)])
+def test_long_runs_of_zero_values(dtype, sequences, pages):
+    """Thousands of shared keys with values of zero, whose scores rise by 12.9 (in base 2) behind the first page: they
+    take nearly all of the weight, and what is left of each sequence's own keys is the result."""
+    rng = np.random.default_rng(sequences)
+    kv_heads, size, page = torch.cuda.get_device_properties(0).multi_processor_count // 2 + 6, 32, 64
+    prefix, tails = 64 * pages, [2 + b % 4 for b in range(sequences)]
+    host = family(rng, prefix, tails, kv_heads=kv_heads, head_size=size, page=page)
+    host.scales[0][np.isfinite(host.scales[0])] = 0.25
+    shared, own = host.table[0, :pages], host.table[:, pages]
+    host.pools[0][0, shared] = 0
+    host.pools[0][0, shared[1:], :, :, 0] = 56
+    host.scales[1][0, shared] = 0
+    host.pools[1][0, shared] = 0
+    for slot, n in enumerate(tails):
+        host.pools[0][0, own[slot], :, :n] = 0
+        host.pools[0][0, own[slot], :, :n, 0] = 56
+    q = torch.zeros(sequences, 1, kv_heads, size, device="cuda", dtype=DTYPE[dtype])
+    q[..., 0] = 12.9 * math.log(2.0) / (0.25 * 56)
+    cache = to_device(host)
+    got = wide(cache.attend_shared(0, q, scale=1.0, least_bytes=0))
+    cache.check_errors()
+    score, info = float(q[0, 0, 0, 0]) * 0.25 * 56, torch.finfo(DTYPE[dtype])
+    for slot, n in enumerate(tails):
+        values = host.pools[1][0, own[slot], :, :n].astype(np.float64) * host.scales[1][0, own[slot], :, None, None]
+        total = (prefix - 64 + n) + 64 * math.exp(-score)
+        want, share = values.sum(1) / total, n / total  # (kv_heads, size)
+        bound = 2 * WEIGHTS[dtype] * share * np.abs(values).max() + info.eps / 2 * np.abs(want) + info.tiny * info.eps
+        assert (np.abs(want) > bound).any() and (np.abs(got[slot, 0] - want) <= bound).all()
