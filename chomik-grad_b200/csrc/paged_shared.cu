@@ -21,10 +21,10 @@
 // cycles on the tensor cores (scores 8 x 48, values 4 x 64), but 8192 exponentials with their
 // conversions about 1700 cycles on the four schedulers: that, and the hand-offs
 // between warps that it delays, is what is left (2600 to 2900 cycles a tile of two
-// sets, 3400 where the weights have two parts; 64 samples of 16384 keys 82 us on the
-// device, 90 in float16 and 95 in float32, 16 blocks of 5 tokens at 32700 keys 151 and
-// 176 in float16, by cb_paged_attention, each sequence for itself, 351 and 292; 8
-// samples of 32768 keys, both sets the same rows, 65 and 71).
+// sets, 3400 where the weights have two parts; 64 samples of 16384 keys 83 us on the
+// device, 91 in float16 and 95 in float32, 16 blocks of 5 tokens at 32700 keys 154 and
+// 177 in float16, by cb_paged_attention, each sequence for itself, 351 and 292; 8
+// samples of 32768 keys, both sets the same rows, 65 and 72).
 //
 // Three launches, each begun while the one before ends: the common pages of each
 // sequence; the shared keys, a block to an SM, whose warps are divided by what they
